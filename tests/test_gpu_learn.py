@@ -1,0 +1,618 @@
+"""The training operators on the device (include/wc_learn.h), through the binding, against plain float64 code.
+
+Tolerances. Statistics and sums are float32: with logits up to 16 in magnitude a row's log-sum is off by a few ulps of 16
+(2^-20 each), so log-probabilities, ratios and probabilities are held to 2e-5 (relative, or of the output's largest). An
+output in a 16-bit type adds its own rounding: 2^-11 of the value in f16 (2^-24 at least: half its smallest step twice),
+2^-8 in bf16. Sums over R rows in float32 add at most 2^-24 of the sum of magnitudes for each of the (tree's) additions:
+2e-5 of that sum covers 300. The 8-bit checkpoint is exact: its integers, exponents and values are compared for equality.
+"""
+import math
+
+import pytest
+import torch
+
+import learn_ref as R
+import warchest_learn as wl
+import warchest_wave as ww
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+TYPES = {"f32": torch.float32, "f16": torch.float16, "bf16": torch.bfloat16}
+ROUND = {torch.float32: 2.0 ** -23, torch.float16: 2.0 ** -11, torch.bfloat16: 2.0 ** -8}
+STEP = {torch.float32: 0.0, torch.float16: 2.0 ** -24, torch.bfloat16: 0.0}
+
+
+def say(text):
+    print(text, flush=True)
+
+
+def near(got, want, what, scale=None):
+    """Every element within its type's rounding and 2e-5 of the largest (or of `scale`)."""
+    got64, want = got.detach().cpu().double(), want.double()
+    assert got64.shape == want.shape, (what, got64.shape, want.shape)
+    if not want.numel():
+        return
+    top = want.abs().max() if scale is None else scale
+    bound = want.abs() * ROUND[got.dtype] + STEP[got.dtype] + 2e-5 * top
+    bad = (got64 - want).abs() > bound
+    assert not bad.any(), (what, int(bad.sum()), float((got64 - want).abs().max()), float(torch.as_tensor(top)))
+
+
+def gen(seed):
+    return torch.Generator().manual_seed(seed)
+
+
+def strided(x, extra, fill=float("nan")):
+    """x on the device with `extra` columns more per row in memory (holding `fill`), at an offset of one element."""
+    rows, width = x.shape
+    buf = torch.full((rows * (width + extra) + 1,), fill, dtype=x.dtype, device=DEV)
+    v = buf[1:].view(rows, width + extra)[:, :width]
+    v.copy_(x)
+    return v
+
+
+def to(x):
+    return None if x is None else x.to(DEV)
+
+
+# ------------------------------------------------------------------ policy loss
+
+def policy_inputs(rows, vocab, dtype, seed, legal, ref):
+    g = gen(seed)
+    k = {"logits": (2 * torch.randn(rows, vocab, generator=g)).to(dtype),
+         "actions": torch.randint(0, vocab, (rows,), generator=g),
+         "advantages": torch.randn(rows, generator=g), "weights": torch.rand(rows, generator=g) + 0.1,
+         "legal": None, "ref_logp": None, "ref_logits": None}
+    if legal:
+        k["legal"] = torch.rand(rows, vocab, generator=g) < 0.5
+        k["legal"][torch.arange(rows), k["actions"]] = True
+    x = k["logits"].double()
+    if legal:
+        x = x.masked_fill(~k["legal"], -math.inf)
+    lp = torch.log_softmax(x, 1)[torch.arange(rows), k["actions"]].float()
+    k["behaviour_logp"] = lp + 0.3 * torch.randn(rows, generator=g)
+    if ref == "token":
+        k["ref_logp"] = lp + 0.5 * torch.randn(rows, generator=g)
+    if ref == "full":
+        k["ref_logits"] = (k["logits"].float() + torch.randn(rows, vocab, generator=g)).to(dtype)
+    return k
+
+
+def check_policy(got, k, coefs):
+    want = R.policy(**k, **coefs)
+    for n in ("logp", "kl", "entropy"):
+        near(getattr(got, n), want[n], n, scale=max(1.0, float(want[n].abs().max())) if len(want[n]) else None)
+    near(got.loss, want["loss"], "loss", scale=1.0)
+    near(got.grad, want["grad"], "grad", scale=max(1e-3, float(want["grad"].abs().max())))
+
+
+COEFS = dict(inv_temperature=0.7, clip_low=0.2, clip_high=0.3, kl_coef=0.1, entropy_coef=0.02)
+
+
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("rows,vocab", [(1, 1), (1, 8), (3, 22), (65, 7), (2, 64), (5, 63), (5, 65), (130, 97), (7, 511), (4, 513),
+                                        (7, 1000), (3, 2049), (4, 4099), (300, 567), (2, 20011)])
+def test_policy_loss_over_sizes(rows, vocab, dtype):
+    for i, (legal, ref) in enumerate([(False, "none"), (True, "token"), (True, "full"), (False, "full")]):
+        if rows * vocab > 50000 and i not in (0, 2):
+            continue
+        say(f"case policy: {rows} x {vocab} {dtype}, legal {legal}, ref {ref}")
+        k = policy_inputs(rows, vocab, TYPES[dtype], rows + vocab, legal, ref)
+        got = wl.policy_loss(**{n: to(v) for n, v in k.items()}, **COEFS)
+        check_policy(got, k, COEFS)
+
+
+@pytest.mark.parametrize("rows,vocab,dtype", [(2, 131072, "f32"), (2, 131072, "bf16"), (3, 70001, "f16"), (300, 33001, "bf16"),
+                                              (257, 8200, "f32")])
+def test_policy_loss_with_a_large_vocabulary(rows, vocab, dtype):
+    """Against float64 torch over whole rows (the row-by-row code is for small ones)."""
+    say(f"case policy: {rows} x {vocab} {dtype}")
+    k = policy_inputs(rows, vocab, TYPES[dtype], vocab, False, "full")
+    got = wl.policy_loss(**{n: to(v) for n, v in k.items()}, **COEFS)
+    some = torch.randperm(rows, generator=gen(1))[:3]
+    part = {n: v if v is None else v[some] for n, v in k.items()}
+    want = R.policy(**part, **COEFS)
+    for n in ("logp", "kl", "entropy"):
+        near(getattr(got, n)[some.to(DEV)], want[n], n, scale=max(1.0, float(want[n].abs().max())))
+    near(got.grad[some.to(DEV)], want["grad"], "grad")
+
+
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("vocab", [22, 700, 9001])
+def test_policy_rows_left_out_and_what_lies_in_masked_places(vocab, dtype):
+    """Weight 0 over NaN logits, actions out of range or illegal, rows with nothing legal, NaN and infinities in illegal
+    columns, a row at the type's lowest value, columns at -infinity; strided rows with NaN between them; 32-bit actions."""
+    say(f"case policy: rows left out, vocab {vocab} {dtype}")
+    t = TYPES[dtype]
+    k = policy_inputs(9, vocab, t, 5, True, "full")
+    low = torch.finfo(t).min
+    k["weights"][0], k["logits"][0] = 0.0, math.nan
+    k["actions"][1], k["actions"][2] = -1, vocab
+    k["legal"][3] = False
+    k["legal"][4, k["actions"][4]] = False
+    k["logits"][5] = torch.where(k["legal"][5], k["logits"][5], torch.tensor(math.nan, dtype=t))
+    k["logits"][6] = torch.where(k["legal"][6], k["logits"][6], torch.tensor(math.inf, dtype=t))
+    k["ref_logits"][5] = torch.where(k["legal"][5], k["ref_logits"][5], torch.tensor(-math.inf, dtype=t))
+    k["logits"][7], k["ref_logits"][7] = low, low
+    other = (torch.arange(vocab) != k["actions"][8]) & (torch.arange(vocab) % 3 == 0)
+    k["logits"][8] = torch.where(other, torch.tensor(-math.inf, dtype=t), k["logits"][8])
+    k["behaviour_logp"][7] = -math.log(float(k["legal"][7].sum()))
+    want = R.policy(**k, **COEFS)
+    dev = {n: to(v) for n, v in k.items()}
+    dev["logits"], dev["ref_logits"] = strided(k["logits"], 5), strided(k["ref_logits"], 3)
+    dev["actions"] = dev["actions"].int()
+    got = wl.policy_loss(**dev, **COEFS)
+    for n in ("logp", "kl", "entropy"):
+        near(getattr(got, n), want[n], n, scale=max(1.0, float(want[n].abs().max())))
+    near(got.grad, want["grad"], "grad")
+    near(got.loss, want["loss"], "loss", scale=1.0)
+    assert not got.grad[:5].any() and not got.logp[:5].any()
+
+
+def test_policy_nan_in_a_counted_row_shows():
+    k = policy_inputs(4, 40, torch.float32, 6, False, "none")
+    k["logits"][2, 7] = math.nan
+    got = wl.policy_loss(**{n: to(v) for n, v in k.items()}, **COEFS)
+    assert got.loss.isnan() and got.logp[2].isnan() and got.grad[2].isnan().any()
+    assert got.grad[[0, 1, 3]].isfinite().all()
+
+
+@pytest.mark.parametrize("rows,vocab,dtype", [(5, 22, "f32"), (6, 3001, "bf16"), (2, 40000, "f16")])
+def test_policy_in_place_without_gradient_scaled_and_again(rows, vocab, dtype):
+    """grad written over the logits, not at all, or scaled by what arrives; the same bits every time."""
+    say(f"case policy: ways to call, {rows} x {vocab} {dtype}")
+    k = {n: to(v) for n, v in policy_inputs(rows, vocab, TYPES[dtype], 8, False, "token").items()}
+    first = wl.policy_loss(**k, **COEFS)
+    second = wl.policy_loss(**k, **COEFS)
+    only = wl.policy_loss(**k, **COEFS, grad=False)
+    assert only.grad is None
+    for a, b in zip(first, second):
+        assert torch.equal(a, b)
+    for a, b in zip(first[:4], only[:4]):
+        near(a, b.cpu(), "without gradient", scale=1.0)
+    scaled = wl.policy_loss(**k, **COEFS, grad_out=torch.tensor(2.0, device=DEV))
+    near(scaled.grad, 2 * wl.policy_loss(**k, **COEFS).grad.double().cpu(), "twice")
+    x = k.pop("logits").clone()
+    over = wl.policy_loss(x, grad=x, **k, **COEFS)
+    assert over.grad is x and torch.equal(x, first.grad)
+
+
+def test_policy_no_rows_and_even_weights():
+    z = torch.zeros(0, device=DEV)
+    got = wl.policy_loss(torch.zeros(0, 5, device=DEV), z.long(), z, z)
+    assert float(got.loss) == 0 and got.grad.shape == (0, 5)
+    k = policy_inputs(6, 9, torch.float32, 9, False, "none")
+    k["weights"] = None
+    check_policy(wl.policy_loss(**{n: to(v) for n, v in k.items()}, **COEFS), k, COEFS)
+
+
+def test_policy_gradient_against_differences_of_the_loss():
+    """Float32 losses: steps of 0.05 leave 2e-3 of a unit gradient's curvature and 1e-5 of rounding."""
+    k = policy_inputs(3, 6, torch.float32, 11, True, "full")
+    dev = {n: to(v) for n, v in k.items()}
+    grad = wl.policy_loss(**dev, **COEFS).grad.cpu()
+    for i in range(18):
+        step = []
+        for s in (0.02, -0.02):
+            x = k["logits"].clone()
+            x.view(-1)[i] += s
+            step.append(float(wl.policy_loss(**{**dev, "logits": x.to(DEV)}, **COEFS, grad=False).loss))
+        assert abs((step[0] - step[1]) / 0.04 - float(grad.view(-1)[i])) < 2e-3
+
+
+# -------------------------------------------------------------- preference loss
+
+def preference_inputs(lengths, vocab, dtype, seed, lead=0, tail=0):
+    g = gen(seed)
+    ends = [lead]
+    for n in lengths:
+        ends.append(ends[-1] + n)
+    rows = ends[-1] + tail
+    logits = (2 * torch.randn(rows, vocab, generator=g)).to(dtype)
+    tokens = torch.randint(0, vocab, (rows,), generator=g)
+    lp = torch.log_softmax(logits.double(), 1)[torch.arange(rows), tokens].float()
+    return {"logits": logits, "tokens": tokens, "offsets": torch.tensor(ends),
+            "ref_logp": lp + 0.5 * torch.randn(rows, generator=g), "weights": (torch.rand(rows, generator=g) < 0.8).float()}
+
+
+def check_preference(got, k, **kw):
+    want = R.preference(**k, **kw)
+    for n in ("margins", "ratios", "logp"):
+        near(getattr(got, n), want[n], n, scale=max(1.0, float(want[n].abs().max())) if len(want[n]) else None)
+    near(got.loss, want["loss"], "loss", scale=max(1.0, abs(float(want["loss"]))))
+    near(got.grad, want["grad"], "grad", scale=max(1e-3, float(want["grad"].abs().max())) if len(want["grad"]) else None)
+
+
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("kind,average", [("logistic", False), ("logistic", True), ("squared", True), ("hinge", False)])
+@pytest.mark.parametrize("lengths,vocab", [([1, 1], 8), ([0, 3], 22), ([0, 0], 5), ([4, 0, 7, 2], 63), ([5, 6, 1, 0, 0, 9], 513),
+                                           ([3, 300], 65), ([2, 3], 4099), ([1, 2], 20011)])
+def test_preference_loss_over_sizes(lengths, vocab, dtype, kind, average):
+    say(f"case preference: {lengths} x {vocab} {dtype} {kind} average {average}")
+    k = preference_inputs(lengths, vocab, TYPES[dtype], sum(lengths) + vocab)
+    kw = dict(beta=0.3, smoothing=0.1, kind=kind, average=average, inv_temperature=0.8)
+    check_preference(wl.preference_loss(**{n: to(v) for n, v in k.items()}, **kw), k, **kw)
+
+
+@pytest.mark.parametrize("vocab", [22, 3000])
+def test_preference_rows_that_do_not_count(vocab):
+    """Rows before and after the sequences (NaN logits), tokens out of range, weight 0 over NaN, a row at -infinity;
+    32-bit indices; offsets beyond the rows and backwards; strided logits."""
+    say(f"case preference: rows that do not count, vocab {vocab}")
+    k = preference_inputs([4, 3, 5, 2], vocab, torch.float32, 3, lead=2, tail=3)
+    k["logits"][0] = k["logits"][1] = k["logits"][-1] = math.nan
+    k["tokens"][3], k["tokens"][6] = -1, vocab + 7
+    k["weights"][:] = 1.0
+    k["weights"][4], k["logits"][4] = 0.0, math.nan
+    k["logits"][8] = -math.inf
+    kw = dict(beta=0.5, kind="logistic", average=True)
+    quiet = {**k, "logits": k["logits"].clone()}
+    for r in (0, 1, len(quiet["logits"]) - 1):
+        quiet["logits"][r] = 0.0
+    want = R.preference(**quiet, **kw)
+    dev = {n: to(v) for n, v in k.items()} | {"logits": strided(k["logits"], 3), "tokens": k["tokens"].int().to(DEV),
+                                              "offsets": k["offsets"].int().to(DEV)}
+    got = wl.preference_loss(**dev, **kw)
+    near(got.grad, want["grad"], "grad")
+    near(got.margins, want["margins"], "margins", scale=1.0)
+    assert not got.grad[[0, 1, 3, 4, 6, 8, -1]].any()
+    dev["offsets"] = torch.tensor([-5, 4, 1000, 900, 2000], dtype=torch.int32, device=DEV)
+    quiet["offsets"] = torch.tensor([-5, 4, 1000, 900, 2000])
+    quiet["logits"] = k["logits"].nan_to_num(nan=0.0, neginf=0.0)
+    dev["logits"] = to(quiet["logits"])
+    got = wl.preference_loss(**dev, **kw)
+    want = R.preference(**quiet, **kw)
+    near(got.margins, want["margins"], "margins", scale=1.0)
+    near(got.grad, want["grad"], "grad")
+
+
+def test_preference_far_margins_and_no_pairs():
+    """Margins of +-1e4: the loss is linear or 0 there and its slope exact; no pairs: 0."""
+    k = preference_inputs([2, 2, 2, 2], 9, torch.float32, 5)
+    k["weights"][:] = 1.0
+    k["ref_logp"][:2] += 5e3
+    k["ref_logp"][4:6] -= 5e3
+    got = wl.preference_loss(**{n: to(v) for n, v in k.items()}, beta=1.0)
+    assert got.loss.isfinite() and got.grad.isfinite().all()
+    assert not got.grad[4:].any() and got.grad[:4].any()
+    assert abs(float(got.loss) - 5e3) < 10
+    k["offsets"] = torch.zeros(1, dtype=torch.int64)
+    got = wl.preference_loss(**{n: to(v) for n, v in k.items()})
+    assert float(got.loss) == 0 and not got.grad.any()
+
+
+def test_preference_again_in_place_and_without_gradient():
+    k = {n: to(v) for n, v in preference_inputs([40, 3, 17, 60], 2001, torch.bfloat16, 6).items()}
+    a, b = wl.preference_loss(**k), wl.preference_loss(**k)
+    for x, y in zip(a, b):
+        assert torch.equal(x, y)
+    assert torch.equal(wl.preference_loss(**k, grad=False).margins, a.margins)
+    x = k.pop("logits").clone()
+    assert torch.equal(wl.preference_loss(x, grad=x, **k).grad, a.grad)
+
+
+# ---------------------------------------------------------------- residual norm
+
+def norm_inputs(rows, width, dtype, seed, kind, gate, pdtype=None):
+    g = gen(seed)
+    pdtype = pdtype or dtype
+    k = {"block": (1.5 * torch.randn(rows, width, generator=g) + 0.2).to(dtype),
+         "stream": (2 * torch.randn(rows, width, generator=g)).to(dtype),
+         "post_gain": (1 + 0.1 * torch.randn(width, generator=g)).to(pdtype),
+         "pre_gain": (1 + 0.1 * torch.randn(width, generator=g)).to(pdtype), "post_bias": None, "pre_bias": None,
+         "gate": None}
+    if kind == "layer":
+        k["post_bias"], k["pre_bias"] = ((0.1 * torch.randn(width, generator=g)).to(pdtype) for _ in range(2))
+    if gate == "vector":
+        k["gate"] = (0.5 + 0.3 * torch.randn(width, generator=g)).to(pdtype)
+    if gate == "token":
+        k["gate"] = (0.5 + 0.3 * torch.randn(rows, width, generator=g)).to(dtype)
+    d = [torch.randn(rows, width, generator=g).to(dtype) for _ in range(2)]
+    return k, d
+
+
+def check_norm(k, d, kw, dev=None):
+    v = {n: None if t is None else t.double().requires_grad_(True) for n, t in k.items()}
+    new, out = R.residual_norm(**v, **kw)
+    dev = dev or {n: to(t) for n, t in k.items()}
+    f = wl.residual_norm(**dev, **kw)
+    # a row's normed values are as well known as its variance: widths of a few channels can leave little of it
+    near(f.stream, new.detach(), "stream", scale=max(4.0, float(new.abs().max())) if new.numel() else None)
+    near(f.out, out.detach(), "out", scale=8.0)
+    given = [(o, t) for o, t in ((out, d[0]), (new, d[1])) if t is not None]
+    if given:
+        torch.autograd.backward([o for o, _ in given], [t.double() for _, t in given])
+    b = wl.residual_norm_backward(to(d[0]), to(d[1]), dev["block"], dev["stream"], f.stats, *(
+        dev[n] for n in ("post_gain", "post_bias", "gate", "pre_gain", "pre_bias")), **kw)
+    for n, t in v.items():
+        got = getattr(b, n)
+        if t is None:
+            assert got is None
+            continue
+        want = t.grad if t.grad is not None else torch.zeros_like(t)
+        # sums over the rows of terms of about 1: 2e-5 of their magnitudes' sum
+        near(got, want, n, scale=max(8.0, float(want.abs().max())) if want.numel() else None)
+    return f, b
+
+
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("kind", ["rms", "layer"])
+@pytest.mark.parametrize("rows,width", [(1, 8), (2, 7), (3, 65), (37, 96), (300, 33), (5, 129), (2, 512), (67, 513), (3, 1153),
+                                        (2, 2049), (3, 4096), (2, 5000), (2, 8191), (1, 16384), (2, 9001)])
+def test_residual_norm_over_sizes(rows, width, kind, dtype):
+    for gate, act in (("none", "none"), ("vector", "none"), ("token", "sigmoid"), ("vector", "tanh")):
+        if width > 1000 and gate == "none":
+            continue
+        say(f"case norm: {rows} x {width} {dtype} {kind} gate {gate} {act}")
+        k, d = norm_inputs(rows, width, TYPES[dtype], rows + width, kind, gate)
+        check_norm(k, d, dict(scale=0.7, eps=1e-3, norm=kind, gate_act=act))
+
+
+@pytest.mark.parametrize("kind", ["rms", "layer"])
+def test_residual_norm_other_arguments(kind):
+    """No rows; no parameters at all; float32 parameters beside 16-bit matrices; one of the two gradients missing;
+    strided rows; a broadcast stream."""
+    say(f"case norm: other arguments, {kind}")
+    kw = dict(scale=-1.3, eps=1e-4, norm=kind)
+    k, d = norm_inputs(0, 40, torch.float32, 1, kind, "vector")
+    _, b = check_norm(k, d, kw)
+    assert not b.post_gain.any() and not b.gate.any()
+    k, d = norm_inputs(9, 40, torch.float32, 2, kind, "none")
+    check_norm({n: t if n in ("block", "stream") else None for n, t in k.items()}, d, kw)
+    k, d = norm_inputs(9, 200, torch.bfloat16, 3, kind, "vector", torch.float32)
+    check_norm(k, d, kw)
+    check_norm(k, [d[0], None], kw)
+    check_norm(k, [None, d[1]], kw)
+    k, d = norm_inputs(11, 51, torch.float16, 4, kind, "token")
+    dev = {n: to(t) for n, t in k.items()} | {n: strided(k[n], 3) for n in ("block", "stream", "gate")}
+    check_norm(k, d, kw, dev)
+    k, d = norm_inputs(6, 72, torch.float32, 5, kind, "vector")
+    k["stream"] = k["stream"][:1].expand(6, 72).contiguous()
+    dev = {n: to(t) for n, t in k.items()} | {"stream": to(k["stream"][:1]).expand(6, 72)}
+    check_norm(k, d, kw, dev)
+
+
+def test_residual_norm_of_a_constant_row_and_one_channel():
+    """A row without variance: normed values are 0, gradients stay finite."""
+    x = torch.full((3, 24), 5.0, device=DEV)
+    f = wl.residual_norm(x, torch.full_like(x, -5.0), norm="layer")
+    assert not f.out.any() and torch.equal(f.stream, torch.full_like(x, -5.0))
+    b = wl.residual_norm_backward(x, x, x, torch.full_like(x, -5.0), f.stats, norm="layer")
+    assert b.block.isfinite().all() and b.stream.isfinite().all()
+    one = torch.tensor([[3.0], [-2.0]], device=DEV)
+    f = wl.residual_norm(one, one, norm="rms", eps=0.0)
+    near(f.out, torch.tensor([[1.0], [-1.0]]), "one channel")
+
+
+def test_residual_norm_many_rows_and_the_same_bits_twice():
+    """More rows than workgroups: every workgroup's column sums hold several rows."""
+    for rows, width, kind in ((3001, 96, "layer"), (1500, 1153, "rms"), (700, 4096, "layer")):
+        say(f"case norm: {rows} x {width} {kind}")
+        k, d = norm_inputs(rows, width, torch.float32, 7, kind, "vector")
+        kw = dict(scale=0.5, eps=1e-5, norm=kind)
+        _, b = check_norm(k, d, kw)
+        _, c = check_norm(k, d, kw)
+        for x, y in zip(b, c):
+            assert (x is None and y is None) or torch.equal(x, y)
+
+
+# ------------------------------------------------------- activations in 8 bits
+
+SPECIAL = [0.0, -0.0, 1.0, -1.0, 127.0, 127.4999, 128.0, 0.5, 1.5, 2.5, -2.5, 3e-5, -6e4, 6.5e4, 1e-7, 255.0, 254.0]
+
+
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("rows,width", [(1, 1), (3, 7), (2, 31), (2, 32), (5, 33), (3, 64), (2, 100), (17, 257), (1, 1000)])
+def test_checkpoint_writes_and_reads_exactly(rows, width, dtype):
+    say(f"case checkpoint: {rows} x {width} {dtype}")
+    t = TYPES[dtype]
+    g = gen(rows * width)
+    x = torch.randn(rows, width, generator=g) * torch.exp2(torch.randint(-12, 12, (rows, 1), generator=g).float())
+    x.view(-1)[: min(x.numel(), len(SPECIAL))] = torch.tensor(SPECIAL)[: x.numel()]
+    if rows > 2:
+        x[2] = 0.0
+    x = x.to(t)
+    q, e, value = R.keep8(x)
+    for dev in (x.to(DEV), strided(x, 5)):
+        ck = wl.checkpoint8(dev)
+        assert torch.equal(ck.q.cpu(), q) and torch.equal(ck.exps.cpu(), e)
+        got = wl.checkpoint8_read(ck, torch.float32)
+        assert torch.equal(got.cpu().double(), value)
+        assert torch.equal(wl.checkpoint8_read(ck, torch.bfloat16).cpu().double(), value)  # 8 bits fit bf16
+
+
+def test_checkpoint_extremes():
+    """Subnormals, the type's largest, infinities and NaN (whose group reads back as NaN, the next one untouched)."""
+    for t in (torch.float32, torch.bfloat16):
+        x = torch.zeros(6, 64, dtype=t)
+        x[0, :3] = torch.tensor([1e-39, -3e-39, 2e-41])
+        x[1, 0], x[1, 40] = torch.finfo(t).max, -torch.finfo(t).max
+        x[2, 5], x[2, 33] = math.inf, 1.0
+        x[3, 5], x[3, 33] = math.nan, 1.0
+        x[4, 63] = -math.inf
+        x[5, :32] = 2.0 ** -126
+        q, e, value = R.keep8(x)
+        ck = wl.checkpoint8(x.to(DEV))
+        assert torch.equal(ck.q.cpu(), q) and torch.equal(ck.exps.cpu(), e)
+        got = wl.checkpoint8_read(ck, torch.float32).cpu().double()
+        # the largest number is kept as 64 * 2^122 = 2^128, which a read gives as float32's largest
+        value = value.clamp(-torch.finfo(torch.float32).max, torch.finfo(torch.float32).max)
+        assert torch.equal(got.isnan(), value.isnan())
+        assert torch.equal(got.nan_to_num(), value.nan_to_num())
+    empty = wl.checkpoint8(torch.zeros(0, 40, device=DEV))
+    assert wl.checkpoint8_read(empty).shape == (0, 40)
+
+
+@pytest.mark.parametrize("name", ["none", "relu", "gelu", "silu"])
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("rows,width", [(1, 5), (3, 96), (40, 333)])
+def test_checkpoint_activations_forward_and_backward(rows, width, dtype, name):
+    say(f"case checkpoint {name}: {rows} x {width} {dtype}")
+    t, g = TYPES[dtype], gen(width)
+    x = (3 * torch.randn(rows, width, generator=g)).to(t)
+    x.view(-1)[:4] = torch.tensor([0.0, -30.0, 30.0, 1e-3])
+    d = torch.randn(rows, width, generator=g).to(t)
+    _, _, value = R.keep8(x)
+    z = value.requires_grad_(True)
+    R.act(z, name).backward(d.double())
+    ck, y = wl.checkpoint8_act(strided(x, 3), name)
+    near(y, R.act(x.double(), name), "value", scale=4.0)
+    near(wl.checkpoint8_act_backward(ck, strided(d, 1), name), z.grad, "slope", scale=4.0)
+    near(wl.checkpoint8_read(ck, t, act=name), R.act(value.detach(), name), "read", scale=4.0)
+
+
+def test_activation_tails_are_finite():
+    x = torch.tensor([[-3e38, -1e20, -1e4, -90.0, 90.0, 1e4, 1e20, 3e38]], device=DEV)
+    for name in ("relu", "gelu", "silu"):
+        for i in range(8):
+            ck, y = wl.checkpoint8_act(x[:, i:i + 1].contiguous(), name)
+            d = wl.checkpoint8_act_backward(ck, torch.ones(1, 1, device=DEV), name)
+            want = (max(float(x[0, i]), 0.0), 1.0 if i > 3 else 0.0)
+            assert abs(float(y) - want[0]) <= 1e-6 * abs(want[0]) and abs(float(d) - want[1]) < 1e-6, (name, i)
+
+
+# ----------------------------------------------------------------- weight gradient
+
+def weight_case(rows, width, out, dtype, name, wdtype, seed=0, dev=None):
+    t, g = TYPES[dtype], gen(rows + width + out + seed)
+    x = 1.5 * torch.randn(rows, width, generator=g)
+    d = torch.randn(rows, out, generator=g).to(t)
+    ck = wl.checkpoint8(x.to(DEV))
+    value = wl.checkpoint8_read(ck, torch.float32).cpu().double()
+    weight, bias = wl.checkpoint8_weight_grad(ck, dev(d) if dev else to(d), act=name, bias=True, dtype=wdtype)
+    a = R.act(value, name)
+    want = a.t() @ d.double()
+    size = a.abs().t() @ d.double().abs()  # the sum of the products' magnitudes
+    # exact products: 2e-5 of the magnitudes for the float32 sums; a recomputed activation is rounded to grad's type
+    bound = size * (2e-5 + (ROUND[t] if name in ("gelu", "silu") else 0.0)) + want.abs() * ROUND[weight.dtype] + 1e-30
+    bound = bound + STEP[weight.dtype]
+    off = (weight.cpu().double() - want).abs()
+    assert not (off > bound).any(), (float(off.max()), float(bound.min()))
+    near(bias, d.double().sum(0), "bias", scale=max(1.0, float(d.double().abs().sum(0).max())) if rows else 1.0)
+    return weight, bias, ck
+
+
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("rows,width,out", [(0, 5, 3), (1, 1, 1), (1, 40, 9), (31, 33, 65), (32, 64, 64), (33, 130, 7), (300, 65, 129),
+                                            (1000, 96, 22), (2500, 256, 200), (700, 1, 300), (130, 515, 260)])
+def test_weight_gradient_over_sizes(rows, width, out, dtype):
+    for name in ("none", "relu", "gelu", "silu"):
+        if dtype == "f32" and name in ("gelu", "silu"):
+            continue
+        say(f"case weight: {rows} x {width} x {out} {dtype} {name}")
+        weight_case(rows, width, out, dtype, name, torch.float32)
+        weight_case(rows, width, out, dtype, name, TYPES[dtype])
+
+
+@pytest.mark.parametrize("dtype", list(TYPES))
+def test_weight_gradient_long_sums_strides_and_the_same_bits(dtype):
+    """A long sum over few tiles (split into runs), rows of grad at an odd stride and offset, twice the same bits."""
+    say(f"case weight: long sum {dtype}")
+    w, b, ck = weight_case(20011, 70, 50, dtype, "none", torch.float32, dev=lambda d: strided(d, 3))
+    g = gen(1)
+    d = torch.randn(20011, 50, generator=g).to(TYPES[dtype]).to(DEV)
+    one, two = (wl.checkpoint8_weight_grad(ck, d, bias=True) for _ in range(2))
+    assert torch.equal(one[0], two[0]) and torch.equal(one[1], two[1])
+
+
+def test_weight_gradient_of_a_sliced_checkpoint_and_nan_groups():
+    """A checkpoint's rows may be a slice of a larger one; a group held as NaN reaches its own channels only."""
+    x = torch.randn(64, 96, generator=gen(2))
+    x[20, 40] = math.inf
+    ck = wl.checkpoint8(x.to(DEV))
+    d = torch.randn(50, 8, generator=gen(3)).bfloat16().to(DEV)
+    part = wl.Checkpoint8(ck.q[10:60], ck.exps[10:60])
+    w, _ = wl.checkpoint8_weight_grad(part, d)
+    assert w[32:64].isnan().all() and w[:32].isfinite().all() and w[64:].isfinite().all()
+
+
+def test_f16_weight_gradient_at_the_ends_of_its_range():
+    """A kept value just beyond f16's largest (65504 is kept as 65536) is held there."""
+    x = torch.full((4, 32), 65504.0)
+    ck = wl.checkpoint8(x.to(DEV))
+    d = torch.ones(4, 3, dtype=torch.float16, device=DEV)
+    w, _ = wl.checkpoint8_weight_grad(ck, d)
+    assert torch.equal(w, torch.full_like(w, 4 * 65504.0))
+
+
+# ------------------------------------------------------------------- streams, graphs
+
+def everything(s):
+    p = wl.policy_loss(**s["policy"], **COEFS)
+    f = wl.preference_loss(**s["preference"])
+    n = wl.residual_norm(**s["norm"])
+    b = wl.residual_norm_backward(*s["d"], s["norm"]["block"], s["norm"]["stream"], n.stats, *(
+        s["norm"][i] for i in ("post_gain", "post_bias", "gate", "pre_gain", "pre_bias")))
+    ck, y = wl.checkpoint8_act(s["norm"]["block"], "gelu")
+    z = wl.checkpoint8_act_backward(ck, s["d"][0], "gelu")
+    w, c = wl.checkpoint8_weight_grad(ck, s["d"][1], act="relu", bias=True)
+    return [t for t in (*p, *f, *n, *b, *ck, y, z, w, c) if t is not None]
+
+
+def all_inputs(seed):
+    k, d = norm_inputs(300, 96, torch.bfloat16, seed, "layer", "vector")
+    return {"policy": {n: to(v) for n, v in policy_inputs(40, 700, torch.bfloat16, seed, False, "token").items()},
+            "preference": {n: to(v) for n, v in preference_inputs([5, 9, 0, 3], 333, torch.float16, seed).items()},
+            "norm": {n: to(v) for n, v in k.items()}, "d": [to(x) for x in d]}
+
+
+def test_operators_on_another_stream():
+    s = all_inputs(1)
+    want = everything(s)
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        got = everything(s)
+    side.synchronize()
+    for a, b in zip(got, want):
+        assert torch.equal(a, b)
+
+
+def test_operators_in_a_captured_graph():
+    """Captured once, replayed over new inputs with eager work between: every replay equals the eager result."""
+    held = all_inputs(1)
+    everything(held)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        outs = everything(held)
+    for seed in (2, 3, 4):
+        fresh = all_inputs(seed)
+        want = [t.clone() for t in everything(fresh)]
+        for part in ("policy", "preference", "norm"):
+            for n, t in held[part].items():
+                if t is not None:
+                    t.copy_(fresh[part][n])
+        for a, b in zip(held["d"], fresh["d"]):
+            a.copy_(b)
+        graph.replay()
+        torch.cuda.synchronize()
+        for a, b in zip(outs, want):
+            assert torch.equal(a, b)
+
+
+def test_refusals_of_the_binding():
+    """Shapes, types and layouts that do not fit raise before anything is queued."""
+    x = torch.zeros(4, 8, device=DEV)
+    i = torch.zeros(4, dtype=torch.int64, device=DEV)
+    v = torch.zeros(4, device=DEV)
+    for call in (lambda: wl.policy_loss(x, i[:3], v, v), lambda: wl.policy_loss(x, v, v, v),
+                 lambda: wl.policy_loss(x.t(), i, v, v), lambda: wl.policy_loss(x.double(), i, v, v),
+                 lambda: wl.policy_loss(x, i, v.half(), v), lambda: wl.policy_loss(x, i, v, v, legal=x),
+                 lambda: wl.policy_loss(x, i, v, v, ref_logp=v, ref_logits=x),
+                 lambda: wl.policy_loss(x, i, v, v, grad=x.half()), lambda: wl.policy_loss(x, i, v.cpu(), v),
+                 lambda: wl.preference_loss(x, i, i, v), lambda: wl.preference_loss(x, i, i[:3].int(), v),
+                 lambda: wl.preference_loss(x, i, i[:3], None), lambda: wl.preference_loss(x, i, i[:3], v, kind="odd"),
+                 lambda: wl.preference_loss(x, i, i[:3], v, beta=0.0),
+                 lambda: wl.residual_norm(x, x.half()), lambda: wl.residual_norm(x, x[:, :4]),
+                 lambda: wl.residual_norm(x, x, torch.ones(7, device=DEV)), lambda: wl.residual_norm(x, x, norm="batch"),
+                 lambda: wl.residual_norm(x, x, gate=x[:1].expand(4, 8)),
+                 lambda: wl.residual_norm(torch.zeros(1, 16385, device=DEV), torch.zeros(1, 16385, device=DEV)),
+                 lambda: wl.residual_norm_backward(x, x, x, x, None), lambda: wl.checkpoint8(x.int()),
+                 lambda: wl.checkpoint8_act(x, "tan"), lambda: wl.checkpoint8(x[0]),
+                 lambda: wl.checkpoint8_read(wl.Checkpoint8(x, x)),
+                 lambda: wl.checkpoint8_weight_grad(wl.checkpoint8(x), x, act="gelu"),
+                 lambda: wl.checkpoint8_weight_grad(wl.checkpoint8(x), x[:3])):
+        with pytest.raises(ww.WaveError):
+            call()
+    torch.cuda.synchronize()

@@ -1,0 +1,64 @@
+// Device helpers of the training operators: element types, eight-element
+// loads and stores at any element alignment, and fixed-order reductions.
+#pragma once
+
+#include <hip/hip_runtime.h>
+
+#include <cstdint>
+
+namespace wc {
+namespace learn {
+
+typedef _Float16 f16;
+typedef __bf16 bf16;
+
+// Eight consecutive elements. The type asks for the element's alignment only:
+// the hardware takes wide accesses at any, and splits one that crosses a line.
+template <class T>
+struct Vec8 {
+    typedef T type __attribute__((ext_vector_type(8), aligned(sizeof(T))));
+};
+
+template <class T>
+__device__ __forceinline__ void load8(const T* __restrict__ p, float (&v)[8]) {
+    const typename Vec8<T>::type x = *(const typename Vec8<T>::type*)p;
+#pragma unroll
+    for (int i = 0; i < 8; i++) v[i] = (float)x[i];
+}
+
+// The first n (0 .. 8) of eight elements, `fill` in the place of the others.
+template <class T>
+__device__ __forceinline__ void load_n(const T* __restrict__ p, int n, float fill, float (&v)[8]) {
+    if (n >= 8) {
+        load8(p, v);
+        return;
+    }
+#pragma unroll
+    for (int i = 0; i < 8; i++) v[i] = i < n ? (float)p[i] : fill;
+}
+
+template <class T>
+__device__ __forceinline__ void store_n(T* __restrict__ p, int n, const float (&v)[8]) {
+    if (n >= 8) {
+        typename Vec8<T>::type x;
+#pragma unroll
+        for (int i = 0; i < 8; i++) x[i] = (T)v[i];
+        *(typename Vec8<T>::type*)p = x;
+        return;
+    }
+#pragma unroll
+    for (int i = 0; i < 8; i++)
+        if (i < n) p[i] = (T)v[i];
+}
+
+// e^x by the hardware's 2^x (1 ulp; a result under 2^-126 is 0). Callers take
+// x as a difference to a row's maximum, so that x log2(e) is off by less than
+// an ulp of a small number.
+__device__ __forceinline__ float fast_exp(float x) { return __builtin_amdgcn_exp2f(x * 1.4426950408889634f); }
+
+__device__ __forceinline__ int64_t index_at(const void* p, int bits, int64_t i) {
+    return bits == 64 ? ((const int64_t*)p)[i] : (int64_t)((const int32_t*)p)[i];
+}
+
+}  // namespace learn
+}  // namespace wc

@@ -1,0 +1,429 @@
+"""Python binding of the training operators' C ABI (include/wc_learn.h).
+
+What a trainer of the policy or value network runs on the solver's results, on torch tensors in device memory:
+
+- `policy_loss`: the clipped policy loss with a KL term and an entropy bonus, and its gradient, from rows of logits;
+- `preference_loss`: the paired log-ratio loss over ragged sequences, and its gradient;
+- `residual_norm`, `residual_norm_backward`: a block's output normed, gated, scaled and added to the residual stream, and
+  the norm before the next block;
+- `checkpoint8`, `checkpoint8_act`, `checkpoint8_read`, `checkpoint8_act_backward`, `checkpoint8_weight_grad`:
+  activations kept in 8 bits for the backward pass, and what the backward pass does with them.
+
+Every call is queued on the current stream of its tensors' device and returns at once. Outputs and scratch are allocated
+with torch on that stream; a tensor made on another stream must be ready there, and kept alive by its owner
+(`Tensor.record_stream`), as for torch's own operators. Matrices need unit column stride, rows may be at any stride.
+Arguments that do not fit raise `WaveError`, and then nothing was queued. The `*_objective` functions and `ResidualNorm`
+are the same calls with torch's automatic differentiation.
+
+Nothing here computes: every call goes through the native library.
+"""
+from __future__ import annotations
+
+import ctypes as C
+import functools
+import struct
+from collections import namedtuple
+
+import torch
+
+import warchest_wave as ww
+from warchest_wave import WaveError
+
+# Symbols every build must export (include/wc_learn.h), beside warchest_wave.EXPORTS.
+EXPORTS = [
+    "wc_policy_workspace", "wc_policy_loss", "wc_preference_workspace", "wc_preference_loss",
+    "wc_residual_norm", "wc_residual_norm_workspace", "wc_residual_norm_backward",
+    "wc_ckpt_write", "wc_ckpt_read", "wc_ckpt_act_backward", "wc_ckpt_weight_workspace", "wc_ckpt_weight_grad",
+]
+
+DTYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
+NORMS = {"rms": 0, "layer": 1}
+GATE_ACTS = {"none": 0, "sigmoid": 1, "tanh": 2}
+ACTS = {"none": 0, "relu": 1, "gelu": 2, "silu": 3}
+KINDS = {"logistic": 0, "squared": 1, "hinge": 2}
+GROUP = 32
+
+# The structures of the header, packed in C's own layout: a call fills one in one step.
+_POLICY = struct.Struct("@Qii qq PqPqPq PPPPPP fffffi PPPPPq PQ")
+_PREFERENCE = struct.Struct("@Qii qqq Pq PPPPP fffiii PPPPPq PQ")
+_NORM = struct.Struct("@Qiiii qq PqPq PPPqPP ffii PqPq P")
+_NORM_BACK = struct.Struct("@Qiiii qq PqPq PPPqP fiii PPqPq PqPq PPPPPq PQ")
+_CKPT = struct.Struct("@Qii qq ii PqPq PqPq")
+_WEIGHT = struct.Struct("@Qii qqq ii PqPqPqPq P PQ")
+
+PolicyLoss = namedtuple("PolicyLoss", "loss logp kl entropy grad")
+PreferenceLoss = namedtuple("PreferenceLoss", "loss margins ratios logp grad")
+ResidualNormOut = namedtuple("ResidualNormOut", "stream out stats")
+ResidualNormGrads = namedtuple("ResidualNormGrads", "block stream post_gain post_bias gate pre_gain pre_bias")
+Checkpoint8 = namedtuple("Checkpoint8", "q exps")
+
+_fn = {}
+
+
+def _entry(name):
+    f = _fn.get(name)
+    if f is None:
+        f = getattr(ww.lib(), name)
+        f.argtypes = [C.c_char_p, C.c_void_p] if not name.endswith("workspace") else [C.c_char_p,
+                                                                                     C.POINTER(C.c_uint64)]
+        f.restype = C.c_int
+        _fn[name] = f
+    return f
+
+
+def _call(name, packed, device):
+    rc = _entry(name)(packed, torch.cuda.current_stream(device).cuda_stream)
+    if rc:
+        ww._check(rc)
+
+
+def _scratch_bytes(name, packed):
+    n = C.c_uint64()
+    ww._check(_entry(name)(packed, C.byref(n)))
+    return n.value
+
+
+def _fail(text):
+    raise WaveError(text)
+
+
+def _device(t, name):
+    if not isinstance(t, torch.Tensor):
+        _fail(f"{name} is not a tensor")
+    d = t.device
+    if d.type != "cuda":
+        _fail(f"{name} is not on a GPU")
+    return d
+
+
+def _dtype(t, name):
+    c = DTYPES.get(t.dtype)
+    if c is None:
+        _fail(f"{name}: {t.dtype} is not one of float32, float16, bfloat16")
+    return c
+
+
+def _matrix(t, name, device, dtype, rows, width):
+    """(address, row stride) of a matrix that must be rows x width."""
+    if t.dtype != dtype:
+        _fail(f"{name}: {t.dtype}, expected {dtype}")
+    if t.device != device:
+        _fail(f"{name} is on {t.device}, not on {device}")
+    if t.dim() != 2 or t.shape[0] != rows or t.shape[1] != width:
+        _fail(f"{name}: shape {tuple(t.shape)}, expected ({rows}, {width})")
+    s = t.stride()
+    if s[1] != 1 and width > 1:
+        _fail(f"{name}: columns must be contiguous")
+    return t.data_ptr(), s[0]
+
+
+def _vector(t, name, device, dtype, n):
+    """The address of a contiguous vector of n, 0 for None."""
+    if t is None:
+        return 0
+    if t.dtype != dtype:
+        _fail(f"{name}: {t.dtype}, expected {dtype}")
+    if t.device != device:
+        _fail(f"{name} is on {t.device}, not on {device}")
+    if t.dim() != 1 or t.shape[0] != n:
+        _fail(f"{name}: shape {tuple(t.shape)}, expected ({n},)")
+    if n > 1 and t.stride(0) != 1:
+        _fail(f"{name} must be contiguous")
+    return t.data_ptr()
+
+
+def _scalar(t, name, device):
+    if t is None:
+        return 0
+    if t.dtype != torch.float32 or t.numel() != 1 or t.device != device:
+        _fail(f"{name} is one float32 on {device}")
+    return t.data_ptr()
+
+
+def _indices(t, name, device, n):
+    if t.dtype not in (torch.int64, torch.int32):
+        _fail(f"{name}: {t.dtype}, expected int64 or int32")
+    return _vector(t, name, device, t.dtype, n), 64 if t.dtype == torch.int64 else 32
+
+
+def _known(table, key, name):
+    if key not in table:
+        _fail(f"{name}: {key!r} is not one of {', '.join(table)}")
+    return table[key]
+
+
+def _logits(t):
+    device = _device(t, "logits")
+    code = _dtype(t, "logits")
+    if t.dim() != 2:
+        _fail(f"logits: shape {tuple(t.shape)}, expected rows x vocab")
+    rows, vocab = t.shape
+    return device, code, rows, vocab, _matrix(t, "logits", device, t.dtype, rows, vocab)
+
+
+# Scratch sizes depend on shapes alone.
+@functools.lru_cache(maxsize=4096)
+def _policy_scratch(device, code, rows, vocab):
+    p = 256  # an address that passes for one: the size is computed from the shape, nothing is read
+    return _scratch_bytes("wc_policy_workspace", _POLICY.pack(
+        _POLICY.size, device, code, rows, vocab, p, vocab, 0, 0, 0, 0, p, p, p, 0, 0, 0, 1.0, 0.0, 0.0, 0.0, 0.0, 64,
+        p, p, p, p, 0, 0, 0, 0))
+
+
+@functools.lru_cache(maxsize=4096)
+def _preference_scratch(device, code, rows, vocab, pairs):
+    p = 256
+    return _scratch_bytes("wc_preference_workspace", _PREFERENCE.pack(
+        _PREFERENCE.size, device, code, rows, vocab, pairs, p, vocab, p, p, p, 0, 0, 1.0, 1.0, 0.0, 0, 0, 64, p, p, p,
+        p, 0, 0, 0, 0))
+
+
+@functools.lru_cache(maxsize=4096)
+def _norm_scratch(device, code, rows, width):
+    p = 256
+    return _scratch_bytes("wc_residual_norm_workspace", _NORM_BACK.pack(
+        _NORM_BACK.size, device, code, 0, 0, rows, width, p, width, p, width, 0, 0, 0, 0, 0, 1.0, 0, 0, 0, p, 0, 0, 0, 0,
+        p, width, p, width, 0, 0, 0, 0, 0, 0, 0, 0))
+
+
+@functools.lru_cache(maxsize=4096)
+def _weight_scratch(device, code, rows, width, out, act, weight_code):
+    p = 256
+    return _scratch_bytes("wc_ckpt_weight_workspace", _WEIGHT.pack(
+        _WEIGHT.size, device, code, rows, width, out, act, weight_code, p, width, p, -(-width // GROUP), p, out, p, out,
+        p, 0, 0))
+
+
+def _scratch(n, device):
+    return torch.empty(n, dtype=torch.uint8, device=device)
+
+
+def policy_loss(logits, actions, behaviour_logp, advantages, weights=None, *, legal=None, ref_logp=None, ref_logits=None,
+                inv_temperature=1.0, clip_low=0.2, clip_high=0.2, kl_coef=0.0, entropy_coef=0.0, grad=True,
+                grad_out=None):
+    """The clipped policy loss of rows of logits, and its gradient (wc_policy_loss).
+
+    logits [rows, vocab]; actions [rows] int64 or int32; behaviour_logp, advantages, weights, ref_logp [rows] float32
+    (weights None: 1/rows each); legal [rows, vocab] bool; ref_logits like logits. A row of weight 0, with an action that
+    is out of range or not legal, or without a legal logit above -infinity is left out. grad: True, a tensor like
+    logits to write to (logits itself works), or False; grad_out: one float32, what arrives at the loss.
+    Returns PolicyLoss(loss, logp, kl, entropy, grad): logp of the actions, KL and entropy per row."""
+    device, code, rows, vocab, (x, xs) = _logits(logits)
+    a, bits = _indices(actions, "actions", device, rows)
+    f32 = torch.float32
+    lg, lgs = (0, 0) if legal is None else _matrix(legal, "legal", device, torch.bool, rows, vocab)
+    rl, rls = (0, 0) if ref_logits is None else _matrix(ref_logits, "ref_logits", device, logits.dtype, rows, vocab)
+    if grad is True:
+        grad = torch.empty((rows, vocab), dtype=logits.dtype, device=device)
+    elif grad is False:
+        grad = None
+    g, gs = (0, 0) if grad is None else _matrix(grad, "grad", device, logits.dtype, rows, vocab)
+    loss = torch.empty((), dtype=f32, device=device)
+    logp, kl, entropy = torch.empty((3, rows), dtype=f32, device=device).unbind(0)
+    need = _policy_scratch(device.index, code, rows, vocab)
+    work = _scratch(need, device)
+    _call("wc_policy_loss", _POLICY.pack(
+        _POLICY.size, device.index, code, rows, vocab, x, xs, lg, lgs, rl, rls, a,
+        _vector(behaviour_logp, "behaviour_logp", device, f32, rows),
+        _vector(advantages, "advantages", device, f32, rows), _vector(weights, "weights", device, f32, rows),
+        _vector(ref_logp, "ref_logp", device, f32, rows), _scalar(grad_out, "grad_out", device), inv_temperature,
+        clip_low, clip_high, kl_coef, entropy_coef, bits, loss.data_ptr(), logp.data_ptr(), kl.data_ptr(),
+        entropy.data_ptr(), g, gs, work.data_ptr(), need), device)
+    return PolicyLoss(loss, logp, kl, entropy, grad)
+
+
+def preference_loss(logits, tokens, offsets, ref_logp, weights=None, *, beta=0.1, smoothing=0.0, kind="logistic",
+                    average=False, inv_temperature=1.0, grad=True, grad_out=None):
+    """The paired preference loss of ragged sequences of rows of logits, and its gradient (wc_preference_loss).
+
+    logits [rows, vocab]; tokens [rows] and offsets [2 pairs + 1], both int64 or both int32; ref_logp, weights [rows]
+    float32 (weights None: 1). Sequence s is the rows offsets[s] .. offsets[s + 1]; pair i prefers sequence 2i to
+    2i + 1. kind: "logistic", "squared" or "hinge"; average: ratios per unit of weight. grad, grad_out as policy_loss.
+    Returns PreferenceLoss(loss, margins, ratios, logp, grad)."""
+    device, code, rows, vocab, (x, xs) = _logits(logits)
+    t, bits = _indices(tokens, "tokens", device, rows)
+    if offsets.dim() != 1 or offsets.shape[0] % 2 != 1:
+        _fail(f"offsets: shape {tuple(offsets.shape)}, expected (2 pairs + 1,)")
+    pairs = offsets.shape[0] // 2
+    f32 = torch.float32
+    off = _vector(offsets, "offsets", device, tokens.dtype, 2 * pairs + 1)
+    if ref_logp is None:
+        _fail("ref_logp is missing")
+    if grad is True:
+        grad = torch.empty((rows, vocab), dtype=logits.dtype, device=device)
+    elif grad is False:
+        grad = None
+    g, gs = (0, 0) if grad is None else _matrix(grad, "grad", device, logits.dtype, rows, vocab)
+    loss = torch.empty((), dtype=f32, device=device)
+    margins, ratios, logp = torch.empty(3 * pairs + rows, dtype=f32, device=device).split((pairs, 2 * pairs, rows))
+    need = _preference_scratch(device.index, code, rows, vocab, pairs)
+    work = _scratch(need, device)
+    _call("wc_preference_loss", _PREFERENCE.pack(
+        _PREFERENCE.size, device.index, code, rows, vocab, pairs, x, xs, t, off,
+        _vector(ref_logp, "ref_logp", device, f32, rows), _vector(weights, "weights", device, f32, rows),
+        _scalar(grad_out, "grad_out", device), inv_temperature, beta, smoothing, _known(KINDS, kind, "kind"),
+        int(bool(average)), bits, loss.data_ptr(), margins.data_ptr(), ratios.data_ptr(), logp.data_ptr(), g, gs,
+        work.data_ptr(), need), device)
+    return PreferenceLoss(loss, margins, ratios, logp, grad)
+
+
+def _norm_inputs(block, stream, post_gain, post_bias, gate, pre_gain, pre_bias):
+    """What both directions of residual_norm check: device, codes, shape, addresses."""
+    device = _device(block, "block")
+    code = _dtype(block, "block")
+    if block.dim() != 2:
+        _fail(f"block: shape {tuple(block.shape)}, expected rows x width")
+    rows, width = block.shape
+    b = _matrix(block, "block", device, block.dtype, rows, width)
+    s = _matrix(stream, "stream", device, block.dtype, rows, width)
+    vector = gate is not None and gate.dim() == 1
+    dt = next((p.dtype for p in (post_gain, post_bias, gate if vector else None, pre_gain, pre_bias)
+               if p is not None), block.dtype)
+    pcode = DTYPES.get(dt)
+    if pcode is None:
+        _fail(f"gains and biases: {dt} is not one of float32, float16, bfloat16")
+    if gate is None:
+        g = (0, 0)
+    elif vector:
+        g = (_vector(gate, "gate", device, dt, width), 0)
+    else:
+        g = _matrix(gate, "gate", device, block.dtype, rows, width)
+        if g[1] == 0 and rows > 1:
+            _fail("gate: one row for all is given as a vector")
+        g = (g[0], g[1] or width)
+    return (device, code, pcode, rows, width, b, s, _vector(post_gain, "post_gain", device, dt, width),
+            _vector(post_bias, "post_bias", device, dt, width), g, _vector(pre_gain, "pre_gain", device, dt, width),
+            _vector(pre_bias, "pre_bias", device, dt, width))
+
+
+def residual_norm(block, stream, post_gain=None, post_bias=None, gate=None, pre_gain=None, pre_bias=None, *, scale=1.0,
+                  eps=1e-5, norm="layer", gate_act="none", stats=True):
+    """stream' = stream + scale * act(gate) * (norm(block) * post_gain + post_bias), and
+    out = norm(stream') * pre_gain + pre_bias (wc_residual_norm).
+
+    block, stream [rows, width] of one type; gains and biases [width], in that type or another of the three; gate
+    [width] (learned, in the gains' type), [rows, width] (in the matrices' type) or None. norm: "layer" or "rms";
+    gate_act: "none", "sigmoid" or "tanh". Returns ResidualNormOut(stream, out, stats); stats [rows, 4] is what
+    residual_norm_backward needs (stats=False: not kept)."""
+    device, code, pcode, rows, width, b, s, pg, pb, g, ng, nb = _norm_inputs(block, stream, post_gain, post_bias, gate,
+                                                                             pre_gain, pre_bias)
+    new, out = torch.empty((2, rows, width), dtype=block.dtype, device=device).unbind(0)
+    st = torch.empty((rows, 4), dtype=torch.float32, device=device) if stats else None
+    _call("wc_residual_norm", _NORM.pack(
+        _NORM.size, device.index, code, pcode, 0, rows, width, *b, *s, pg, pb, *g, ng, nb, scale, eps,
+        _known(NORMS, norm, "norm"), _known(GATE_ACTS, gate_act, "gate_act"), new.data_ptr(), width, out.data_ptr(),
+        width, st.data_ptr() if stats else 0), device)
+    return ResidualNormOut(new, out, st)
+
+
+def residual_norm_backward(d_out, d_stream, block, stream, stats, post_gain=None, post_bias=None, gate=None,
+                           pre_gain=None, pre_bias=None, *, scale=1.0, eps=1e-5, norm="layer", gate_act="none"):
+    """The gradients of residual_norm from its inputs and its stats (wc_residual_norm_backward).
+
+    d_out arrives at out, d_stream at stream' (either may be None: 0). Returns ResidualNormGrads(block, stream,
+    post_gain, post_bias, gate, pre_gain, pre_bias): matrices in the inputs' type, parameters in float32, None for a
+    parameter that was None."""
+    device, code, pcode, rows, width, b, s, pg, pb, g, ng, _ = _norm_inputs(block, stream, post_gain, post_bias, gate,
+                                                                            pre_gain, pre_bias)
+    dt, f32 = block.dtype, torch.float32
+    do = (0, 0) if d_out is None else _matrix(d_out, "d_out", device, dt, rows, width)
+    ds = (0, 0) if d_stream is None else _matrix(d_stream, "d_stream", device, dt, rows, width)
+    if stats is None:
+        _fail("stats is missing")
+    st, _ = _matrix(stats, "stats", device, f32, rows, 4)
+    if rows > 1 and stats.stride(0) != 4:
+        _fail("stats must be contiguous")
+    token = gate is not None and gate.dim() == 2
+    mats = torch.empty((3 if token else 2, rows, width), dtype=dt, device=device).unbind(0)
+    wanted = [p is not None and not (token and p is gate) for p in (post_gain, post_bias, gate, pre_gain, pre_bias)]
+    sums = iter(torch.empty((sum(wanted), width), dtype=f32, device=device).unbind(0))
+    dpg, dpb, dg, dng, dnb = (next(sums) if w else None for w in wanted)
+    if token:
+        dg = mats[2]
+    need = _norm_scratch(device.index, code, rows, width)
+    work = _scratch(need, device)
+    at = lambda t: 0 if t is None else t.data_ptr()  # noqa: E731
+    _call("wc_residual_norm_backward", _NORM_BACK.pack(
+        _NORM_BACK.size, device.index, code, pcode, 0, rows, width, *b, *s, pg, pb, *g, ng, scale,
+        _known(NORMS, norm, "norm"), _known(GATE_ACTS, gate_act, "gate_act"), 0, st, *do, *ds, mats[0].data_ptr(), width,
+        mats[1].data_ptr(), width, at(dpg), at(dpb), at(dng), at(dnb), at(dg), width, work.data_ptr(), need), device)
+    return ResidualNormGrads(mats[0], mats[1], dpg, dpb, dg, dng, dnb)
+
+
+def _kept(ck):
+    """A checkpoint's device, shape and addresses."""
+    q, exps = ck
+    device = _device(q, "q")
+    if q.dim() != 2:
+        _fail(f"q: shape {tuple(q.shape)}, expected rows x width")
+    rows, width = q.shape
+    return device, rows, width, _matrix(q, "q", device, torch.int8, rows, width), _matrix(
+        exps, "exps", device, torch.uint8, rows, -(-width // GROUP))
+
+
+def _write(x, act, want):
+    device = _device(x, "x")
+    code = _dtype(x, "x")
+    if x.dim() != 2:
+        _fail(f"x: shape {tuple(x.shape)}, expected rows x width")
+    rows, width = x.shape
+    groups = -(-width // GROUP)
+    at = _matrix(x, "x", device, x.dtype, rows, width)
+    q = torch.empty((rows, width), dtype=torch.int8, device=device)
+    exps = torch.empty((rows, groups), dtype=torch.uint8, device=device)
+    y = torch.empty((rows, width), dtype=x.dtype, device=device) if want else None
+    _call("wc_ckpt_write", _CKPT.pack(_CKPT.size, device.index, code, rows, width, _known(ACTS, act, "act"), 0,
+                                      q.data_ptr(), width, exps.data_ptr(), groups, *at, y.data_ptr() if want else 0,
+                                      width), device)
+    return Checkpoint8(q, exps), y
+
+
+def checkpoint8(x):
+    """x [rows, width] kept in 8 bits: Checkpoint8(q, exps), int8 [rows, width] and one exponent byte for each 32
+    channels of a row (wc_ckpt_write)."""
+    return _write(x, "none", False)[0]
+
+
+def checkpoint8_act(x, act):
+    """(Checkpoint8 of x, act(x)) in one pass. act: "relu", "gelu", "silu" or "none"."""
+    return _write(x, act, True)
+
+
+def _read(name, ck, act, grad, dtype):
+    device, rows, width, q, e = _kept(ck)
+    y = torch.empty((rows, width), dtype=dtype, device=device)
+    x = (0, 0) if grad is None else _matrix(grad, "grad", device, dtype, rows, width)
+    _call(name, _CKPT.pack(_CKPT.size, device.index, _dtype(y, "dtype"), rows, width, _known(ACTS, act, "act"), 0, *q, *e,
+                           *x, y.data_ptr(), width), device)
+    return y
+
+
+def checkpoint8_read(ck, dtype=torch.bfloat16, act="none"):
+    """act(what a checkpoint stands for) (wc_ckpt_read)."""
+    return _read("wc_ckpt_read", ck, act, None, dtype)
+
+
+def checkpoint8_act_backward(ck, grad, act):
+    """grad * act'(what a checkpoint stands for) (wc_ckpt_act_backward)."""
+    _device(grad, "grad")
+    return _read("wc_ckpt_act_backward", ck, act, grad, grad.dtype)
+
+
+def checkpoint8_weight_grad(ck, grad, *, act="none", bias=False, dtype=None):
+    """(weight, bias): weight [width, out] = act(kept)^T grad, the gradient of x @ weight; bias [out] float32 = grad's
+    column sums (None unless asked for) (wc_ckpt_weight_grad). dtype: float32 (the default) or grad's."""
+    device, rows, width, q, e = _kept(ck)
+    if _device(grad, "grad") != device or grad.dim() != 2:
+        _fail(f"grad: shape {tuple(grad.shape)} on {grad.device}, expected rows x out on {device}")
+    code, out = _dtype(grad, "grad"), grad.shape[1]
+    g = _matrix(grad, "grad", device, grad.dtype, rows, out)
+    weight = torch.empty((width, out), dtype=dtype or torch.float32, device=device)
+    wcode = _dtype(weight, "dtype")
+    b = torch.empty(out, dtype=torch.float32, device=device) if bias else None
+    a = _known(ACTS, act, "act")
+    need = _weight_scratch(device.index, code, rows, width, out, a, wcode)
+    work = _scratch(need, device)
+    _call("wc_ckpt_weight_grad", _WEIGHT.pack(
+        _WEIGHT.size, device.index, code, rows, width, out, a, wcode, *q, *e, *g, weight.data_ptr(), out,
+        b.data_ptr() if bias else 0, work.data_ptr(), need), device)
+    return weight, b
