@@ -12,12 +12,14 @@ namespace learn {
 typedef _Float16 f16;
 typedef __bf16 bf16;
 
-// Eight consecutive elements. The type asks for the element's alignment only:
+// Consecutive elements. The type asks for the element's alignment only:
 // the hardware takes wide accesses at any, and splits one that crosses a line.
-template <class T>
-struct Vec8 {
-    typedef T type __attribute__((ext_vector_type(8), aligned(sizeof(T))));
+template <class T, int N>
+struct VecN {
+    typedef T type __attribute__((ext_vector_type(N), aligned(sizeof(T))));
 };
+template <class T>
+using Vec8 = VecN<T, 8>;
 
 template <class T>
 __device__ __forceinline__ void load8(const T* __restrict__ p, float (&v)[8]) {

@@ -1,4 +1,13 @@
 // Policy and preference losses over rows of logits (include/wc_learn.h).
+//
+// A row's softmax needs its maximum, then sums over all of it, then, for the
+// gradient, every logit again. Memory bounds it: 4 bytes moved per 16-bit
+// logit against some 20 operations. So a row is read once and held in
+// registers, as it came, from its load to its gradient's store (k_rows), by as
+// few threads as hold it: part of a wavefront for a few heads, one wavefront up
+// to 4 KB, a workgroup up to 256 KB. Longer rows are read twice (k_row_parts,
+// k_row_grads), and so are the preference loss's, whose gradient waits for
+// whole sequences.
 #include <algorithm>
 
 #include "learn.h"
@@ -10,16 +19,14 @@ namespace wc {
 namespace learn {
 namespace {
 
-constexpr int BLOCK = 256;
+// ------------------------------------------------------------------- softmax
 
-// A softmax's running statistics over part of a row: the maximum, the sum of
+// A softmax's statistics over part of a row: the maximum, the sum of
 // e^(x - m), the sum of e^(x - m) (x - m) (for the entropy) and of
 // e^(x - m) (x - y) (for the KL sum), and y's maximum and sum.
 struct Part {
     float m, s, t, d, my, sy;
 };
-
-__device__ __forceinline__ Part none() { return {-INFINITY, 0.f, 0.f, 0.f, -INFINITY, 0.f}; }
 
 // The statistics of two parts together. A part without a finite logit has
 // m = -infinity and adds nothing (its differences would be NaN).
@@ -29,18 +36,14 @@ __device__ __forceinline__ Part join(const Part& a, const Part& b) {
     r.my = fmaxf(a.my, b.my);
     const float da = a.m - r.m, db = b.m - r.m;
     const bool ha = a.m != -INFINITY, hb = b.m != -INFINITY;
-    const float fa = ha ? fast_exp(da) : 0.f, fb = hb ? fast_exp(db) : 0.f;
+    // s alone is kept of a part without a maximum: 0, or the NaN that it found
+    const float fa = ha ? fast_exp(da) : 1.f, fb = hb ? fast_exp(db) : 1.f;
     r.s = a.s * fa + b.s * fb;
     r.t = (ha ? fa * (a.t + a.s * da) : 0.f) + (hb ? fb * (b.t + b.s * db) : 0.f);
     r.d = a.d * fa + b.d * fb;
-    r.sy = (a.my != -INFINITY ? a.sy * fast_exp(a.my - r.my) : 0.f) +
-           (b.my != -INFINITY ? b.sy * fast_exp(b.my - r.my) : 0.f);
+    r.sy = (a.my != -INFINITY ? a.sy * fast_exp(a.my - r.my) : a.sy) +
+           (b.my != -INFINITY ? b.sy * fast_exp(b.my - r.my) : b.sy);
     return r;
-}
-
-__device__ __forceinline__ Part shuffle(const Part& a, int mask) {
-    return {__shfl_xor(a.m, mask), __shfl_xor(a.s, mask), __shfl_xor(a.t, mask),
-            __shfl_xor(a.d, mask), __shfl_xor(a.my, mask), __shfl_xor(a.sy, mask)};
 }
 
 // A logit times the inverse temperature, rounded once and the same everywhere:
@@ -52,7 +55,14 @@ __device__ __forceinline__ float scaled(float x, float inv_temp) {
     return x * inv_temp;
 }
 
-// What one row needs of its logits, and where they are.
+// Logits per 16-byte load.
+template <class T>
+constexpr int EACH = 16 / sizeof(T);
+
+template <class T>
+using Raw = typename VecN<T, EACH<T>>::type;
+
+// What the rows are.
 template <class T>
 struct Rows {
     const T* x;
@@ -75,80 +85,242 @@ struct Rows {
         if (legal && !legal[r * legal_stride + a]) return -1;
         return a;
     }
+};
 
-    // Up to eight logits from column c: illegal and missing ones are -infinity.
-    __device__ __forceinline__ void get(int64_t r, int64_t c, int n, float (&v)[8], float (&u)[8]) const {
-        load_n(x + r * x_stride + c, n, -INFINITY, v);
-        if (y) load_n(y + r * y_stride + c, n, -INFINITY, u);
-        bool on[8];
+// Part of a row as G threads hold it: NV whole 16-byte loads each (-infinity
+// where the row has none), and the columns past the last whole load, one a
+// thread. Wide accesses at one place and single ones at another keep both
+// short: a check per column in each of the NV would cost more registers than
+// the logits.
+template <class T, int G, int NV>
+struct Held {
+    static constexpr int E = EACH<T>;
+    Raw<T> v[NV];
+    T one;
+
+    // Columns 0 .. n of `row`; legal (may be null) alike.
+    __device__ __forceinline__ void load(const T* row, const uint8_t* legal, int n, int lane) {
+        typedef uint8_t Bytes __attribute__((ext_vector_type(E), aligned(1)));
+        const int whole = n / E;
 #pragma unroll
-        for (int i = 0; i < 8; i++) on[i] = i < n && (!legal || legal[r * legal_stride + c + i]);
+        for (int k = 0; k < NV; k++) {
+            const int c = lane + k * G;
+            if (c < whole) {
+                v[k] = *(const Raw<T>*)(row + c * E);
+            } else {
 #pragma unroll
-        for (int i = 0; i < 8; i++) {
-            v[i] = on[i] ? scaled(v[i], inv_temp) : -INFINITY;
-            u[i] = y ? (on[i] ? scaled(u[i], inv_temp) : -INFINITY) : 0.f;
+                for (int i = 0; i < E; i++) v[k][i] = (T)-INFINITY;
+            }
+        }
+        const int last = whole * E + lane;
+        one = last < n && (!legal || legal[last]) ? row[last] : (T)-INFINITY;
+        if (legal) {
+#pragma unroll
+            for (int k = 0; k < NV; k++) {
+                const int c = lane + k * G;
+                if (c < whole) {
+                    const Bytes on = *(const Bytes*)(legal + c * E);
+#pragma unroll
+                    for (int i = 0; i < E; i++) v[k][i] = on[i] ? v[k][i] : (T)-INFINITY;
+                }
+            }
+        }
+    }
+    __device__ __forceinline__ void none() {
+#pragma unroll
+        for (int k = 0; k < NV; k++)
+#pragma unroll
+            for (int i = 0; i < E; i++) v[k][i] = (T)-INFINITY;
+        one = (T)-INFINITY;
+    }
+    // Takes away what the compiler knows of the logits, so that each pass over
+    // them converts them anew: kept as floats from one pass to the next they
+    // would not fit the registers.
+    __device__ __forceinline__ void forget() {
+        typedef uint32_t Words __attribute__((ext_vector_type(4)));
+#pragma unroll
+        for (int k = 0; k < NV; k++) {
+            Words w = __builtin_bit_cast(Words, v[k]);
+            asm volatile("" : "+v"(w));
+            v[k] = __builtin_bit_cast(Raw<T>, w);
         }
     }
 };
 
-__device__ __forceinline__ void add8(Part& p, const float (&v)[8], const float (&u)[8], bool has_y) {
-    Part q = none();
+// Sums and maxima over the G threads that hold a row, the same bits in each: a
+// butterfly in a wavefront, then the wavefronts' values in order through LDS.
+// The slots alternate, so one barrier each is enough: a slot is written again
+// only after a barrier that every reader of its last use has passed.
+template <int G>
+struct Group {
+    static constexpr int WAVES = G > 64 ? G / 64 : 1;
+    typedef float4 Slots[2][WAVES];
+    Slots& lds;
+    int slot = 0;
+
+    template <int N, bool MAX>
+    __device__ __forceinline__ void all(float (&v)[N]) {
 #pragma unroll
-    for (int i = 0; i < 8; i++) q.m = fmaxf(q.m, v[i]);
-    if (q.m == -INFINITY && !has_y) {
-        // nothing here, unless a NaN, which the maximum passes over
-        for (int i = 0; i < 8; i++) q.s += v[i] == -INFINITY ? 0.f : v[i];
-        p.s += q.s;
-        return;
+        for (int mask = (G < 64 ? G : 64) / 2; mask; mask >>= 1)
+#pragma unroll
+            for (int i = 0; i < N; i++) {
+                const float o = __shfl_xor(v[i], mask);
+                v[i] = MAX ? fmaxf(v[i], o) : v[i] + o;
+            }
+        if constexpr (G > 64) {
+            static_assert(N <= 4, "a slot holds four");
+            float* mine = (float*)&lds[slot][threadIdx.x >> 6];
+            if ((threadIdx.x & 63) == 0) {
+#pragma unroll
+                for (int i = 0; i < N; i++) mine[i] = v[i];
+            }
+            __syncthreads();
+#pragma unroll
+            for (int i = 0; i < N; i++) v[i] = MAX ? -INFINITY : 0.f;
+#pragma unroll
+            for (int w = 0; w < WAVES; w++) {
+                const float* o = (const float*)&lds[slot][w];
+#pragma unroll
+                for (int i = 0; i < N; i++) v[i] = MAX ? fmaxf(v[i], o[i]) : v[i] + o[i];
+            }
+            slot ^= 1;
+        }
     }
-#pragma unroll
-    for (int i = 0; i < 8; i++) {
-        const bool in = v[i] != -INFINITY;
-        const float z = v[i] - q.m, e = in ? fast_exp(z) : 0.f;
-        q.s += e;
-        q.t += in ? e * z : 0.f;
-        q.d += in ? e * (v[i] - u[i]) : 0.f;
+};
+
+// Adds one logit to the sums; m and my are the maxima.
+template <bool FULL>
+__device__ __forceinline__ void count(Part& p, float x, float y, float m, float my, float inv_temp) {
+    const float v = scaled(x, inv_temp), z = v - m, e = fast_exp(z);
+    p.s += e;
+    p.t += e * fmaxf(z, -200.f);  // e is 0 there, and 0 * -infinity would be NaN
+    if (FULL) {
+        const float u = scaled(y, inv_temp);
+        p.d += v == -INFINITY ? 0.f : e * (v - u);
+        p.sy += fast_exp(u - my);
     }
-    if (has_y) {
-#pragma unroll
-        for (int i = 0; i < 8; i++) q.my = fmaxf(q.my, u[i]);
-#pragma unroll
-        for (int i = 0; i < 8; i++) q.sy += u[i] != -INFINITY ? fast_exp(u[i] - q.my) : 0.f;
-    }
-    p = join(p, q);
 }
 
-// One row's part [chunk * blockIdx.y ..) of its statistics.
-template <class T>
-__global__ __launch_bounds__(BLOCK) void k_row_parts(Rows<T> in, int64_t rows, int64_t chunk, int splits, Part* parts) {
-    __shared__ Part lds[BLOCK / 64];
-    for (int64_t r = blockIdx.x; r < rows; r += gridDim.x) {
-        if (in.action(r) < 0) continue;
-        const int64_t lo = blockIdx.y * chunk, hi = min(lo + chunk, in.vocab);
-        Part p = none();
-        for (int64_t c = lo + 8 * threadIdx.x; c < hi; c += 8 * BLOCK) {
-            float v[8], u[8];
-            in.get(r, c, (int)min<int64_t>(8, hi - c), v, u);
-            add8(p, v, u, in.y != nullptr);
+// The statistics of the logits that G threads hold. Everything is relative to
+// the common maximum, so one exponential per logit is enough.
+template <class T, int G, int NV, bool FULL>
+__device__ __forceinline__ Part held_stats(Held<T, G, NV>& x, Held<T, G, FULL ? NV : 1>& y, float inv_temp,
+                                           Group<G>& group) {
+    constexpr int E = EACH<T>;
+    Part p = {(float)x.one, 0.f, 0.f, 0.f, FULL ? (float)y.one : -INFINITY, 0.f};
+#pragma unroll
+    for (int k = 0; k < NV; k++) {
+#pragma unroll
+        for (int i = 0; i < E; i++) {
+            p.m = fmaxf(p.m, (float)x.v[k][i]);
+            if (FULL) p.my = fmaxf(p.my, (float)y.v[k][i]);
         }
-        for (int mask = 32; mask; mask >>= 1) p = join(p, shuffle(p, mask));
-        if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = p;
-        __syncthreads();
-        if (threadIdx.x == 0) {
-            for (int w = 1; w < BLOCK / 64; w++) p = join(p, lds[w]);
-            parts[r * splits + blockIdx.y] = p;
-        }
-        __syncthreads();
+        __builtin_amdgcn_sched_barrier(0);  // one load's values converted at a time
     }
+    if constexpr (FULL) {
+        float top[2] = {p.m, p.my};
+        group.template all<2, true>(top);
+        p.m = top[0], p.my = scaled(top[1], inv_temp);
+    } else {
+        float top[1] = {p.m};
+        group.template all<1, true>(top);
+        p.m = top[0];
+    }
+    p.m = scaled(p.m, inv_temp);  // the scale is positive
+    x.forget();
+    if (FULL) y.forget();
+    // a row of nothing but -infinity: 0 keeps its differences -infinity
+    const float m = p.m == -INFINITY ? 0.f : p.m, my = p.my == -INFINITY ? 0.f : p.my;
+    count<FULL>(p, (float)x.one, (float)y.one, m, my, inv_temp);
+#pragma unroll
+    for (int k = 0; k < NV; k++) {
+#pragma unroll
+        for (int i = 0; i < E; i++)
+            count<FULL>(p, (float)x.v[k][i], FULL ? (float)y.v[FULL ? k : 0][i] : 0.f, m, my, inv_temp);
+        __builtin_amdgcn_sched_barrier(0);
+    }
+    if constexpr (FULL) {
+        float sum[4] = {p.s, p.t, p.d, p.sy};
+        group.template all<4, false>(sum);
+        p.s = sum[0], p.t = sum[1], p.d = sum[2], p.sy = sum[3];
+    } else {
+        float sum[2] = {p.s, p.t};
+        group.template all<2, false>(sum);
+        p.s = sum[0], p.t = sum[1];
+    }
+    x.forget();
+    if (FULL) y.forget();
+    return p;
 }
 
-// What a row's gradient needs: inv_temp * (coef ([j = a] - p) + ent p (logp + h) + klc p (logp - logq - kl)).
+// Whether a row has anything to count: a logit above -infinity, or a NaN.
+__device__ __forceinline__ bool counts(const Part& p) { return p.m != -INFINITY || p.s != 0.f; }
+
+// What a row's gradient needs: coef ([j = a] - p) + ent p (logp + h) + klc p (logp - logq - kl).
 // The maximum and the sum's logarithm stay apart: together, a row at a mask's
 // value would lose the second.
 struct RowGrad {
     float m, log_s, my, log_sy, coef, ent, h, klc, kl;
     int32_t on;
+
+    // Without a coefficient (clipped, left out, in no sequence) the gradient is 0 whatever the logits.
+    __device__ __forceinline__ bool any() const { return on && (coef != 0.f || ent != 0.f || klc != 0.f); }
 };
+
+// A row's gradient as a function of a logit: p (base + slope logp - toward logq).
+struct Slope {
+    float m, log_s, my, log_sy, base, slope, toward, hit;
+
+    __device__ __forceinline__ Slope(const RowGrad& g, float go)
+        : m(g.m), log_s(g.log_s), my(g.my), log_sy(g.log_sy), base(go * (g.ent * g.h - g.klc * g.kl - g.coef)),
+          slope(go * (g.ent + g.klc)), toward(go * g.klc), hit(go * g.coef) {}
+
+    template <bool FULL>
+    __device__ __forceinline__ float at(float x, float y, float inv_temp) const {
+        const float v = scaled(x, inv_temp), lp = (v - m) - log_s;
+        // where p is 0 the gradient is, and 0 * infinity would be NaN
+        float d = base + slope * fmaxf(lp, -200.f);
+        if (FULL) d = v == -INFINITY ? 0.f : d - toward * ((scaled(y, inv_temp) - my) - log_sy);
+        return fast_exp(lp) * d;
+    }
+};
+
+// The gradient of the n columns that G threads hold, from column c0 of the
+// row; `a` the action's column, whose gradient has the coefficient more.
+template <class T, int G, int NV, bool FULL>
+__device__ __forceinline__ void put_grad(T* row, int n, int lane, const Held<T, G, NV>& x,
+                                         const Held<T, G, FULL ? NV : 1>& y, const Slope& g, float inv_temp, int a) {
+    constexpr int E = EACH<T>;
+    const int whole = n / E, last = whole * E + lane;
+#pragma unroll
+    for (int k = 0; k < NV; k++) {
+        const int c = lane + k * G;
+        if (c < whole) {
+            Raw<T> o;
+#pragma unroll
+            for (int i = 0; i < E; i++) {
+                const float d = g.at<FULL>((float)x.v[k][i], FULL ? (float)y.v[FULL ? k : 0][i] : 0.f, inv_temp);
+                o[i] = (T)(c * E + i == a ? d + g.hit : d);
+            }
+            *(Raw<T>*)(row + c * E) = o;
+        }
+        __builtin_amdgcn_sched_barrier(0);
+    }
+    if (last < n) {
+        const float d = g.at<FULL>((float)x.one, (float)y.one, inv_temp);
+        row[last] = (T)(last == a ? d + g.hit : d);
+    }
+}
+
+template <class T, int G, int NV>
+__device__ __forceinline__ void put_zero(T* row, int n, int lane) {
+    constexpr int E = EACH<T>;
+    const int whole = n / E, last = whole * E + lane;
+#pragma unroll
+    for (int k = 0; k < NV; k++)
+        if (lane + k * G < whole) *(Raw<T>*)(row + (lane + k * G) * E) = Raw<T>{};
+    if (last < n) row[last] = (T)0.f;
+}
 
 // A counted row's loss, outputs and gradient coefficients from its statistics.
 // The loss's own terms are 64-bit: rows' losses cancel in their sum, and the
@@ -158,50 +330,173 @@ struct PolicyRow {
     float clip_low, clip_high, kl_coef, entropy_coef, even;
     bool full;
     float *logp, *kl, *entropy;
+    double* losses;
+    float* loss;
 
-    __device__ __forceinline__ double finish(int64_t r, const Part& p, float xa, RowGrad* g) const {
+    __device__ __forceinline__ double finish(int64_t r, const Part& p, float xa, RowGrad* g, float3* out) const {
         const float log_s = logf(p.s), lp = (xa - p.m) - log_s, h = log_s - p.t / p.s;
         const float w = weights ? weights[r] : even;
         // e^(x_a - m - behaviour) / s: without the logarithm's rounding and the difference's
         const double adv = advantages[r], ratio = expf((xa - p.m) - behaviour_logp[r]) / p.s;
         const double open = ratio * adv, held = fmin(fmax(ratio, 1.0 - clip_low), 1.0 + clip_high) * adv;
         const bool first = !(open > held);  // a NaN takes this side, and shows
-        float slope = first ? -(float)open : 0.f, k = 0.f;
+        float slope = first ? -(float)open : 0.f, k = 0.f, log_sy = 0.f;
         if (ref_logp) {
             const float off = ref_logp[r] - lp, e = expm1f(off);
             k = e - off;
             slope -= kl_coef * e;
         }
-        if (full) k = p.d / p.s - (p.m - p.my) - (log_s - logf(p.sy));
-        logp[r] = lp;
-        kl[r] = k;
-        entropy[r] = h;
-        *g = {p.m, log_s, p.my, logf(p.sy), w * slope, w * entropy_coef, h, full ? w * kl_coef : 0.f, k, 1};
+        if (full) {
+            log_sy = logf(p.sy);
+            k = p.d / p.s - (p.m - p.my) - (log_s - log_sy);
+        }
+        *out = make_float3(lp, k, h);
+        *g = {p.m, log_s, p.my, log_sy, w * slope, w * entropy_coef, h, full ? w * kl_coef : 0.f, k, 1};
         return w * ((double)kl_coef * k - (first ? open : held) - (double)entropy_coef * h);
     }
 };
 
+// ------------------------------------------------- rows that registers hold
+
+template <int G>
+constexpr int group_block() {
+    return G > 64 ? G : 1024;  // the most; rows of up to a wavefront are launched with 256, or all in one workgroup
+}
+
+// A row on G threads, NV 16-byte loads of logits (FULL: and of the reference's)
+// each. TOKEN: log-probabilities and statistics only, for the preference loss.
+template <class T, int G, int NV, bool FULL, bool TOKEN>
+__global__ __launch_bounds__(group_block<G>()) void k_rows(Rows<T> in, PolicyRow row, int64_t rows, RowGrad* grads,
+                                                           const float* grad_out, T* grad, int64_t grad_stride) {
+    __shared__ typename Group<G>::Slots slots;
+    __shared__ double total[G > 64 ? 1 : 1024 / G];
+    Group<G> group{slots};
+    const int lane = threadIdx.x % G, per = G > 64 ? 1 : blockDim.x / G, n = (int)in.vocab;
+    const float go = (grad_out ? *grad_out : 1.f) * in.inv_temp;
+    double sum = 0.0;
+    for (int64_t r0 = int64_t(blockIdx.x) * per; r0 < rows; r0 += int64_t(gridDim.x) * per) {
+        const int64_t r = r0 + (G > 64 ? 0 : threadIdx.x / G);
+        const int64_t a = r < rows ? in.action(r) : -1;
+        Held<T, G, NV> x;
+        Held<T, G, FULL ? NV : 1> y;
+        y.one = (T)0.f;
+        if (a >= 0) {
+            const uint8_t* legal = in.legal ? in.legal + r * in.legal_stride : nullptr;
+            x.load(in.x + r * in.x_stride, legal, n, lane);
+            if constexpr (FULL) y.load(in.y + r * in.y_stride, legal, n, lane);
+        } else {
+            x.none();
+            if constexpr (FULL) y.none();
+        }
+        RowGrad g;
+        g.m = g.log_s = g.my = g.log_sy = g.coef = g.ent = g.h = g.klc = g.kl = 0.f;
+        g.on = 0;
+        float3 out = make_float3(0.f, 0.f, 0.f);
+        double loss = 0.0;
+        if (G <= 64 || a >= 0) {  // a workgroup's row is left out as one
+            const Part p = held_stats<T, G, NV, FULL>(x, y, in.inv_temp, group);
+            if (a >= 0 && counts(p)) {
+                const float xa = scaled((float)in.x[r * in.x_stride + a], in.inv_temp);
+                if constexpr (TOKEN) {
+                    g.m = p.m;
+                    g.log_s = logf(p.s);
+                    g.on = 1;
+                    out.x = (xa - p.m) - g.log_s;
+                } else {
+                    loss = row.finish(r, p, xa, &g, &out);
+                }
+            }
+        }
+        if (r < rows) {
+            if (lane == 0) {
+                row.logp[r] = out.x;
+                if constexpr (TOKEN) {
+                    grads[r] = g;
+                } else {
+                    row.kl[r] = out.y;
+                    row.entropy[r] = out.z;
+                    if (gridDim.x > 1) row.losses[r] = loss;
+                    else sum += loss;
+                }
+            }
+            if (!TOKEN && grad) {
+                T* to = grad + r * grad_stride;
+                if (g.any()) put_grad<T, G, NV, FULL>(to, n, lane, x, y, Slope(g, go), in.inv_temp, (int)a);
+                else put_zero<T, G, NV>(to, n, lane);
+            }
+        }
+    }
+    if (!TOKEN && gridDim.x == 1) {  // one workgroup: its rows' losses, in order
+        if (lane == 0) total[threadIdx.x / G] = sum;
+        __syncthreads();
+        if (threadIdx.x == 0) {
+            for (int k = 1; k < per; k++) sum += total[k];
+            *row.loss = (float)sum;
+        }
+    }
+}
+
+// -------------------------------------------------------------- longer rows
+
+constexpr int BLOCK = 256;
+constexpr int64_t CHUNK = 8192;  // columns per workgroup
 template <class T>
-__global__ void k_policy_rows(Rows<T> in, PolicyRow row, int64_t rows, int splits, const Part* parts, RowGrad* grads,
-                              double* losses) {
+constexpr int CHUNK_LOADS = CHUNK / (BLOCK * EACH<T>);
+
+// The statistics of one chunk of one row: workgroup r * splits + chunk.
+template <class T, bool FULL>
+__global__ __launch_bounds__(BLOCK) void k_row_parts(Rows<T> in, int64_t tiles, int splits, Part* parts) {
+    constexpr int NV = CHUNK_LOADS<T>;
+    __shared__ typename Group<BLOCK>::Slots slots;
+    Group<BLOCK> group{slots};
+    for (int64_t t = blockIdx.x; t < tiles; t += gridDim.x) {
+        const int64_t r = t / splits, c0 = (t - r * splits) * CHUNK;
+        if (in.action(r) < 0) continue;
+        const uint8_t* legal = in.legal ? in.legal + r * in.legal_stride + c0 : nullptr;
+        const int n = (int)min(CHUNK, in.vocab - c0);
+        Held<T, BLOCK, NV> x;
+        Held<T, BLOCK, FULL ? NV : 1> y;
+        y.one = (T)0.f;
+        x.load(in.x + r * in.x_stride + c0, legal, n, threadIdx.x);
+        if constexpr (FULL) y.load(in.y + r * in.y_stride + c0, legal, n, threadIdx.x);
+        const Part p = held_stats<T, BLOCK, NV, FULL>(x, y, in.inv_temp, group);
+        if (threadIdx.x == 0) parts[t] = p;
+    }
+}
+
+// A row's parts joined, its outputs and coefficients: one thread per row.
+template <class T, bool TOKEN>
+__global__ void k_row_ends(Rows<T> in, PolicyRow row, int64_t rows, int splits, const Part* parts, RowGrad* grads) {
     const int64_t r = int64_t(blockIdx.x) * blockDim.x + threadIdx.x;
     if (r >= rows) return;
     const int64_t a = in.action(r);
-    Part p = none();
+    Part p = {-INFINITY, 0.f, 0.f, 0.f, -INFINITY, 0.f};
     if (a >= 0)
         for (int k = 0; k < splits; k++) p = join(p, parts[r * splits + k]);
     RowGrad g = {};
+    float3 out = make_float3(0.f, 0.f, 0.f);
     double loss = 0.0;
-    if (p.m != -INFINITY || p.s != 0.f) {
-        loss = row.finish(r, p, scaled((float)in.x[r * in.x_stride + a], in.inv_temp), &g);
-    } else {
-        row.logp[r] = row.kl[r] = row.entropy[r] = 0.f;
+    if (counts(p)) {
+        const float xa = scaled((float)in.x[r * in.x_stride + a], in.inv_temp);
+        if (TOKEN) {
+            g.m = p.m;
+            g.log_s = logf(p.s);
+            g.on = 1;
+            out.x = (xa - p.m) - g.log_s;
+        } else {
+            loss = row.finish(r, p, xa, &g, &out);
+        }
     }
+    row.logp[r] = out.x;
     grads[r] = g;
-    losses[r] = loss;
+    if (!TOKEN) {
+        row.kl[r] = out.y;
+        row.entropy[r] = out.z;
+        row.losses[r] = loss;
+    }
 }
 
-// The sum of n row losses in a fixed order, in 64 bits.
+// The sum of n losses in a fixed order.
 __global__ __launch_bounds__(1024) void k_sum(const double* v, int64_t n, double scale, float* out) {
     __shared__ double lds[16];
     double s = 0;
@@ -215,45 +510,34 @@ __global__ __launch_bounds__(1024) void k_sum(const double* v, int64_t n, double
     }
 }
 
-template <class T>
-__global__ __launch_bounds__(BLOCK) void k_row_grads(Rows<T> in, int64_t rows, int64_t chunk, const RowGrad* grads,
+// The gradient from the rows' coefficients, a second read of the logits. The
+// last rows go first: they are what the pass before left in the caches.
+template <class T, bool FULL>
+__global__ __launch_bounds__(BLOCK) void k_row_grads(Rows<T> in, int64_t tiles, int splits, const RowGrad* grads,
                                                      const float* grad_out, T* out, int64_t out_stride) {
+    constexpr int NV = CHUNK_LOADS<T>;
     const float go = (grad_out ? *grad_out : 1.f) * in.inv_temp;
-    for (int64_t r = blockIdx.x; r < rows; r += gridDim.x) {
+    for (int64_t i = blockIdx.x; i < tiles; i += gridDim.x) {
+        const int64_t t = tiles - 1 - i, r = t / splits, c0 = (t - r * splits) * CHUNK;
         const RowGrad g = grads[r];
-        // without a coefficient (clipped, left out, in no sequence) the gradient is 0 whatever the logits
-        const bool on = g.on && (g.coef != 0.f || g.ent != 0.f || g.klc != 0.f);
-        const int64_t a = on ? index_at(in.actions, in.bits, r) : -1;
-        const int64_t lo = blockIdx.y * chunk, hi = min(lo + chunk, in.vocab);
-        for (int64_t c = lo + 8 * threadIdx.x; c < hi; c += 8 * BLOCK) {
-            const int n = (int)min<int64_t>(8, hi - c);
-            float o[8] = {};
-            if (on) {
-                float v[8], u[8];
-                in.get(r, c, n, v, u);
-#pragma unroll
-                for (int i = 0; i < 8; i++) {
-                    if (v[i] == -INFINITY) continue;
-                    const float lp = (v[i] - g.m) - g.log_s, p = fast_exp(lp);
-                    float d = -g.coef;
-                    if (g.ent != 0.f) d += g.ent * (lp + g.h);
-                    if (g.klc != 0.f) d += g.klc * (lp - ((u[i] - g.my) - g.log_sy) - g.kl);
-                    o[i] = go * (p * d + (c + i == a ? g.coef : 0.f));
-                }
-            }
-            store_n(out + r * out_stride + c, n, o);
+        T* to = out + r * out_stride + c0;
+        const int n = (int)min(CHUNK, in.vocab - c0);
+        if (!g.any()) {
+            put_zero<T, BLOCK, NV>(to, n, threadIdx.x);
+            continue;
         }
+        const int64_t a = index_at(in.actions, in.bits, r) - c0;
+        const uint8_t* legal = in.legal ? in.legal + r * in.legal_stride + c0 : nullptr;
+        Held<T, BLOCK, NV> x;
+        Held<T, BLOCK, FULL ? NV : 1> y;
+        y.one = (T)0.f;
+        x.load(in.x + r * in.x_stride + c0, legal, n, threadIdx.x);
+        if constexpr (FULL) y.load(in.y + r * in.y_stride + c0, legal, n, threadIdx.x);
+        put_grad<T, BLOCK, NV, FULL>(to, n, threadIdx.x, x, y, Slope(g, go), in.inv_temp, a >= 0 && a < n ? (int)a : -1);
     }
 }
 
-// Columns of one row go to workgroups in chunks of at least 4096, so that few
-// rows still fill the device.
-void split(int64_t rows, int64_t vocab, int cus, int64_t* chunk, int* splits) {
-    const int64_t most = (vocab + 4095) / 4096, want = std::max<int64_t>(1, 8 * cus / std::max<int64_t>(rows, 1));
-    const int64_t n = std::max<int64_t>(1, std::min(most, want));
-    *chunk = ((vocab + n - 1) / n + 7) / 8 * 8;
-    *splits = (int)((vocab + *chunk - 1) / *chunk);
-}
+// ------------------------------------------------------------------ launches
 
 template <class T>
 Rows<T> rows_of(const wc_policy_args& a) {
@@ -267,54 +551,73 @@ Rows<T> rows_of(const wc_preference_args& a) {
             a.inv_temperature, a.index_bits};
 }
 
-uint32_t grid_rows(int64_t rows) { return (uint32_t)std::min<int64_t>(rows, 1 << 20); }
+int splits_of(int64_t vocab) { return (int)((vocab + CHUNK - 1) / CHUNK); }
 
-template <class T>
-void policy(const wc_policy_args& a, int cus, hipStream_t s) {
-    int64_t chunk;
-    int splits;
-    split(a.rows, a.vocab, cus, &chunk, &splits);
-    uint8_t* w = (uint8_t*)a.workspace;
-    Part* parts = (Part*)w;
-    RowGrad* grads = (RowGrad*)(w += pad256(size_t(a.rows) * splits * sizeof(Part)));
-    double* losses = (double*)(w += pad256(size_t(a.rows) * sizeof(RowGrad)));
+uint32_t tile_grid(int64_t tiles) { return (uint32_t)std::min<int64_t>(tiles, 1 << 22); }
+
+// Whether k_rows holds a row: up to 64 registers per thread of 1,024.
+bool holds(int dtype, int64_t vocab, bool full) {
+    return vocab * (dtype == WC_DTYPE_F32 ? 4 : 2) * (full ? 2 : 1) <= 256 << 10;
+}
+
+template <class T, int G, int NV, bool FULL, bool TOKEN>
+void rows_at(const Rows<T>& in, const PolicyRow& row, int64_t rows, RowGrad* grads, const float* grad_out, T* grad,
+             int64_t grad_stride, hipStream_t s, bool* whole) {
+    // rows that one workgroup holds at once go to one, which then sums their losses itself
+    const int block = G > 64 ? G : rows * G <= 1024 ? (int)std::max<int64_t>(64, (rows * G + 63) / 64 * 64) : 256;
+    const int64_t per = block / G, grid = std::min<int64_t>((rows + per - 1) / per, 1 << 22);
+    *whole = grid == 1;
+    k_rows<T, G, NV, FULL, TOKEN><<<dim3((uint32_t)grid), block, 0, s>>>(in, row, rows, grads, grad_out, grad,
+                                                                         grad_stride);
+}
+
+// The fewest threads that hold a row in at most four loads each while they are
+// one wavefront, and in at most sixteen (eight with the reference's logits)
+// beyond.
+template <class T, bool FULL, bool TOKEN>
+void rows_held(const Rows<T>& in, const PolicyRow& row, int64_t rows, RowGrad* grads, const float* go, T* grad,
+               int64_t gs, hipStream_t s, bool* whole) {
+    const int64_t n = (in.vocab + EACH<T> - 1) / EACH<T>;
+    if (n <= 8) rows_at<T, 8, 1, FULL, TOKEN>(in, row, rows, grads, go, grad, gs, s, whole);
+    else if (n <= 16) rows_at<T, 16, 1, FULL, TOKEN>(in, row, rows, grads, go, grad, gs, s, whole);
+    else if (n <= 32) rows_at<T, 32, 1, FULL, TOKEN>(in, row, rows, grads, go, grad, gs, s, whole);
+    else if (n <= 64) rows_at<T, 64, 1, FULL, TOKEN>(in, row, rows, grads, go, grad, gs, s, whole);
+    else if (n <= 128) rows_at<T, 64, 2, FULL, TOKEN>(in, row, rows, grads, go, grad, gs, s, whole);
+    else if (n <= 192) rows_at<T, 64, 3, FULL, TOKEN>(in, row, rows, grads, go, grad, gs, s, whole);
+    else if (n <= 256) rows_at<T, 64, 4, FULL, TOKEN>(in, row, rows, grads, go, grad, gs, s, whole);
+    else if (n <= 512) rows_at<T, 256, 2, FULL, TOKEN>(in, row, rows, grads, go, grad, gs, s, whole);
+    else if (n <= 1024) rows_at<T, 256, 4, FULL, TOKEN>(in, row, rows, grads, go, grad, gs, s, whole);
+    else if (n <= 2048) rows_at<T, 1024, 2, FULL, TOKEN>(in, row, rows, grads, go, grad, gs, s, whole);
+    else if (n <= 4096) rows_at<T, 1024, 4, FULL, TOKEN>(in, row, rows, grads, go, grad, gs, s, whole);
+    else if (n <= 8192) rows_at<T, 1024, 8, FULL, TOKEN>(in, row, rows, grads, go, grad, gs, s, whole);
+    else if constexpr (!FULL) rows_at<T, 1024, 16, FULL, TOKEN>(in, row, rows, grads, go, grad, gs, s, whole);
+}
+
+template <class T, bool FULL>
+void policy(const wc_policy_args& a, hipStream_t s) {
     const Rows<T> in = rows_of<T>(a);
-    const PolicyRow row = {a.behaviour_logp, a.advantages, a.weights, a.ref_logp, a.clip_low, a.clip_high, a.kl_coef,
-                           a.entropy_coef, 1.f / (float)std::max<int64_t>(a.rows, 1), a.ref_logits != nullptr, a.logp, a.kl, a.entropy};
-    if (a.rows) {
-        const dim3 grid(grid_rows(a.rows), splits);
-        k_row_parts<T><<<grid, BLOCK, 0, s>>>(in, a.rows, chunk, splits, parts);
-        k_policy_rows<T><<<dim3((a.rows + 63) / 64), 64, 0, s>>>(in, row, a.rows, splits, parts, grads, losses);
+    uint8_t* w = (uint8_t*)a.workspace;
+    PolicyRow row = {a.behaviour_logp, a.advantages, a.weights, a.ref_logp, a.clip_low, a.clip_high, a.kl_coef,
+                     a.entropy_coef, 1.f / (float)std::max<int64_t>(a.rows, 1), FULL, a.logp, a.kl, a.entropy,
+                     (double*)w, a.loss};
+    bool whole = false;
+    if (a.rows && holds(a.dtype, a.vocab, FULL)) {
+        rows_held<T, FULL, false>(in, row, a.rows, nullptr, a.grad_out, (T*)a.grad, a.grad_stride, s, &whole);
+    } else if (a.rows) {
+        const int splits = splits_of(a.vocab);
+        const int64_t tiles = a.rows * splits;
+        RowGrad* grads = (RowGrad*)(w += pad256(size_t(a.rows) * sizeof(double)));
+        Part* parts = (Part*)(w += pad256(size_t(a.rows) * sizeof(RowGrad)));
+        k_row_parts<T, FULL><<<tile_grid(tiles), BLOCK, 0, s>>>(in, tiles, splits, parts);
+        k_row_ends<T, false><<<dim3((uint32_t)((a.rows + 63) / 64)), 64, 0, s>>>(in, row, a.rows, splits, parts, grads);
+        if (a.grad)
+            k_row_grads<T, FULL><<<tile_grid(tiles), BLOCK, 0, s>>>(in, tiles, splits, grads, a.grad_out, (T*)a.grad,
+                                                                    a.grad_stride);
     }
-    k_sum<<<1, 1024, 0, s>>>(losses, a.rows, 1.0, a.loss);
-    if (a.grad && a.rows) {
-        const dim3 grid(grid_rows(a.rows), splits);
-        k_row_grads<T><<<grid, BLOCK, 0, s>>>(in, a.rows, chunk, grads, a.grad_out, (T*)a.grad, a.grad_stride);
-    }
+    if (!whole) k_sum<<<1, 1024, 0, s>>>(row.losses, a.rows, 1.0, a.loss);
 }
 
-// -------------------------------------------------------------- preference
-
-template <class T>
-__global__ void k_token_rows(Rows<T> in, int64_t rows, int splits, const Part* parts, float* logp, RowGrad* grads) {
-    const int64_t r = int64_t(blockIdx.x) * blockDim.x + threadIdx.x;
-    if (r >= rows) return;
-    const int64_t a = in.action(r);
-    Part p = none();
-    if (a >= 0)
-        for (int k = 0; k < splits; k++) p = join(p, parts[r * splits + k]);
-    RowGrad g = {};
-    float lp = 0.f;
-    if (p.m != -INFINITY || p.s != 0.f) {
-        const float log_s = logf(p.s);
-        lp = (scaled((float)in.x[r * in.x_stride + a], in.inv_temp) - p.m) - log_s;
-        g.m = p.m;
-        g.log_s = log_s;
-        g.on = 1;
-    }
-    logp[r] = lp;
-    grads[r] = g;
-}
+// ---------------------------------------------------------------- preference
 
 struct Pairs {
     const void* offsets;
@@ -359,7 +662,7 @@ __global__ __launch_bounds__(BLOCK) void k_pairs(Pairs p, const float* logp, Row
     const double h = ratio[0] - ratio[1], z = p.beta * h;
     double loss, d;
     if (p.kind == WC_PREFERENCE_LOGISTIC) {
-        const double tail = log1p(exp(-fabs(z))), e = exp(-fabs(z));
+        const double e = exp(-fabs(z)), tail = log1p(e);
         loss = tail + (1.0 - p.smoothing) * fmax(-z, 0.0) + p.smoothing * fmax(z, 0.0);
         d = p.beta * ((z >= 0 ? 1.0 / (1.0 + e) : e / (1.0 + e)) - (1.0 - p.smoothing));
         if (z != z) loss = z;
@@ -387,56 +690,63 @@ __global__ __launch_bounds__(BLOCK) void k_pairs(Pairs p, const float* logp, Row
 }
 
 template <class T>
-void preference(const wc_preference_args& a, int cus, hipStream_t s) {
-    int64_t chunk;
-    int splits;
-    split(a.rows, a.vocab, cus, &chunk, &splits);
-    uint8_t* w = (uint8_t*)a.workspace;
-    Part* parts = (Part*)w;
-    RowGrad* grads = (RowGrad*)(w += pad256(size_t(a.rows) * splits * sizeof(Part)));
-    double* losses = (double*)(w += pad256(size_t(a.rows) * sizeof(RowGrad)));
+void preference(const wc_preference_args& a, hipStream_t s) {
     const Rows<T> in = rows_of<T>(a);
+    const int splits = splits_of(a.vocab);
+    const int64_t tiles = a.rows * splits;
+    uint8_t* w = (uint8_t*)a.workspace;
+    RowGrad* grads = (RowGrad*)w;
+    double* losses = (double*)(w += pad256(size_t(a.rows) * sizeof(RowGrad)));
+    PolicyRow row = {};
+    row.logp = a.logp;
+    if (a.rows && holds(a.dtype, a.vocab, false)) {
+        bool whole;
+        rows_held<T, false, true>(in, row, a.rows, grads, nullptr, nullptr, 0, s, &whole);
+    } else if (a.rows) {
+        Part* parts = (Part*)(w += pad256(size_t(a.pairs) * sizeof(double)));
+        k_row_parts<T, false><<<tile_grid(tiles), BLOCK, 0, s>>>(in, tiles, splits, parts);
+        k_row_ends<T, true><<<dim3((uint32_t)((a.rows + 63) / 64)), 64, 0, s>>>(in, row, a.rows, splits, parts, grads);
+    }
     const Pairs p = {a.offsets, a.ref_logp, a.weights, a.rows, a.pairs, a.beta, a.smoothing, a.kind, a.average,
                      a.index_bits};
-    if (a.rows) {
-        k_row_parts<T><<<dim3(grid_rows(a.rows), splits), BLOCK, 0, s>>>(in, a.rows, chunk, splits, parts);
-        k_token_rows<T><<<dim3((a.rows + 63) / 64), 64, 0, s>>>(in, a.rows, splits, parts, a.logp, grads);
-    }
-    if (a.pairs) k_pairs<<<dim3(a.pairs), BLOCK, 0, s>>>(p, a.logp, grads, losses, a.margins, a.ratios);
+    if (a.pairs) k_pairs<<<dim3((uint32_t)a.pairs), BLOCK, 0, s>>>(p, a.logp, grads, losses, a.margins, a.ratios);
     k_sum<<<1, 1024, 0, s>>>(losses, a.pairs, a.pairs ? 1.0 / (double)a.pairs : 0.0, a.loss);
     if (a.grad && a.rows)
-        k_row_grads<T><<<dim3(grid_rows(a.rows), splits), BLOCK, 0, s>>>(in, a.rows, chunk, grads, a.grad_out,
-                                                                         (T*)a.grad, a.grad_stride);
+        k_row_grads<T, false><<<tile_grid(tiles), BLOCK, 0, s>>>(in, tiles, splits, grads, a.grad_out, (T*)a.grad,
+                                                                 a.grad_stride);
+}
+
+template <class T>
+void policy_of(const wc_policy_args& a, hipStream_t s) {
+    if (a.ref_logits) policy<T, true>(a, s);
+    else policy<T, false>(a, s);
 }
 
 }  // namespace
 
-size_t policy_scratch(const wc_policy_args& a, int cus) {
-    int64_t chunk;
-    int splits;
-    split(a.rows, a.vocab, cus, &chunk, &splits);
-    return pad256(size_t(a.rows) * splits * sizeof(Part)) + pad256(size_t(a.rows) * sizeof(RowGrad)) +
-           pad256(size_t(a.rows) * sizeof(double));
+size_t policy_scratch(const wc_policy_args& a, int) {
+    const size_t losses = pad256(size_t(a.rows) * sizeof(double));
+    // the size of the two-pass form, whether or not the call has a reference: the binding asks by shape
+    return holds(a.dtype, a.vocab, true) ? losses
+                                         : losses + pad256(size_t(a.rows) * sizeof(RowGrad)) +
+                                               pad256(size_t(a.rows) * splits_of(a.vocab) * sizeof(Part));
 }
 
-size_t preference_scratch(const wc_preference_args& a, int cus) {
-    int64_t chunk;
-    int splits;
-    split(a.rows, a.vocab, cus, &chunk, &splits);
-    return pad256(size_t(a.rows) * splits * sizeof(Part)) + pad256(size_t(a.rows) * sizeof(RowGrad)) +
-           pad256(size_t(a.pairs) * sizeof(double));
+size_t preference_scratch(const wc_preference_args& a, int) {
+    const size_t base = pad256(size_t(a.rows) * sizeof(RowGrad)) + pad256(size_t(a.pairs) * sizeof(double));
+    return holds(a.dtype, a.vocab, false) ? base : base + pad256(size_t(a.rows) * splits_of(a.vocab) * sizeof(Part));
 }
 
-void launch_policy(const wc_policy_args& a, int cus, hipStream_t s) {
-    if (a.dtype == WC_DTYPE_F32) policy<float>(a, cus, s);
-    else if (a.dtype == WC_DTYPE_F16) policy<f16>(a, cus, s);
-    else policy<bf16>(a, cus, s);
+void launch_policy(const wc_policy_args& a, int, hipStream_t s) {
+    if (a.dtype == WC_DTYPE_F32) policy_of<float>(a, s);
+    else if (a.dtype == WC_DTYPE_F16) policy_of<f16>(a, s);
+    else policy_of<bf16>(a, s);
 }
 
-void launch_preference(const wc_preference_args& a, int cus, hipStream_t s) {
-    if (a.dtype == WC_DTYPE_F32) preference<float>(a, cus, s);
-    else if (a.dtype == WC_DTYPE_F16) preference<f16>(a, cus, s);
-    else preference<bf16>(a, cus, s);
+void launch_preference(const wc_preference_args& a, int, hipStream_t s) {
+    if (a.dtype == WC_DTYPE_F32) preference<float>(a, s);
+    else if (a.dtype == WC_DTYPE_F16) preference<f16>(a, s);
+    else preference<bf16>(a, s);
 }
 
 }  // namespace learn
