@@ -20,7 +20,7 @@ ARCH = os.environ.get("WC_OFFLOAD_ARCH", "gfx950")
 
 SOURCES = ["job.cpp", "synth.cpp", "wave.cpp", "capi_host.cpp", "executor.cpp", "service.cpp", "capi_gpu.cpp",
            "kernels.hip", "exact.hip", "noalloc.hip", "v5.hip", "probe.hip", "check.hip",
-           "capi_learn.cpp", "policy.hip", "resnorm.hip", "ckpt8.hip", "ckpt8_weight.hip"]
+           "capi_learn.cpp", "policy.hip", "policy_f32.hip", "policy_f16.hip", "policy_bf16.hip", "resnorm.hip", "ckpt8.hip", "ckpt8_weight.hip"]
 
 COMMON = ["-O3", "-std=c++17", "-fPIC", "-Wall", "-Wno-unused-result", "-ffp-contract=off"]
 DEVICE = [f"--offload-arch={ARCH}", "-fhip-fp32-correctly-rounded-divide-sqrt", "-fno-gpu-flush-denormals-to-zero",

@@ -26,6 +26,14 @@ void launch_ckpt_read(const wc_ckpt_args& a, int cus, hipStream_t s);
 void launch_ckpt_act_back(const wc_ckpt_args& a, int cus, hipStream_t s);
 void launch_ckpt_weight(const wc_ckpt_weight_args& a, int cus, hipStream_t s);
 
+// The losses by element type.
+void policy_f32(const wc_policy_args& a, hipStream_t s);
+void policy_f16(const wc_policy_args& a, hipStream_t s);
+void policy_bf16(const wc_policy_args& a, hipStream_t s);
+void preference_f32(const wc_preference_args& a, hipStream_t s);
+void preference_f16(const wc_preference_args& a, hipStream_t s);
+void preference_bf16(const wc_preference_args& a, hipStream_t s);
+
 inline size_t pad256(size_t x) { return (x + 255) & ~size_t(255); }
 
 }  // namespace learn

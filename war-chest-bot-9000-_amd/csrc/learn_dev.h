@@ -53,10 +53,12 @@ __device__ __forceinline__ void store_n(T* __restrict__ p, int n, const float (&
         if (i < n) p[i] = (T)v[i];
 }
 
-// e^x by the hardware's 2^x (1 ulp; a result under 2^-126 is 0). Callers take
-// x as a difference to a row's maximum, so that x log2(e) is off by less than
-// an ulp of a small number.
-__device__ __forceinline__ float fast_exp(float x) { return __builtin_amdgcn_exp2f(x * 1.4426950408889634f); }
+// 2^x by the hardware (1 ulp; a result under 2^-126 is 0).
+__device__ __forceinline__ float power(float x) { return __builtin_amdgcn_exp2f(x); }
+
+// e^x for the sigmoids: for the arguments that matter there x log2(e) is off by
+// less than a millionth.
+__device__ __forceinline__ float fast_exp(float x) { return power(x * 1.4426950408889634f); }
 
 __device__ __forceinline__ int64_t index_at(const void* p, int bits, int64_t i) {
     return bits == 64 ? ((const int64_t*)p)[i] : (int64_t)((const int32_t*)p)[i];

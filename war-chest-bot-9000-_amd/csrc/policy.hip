@@ -1,728 +1,8 @@
-// Policy and preference losses over rows of logits (include/wc_learn.h).
-//
-// A row's softmax needs its maximum, then sums over all of it, then, for the
-// gradient, every logit again. Memory bounds it: 4 bytes moved per 16-bit
-// logit against some 20 operations. So a row is read once and held in
-// registers, as it came, from its load to its gradient's store (k_rows), by as
-// few threads as hold it: part of a wavefront for a few heads, one wavefront up
-// to 4 KB, a workgroup up to 256 KB. Longer rows are read twice (k_row_parts,
-// k_row_grads), and so are the preference loss's, whose gradient waits for
-// whole sequences.
-#include <algorithm>
-
-#include "learn.h"
-#include "learn_dev.h"
-
-#pragma clang fp contract(fast)
+// The losses' scratch sizes, and their launches by element type (policy_dev.h).
+#include "policy_dev.h"
 
 namespace wc {
 namespace learn {
-namespace {
-
-// ------------------------------------------------------------------- softmax
-
-// A softmax's statistics over part of a row: the maximum, the sum of
-// e^(x - m), the sum of e^(x - m) (x - m) (for the entropy) and of
-// e^(x - m) (x - y) (for the KL sum), and y's maximum and sum.
-struct Part {
-    float m, s, t, d, my, sy;
-};
-
-// The statistics of two parts together. A part without a finite logit has
-// m = -infinity and adds nothing (its differences would be NaN).
-__device__ __forceinline__ Part join(const Part& a, const Part& b) {
-    Part r;
-    r.m = fmaxf(a.m, b.m);
-    r.my = fmaxf(a.my, b.my);
-    const float da = a.m - r.m, db = b.m - r.m;
-    const bool ha = a.m != -INFINITY, hb = b.m != -INFINITY;
-    // s alone is kept of a part without a maximum: 0, or the NaN that it found
-    const float fa = ha ? fast_exp(da) : 1.f, fb = hb ? fast_exp(db) : 1.f;
-    r.s = a.s * fa + b.s * fb;
-    r.t = (ha ? fa * (a.t + a.s * da) : 0.f) + (hb ? fb * (b.t + b.s * db) : 0.f);
-    r.d = a.d * fa + b.d * fb;
-    r.sy = (a.my != -INFINITY ? a.sy * fast_exp(a.my - r.my) : a.sy) +
-           (b.my != -INFINITY ? b.sy * fast_exp(b.my - r.my) : b.sy);
-    return r;
-}
-
-// A logit times the inverse temperature, rounded once and the same everywhere:
-// contracted into a later difference, the product of a row's maximum would
-// differ from itself by its rounding, which for a mask of the type's lowest
-// value is 1e30.
-__device__ __forceinline__ float scaled(float x, float inv_temp) {
-#pragma clang fp contract(off)
-    return x * inv_temp;
-}
-
-// Logits per 16-byte load.
-template <class T>
-constexpr int EACH = 16 / sizeof(T);
-
-template <class T>
-using Raw = typename VecN<T, EACH<T>>::type;
-
-// What the rows are.
-template <class T>
-struct Rows {
-    const T* x;
-    int64_t x_stride;
-    const uint8_t* legal;
-    int64_t legal_stride;
-    const T* y;
-    int64_t y_stride;
-    const void* actions;
-    const float* weights;
-    int64_t vocab;
-    float inv_temp;
-    int bits;
-
-    // The row's action, or -1 for a row that is left out before its logits are read.
-    __device__ __forceinline__ int64_t action(int64_t r) const {
-        if (weights && weights[r] == 0.f) return -1;
-        const int64_t a = index_at(actions, bits, r);
-        if (a < 0 || a >= vocab) return -1;
-        if (legal && !legal[r * legal_stride + a]) return -1;
-        return a;
-    }
-};
-
-// Part of a row as G threads hold it: NV whole 16-byte loads each (-infinity
-// where the row has none), and the columns past the last whole load, one a
-// thread. Wide accesses at one place and single ones at another keep both
-// short: a check per column in each of the NV would cost more registers than
-// the logits.
-template <class T, int G, int NV>
-struct Held {
-    static constexpr int E = EACH<T>;
-    Raw<T> v[NV];
-    T one;
-
-    // Columns 0 .. n of `row`; legal (may be null) alike.
-    __device__ __forceinline__ void load(const T* row, const uint8_t* legal, int n, int lane) {
-        typedef uint8_t Bytes __attribute__((ext_vector_type(E), aligned(1)));
-        const int whole = n / E;
-#pragma unroll
-        for (int k = 0; k < NV; k++) {
-            const int c = lane + k * G;
-            if (c < whole) {
-                v[k] = *(const Raw<T>*)(row + c * E);
-            } else {
-#pragma unroll
-                for (int i = 0; i < E; i++) v[k][i] = (T)-INFINITY;
-            }
-        }
-        const int last = whole * E + lane;
-        one = last < n && (!legal || legal[last]) ? row[last] : (T)-INFINITY;
-        if (legal) {
-#pragma unroll
-            for (int k = 0; k < NV; k++) {
-                const int c = lane + k * G;
-                if (c < whole) {
-                    const Bytes on = *(const Bytes*)(legal + c * E);
-#pragma unroll
-                    for (int i = 0; i < E; i++) v[k][i] = on[i] ? v[k][i] : (T)-INFINITY;
-                }
-            }
-        }
-    }
-    __device__ __forceinline__ void none() {
-#pragma unroll
-        for (int k = 0; k < NV; k++)
-#pragma unroll
-            for (int i = 0; i < E; i++) v[k][i] = (T)-INFINITY;
-        one = (T)-INFINITY;
-    }
-    // Takes away what the compiler knows of the logits, so that each pass over
-    // them converts them anew: kept as floats from one pass to the next they
-    // would not fit the registers.
-    __device__ __forceinline__ void forget() {
-        typedef uint32_t Words __attribute__((ext_vector_type(4)));
-#pragma unroll
-        for (int k = 0; k < NV; k++) {
-            Words w = __builtin_bit_cast(Words, v[k]);
-            asm volatile("" : "+v"(w));
-            v[k] = __builtin_bit_cast(Raw<T>, w);
-        }
-    }
-};
-
-// Sums and maxima over the G threads that hold a row, the same bits in each: a
-// butterfly in a wavefront, then the wavefronts' values in order through LDS.
-// The slots alternate, so one barrier each is enough: a slot is written again
-// only after a barrier that every reader of its last use has passed.
-template <int G>
-struct Group {
-    static constexpr int WAVES = G > 64 ? G / 64 : 1;
-    typedef float4 Slots[2][WAVES];
-    Slots& lds;
-    int slot = 0;
-
-    template <int N, bool MAX>
-    __device__ __forceinline__ void all(float (&v)[N]) {
-#pragma unroll
-        for (int mask = (G < 64 ? G : 64) / 2; mask; mask >>= 1)
-#pragma unroll
-            for (int i = 0; i < N; i++) {
-                const float o = __shfl_xor(v[i], mask);
-                v[i] = MAX ? fmaxf(v[i], o) : v[i] + o;
-            }
-        if constexpr (G > 64) {
-            static_assert(N <= 4, "a slot holds four");
-            float* mine = (float*)&lds[slot][threadIdx.x >> 6];
-            if ((threadIdx.x & 63) == 0) {
-#pragma unroll
-                for (int i = 0; i < N; i++) mine[i] = v[i];
-            }
-            __syncthreads();
-#pragma unroll
-            for (int i = 0; i < N; i++) v[i] = MAX ? -INFINITY : 0.f;
-#pragma unroll
-            for (int w = 0; w < WAVES; w++) {
-                const float* o = (const float*)&lds[slot][w];
-#pragma unroll
-                for (int i = 0; i < N; i++) v[i] = MAX ? fmaxf(v[i], o[i]) : v[i] + o[i];
-            }
-            slot ^= 1;
-        }
-    }
-};
-
-// Adds one logit to the sums; m and my are the maxima.
-template <bool FULL>
-__device__ __forceinline__ void count(Part& p, float x, float y, float m, float my, float inv_temp) {
-    const float v = scaled(x, inv_temp), z = v - m, e = fast_exp(z);
-    p.s += e;
-    p.t += e * fmaxf(z, -200.f);  // e is 0 there, and 0 * -infinity would be NaN
-    if (FULL) {
-        const float u = scaled(y, inv_temp);
-        p.d += v == -INFINITY ? 0.f : e * (v - u);
-        p.sy += fast_exp(u - my);
-    }
-}
-
-// The statistics of the logits that G threads hold. Everything is relative to
-// the common maximum, so one exponential per logit is enough.
-template <class T, int G, int NV, bool FULL>
-__device__ __forceinline__ Part held_stats(Held<T, G, NV>& x, Held<T, G, FULL ? NV : 1>& y, float inv_temp,
-                                           Group<G>& group) {
-    constexpr int E = EACH<T>;
-    Part p = {(float)x.one, 0.f, 0.f, 0.f, FULL ? (float)y.one : -INFINITY, 0.f};
-#pragma unroll
-    for (int k = 0; k < NV; k++) {
-#pragma unroll
-        for (int i = 0; i < E; i++) {
-            p.m = fmaxf(p.m, (float)x.v[k][i]);
-            if (FULL) p.my = fmaxf(p.my, (float)y.v[k][i]);
-        }
-        __builtin_amdgcn_sched_barrier(0);  // one load's values converted at a time
-    }
-    if constexpr (FULL) {
-        float top[2] = {p.m, p.my};
-        group.template all<2, true>(top);
-        p.m = top[0], p.my = scaled(top[1], inv_temp);
-    } else {
-        float top[1] = {p.m};
-        group.template all<1, true>(top);
-        p.m = top[0];
-    }
-    p.m = scaled(p.m, inv_temp);  // the scale is positive
-    x.forget();
-    if (FULL) y.forget();
-    // a row of nothing but -infinity: 0 keeps its differences -infinity
-    const float m = p.m == -INFINITY ? 0.f : p.m, my = p.my == -INFINITY ? 0.f : p.my;
-    count<FULL>(p, (float)x.one, (float)y.one, m, my, inv_temp);
-#pragma unroll
-    for (int k = 0; k < NV; k++) {
-#pragma unroll
-        for (int i = 0; i < E; i++)
-            count<FULL>(p, (float)x.v[k][i], FULL ? (float)y.v[FULL ? k : 0][i] : 0.f, m, my, inv_temp);
-        __builtin_amdgcn_sched_barrier(0);
-    }
-    if constexpr (FULL) {
-        float sum[4] = {p.s, p.t, p.d, p.sy};
-        group.template all<4, false>(sum);
-        p.s = sum[0], p.t = sum[1], p.d = sum[2], p.sy = sum[3];
-    } else {
-        float sum[2] = {p.s, p.t};
-        group.template all<2, false>(sum);
-        p.s = sum[0], p.t = sum[1];
-    }
-    x.forget();
-    if (FULL) y.forget();
-    return p;
-}
-
-// Whether a row has anything to count: a logit above -infinity, or a NaN.
-__device__ __forceinline__ bool counts(const Part& p) { return p.m != -INFINITY || p.s != 0.f; }
-
-// What a row's gradient needs: coef ([j = a] - p) + ent p (logp + h) + klc p (logp - logq - kl).
-// The maximum and the sum's logarithm stay apart: together, a row at a mask's
-// value would lose the second.
-struct RowGrad {
-    float m, log_s, my, log_sy, coef, ent, h, klc, kl;
-    int32_t on;
-
-    // Without a coefficient (clipped, left out, in no sequence) the gradient is 0 whatever the logits.
-    __device__ __forceinline__ bool any() const { return on && (coef != 0.f || ent != 0.f || klc != 0.f); }
-};
-
-// A row's gradient as a function of a logit: p (base + slope logp - toward logq).
-struct Slope {
-    float m, log_s, my, log_sy, base, slope, toward, hit;
-
-    __device__ __forceinline__ Slope(const RowGrad& g, float go)
-        : m(g.m), log_s(g.log_s), my(g.my), log_sy(g.log_sy), base(go * (g.ent * g.h - g.klc * g.kl - g.coef)),
-          slope(go * (g.ent + g.klc)), toward(go * g.klc), hit(go * g.coef) {}
-
-    template <bool FULL>
-    __device__ __forceinline__ float at(float x, float y, float inv_temp) const {
-        const float v = scaled(x, inv_temp), lp = (v - m) - log_s;
-        // where p is 0 the gradient is, and 0 * infinity would be NaN
-        float d = base + slope * fmaxf(lp, -200.f);
-        if (FULL) d = v == -INFINITY ? 0.f : d - toward * ((scaled(y, inv_temp) - my) - log_sy);
-        return fast_exp(lp) * d;
-    }
-};
-
-// The gradient of the n columns that G threads hold, from column c0 of the
-// row; `a` the action's column, whose gradient has the coefficient more.
-template <class T, int G, int NV, bool FULL>
-__device__ __forceinline__ void put_grad(T* row, int n, int lane, const Held<T, G, NV>& x,
-                                         const Held<T, G, FULL ? NV : 1>& y, const Slope& g, float inv_temp, int a) {
-    constexpr int E = EACH<T>;
-    const int whole = n / E, last = whole * E + lane;
-#pragma unroll
-    for (int k = 0; k < NV; k++) {
-        const int c = lane + k * G;
-        if (c < whole) {
-            Raw<T> o;
-#pragma unroll
-            for (int i = 0; i < E; i++) {
-                const float d = g.at<FULL>((float)x.v[k][i], FULL ? (float)y.v[FULL ? k : 0][i] : 0.f, inv_temp);
-                o[i] = (T)(c * E + i == a ? d + g.hit : d);
-            }
-            *(Raw<T>*)(row + c * E) = o;
-        }
-        __builtin_amdgcn_sched_barrier(0);
-    }
-    if (last < n) {
-        const float d = g.at<FULL>((float)x.one, (float)y.one, inv_temp);
-        row[last] = (T)(last == a ? d + g.hit : d);
-    }
-}
-
-template <class T, int G, int NV>
-__device__ __forceinline__ void put_zero(T* row, int n, int lane) {
-    constexpr int E = EACH<T>;
-    const int whole = n / E, last = whole * E + lane;
-#pragma unroll
-    for (int k = 0; k < NV; k++)
-        if (lane + k * G < whole) *(Raw<T>*)(row + (lane + k * G) * E) = Raw<T>{};
-    if (last < n) row[last] = (T)0.f;
-}
-
-// A counted row's loss, outputs and gradient coefficients from its statistics.
-// The loss's own terms are 64-bit: rows' losses cancel in their sum, and the
-// clip's bounds rounded to 32 bits would shift all clipped rows alike.
-struct PolicyRow {
-    const float *behaviour_logp, *advantages, *weights, *ref_logp;
-    float clip_low, clip_high, kl_coef, entropy_coef, even;
-    bool full;
-    float *logp, *kl, *entropy;
-    double* losses;
-    float* loss;
-
-    __device__ __forceinline__ double finish(int64_t r, const Part& p, float xa, RowGrad* g, float3* out) const {
-        const float log_s = logf(p.s), lp = (xa - p.m) - log_s, h = log_s - p.t / p.s;
-        const float w = weights ? weights[r] : even;
-        // e^(x_a - m - behaviour) / s: without the logarithm's rounding and the difference's
-        const double adv = advantages[r], ratio = expf((xa - p.m) - behaviour_logp[r]) / p.s;
-        const double open = ratio * adv, held = fmin(fmax(ratio, 1.0 - clip_low), 1.0 + clip_high) * adv;
-        const bool first = !(open > held);  // a NaN takes this side, and shows
-        float slope = first ? -(float)open : 0.f, k = 0.f, log_sy = 0.f;
-        if (ref_logp) {
-            const float off = ref_logp[r] - lp, e = expm1f(off);
-            k = e - off;
-            slope -= kl_coef * e;
-        }
-        if (full) {
-            log_sy = logf(p.sy);
-            k = p.d / p.s - (p.m - p.my) - (log_s - log_sy);
-        }
-        *out = make_float3(lp, k, h);
-        *g = {p.m, log_s, p.my, log_sy, w * slope, w * entropy_coef, h, full ? w * kl_coef : 0.f, k, 1};
-        return w * ((double)kl_coef * k - (first ? open : held) - (double)entropy_coef * h);
-    }
-};
-
-// ------------------------------------------------- rows that registers hold
-
-template <int G>
-constexpr int group_block() {
-    return G > 64 ? G : 1024;  // the most; rows of up to a wavefront are launched with 256, or all in one workgroup
-}
-
-// A row on G threads, NV 16-byte loads of logits (FULL: and of the reference's)
-// each. TOKEN: log-probabilities and statistics only, for the preference loss.
-template <class T, int G, int NV, bool FULL, bool TOKEN>
-__global__ __launch_bounds__(group_block<G>()) void k_rows(Rows<T> in, PolicyRow row, int64_t rows, RowGrad* grads,
-                                                           const float* grad_out, T* grad, int64_t grad_stride) {
-    __shared__ typename Group<G>::Slots slots;
-    __shared__ double total[G > 64 ? 1 : 1024 / G];
-    Group<G> group{slots};
-    const int lane = threadIdx.x % G, per = G > 64 ? 1 : blockDim.x / G, n = (int)in.vocab;
-    const float go = (grad_out ? *grad_out : 1.f) * in.inv_temp;
-    double sum = 0.0;
-    for (int64_t r0 = int64_t(blockIdx.x) * per; r0 < rows; r0 += int64_t(gridDim.x) * per) {
-        const int64_t r = r0 + (G > 64 ? 0 : threadIdx.x / G);
-        const int64_t a = r < rows ? in.action(r) : -1;
-        Held<T, G, NV> x;
-        Held<T, G, FULL ? NV : 1> y;
-        y.one = (T)0.f;
-        if (a >= 0) {
-            const uint8_t* legal = in.legal ? in.legal + r * in.legal_stride : nullptr;
-            x.load(in.x + r * in.x_stride, legal, n, lane);
-            if constexpr (FULL) y.load(in.y + r * in.y_stride, legal, n, lane);
-        } else {
-            x.none();
-            if constexpr (FULL) y.none();
-        }
-        RowGrad g;
-        g.m = g.log_s = g.my = g.log_sy = g.coef = g.ent = g.h = g.klc = g.kl = 0.f;
-        g.on = 0;
-        float3 out = make_float3(0.f, 0.f, 0.f);
-        double loss = 0.0;
-        if (G <= 64 || a >= 0) {  // a workgroup's row is left out as one
-            const Part p = held_stats<T, G, NV, FULL>(x, y, in.inv_temp, group);
-            if (a >= 0 && counts(p)) {
-                const float xa = scaled((float)in.x[r * in.x_stride + a], in.inv_temp);
-                if constexpr (TOKEN) {
-                    g.m = p.m;
-                    g.log_s = logf(p.s);
-                    g.on = 1;
-                    out.x = (xa - p.m) - g.log_s;
-                } else {
-                    loss = row.finish(r, p, xa, &g, &out);
-                }
-            }
-        }
-        if (r < rows) {
-            if (lane == 0) {
-                row.logp[r] = out.x;
-                if constexpr (TOKEN) {
-                    grads[r] = g;
-                } else {
-                    row.kl[r] = out.y;
-                    row.entropy[r] = out.z;
-                    if (gridDim.x > 1) row.losses[r] = loss;
-                    else sum += loss;
-                }
-            }
-            if (!TOKEN && grad) {
-                T* to = grad + r * grad_stride;
-                if (g.any()) put_grad<T, G, NV, FULL>(to, n, lane, x, y, Slope(g, go), in.inv_temp, (int)a);
-                else put_zero<T, G, NV>(to, n, lane);
-            }
-        }
-    }
-    if (!TOKEN && gridDim.x == 1) {  // one workgroup: its rows' losses, in order
-        if (lane == 0) total[threadIdx.x / G] = sum;
-        __syncthreads();
-        if (threadIdx.x == 0) {
-            for (int k = 1; k < per; k++) sum += total[k];
-            *row.loss = (float)sum;
-        }
-    }
-}
-
-// -------------------------------------------------------------- longer rows
-
-constexpr int BLOCK = 256;
-constexpr int64_t CHUNK = 8192;  // columns per workgroup
-template <class T>
-constexpr int CHUNK_LOADS = CHUNK / (BLOCK * EACH<T>);
-
-// The statistics of one chunk of one row: workgroup r * splits + chunk.
-template <class T, bool FULL>
-__global__ __launch_bounds__(BLOCK) void k_row_parts(Rows<T> in, int64_t tiles, int splits, Part* parts) {
-    constexpr int NV = CHUNK_LOADS<T>;
-    __shared__ typename Group<BLOCK>::Slots slots;
-    Group<BLOCK> group{slots};
-    for (int64_t t = blockIdx.x; t < tiles; t += gridDim.x) {
-        const int64_t r = t / splits, c0 = (t - r * splits) * CHUNK;
-        if (in.action(r) < 0) continue;
-        const uint8_t* legal = in.legal ? in.legal + r * in.legal_stride + c0 : nullptr;
-        const int n = (int)min(CHUNK, in.vocab - c0);
-        Held<T, BLOCK, NV> x;
-        Held<T, BLOCK, FULL ? NV : 1> y;
-        y.one = (T)0.f;
-        x.load(in.x + r * in.x_stride + c0, legal, n, threadIdx.x);
-        if constexpr (FULL) y.load(in.y + r * in.y_stride + c0, legal, n, threadIdx.x);
-        const Part p = held_stats<T, BLOCK, NV, FULL>(x, y, in.inv_temp, group);
-        if (threadIdx.x == 0) parts[t] = p;
-    }
-}
-
-// A row's parts joined, its outputs and coefficients: one thread per row.
-template <class T, bool TOKEN>
-__global__ void k_row_ends(Rows<T> in, PolicyRow row, int64_t rows, int splits, const Part* parts, RowGrad* grads) {
-    const int64_t r = int64_t(blockIdx.x) * blockDim.x + threadIdx.x;
-    if (r >= rows) return;
-    const int64_t a = in.action(r);
-    Part p = {-INFINITY, 0.f, 0.f, 0.f, -INFINITY, 0.f};
-    if (a >= 0)
-        for (int k = 0; k < splits; k++) p = join(p, parts[r * splits + k]);
-    RowGrad g = {};
-    float3 out = make_float3(0.f, 0.f, 0.f);
-    double loss = 0.0;
-    if (counts(p)) {
-        const float xa = scaled((float)in.x[r * in.x_stride + a], in.inv_temp);
-        if (TOKEN) {
-            g.m = p.m;
-            g.log_s = logf(p.s);
-            g.on = 1;
-            out.x = (xa - p.m) - g.log_s;
-        } else {
-            loss = row.finish(r, p, xa, &g, &out);
-        }
-    }
-    row.logp[r] = out.x;
-    grads[r] = g;
-    if (!TOKEN) {
-        row.kl[r] = out.y;
-        row.entropy[r] = out.z;
-        row.losses[r] = loss;
-    }
-}
-
-// The sum of n losses in a fixed order.
-__global__ __launch_bounds__(1024) void k_sum(const double* v, int64_t n, double scale, float* out) {
-    __shared__ double lds[16];
-    double s = 0;
-    for (int64_t i = threadIdx.x; i < n; i += 1024) s += v[i];
-    for (int mask = 32; mask; mask >>= 1) s += __shfl_xor(s, mask);
-    if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = s;
-    __syncthreads();
-    if (threadIdx.x == 0) {
-        for (int w = 1; w < 16; w++) s += lds[w];
-        *out = (float)(s * scale);
-    }
-}
-
-// The gradient from the rows' coefficients, a second read of the logits. The
-// last rows go first: they are what the pass before left in the caches.
-template <class T, bool FULL>
-__global__ __launch_bounds__(BLOCK) void k_row_grads(Rows<T> in, int64_t tiles, int splits, const RowGrad* grads,
-                                                     const float* grad_out, T* out, int64_t out_stride) {
-    constexpr int NV = CHUNK_LOADS<T>;
-    const float go = (grad_out ? *grad_out : 1.f) * in.inv_temp;
-    for (int64_t i = blockIdx.x; i < tiles; i += gridDim.x) {
-        const int64_t t = tiles - 1 - i, r = t / splits, c0 = (t - r * splits) * CHUNK;
-        const RowGrad g = grads[r];
-        T* to = out + r * out_stride + c0;
-        const int n = (int)min(CHUNK, in.vocab - c0);
-        if (!g.any()) {
-            put_zero<T, BLOCK, NV>(to, n, threadIdx.x);
-            continue;
-        }
-        const int64_t a = index_at(in.actions, in.bits, r) - c0;
-        const uint8_t* legal = in.legal ? in.legal + r * in.legal_stride + c0 : nullptr;
-        Held<T, BLOCK, NV> x;
-        Held<T, BLOCK, FULL ? NV : 1> y;
-        y.one = (T)0.f;
-        x.load(in.x + r * in.x_stride + c0, legal, n, threadIdx.x);
-        if constexpr (FULL) y.load(in.y + r * in.y_stride + c0, legal, n, threadIdx.x);
-        put_grad<T, BLOCK, NV, FULL>(to, n, threadIdx.x, x, y, Slope(g, go), in.inv_temp, a >= 0 && a < n ? (int)a : -1);
-    }
-}
-
-// ------------------------------------------------------------------ launches
-
-template <class T>
-Rows<T> rows_of(const wc_policy_args& a) {
-    return {(const T*)a.logits, a.logits_stride, a.legal, a.legal_stride, (const T*)a.ref_logits, a.ref_stride,
-            a.actions, a.weights, a.vocab, a.inv_temperature, a.index_bits};
-}
-
-template <class T>
-Rows<T> rows_of(const wc_preference_args& a) {
-    return {(const T*)a.logits, a.logits_stride, nullptr, 0, nullptr, 0, a.tokens, a.weights, a.vocab,
-            a.inv_temperature, a.index_bits};
-}
-
-int splits_of(int64_t vocab) { return (int)((vocab + CHUNK - 1) / CHUNK); }
-
-uint32_t tile_grid(int64_t tiles) { return (uint32_t)std::min<int64_t>(tiles, 1 << 22); }
-
-// Whether k_rows holds a row: up to 64 registers per thread of 1,024.
-bool holds(int dtype, int64_t vocab, bool full) {
-    return vocab * (dtype == WC_DTYPE_F32 ? 4 : 2) * (full ? 2 : 1) <= 256 << 10;
-}
-
-template <class T, int G, int NV, bool FULL, bool TOKEN>
-void rows_at(const Rows<T>& in, const PolicyRow& row, int64_t rows, RowGrad* grads, const float* grad_out, T* grad,
-             int64_t grad_stride, hipStream_t s, bool* whole) {
-    // rows that one workgroup holds at once go to one, which then sums their losses itself
-    const int block = G > 64 ? G : rows * G <= 1024 ? (int)std::max<int64_t>(64, (rows * G + 63) / 64 * 64) : 256;
-    const int64_t per = block / G, grid = std::min<int64_t>((rows + per - 1) / per, 1 << 22);
-    *whole = grid == 1;
-    k_rows<T, G, NV, FULL, TOKEN><<<dim3((uint32_t)grid), block, 0, s>>>(in, row, rows, grads, grad_out, grad,
-                                                                         grad_stride);
-}
-
-// The fewest threads that hold a row in at most four loads each while they are
-// one wavefront, and in at most sixteen (eight with the reference's logits)
-// beyond.
-template <class T, bool FULL, bool TOKEN>
-void rows_held(const Rows<T>& in, const PolicyRow& row, int64_t rows, RowGrad* grads, const float* go, T* grad,
-               int64_t gs, hipStream_t s, bool* whole) {
-    const int64_t n = (in.vocab + EACH<T> - 1) / EACH<T>;
-    if (n <= 8) rows_at<T, 8, 1, FULL, TOKEN>(in, row, rows, grads, go, grad, gs, s, whole);
-    else if (n <= 16) rows_at<T, 16, 1, FULL, TOKEN>(in, row, rows, grads, go, grad, gs, s, whole);
-    else if (n <= 32) rows_at<T, 32, 1, FULL, TOKEN>(in, row, rows, grads, go, grad, gs, s, whole);
-    else if (n <= 64) rows_at<T, 64, 1, FULL, TOKEN>(in, row, rows, grads, go, grad, gs, s, whole);
-    else if (n <= 128) rows_at<T, 64, 2, FULL, TOKEN>(in, row, rows, grads, go, grad, gs, s, whole);
-    else if (n <= 192) rows_at<T, 64, 3, FULL, TOKEN>(in, row, rows, grads, go, grad, gs, s, whole);
-    else if (n <= 256) rows_at<T, 64, 4, FULL, TOKEN>(in, row, rows, grads, go, grad, gs, s, whole);
-    else if (n <= 512) rows_at<T, 256, 2, FULL, TOKEN>(in, row, rows, grads, go, grad, gs, s, whole);
-    else if (n <= 1024) rows_at<T, 256, 4, FULL, TOKEN>(in, row, rows, grads, go, grad, gs, s, whole);
-    else if (n <= 2048) rows_at<T, 1024, 2, FULL, TOKEN>(in, row, rows, grads, go, grad, gs, s, whole);
-    else if (n <= 4096) rows_at<T, 1024, 4, FULL, TOKEN>(in, row, rows, grads, go, grad, gs, s, whole);
-    else if (n <= 8192) rows_at<T, 1024, 8, FULL, TOKEN>(in, row, rows, grads, go, grad, gs, s, whole);
-    else if constexpr (!FULL) rows_at<T, 1024, 16, FULL, TOKEN>(in, row, rows, grads, go, grad, gs, s, whole);
-}
-
-template <class T, bool FULL>
-void policy(const wc_policy_args& a, hipStream_t s) {
-    const Rows<T> in = rows_of<T>(a);
-    uint8_t* w = (uint8_t*)a.workspace;
-    PolicyRow row = {a.behaviour_logp, a.advantages, a.weights, a.ref_logp, a.clip_low, a.clip_high, a.kl_coef,
-                     a.entropy_coef, 1.f / (float)std::max<int64_t>(a.rows, 1), FULL, a.logp, a.kl, a.entropy,
-                     (double*)w, a.loss};
-    bool whole = false;
-    if (a.rows && holds(a.dtype, a.vocab, FULL)) {
-        rows_held<T, FULL, false>(in, row, a.rows, nullptr, a.grad_out, (T*)a.grad, a.grad_stride, s, &whole);
-    } else if (a.rows) {
-        const int splits = splits_of(a.vocab);
-        const int64_t tiles = a.rows * splits;
-        RowGrad* grads = (RowGrad*)(w += pad256(size_t(a.rows) * sizeof(double)));
-        Part* parts = (Part*)(w += pad256(size_t(a.rows) * sizeof(RowGrad)));
-        k_row_parts<T, FULL><<<tile_grid(tiles), BLOCK, 0, s>>>(in, tiles, splits, parts);
-        k_row_ends<T, false><<<dim3((uint32_t)((a.rows + 63) / 64)), 64, 0, s>>>(in, row, a.rows, splits, parts, grads);
-        if (a.grad)
-            k_row_grads<T, FULL><<<tile_grid(tiles), BLOCK, 0, s>>>(in, tiles, splits, grads, a.grad_out, (T*)a.grad,
-                                                                    a.grad_stride);
-    }
-    if (!whole) k_sum<<<1, 1024, 0, s>>>(row.losses, a.rows, 1.0, a.loss);
-}
-
-// ---------------------------------------------------------------- preference
-
-struct Pairs {
-    const void* offsets;
-    const float *ref_logp, *weights;
-    int64_t rows, pairs;
-    float beta, smoothing;
-    int kind, average, bits;
-};
-
-__device__ __forceinline__ int64_t clamp_row(int64_t x, int64_t rows) { return x < 0 ? 0 : x > rows ? rows : x; }
-
-// One pair per workgroup: both sequences' ratios in 64-bit sums (long sums of
-// differences that nearly cancel), the pair's loss, and the coefficient of
-// every row of both.
-__global__ __launch_bounds__(BLOCK) void k_pairs(Pairs p, const float* logp, RowGrad* grads, double* losses,
-                                                 float* margins, float* ratios) {
-    __shared__ double lds[4][BLOCK / 64];
-    const int64_t i = blockIdx.x;
-    int64_t lo[2], hi[2];
-    double sum[4] = {};
-    for (int k = 0; k < 2; k++) {
-        lo[k] = clamp_row(index_at(p.offsets, p.bits, 2 * i + k), p.rows);
-        hi[k] = clamp_row(index_at(p.offsets, p.bits, 2 * i + k + 1), p.rows);
-        for (int64_t r = lo[k] + threadIdx.x; r < hi[k]; r += BLOCK) {
-            if (!grads[r].on) continue;
-            const float w = p.weights ? p.weights[r] : 1.f;
-            sum[2 * k] += (double)w * ((double)logp[r] - p.ref_logp[r]);
-            sum[2 * k + 1] += w;
-        }
-    }
-    for (int q = 0; q < 4; q++) {
-        for (int mask = 32; mask; mask >>= 1) sum[q] += __shfl_xor(sum[q], mask);
-        if ((threadIdx.x & 63) == 0) lds[q][threadIdx.x >> 6] = sum[q];
-    }
-    __syncthreads();
-    for (int q = 0; q < 4; q++) sum[q] = (lds[q][0] + lds[q][1]) + (lds[q][2] + lds[q][3]);
-    double share[2], ratio[2];
-    for (int k = 0; k < 2; k++) {
-        share[k] = !p.average ? 1.0 : sum[2 * k + 1] != 0.0 ? 1.0 / sum[2 * k + 1] : 0.0;
-        ratio[k] = sum[2 * k] * share[k];
-    }
-    const double h = ratio[0] - ratio[1], z = p.beta * h;
-    double loss, d;
-    if (p.kind == WC_PREFERENCE_LOGISTIC) {
-        const double e = exp(-fabs(z)), tail = log1p(e);
-        loss = tail + (1.0 - p.smoothing) * fmax(-z, 0.0) + p.smoothing * fmax(z, 0.0);
-        d = p.beta * ((z >= 0 ? 1.0 / (1.0 + e) : e / (1.0 + e)) - (1.0 - p.smoothing));
-        if (z != z) loss = z;
-    } else if (p.kind == WC_PREFERENCE_SQUARED) {
-        const double t = h - 0.5 / p.beta;
-        loss = t * t;
-        d = 2.0 * t;
-    } else {
-        loss = z < 1.0 ? 1.0 - z : 0.0;
-        d = z < 1.0 ? -(double)p.beta : 0.0;
-        if (z != z) loss = d = z;
-    }
-    d /= (double)p.pairs;
-    for (int k = 0; k < 2; k++) {
-        const float c = (float)((k ? -d : d) * share[k]);
-        for (int64_t r = lo[k] + threadIdx.x; r < hi[k]; r += BLOCK)
-            if (grads[r].on) grads[r].coef = c * (p.weights ? p.weights[r] : 1.f);
-    }
-    if (threadIdx.x == 0) {
-        losses[i] = loss;
-        margins[i] = (float)z;
-        ratios[2 * i] = (float)ratio[0];
-        ratios[2 * i + 1] = (float)ratio[1];
-    }
-}
-
-template <class T>
-void preference(const wc_preference_args& a, hipStream_t s) {
-    const Rows<T> in = rows_of<T>(a);
-    const int splits = splits_of(a.vocab);
-    const int64_t tiles = a.rows * splits;
-    uint8_t* w = (uint8_t*)a.workspace;
-    RowGrad* grads = (RowGrad*)w;
-    double* losses = (double*)(w += pad256(size_t(a.rows) * sizeof(RowGrad)));
-    PolicyRow row = {};
-    row.logp = a.logp;
-    if (a.rows && holds(a.dtype, a.vocab, false)) {
-        bool whole;
-        rows_held<T, false, true>(in, row, a.rows, grads, nullptr, nullptr, 0, s, &whole);
-    } else if (a.rows) {
-        Part* parts = (Part*)(w += pad256(size_t(a.pairs) * sizeof(double)));
-        k_row_parts<T, false><<<tile_grid(tiles), BLOCK, 0, s>>>(in, tiles, splits, parts);
-        k_row_ends<T, true><<<dim3((uint32_t)((a.rows + 63) / 64)), 64, 0, s>>>(in, row, a.rows, splits, parts, grads);
-    }
-    const Pairs p = {a.offsets, a.ref_logp, a.weights, a.rows, a.pairs, a.beta, a.smoothing, a.kind, a.average,
-                     a.index_bits};
-    if (a.pairs) k_pairs<<<dim3((uint32_t)a.pairs), BLOCK, 0, s>>>(p, a.logp, grads, losses, a.margins, a.ratios);
-    k_sum<<<1, 1024, 0, s>>>(losses, a.pairs, a.pairs ? 1.0 / (double)a.pairs : 0.0, a.loss);
-    if (a.grad && a.rows)
-        k_row_grads<T, false><<<tile_grid(tiles), BLOCK, 0, s>>>(in, tiles, splits, grads, a.grad_out, (T*)a.grad,
-                                                                 a.grad_stride);
-}
-
-template <class T>
-void policy_of(const wc_policy_args& a, hipStream_t s) {
-    if (a.ref_logits) policy<T, true>(a, s);
-    else policy<T, false>(a, s);
-}
-
-}  // namespace
 
 size_t policy_scratch(const wc_policy_args& a, int) {
     const size_t losses = pad256(size_t(a.rows) * sizeof(double));
@@ -738,15 +18,15 @@ size_t preference_scratch(const wc_preference_args& a, int) {
 }
 
 void launch_policy(const wc_policy_args& a, int, hipStream_t s) {
-    if (a.dtype == WC_DTYPE_F32) policy_of<float>(a, s);
-    else if (a.dtype == WC_DTYPE_F16) policy_of<f16>(a, s);
-    else policy_of<bf16>(a, s);
+    if (a.dtype == WC_DTYPE_F32) policy_f32(a, s);
+    else if (a.dtype == WC_DTYPE_F16) policy_f16(a, s);
+    else policy_bf16(a, s);
 }
 
 void launch_preference(const wc_preference_args& a, int, hipStream_t s) {
-    if (a.dtype == WC_DTYPE_F32) preference<float>(a, s);
-    else if (a.dtype == WC_DTYPE_F16) preference<f16>(a, s);
-    else preference<bf16>(a, s);
+    if (a.dtype == WC_DTYPE_F32) preference_f32(a, s);
+    else if (a.dtype == WC_DTYPE_F16) preference_f16(a, s);
+    else preference_bf16(a, s);
 }
 
 }  // namespace learn
