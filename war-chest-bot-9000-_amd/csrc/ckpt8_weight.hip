@@ -1,4 +1,15 @@
 // The weight gradient from activations kept in 8 bits, on the matrix cores (include/wc_learn.h).
+//
+// weight[i][j] = sum over rows r of a[r][i] g[r][j]: both operands have the
+// summed index outermost, while a matrix instruction takes several values of
+// it from one lane. Tiles go to LDS as they lie in memory, the 8-bit one
+// expanded to the 16-bit type on the way, and come back through the transposing
+// LDS read (four rows of sixteen columns become four values of one column per
+// lane). A workgroup of four wavefronts owns a square tile of weight, each
+// wavefront a quarter in its accumulators; two LDS buffers alternate, the next
+// tile's global loads in registers meanwhile. Where the tiles are too few for
+// the device the rows are cut into runs, whose partial products are added in
+// order.
 #include <algorithm>
 
 #include "ckpt8_dev.h"
@@ -7,22 +18,25 @@ namespace wc {
 namespace learn {
 namespace {
 
-constexpr int BLOCK = 256, TILE = 64, DEPTH = 32, LD = DEPTH + 8;
+constexpr int BLOCK = 256;
+constexpr int DEPTH = 64;  // rows per step
 
 typedef f16 f16x8 __attribute__((ext_vector_type(8)));
 typedef bf16 bf16x8 __attribute__((ext_vector_type(8)));
-typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef short s16x8 __attribute__((ext_vector_type(8)));
 
-__device__ __forceinline__ f32x4 mfma(f16x8 a, f16x8 b, f32x4 c) {
-    return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+__device__ __forceinline__ f32x16 mfma(f16x8 a, f16x8 b, f32x16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
 }
-__device__ __forceinline__ f32x4 mfma(bf16x8 a, bf16x8 b, f32x4 c) {
-    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+__device__ __forceinline__ f32x16 mfma(bf16x8 a, bf16x8 b, f32x16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
 }
 
 // The operand's type and how many parts a gradient element is taken in: a
 // float32 is the sum of three bf16 (8 + 8 + 8 mantissa bits), whose products
-// with a kept value (8 bits) are exact.
+// with a kept value (8 bits) are exact. The parts are three passes over the rows.
 template <class T>
 struct Operand {
     typedef T type;
@@ -34,124 +48,305 @@ struct Operand<float> {
     static constexpr int PARTS = 3;
 };
 
+// One tile: 2 x 2 wavefronts of F x F fragments of 32 x 32.
+template <int F>
+struct Shape {
+    static constexpr int TILE = 64 * F;
+    // bytes from one row of a tile to the next: four consecutive rows, which one
+    // transposing read takes 32 bytes of each, start 64 bytes apart modulo 256,
+    // all the banks
+    static constexpr int PITCH = 2 * TILE + 64;
+    static constexpr int A_CHUNKS = DEPTH * TILE / 16 / BLOCK;  // 16 kept values each
+    static constexpr int B_CHUNKS = DEPTH * TILE / 8 / BLOCK;   // 8 gradient values each
+};
 
-// One 64 x 64 tile of weight over one run of rows; part: runs x width x out.
-template <class T>
-__global__ __launch_bounds__(BLOCK) void k_weight(wc_ckpt_weight_args a, int64_t run, float* part) {
-    typedef typename Operand<T>::type E;
-    typedef E E8 __attribute__((ext_vector_type(8)));
-    constexpr int PARTS = Operand<T>::PARTS;
-    __shared__ __align__(16) E as[TILE][LD];
-    __shared__ __align__(16) E bs[PARTS][TILE][LD];
-    const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
-    const int64_t i0 = int64_t(blockIdx.x) * TILE, j0 = int64_t(blockIdx.y) * TILE;
-    const int64_t lo = int64_t(blockIdx.z) * run, hi = min(lo + run, a.rows);
-    const int kk = t >> 3, cc = (t & 7) * 8;
-    const int wi = (wave >> 1) * 32, wj = (wave & 1) * 32;
-    const int na = (int)min<int64_t>(8, max<int64_t>(0, a.width - i0 - cc));
-    const int nb = (int)min<int64_t>(8, max<int64_t>(0, a.out - j0 - cc));
-    f32x4 acc[2][2] = {};
-    for (int64_t k0 = lo; k0 < hi; k0 += DEPTH) {
-        const int64_t r = k0 + kk;
-        float z[8] = {}, g[8] = {};
-        if (r < hi && na > 0) {
-            const float step = step_of(a.exps[r * a.exps_stride + ((i0 + cc) >> 5)]);
-            for (int k = 0; k < na; k++) z[k] = act_value(held<E>((float)a.q[r * a.q_stride + i0 + cc + k] * step), a.act);
-        }
-        if (r < hi) load_n((const T*)a.grad + r * a.grad_stride + j0 + cc, nb, 0.f, g);
-        __syncthreads();
+struct Job {
+    wc_ckpt_weight_args a;
+    int64_t run;        // rows per run, a multiple of DEPTH
+    int tiles_i, tiles_j, runs;
+    float* part;        // runs x width x out, where there are several runs
+    float* bias_part;   // runs x out, likewise
+};
+
+// Sixteen kept values of one row, from column c.
+struct Kept {
+    uint32_t q[4], e;
+};
+
+__device__ __forceinline__ Kept load_kept(const wc_ckpt_weight_args& a, int64_t r, int64_t hi, int64_t c) {
+    typedef uint32_t Words __attribute__((ext_vector_type(4), aligned(1)));
+    Kept k = {{0, 0, 0, 0}, 1};
+    if (r < hi && c < a.width) {
+        const int8_t* p = a.q + r * a.q_stride + c;
+        k.e = a.exps[r * a.exps_stride + (c >> 5)];
+        if (c + 16 <= a.width) {
+            const Words w = *(const Words*)p;
 #pragma unroll
-        for (int k = 0; k < 8; k++) {
-            as[cc + k][kk] = (E)z[k];
-            float rest = g[k];
-#pragma unroll
-            for (int p = 0; p < PARTS; p++) {
-                const E e = (E)rest;
-                bs[p][cc + k][kk] = e;
-                rest -= (float)e;
-            }
-        }
-        __syncthreads();
-        E8 fa[2], fb[2];
-#pragma unroll
-        for (int m = 0; m < 2; m++) fa[m] = *(const E8*)&as[wi + 16 * m + (lane & 15)][(lane >> 4) * 8];
-#pragma unroll
-        for (int p = 0; p < PARTS; p++) {
-#pragma unroll
-            for (int n = 0; n < 2; n++) fb[n] = *(const E8*)&bs[p][wj + 16 * n + (lane & 15)][(lane >> 4) * 8];
-#pragma unroll
-            for (int m = 0; m < 2; m++)
-#pragma unroll
-                for (int n = 0; n < 2; n++) acc[m][n] = mfma(fa[m], fb[n], acc[m][n]);
+            for (int i = 0; i < 4; i++) k.q[i] = w[i];
+        } else {
+            for (int i = 0; i < (int)(a.width - c); i++) k.q[i >> 2] |= (uint32_t)(uint8_t)p[i] << (8 * (i & 3));
         }
     }
-#pragma unroll
-    for (int m = 0; m < 2; m++)
-#pragma unroll
-        for (int n = 0; n < 2; n++)
-#pragma unroll
-            for (int k = 0; k < 4; k++) {
-                const int64_t i = i0 + wi + 16 * m + (lane >> 4) * 4 + k, j = j0 + wj + 16 * n + (lane & 15);
-                if (i < a.width && j < a.out) part[(int64_t(blockIdx.z) * a.width + i) * a.out + j] = acc[m][n][k];
-            }
+    return k;
 }
 
-template <class W>
-__global__ __launch_bounds__(BLOCK) void k_weight_sum(const float* part, int runs, int64_t width, int64_t out,
-                                                      W* weight, int64_t stride) {
-    const int64_t i = int64_t(blockIdx.x) * BLOCK + threadIdx.x;
-    if (i >= width * out) return;
-    float s = 0.f;
-    for (int k = 0; k < runs; k++) s += part[k * width * out + i];
-    weight[i / out * stride + i % out] = (W)s;
+template <class E>
+__device__ __forceinline__ void put_kept(const Kept& k, int act, char* to) {
+    typedef E E8 __attribute__((ext_vector_type(8)));
+    const float step = step_of(k.e);
+#pragma unroll
+    for (int h = 0; h < 2; h++) {
+        float v[8];
+#pragma unroll
+        for (int i = 0; i < 8; i++) v[i] = (float)(int8_t)(k.q[2 * h + (i >> 2)] >> (8 * (i & 3))) * step;
+        if (may_pass<E>(k.e)) {
+#pragma unroll
+            for (int i = 0; i < 8; i++) v[i] = held<E>(v[i]);
+        }
+        if (act != WC_ACT_NONE) {
+#pragma unroll
+            for (int i = 0; i < 8; i++) v[i] = act_value(v[i], act);
+        }
+        E8 o;
+#pragma unroll
+        for (int i = 0; i < 8; i++) o[i] = (E)v[i];
+        *(E8*)(to + 16 * h) = o;
+    }
 }
 
-// Column sums of grad over one run of rows, and their sum.
+// Eight gradient values of one row, from column c; 0 beyond the run and the row.
 template <class T>
-__global__ __launch_bounds__(BLOCK) void k_bias(const T* grad, int64_t stride, int64_t rows, int64_t out, int64_t run,
-                                                float* part) {
-    const int64_t j = int64_t(blockIdx.x) * BLOCK + threadIdx.x;
-    if (j >= out) return;
-    const int64_t lo = int64_t(blockIdx.y) * run, hi = min(lo + run, rows);
-    float s = 0.f;
-    for (int64_t r = lo; r < hi; r++) s += (float)grad[r * stride + j];
-    part[int64_t(blockIdx.y) * out + j] = s;
+__device__ __forceinline__ typename Vec8<T>::type load_grad(const wc_ckpt_weight_args& a, int64_t r, int64_t hi,
+                                                            int64_t c) {
+    typename Vec8<T>::type v = {};
+    if (r < hi && c < a.out) {
+        const T* p = (const T*)a.grad + r * a.grad_stride + c;
+        if (c + 8 <= a.out) {
+            v = *(const typename Vec8<T>::type*)p;
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; i++)
+                if (c + i < a.out) v[i] = p[i];
+        }
+    }
+    return v;
 }
 
-constexpr int BIAS_RUNS = 64;
+// A fragment's eight values for the lane: rows k0 + 8 (lane / 32) .. + 7 of
+// column c0 + lane % 32, by two transposing reads of four rows.
+template <class E8, int PITCH>
+__device__ __forceinline__ E8 fragment(const char* tile, int k0, int c0, int lane) {
+    typedef __attribute__((address_space(3))) s16x4* Lds;
+    const char* p = tile + (k0 + 8 * (lane >> 5) + ((lane & 15) >> 2)) * PITCH + 2 * (c0 + (lane & 16) + 4 * (lane & 3));
+    const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Lds)p);
+    const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Lds)(p + 4 * PITCH));
+    return __builtin_bit_cast(E8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+}
 
-int runs_of(const wc_ckpt_weight_args& a, int cus) {
-    const int64_t tiles = ((a.width + TILE - 1) / TILE) * ((a.out + TILE - 1) / TILE);
-    const int64_t want = std::max<int64_t>(1, 4 * cus / tiles), most = std::max<int64_t>(1, a.rows / 256);
-    return (int)std::min(want, most);
+template <class T, int F>
+__global__ __launch_bounds__(BLOCK, F == 4 ? 1 : 2) void k_weight(Job job) {
+    typedef typename Operand<T>::type E;
+    typedef E E8 __attribute__((ext_vector_type(8)));
+    typedef Shape<F> S;
+    constexpr int PARTS = Operand<T>::PARTS, TILE = S::TILE, PITCH = S::PITCH;
+    constexpr int SIDE = DEPTH * PITCH;
+    __shared__ __align__(16) char lds[4 * SIDE];  // two buffers of an A tile and a B tile
+    const wc_ckpt_weight_args& a = job.a;
+    const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
+    // Workgroups go round the eight XCDs; consecutive tiles of a run, which share
+    // rows of both operands, go to one XCD's cache.
+    const int total = job.tiles_i * job.tiles_j * job.runs, per = total / 8;
+    const int id = blockIdx.x < (unsigned)per * 8 ? (blockIdx.x % 8) * per + blockIdx.x / 8 : blockIdx.x;
+    const int run = id / (job.tiles_i * job.tiles_j), tile = id - run * (job.tiles_i * job.tiles_j);
+    const int ti = tile % job.tiles_i, tj = tile / job.tiles_i;
+    const int64_t i0 = int64_t(ti) * TILE, j0 = int64_t(tj) * TILE;
+    const int64_t lo = run * job.run, hi = min(lo + job.run, a.rows);
+    const int steps = (int)((max<int64_t>(hi - lo, 0) + DEPTH - 1) / DEPTH), all = steps * PARTS;
+    const int ac = (t % (TILE / 16)) * 16, ar = t / (TILE / 16);
+    const int bc = (t % (TILE / 8)) * 8, br = t / (TILE / 8);
+    constexpr int AR = BLOCK / (TILE / 16), BR = BLOCK / (TILE / 8);
+    const bool sums = a.bias && ti == 0;
+
+    Kept ka[S::A_CHUNKS];
+    typename Vec8<T>::type kb[S::B_CHUNKS];
+    float bias[8] = {};
+    auto load = [&](int s) {
+        const int64_t r0 = lo + int64_t(PARTS == 1 ? s : s % steps) * DEPTH;
+#pragma unroll
+        for (int m = 0; m < S::A_CHUNKS; m++) ka[m] = load_kept(a, r0 + ar + m * AR, hi, i0 + ac);
+#pragma unroll
+        for (int m = 0; m < S::B_CHUNKS; m++) kb[m] = load_grad<T>(a, r0 + br + m * BR, hi, j0 + bc);
+    };
+    auto put = [&](int s) {
+        char* to = lds + (s & 1) * 2 * SIDE;
+        const int plane = PARTS == 1 ? 0 : s / steps;
+#pragma unroll
+        for (int m = 0; m < S::A_CHUNKS; m++) put_kept<E>(ka[m], a.act, to + (ar + m * AR) * PITCH + 2 * ac);
+#pragma unroll
+        for (int m = 0; m < S::B_CHUNKS; m++) {
+            E8 o;
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                float v = (float)kb[m][i];
+                if (sums && plane == 0) bias[i] += v;
+                if (PARTS > 1) {
+                    if (plane > 0) v -= (float)(E)v;
+                    if (plane > 1) v -= (float)(E)v;
+                    o[i] = (E)v;
+                } else {
+                    o[i] = (E)kb[m][i];
+                }
+            }
+            *(E8*)(to + SIDE + (br + m * BR) * PITCH + 2 * bc) = o;
+        }
+    };
+
+    f32x16 acc[F][F] = {};
+    if (all > 0) {
+        load(0);
+        put(0);
+        if (all > 1) load(1);
+    }
+    __syncthreads();
+    const int wi = (wave >> 1) * 32 * F, wj = (wave & 1) * 32 * F;
+    for (int s = 0; s < all; s++) {
+        const char* from = lds + (s & 1) * 2 * SIDE;
+        if (s + 1 < all) {
+            put(s + 1);
+            if (s + 2 < all) load(s + 2);
+        }
+#pragma unroll
+        for (int k0 = 0; k0 < DEPTH; k0 += 16) {
+            E8 fa[F], fb[F];
+#pragma unroll
+            for (int m = 0; m < F; m++) fa[m] = fragment<E8, PITCH>(from, k0, wi + 32 * m, lane);
+#pragma unroll
+            for (int n = 0; n < F; n++) fb[n] = fragment<E8, PITCH>(from + SIDE, k0, wj + 32 * n, lane);
+#pragma unroll
+            for (int m = 0; m < F; m++)
+#pragma unroll
+                for (int n = 0; n < F; n++) acc[m][n] = mfma(fa[m], fb[n], acc[m][n]);
+        }
+        __syncthreads();
+    }
+
+    const bool last = job.runs == 1;
+    float* part = job.part + int64_t(run) * a.width * a.out;
+#pragma unroll
+    for (int m = 0; m < F; m++)
+#pragma unroll
+        for (int n = 0; n < F; n++)
+#pragma unroll
+            for (int k = 0; k < 16; k++) {
+                const int64_t i = i0 + wi + 32 * m + 8 * (k / 4) + 4 * (lane >> 5) + k % 4, j = j0 + wj + 32 * n + (lane & 31);
+                if (i >= a.width || j >= a.out) continue;
+                if (!last) part[i * a.out + j] = acc[m][n][k];
+                else if (a.weight_dtype == WC_DTYPE_F32) ((float*)a.weight)[i * a.weight_stride + j] = acc[m][n][k];
+                else ((T*)a.weight)[i * a.weight_stride + j] = (T)acc[m][n][k];
+            }
+    if (sums) {  // the threads of one column chunk, in order
+        float* rows = (float*)lds;
+#pragma unroll
+        for (int i = 0; i < 8; i++) rows[br * TILE + bc + i] = bias[i];
+        __syncthreads();
+        if (t < TILE && j0 + t < a.out) {
+            float s = 0.f;
+            for (int k = 0; k < BR; k++) s += rows[k * TILE + t];
+            if (last) a.bias[j0 + t] = s;
+            else job.bias_part[int64_t(run) * a.out + j0 + t] = s;
+        }
+    }
+}
+
+// The runs' partial products, added in order; the workgroups past the weights'
+// add the bias's.
+template <class W>
+__global__ __launch_bounds__(BLOCK) void k_weight_sum(Job job, int64_t weight_blocks) {
+    const wc_ckpt_weight_args& a = job.a;
+    if (blockIdx.x >= weight_blocks) {
+        const int64_t j = (int64_t(blockIdx.x) - weight_blocks) * BLOCK + threadIdx.x;
+        if (j >= a.out) return;
+        float s = 0.f;
+        for (int k = 0; k < job.runs; k++) s += job.bias_part[int64_t(k) * a.out + j];
+        a.bias[j] = s;
+        return;
+    }
+    const int64_t i = int64_t(blockIdx.x) * BLOCK + threadIdx.x, n = a.width * a.out;
+    if (i >= n) return;
+    float s = 0.f;
+    int k = 0;
+    for (; k + 8 <= job.runs; k += 8) {
+        float v[8];
+#pragma unroll
+        for (int u = 0; u < 8; u++) v[u] = job.part[(k + u) * n + i];
+#pragma unroll
+        for (int u = 0; u < 8; u++) s += v[u];
+    }
+    for (; k < job.runs; k++) s += job.part[k * n + i];
+    ((W*)a.weight)[i / a.out * a.weight_stride + i % a.out] = (W)s;
+}
+
+// Tile and runs.
+struct Plan {
+    int f, tiles_i, tiles_j, runs;
+    int64_t run;
+};
+
+Plan plan_of(const wc_ckpt_weight_args& a, int cus) {
+    Plan best = {};
+    double least = 0;
+    for (int f : {4, 2}) {
+        if (f == 4 && a.dtype == WC_DTYPE_F32) continue;  // the wider chunks leave no registers for it
+        const int tile = 64 * f;
+        const int64_t ti = (a.width + tile - 1) / tile, tj = (a.out + tile - 1) / tile, tiles = ti * tj;
+        const int64_t steps = (a.rows + DEPTH - 1) / DEPTH;
+        const int64_t slots = f == 4 ? cus : 2 * cus;
+        // microseconds of one step of all slots, and of a partial product written and read
+        const double step = f == 4 ? 1.4 : 0.9;
+        for (int64_t runs = 1; runs <= std::max<int64_t>(1, std::min<int64_t>(steps / 4, 4 * slots)); runs++) {
+            if (runs > 1 && tiles * runs > 4 * slots) break;
+            const int64_t per = std::max<int64_t>(1, (steps + runs - 1) / runs);
+            const double t = double((tiles * runs + slots - 1) / slots) * (per * step + 3.0) +
+                             (runs > 1 ? 4.0 + double(runs) * a.width * a.out * 8 / 4e6 : 0.0);
+            if (!best.f || t < least) {
+                least = t;
+                best = {f, (int)ti, (int)tj, (int)((steps + per - 1) / std::max<int64_t>(per, 1)), per * DEPTH};
+                best.runs = std::max(best.runs, 1);
+            }
+        }
+    }
+    return best;
+}
+
+template <class T, int F>
+void weight_at(const Job& job, hipStream_t s) {
+    k_weight<T, F><<<dim3(job.tiles_i * job.tiles_j * job.runs), BLOCK, 0, s>>>(job);
 }
 
 template <class T>
 void weight(const wc_ckpt_weight_args& a, int cus, hipStream_t s) {
-    const int runs = runs_of(a, cus);
-    const int64_t run = ((a.rows + runs - 1) / runs + DEPTH - 1) / DEPTH * DEPTH;
-    float* part = (float*)a.workspace;
-    float* bias = (float*)((uint8_t*)a.workspace + pad256(size_t(runs) * a.width * a.out * 4));
-    k_weight<T><<<dim3((uint32_t)((a.width + TILE - 1) / TILE), (uint32_t)((a.out + TILE - 1) / TILE), runs), BLOCK, 0,
-                  s>>>(a, run, part);
-    const dim3 g((uint32_t)((a.width * a.out + BLOCK - 1) / BLOCK));
-    if (a.weight_dtype == WC_DTYPE_F32)
-        k_weight_sum<float><<<g, BLOCK, 0, s>>>(part, runs, a.width, a.out, (float*)a.weight, a.weight_stride);
-    else
-        k_weight_sum<T><<<g, BLOCK, 0, s>>>(part, runs, a.width, a.out, (T*)a.weight, a.weight_stride);
-    if (a.bias) {
-        const int64_t brun = (a.rows + BIAS_RUNS - 1) / BIAS_RUNS;
-        const dim3 bg((uint32_t)((a.out + BLOCK - 1) / BLOCK), BIAS_RUNS);
-        k_bias<T><<<bg, BLOCK, 0, s>>>((const T*)a.grad, a.grad_stride, a.rows, a.out, brun, bias);
-        k_weight_sum<float><<<dim3((uint32_t)((a.out + BLOCK - 1) / BLOCK)), BLOCK, 0, s>>>(bias, BIAS_RUNS, 1, a.out,
-                                                                                           a.bias, a.out);
+    const Plan p = plan_of(a, cus);
+    Job job = {a, p.run, p.tiles_i, p.tiles_j, p.runs, (float*)a.workspace, nullptr};
+    job.bias_part = (float*)((uint8_t*)a.workspace + pad256(size_t(p.runs) * a.width * a.out * 4));
+    if constexpr (sizeof(T) == 2) {
+        if (p.f == 4) weight_at<T, 4>(job, s);
+        else weight_at<T, 2>(job, s);
+    } else {
+        weight_at<T, 2>(job, s);
+    }
+    if (p.runs > 1) {
+        const int64_t blocks = (a.width * a.out + BLOCK - 1) / BLOCK;
+        const dim3 g((uint32_t)(blocks + (a.bias ? (a.out + BLOCK - 1) / BLOCK : 0)));
+        if (a.weight_dtype == WC_DTYPE_F32) k_weight_sum<float><<<g, BLOCK, 0, s>>>(job, blocks);
+        else k_weight_sum<T><<<g, BLOCK, 0, s>>>(job, blocks);
     }
 }
 
 }  // namespace
 
 size_t ckpt_weight_scratch(const wc_ckpt_weight_args& a, int cus) {
-    return pad256(size_t(runs_of(a, cus)) * a.width * a.out * 4) + pad256(size_t(BIAS_RUNS) * a.out * 4);
+    const Plan p = plan_of(a, cus);
+    return p.runs == 1 ? 0 : pad256(size_t(p.runs) * a.width * a.out * 4) + pad256(size_t(p.runs) * a.out * 4);
 }
 
 void launch_ckpt_weight(const wc_ckpt_weight_args& a, int cus, hipStream_t s) {
