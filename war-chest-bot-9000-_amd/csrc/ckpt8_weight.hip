@@ -258,6 +258,192 @@ __global__ __launch_bounds__(BLOCK, F == 4 ? 1 : 2) void k_weight(Job job) {
     }
 }
 
+// --------------------------------------------------- large products, 16-bit
+
+// Both operands in 16 bits with rows on 16 bytes: the kept values expanded once
+// (an activation recomputed for every column tile would cost more than the
+// products), the gradient as it is or copied. 256 x 256 tiles, four wavefronts
+// of 128 x 128; tiles go from memory to LDS without passing registers, four
+// buffers of 32 rows, three of them in flight.
+constexpr int BIG = 256, BIG_DEPTH = 32, BIG_ROW = 2 * BIG, BIG_SIDE = BIG_DEPTH * BIG_ROW, BUFFERS = 4;
+
+static __device__ __align__(16) uint4 g_zeros;  // what rows past the end are read from
+
+struct BigJob {
+    Job job;
+    const char* x;     // rows x width, x_pitch bytes a row
+    const char* g;     // rows x out, g_pitch bytes a row
+    int64_t x_pitch, g_pitch;
+};
+
+__device__ __forceinline__ float plus(bf16x8 v, float s) {
+    typedef bf16 bf16x2 __attribute__((ext_vector_type(2)));
+    const bf16x2 one = {(bf16)1.f, (bf16)1.f};
+#pragma unroll
+    for (int i = 0; i < 8; i += 2) s = __builtin_amdgcn_fdot2_f32_bf16(bf16x2{v[i], v[i + 1]}, one, s, false);
+    return s;
+}
+__device__ __forceinline__ float plus(f16x8 v, float s) {
+    typedef f16 f16x2 __attribute__((ext_vector_type(2)));
+    const f16x2 one = {(f16)1.f, (f16)1.f};
+#pragma unroll
+    for (int i = 0; i < 8; i += 2) s = __builtin_amdgcn_fdot2(f16x2{v[i], v[i + 1]}, one, s, false);
+    return s;
+}
+
+template <class E>
+__global__ __launch_bounds__(BLOCK, 1) void k_weight_big(BigJob big) {
+    typedef E E8 __attribute__((ext_vector_type(8)));
+    typedef __attribute__((address_space(3))) char* Lds;
+    typedef __attribute__((address_space(3))) s16x4* Lds4;
+    __shared__ __align__(16) char lds[BUFFERS * 2 * BIG_SIDE];
+    const Job& job = big.job;
+    const wc_ckpt_weight_args& a = job.a;
+    const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
+    const int tiles = job.tiles_i * job.tiles_j, per = tiles * job.runs / 8;
+    const int id = blockIdx.x < (unsigned)per * 8 ? (blockIdx.x % 8) * per + blockIdx.x / 8 : blockIdx.x;
+    const int run = id / tiles, tile = id - run * tiles;
+    // four rows of tiles at a time: 32 neighbouring workgroups share 4 + 8 panels
+    const int band = tile / (4 * job.tiles_j), high = min(4, job.tiles_i - 4 * band), in = tile - band * 4 * job.tiles_j;
+    const int ti = 4 * band + in % high, tj = in / high;
+    const int64_t i0 = int64_t(ti) * BIG, j0 = int64_t(tj) * BIG;
+    const int64_t lo = run * job.run, hi = min(lo + job.run, a.rows);
+    const int steps = (int)((max<int64_t>(hi - lo, 0) + BIG_DEPTH - 1) / BIG_DEPTH);
+
+    // A wavefront's load moves two rows of a tile, 32 lanes of 16 bytes each, to
+    // the place in LDS that its lanes follow in order. A transposing read takes 64
+    // bytes of four consecutive rows: so that they lie in different banks, row r's
+    // 64-byte units are exchanged by r modulo 4, by which lane loads what.
+    int ox[2], og[2];
+#pragma unroll
+    for (int odd = 0; odd < 2; odd++) {
+        const int chunk = (lane & 31) ^ ((2 * odd + (lane >> 5)) << 2);
+        // past the last column any column will do: its products are not stored
+        ox[odd] = (int)(i0 + 8 * chunk < a.width ? 16 * chunk : 0);
+        og[odd] = (int)(j0 + 8 * chunk < a.out ? 16 * chunk : 0);
+    }
+    const char* x0 = big.x + lo * big.x_pitch + 2 * i0 + (lane >> 5) * big.x_pitch;
+    const char* g0 = big.g + lo * big.g_pitch + 2 * j0 + (lane >> 5) * big.g_pitch;
+    auto fetch = [&](int s) {
+        char* to = lds + (s % BUFFERS) * 2 * BIG_SIDE + wave * 8 * BIG_ROW;
+        const int64_t r0 = int64_t(s) * BIG_DEPTH + wave * 8, left = hi - lo - r0;
+        const char* x = x0 + r0 * big.x_pitch;
+        const char* g = g0 + r0 * big.g_pitch;
+#pragma unroll
+        for (int m = 0; m < 4; m++) {
+            const bool there = 2 * m + (lane >> 5) < left;
+            const char* px = there ? x + 2 * m * big.x_pitch + ox[m & 1] : (const char*)&g_zeros;
+            const char* pg = there ? g + 2 * m * big.g_pitch + og[m & 1] : (const char*)&g_zeros;
+            __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)px,
+                                             (__attribute__((address_space(3))) void*)(to + 2 * m * BIG_ROW), 16, 0, 0);
+            __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)pg,
+                                             (__attribute__((address_space(3))) void*)(to + BIG_SIDE + 2 * m * BIG_ROW),
+                                             16, 0, 0);
+        }
+    };
+
+    const int wi = (wave >> 1) * 128, wj = (wave & 1) * 128;
+    const int row = 8 * (lane >> 5) + ((lane & 15) >> 2), turn = ((lane & 15) >> 2) << 6;
+    int at[4];
+#pragma unroll
+    for (int m = 0; m < 4; m++) at[m] = row * BIG_ROW + ((64 * m + 2 * ((lane & 16) + 4 * (lane & 3))) ^ turn);
+    auto take = [&](int s, int k0, E8 (&fa)[4], E8 (&fb)[4]) {
+        const Lds from = (Lds)lds + (s % BUFFERS) * 2 * BIG_SIDE + k0 * BIG_ROW;
+#pragma unroll
+        for (int m = 0; m < 4; m++) {
+            const Lds pa = from + at[m] + 2 * wi, pb = from + at[m] + 2 * wj + BIG_SIDE;
+            const s16x4 a0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Lds4)pa);
+            const s16x4 a1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Lds4)(pa + 4 * BIG_ROW));
+            const s16x4 b0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Lds4)pb);
+            const s16x4 b1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Lds4)(pb + 4 * BIG_ROW));
+            fa[m] = __builtin_bit_cast(E8, __builtin_shufflevector(a0, a1, 0, 1, 2, 3, 4, 5, 6, 7));
+            fb[m] = __builtin_bit_cast(E8, __builtin_shufflevector(b0, b1, 0, 1, 2, 3, 4, 5, 6, 7));
+        }
+    };
+
+    f32x16 acc[4][4] = {};
+    float bias[4] = {};
+    const bool sums = a.bias && ti == 0 && wi == 0;
+    auto multiply = [&](const E8 (&fa)[4], const E8 (&fb)[4]) {
+#pragma unroll
+        for (int m = 0; m < 4; m++)
+#pragma unroll
+            for (int n = 0; n < 4; n++) acc[m][n] = mfma(fa[m], fb[n], acc[m][n]);
+        if (sums) {
+#pragma unroll
+            for (int n = 0; n < 4; n++) bias[n] = plus(fb[n], bias[n]);
+        }
+    };
+    // Of the 24 loads that three buffers take, the first 8 have arrived when 16 are left.
+    auto arrived = [&]() {
+        asm volatile("s_waitcnt vmcnt(16) lgkmcnt(0)" ::: "memory");
+        __builtin_amdgcn_s_barrier();
+    };
+    fetch(0);
+    fetch(1);
+    fetch(2);
+    arrived();
+    E8 fa[4], fb[4], na[4], nb[4];
+    take(0, 0, fa, fb);
+    for (int s = 0; s < steps; s++) {
+        fetch(s + 3);  // past the end it reads zeros, and the count of loads in flight stays the same
+        take(s, 16, na, nb);
+        multiply(fa, fb);
+        arrived();  // the next buffer's, and every wavefront has read this one's
+        take(s + 1, 0, fa, fb);
+        multiply(na, nb);
+    }
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+
+    const bool last = job.runs == 1;
+    float* part = job.part + int64_t(run) * a.width * a.out;
+#pragma unroll
+    for (int m = 0; m < 4; m++)
+#pragma unroll
+        for (int n = 0; n < 4; n++)
+#pragma unroll
+            for (int k = 0; k < 16; k++) {
+                const int64_t i = i0 + wi + 32 * m + 8 * (k / 4) + 4 * (lane >> 5) + k % 4, j = j0 + wj + 32 * n + (lane & 31);
+                if (i >= a.width || j >= a.out) continue;
+                if (!last) part[i * a.out + j] = acc[m][n][k];
+                else if (a.weight_dtype == WC_DTYPE_F32) ((float*)a.weight)[i * a.weight_stride + j] = acc[m][n][k];
+                else ((E*)a.weight)[i * a.weight_stride + j] = (E)acc[m][n][k];
+            }
+    if (sums) {  // a column's rows are in two lanes
+#pragma unroll
+        for (int n = 0; n < 4; n++) {
+            const float s = bias[n] + __shfl_xor(bias[n], 32);
+            const int64_t j = j0 + wj + 32 * n + lane;
+            if (lane < 32 && j < a.out) (last ? a.bias : job.bias_part + int64_t(run) * a.out)[j] = s;
+        }
+    }
+}
+
+// What the large product reads: act(kept) in 16 bits, rows of `pitch` elements.
+template <class E>
+__global__ __launch_bounds__(BLOCK) void k_expand(wc_ckpt_weight_args a, E* to, int64_t pitch, int64_t per_row) {
+    typedef E E8 __attribute__((ext_vector_type(8)));
+    const int64_t total = a.rows * per_row;
+    for (int64_t i = int64_t(blockIdx.x) * BLOCK + threadIdx.x; i < total; i += int64_t(gridDim.x) * BLOCK) {
+        const int64_t r = i / per_row, c = (i - r * per_row) * 16;
+        __align__(16) char out[32];
+        put_kept<E>(load_kept(a, r, a.rows, c), a.act, out);
+        E8* p = (E8*)(to + r * pitch + c);
+        p[0] = ((const E8*)out)[0];
+        p[1] = ((const E8*)out)[1];
+    }
+}
+
+// A gradient whose rows do not start on 16 bytes, copied to rows that do.
+template <class T>
+__global__ __launch_bounds__(BLOCK) void k_align(wc_ckpt_weight_args a, T* to, int64_t pitch, int64_t per_row) {
+    const int64_t total = a.rows * per_row;
+    for (int64_t i = int64_t(blockIdx.x) * BLOCK + threadIdx.x; i < total; i += int64_t(gridDim.x) * BLOCK) {
+        const int64_t r = i / per_row, c = (i - r * per_row) * 8;
+        *(typename Vec8<T>::type*)(to + r * pitch + c) = load_grad<T>(a, r, a.rows, c);
+    }
+}
+
 // The runs' partial products, added in order; the workgroups past the weights'
 // add the bias's.
 template <class W>
@@ -286,54 +472,88 @@ __global__ __launch_bounds__(BLOCK) void k_weight_sum(Job job, int64_t weight_bl
     ((W*)a.weight)[i / a.out * a.weight_stride + i % a.out] = (W)s;
 }
 
-// Tile and runs.
+// Which kernel, its tiles and runs, and where its scratch lies.
 struct Plan {
-    int f, tiles_i, tiles_j, runs;
+    bool big;
+    int tiles_i, tiles_j, runs;
     int64_t run;
+    bool copy;             // big: the gradient is copied to aligned rows
+    int64_t xp, gp;        // big: elements from row to row
+    size_t x, g, part, bias, bytes;
 };
 
+// Microseconds that a product takes, from measured parts: a step of a
+// workgroup's, its start and end, a partial product written and read, and
+// what the large product's operands cost to lay out.
 Plan plan_of(const wc_ckpt_weight_args& a, int cus) {
     Plan best = {};
-    double least = 0;
-    for (int f : {4, 2}) {
-        if (f == 4 && a.dtype == WC_DTYPE_F32) continue;  // the wider chunks leave no registers for it
-        const int tile = 64 * f;
+    double least = -1;
+    const bool aligned = a.out % 8 == 0 && a.grad_stride % 8 == 0 && ((uintptr_t)a.grad & 15) == 0;
+    for (int big = 0; big < 2; big++) {
+        if (big && a.dtype == WC_DTYPE_F32) continue;
+        const int tile = big ? BIG : Shape<2>::TILE, depth = big ? BIG_DEPTH : DEPTH;
         const int64_t ti = (a.width + tile - 1) / tile, tj = (a.out + tile - 1) / tile, tiles = ti * tj;
-        const int64_t steps = (a.rows + DEPTH - 1) / DEPTH;
-        const int64_t slots = f == 4 ? cus : 2 * cus;
-        // microseconds of one step of all slots, and of a partial product written and read
-        const double step = f == 4 ? 1.4 : 0.9;
-        for (int64_t runs = 1; runs <= std::max<int64_t>(1, std::min<int64_t>(steps / 4, 4 * slots)); runs++) {
-            if (runs > 1 && tiles * runs > 4 * slots) break;
+        const int64_t steps = (a.rows + depth - 1) / depth, slots = big ? cus : 2 * cus;
+        const double value = a.act == WC_ACT_GELU || a.act == WC_ACT_SILU ? 1.3 : 0.0;
+        const double step = big ? 0.55 : 0.95 + value;
+        const double lay = big ? 3.0 + double(a.rows) * (a.width * 3 + (aligned ? 0 : a.out * 4)) / 4e6 : 0.0;
+        const int64_t most = std::max<int64_t>(1, std::min<int64_t>(steps / 8, 4 * slots / tiles));
+        for (int64_t runs = 1; runs <= most; runs++) {
             const int64_t per = std::max<int64_t>(1, (steps + runs - 1) / runs);
-            const double t = double((tiles * runs + slots - 1) / slots) * (per * step + 3.0) +
-                             (runs > 1 ? 4.0 + double(runs) * a.width * a.out * 8 / 4e6 : 0.0);
-            if (!best.f || t < least) {
-                least = t;
-                best = {f, (int)ti, (int)tj, (int)((steps + per - 1) / std::max<int64_t>(per, 1)), per * DEPTH};
-                best.runs = std::max(best.runs, 1);
-            }
+            const double t = lay + double((tiles * runs + slots - 1) / slots) * (per * step + 4.0) +
+                             (runs > 1 ? 3.0 + double(runs) * a.width * a.out * 8 / 4e6 : 0.0);
+            if (least >= 0 && t >= least) continue;
+            least = t;
+            best = {};
+            best.big = big;
+            best.tiles_i = (int)ti;
+            best.tiles_j = (int)tj;
+            best.runs = (int)std::max<int64_t>(1, (steps + per - 1) / per);
+            best.run = per * depth;
+            best.copy = big && !aligned;
         }
     }
+    size_t at = 0;
+    auto take = [&](size_t n) {
+        const size_t here = at;
+        at += pad256(n);
+        return here;
+    };
+    if (best.big) {
+        best.xp = (a.width + 15) / 16 * 16;
+        best.gp = best.copy ? (a.out + 7) / 8 * 8 : a.grad_stride;
+        best.x = take(size_t(a.rows) * best.xp * 2);
+        best.g = best.copy ? take(size_t(a.rows) * best.gp * 2) : 0;
+    }
+    if (best.runs > 1) {
+        best.part = take(size_t(best.runs) * a.width * a.out * 4);
+        best.bias = take(size_t(best.runs) * a.out * 4);
+    }
+    best.bytes = at;
     return best;
-}
-
-template <class T, int F>
-void weight_at(const Job& job, hipStream_t s) {
-    k_weight<T, F><<<dim3(job.tiles_i * job.tiles_j * job.runs), BLOCK, 0, s>>>(job);
 }
 
 template <class T>
 void weight(const wc_ckpt_weight_args& a, int cus, hipStream_t s) {
     const Plan p = plan_of(a, cus);
-    Job job = {a, p.run, p.tiles_i, p.tiles_j, p.runs, (float*)a.workspace, nullptr};
-    job.bias_part = (float*)((uint8_t*)a.workspace + pad256(size_t(p.runs) * a.width * a.out * 4));
+    char* w = (char*)a.workspace;
+    const Job job = {a, p.run, p.tiles_i, p.tiles_j, p.runs, (float*)(w + p.part), (float*)(w + p.bias)};
+    const dim3 grid(p.tiles_i * p.tiles_j * p.runs);
     if constexpr (sizeof(T) == 2) {
-        if (p.f == 4) weight_at<T, 4>(job, s);
-        else weight_at<T, 2>(job, s);
-    } else {
-        weight_at<T, 2>(job, s);
+        if (p.big) {
+            auto lay_grid = [&](int64_t n) {
+                return dim3((uint32_t)std::max<int64_t>(1, std::min<int64_t>((n + BLOCK - 1) / BLOCK, cus * 64)));
+            };
+            if (a.rows) {
+                const int64_t x = p.xp / 16, g = p.gp / 8;
+                k_expand<T><<<lay_grid(a.rows * x), BLOCK, 0, s>>>(a, (T*)(w + p.x), p.xp, x);
+                if (p.copy) k_align<T><<<lay_grid(a.rows * g), BLOCK, 0, s>>>(a, (T*)(w + p.g), p.gp, g);
+            }
+            const BigJob big = {job, w + p.x, p.copy ? w + p.g : (const char*)a.grad, 2 * p.xp, 2 * p.gp};
+            k_weight_big<T><<<grid, BLOCK, 0, s>>>(big);
+        }
     }
+    if (!p.big) k_weight<T, 2><<<grid, BLOCK, 0, s>>>(job);
     if (p.runs > 1) {
         const int64_t blocks = (a.width * a.out + BLOCK - 1) / BLOCK;
         const dim3 g((uint32_t)(blocks + (a.bias ? (a.out + BLOCK - 1) / BLOCK : 0)));
@@ -344,10 +564,7 @@ void weight(const wc_ckpt_weight_args& a, int cus, hipStream_t s) {
 
 }  // namespace
 
-size_t ckpt_weight_scratch(const wc_ckpt_weight_args& a, int cus) {
-    const Plan p = plan_of(a, cus);
-    return p.runs == 1 ? 0 : pad256(size_t(p.runs) * a.width * a.out * 4) + pad256(size_t(p.runs) * a.out * 4);
-}
+size_t ckpt_weight_scratch(const wc_ckpt_weight_args& a, int cus) { return plan_of(a, cus).bytes; }
 
 void launch_ckpt_weight(const wc_ckpt_weight_args& a, int cus, hipStream_t s) {
     if (a.dtype == WC_DTYPE_F32) weight<float>(a, cus, s);
