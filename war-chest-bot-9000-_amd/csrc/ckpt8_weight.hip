@@ -291,11 +291,119 @@ __device__ __forceinline__ float plus(f16x8 v, float s) {
     return s;
 }
 
-template <class E>
+// LDS as the large product addresses it.
+typedef __attribute__((address_space(3))) char* Lds;
+
+// One wavefront's share of a step's tiles, from memory to LDS: eight rows of
+// each, in four parts of two. A load's 64 lanes bring 16 bytes each to places
+// in LDS that follow each other. A transposing read takes 64 bytes of four
+// consecutive rows: so that they lie in different banks, row r's 64-byte units
+// are exchanged by r modulo 4, by which lane loads what.
+struct Fetch {
+    const char *x, *g;  // the wavefront's first row: the same for all lanes
+    int64_t x_pitch, g_pitch, rows;
+    uint32_t ox[2], og[2];  // the lane's place in two rows, for the even parts and the odd ones
+    int half;
+
+    // ENDS: rows past the end are read from zeros.
+    template <bool ENDS>
+    __device__ __forceinline__ void part(int s, int m, Lds to) const {
+        const int64_t r0 = int64_t(s) * BIG_DEPTH + 2 * m;
+        const char* fx = x + r0 * x_pitch;
+        const char* fg = g + r0 * g_pitch;
+        if (ENDS) {
+            const bool there = r0 + half < rows;
+            load(there ? fx + ox[m & 1] : (const char*)&g_zeros, to + 2 * m * BIG_ROW);
+            load(there ? fg + og[m & 1] : (const char*)&g_zeros, to + BIG_SIDE + 2 * m * BIG_ROW);
+        } else {
+            load(fx + ox[m & 1], to + 2 * m * BIG_ROW);
+            load(fg + og[m & 1], to + BIG_SIDE + 2 * m * BIG_ROW);
+        }
+    }
+    static __device__ __forceinline__ void load(const char* from, Lds to) {
+        __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)from,
+                                         (__attribute__((address_space(3))) void*)to, 16, 0, 0);
+    }
+};
+
+// Sixteen rows of a buffer: one fragment of each operand.
+template <class E8>
+__device__ __forceinline__ void take(Lds from, int at, int wi, int wj, E8& fa, E8& fb) {
+    typedef __attribute__((address_space(3))) s16x4* Lds4;
+    const Lds pa = from + at + 2 * wi, pb = from + at + 2 * wj + BIG_SIDE;
+    const s16x4 a0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Lds4)pa);
+    const s16x4 a1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Lds4)(pa + 4 * BIG_ROW));
+    const s16x4 b0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Lds4)pb);
+    const s16x4 b1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Lds4)(pb + 4 * BIG_ROW));
+    fa = __builtin_bit_cast(E8, __builtin_shufflevector(a0, a1, 0, 1, 2, 3, 4, 5, 6, 7));
+    fb = __builtin_bit_cast(E8, __builtin_shufflevector(b0, b1, 0, 1, 2, 3, 4, 5, 6, 7));
+}
+
+// Of the 24 loads that three buffers take, the first 8 have arrived when 16 are left.
+__device__ __forceinline__ void arrived() {
+    asm volatile("s_waitcnt vmcnt(16) lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+}
+
+// One step: the buffer `from`, whose first fragments are in fa and fb, and the
+// first of `next`; the loads of three steps on go to `to`. The three are
+// different buffers: told so, the compiler lets reads pass loads in flight.
+// Everything else goes between the matrix instructions, which take 32 cycles
+// each: four of them, then the loads and reads of one part.
+template <class E8, bool SUMS, bool ENDS>
+__device__ __forceinline__ void step(Lds __restrict__ from, Lds __restrict__ next, Lds __restrict__ to,
+                                     const Fetch& fetch, int s, const int (&at)[4], int wi, int wj, E8 (&fa)[4],
+                                     E8 (&fb)[4], f32x16 (&acc)[4][4], float (&bias)[4]) {
+    E8 na[4], nb[4];
+#pragma unroll
+    for (int m = 0; m < 4; m++) {
+        fetch.part<ENDS>(s + 3, m, to);
+        take(from + 16 * BIG_ROW, at[m], wi, wj, na[m], nb[m]);
+#pragma unroll
+        for (int n = 0; n < 4; n++) acc[m][n] = mfma(fa[m], fb[n], acc[m][n]);
+        if (SUMS) bias[m] = plus(fb[m], bias[m]);
+        __builtin_amdgcn_sched_barrier(0);
+    }
+    E8 oa[4], ob[4];
+#pragma unroll
+    for (int m = 0; m < 4; m++) {
+#pragma unroll
+        for (int n = 0; n < 4; n++) acc[m][n] = mfma(na[m], nb[n], acc[m][n]);
+        if (SUMS) bias[m] = plus(nb[m], bias[m]);
+        __builtin_amdgcn_sched_barrier(0);
+        if (m == 0) arrived();  // the next buffer's, and every wavefront has read this one's
+        take(next, at[m], wi, wj, oa[m], ob[m]);
+    }
+#pragma unroll
+    for (int m = 0; m < 4; m++) fa[m] = oa[m], fb[m] = ob[m];
+}
+
+template <class E8, bool SUMS>
+__device__ __forceinline__ void steps_of(Lds base, const Fetch& fetch, Lds mine, int64_t rows, const int (&at)[4],
+                                         int wi, int wj, f32x16 (&acc)[4][4], float (&bias)[4]) {
+    const int whole = (int)(rows / BIG_DEPTH), steps = (int)((rows + BIG_DEPTH - 1) / BIG_DEPTH);
+    E8 fa[4], fb[4];
+    for (int s = 0; s < 3; s++)
+#pragma unroll
+        for (int m = 0; m < 4; m++) fetch.part<true>(s, m, mine + s * 2 * BIG_SIDE);
+    arrived();
+#pragma unroll
+    for (int m = 0; m < 4; m++) take(base, at[m], wi, wj, fa[m], fb[m]);
+    int s = 0;
+    for (; s + 3 < whole; s++)
+        step<E8, SUMS, false>(base + (s & 3) * 2 * BIG_SIDE, base + (s + 1 & 3) * 2 * BIG_SIDE,
+                              mine + (s + 3 & 3) * 2 * BIG_SIDE, fetch, s, at, wi, wj, fa, fb, acc, bias);
+    // the last steps load zeros past the end: the count of loads in flight stays the same
+    for (; s < steps; s++)
+        step<E8, SUMS, true>(base + (s & 3) * 2 * BIG_SIDE, base + (s + 1 & 3) * 2 * BIG_SIDE,
+                             mine + (s + 3 & 3) * 2 * BIG_SIDE, fetch, s, at, wi, wj, fa, fb, acc, bias);
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+}
+
+// W: what is written, the weights' type or a run's float32 products.
+template <class E, class W>
 __global__ __launch_bounds__(BLOCK, 1) void k_weight_big(BigJob big) {
     typedef E E8 __attribute__((ext_vector_type(8)));
-    typedef __attribute__((address_space(3))) char* Lds;
-    typedef __attribute__((address_space(3))) s16x4* Lds4;
     __shared__ __align__(16) char lds[BUFFERS * 2 * BIG_SIDE];
     const Job& job = big.job;
     const wc_ckpt_weight_args& a = job.a;
@@ -308,107 +416,50 @@ __global__ __launch_bounds__(BLOCK, 1) void k_weight_big(BigJob big) {
     const int ti = 4 * band + in % high, tj = in / high;
     const int64_t i0 = int64_t(ti) * BIG, j0 = int64_t(tj) * BIG;
     const int64_t lo = run * job.run, hi = min(lo + job.run, a.rows);
-    const int steps = (int)((max<int64_t>(hi - lo, 0) + BIG_DEPTH - 1) / BIG_DEPTH);
 
-    // A wavefront's load moves two rows of a tile, 32 lanes of 16 bytes each, to
-    // the place in LDS that its lanes follow in order. A transposing read takes 64
-    // bytes of four consecutive rows: so that they lie in different banks, row r's
-    // 64-byte units are exchanged by r modulo 4, by which lane loads what.
-    int ox[2], og[2];
+    Fetch fetch;
+    const int64_t first = lo + wave * 8;
+    fetch.x = big.x + first * big.x_pitch + 2 * i0;
+    fetch.g = big.g + first * big.g_pitch + 2 * j0;
+    fetch.x_pitch = big.x_pitch;
+    fetch.g_pitch = big.g_pitch;
+    fetch.rows = hi - first;
+    fetch.half = lane >> 5;
 #pragma unroll
     for (int odd = 0; odd < 2; odd++) {
         const int chunk = (lane & 31) ^ ((2 * odd + (lane >> 5)) << 2);
         // past the last column any column will do: its products are not stored
-        ox[odd] = (int)(i0 + 8 * chunk < a.width ? 16 * chunk : 0);
-        og[odd] = (int)(j0 + 8 * chunk < a.out ? 16 * chunk : 0);
+        fetch.ox[odd] = (uint32_t)(fetch.half * big.x_pitch) + (i0 + 8 * chunk < a.width ? 16 * chunk : 0);
+        fetch.og[odd] = (uint32_t)(fetch.half * big.g_pitch) + (j0 + 8 * chunk < a.out ? 16 * chunk : 0);
     }
-    const char* x0 = big.x + lo * big.x_pitch + 2 * i0 + (lane >> 5) * big.x_pitch;
-    const char* g0 = big.g + lo * big.g_pitch + 2 * j0 + (lane >> 5) * big.g_pitch;
-    auto fetch = [&](int s) {
-        char* to = lds + (s % BUFFERS) * 2 * BIG_SIDE + wave * 8 * BIG_ROW;
-        const int64_t r0 = int64_t(s) * BIG_DEPTH + wave * 8, left = hi - lo - r0;
-        const char* x = x0 + r0 * big.x_pitch;
-        const char* g = g0 + r0 * big.g_pitch;
-#pragma unroll
-        for (int m = 0; m < 4; m++) {
-            const bool there = 2 * m + (lane >> 5) < left;
-            const char* px = there ? x + 2 * m * big.x_pitch + ox[m & 1] : (const char*)&g_zeros;
-            const char* pg = there ? g + 2 * m * big.g_pitch + og[m & 1] : (const char*)&g_zeros;
-            __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)px,
-                                             (__attribute__((address_space(3))) void*)(to + 2 * m * BIG_ROW), 16, 0, 0);
-            __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)pg,
-                                             (__attribute__((address_space(3))) void*)(to + BIG_SIDE + 2 * m * BIG_ROW),
-                                             16, 0, 0);
-        }
-    };
 
     const int wi = (wave >> 1) * 128, wj = (wave & 1) * 128;
     const int row = 8 * (lane >> 5) + ((lane & 15) >> 2), turn = ((lane & 15) >> 2) << 6;
     int at[4];
 #pragma unroll
     for (int m = 0; m < 4; m++) at[m] = row * BIG_ROW + ((64 * m + 2 * ((lane & 16) + 4 * (lane & 3))) ^ turn);
-    auto take = [&](int s, int k0, E8 (&fa)[4], E8 (&fb)[4]) {
-        const Lds from = (Lds)lds + (s % BUFFERS) * 2 * BIG_SIDE + k0 * BIG_ROW;
-#pragma unroll
-        for (int m = 0; m < 4; m++) {
-            const Lds pa = from + at[m] + 2 * wi, pb = from + at[m] + 2 * wj + BIG_SIDE;
-            const s16x4 a0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Lds4)pa);
-            const s16x4 a1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Lds4)(pa + 4 * BIG_ROW));
-            const s16x4 b0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Lds4)pb);
-            const s16x4 b1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Lds4)(pb + 4 * BIG_ROW));
-            fa[m] = __builtin_bit_cast(E8, __builtin_shufflevector(a0, a1, 0, 1, 2, 3, 4, 5, 6, 7));
-            fb[m] = __builtin_bit_cast(E8, __builtin_shufflevector(b0, b1, 0, 1, 2, 3, 4, 5, 6, 7));
-        }
-    };
 
     f32x16 acc[4][4] = {};
     float bias[4] = {};
     const bool sums = a.bias && ti == 0 && wi == 0;
-    auto multiply = [&](const E8 (&fa)[4], const E8 (&fb)[4]) {
-#pragma unroll
-        for (int m = 0; m < 4; m++)
-#pragma unroll
-            for (int n = 0; n < 4; n++) acc[m][n] = mfma(fa[m], fb[n], acc[m][n]);
-        if (sums) {
-#pragma unroll
-            for (int n = 0; n < 4; n++) bias[n] = plus(fb[n], bias[n]);
-        }
-    };
-    // Of the 24 loads that three buffers take, the first 8 have arrived when 16 are left.
-    auto arrived = [&]() {
-        asm volatile("s_waitcnt vmcnt(16) lgkmcnt(0)" ::: "memory");
-        __builtin_amdgcn_s_barrier();
-    };
-    fetch(0);
-    fetch(1);
-    fetch(2);
-    arrived();
-    E8 fa[4], fb[4], na[4], nb[4];
-    take(0, 0, fa, fb);
-    for (int s = 0; s < steps; s++) {
-        fetch(s + 3);  // past the end it reads zeros, and the count of loads in flight stays the same
-        take(s, 16, na, nb);
-        multiply(fa, fb);
-        arrived();  // the next buffer's, and every wavefront has read this one's
-        take(s + 1, 0, fa, fb);
-        multiply(na, nb);
-    }
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    const Lds base = (Lds)lds, mine = base + wave * 8 * BIG_ROW;
+    if (sums) steps_of<E8, true>(base, fetch, mine, max<int64_t>(hi - lo, 0), at, wi, wj, acc, bias);
+    else steps_of<E8, false>(base, fetch, mine, max<int64_t>(hi - lo, 0), at, wi, wj, acc, bias);
 
     const bool last = job.runs == 1;
-    float* part = job.part + int64_t(run) * a.width * a.out;
+    const int64_t stride = last ? a.weight_stride : a.out;
+    W* to = last ? (W*)a.weight : (W*)(job.part + int64_t(run) * a.width * a.out);
+    const int64_t i1 = i0 + wi + 4 * (lane >> 5), j1 = j0 + wj + (lane & 31);
+    to += i1 * stride + j1;
 #pragma unroll
     for (int m = 0; m < 4; m++)
 #pragma unroll
-        for (int n = 0; n < 4; n++)
+        for (int k = 0; k < 16; k++) {
+            const int di = 32 * m + 8 * (k / 4) + k % 4;
 #pragma unroll
-            for (int k = 0; k < 16; k++) {
-                const int64_t i = i0 + wi + 32 * m + 8 * (k / 4) + 4 * (lane >> 5) + k % 4, j = j0 + wj + 32 * n + (lane & 31);
-                if (i >= a.width || j >= a.out) continue;
-                if (!last) part[i * a.out + j] = acc[m][n][k];
-                else if (a.weight_dtype == WC_DTYPE_F32) ((float*)a.weight)[i * a.weight_stride + j] = acc[m][n][k];
-                else ((E*)a.weight)[i * a.weight_stride + j] = (E)acc[m][n][k];
-            }
+            for (int n = 0; n < 4; n++)
+                if (i1 + di < a.width && j1 + 32 * n < a.out) to[di * stride + 32 * n] = (W)acc[m][n][k];
+        }
     if (sums) {  // a column's rows are in two lanes
 #pragma unroll
         for (int n = 0; n < 4; n++) {
@@ -488,7 +539,9 @@ struct Plan {
 Plan plan_of(const wc_ckpt_weight_args& a, int cus) {
     Plan best = {};
     double least = -1;
-    const bool aligned = a.out % 8 == 0 && a.grad_stride % 8 == 0 && ((uintptr_t)a.grad & 15) == 0;
+    // (a lane's offset in two rows is held in 32 bits)
+    const bool aligned = a.out % 8 == 0 && a.grad_stride % 8 == 0 && ((uintptr_t)a.grad & 15) == 0 &&
+                         a.grad_stride < (1 << 29);
     for (int big = 0; big < 2; big++) {
         if (big && a.dtype == WC_DTYPE_F32) continue;
         const int tile = big ? BIG : Shape<2>::TILE, depth = big ? BIG_DEPTH : DEPTH;
@@ -550,7 +603,8 @@ void weight(const wc_ckpt_weight_args& a, int cus, hipStream_t s) {
                 if (p.copy) k_align<T><<<lay_grid(a.rows * g), BLOCK, 0, s>>>(a, (T*)(w + p.g), p.gp, g);
             }
             const BigJob big = {job, w + p.x, p.copy ? w + p.g : (const char*)a.grad, 2 * p.xp, 2 * p.gp};
-            k_weight_big<T><<<grid, BLOCK, 0, s>>>(big);
+            if (p.runs > 1 || a.weight_dtype == WC_DTYPE_F32) k_weight_big<T, float><<<grid, BLOCK, 0, s>>>(big);
+            else k_weight_big<T, T><<<grid, BLOCK, 0, s>>>(big);
         }
     }
     if (!p.big) k_weight<T, 2><<<grid, BLOCK, 0, s>>>(job);

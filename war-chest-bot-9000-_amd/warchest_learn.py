@@ -161,7 +161,7 @@ def _logits(t):
     return device, code, rows, vocab, _matrix(t, "logits", device, t.dtype, rows, vocab)
 
 
-# Scratch sizes depend on shapes alone.
+# Scratch sizes depend on shapes (and, for the weight gradient, on whether its rows start on 16 bytes).
 @functools.lru_cache(maxsize=4096)
 def _policy_scratch(device, code, rows, vocab):
     p = 256  # an address that passes for one: the size is computed from the shape, nothing is read
@@ -187,11 +187,11 @@ def _norm_scratch(device, code, rows, width):
 
 
 @functools.lru_cache(maxsize=4096)
-def _weight_scratch(device, code, rows, width, out, act, weight_code):
-    p = 256
+def _weight_scratch(device, code, rows, width, out, act, weight_code, aligned):
+    p, stride = 256, out if aligned else out + 1 - out % 2
     return _scratch_bytes("wc_ckpt_weight_workspace", _WEIGHT.pack(
-        _WEIGHT.size, device, code, rows, width, out, act, weight_code, p, width, p, -(-width // GROUP), p, out, p, out,
-        p, 0, 0))
+        _WEIGHT.size, device, code, rows, width, out, act, weight_code, p, width, p, -(-width // GROUP), p, stride, p,
+        out, p, 0, 0))
 
 
 def _scratch(n, device):
@@ -421,7 +421,7 @@ def checkpoint8_weight_grad(ck, grad, *, act="none", bias=False, dtype=None):
     wcode = _dtype(weight, "dtype")
     b = torch.empty(out, dtype=torch.float32, device=device) if bias else None
     a = _known(ACTS, act, "act")
-    need = _weight_scratch(device.index, code, rows, width, out, a, wcode)
+    need = _weight_scratch(device.index, code, rows, width, out, a, wcode, (g[0] | 2 * g[1] | 2 * out) % 16 == 0)
     work = _scratch(need, device)
     _call("wc_ckpt_weight_grad", _WEIGHT.pack(
         _WEIGHT.size, device.index, code, rows, width, out, a, wcode, *q, *e, *g, weight.data_ptr(), out,
