@@ -515,6 +515,35 @@ def test_weight_gradient_long_sums_strides_and_the_same_bits(dtype):
     assert torch.equal(one[0], two[0]) and torch.equal(one[1], two[1])
 
 
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("rows,width,out,name,pad", [
+    (9000, 1500, 1504, "gelu", 0),     # 256-wide tiles past both ends, several runs of rows, rows past the last step
+    (9001, 1500, 1501, "silu", 0),     # the gradient's rows at odd places: copied first
+    (9000, 1500, 1504, "gelu", 8),     # its rows apart in memory
+    (16384, 4096, 2048, "none", 0),    # whole tiles, whole steps
+    (16411, 2050, 4090, "relu", 2),
+])
+def test_weight_gradient_of_large_products(rows, width, out, name, pad, dtype):
+    """Sizes that the large tiles are taken for, against a float64 product on the device."""
+    say(f"case weight: {rows} x {width} x {out} {dtype} {name}, {pad} between rows")
+    t = TYPES[dtype]
+    g = torch.Generator(device=DEV).manual_seed(rows + out)
+    x = 1.5 * torch.randn(rows, width, generator=g, device=DEV)
+    d = torch.full((rows, out + pad), math.nan, dtype=t, device=DEV)[:, :out]
+    d.copy_(torch.randn(rows, out, generator=g, device=DEV))
+    ck = wl.checkpoint8(x)
+    a = R.act(wl.checkpoint8_read(ck, torch.float32).double(), name)
+    want = a.t().contiguous() @ d.double()
+    size = a.abs().t().contiguous() @ d.double().abs()
+    for wdtype in (torch.float32, t):
+        weight, bias = wl.checkpoint8_weight_grad(ck, d, act=name, bias=True, dtype=wdtype)
+        again, _ = wl.checkpoint8_weight_grad(ck, d, act=name, bias=True, dtype=wdtype)
+        assert torch.equal(weight, again)
+        bound = size * (2e-5 + (ROUND[t] if name in ("gelu", "silu") else 0.0)) + want.abs() * ROUND[wdtype] + STEP[wdtype]
+        assert not ((weight.double() - want).abs() > bound).any()
+        near(bias, d.double().sum(0).cpu(), "bias", scale=float(d.double().abs().sum(0).max()))
+
+
 def test_weight_gradient_of_a_sliced_checkpoint_and_nan_groups():
     """A checkpoint's rows may be a slice of a larger one; a group held as NaN reaches its own channels only."""
     x = torch.randn(64, 96, generator=gen(2))

@@ -73,10 +73,21 @@ struct Kept {
     uint32_t q[4], e;
 };
 
+// Zeros beyond the run and, with EDGE, beyond the row. Without it the load is
+// unconditional, from the run's last row where there is none: what the
+// compiler cannot count it would wait for at once.
+template <bool EDGE>
 __device__ __forceinline__ Kept load_kept(const wc_ckpt_weight_args& a, int64_t r, int64_t hi, int64_t c) {
     typedef uint32_t Words __attribute__((ext_vector_type(4), aligned(1)));
     Kept k = {{0, 0, 0, 0}, 1};
-    if (r < hi && c < a.width) {
+    if (!EDGE) {
+        const int64_t at = min(r, hi - 1);
+        const Words w = *(const Words*)(a.q + at * a.q_stride + c);
+        const uint32_t e = a.exps[at * a.exps_stride + (c >> 5)];
+#pragma unroll
+        for (int i = 0; i < 4; i++) k.q[i] = r < hi ? w[i] : 0u;
+        k.e = r < hi ? e : 1u;
+    } else if (r < hi && c < a.width) {
         const int8_t* p = a.q + r * a.q_stride + c;
         k.e = a.exps[r * a.exps_stride + (c >> 5)];
         if (c + 16 <= a.width) {
@@ -84,42 +95,49 @@ __device__ __forceinline__ Kept load_kept(const wc_ckpt_weight_args& a, int64_t 
 #pragma unroll
             for (int i = 0; i < 4; i++) k.q[i] = w[i];
         } else {
-            for (int i = 0; i < (int)(a.width - c); i++) k.q[i >> 2] |= (uint32_t)(uint8_t)p[i] << (8 * (i & 3));
+#pragma unroll
+            for (int i = 0; i < 16; i++)
+                if (c + i < a.width) k.q[i >> 2] |= (uint32_t)(uint8_t)p[i] << (8 * (i & 3));
         }
     }
     return k;
 }
 
+// Eight of them, in 16 bits.
 template <class E>
-__device__ __forceinline__ void put_kept(const Kept& k, int act, char* to) {
-    typedef E E8 __attribute__((ext_vector_type(8)));
+struct Eight {
+    typedef E type __attribute__((ext_vector_type(8)));
+};
+template <class E>
+__device__ __forceinline__ typename Eight<E>::type expand(const Kept& k, int act, int half) {
     const float step = step_of(k.e);
+    float v[8];
 #pragma unroll
-    for (int h = 0; h < 2; h++) {
-        float v[8];
+    for (int i = 0; i < 8; i++) v[i] = (float)(int8_t)(k.q[2 * half + (i >> 2)] >> (8 * (i & 3))) * step;
+    if (may_pass<E>(k.e)) {
 #pragma unroll
-        for (int i = 0; i < 8; i++) v[i] = (float)(int8_t)(k.q[2 * h + (i >> 2)] >> (8 * (i & 3))) * step;
-        if (may_pass<E>(k.e)) {
-#pragma unroll
-            for (int i = 0; i < 8; i++) v[i] = held<E>(v[i]);
-        }
-        if (act != WC_ACT_NONE) {
-#pragma unroll
-            for (int i = 0; i < 8; i++) v[i] = act_value(v[i], act);
-        }
-        E8 o;
-#pragma unroll
-        for (int i = 0; i < 8; i++) o[i] = (E)v[i];
-        *(E8*)(to + 16 * h) = o;
+        for (int i = 0; i < 8; i++) v[i] = held<E>(v[i]);
     }
+    if (act != WC_ACT_NONE) {
+#pragma unroll
+        for (int i = 0; i < 8; i++) v[i] = act_value(v[i], act);
+    }
+    typename Eight<E>::type o;
+#pragma unroll
+    for (int i = 0; i < 8; i++) o[i] = (E)v[i];
+    return o;
 }
 
-// Eight gradient values of one row, from column c; 0 beyond the run and the row.
-template <class T>
+// Eight gradient values of one row, from column c, alike.
+template <bool EDGE, class T>
 __device__ __forceinline__ typename Vec8<T>::type load_grad(const wc_ckpt_weight_args& a, int64_t r, int64_t hi,
                                                             int64_t c) {
     typename Vec8<T>::type v = {};
-    if (r < hi && c < a.out) {
+    if (!EDGE) {
+        v = *(const typename Vec8<T>::type*)((const T*)a.grad + min(r, hi - 1) * a.grad_stride + c);
+#pragma unroll
+        for (int i = 0; i < 8; i++) v[i] = r < hi ? v[i] : (T)0.f;
+    } else if (r < hi && c < a.out) {
         const T* p = (const T*)a.grad + r * a.grad_stride + c;
         if (c + 8 <= a.out) {
             v = *(const typename Vec8<T>::type*)p;
@@ -143,92 +161,135 @@ __device__ __forceinline__ E8 fragment(const char* tile, int k0, int c0, int lan
     return __builtin_bit_cast(E8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
 }
 
-template <class T, int F>
-__global__ __launch_bounds__(BLOCK, F == 4 ? 1 : 2) void k_weight(Job job) {
+// What a workgroup of k_weight works on.
+struct Tile {
+    int64_t i0, j0, lo, hi;
+    int steps;
+    bool sums;
+};
+
+// The tile's products, and with `sums` the gradient's column sums of the
+// columns that the thread loads. EDGE: the tile reaches past the weights'.
+template <class T, int F, bool EDGE>
+__device__ __forceinline__ void products(const wc_ckpt_weight_args& a, const Tile& tile, char* lds, f32x16 (&acc)[F][F],
+                                         float (&bias)[8]) {
     typedef typename Operand<T>::type E;
     typedef E E8 __attribute__((ext_vector_type(8)));
     typedef Shape<F> S;
-    constexpr int PARTS = Operand<T>::PARTS, TILE = S::TILE, PITCH = S::PITCH;
-    constexpr int SIDE = DEPTH * PITCH;
-    __shared__ __align__(16) char lds[4 * SIDE];  // two buffers of an A tile and a B tile
-    const wc_ckpt_weight_args& a = job.a;
+    constexpr int PARTS = Operand<T>::PARTS, TILE = S::TILE, PITCH = S::PITCH, SIDE = DEPTH * PITCH;
     const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
-    // Workgroups go round the eight XCDs; consecutive tiles of a run, which share
-    // rows of both operands, go to one XCD's cache.
-    const int total = job.tiles_i * job.tiles_j * job.runs, per = total / 8;
-    const int id = blockIdx.x < (unsigned)per * 8 ? (blockIdx.x % 8) * per + blockIdx.x / 8 : blockIdx.x;
-    const int run = id / (job.tiles_i * job.tiles_j), tile = id - run * (job.tiles_i * job.tiles_j);
-    const int ti = tile % job.tiles_i, tj = tile / job.tiles_i;
-    const int64_t i0 = int64_t(ti) * TILE, j0 = int64_t(tj) * TILE;
-    const int64_t lo = run * job.run, hi = min(lo + job.run, a.rows);
-    const int steps = (int)((max<int64_t>(hi - lo, 0) + DEPTH - 1) / DEPTH), all = steps * PARTS;
     const int ac = (t % (TILE / 16)) * 16, ar = t / (TILE / 16);
     const int bc = (t % (TILE / 8)) * 8, br = t / (TILE / 8);
     constexpr int AR = BLOCK / (TILE / 16), BR = BLOCK / (TILE / 8);
-    const bool sums = a.bias && ti == 0;
+    const int64_t i0 = tile.i0, j0 = tile.j0, lo = tile.lo, hi = tile.hi;
+    const int steps = tile.steps, all = steps * PARTS;
+    const bool sums = tile.sums;
 
-    Kept ka[S::A_CHUNKS];
-    typename Vec8<T>::type kb[S::B_CHUNKS];
-    float bias[8] = {};
-    auto load = [&](int s) {
-        const int64_t r0 = lo + int64_t(PARTS == 1 ? s : s % steps) * DEPTH;
+    // Loads of the next AHEAD steps wait in registers: a step is shorter than a load takes.
+    constexpr int AHEAD = sizeof(T) == 2 ? 3 : 1;
+    struct Loads {
+        Kept a[S::A_CHUNKS];
+        typename Vec8<T>::type g[S::B_CHUNKS];
+    } held_back[AHEAD];
+    auto load = [&](Loads& l, int s) {
+        const int64_t r0 = s < all ? lo + int64_t(PARTS == 1 ? s : s % steps) * DEPTH : hi;  // past the end: zeros
 #pragma unroll
-        for (int m = 0; m < S::A_CHUNKS; m++) ka[m] = load_kept(a, r0 + ar + m * AR, hi, i0 + ac);
+        for (int m = 0; m < S::A_CHUNKS; m++) l.a[m] = load_kept<EDGE>(a, r0 + ar + m * AR, hi, i0 + ac);
 #pragma unroll
-        for (int m = 0; m < S::B_CHUNKS; m++) kb[m] = load_grad<T>(a, r0 + br + m * BR, hi, j0 + bc);
+        for (int m = 0; m < S::B_CHUNKS; m++) l.g[m] = load_grad<EDGE, T>(a, r0 + br + m * BR, hi, j0 + bc);
     };
-    auto put = [&](int s) {
+    auto put = [&](const Loads& l, int s) {
         char* to = lds + (s & 1) * 2 * SIDE;
         const int plane = PARTS == 1 ? 0 : s / steps;
 #pragma unroll
-        for (int m = 0; m < S::A_CHUNKS; m++) put_kept<E>(ka[m], a.act, to + (ar + m * AR) * PITCH + 2 * ac);
+        for (int m = 0; m < S::A_CHUNKS; m++) {
+            E8* p = (E8*)(to + (ar + m * AR) * PITCH + 2 * ac);
+            p[0] = expand<E>(l.a[m], a.act, 0);
+            p[1] = expand<E>(l.a[m], a.act, 1);
+        }
 #pragma unroll
         for (int m = 0; m < S::B_CHUNKS; m++) {
             E8 o;
+            if constexpr (PARTS == 1) {
+                o = l.g[m];
+                if (sums) {
 #pragma unroll
-            for (int i = 0; i < 8; i++) {
-                float v = (float)kb[m][i];
-                if (sums && plane == 0) bias[i] += v;
-                if (PARTS > 1) {
+                    for (int i = 0; i < 8; i++) bias[i] += (float)o[i];
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < 8; i++) {
+                    float v = l.g[m][i];
+                    if (sums && plane == 0) bias[i] += v;
                     if (plane > 0) v -= (float)(E)v;
                     if (plane > 1) v -= (float)(E)v;
                     o[i] = (E)v;
-                } else {
-                    o[i] = (E)kb[m][i];
                 }
             }
             *(E8*)(to + SIDE + (br + m * BR) * PITCH + 2 * bc) = o;
         }
     };
 
-    f32x16 acc[F][F] = {};
-    if (all > 0) {
-        load(0);
-        put(0);
-        if (all > 1) load(1);
-    }
-    __syncthreads();
     const int wi = (wave >> 1) * 32 * F, wj = (wave & 1) * 32 * F;
-    for (int s = 0; s < all; s++) {
-        const char* from = lds + (s & 1) * 2 * SIDE;
-        if (s + 1 < all) {
-            put(s + 1);
-            if (s + 2 < all) load(s + 2);
+    load(held_back[0], 0);
+    put(held_back[0], 0);
+#pragma unroll
+    for (int k = 0; k < AHEAD; k++) load(held_back[k], 1 + k);
+    __syncthreads();
+    for (int s0 = 0; s0 < all; s0 += AHEAD) {
+#pragma unroll
+        for (int u = 0; u < AHEAD; u++) {
+            const int s = s0 + u;
+            if (s >= all) break;
+            const char* from = lds + (s & 1) * 2 * SIDE;
+            put(held_back[u], s + 1);  // past the end: zeros, never read
+            load(held_back[u], s + 1 + AHEAD);
+#pragma unroll
+            for (int k0 = 0; k0 < DEPTH; k0 += 16) {
+                E8 fa[F], fb[F];
+#pragma unroll
+                for (int m = 0; m < F; m++) fa[m] = fragment<E8, PITCH>(from, k0, wi + 32 * m, lane);
+#pragma unroll
+                for (int n = 0; n < F; n++) fb[n] = fragment<E8, PITCH>(from + SIDE, k0, wj + 32 * n, lane);
+#pragma unroll
+                for (int m = 0; m < F; m++)
+#pragma unroll
+                    for (int n = 0; n < F; n++) acc[m][n] = mfma(fa[m], fb[n], acc[m][n]);
+            }
+            __syncthreads();
         }
-#pragma unroll
-        for (int k0 = 0; k0 < DEPTH; k0 += 16) {
-            E8 fa[F], fb[F];
-#pragma unroll
-            for (int m = 0; m < F; m++) fa[m] = fragment<E8, PITCH>(from, k0, wi + 32 * m, lane);
-#pragma unroll
-            for (int n = 0; n < F; n++) fb[n] = fragment<E8, PITCH>(from + SIDE, k0, wj + 32 * n, lane);
-#pragma unroll
-            for (int m = 0; m < F; m++)
-#pragma unroll
-                for (int n = 0; n < F; n++) acc[m][n] = mfma(fa[m], fb[n], acc[m][n]);
-        }
-        __syncthreads();
     }
+}
+
+template <class T, int F>
+__global__ __launch_bounds__(BLOCK, 2) void k_weight(Job job) {
+    typedef Shape<F> S;
+    constexpr int TILE = S::TILE;
+    __shared__ __align__(16) char lds[4 * DEPTH * S::PITCH];  // two buffers of a tile of each operand
+    const wc_ckpt_weight_args& a = job.a;
+    const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
+    // Workgroups go round the eight XCDs; consecutive tiles of a run, which share
+    // rows of both operands, go to one XCD's cache.
+    const int total = job.tiles_i * job.tiles_j * job.runs, per = total / 8;
+    const int id = blockIdx.x < (unsigned)per * 8 ? (blockIdx.x % 8) * per + blockIdx.x / 8 : blockIdx.x;
+    const int run = id / (job.tiles_i * job.tiles_j), at = id - run * (job.tiles_i * job.tiles_j);
+    Tile tile;
+    tile.i0 = int64_t(at % job.tiles_i) * TILE;
+    tile.j0 = int64_t(at / job.tiles_i) * TILE;
+    tile.lo = run * job.run;
+    tile.hi = min(tile.lo + job.run, a.rows);
+    tile.steps = (int)((max<int64_t>(tile.hi - tile.lo, 0) + DEPTH - 1) / DEPTH);
+    tile.sums = a.bias && tile.i0 == 0;
+    f32x16 acc[F][F] = {};
+    float bias[8] = {};
+    if (tile.steps) {
+        if (tile.i0 + TILE <= a.width && tile.j0 + TILE <= a.out) products<T, F, false>(a, tile, lds, acc, bias);
+        else products<T, F, true>(a, tile, lds, acc, bias);
+    }
+    const int wi = (wave >> 1) * 32 * F, wj = (wave & 1) * 32 * F, bc = (t % (TILE / 8)) * 8, br = t / (TILE / 8);
+    const int64_t i0 = tile.i0, j0 = tile.j0;
+    const bool sums = tile.sums;
+    constexpr int BR = BLOCK / (TILE / 8);
 
     const bool last = job.runs == 1;
     float* part = job.part + int64_t(run) * a.width * a.out;
@@ -477,11 +538,10 @@ __global__ __launch_bounds__(BLOCK) void k_expand(wc_ckpt_weight_args a, E* to, 
     const int64_t total = a.rows * per_row;
     for (int64_t i = int64_t(blockIdx.x) * BLOCK + threadIdx.x; i < total; i += int64_t(gridDim.x) * BLOCK) {
         const int64_t r = i / per_row, c = (i - r * per_row) * 16;
-        __align__(16) char out[32];
-        put_kept<E>(load_kept(a, r, a.rows, c), a.act, out);
+        const Kept k = load_kept<true>(a, r, a.rows, c);
         E8* p = (E8*)(to + r * pitch + c);
-        p[0] = ((const E8*)out)[0];
-        p[1] = ((const E8*)out)[1];
+        p[0] = expand<E>(k, a.act, 0);
+        p[1] = expand<E>(k, a.act, 1);
     }
 }
 
@@ -491,7 +551,7 @@ __global__ __launch_bounds__(BLOCK) void k_align(wc_ckpt_weight_args a, T* to, i
     const int64_t total = a.rows * per_row;
     for (int64_t i = int64_t(blockIdx.x) * BLOCK + threadIdx.x; i < total; i += int64_t(gridDim.x) * BLOCK) {
         const int64_t r = i / per_row, c = (i - r * per_row) * 8;
-        *(typename Vec8<T>::type*)(to + r * pitch + c) = load_grad<T>(a, r, a.rows, c);
+        *(typename Vec8<T>::type*)(to + r * pitch + c) = load_grad<true, T>(a, r, a.rows, c);
     }
 }
 
