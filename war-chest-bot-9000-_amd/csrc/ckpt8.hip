@@ -58,8 +58,7 @@ __global__ __launch_bounds__(BLOCK) void k_ckpt_write(wc_ckpt_args a, int64_t pe
             }
             if ((p.col & 31) == 0) a.exps[p.row * a.exps_stride + (p.col >> 5)] = lost ? 255 : (uint8_t)e;
             if (a.y) {
-#pragma unroll
-                for (int k = 0; k < 8; k++) v[k] = act_value(v[k], a.act);
+                act_values(v, a.act);
                 store_n((T*)a.y + p.row * a.y_stride + p.col, p.n, v);
             }
         }
@@ -92,8 +91,13 @@ __global__ __launch_bounds__(BLOCK) void k_ckpt_read(wc_ckpt_args a, int64_t per
 #pragma unroll
             for (int k = 0; k < 8; k++) v[k] = held<T>(v[k]);
         }
+        if (BACK) {
+            act_slopes(v, a.act);
 #pragma unroll
-        for (int k = 0; k < 8; k++) v[k] = BACK ? g[k] * act_slope(v[k], a.act) : act_value(v[k], a.act);
+            for (int k = 0; k < 8; k++) v[k] *= g[k];
+        } else {
+            act_values(v, a.act);
+        }
         store_n((T*)a.y + p.row * a.y_stride + p.col, p.n, v);
     }
 }

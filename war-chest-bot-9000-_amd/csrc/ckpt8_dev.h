@@ -57,5 +57,35 @@ __device__ __forceinline__ float act_slope(float x, int act) {
     return x != x ? x : 1.f;
 }
 
+// Eight at a time: the choice once, not for each.
+__device__ __forceinline__ void act_values(float (&v)[8], int act) {
+    if (act == WC_ACT_NONE) return;
+    if (act == WC_ACT_RELU) {
+#pragma unroll
+        for (int i = 0; i < 8; i++) v[i] = act_value(v[i], WC_ACT_RELU);
+    } else if (act == WC_ACT_GELU) {
+#pragma unroll
+        for (int i = 0; i < 8; i++) v[i] = act_value(v[i], WC_ACT_GELU);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; i++) v[i] = act_value(v[i], WC_ACT_SILU);
+    }
+}
+__device__ __forceinline__ void act_slopes(float (&v)[8], int act) {
+    if (act == WC_ACT_NONE) {
+#pragma unroll
+        for (int i = 0; i < 8; i++) v[i] = act_slope(v[i], WC_ACT_NONE);
+    } else if (act == WC_ACT_RELU) {
+#pragma unroll
+        for (int i = 0; i < 8; i++) v[i] = act_slope(v[i], WC_ACT_RELU);
+    } else if (act == WC_ACT_GELU) {
+#pragma unroll
+        for (int i = 0; i < 8; i++) v[i] = act_slope(v[i], WC_ACT_GELU);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; i++) v[i] = act_slope(v[i], WC_ACT_SILU);
+    }
+}
+
 }  // namespace learn
 }  // namespace wc

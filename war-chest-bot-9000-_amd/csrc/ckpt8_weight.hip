@@ -11,6 +11,7 @@
 // the device the rows are cut into runs, whose partial products are added in
 // order.
 #include <algorithm>
+#include <type_traits>
 
 #include "ckpt8_dev.h"
 
@@ -52,10 +53,10 @@ struct Operand<float> {
 template <int F>
 struct Shape {
     static constexpr int TILE = 64 * F;
-    // bytes from one row of a tile to the next: four consecutive rows, which one
-    // transposing read takes 32 bytes of each, start 64 bytes apart modulo 256,
-    // all the banks
-    static constexpr int PITCH = 2 * TILE + 64;
+    // Bytes from one row of a tile to the next. A transposing read takes 64 bytes
+    // of four consecutive rows: row r's 64-byte units are exchanged by r modulo 4,
+    // so that they lie in different banks.
+    static constexpr int PITCH = 2 * TILE;
     static constexpr int A_CHUNKS = DEPTH * TILE / 16 / BLOCK;  // 16 kept values each
     static constexpr int B_CHUNKS = DEPTH * TILE / 8 / BLOCK;   // 8 gradient values each
 };
@@ -68,26 +69,16 @@ struct Job {
     float* bias_part;   // runs x out, likewise
 };
 
-// Sixteen kept values of one row, from column c.
+// Sixteen kept values of one row.
 struct Kept {
     uint32_t q[4], e;
 };
 
-// Zeros beyond the run and, with EDGE, beyond the row. Without it the load is
-// unconditional, from the run's last row where there is none: what the
-// compiler cannot count it would wait for at once.
-template <bool EDGE>
+// From column c; zeros beyond the rows and the row.
 __device__ __forceinline__ Kept load_kept(const wc_ckpt_weight_args& a, int64_t r, int64_t hi, int64_t c) {
     typedef uint32_t Words __attribute__((ext_vector_type(4), aligned(1)));
     Kept k = {{0, 0, 0, 0}, 1};
-    if (!EDGE) {
-        const int64_t at = min(r, hi - 1);
-        const Words w = *(const Words*)(a.q + at * a.q_stride + c);
-        const uint32_t e = a.exps[at * a.exps_stride + (c >> 5)];
-#pragma unroll
-        for (int i = 0; i < 4; i++) k.q[i] = r < hi ? w[i] : 0u;
-        k.e = r < hi ? e : 1u;
-    } else if (r < hi && c < a.width) {
+    if (r < hi && c < a.width) {
         const int8_t* p = a.q + r * a.q_stride + c;
         k.e = a.exps[r * a.exps_stride + (c >> 5)];
         if (c + 16 <= a.width) {
@@ -103,13 +94,20 @@ __device__ __forceinline__ Kept load_kept(const wc_ckpt_weight_args& a, int64_t 
     return k;
 }
 
+// All of them there.
+__device__ __forceinline__ Kept load_kept(const int8_t* q, const uint8_t* e) {
+    typedef uint32_t Words __attribute__((ext_vector_type(4), aligned(1)));
+    const Words w = *(const Words*)q;
+    return {{w[0], w[1], w[2], w[3]}, *e};
+}
+
 // Eight of them, in 16 bits.
 template <class E>
 struct Eight {
     typedef E type __attribute__((ext_vector_type(8)));
 };
 template <class E>
-__device__ __forceinline__ typename Eight<E>::type expand(const Kept& k, int act, int half) {
+__device__ __forceinline__ typename Eight<E>::type expand(const Kept& k, const int act, int half) {
     const float step = step_of(k.e);
     float v[8];
 #pragma unroll
@@ -118,26 +116,19 @@ __device__ __forceinline__ typename Eight<E>::type expand(const Kept& k, int act
 #pragma unroll
         for (int i = 0; i < 8; i++) v[i] = held<E>(v[i]);
     }
-    if (act != WC_ACT_NONE) {
-#pragma unroll
-        for (int i = 0; i < 8; i++) v[i] = act_value(v[i], act);
-    }
+    act_values(v, act);
     typename Eight<E>::type o;
 #pragma unroll
     for (int i = 0; i < 8; i++) o[i] = (E)v[i];
     return o;
 }
 
-// Eight gradient values of one row, from column c, alike.
-template <bool EDGE, class T>
+// Eight gradient values of one row, from column c; zeros beyond the rows and the row.
+template <class T>
 __device__ __forceinline__ typename Vec8<T>::type load_grad(const wc_ckpt_weight_args& a, int64_t r, int64_t hi,
                                                             int64_t c) {
     typename Vec8<T>::type v = {};
-    if (!EDGE) {
-        v = *(const typename Vec8<T>::type*)((const T*)a.grad + min(r, hi - 1) * a.grad_stride + c);
-#pragma unroll
-        for (int i = 0; i < 8; i++) v[i] = r < hi ? v[i] : (T)0.f;
-    } else if (r < hi && c < a.out) {
+    if (r < hi && c < a.out) {
         const T* p = (const T*)a.grad + r * a.grad_stride + c;
         if (c + 8 <= a.out) {
             v = *(const typename Vec8<T>::type*)p;
@@ -155,7 +146,8 @@ __device__ __forceinline__ typename Vec8<T>::type load_grad(const wc_ckpt_weight
 template <class E8, int PITCH>
 __device__ __forceinline__ E8 fragment(const char* tile, int k0, int c0, int lane) {
     typedef __attribute__((address_space(3))) s16x4* Lds;
-    const char* p = tile + (k0 + 8 * (lane >> 5) + ((lane & 15) >> 2)) * PITCH + 2 * (c0 + (lane & 16) + 4 * (lane & 3));
+    const int row = (lane & 15) >> 2;
+    const char* p = tile + (k0 + 8 * (lane >> 5) + row) * PITCH + ((2 * (c0 + (lane & 16) + 4 * (lane & 3))) ^ (row << 6));
     const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Lds)p);
     const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Lds)(p + 4 * PITCH));
     return __builtin_bit_cast(E8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
@@ -170,7 +162,7 @@ struct Tile {
 
 // The tile's products, and with `sums` the gradient's column sums of the
 // columns that the thread loads. EDGE: the tile reaches past the weights'.
-template <class T, int F, bool EDGE>
+template <class T, int F, int ACT, bool EDGE>
 __device__ __forceinline__ void products(const wc_ckpt_weight_args& a, const Tile& tile, char* lds, f32x16 (&acc)[F][F],
                                          float (&bias)[8]) {
     typedef typename Operand<T>::type E;
@@ -181,6 +173,7 @@ __device__ __forceinline__ void products(const wc_ckpt_weight_args& a, const Til
     const int ac = (t % (TILE / 16)) * 16, ar = t / (TILE / 16);
     const int bc = (t % (TILE / 8)) * 8, br = t / (TILE / 8);
     constexpr int AR = BLOCK / (TILE / 16), BR = BLOCK / (TILE / 8);
+    static_assert(AR % 4 == 0 && BR % 4 == 0, "a thread's rows have one place modulo 4");
     const int64_t i0 = tile.i0, j0 = tile.j0, lo = tile.lo, hi = tile.hi;
     const int steps = tile.steps, all = steps * PARTS;
     const bool sums = tile.sums;
@@ -191,21 +184,35 @@ __device__ __forceinline__ void products(const wc_ckpt_weight_args& a, const Til
         Kept a[S::A_CHUNKS];
         typename Vec8<T>::type g[S::B_CHUNKS];
     } held_back[AHEAD];
-    auto load = [&](Loads& l, int s) {
-        const int64_t r0 = s < all ? lo + int64_t(PARTS == 1 ? s : s % steps) * DEPTH : hi;  // past the end: zeros
+    // Whole steps of whole tiles need no checks: from the thread's first row a
+    // step, and a chunk, is as far for every lane.
+    const int8_t* q0 = a.q + (lo + ar) * a.q_stride + i0 + ac;
+    const uint8_t* e0 = a.exps + (lo + ar) * a.exps_stride + ((i0 + ac) >> 5);
+    const T* g0 = (const T*)a.grad + (lo + br) * a.grad_stride + j0 + bc;
+    auto load = [&](Loads& l, int s, auto checked) {
+        const int64_t r0 = s < all ? int64_t(PARTS == 1 ? s : s % steps) * DEPTH : hi - lo;  // past the end: zeros
+        if constexpr (!decltype(checked)::value) {
 #pragma unroll
-        for (int m = 0; m < S::A_CHUNKS; m++) l.a[m] = load_kept<EDGE>(a, r0 + ar + m * AR, hi, i0 + ac);
+            for (int m = 0; m < S::A_CHUNKS; m++)
+                l.a[m] = load_kept(q0 + (r0 + m * AR) * a.q_stride, e0 + (r0 + m * AR) * a.exps_stride);
 #pragma unroll
-        for (int m = 0; m < S::B_CHUNKS; m++) l.g[m] = load_grad<EDGE, T>(a, r0 + br + m * BR, hi, j0 + bc);
+            for (int m = 0; m < S::B_CHUNKS; m++)
+                l.g[m] = *(const typename Vec8<T>::type*)(g0 + (r0 + m * BR) * a.grad_stride);
+        } else {
+#pragma unroll
+            for (int m = 0; m < S::A_CHUNKS; m++) l.a[m] = load_kept(a, lo + r0 + ar + m * AR, hi, i0 + ac);
+#pragma unroll
+            for (int m = 0; m < S::B_CHUNKS; m++) l.g[m] = load_grad<T>(a, lo + r0 + br + m * BR, hi, j0 + bc);
+        }
     };
     auto put = [&](const Loads& l, int s) {
         char* to = lds + (s & 1) * 2 * SIDE;
         const int plane = PARTS == 1 ? 0 : s / steps;
 #pragma unroll
         for (int m = 0; m < S::A_CHUNKS; m++) {
-            E8* p = (E8*)(to + (ar + m * AR) * PITCH + 2 * ac);
-            p[0] = expand<E>(l.a[m], a.act, 0);
-            p[1] = expand<E>(l.a[m], a.act, 1);
+            E8* p = (E8*)(to + (ar + m * AR) * PITCH + ((2 * ac) ^ ((ar & 3) << 6)));
+            p[0] = expand<E>(l.a[m], ACT, 0);
+            p[1] = expand<E>(l.a[m], ACT, 1);
         }
 #pragma unroll
         for (int m = 0; m < S::B_CHUNKS; m++) {
@@ -226,42 +233,52 @@ __device__ __forceinline__ void products(const wc_ckpt_weight_args& a, const Til
                     o[i] = (E)v;
                 }
             }
-            *(E8*)(to + SIDE + (br + m * BR) * PITCH + 2 * bc) = o;
+            *(E8*)(to + SIDE + (br + m * BR) * PITCH + ((2 * bc) ^ ((br & 3) << 6))) = o;
         }
     };
 
     const int wi = (wave >> 1) * 32 * F, wj = (wave & 1) * 32 * F;
-    load(held_back[0], 0);
+    const std::true_type checked;
+    const std::false_type unchecked;
+    load(held_back[0], 0, checked);
     put(held_back[0], 0);
 #pragma unroll
-    for (int k = 0; k < AHEAD; k++) load(held_back[k], 1 + k);
+    for (int k = 0; k < AHEAD; k++) load(held_back[k], 1 + k, checked);
     __syncthreads();
-    for (int s0 = 0; s0 < all; s0 += AHEAD) {
+    auto step = [&](Loads& l, int s, auto check) {
+        const char* from = lds + (s & 1) * 2 * SIDE;
+        put(l, s + 1);  // past the end: zeros, never read
+        load(l, s + 1 + AHEAD, check);
+#pragma unroll
+        for (int k0 = 0; k0 < DEPTH; k0 += 16) {
+            E8 fa[F], fb[F];
+#pragma unroll
+            for (int m = 0; m < F; m++) fa[m] = fragment<E8, PITCH>(from, k0, wi + 32 * m, lane);
+#pragma unroll
+            for (int n = 0; n < F; n++) fb[n] = fragment<E8, PITCH>(from + SIDE, k0, wj + 32 * n, lane);
+#pragma unroll
+            for (int m = 0; m < F; m++)
+#pragma unroll
+                for (int n = 0; n < F; n++) acc[m][n] = mfma(fa[m], fb[n], acc[m][n]);
+        }
+        __syncthreads();
+    };
+    // The steps whose loads are whole ones go in a loop of their own: loads that
+    // the compiler cannot count it would wait for at once.
+    const int whole = EDGE ? 0 : (int)((hi - lo) / DEPTH), fast = whole == steps ? all : PARTS == 1 ? whole : 0;
+    int s0 = 0;
+    for (; s0 + 2 * AHEAD < fast; s0 += AHEAD)
+#pragma unroll
+        for (int u = 0; u < AHEAD; u++) step(held_back[u], s0 + u, unchecked);
+    for (; s0 < all; s0 += AHEAD)
 #pragma unroll
         for (int u = 0; u < AHEAD; u++) {
-            const int s = s0 + u;
-            if (s >= all) break;
-            const char* from = lds + (s & 1) * 2 * SIDE;
-            put(held_back[u], s + 1);  // past the end: zeros, never read
-            load(held_back[u], s + 1 + AHEAD);
-#pragma unroll
-            for (int k0 = 0; k0 < DEPTH; k0 += 16) {
-                E8 fa[F], fb[F];
-#pragma unroll
-                for (int m = 0; m < F; m++) fa[m] = fragment<E8, PITCH>(from, k0, wi + 32 * m, lane);
-#pragma unroll
-                for (int n = 0; n < F; n++) fb[n] = fragment<E8, PITCH>(from + SIDE, k0, wj + 32 * n, lane);
-#pragma unroll
-                for (int m = 0; m < F; m++)
-#pragma unroll
-                    for (int n = 0; n < F; n++) acc[m][n] = mfma(fa[m], fb[n], acc[m][n]);
-            }
-            __syncthreads();
+            if (s0 + u >= all) break;
+            step(held_back[u], s0 + u, checked);
         }
-    }
 }
 
-template <class T, int F>
+template <class T, int F, int ACT>
 __global__ __launch_bounds__(BLOCK, 2) void k_weight(Job job) {
     typedef Shape<F> S;
     constexpr int TILE = S::TILE;
@@ -283,8 +300,8 @@ __global__ __launch_bounds__(BLOCK, 2) void k_weight(Job job) {
     f32x16 acc[F][F] = {};
     float bias[8] = {};
     if (tile.steps) {
-        if (tile.i0 + TILE <= a.width && tile.j0 + TILE <= a.out) products<T, F, false>(a, tile, lds, acc, bias);
-        else products<T, F, true>(a, tile, lds, acc, bias);
+        if (tile.i0 + TILE <= a.width && tile.j0 + TILE <= a.out) products<T, F, ACT, false>(a, tile, lds, acc, bias);
+        else products<T, F, ACT, true>(a, tile, lds, acc, bias);
     }
     const int wi = (wave >> 1) * 32 * F, wj = (wave & 1) * 32 * F, bc = (t % (TILE / 8)) * 8, br = t / (TILE / 8);
     const int64_t i0 = tile.i0, j0 = tile.j0;
@@ -538,7 +555,7 @@ __global__ __launch_bounds__(BLOCK) void k_expand(wc_ckpt_weight_args a, E* to, 
     const int64_t total = a.rows * per_row;
     for (int64_t i = int64_t(blockIdx.x) * BLOCK + threadIdx.x; i < total; i += int64_t(gridDim.x) * BLOCK) {
         const int64_t r = i / per_row, c = (i - r * per_row) * 16;
-        const Kept k = load_kept<true>(a, r, a.rows, c);
+        const Kept k = load_kept(a, r, a.rows, c);
         E8* p = (E8*)(to + r * pitch + c);
         p[0] = expand<E>(k, a.act, 0);
         p[1] = expand<E>(k, a.act, 1);
@@ -551,36 +568,45 @@ __global__ __launch_bounds__(BLOCK) void k_align(wc_ckpt_weight_args a, T* to, i
     const int64_t total = a.rows * per_row;
     for (int64_t i = int64_t(blockIdx.x) * BLOCK + threadIdx.x; i < total; i += int64_t(gridDim.x) * BLOCK) {
         const int64_t r = i / per_row, c = (i - r * per_row) * 8;
-        *(typename Vec8<T>::type*)(to + r * pitch + c) = load_grad<true, T>(a, r, a.rows, c);
+        *(typename Vec8<T>::type*)(to + r * pitch + c) = load_grad<T>(a, r, a.rows, c);
     }
 }
 
-// The runs' partial products, added in order; the workgroups past the weights'
-// add the bias's.
-template <class W>
+// The runs' partial products added, in an order that does not change: N
+// elements a thread, a quarter of the runs each wavefront. The workgroups past
+// the weights' add the bias's.
+template <class W, int N>
 __global__ __launch_bounds__(BLOCK) void k_weight_sum(Job job, int64_t weight_blocks) {
+    typedef float Some __attribute__((ext_vector_type(N)));
+    __shared__ Some quarters[BLOCK / 64][64];
     const wc_ckpt_weight_args& a = job.a;
-    if (blockIdx.x >= weight_blocks) {
-        const int64_t j = (int64_t(blockIdx.x) - weight_blocks) * BLOCK + threadIdx.x;
-        if (j >= a.out) return;
-        float s = 0.f;
-        for (int k = 0; k < job.runs; k++) s += job.bias_part[int64_t(k) * a.out + j];
-        a.bias[j] = s;
-        return;
-    }
-    const int64_t i = int64_t(blockIdx.x) * BLOCK + threadIdx.x, n = a.width * a.out;
-    if (i >= n) return;
-    float s = 0.f;
-    int k = 0;
-    for (; k + 8 <= job.runs; k += 8) {
-        float v[8];
+    const bool bias = blockIdx.x >= weight_blocks;
+    const int quarter = threadIdx.x >> 6, lane = threadIdx.x & 63;
+    const int64_t n = bias ? a.out : a.width * a.out, block = blockIdx.x - (bias ? weight_blocks : 0);
+    const int64_t i = (block * 64 + lane) * N;
+    const float* part = (bias ? job.bias_part : job.part) + i;
+    Some s = {};
+    if (i < n) {
+        int k = quarter;
+        for (; k + 28 < job.runs; k += 32) {
+            Some v[8];
 #pragma unroll
-        for (int u = 0; u < 8; u++) v[u] = job.part[(k + u) * n + i];
+            for (int u = 0; u < 8; u++) v[u] = *(const Some*)(part + (k + 4 * u) * n);
 #pragma unroll
-        for (int u = 0; u < 8; u++) s += v[u];
+            for (int u = 0; u < 8; u++) s += v[u];
+        }
+        for (; k < job.runs; k += 4) s += *(const Some*)(part + k * n);
     }
-    for (; k < job.runs; k++) s += job.part[k * n + i];
-    ((W*)a.weight)[i / a.out * a.weight_stride + i % a.out] = (W)s;
+    quarters[quarter][lane] = s;
+    __syncthreads();
+    if (quarter || i >= n) return;
+    s = (s + quarters[1][lane]) + (quarters[2][lane] + quarters[3][lane]);
+#pragma unroll
+    for (int u = 0; u < N; u++) {
+        const float v = s[u];
+        if (bias) a.bias[i + u] = v;
+        else ((W*)a.weight)[(i + u) / a.out * a.weight_stride + (i + u) % a.out] = (W)v;
+    }
 }
 
 // Which kernel, its tiles and runs, and where its scratch lies.
@@ -667,12 +693,25 @@ void weight(const wc_ckpt_weight_args& a, int cus, hipStream_t s) {
             else k_weight_big<T, T><<<grid, BLOCK, 0, s>>>(big);
         }
     }
-    if (!p.big) k_weight<T, 2><<<grid, BLOCK, 0, s>>>(job);
+    if (!p.big) {
+        if (a.act == WC_ACT_NONE) k_weight<T, 2, WC_ACT_NONE><<<grid, BLOCK, 0, s>>>(job);
+        else if (a.act == WC_ACT_RELU) k_weight<T, 2, WC_ACT_RELU><<<grid, BLOCK, 0, s>>>(job);
+        if constexpr (sizeof(T) == 2) {
+            if (a.act == WC_ACT_GELU) k_weight<T, 2, WC_ACT_GELU><<<grid, BLOCK, 0, s>>>(job);
+            else if (a.act == WC_ACT_SILU) k_weight<T, 2, WC_ACT_SILU><<<grid, BLOCK, 0, s>>>(job);
+        }
+    }
     if (p.runs > 1) {
-        const int64_t blocks = (a.width * a.out + BLOCK - 1) / BLOCK;
-        const dim3 g((uint32_t)(blocks + (a.bias ? (a.out + BLOCK - 1) / BLOCK : 0)));
-        if (a.weight_dtype == WC_DTYPE_F32) k_weight_sum<float><<<g, BLOCK, 0, s>>>(job, blocks);
-        else k_weight_sum<T><<<g, BLOCK, 0, s>>>(job, blocks);
+        // 16-byte reads where every run's part starts on 16 bytes
+        const int64_t n = a.out % 4 == 0 ? 4 : 1, blocks = (a.width * a.out + 64 * n - 1) / (64 * n);
+        const dim3 g((uint32_t)(blocks + (a.bias ? (a.out + 64 * n - 1) / (64 * n) : 0)));
+        if (a.weight_dtype == WC_DTYPE_F32) {
+            if (n == 4) k_weight_sum<float, 4><<<g, BLOCK, 0, s>>>(job, blocks);
+            else k_weight_sum<float, 1><<<g, BLOCK, 0, s>>>(job, blocks);
+        } else {
+            if (n == 4) k_weight_sum<T, 4><<<g, BLOCK, 0, s>>>(job, blocks);
+            else k_weight_sum<T, 1><<<g, BLOCK, 0, s>>>(job, blocks);
+        }
     }
 }
 
