@@ -11,7 +11,6 @@
 // the device the rows are cut into runs, whose partial products are added in
 // order.
 #include <algorithm>
-#include <type_traits>
 
 #include "ckpt8_dev.h"
 
@@ -33,6 +32,22 @@ __device__ __forceinline__ f32x16 mfma(f16x8 a, f16x8 b, f32x16 c) {
 }
 __device__ __forceinline__ f32x16 mfma(bf16x8 a, bf16x8 b, f32x16 c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+}
+
+// A lane's eight rows of a column added to s.
+__device__ __forceinline__ float plus(bf16x8 v, float s) {
+    typedef bf16 bf16x2 __attribute__((ext_vector_type(2)));
+    const bf16x2 one = {(bf16)1.f, (bf16)1.f};
+#pragma unroll
+    for (int i = 0; i < 8; i += 2) s = __builtin_amdgcn_fdot2_f32_bf16(bf16x2{v[i], v[i + 1]}, one, s, false);
+    return s;
+}
+__device__ __forceinline__ float plus(f16x8 v, float s) {
+    typedef f16 f16x2 __attribute__((ext_vector_type(2)));
+    const f16x2 one = {(f16)1.f, (f16)1.f};
+#pragma unroll
+    for (int i = 0; i < 8; i += 2) s = __builtin_amdgcn_fdot2(f16x2{v[i], v[i + 1]}, one, s, false);
+    return s;
 }
 
 // The operand's type and how many parts a gradient element is taken in: a
@@ -64,6 +79,7 @@ struct Shape {
 struct Job {
     wc_ckpt_weight_args a;
     int64_t run;        // rows per run, a multiple of DEPTH
+    int64_t open;       // the rows after which there is room for loads past a row's end
     int tiles_i, tiles_j, runs;
     float* part;        // runs x width x out, where there are several runs
     float* bias_part;   // runs x out, likewise
@@ -155,127 +171,148 @@ __device__ __forceinline__ E8 fragment(const char* tile, int k0, int c0, int lan
 
 // What a workgroup of k_weight works on.
 struct Tile {
-    int64_t i0, j0, lo, hi;
-    int steps;
+    int64_t i0, j0, lo, hi, open;
     bool sums;
 };
 
-// The tile's products, and with `sums` the gradient's column sums of the
-// columns that the thread loads. EDGE: the tile reaches past the weights'.
-template <class T, int F, int ACT, bool EDGE>
+// The tile's products, and with `sums` the gradient's column sums, of half a
+// fragment's rows a lane, by the wavefronts of the tile's first half.
+//
+// All steps but the last loads unchecked: where the tile reaches past the last
+// column a lane loads columns before it, or past the row's end the next row's
+// first bytes, and the products of what is no column are not stored. The last
+// rows of all, after which nothing need follow, and a step that is not whole go
+// through checked loads at the end. (Checks in the loop would be loads that the
+// compiler cannot count, and so waits for at once; and several kilobytes of
+// code that every workgroup would fetch.)
+template <class T, int F, int ACT>
 __device__ __forceinline__ void products(const wc_ckpt_weight_args& a, const Tile& tile, char* lds, f32x16 (&acc)[F][F],
-                                         float (&bias)[8]) {
+                                         float (&bias)[F]) {
     typedef typename Operand<T>::type E;
     typedef E E8 __attribute__((ext_vector_type(8)));
     typedef Shape<F> S;
     constexpr int PARTS = Operand<T>::PARTS, TILE = S::TILE, PITCH = S::PITCH, SIDE = DEPTH * PITCH;
-    const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
-    const int ac = (t % (TILE / 16)) * 16, ar = t / (TILE / 16);
-    const int bc = (t % (TILE / 8)) * 8, br = t / (TILE / 8);
     constexpr int AR = BLOCK / (TILE / 16), BR = BLOCK / (TILE / 8);
     static_assert(AR % 4 == 0 && BR % 4 == 0, "a thread's rows have one place modulo 4");
-    const int64_t i0 = tile.i0, j0 = tile.j0, lo = tile.lo, hi = tile.hi;
-    const int steps = tile.steps, all = steps * PARTS;
-    const bool sums = tile.sums;
+    static_assert(DEPTH / 16 == S::B_CHUNKS && S::B_CHUNKS == 2 * S::A_CHUNKS, "four parts");
+    const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
+    const int ac = (t % (TILE / 16)) * 16, ar = t / (TILE / 16);
+    const int bc = (t % (TILE / 8)) * 8, br = t / (TILE / 8);
+    const int wi = (wave >> 1) * 32 * F, wj = (wave & 1) * 32 * F;
+    const int64_t lo = tile.lo, hi = tile.hi;
+    const int whole = (int)(max<int64_t>(0, min(hi, tile.open) - lo) / DEPTH), all = whole * PARTS;
 
     // Loads of the next AHEAD steps wait in registers: a step is shorter than a load takes.
     constexpr int AHEAD = sizeof(T) == 2 ? 3 : 1;
     struct Loads {
         Kept a[S::A_CHUNKS];
         typename Vec8<T>::type g[S::B_CHUNKS];
-    } held_back[AHEAD];
-    // Whole steps of whole tiles need no checks: from the thread's first row a
-    // step, and a chunk, is as far for every lane.
-    const int8_t* q0 = a.q + (lo + ar) * a.q_stride + i0 + ac;
-    const uint8_t* e0 = a.exps + (lo + ar) * a.exps_stride + ((i0 + ac) >> 5);
-    const T* g0 = (const T*)a.grad + (lo + br) * a.grad_stride + j0 + bc;
-    auto load = [&](Loads& l, int s, auto checked) {
-        const int64_t r0 = s < all ? int64_t(PARTS == 1 ? s : s % steps) * DEPTH : hi - lo;  // past the end: zeros
-        if constexpr (!decltype(checked)::value) {
-#pragma unroll
-            for (int m = 0; m < S::A_CHUNKS; m++)
-                l.a[m] = load_kept(q0 + (r0 + m * AR) * a.q_stride, e0 + (r0 + m * AR) * a.exps_stride);
-#pragma unroll
-            for (int m = 0; m < S::B_CHUNKS; m++)
-                l.g[m] = *(const typename Vec8<T>::type*)(g0 + (r0 + m * BR) * a.grad_stride);
+    } ahead[AHEAD];
+    const int64_t ca = min(tile.i0 + ac, (a.width - 1) / 16 * 16), cb = min(tile.j0 + bc, (a.out - 1) / 8 * 8);
+    const int8_t* q0 = a.q + (lo + ar) * a.q_stride + ca;
+    const uint8_t* e0 = a.exps + (lo + ar) * a.exps_stride + (ca >> 5);
+    const T* g0 = (const T*)a.grad + (lo + br) * a.grad_stride + cb;
+    auto first_row = [&](int s) {
+        s = min(s, all - 1);  // past the end the last step's again: the count of loads stays the same
+        return int64_t(PARTS == 1 ? s : s % whole) * DEPTH;
+    };
+    auto load_a = [&](Loads& l, int m, int64_t r0) {
+        l.a[m] = load_kept(q0 + (r0 + m * AR) * a.q_stride, e0 + (r0 + m * AR) * a.exps_stride);
+    };
+    auto load_g = [&](Loads& l, int m, int64_t r0) {
+        l.g[m] = *(const typename Vec8<T>::type*)(g0 + (r0 + m * BR) * a.grad_stride);
+    };
+    // A step's loads and LDS writes are in four parts, between its matrix instructions:
+    // part k has chunk k of the gradient and half a chunk of the kept values.
+    auto put = [&](const Loads& l, int k, char* to, int plane) {
+        E8* p = (E8*)(to + (ar + k / 2 * AR) * PITCH + ((2 * ac) ^ ((ar & 3) << 6)));
+        p[k % 2] = expand<E>(l.a[k / 2], ACT, k % 2);
+        E8 o;
+        if constexpr (PARTS == 1) {
+            o = l.g[k];
         } else {
 #pragma unroll
-            for (int m = 0; m < S::A_CHUNKS; m++) l.a[m] = load_kept(a, lo + r0 + ar + m * AR, hi, i0 + ac);
-#pragma unroll
-            for (int m = 0; m < S::B_CHUNKS; m++) l.g[m] = load_grad<T>(a, lo + r0 + br + m * BR, hi, j0 + bc);
-        }
-    };
-    auto put = [&](const Loads& l, int s) {
-        char* to = lds + (s & 1) * 2 * SIDE;
-        const int plane = PARTS == 1 ? 0 : s / steps;
-#pragma unroll
-        for (int m = 0; m < S::A_CHUNKS; m++) {
-            E8* p = (E8*)(to + (ar + m * AR) * PITCH + ((2 * ac) ^ ((ar & 3) << 6)));
-            p[0] = expand<E>(l.a[m], ACT, 0);
-            p[1] = expand<E>(l.a[m], ACT, 1);
-        }
-#pragma unroll
-        for (int m = 0; m < S::B_CHUNKS; m++) {
-            E8 o;
-            if constexpr (PARTS == 1) {
-                o = l.g[m];
-                if (sums) {
-#pragma unroll
-                    for (int i = 0; i < 8; i++) bias[i] += (float)o[i];
-                }
-            } else {
-#pragma unroll
-                for (int i = 0; i < 8; i++) {
-                    float v = l.g[m][i];
-                    if (sums && plane == 0) bias[i] += v;
-                    if (plane > 0) v -= (float)(E)v;
-                    if (plane > 1) v -= (float)(E)v;
-                    o[i] = (E)v;
-                }
+            for (int i = 0; i < 8; i++) {
+                float v = l.g[k][i];
+                if (plane > 0) v -= (float)(E)v;
+                if (plane > 1) v -= (float)(E)v;
+                o[i] = (E)v;
             }
-            *(E8*)(to + SIDE + (br + m * BR) * PITCH + ((2 * bc) ^ ((br & 3) << 6))) = o;
+        }
+        *(E8*)(to + SIDE + (br + k * BR) * PITCH + ((2 * bc) ^ ((br & 3) << 6))) = o;
+    };
+    E8 fa[2][F], fb[2][F];
+    auto take = [&](const char* from, int k) {
+#pragma unroll
+        for (int m = 0; m < F; m++) fa[k & 1][m] = fragment<E8, PITCH>(from, 16 * k, wi + 32 * m, lane);
+#pragma unroll
+        for (int n = 0; n < F; n++) fb[k & 1][n] = fragment<E8, PITCH>(from + SIDE, 16 * k, wj + 32 * n, lane);
+    };
+    auto multiply = [&](int k) {
+#pragma unroll
+        for (int m = 0; m < F; m++)
+#pragma unroll
+            for (int n = 0; n < F; n++) acc[m][n] = mfma(fa[k & 1][m], fb[k & 1][n], acc[m][n]);
+        if (tile.sums && wi == 0) {
+#pragma unroll
+            for (int n = 0; n < F; n++) bias[n] = plus(fb[k & 1][n], bias[n]);
         }
     };
 
-    const int wi = (wave >> 1) * 32 * F, wj = (wave & 1) * 32 * F;
-    const std::true_type checked;
-    const std::false_type unchecked;
-    load(held_back[0], 0, checked);
-    put(held_back[0], 0);
+    if (all > 0) {
+        auto load = [&](Loads& l, int s) {
+            const int64_t r0 = first_row(s);
 #pragma unroll
-    for (int k = 0; k < AHEAD; k++) load(held_back[k], 1 + k, checked);
-    __syncthreads();
-    auto step = [&](Loads& l, int s, auto check) {
-        const char* from = lds + (s & 1) * 2 * SIDE;
-        put(l, s + 1);  // past the end: zeros, never read
-        load(l, s + 1 + AHEAD, check);
+            for (int m = 0; m < S::A_CHUNKS; m++) load_a(l, m, r0);
 #pragma unroll
-        for (int k0 = 0; k0 < DEPTH; k0 += 16) {
-            E8 fa[F], fb[F];
+            for (int m = 0; m < S::B_CHUNKS; m++) load_g(l, m, r0);
+        };
+        load(ahead[0], 0);
 #pragma unroll
-            for (int m = 0; m < F; m++) fa[m] = fragment<E8, PITCH>(from, k0, wi + 32 * m, lane);
+        for (int k = 0; k < 4; k++) put(ahead[0], k, lds, 0);
 #pragma unroll
-            for (int n = 0; n < F; n++) fb[n] = fragment<E8, PITCH>(from + SIDE, k0, wj + 32 * n, lane);
-#pragma unroll
-            for (int m = 0; m < F; m++)
-#pragma unroll
-                for (int n = 0; n < F; n++) acc[m][n] = mfma(fa[m], fb[n], acc[m][n]);
-        }
+        for (int k = 0; k < AHEAD; k++) load(ahead[k], 1 + k);
         __syncthreads();
-    };
-    // The steps whose loads are whole ones go in a loop of their own: loads that
-    // the compiler cannot count it would wait for at once.
-    const int whole = EDGE ? 0 : (int)((hi - lo) / DEPTH), fast = whole == steps ? all : PARTS == 1 ? whole : 0;
-    int s0 = 0;
-    for (; s0 + 2 * AHEAD < fast; s0 += AHEAD)
+        for (int s0 = 0; s0 < all; s0 += AHEAD) {
 #pragma unroll
-        for (int u = 0; u < AHEAD; u++) step(held_back[u], s0 + u, unchecked);
-    for (; s0 < all; s0 += AHEAD)
+            for (int u = 0; u < AHEAD; u++) {
+                const int s = s0 + u;
+                if (s >= all) break;
+                const char* from = lds + (s & 1) * 2 * SIDE;
+                char* to = lds + (s + 1 & 1) * 2 * SIDE;
+                const int64_t r0 = first_row(s + 1 + AHEAD);
+                take(from, 0);
 #pragma unroll
-        for (int u = 0; u < AHEAD; u++) {
-            if (s0 + u >= all) break;
-            step(held_back[u], s0 + u, checked);
+                for (int k = 0; k < 4; k++) {
+                    if (k < 3) take(from, k + 1);
+                    put(ahead[u], k, to, PARTS == 1 ? 0 : (s + 1) / whole);
+                    if (k % 2) load_a(ahead[u], k / 2, r0);
+                    load_g(ahead[u], k, r0);
+                    multiply(k);
+                }
+                __syncthreads();
+            }
         }
+    }
+    // what is left
+    for (int64_t r0 = lo + int64_t(whole) * DEPTH; r0 < hi; r0 += DEPTH) {
+        Loads& l = ahead[0];
+#pragma unroll
+        for (int m = 0; m < S::A_CHUNKS; m++) l.a[m] = load_kept(a, r0 + ar + m * AR, hi, tile.i0 + ac);
+#pragma unroll
+        for (int m = 0; m < S::B_CHUNKS; m++) l.g[m] = load_grad<T>(a, r0 + br + m * BR, hi, tile.j0 + bc);
+        for (int plane = 0; plane < PARTS; plane++) {
+#pragma unroll
+            for (int k = 0; k < 4; k++) put(l, k, lds, plane);
+            __syncthreads();
+#pragma unroll
+            for (int k = 0; k < 4; k++) {
+                take(lds, k);
+                multiply(k);
+            }
+            __syncthreads();
+        }
+    }
 }
 
 template <class T, int F, int ACT>
@@ -284,7 +321,7 @@ __global__ __launch_bounds__(BLOCK, 2) void k_weight(Job job) {
     constexpr int TILE = S::TILE;
     __shared__ __align__(16) char lds[4 * DEPTH * S::PITCH];  // two buffers of a tile of each operand
     const wc_ckpt_weight_args& a = job.a;
-    const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
+    const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
     // Workgroups go round the eight XCDs; consecutive tiles of a run, which share
     // rows of both operands, go to one XCD's cache.
     const int total = job.tiles_i * job.tiles_j * job.runs, per = total / 8;
@@ -295,18 +332,13 @@ __global__ __launch_bounds__(BLOCK, 2) void k_weight(Job job) {
     tile.j0 = int64_t(at / job.tiles_i) * TILE;
     tile.lo = run * job.run;
     tile.hi = min(tile.lo + job.run, a.rows);
-    tile.steps = (int)((max<int64_t>(tile.hi - tile.lo, 0) + DEPTH - 1) / DEPTH);
+    tile.open = job.open;
     tile.sums = a.bias && tile.i0 == 0;
     f32x16 acc[F][F] = {};
-    float bias[8] = {};
-    if (tile.steps) {
-        if (tile.i0 + TILE <= a.width && tile.j0 + TILE <= a.out) products<T, F, ACT, false>(a, tile, lds, acc, bias);
-        else products<T, F, ACT, true>(a, tile, lds, acc, bias);
-    }
-    const int wi = (wave >> 1) * 32 * F, wj = (wave & 1) * 32 * F, bc = (t % (TILE / 8)) * 8, br = t / (TILE / 8);
+    float bias[F] = {};
+    if (tile.lo < tile.hi) products<T, F, ACT>(a, tile, lds, acc, bias);
+    const int wi = (wave >> 1) * 32 * F, wj = (wave & 1) * 32 * F;
     const int64_t i0 = tile.i0, j0 = tile.j0;
-    const bool sums = tile.sums;
-    constexpr int BR = BLOCK / (TILE / 8);
 
     const bool last = job.runs == 1;
     float* part = job.part + int64_t(run) * a.width * a.out;
@@ -322,16 +354,12 @@ __global__ __launch_bounds__(BLOCK, 2) void k_weight(Job job) {
                 else if (a.weight_dtype == WC_DTYPE_F32) ((float*)a.weight)[i * a.weight_stride + j] = acc[m][n][k];
                 else ((T*)a.weight)[i * a.weight_stride + j] = (T)acc[m][n][k];
             }
-    if (sums) {  // the threads of one column chunk, in order
-        float* rows = (float*)lds;
+    if (tile.sums && wi == 0) {  // a column's rows are in two lanes
 #pragma unroll
-        for (int i = 0; i < 8; i++) rows[br * TILE + bc + i] = bias[i];
-        __syncthreads();
-        if (t < TILE && j0 + t < a.out) {
-            float s = 0.f;
-            for (int k = 0; k < BR; k++) s += rows[k * TILE + t];
-            if (last) a.bias[j0 + t] = s;
-            else job.bias_part[int64_t(run) * a.out + j0 + t] = s;
+        for (int n = 0; n < F; n++) {
+            const float s = bias[n] + __shfl_xor(bias[n], 32);
+            const int64_t j = j0 + wj + 32 * n + lane;
+            if (lane < 32 && j < a.out) (last ? a.bias : job.bias_part + int64_t(run) * a.out)[j] = s;
         }
     }
 }
@@ -353,21 +381,6 @@ struct BigJob {
     const char* g;     // rows x out, g_pitch bytes a row
     int64_t x_pitch, g_pitch;
 };
-
-__device__ __forceinline__ float plus(bf16x8 v, float s) {
-    typedef bf16 bf16x2 __attribute__((ext_vector_type(2)));
-    const bf16x2 one = {(bf16)1.f, (bf16)1.f};
-#pragma unroll
-    for (int i = 0; i < 8; i += 2) s = __builtin_amdgcn_fdot2_f32_bf16(bf16x2{v[i], v[i + 1]}, one, s, false);
-    return s;
-}
-__device__ __forceinline__ float plus(f16x8 v, float s) {
-    typedef f16 f16x2 __attribute__((ext_vector_type(2)));
-    const f16x2 one = {(f16)1.f, (f16)1.f};
-#pragma unroll
-    for (int i = 0; i < 8; i += 2) s = __builtin_amdgcn_fdot2(f16x2{v[i], v[i + 1]}, one, s, false);
-    return s;
-}
 
 // LDS as the large product addresses it.
 typedef __attribute__((address_space(3))) char* Lds;
@@ -676,7 +689,13 @@ template <class T>
 void weight(const wc_ckpt_weight_args& a, int cus, hipStream_t s) {
     const Plan p = plan_of(a, cus);
     char* w = (char*)a.workspace;
-    const Job job = {a, p.run, p.tiles_i, p.tiles_j, p.runs, (float*)(w + p.part), (float*)(w + p.bias)};
+    // whole chunks of the last columns reach this far past a row's end, which the rows that follow must hold
+    const int64_t past_q = (a.width + 15) / 16 * 16 - a.width, past_g = (a.out + 7) / 8 * 8 - a.out;
+    auto rows_past = [&](int64_t past, int64_t stride) {
+        return !past ? 0 : !stride ? a.rows : std::min(a.rows, (past + stride - 1) / stride);
+    };
+    const int64_t open = a.rows - std::max(rows_past(past_q, a.q_stride), rows_past(past_g, a.grad_stride));
+    const Job job = {a, p.run, open, p.tiles_i, p.tiles_j, p.runs, (float*)(w + p.part), (float*)(w + p.bias)};
     const dim3 grid(p.tiles_i * p.tiles_j * p.runs);
     if constexpr (sizeof(T) == 2) {
         if (p.big) {
