@@ -1,4 +1,12 @@
 // The residual update between two norms, forward and backward (include/wc_learn.h).
+//
+// Memory bounds both: the forward reads two matrices and writes two, the
+// backward reads four and writes two (a gate with a row each: one more read,
+// and one more written). Each is read once: a row's values stay in registers,
+// eight to a thread, from the load through both norms to the store. A
+// workgroup takes row after row with the parameters in registers and the next
+// row's loads in flight, and in the backward with the columns' sums of all its
+// rows; a small kernel adds the workgroups' sums in order.
 #include <algorithm>
 
 #include "learn.h"
@@ -10,46 +18,70 @@ namespace wc {
 namespace learn {
 namespace {
 
+// Eight elements from p as they are; NARROW: the first n, and zeros.
+template <class T, bool NARROW>
+__device__ __forceinline__ typename Vec8<T>::type raw8(const T* p, int n) {
+    typename Vec8<T>::type v = {};
+    if (!NARROW) return *(const typename Vec8<T>::type*)p;
+#pragma unroll
+    for (int i = 0; i < 8; i++)
+        if (i < n) v[i] = p[i];
+    return v;
+}
+
+template <class T, bool NARROW>
+__device__ __forceinline__ void put8(T* p, int n, const float (&v)[8]) {
+    store_n(p, NARROW ? n : 8, v);
+}
+
 // Eight values of a parameter vector from column c; `fill` where there is none.
+template <bool NARROW>
 __device__ __forceinline__ void load_param(const void* p, int dtype, int64_t c, int n, float fill, float (&v)[8]) {
     if (!p) {
 #pragma unroll
         for (int i = 0; i < 8; i++) v[i] = fill;
     } else if (dtype == WC_DTYPE_F32) {
-        load_n((const float*)p + c, n, 0.f, v);
+        const auto r = raw8<float, NARROW>((const float*)p + c, n);
+#pragma unroll
+        for (int i = 0; i < 8; i++) v[i] = r[i];
     } else if (dtype == WC_DTYPE_F16) {
-        load_n((const f16*)p + c, n, 0.f, v);
+        const auto r = raw8<f16, NARROW>((const f16*)p + c, n);
+#pragma unroll
+        for (int i = 0; i < 8; i++) v[i] = (float)r[i];
     } else {
-        load_n((const bf16*)p + c, n, 0.f, v);
+        const auto r = raw8<bf16, NARROW>((const bf16*)p + c, n);
+#pragma unroll
+        for (int i = 0; i < 8; i++) v[i] = (float)r[i];
     }
 }
 
-// Sums over the G threads that hold a row, the same bits in each of them: a
-// butterfly inside a wavefront, then the wavefronts' sums in order through LDS.
-// Two slots alternate, so one barrier per sum is enough: a wavefront writes a
-// slot again only after a barrier that every reader of its last use has passed.
-// `lds` is the row's own slots: a workgroup of several such rows has as many.
+constexpr int MOST_WAVES = 16;
+
+// Sums over the threads that hold a row, the same bits in each of them: over G
+// lanes of a wavefront by a butterfly, or with G 0 over the workgroup: then
+// the wavefronts' sums, in order, through LDS. Two slots alternate, so one
+// barrier per sum is enough: a wavefront writes a slot again only after a
+// barrier that every reader of its last use has passed.
 template <int G>
 struct RowSum {
-    static constexpr int WAVES = G > 64 ? G / 64 : 1;
-    typedef float2 Slots[2][WAVES];
-    Slots& lds;
-    int slot = 0;
+    float2* lds;  // 2 x MOST_WAVES
+    int waves, slot = 0;
 
     __device__ __forceinline__ float2 operator()(float a, float b) {
 #pragma unroll
-        for (int mask = (G < 64 ? G : 64) / 2; mask; mask >>= 1) {
+        for (int mask = (G ? G : 64) / 2; mask; mask >>= 1) {
             a += __shfl_xor(a, mask);
             b += __shfl_xor(b, mask);
         }
-        if constexpr (G > 64) {
-            if ((threadIdx.x & 63) == 0) lds[slot][threadIdx.x % G >> 6] = make_float2(a, b);
+        if constexpr (G == 0) {
+            float2* at = lds + slot * MOST_WAVES;
+            if ((threadIdx.x & 63) == 0) at[threadIdx.x >> 6] = make_float2(a, b);
             __syncthreads();
             a = b = 0.f;
-#pragma unroll
-            for (int w = 0; w < WAVES; w++) {
-                a += lds[slot][w].x;
-                b += lds[slot][w].y;
+            for (int w = 0; w < waves; w++) {
+                const float2 o = at[w];
+                a += o.x;
+                b += o.y;
             }
             slot ^= 1;
         }
@@ -60,7 +92,7 @@ struct RowSum {
 // act(g), and its slope in *d.
 __device__ __forceinline__ float gate_of(float g, int act, float* d) {
     if (act == WC_GATE_SIGMOID) {
-        const float s = 1.f / (1.f + expf(-g));
+        const float s = __builtin_amdgcn_rcpf(1.f + fast_exp(-g));
         *d = s * (1.f - s);
         return s;
     }
@@ -73,309 +105,418 @@ __device__ __forceinline__ float gate_of(float g, int act, float* d) {
     return g;
 }
 
-template <int G>
-constexpr int block_of() {
-    return G < 256 ? 256 : G;
-}
+// How a workgroup's threads hold rows: G lanes a row, or with G 0 all of them,
+// a chunk of eight columns each (NV: and one every `step` threads on). The last
+// chunk of a width that eight does not divide is moved back to end with the
+// row: its first columns are then the chunk before's too. Both threads compute
+// and write the same values there; sums over the row leave out the second's
+// (`skip` of them, or all eight of a thread past the end). So every load is a
+// whole one. NARROW, of rows of less than eight: single elements.
+template <int G, int NV, bool NARROW>
+struct Layout {
+    int lane, group, per;  // of the row; which row; rows at once
+    int col[NV], skip[NV], n;
+
+    __device__ __forceinline__ explicit Layout(int width) {
+        const int step = G ? G : blockDim.x;
+        lane = G ? threadIdx.x % (G ? G : 1) : threadIdx.x;
+        group = G ? threadIdx.x / (G ? G : 1) : 0;
+        per = G ? blockDim.x / (G ? G : 1) : 1;
+        n = width;
+#pragma unroll
+        for (int k = 0; k < NV; k++) {
+            const int c = 8 * (lane + k * step);
+            col[k] = NARROW ? 0 : min(c, width - 8);
+            skip[k] = NARROW ? (lane ? 8 : 0) : min(c - col[k], 8);
+        }
+    }
+    __device__ __forceinline__ bool counts(int k, int i) const { return i >= skip[k] && (!NARROW || i < n); }
+    __device__ __forceinline__ bool holds(int k) const { return skip[k] < 8; }
+};
 
 // Mean (0 for RMS) and 1 / sqrt(variance + eps) of the row's values, from two
 // passes over registers.
-template <int G, int NV>
-__device__ __forceinline__ float2 row_stats(const float (&v)[NV][8], const int (&n)[NV], int width, bool layer,
-                                            float eps, RowSum<G>& sum) {
-    float mean = 0.f;
-    if (layer) {
+template <int G, int NV, bool LAYER, class L>
+__device__ __forceinline__ float2 row_stats(const float (&v)[NV][8], const L& at, float width, float eps,
+                                            RowSum<G>& sum) {
+    float mean = 0.f, q = 0.f;
+    if (LAYER) {
         float s = 0.f;
 #pragma unroll
         for (int k = 0; k < NV; k++)
 #pragma unroll
-            for (int i = 0; i < 8; i++) s += v[k][i];  // 0 beyond the row's end
-        mean = sum(s, 0.f).x / (float)width;
+            for (int i = 0; i < 8; i++) s += at.counts(k, i) ? v[k][i] : 0.f;
+        mean = sum(s, 0.f).x / width;
     }
-    float q = 0.f;
 #pragma unroll
     for (int k = 0; k < NV; k++)
 #pragma unroll
         for (int i = 0; i < 8; i++) {
-            const float d = i < n[k] ? v[k][i] - mean : 0.f;
+            const float d = at.counts(k, i) ? v[k][i] - mean : 0.f;
             q += d * d;
         }
-    const float var = sum(q, 0.f).x / (float)width;
-    return make_float2(mean, 1.f / sqrtf(var + eps));
+    return make_float2(mean, 1.f / sqrtf(sum(q, 0.f).x / width + eps));
 }
 
-template <class T, int G, int NV>
-__global__ __launch_bounds__(block_of<G>()) void k_norm(wc_norm_args a) {
-    constexpr int PER = block_of<G>() / G;
-    __shared__ typename RowSum<G>::Slots lds[PER];
-    RowSum<G> sum{lds[threadIdx.x / G]};
-    const int lane = threadIdx.x % G;
-    const int width = (int)a.width;
-    int n[NV];
+// The update of a column is gain * norm(block) + bias, with the scale, the gate
+// vector and the parameters folded together where the gate is not the row's own.
+template <bool NARROW, class A>
+__device__ __forceinline__ void fold(const A& a, bool token, int col, int n, float (&gain)[8], float (&bias)[8]) {
+    float g[8];
+    load_param<NARROW>(a.post_gain, a.param_dtype, col, n, 1.f, gain);
+    load_param<NARROW>(a.post_bias, a.param_dtype, col, n, 0.f, bias);
+    load_param<NARROW>(token ? nullptr : a.gate, a.param_dtype, col, n, 1.f, g);
 #pragma unroll
-    for (int k = 0; k < NV; k++) n[k] = min(8, max(0, width - 8 * (lane + k * G)));
-    for (int64_t r0 = int64_t(blockIdx.x) * PER; r0 < a.rows; r0 += int64_t(gridDim.x) * PER) {
-        const int64_t row = r0 + threadIdx.x / G;
-        const bool here = row < a.rows;  // the others go along: the sums are taken by whole wavefronts
-        const int64_t r = here ? row : a.rows - 1;
-        float u[NV][8], x[NV][8];
-#pragma unroll
-        for (int k = 0; k < NV; k++) load_n((const T*)a.block + r * a.block_stride + 8 * (lane + k * G), n[k], 0.f, u[k]);
-#pragma unroll
-        for (int k = 0; k < NV; k++) load_n((const T*)a.stream + r * a.stream_stride + 8 * (lane + k * G), n[k], 0.f, x[k]);
-        const float2 s1 = row_stats<G, NV>(u, n, width, a.norm == WC_NORM_LAYER, a.eps, sum);
-#pragma unroll
-        for (int k = 0; k < NV; k++) {
-            const int64_t c = 8 * (lane + k * G);
-            float g[8], b[8], w[8];
-            load_param(a.post_gain, a.param_dtype, c, n[k], 1.f, g);
-            load_param(a.post_bias, a.param_dtype, c, n[k], 0.f, b);
-            if (a.gate && a.gate_stride) load_n((const T*)a.gate + r * a.gate_stride + c, n[k], 0.f, w);
-            else load_param(a.gate, a.param_dtype, c, n[k], 1.f, w);
-#pragma unroll
-            for (int i = 0; i < 8; i++) {
-                float slope;
-                const float gate = a.gate ? gate_of(w[i], a.gate_act, &slope) : 1.f;
-                x[k][i] = i < n[k] ? x[k][i] + a.scale * gate * ((u[k][i] - s1.x) * s1.y * g[i] + b[i]) : 0.f;
-            }
-            if (here) store_n((T*)a.new_stream + r * a.new_stream_stride + c, n[k], x[k]);
-        }
-        const float2 s2 = row_stats<G, NV>(x, n, width, a.norm == WC_NORM_LAYER, a.eps, sum);
-#pragma unroll
-        for (int k = 0; k < NV; k++) {
-            const int64_t c = 8 * (lane + k * G);
-            float g[8], b[8];
-            load_param(a.pre_gain, a.param_dtype, c, n[k], 1.f, g);
-            load_param(a.pre_bias, a.param_dtype, c, n[k], 0.f, b);
-#pragma unroll
-            for (int i = 0; i < 8; i++) g[i] = (x[k][i] - s2.x) * s2.y * g[i] + b[i];
-            if (here) store_n((T*)a.out + r * a.out_stride + c, n[k], g);
-        }
-        if (a.stats && here && lane == 0) ((float4*)a.stats)[r] = make_float4(s1.x, s1.y, s2.x, s2.y);
+    for (int i = 0; i < 8; i++) {
+        float slope;
+        const float f = a.scale * (a.gate && !token ? gate_of(g[i], a.gate_act, &slope) : 1.f);
+        gain[i] *= f;
+        bias[i] *= f;
     }
 }
 
-// The parameters' gradients in the order their column sums are kept.
-constexpr int SUMS = 5;  // post gain, post bias, gate vector, pre gain, pre bias
-
-// One workgroup takes rows blockIdx.x * PER, + gridDim.x * PER, ... and writes
-// its column sums to part[blockIdx.x][SUMS][width].
-template <class T, int G, int NV>
-__global__ __launch_bounds__(block_of<G>()) void k_norm_back(wc_norm_back_args a, float* part) {
-    constexpr int PER = block_of<G>() / G;
-    __shared__ typename RowSum<G>::Slots lds[PER];
-    __shared__ float cols[PER > 1 ? G * NV * 8 : 1];
-    RowSum<G> sum{lds[threadIdx.x / G]};
-    const int lane = threadIdx.x % G;
-    const int width = (int)a.width;
-    const bool layer = a.norm == WC_NORM_LAYER, vector = a.gate && !a.gate_stride;
-    const float inv = 1.f / (float)width;
-    int n[NV];
-    float acc[SUMS][NV][8];
+template <class T, int G, int NV, bool LAYER, bool TOKEN, bool NARROW>
+__global__ __launch_bounds__(G ? 256 : 1024) void k_norm(wc_norm_args a) {
+    typedef typename Vec8<T>::type Raw;
+    __shared__ float2 lds[2 * MOST_WAVES];
+    const Layout<G, NV, NARROW> at((int)a.width);
+    RowSum<G> sum{lds, (int)blockDim.x / 64};
+    const float width = (float)(int)a.width;
+    float g1[NV][8], b1[NV][8], g2[NV][8], b2[NV][8];
 #pragma unroll
     for (int k = 0; k < NV; k++) {
-        n[k] = min(8, max(0, width - 8 * (lane + k * G)));
-#pragma unroll
-        for (int q = 0; q < SUMS; q++)
-#pragma unroll
-            for (int i = 0; i < 8; i++) acc[q][k][i] = 0.f;
+        fold<NARROW>(a, TOKEN, at.col[k], at.n, g1[k], b1[k]);
+        load_param<NARROW>(a.pre_gain, a.param_dtype, at.col[k], at.n, 1.f, g2[k]);
+        load_param<NARROW>(a.pre_bias, a.param_dtype, at.col[k], at.n, 0.f, b2[k]);
     }
-    for (int64_t r0 = int64_t(blockIdx.x) * PER; r0 < a.rows; r0 += int64_t(gridDim.x) * PER) {
-        const int64_t row = r0 + threadIdx.x / G;
-        const bool here = row < a.rows;
-        const int64_t r = here ? row : a.rows - 1;
-        const float4 st = ((const float4*)a.stats)[r];
-        // norm of the block, the update's factor, and the stream after it, as the forward computed them
-        float uh[NV][8], xh[NV][8], fac[NV][8], dx[NV][8];
+    const int64_t stride = int64_t(gridDim.x) * at.per;
+    Raw ru[NV], rx[NV], rg[TOKEN ? NV : 1];
+    auto load = [&](int64_t row) {
+        const int64_t r = min(row, a.rows - 1);  // rows past the end go along: the sums are taken by whole wavefronts
+#pragma unroll
+        for (int k = 0; k < NV; k++) {
+            ru[k] = raw8<T, NARROW>((const T*)a.block + r * a.block_stride + at.col[k], at.n);
+            rx[k] = raw8<T, NARROW>((const T*)a.stream + r * a.stream_stride + at.col[k], at.n);
+            if (TOKEN) rg[k] = raw8<T, NARROW>((const T*)a.gate + r * a.gate_stride + at.col[k], at.n);
+        }
+    };
+    int64_t r = int64_t(blockIdx.x) * at.per + at.group;
+    load(r);
+    for (int64_t r0 = int64_t(blockIdx.x) * at.per; r0 < a.rows; r0 += stride, r += stride) {
+        float u[NV][8], x[NV][8];
+        Raw g[TOKEN ? NV : 1];
+#pragma unroll
+        for (int k = 0; k < NV; k++) {
+#pragma unroll
+            for (int i = 0; i < 8; i++) u[k][i] = (float)ru[k][i], x[k][i] = (float)rx[k][i];
+            if (TOKEN) g[k] = rg[k];
+        }
+        if (r0 + stride < a.rows) load(r + stride);
+        const bool here = r < a.rows;
+        const float2 s1 = row_stats<G, NV, LAYER>(u, at, width, a.eps, sum);
+#pragma unroll
+        for (int k = 0; k < NV; k++) {
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                float w = 1.f, slope;
+                if (TOKEN) w = gate_of((float)g[k][i], a.gate_act, &slope);
+                x[k][i] += w * ((u[k][i] - s1.x) * s1.y * g1[k][i] + b1[k][i]);
+            }
+            if (here && at.holds(k)) put8<T, NARROW>((T*)a.new_stream + r * a.new_stream_stride + at.col[k], at.n, x[k]);
+        }
+        const float2 s2 = row_stats<G, NV, LAYER>(x, at, width, a.eps, sum);
+#pragma unroll
+        for (int k = 0; k < NV; k++) {
+#pragma unroll
+            for (int i = 0; i < 8; i++) x[k][i] = (x[k][i] - s2.x) * s2.y * g2[k][i] + b2[k][i];
+            if (here && at.holds(k)) put8<T, NARROW>((T*)a.out + r * a.out_stride + at.col[k], at.n, x[k]);
+        }
+        if (a.stats && here && at.lane == 0) ((float4*)a.stats)[r] = make_float4(s1.x, s1.y, s2.x, s2.y);
+    }
+}
+
+// The parameters' gradients: which of them are wanted, and where the column
+// sums go. The workgroups' sums lie one wanted parameter after the other.
+constexpr int SUMS = 5;  // post gain, post bias, gate vector, pre gain, pre bias
+struct ColumnSums {
+    float* out[SUMS];
+    int at[SUMS];  // the parameter's place among the wanted, or -1
+    int wanted;
+};
+
+// With v what arrives at stream' in all and w the update's factor of a column,
+// the parameters' gradients are of four sums over the rows: of w v norm(block)
+// and w v, of d_out norm(stream') and d_out. A factor that is the column's own
+// stays out of the sums: the gate vector's gradient is of the same two.
+// MOST: threads of the widest workgroup; 512 leave a thread the registers that it needs.
+template <class T, int G, int NV, bool LAYER, bool TOKEN, bool NARROW, int MOST>
+__global__ __launch_bounds__(G ? 256 : MOST) void k_norm_back(wc_norm_back_args a, ColumnSums sums, float* part) {
+    typedef typename Vec8<T>::type Raw;
+    __shared__ float2 lds[2 * MOST_WAVES];
+    __shared__ float cols[G ? G * NV * 8 : 1];
+    const Layout<G, NV, NARROW> at((int)a.width);
+    RowSum<G> sum{lds, (int)blockDim.x / 64};
+    const float width = (float)(int)a.width;
+    float g1[NV][8], b1[NV][8], g2[NV][8], acc[4][NV][8] = {};
+#pragma unroll
+    for (int k = 0; k < NV; k++) {
+        fold<NARROW>(a, TOKEN, at.col[k], at.n, g1[k], b1[k]);
+        load_param<NARROW>(a.pre_gain, a.param_dtype, at.col[k], at.n, 1.f, g2[k]);
+    }
+    const int64_t stride = int64_t(gridDim.x) * at.per;
+    Raw ru[NV], rx[NV], rh[NV], rd[NV], rg[TOKEN ? NV : 1];
+    float4 rs;
+    auto load = [&](int64_t row) {
+        const int64_t r = min(row, a.rows - 1);
+        rs = ((const float4*)a.stats)[r];
+#pragma unroll
+        for (int k = 0; k < NV; k++) {
+            ru[k] = raw8<T, NARROW>((const T*)a.block + r * a.block_stride + at.col[k], at.n);
+            rx[k] = raw8<T, NARROW>((const T*)a.stream + r * a.stream_stride + at.col[k], at.n);
+            rh[k] = Raw{}, rd[k] = Raw{};
+            if (a.d_out) rh[k] = raw8<T, NARROW>((const T*)a.d_out + r * a.d_out_stride + at.col[k], at.n);
+            if (a.d_new_stream)
+                rd[k] = raw8<T, NARROW>((const T*)a.d_new_stream + r * a.d_new_stream_stride + at.col[k], at.n);
+            if (TOKEN) rg[k] = raw8<T, NARROW>((const T*)a.gate + r * a.gate_stride + at.col[k], at.n);
+        }
+    };
+    int64_t r = int64_t(blockIdx.x) * at.per + at.group;
+    if (a.rows) load(r);
+    for (int64_t r0 = int64_t(blockIdx.x) * at.per; r0 < a.rows; r0 += stride, r += stride) {
+        const bool here = r < a.rows;
+        const float4 st = rs;
+        // the block's norm, and the stream's after the update, as the forward computed them
+        float uh[NV][8], xh[NV][8], dx[NV][8];
+        Raw d[NV], g[TOKEN ? NV : 1];
         float s1 = 0.f, s2 = 0.f;
 #pragma unroll
         for (int k = 0; k < NV; k++) {
-            const int64_t c = 8 * (lane + k * G);
-            float g[8], b[8], w[8], d[8], pg[8];
-            load_n((const T*)a.block + r * a.block_stride + c, n[k], 0.f, uh[k]);
-            load_n((const T*)a.stream + r * a.stream_stride + c, n[k], 0.f, xh[k]);
-            if (a.d_out) load_n((const T*)a.d_out + r * a.d_out_stride + c, n[k], 0.f, d);
-            load_param(a.post_gain, a.param_dtype, c, n[k], 1.f, g);
-            load_param(a.post_bias, a.param_dtype, c, n[k], 0.f, b);
-            load_param(a.pre_gain, a.param_dtype, c, n[k], 1.f, pg);
-            if (a.gate && a.gate_stride) load_n((const T*)a.gate + r * a.gate_stride + c, n[k], 0.f, w);
-            else load_param(a.gate, a.param_dtype, c, n[k], 1.f, w);
+            d[k] = rd[k];
+            if (TOKEN) g[k] = rg[k];
 #pragma unroll
             for (int i = 0; i < 8; i++) {
-                const bool in = i < n[k];
-                float slope;
-                const float gate = a.gate ? gate_of(w[i], a.gate_act, &slope) : 1.f;
-                uh[k][i] = in ? (uh[k][i] - st.x) * st.y : 0.f;
-                fac[k][i] = a.scale * gate;
-                const float x = xh[k][i] + fac[k][i] * (uh[k][i] * g[i] + b[i]);
-                xh[k][i] = in ? (x - st.z) * st.w : 0.f;
-                const float dh = a.d_out && in ? d[i] : 0.f;
-                if (here) {
-                    acc[3][k][i] += dh * xh[k][i];
-                    acc[4][k][i] += dh;
-                }
-                dx[k][i] = dh * pg[i];
-                s1 += dx[k][i];
-                s2 += dx[k][i] * xh[k][i];
+                float w = 1.f, slope;
+                if (TOKEN) w = gate_of((float)g[k][i], a.gate_act, &slope);
+                uh[k][i] = ((float)ru[k][i] - st.x) * st.y;
+                const float x = (float)rx[k][i] + w * (uh[k][i] * g1[k][i] + b1[k][i]);
+                xh[k][i] = (x - st.z) * st.w;
+                const float dh = here ? (float)rh[k][i] : 0.f;
+                acc[2][k][i] += dh * xh[k][i];
+                acc[3][k][i] += dh;
+                dx[k][i] = dh * g2[k][i];
+                const float t = at.counts(k, i) ? dx[k][i] : 0.f;
+                s1 += t;
+                s2 += t * xh[k][i];
             }
         }
+        if (r0 + stride < a.rows) load(r + stride);
         float2 m = sum(s1, s2);
-        m.x *= inv;
-        m.y *= inv;
-        if (!layer) m.x = 0.f;
+        const float c1 = LAYER ? m.x / width : 0.f, c2 = m.y / width;
         s1 = s2 = 0.f;
 #pragma unroll
         for (int k = 0; k < NV; k++) {
-            const int64_t c = 8 * (lane + k * G);
-            float g[8], b[8], w[8], d[8], dg[8];
-            if (a.d_new_stream) load_n((const T*)a.d_new_stream + r * a.d_new_stream_stride + c, n[k], 0.f, d);
-            load_param(a.post_gain, a.param_dtype, c, n[k], 1.f, g);
-            load_param(a.post_bias, a.param_dtype, c, n[k], 0.f, b);
-            if (a.gate && a.gate_stride) load_n((const T*)a.gate + r * a.gate_stride + c, n[k], 0.f, w);
-            else load_param(a.gate, a.param_dtype, c, n[k], 1.f, w);
+            float o[8], dg[8];
 #pragma unroll
             for (int i = 0; i < 8; i++) {
-                const bool in = i < n[k];
-                float slope = 0.f;
-                if (a.gate) gate_of(w[i], a.gate_act, &slope);
-                const float v = st.w * (dx[k][i] - m.x - xh[k][i] * m.y) + (a.d_new_stream ? d[i] : 0.f);
-                d[i] = v;
-                const float dn = in ? fac[k][i] * v : 0.f;
-                dg[i] = a.scale * slope * v * (uh[k][i] * g[i] + b[i]);
-                if (here) {
-                    acc[0][k][i] += dn * uh[k][i];
-                    acc[1][k][i] += dn;
-                    if (vector) acc[2][k][i] += in ? dg[i] : 0.f;
+                const float v = st.w * (dx[k][i] - c1 - xh[k][i] * c2) + (float)d[k][i];
+                o[i] = v;
+                float wv = v;
+                if (TOKEN) {
+                    float slope;
+                    wv = gate_of((float)g[k][i], a.gate_act, &slope) * v;
+                    dg[i] = slope * v * (uh[k][i] * g1[k][i] + b1[k][i]);
                 }
-                dx[k][i] = dn * g[i];
-                s1 += dx[k][i];
-                s2 += dx[k][i] * uh[k][i];
+                if (!here) wv = 0.f;
+                acc[0][k][i] += wv * uh[k][i];
+                acc[1][k][i] += wv;
+                dx[k][i] = wv * g1[k][i];
+                const float t = at.counts(k, i) ? dx[k][i] : 0.f;
+                s1 += t;
+                s2 += t * uh[k][i];
             }
-            if (here) {
-                store_n((T*)a.d_stream + r * a.d_stream_stride + c, n[k], d);
-                if (a.d_gate && a.gate_stride) store_n((T*)a.d_gate + r * a.d_gate_stride + c, n[k], dg);
+            if (here && at.holds(k)) {
+                put8<T, NARROW>((T*)a.d_stream + r * a.d_stream_stride + at.col[k], at.n, o);
+                if (TOKEN && a.d_gate) put8<T, NARROW>((T*)a.d_gate + r * a.d_gate_stride + at.col[k], at.n, dg);
             }
         }
         m = sum(s1, s2);
-        m.x *= inv;
-        m.y *= inv;
-        if (!layer) m.x = 0.f;
+        const float e1 = LAYER ? m.x / width : 0.f, e2 = m.y / width;
 #pragma unroll
         for (int k = 0; k < NV; k++) {
-            const int64_t c = 8 * (lane + k * G);
             float o[8];
 #pragma unroll
-            for (int i = 0; i < 8; i++) o[i] = st.y * (dx[k][i] - m.x - uh[k][i] * m.y);
-            if (here) store_n((T*)a.d_block + r * a.d_block_stride + c, n[k], o);
+            for (int i = 0; i < 8; i++) o[i] = st.y * (dx[k][i] - e1 - uh[k][i] * e2);
+            if (here && at.holds(k)) put8<T, NARROW>((T*)a.d_block + r * a.d_block_stride + at.col[k], at.n, o);
         }
     }
-    // the workgroup's column sums: its row groups in order
+    // the parameters' gradients from the four sums, and the workgroup's: its row groups in order
+#pragma unroll
     for (int q = 0; q < SUMS; q++) {
-        float* to = part + (size_t(blockIdx.x) * SUMS + q) * width;
-        if constexpr (PER == 1) {
+        if (sums.at[q] < 0) continue;
+        float* to = part + (size_t(blockIdx.x) * sums.wanted + sums.at[q]) * a.width;
+        float v[NV][8];
+#pragma unroll
+        for (int k = 0; k < NV; k++) {
+            float gain[8], bias[8], gate[8];
+            if (q < 3) {
+                load_param<NARROW>(a.post_gain, a.param_dtype, at.col[k], at.n, 1.f, gain);
+                load_param<NARROW>(a.post_bias, a.param_dtype, at.col[k], at.n, 0.f, bias);
+                load_param<NARROW>(TOKEN ? nullptr : a.gate, a.param_dtype, at.col[k], at.n, 1.f, gate);
+            }
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                float w = 1.f, slope = 1.f;
+                if (q < 3 && !TOKEN && a.gate) w = gate_of(gate[i], a.gate_act, &slope);
+                if (q < 2) v[k][i] = a.scale * w * acc[q][k][i];
+                else if (q == 2) v[k][i] = a.scale * slope * (gain[i] * acc[0][k][i] + bias[i] * acc[1][k][i]);
+                else v[k][i] = acc[q - 1][k][i];
+            }
+        }
+        if constexpr (G == 0) {
 #pragma unroll
             for (int k = 0; k < NV; k++)
-                if (n[k] > 0) store_n(to + 8 * (lane + k * G), n[k], acc[q][k]);
+                if (at.holds(k)) put8<float, NARROW>(to + at.col[k], at.n, v[k]);
         } else {
-            for (int g = 0; g < PER; g++) {
+            for (int g = 0; g < at.per; g++) {
                 __syncthreads();
-                if ((int)threadIdx.x / G == g) {
+                if (at.group == g) {
 #pragma unroll
-                    for (int k = 0; k < NV; k++)
+                    for (int k = 0; k < NV; k++) {
+                        if (!at.holds(k)) continue;
+                        float o[8];
 #pragma unroll
-                        for (int i = 0; i < 8; i++) {
-                            const int c = 8 * (lane + k * G) + i;
-                            cols[c] = (g ? cols[c] : 0.f) + acc[q][k][i];
-                        }
+                        for (int i = 0; i < 8; i++) o[i] = (g ? cols[at.col[k] + i] : 0.f) + v[k][i];
+#pragma unroll
+                        for (int i = 0; i < 8; i++) cols[at.col[k] + i] = o[i];
+                    }
                 }
             }
             __syncthreads();
-            for (int c = threadIdx.x; c < width; c += block_of<G>()) to[c] = cols[c];
+            for (int c = threadIdx.x; c < a.width; c += blockDim.x) to[c] = cols[c];
         }
     }
 }
 
-struct ColumnSums {
-    float* out[SUMS];
-};
-
-// Sums the workgroups' column sums in order: 64 columns by 4 interleaved runs.
-__global__ __launch_bounds__(256) void k_norm_cols(const float* part, int blocks, int width, ColumnSums o) {
-    __shared__ float lds[4][64];
-    const int q = blockIdx.y, c = blockIdx.x * 64 + (threadIdx.x & 63), run = threadIdx.x >> 6;
-    if (!o.out[q]) return;
-    float s = 0.f;
-    if (c < width)
-        for (int b = run; b < blocks; b += 4) s += part[(size_t(b) * SUMS + q) * width + c];
-    lds[run][threadIdx.x & 63] = s;
+// Adds the workgroups' column sums: N columns a thread, 8 threads side by side,
+// every 32nd workgroup to each of 32 rows of threads, whose sums are added in
+// order.
+template <int N>
+__global__ __launch_bounds__(256) void k_norm_cols(const float* part, int blocks, int64_t width, ColumnSums sums) {
+    typedef float Some __attribute__((ext_vector_type(N)));
+    __shared__ Some lds[32][8];
+    const int x = threadIdx.x & 7, y = threadIdx.x >> 3;
+    int q = 0;
+    while (sums.at[q] != (int)blockIdx.y) q++;
+    const int64_t c = (int64_t(blockIdx.x) * 8 + x) * N, pitch = width * sums.wanted;
+    const float* from = part + blockIdx.y * width + c;
+    Some s = {};
+    if (c < width) {
+        int b = y;
+        for (; b + 96 < blocks; b += 128) {
+            Some v[4];
+#pragma unroll
+            for (int u = 0; u < 4; u++) v[u] = *(const Some*)(from + (b + 32 * u) * pitch);
+            s += (v[0] + v[1]) + (v[2] + v[3]);
+        }
+        for (; b < blocks; b += 32) s += *(const Some*)(from + b * pitch);
+    }
+    lds[y][x] = s;
     __syncthreads();
-    if (run == 0 && c < width) o.out[q][c] = (lds[0][c & 63] + lds[1][c & 63]) + (lds[2][c & 63] + lds[3][c & 63]);
+    if (y || c >= width) return;
+    for (int k = 1; k < 32; k++) s += lds[k][x];
+    *(Some*)(sums.out[q] + c) = s;
 }
 
-// Threads per row: eight channels each, a power of two.
-int group_of(int64_t width) {
-    int g = 8;
-    while (g < 1024 && 8 * g < width) g *= 2;
-    return g;
+// ------------------------------------------------------------------ launches
+
+// Lanes per row (0: the workgroup) and threads of the workgroup: as many as the
+// row has chunks of eight, by powers of two inside a wavefront and by whole
+// wavefronts beyond; past 8,192 columns two chunks a thread.
+struct Threads {
+    int g, block, nv;
+};
+Threads threads_of(int64_t width) {
+    const int64_t chunks = (width + 7) / 8;
+    if (chunks <= 64) {
+        int g = 8;
+        while (g < chunks) g *= 2;
+        return {g, 256, 1};
+    }
+    if (chunks <= 1024) return {0, (int)((chunks + 63) / 64 * 64), 1};
+    return {0, 1024, 2};
 }
 
-int back_blocks(int64_t rows, int64_t width, int cus) {
-    const int g = group_of(width), per = g < 256 ? 256 / g : 1;
-    const int64_t want = (rows + per - 1) / per;
-    return (int)std::max<int64_t>(1, std::min<int64_t>(want, int64_t(cus) * std::max(1, 1024 / std::max(256, g))));
+// Workgroups: enough to fill the device, few enough that each has several rows
+// for its parameters (and in the backward for its column sums, which are
+// written and read again).
+int blocks_of(int64_t rows, const Threads& t, int waves_per_cu, int cus) {
+    const int64_t per = t.g ? t.block / t.g : 1, want = (rows + per - 1) / per;
+    const int64_t most = int64_t(cus) * std::max(1, waves_per_cu * 64 / t.block);
+    return (int)std::max<int64_t>(1, std::min(want, most));
 }
 
-template <class T, int G, int NV>
-void norm_at(const wc_norm_args& a, int cus, hipStream_t s) {
-    constexpr int PER = block_of<G>() / G;
-    const int64_t want = (a.rows + PER - 1) / PER;
-    k_norm<T, G, NV><<<dim3((uint32_t)std::min<int64_t>(want, 1 << 20)), block_of<G>(), 0, s>>>(a);
-}
+constexpr int FORWARD_WAVES = 16, BACKWARD_WAVES = 16;
 
-template <class T, int G, int NV>
-void back_at(const wc_norm_back_args& a, int blocks, hipStream_t s) {
-    k_norm_back<T, G, NV><<<dim3(blocks), block_of<G>(), 0, s>>>(a, (float*)a.workspace);
+template <class T, int G, int NV, bool NARROW = false>
+void norm_at(const wc_norm_args& a, const Threads& t, int cus, hipStream_t s) {
+    const dim3 grid(blocks_of(a.rows, t, FORWARD_WAVES, cus));
+    const bool layer = a.norm == WC_NORM_LAYER, token = a.gate && a.gate_stride;
+    if (layer && token) k_norm<T, G, NV, true, true, NARROW><<<grid, t.block, 0, s>>>(a);
+    else if (layer) k_norm<T, G, NV, true, false, NARROW><<<grid, t.block, 0, s>>>(a);
+    else if (token) k_norm<T, G, NV, false, true, NARROW><<<grid, t.block, 0, s>>>(a);
+    else k_norm<T, G, NV, false, false, NARROW><<<grid, t.block, 0, s>>>(a);
 }
 
 template <class T>
 void norm(const wc_norm_args& a, int cus, hipStream_t s) {
-    switch (group_of(a.width)) {
-        case 8: return norm_at<T, 8, 1>(a, cus, s);
-        case 16: return norm_at<T, 16, 1>(a, cus, s);
-        case 32: return norm_at<T, 32, 1>(a, cus, s);
-        case 64: return norm_at<T, 64, 1>(a, cus, s);
-        case 128: return norm_at<T, 128, 1>(a, cus, s);
-        case 256: return norm_at<T, 256, 1>(a, cus, s);
-        case 512: return norm_at<T, 512, 1>(a, cus, s);
-        default: return a.width <= 8192 ? norm_at<T, 1024, 1>(a, cus, s) : norm_at<T, 1024, 2>(a, cus, s);
-    }
+    const Threads t = threads_of(a.width);
+    if (a.width < 8) norm_at<T, 8, 1, true>(a, t, cus, s);
+    else if (t.g == 8) norm_at<T, 8, 1>(a, t, cus, s);
+    else if (t.g == 16) norm_at<T, 16, 1>(a, t, cus, s);
+    else if (t.g == 32) norm_at<T, 32, 1>(a, t, cus, s);
+    else if (t.g == 64) norm_at<T, 64, 1>(a, t, cus, s);
+    else if (t.nv == 1) norm_at<T, 0, 1>(a, t, cus, s);
+    else norm_at<T, 0, 2>(a, t, cus, s);
+}
+
+template <class T, int G, int NV, int MOST, bool NARROW = false>
+void back_at(const wc_norm_back_args& a, const Threads& t, int blocks, const ColumnSums& c, hipStream_t s) {
+    const bool layer = a.norm == WC_NORM_LAYER, token = a.gate && a.gate_stride;
+    float* w = (float*)a.workspace;
+    if (layer && token) k_norm_back<T, G, NV, true, true, NARROW, MOST><<<dim3(blocks), t.block, 0, s>>>(a, c, w);
+    else if (layer) k_norm_back<T, G, NV, true, false, NARROW, MOST><<<dim3(blocks), t.block, 0, s>>>(a, c, w);
+    else if (token) k_norm_back<T, G, NV, false, true, NARROW, MOST><<<dim3(blocks), t.block, 0, s>>>(a, c, w);
+    else k_norm_back<T, G, NV, false, false, NARROW, MOST><<<dim3(blocks), t.block, 0, s>>>(a, c, w);
 }
 
 template <class T>
 void norm_back(const wc_norm_back_args& a, int cus, hipStream_t s) {
-    const int blocks = back_blocks(a.rows, a.width, cus);
-    switch (group_of(a.width)) {
-        case 8: back_at<T, 8, 1>(a, blocks, s); break;
-        case 16: back_at<T, 16, 1>(a, blocks, s); break;
-        case 32: back_at<T, 32, 1>(a, blocks, s); break;
-        case 64: back_at<T, 64, 1>(a, blocks, s); break;
-        case 128: back_at<T, 128, 1>(a, blocks, s); break;
-        case 256: back_at<T, 256, 1>(a, blocks, s); break;
-        case 512: back_at<T, 512, 1>(a, blocks, s); break;
-        default:
-            if (a.width <= 8192) back_at<T, 1024, 1>(a, blocks, s);
-            else back_at<T, 1024, 2>(a, blocks, s);
-    }
-    const ColumnSums o = {{a.d_post_gain, a.d_post_bias, a.gate && !a.gate_stride ? (float*)a.d_gate : nullptr,
-                           a.d_pre_gain, a.d_pre_bias}};
-    k_norm_cols<<<dim3((uint32_t)(a.width + 63) / 64, SUMS), 256, 0, s>>>((const float*)a.workspace, blocks,
-                                                                        (int)a.width, o);
+    const Threads t = threads_of(a.width);
+    const int blocks = blocks_of(a.rows, t, BACKWARD_WAVES, cus);
+    ColumnSums c = {{a.d_post_gain, a.d_post_bias, a.gate && !a.gate_stride ? (float*)a.d_gate : nullptr, a.d_pre_gain,
+                     a.d_pre_bias}, {}, 0};
+    for (int q = 0; q < SUMS; q++) c.at[q] = c.out[q] ? c.wanted++ : -1;
+    if (a.width < 8) back_at<T, 8, 1, 256, true>(a, t, blocks, c, s);
+    else if (t.g == 8) back_at<T, 8, 1, 256>(a, t, blocks, c, s);
+    else if (t.g == 16) back_at<T, 16, 1, 256>(a, t, blocks, c, s);
+    else if (t.g == 32) back_at<T, 32, 1, 256>(a, t, blocks, c, s);
+    else if (t.g == 64) back_at<T, 64, 1, 256>(a, t, blocks, c, s);
+    else if (t.block <= 512) back_at<T, 0, 1, 512>(a, t, blocks, c, s);
+    else if (t.nv == 1) back_at<T, 0, 1, 1024>(a, t, blocks, c, s);
+    else back_at<T, 0, 2, 1024>(a, t, blocks, c, s);
+    if (!c.wanted) return;
+    bool four = a.width % 4 == 0;
+    for (int q = 0; q < SUMS; q++) four = four && ((uintptr_t)c.out[q] & 15) == 0;
+    const int64_t n = four ? 32 : 8;
+    const dim3 grid((uint32_t)((a.width + n - 1) / n), c.wanted);
+    if (four) k_norm_cols<4><<<grid, 256, 0, s>>>((const float*)a.workspace, blocks, a.width, c);
+    else k_norm_cols<1><<<grid, 256, 0, s>>>((const float*)a.workspace, blocks, a.width, c);
 }
 
 }  // namespace
 
 size_t norm_back_scratch(const wc_norm_back_args& a, int cus) {
-    return pad256(size_t(back_blocks(a.rows, a.width, cus)) * SUMS * size_t(a.width) * 4);
+    return pad256(size_t(blocks_of(a.rows, threads_of(a.width), BACKWARD_WAVES, cus)) * SUMS * size_t(a.width) * 4);
 }
 
 void launch_norm(const wc_norm_args& a, int cus, hipStream_t s) {
