@@ -397,20 +397,20 @@ __global__ __launch_bounds__(G ? 256 : MOST) void k_norm_back(wc_norm_back_args 
     }
 }
 
-// Adds the workgroups' column sums: N columns a thread, 8 threads side by side,
-// every 32nd workgroup to each of 32 rows of threads, whose sums are added in
-// order.
+// Adds the workgroups' column sums: N columns a thread (the last ones moved back
+// to end with the row), 8 threads side by side, every 32nd workgroup to each of
+// 32 rows of threads, whose sums are added in order.
 template <int N>
 __global__ __launch_bounds__(256) void k_norm_cols(const float* part, int blocks, int64_t width, ColumnSums sums) {
-    typedef float Some __attribute__((ext_vector_type(N)));
+    typedef float Some __attribute__((ext_vector_type(N), aligned(4)));
     __shared__ Some lds[32][8];
     const int x = threadIdx.x & 7, y = threadIdx.x >> 3;
     int q = 0;
     while (sums.at[q] != (int)blockIdx.y) q++;
-    const int64_t c = (int64_t(blockIdx.x) * 8 + x) * N, pitch = width * sums.wanted;
+    const int64_t c0 = (int64_t(blockIdx.x) * 8 + x) * N, c = min(c0, width - N), pitch = width * sums.wanted;
     const float* from = part + blockIdx.y * width + c;
     Some s = {};
-    if (c < width) {
+    if (c0 < width) {
         int b = y;
         for (; b + 96 < blocks; b += 128) {
             Some v[4];
@@ -422,7 +422,7 @@ __global__ __launch_bounds__(256) void k_norm_cols(const float* part, int blocks
     }
     lds[y][x] = s;
     __syncthreads();
-    if (y || c >= width) return;
+    if (y || c0 >= width) return;
     for (int k = 1; k < 32; k++) s += lds[k][x];
     *(Some*)(sums.out[q] + c) = s;
 }
@@ -446,20 +446,20 @@ Threads threads_of(int64_t width) {
     return {0, 1024, 2};
 }
 
-// Workgroups: enough to fill the device, few enough that each has several rows
-// for its parameters (and in the backward for its column sums, which are
-// written and read again).
-int blocks_of(int64_t rows, const Threads& t, int waves_per_cu, int cus) {
+// Workgroups: enough wavefronts to fill the device, and in the backward, whose
+// column sums are written and read again for each, no more than leave each
+// `turns` rows while every CU has one.
+int blocks_of(int64_t rows, const Threads& t, int64_t turns, int cus) {
     const int64_t per = t.g ? t.block / t.g : 1, want = (rows + per - 1) / per;
-    const int64_t most = int64_t(cus) * std::max(1, waves_per_cu * 64 / t.block);
-    return (int)std::max<int64_t>(1, std::min(want, most));
+    const int64_t full = int64_t(cus) * std::max(1, 16 * 64 / t.block);
+    return (int)std::max<int64_t>(1, std::min({want, full, std::max<int64_t>(cus, want / turns)}));
 }
 
-constexpr int FORWARD_WAVES = 16, BACKWARD_WAVES = 16;
+constexpr int64_t FORWARD_TURNS = 1, BACKWARD_TURNS = 8;
 
 template <class T, int G, int NV, bool NARROW = false>
 void norm_at(const wc_norm_args& a, const Threads& t, int cus, hipStream_t s) {
-    const dim3 grid(blocks_of(a.rows, t, FORWARD_WAVES, cus));
+    const dim3 grid(blocks_of(a.rows, t, FORWARD_TURNS, cus));
     const bool layer = a.norm == WC_NORM_LAYER, token = a.gate && a.gate_stride;
     if (layer && token) k_norm<T, G, NV, true, true, NARROW><<<grid, t.block, 0, s>>>(a);
     else if (layer) k_norm<T, G, NV, true, false, NARROW><<<grid, t.block, 0, s>>>(a);
@@ -492,7 +492,7 @@ void back_at(const wc_norm_back_args& a, const Threads& t, int blocks, const Col
 template <class T>
 void norm_back(const wc_norm_back_args& a, int cus, hipStream_t s) {
     const Threads t = threads_of(a.width);
-    const int blocks = blocks_of(a.rows, t, BACKWARD_WAVES, cus);
+    const int blocks = blocks_of(a.rows, t, BACKWARD_TURNS, cus);
     ColumnSums c = {{a.d_post_gain, a.d_post_bias, a.gate && !a.gate_stride ? (float*)a.d_gate : nullptr, a.d_pre_gain,
                      a.d_pre_bias}, {}, 0};
     for (int q = 0; q < SUMS; q++) c.at[q] = c.out[q] ? c.wanted++ : -1;
@@ -505,18 +505,16 @@ void norm_back(const wc_norm_back_args& a, int cus, hipStream_t s) {
     else if (t.nv == 1) back_at<T, 0, 1, 1024>(a, t, blocks, c, s);
     else back_at<T, 0, 2, 1024>(a, t, blocks, c, s);
     if (!c.wanted) return;
-    bool four = a.width % 4 == 0;
-    for (int q = 0; q < SUMS; q++) four = four && ((uintptr_t)c.out[q] & 15) == 0;
-    const int64_t n = four ? 32 : 8;
+    const int64_t n = a.width >= 4 ? 32 : 8;
     const dim3 grid((uint32_t)((a.width + n - 1) / n), c.wanted);
-    if (four) k_norm_cols<4><<<grid, 256, 0, s>>>((const float*)a.workspace, blocks, a.width, c);
+    if (n == 32) k_norm_cols<4><<<grid, 256, 0, s>>>((const float*)a.workspace, blocks, a.width, c);
     else k_norm_cols<1><<<grid, 256, 0, s>>>((const float*)a.workspace, blocks, a.width, c);
 }
 
 }  // namespace
 
 size_t norm_back_scratch(const wc_norm_back_args& a, int cus) {
-    return pad256(size_t(blocks_of(a.rows, threads_of(a.width), BACKWARD_WAVES, cus)) * SUMS * size_t(a.width) * 4);
+    return pad256(size_t(blocks_of(a.rows, threads_of(a.width), BACKWARD_TURNS, cus)) * SUMS * size_t(a.width) * 4);
 }
 
 void launch_norm(const wc_norm_args& a, int cus, hipStream_t s) {
