@@ -6,10 +6,11 @@ namespace learn {
 
 size_t policy_scratch(const wc_policy_args& a, int) {
     const size_t losses = pad256(size_t(a.rows) * sizeof(double));
-    // the size of the two-pass form, whether or not the call has a reference: the binding asks by shape
-    return holds(a.dtype, a.vocab, true) ? losses
-                                         : losses + pad256(size_t(a.rows) * sizeof(RowGrad)) +
-                                               pad256(size_t(a.rows) * splits_of(a.vocab) * sizeof(Part));
+    // the larger of both forms, with and without a reference's logits
+    if (holds(a.dtype, a.vocab, true))
+        return one_group(a.rows, lanes_of(a.vocab / (a.dtype == WC_DTYPE_F32 ? 4 : 8))) ? 0 : losses;
+    return losses + pad256(size_t(a.rows) * sizeof(RowGrad)) +
+           pad256(size_t(a.rows) * splits_of(a.vocab) * sizeof(Part));
 }
 
 size_t preference_scratch(const wc_preference_args& a, int) {

@@ -415,7 +415,7 @@ template <class T, int G, int NV, bool FULL, bool TOKEN>
 __global__ __launch_bounds__(group_block<G>(), 4) void k_rows(Rows<T> in, PolicyRow row, int64_t rows, RowGrad* grads,
                                                               const float* grad_out, T* grad, int64_t grad_stride) {
     __shared__ typename Group<G>::Slots slots;
-    __shared__ double total[G > 64 ? 1 : 1024 / G];
+    __shared__ double total[1024 / (G > 64 ? 1024 : G)];
     Group<G> group{slots};
     const int lane = threadIdx.x % G, per = G > 64 ? 1 : blockDim.x / G, n = (int)in.vocab;
     const float go = (grad_out ? *grad_out : 1.f) * in.rate.inv_temp;
@@ -457,8 +457,7 @@ __global__ __launch_bounds__(group_block<G>(), 4) void k_rows(Rows<T> in, Policy
                 } else {
                     row.kl[r] = out.y;
                     row.entropy[r] = out.z;
-                    if (gridDim.x > 1) row.losses[r] = loss;
-                    else sum += loss;
+                    sum += loss;
                 }
             }
             if (!TOKEN && grad) {
@@ -472,12 +471,18 @@ __global__ __launch_bounds__(group_block<G>(), 4) void k_rows(Rows<T> in, Policy
             }
         }
     }
-    if (!TOKEN && gridDim.x == 1) {  // one workgroup: its rows' losses, in order
-        if (lane == 0) total[threadIdx.x / G] = sum;
-        __syncthreads();
+    if constexpr (!TOKEN) {  // the workgroup's losses, in an order that does not change
+        if constexpr (G <= 64) {
+            if (lane == 0) total[threadIdx.x / G] = sum;
+            __syncthreads();
+            if (threadIdx.x >= 64) return;
+            sum = 0.0;
+            for (int k = threadIdx.x; k < per; k += 64) sum += total[k];
+            for (int mask = 32; mask; mask >>= 1) sum += __shfl_xor(sum, mask);
+        }
         if (threadIdx.x == 0) {
-            for (int k = 1; k < per; k++) sum += total[k];
-            *row.loss = (float)sum;
+            if (gridDim.x == 1) *row.loss = (float)sum;
+            else row.losses[blockIdx.x] = sum;
         }
     }
 }
@@ -539,7 +544,9 @@ __global__ void k_row_ends(Rows<T> in, PolicyRow row, int64_t rows, int splits, 
 __global__ __launch_bounds__(1024) void k_sum(const double* v, int64_t n, double scale, float* out) {
     __shared__ double lds[16];
     double s = 0;
-    for (int64_t i = threadIdx.x; i < n; i += 1024) s += v[i];
+    int64_t i = threadIdx.x;
+    for (; i + 3 * 1024 < n; i += 4 * 1024) s += (v[i] + v[i + 1024]) + (v[i + 2048] + v[i + 3072]);
+    for (; i < n; i += 1024) s += v[i];
     for (int mask = 32; mask; mask >>= 1) s += __shfl_xor(s, mask);
     if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = s;
     __syncthreads();
@@ -611,45 +618,52 @@ inline bool holds(int dtype, int64_t vocab, bool full) {
     return vocab * (dtype == WC_DTYPE_F32 ? 4 : 2) * (full ? 2 : 1) <= 256 << 10;
 }
 
+// Rows that one workgroup of up to 1,024 holds at once go to one, which then
+// sums their losses itself.
+inline bool one_group(int64_t rows, int lanes) { return rows == 1 || (lanes <= 64 && rows * lanes <= 1024); }
+
+// Lanes that hold a row of n 16-byte loads, while one wavefront does.
+inline int lanes_of(int64_t n) { return n <= 64 ? 8 : n <= 128 ? 16 : n <= 256 ? 32 : n <= 512 ? 64 : 256; }
+
+// Returns the workgroups: as many losses.
 template <class T, int G, int NV, bool FULL, bool TOKEN>
-void rows_at(const Rows<T>& in, const PolicyRow& row, int64_t rows, RowGrad* grads, const float* grad_out, T* grad,
-             int64_t grad_stride, hipStream_t s, bool* whole) {
-    // rows that one workgroup holds at once go to one, which then sums their losses itself
-    const int block = G > 64 ? G : rows * G <= 1024 ? (int)std::max<int64_t>(64, (rows * G + 63) / 64 * 64) : 256;
-    const int64_t per = block / G, grid = std::min<int64_t>((rows + per - 1) / per, 1 << 22);
-    *whole = grid == 1;
+int64_t rows_at(const Rows<T>& in, const PolicyRow& row, int64_t rows, RowGrad* grads, const float* grad_out, T* grad,
+                int64_t grad_stride, hipStream_t s) {
+    const int block = G > 64 ? G : one_group(rows, G) ? (int)((rows * G + 63) / 64 * 64) : 256;
+    const int64_t per = block / (G > 64 ? block : G), grid = std::min<int64_t>((rows + per - 1) / per, 1 << 22);
     k_rows<T, G, NV, FULL, TOKEN><<<dim3((uint32_t)grid), block, 0, s>>>(in, row, rows, grads, grad_out, grad,
                                                                          grad_stride);
+    return grid;
 }
 
 // The fewest threads that hold a row in at most eight loads each, and with the
 // least left empty: what a wavefront does once a row (the sums' butterflies,
 // the logarithms) it then does for several rows at once.
 template <class T, bool FULL, bool TOKEN>
-void rows_held(const Rows<T>& in, const PolicyRow& row, int64_t rows, RowGrad* grads, const float* go, T* grad,
-               int64_t gs, hipStream_t s, bool* whole) {
+int64_t rows_held(const Rows<T>& in, const PolicyRow& row, int64_t rows, RowGrad* grads, const float* go, T* grad,
+                  int64_t gs, hipStream_t s) {
     const int64_t n = in.vocab / EACH<T>;
-    if (n <= 8) rows_at<T, 8, 1, FULL, TOKEN>(in, row, rows, grads, go, grad, gs, s, whole);
-    else if (n <= 16) rows_at<T, 8, 2, FULL, TOKEN>(in, row, rows, grads, go, grad, gs, s, whole);
-    else if (n <= 24) rows_at<T, 8, 3, FULL, TOKEN>(in, row, rows, grads, go, grad, gs, s, whole);
-    else if (n <= 32) rows_at<T, 8, 4, FULL, TOKEN>(in, row, rows, grads, go, grad, gs, s, whole);
-    else if (n <= 48) rows_at<T, 8, 6, FULL, TOKEN>(in, row, rows, grads, go, grad, gs, s, whole);
-    else if (n <= 64) rows_at<T, 8, 8, FULL, TOKEN>(in, row, rows, grads, go, grad, gs, s, whole);
-    else if (n <= 80) rows_at<T, 16, 5, FULL, TOKEN>(in, row, rows, grads, go, grad, gs, s, whole);
-    else if (n <= 96) rows_at<T, 16, 6, FULL, TOKEN>(in, row, rows, grads, go, grad, gs, s, whole);
-    else if (n <= 128) rows_at<T, 16, 8, FULL, TOKEN>(in, row, rows, grads, go, grad, gs, s, whole);
-    else if (n <= 160) rows_at<T, 32, 5, FULL, TOKEN>(in, row, rows, grads, go, grad, gs, s, whole);
-    else if (n <= 192) rows_at<T, 32, 6, FULL, TOKEN>(in, row, rows, grads, go, grad, gs, s, whole);
-    else if (n <= 256) rows_at<T, 32, 8, FULL, TOKEN>(in, row, rows, grads, go, grad, gs, s, whole);
-    else if (n <= 320) rows_at<T, 64, 5, FULL, TOKEN>(in, row, rows, grads, go, grad, gs, s, whole);
-    else if (n <= 384) rows_at<T, 64, 6, FULL, TOKEN>(in, row, rows, grads, go, grad, gs, s, whole);
-    else if (n <= 512) rows_at<T, 64, 8, FULL, TOKEN>(in, row, rows, grads, go, grad, gs, s, whole);
-    else if (n <= 1024) rows_at<T, 256, 4, FULL, TOKEN>(in, row, rows, grads, go, grad, gs, s, whole);
-    else if (n <= 2048) rows_at<T, 256, 8, FULL, TOKEN>(in, row, rows, grads, go, grad, gs, s, whole);
-    else if (n <= 4096) rows_at<T, 512, 8, FULL, TOKEN>(in, row, rows, grads, go, grad, gs, s, whole);
-    else if constexpr (FULL) rows_at<T, 1024, 8, FULL, TOKEN>(in, row, rows, grads, go, grad, gs, s, whole);
-    else if (n <= 8192) rows_at<T, 512, 16, FULL, TOKEN>(in, row, rows, grads, go, grad, gs, s, whole);
-    else rows_at<T, 1024, 16, FULL, TOKEN>(in, row, rows, grads, go, grad, gs, s, whole);
+    if (n <= 8) return rows_at<T, 8, 1, FULL, TOKEN>(in, row, rows, grads, go, grad, gs, s);
+    if (n <= 16) return rows_at<T, 8, 2, FULL, TOKEN>(in, row, rows, grads, go, grad, gs, s);
+    if (n <= 24) return rows_at<T, 8, 3, FULL, TOKEN>(in, row, rows, grads, go, grad, gs, s);
+    if (n <= 32) return rows_at<T, 8, 4, FULL, TOKEN>(in, row, rows, grads, go, grad, gs, s);
+    if (n <= 48) return rows_at<T, 8, 6, FULL, TOKEN>(in, row, rows, grads, go, grad, gs, s);
+    if (n <= 64) return rows_at<T, 8, 8, FULL, TOKEN>(in, row, rows, grads, go, grad, gs, s);
+    if (n <= 80) return rows_at<T, 16, 5, FULL, TOKEN>(in, row, rows, grads, go, grad, gs, s);
+    if (n <= 96) return rows_at<T, 16, 6, FULL, TOKEN>(in, row, rows, grads, go, grad, gs, s);
+    if (n <= 128) return rows_at<T, 16, 8, FULL, TOKEN>(in, row, rows, grads, go, grad, gs, s);
+    if (n <= 160) return rows_at<T, 32, 5, FULL, TOKEN>(in, row, rows, grads, go, grad, gs, s);
+    if (n <= 192) return rows_at<T, 32, 6, FULL, TOKEN>(in, row, rows, grads, go, grad, gs, s);
+    if (n <= 256) return rows_at<T, 32, 8, FULL, TOKEN>(in, row, rows, grads, go, grad, gs, s);
+    if (n <= 320) return rows_at<T, 64, 5, FULL, TOKEN>(in, row, rows, grads, go, grad, gs, s);
+    if (n <= 384) return rows_at<T, 64, 6, FULL, TOKEN>(in, row, rows, grads, go, grad, gs, s);
+    if (n <= 512) return rows_at<T, 64, 8, FULL, TOKEN>(in, row, rows, grads, go, grad, gs, s);
+    if (n <= 1024) return rows_at<T, 256, 4, FULL, TOKEN>(in, row, rows, grads, go, grad, gs, s);
+    if (n <= 2048) return rows_at<T, 256, 8, FULL, TOKEN>(in, row, rows, grads, go, grad, gs, s);
+    if (n <= 4096) return rows_at<T, 512, 8, FULL, TOKEN>(in, row, rows, grads, go, grad, gs, s);
+    if constexpr (FULL) return rows_at<T, 1024, 8, FULL, TOKEN>(in, row, rows, grads, go, grad, gs, s);
+    if (n <= 8192) return rows_at<T, 512, 16, FULL, TOKEN>(in, row, rows, grads, go, grad, gs, s);
+    return rows_at<T, 1024, 16, FULL, TOKEN>(in, row, rows, grads, go, grad, gs, s);
 }
 
 template <class T, bool FULL>
@@ -658,9 +672,10 @@ void policy(const wc_policy_args& a, hipStream_t s) {
     uint8_t* w = (uint8_t*)a.workspace;
     const PolicyRow row = {a.behaviour_logp, a.advantages, a.ref_logp, a.clip_low, a.clip_high, a.kl_coef,
                            a.entropy_coef, FULL, a.logp, a.kl, a.entropy, (double*)w, a.loss};
-    bool whole = false;
+    int64_t losses = a.rows;
     if (a.rows && holds(a.dtype, a.vocab, FULL)) {
-        rows_held<T, FULL, false>(in, row, a.rows, nullptr, a.grad_out, (T*)a.grad, a.grad_stride, s, &whole);
+        losses = rows_held<T, FULL, false>(in, row, a.rows, nullptr, a.grad_out, (T*)a.grad, a.grad_stride, s);
+        if (losses == 1) return;
     } else if (a.rows) {
         const int splits = splits_of(a.vocab);
         const int64_t tiles = a.rows * splits;
@@ -672,7 +687,7 @@ void policy(const wc_policy_args& a, hipStream_t s) {
             k_row_grads<T, FULL><<<tile_grid(tiles), BLOCK, 0, s>>>(in, tiles, splits, grads, a.grad_out, (T*)a.grad,
                                                                     a.grad_stride);
     }
-    if (!whole) k_sum<<<1, 1024, 0, s>>>(row.losses, a.rows, 1.0, a.loss);
+    k_sum<<<1, 1024, 0, s>>>(row.losses, losses, 1.0, a.loss);
 }
 
 // ---------------------------------------------------------------- preference
@@ -758,8 +773,7 @@ void preference(const wc_preference_args& a, hipStream_t s) {
     PolicyRow row = {};
     row.logp = a.logp;
     if (a.rows && holds(a.dtype, a.vocab, false)) {
-        bool whole;
-        rows_held<T, false, true>(in, row, a.rows, grads, nullptr, nullptr, 0, s, &whole);
+        rows_held<T, false, true>(in, row, a.rows, grads, nullptr, nullptr, 0, s);
     } else if (a.rows) {
         Part* parts = (Part*)(w += pad256(size_t(a.pairs) * sizeof(double)));
         k_row_parts<T, false><<<tile_grid(tiles), BLOCK, 0, s>>>(in, tiles, splits, parts);

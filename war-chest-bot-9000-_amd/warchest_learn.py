@@ -71,8 +71,13 @@ def _entry(name):
     return f
 
 
+# The current stream's handle by device index, without a Stream object where torch has that (2 us a call).
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
+    lambda index: torch.cuda.current_stream(index).cuda_stream)
+
+
 def _call(name, packed, device):
-    rc = _entry(name)(packed, torch.cuda.current_stream(device).cuda_stream)
+    rc = (_fn.get(name) or _entry(name))(packed, _raw_stream(device.index))
     if rc:
         ww._check(rc)
 
@@ -105,11 +110,11 @@ def _dtype(t, name):
 
 def _matrix(t, name, device, dtype, rows, width):
     """(address, row stride) of a matrix that must be rows x width."""
-    if t.dtype != dtype:
+    if t.dtype is not dtype:
         _fail(f"{name}: {t.dtype}, expected {dtype}")
     if t.device != device:
         _fail(f"{name} is on {t.device}, not on {device}")
-    if t.dim() != 2 or t.shape[0] != rows or t.shape[1] != width:
+    if t.shape != (rows, width):
         _fail(f"{name}: shape {tuple(t.shape)}, expected ({rows}, {width})")
     s = t.stride()
     if s[1] != 1 and width > 1:
@@ -121,15 +126,15 @@ def _vector(t, name, device, dtype, n):
     """The address of a contiguous vector of n, 0 for None."""
     if t is None:
         return 0
-    if t.dtype != dtype:
+    if t.dtype is dtype and t.device == device and t.shape == (n,) and t.is_contiguous():
+        return t.data_ptr()
+    if t.dtype is not dtype:
         _fail(f"{name}: {t.dtype}, expected {dtype}")
     if t.device != device:
         _fail(f"{name} is on {t.device}, not on {device}")
-    if t.dim() != 1 or t.shape[0] != n:
+    if t.shape != (n,):
         _fail(f"{name}: shape {tuple(t.shape)}, expected ({n},)")
-    if n > 1 and t.stride(0) != 1:
-        _fail(f"{name} must be contiguous")
-    return t.data_ptr()
+    _fail(f"{name} must be contiguous")
 
 
 def _scalar(t, name, device):
@@ -195,7 +200,16 @@ def _weight_scratch(device, code, rows, width, out, act, weight_code, aligned):
 
 
 def _scratch(n, device):
-    return torch.empty(n, dtype=torch.uint8, device=device)
+    """(tensor, address) of a call's workspace; nothing is allocated for none."""
+    if not n:
+        return None, 0
+    t = torch.empty(n, dtype=torch.uint8, device=device)
+    return t, t.data_ptr()
+
+
+def _like(t):
+    """A new contiguous tensor of t's shape, type and device."""
+    return torch.empty_like(t, memory_format=torch.contiguous_format)
 
 
 def policy_loss(logits, actions, behaviour_logp, advantages, weights=None, *, legal=None, ref_logp=None, ref_logits=None,
@@ -214,21 +228,24 @@ def policy_loss(logits, actions, behaviour_logp, advantages, weights=None, *, le
     lg, lgs = (0, 0) if legal is None else _matrix(legal, "legal", device, torch.bool, rows, vocab)
     rl, rls = (0, 0) if ref_logits is None else _matrix(ref_logits, "ref_logits", device, logits.dtype, rows, vocab)
     if grad is True:
-        grad = torch.empty((rows, vocab), dtype=logits.dtype, device=device)
-    elif grad is False:
-        grad = None
-    g, gs = (0, 0) if grad is None else _matrix(grad, "grad", device, logits.dtype, rows, vocab)
+        grad = _like(logits)
+        g, gs = grad.data_ptr(), vocab
+    elif grad is False or grad is None:
+        grad, g, gs = None, 0, 0
+    else:
+        g, gs = _matrix(grad, "grad", device, logits.dtype, rows, vocab)
     loss = torch.empty((), dtype=f32, device=device)
     logp, kl, entropy = torch.empty((3, rows), dtype=f32, device=device).unbind(0)
     need = _policy_scratch(device.index, code, rows, vocab)
-    work = _scratch(need, device)
+    held, work = _scratch(need, device)
+    at = logp.data_ptr()
     _call("wc_policy_loss", _POLICY.pack(
         _POLICY.size, device.index, code, rows, vocab, x, xs, lg, lgs, rl, rls, a,
         _vector(behaviour_logp, "behaviour_logp", device, f32, rows),
         _vector(advantages, "advantages", device, f32, rows), _vector(weights, "weights", device, f32, rows),
         _vector(ref_logp, "ref_logp", device, f32, rows), _scalar(grad_out, "grad_out", device), inv_temperature,
-        clip_low, clip_high, kl_coef, entropy_coef, bits, loss.data_ptr(), logp.data_ptr(), kl.data_ptr(),
-        entropy.data_ptr(), g, gs, work.data_ptr(), need), device)
+        clip_low, clip_high, kl_coef, entropy_coef, bits, loss.data_ptr(), at, at + 4 * rows, at + 8 * rows, g, gs, work,
+        need), device)
     return PolicyLoss(loss, logp, kl, entropy, grad)
 
 
@@ -250,20 +267,23 @@ def preference_loss(logits, tokens, offsets, ref_logp, weights=None, *, beta=0.1
     if ref_logp is None:
         _fail("ref_logp is missing")
     if grad is True:
-        grad = torch.empty((rows, vocab), dtype=logits.dtype, device=device)
-    elif grad is False:
-        grad = None
-    g, gs = (0, 0) if grad is None else _matrix(grad, "grad", device, logits.dtype, rows, vocab)
+        grad = _like(logits)
+        g, gs = grad.data_ptr(), vocab
+    elif grad is False or grad is None:
+        grad, g, gs = None, 0, 0
+    else:
+        g, gs = _matrix(grad, "grad", device, logits.dtype, rows, vocab)
     loss = torch.empty((), dtype=f32, device=device)
-    margins, ratios, logp = torch.empty(3 * pairs + rows, dtype=f32, device=device).split((pairs, 2 * pairs, rows))
+    outs = torch.empty(3 * pairs + rows, dtype=f32, device=device)
+    margins, ratios, logp = outs.split((pairs, 2 * pairs, rows))
     need = _preference_scratch(device.index, code, rows, vocab, pairs)
-    work = _scratch(need, device)
+    held, work = _scratch(need, device)
+    at = outs.data_ptr()
     _call("wc_preference_loss", _PREFERENCE.pack(
         _PREFERENCE.size, device.index, code, rows, vocab, pairs, x, xs, t, off,
         _vector(ref_logp, "ref_logp", device, f32, rows), _vector(weights, "weights", device, f32, rows),
         _scalar(grad_out, "grad_out", device), inv_temperature, beta, smoothing, _known(KINDS, kind, "kind"),
-        int(bool(average)), bits, loss.data_ptr(), margins.data_ptr(), ratios.data_ptr(), logp.data_ptr(), g, gs,
-        work.data_ptr(), need), device)
+        int(bool(average)), bits, loss.data_ptr(), at, at + 4 * pairs, at + 12 * pairs, g, gs, work, need), device)
     return PreferenceLoss(loss, margins, ratios, logp, grad)
 
 
@@ -307,7 +327,7 @@ def residual_norm(block, stream, post_gain=None, post_bias=None, gate=None, pre_
     residual_norm_backward needs (stats=False: not kept)."""
     device, code, pcode, rows, width, b, s, pg, pb, g, ng, nb = _norm_inputs(block, stream, post_gain, post_bias, gate,
                                                                              pre_gain, pre_bias)
-    new, out = torch.empty((2, rows, width), dtype=block.dtype, device=device).unbind(0)
+    new, out = _like(block), _like(block)
     st = torch.empty((rows, 4), dtype=torch.float32, device=device) if stats else None
     _call("wc_residual_norm", _NORM.pack(
         _NORM.size, device.index, code, pcode, 0, rows, width, *b, *s, pg, pb, *g, ng, nb, scale, eps,
@@ -334,19 +354,19 @@ def residual_norm_backward(d_out, d_stream, block, stream, stats, post_gain=None
     if rows > 1 and stats.stride(0) != 4:
         _fail("stats must be contiguous")
     token = gate is not None and gate.dim() == 2
-    mats = torch.empty((3 if token else 2, rows, width), dtype=dt, device=device).unbind(0)
+    mats = [_like(block) for _ in range(3 if token else 2)]
     wanted = [p is not None and not (token and p is gate) for p in (post_gain, post_bias, gate, pre_gain, pre_bias)]
     sums = iter(torch.empty((sum(wanted), width), dtype=f32, device=device).unbind(0))
     dpg, dpb, dg, dng, dnb = (next(sums) if w else None for w in wanted)
     if token:
         dg = mats[2]
     need = _norm_scratch(device.index, code, rows, width)
-    work = _scratch(need, device)
+    held, work = _scratch(need, device)
     at = lambda t: 0 if t is None else t.data_ptr()  # noqa: E731
     _call("wc_residual_norm_backward", _NORM_BACK.pack(
         _NORM_BACK.size, device.index, code, pcode, 0, rows, width, *b, *s, pg, pb, *g, ng, scale,
         _known(NORMS, norm, "norm"), _known(GATE_ACTS, gate_act, "gate_act"), 0, st, *do, *ds, mats[0].data_ptr(), width,
-        mats[1].data_ptr(), width, at(dpg), at(dpb), at(dng), at(dnb), at(dg), width, work.data_ptr(), need), device)
+        mats[1].data_ptr(), width, at(dpg), at(dpb), at(dng), at(dnb), at(dg), width, work, need), device)
     return ResidualNormGrads(mats[0], mats[1], dpg, dpb, dg, dng, dnb)
 
 
@@ -422,8 +442,8 @@ def checkpoint8_weight_grad(ck, grad, *, act="none", bias=False, dtype=None):
     b = torch.empty(out, dtype=torch.float32, device=device) if bias else None
     a = _known(ACTS, act, "act")
     need = _weight_scratch(device.index, code, rows, width, out, a, wcode, (g[0] | 2 * g[1] | 2 * out) % 16 == 0)
-    work = _scratch(need, device)
+    held, work = _scratch(need, device)
     _call("wc_ckpt_weight_grad", _WEIGHT.pack(
         _WEIGHT.size, device.index, code, rows, width, out, a, wcode, *q, *e, *g, weight.data_ptr(), out,
-        b.data_ptr() if bias else 0, work.data_ptr(), need), device)
+        b.data_ptr() if bias else 0, work, need), device)
     return weight, b
