@@ -403,16 +403,22 @@ __device__ __forceinline__ float token(const Rate& k, const Part& p, float xa, R
 // ------------------------------------------------- rows that registers hold
 
 // Rows of up to a wavefront are launched with 256 threads, or all in one
-// workgroup; four wavefronts a SIMD leave the registers that the longest need.
+// workgroup. Four wavefronts a SIMD, three where a thread holds 64 registers of
+// logits, two where it holds 128: few threads with much of a row each leave
+// more of the registers to logits than many with little.
 template <int G>
 constexpr int group_block() {
     return G > 64 ? G : 1024;
+}
+template <int LOADS>
+constexpr int group_waves() {
+    return LOADS > 16 ? 2 : LOADS == 16 ? 3 : 4;
 }
 
 // A row on G threads, NV 16-byte loads of logits (FULL: and of the reference's)
 // each. TOKEN: log-probabilities and statistics only, for the preference loss.
 template <class T, int G, int NV, bool FULL, bool TOKEN>
-__global__ __launch_bounds__(group_block<G>(), 4) void k_rows(Rows<T> in, PolicyRow row, int64_t rows, RowGrad* grads,
+__global__ __launch_bounds__(group_block<G>(), (group_waves<NV * (FULL ? 2 : 1)>())) void k_rows(Rows<T> in, PolicyRow row, int64_t rows, RowGrad* grads,
                                                               const float* grad_out, T* grad, int64_t grad_stride) {
     __shared__ typename Group<G>::Slots slots;
     __shared__ double total[1024 / (G > 64 ? 1024 : G)];
@@ -540,30 +546,43 @@ __global__ void k_row_ends(Rows<T> in, PolicyRow row, int64_t rows, int splits, 
     }
 }
 
-// The sum of n losses in a fixed order.
-__global__ __launch_bounds__(1024) void k_sum(const double* v, int64_t n, double scale, float* out) {
-    __shared__ double lds[16];
+// The sum of n losses in a fixed order, by one workgroup.
+struct LossSum {
+    const double* losses;
+    int64_t n;
+    double scale;
+    float* out;
+};
+template <int THREADS>
+__device__ __forceinline__ void sum_losses(const LossSum& l) {
+    __shared__ double lds[THREADS / 64];
+    const double* v = l.losses;
     double s = 0;
     int64_t i = threadIdx.x;
-    for (; i + 3 * 1024 < n; i += 4 * 1024) s += (v[i] + v[i + 1024]) + (v[i + 2048] + v[i + 3072]);
-    for (; i < n; i += 1024) s += v[i];
+    for (; i + 3 * THREADS < l.n; i += 4 * THREADS)
+        s += (v[i] + v[i + THREADS]) + (v[i + 2 * THREADS] + v[i + 3 * THREADS]);
+    for (; i < l.n; i += THREADS) s += v[i];
     for (int mask = 32; mask; mask >>= 1) s += __shfl_xor(s, mask);
     if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = s;
     __syncthreads();
     if (threadIdx.x == 0) {
-        for (int w = 1; w < 16; w++) s += lds[w];
-        *out = (float)(s * scale);
+        for (int w = 1; w < THREADS / 64; w++) s += lds[w];
+        *l.out = (float)(s * l.scale);
     }
 }
+__global__ __launch_bounds__(1024) void k_sum(LossSum l) { sum_losses<1024>(l); }
 
 // The gradient from the rows' coefficients, a second read of the logits. The
-// last rows go first: they are what the pass before left in the caches.
+// last rows go first: they are what the pass before left in the caches. The
+// last workgroup adds the losses beside the others.
 template <class T, bool FULL>
 __global__ __launch_bounds__(BLOCK) void k_row_grads(Rows<T> in, int64_t tiles, int splits, const RowGrad* grads,
-                                                     const float* grad_out, T* out, int64_t out_stride) {
+                                                     const float* grad_out, T* out, int64_t out_stride,
+                                                     LossSum losses) {
     constexpr int NV = CHUNK_LOADS<T>;
+    if (blockIdx.x == gridDim.x - 1) return sum_losses<BLOCK>(losses);
     const float go = (grad_out ? *grad_out : 1.f) * in.rate.inv_temp;
-    for (int64_t i = blockIdx.x; i < tiles; i += gridDim.x) {
+    for (int64_t i = blockIdx.x; i < tiles; i += gridDim.x - 1) {
         const int64_t t = tiles - 1 - i, r = t / splits, c0 = (t - r * splits) * CHUNK;
         const RowGrad g = grads[r];
         T* to = out + r * out_stride + c0;
@@ -613,7 +632,7 @@ inline int splits_of(int64_t vocab) { return (int)((vocab + CHUNK - 1) / CHUNK);
 
 inline uint32_t tile_grid(int64_t tiles) { return (uint32_t)std::min<int64_t>(tiles, 1 << 22); }
 
-// Whether k_rows holds a row: up to 64 registers per thread of 1,024.
+// Whether k_rows holds a row: up to 128 registers per thread of 512.
 inline bool holds(int dtype, int64_t vocab, bool full) {
     return vocab * (dtype == WC_DTYPE_F32 ? 4 : 2) * (full ? 2 : 1) <= 256 << 10;
 }
@@ -660,10 +679,18 @@ int64_t rows_held(const Rows<T>& in, const PolicyRow& row, int64_t rows, RowGrad
     if (n <= 512) return rows_at<T, 64, 8, FULL, TOKEN>(in, row, rows, grads, go, grad, gs, s);
     if (n <= 1024) return rows_at<T, 256, 4, FULL, TOKEN>(in, row, rows, grads, go, grad, gs, s);
     if (n <= 2048) return rows_at<T, 256, 8, FULL, TOKEN>(in, row, rows, grads, go, grad, gs, s);
-    if (n <= 4096) return rows_at<T, 512, 8, FULL, TOKEN>(in, row, rows, grads, go, grad, gs, s);
-    if constexpr (FULL) return rows_at<T, 1024, 8, FULL, TOKEN>(in, row, rows, grads, go, grad, gs, s);
-    if (n <= 8192) return rows_at<T, 512, 16, FULL, TOKEN>(in, row, rows, grads, go, grad, gs, s);
-    return rows_at<T, 1024, 16, FULL, TOKEN>(in, row, rows, grads, go, grad, gs, s);
+    if constexpr (TOKEN) {  // no gradient to write: more threads, with less each, load faster
+        if (n <= 4096) return rows_at<T, 512, 8, FULL, TOKEN>(in, row, rows, grads, go, grad, gs, s);
+        if (n <= 8192) return rows_at<T, 512, 16, FULL, TOKEN>(in, row, rows, grads, go, grad, gs, s);
+        return rows_at<T, 512, 32, FULL, TOKEN>(in, row, rows, grads, go, grad, gs, s);
+    } else if constexpr (FULL) {
+        if (n <= 4096) return rows_at<T, 256, 16, FULL, TOKEN>(in, row, rows, grads, go, grad, gs, s);
+        return rows_at<T, 512, 16, FULL, TOKEN>(in, row, rows, grads, go, grad, gs, s);
+    } else {
+        if (n <= 4096) return rows_at<T, 256, 16, FULL, TOKEN>(in, row, rows, grads, go, grad, gs, s);
+        if (n <= 8192) return rows_at<T, 256, 32, FULL, TOKEN>(in, row, rows, grads, go, grad, gs, s);
+        return rows_at<T, 512, 32, FULL, TOKEN>(in, row, rows, grads, go, grad, gs, s);
+    }
 }
 
 template <class T, bool FULL>
@@ -683,11 +710,13 @@ void policy(const wc_policy_args& a, hipStream_t s) {
         Part* parts = (Part*)(w += pad256(size_t(a.rows) * sizeof(RowGrad)));
         k_row_parts<T, FULL><<<tile_grid(tiles), BLOCK, 0, s>>>(in, tiles, splits, parts);
         k_row_ends<T, false><<<dim3((uint32_t)((a.rows + 63) / 64)), 64, 0, s>>>(in, row, a.rows, splits, parts, grads);
-        if (a.grad)
-            k_row_grads<T, FULL><<<tile_grid(tiles), BLOCK, 0, s>>>(in, tiles, splits, grads, a.grad_out, (T*)a.grad,
-                                                                    a.grad_stride);
+        if (a.grad) {
+            k_row_grads<T, FULL><<<tile_grid(tiles) + 1, BLOCK, 0, s>>>(in, tiles, splits, grads, a.grad_out, (T*)a.grad,
+                                                                        a.grad_stride, {row.losses, losses, 1.0, a.loss});
+            return;
+        }
     }
-    k_sum<<<1, 1024, 0, s>>>(row.losses, losses, 1.0, a.loss);
+    k_sum<<<1, 1024, 0, s>>>({row.losses, losses, 1.0, a.loss});
 }
 
 // ---------------------------------------------------------------- preference
@@ -782,10 +811,12 @@ void preference(const wc_preference_args& a, hipStream_t s) {
     const Pairs p = {a.offsets, a.ref_logp, a.weights, a.rows, a.pairs, a.beta, a.smoothing, a.kind, a.average,
                      a.index_bits};
     if (a.pairs) k_pairs<<<dim3((uint32_t)a.pairs), BLOCK, 0, s>>>(p, a.logp, grads, losses, a.margins, a.ratios);
-    k_sum<<<1, 1024, 0, s>>>(losses, a.pairs, a.pairs ? 1.0 / (double)a.pairs : 0.0, a.loss);
+    const LossSum sum = {losses, a.pairs, a.pairs ? 1.0 / (double)a.pairs : 0.0, a.loss};
     if (a.grad && a.rows)
-        k_row_grads<T, false><<<tile_grid(tiles), BLOCK, 0, s>>>(in, tiles, splits, grads, a.grad_out, (T*)a.grad,
-                                                                 a.grad_stride);
+        k_row_grads<T, false><<<tile_grid(tiles) + 1, BLOCK, 0, s>>>(in, tiles, splits, grads, a.grad_out, (T*)a.grad,
+                                                                     a.grad_stride, sum);
+    else
+        k_sum<<<1, 1024, 0, s>>>(sum);
 }
 
 template <class T>
