@@ -1,0 +1,80 @@
+"""The training operators under torch's automatic differentiation, and the training example end to end."""
+import pytest
+import torch
+
+import learn_ref as R
+import train_policy
+import warchest_learn as wl
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+
+
+def close(got, want, what, bound):
+    off = float((got.double().cpu() - want.double().cpu()).abs().max())
+    assert off <= bound * max(1.0, float(want.abs().max())), (what, off)
+
+
+def test_objectives_scale_with_what_arrives_and_may_run_backward_twice():
+    """Gradients of 3 times the loss, twice over one graph, against the call's own gradient (the same float32 sums: 1e-6)."""
+    g = torch.Generator(device=DEV).manual_seed(1)
+    x = torch.randn(40, 30, generator=g, device=DEV, requires_grad=True)
+    a = torch.randint(0, 30, (40,), generator=g, device=DEV)
+    v = torch.randn(40, generator=g, device=DEV)
+    b = torch.log_softmax(x.detach(), 1).gather(1, a[:, None])[:, 0].contiguous()
+    loss, *_ = wl.policy_objective(x, a, b, v, ref_logits=torch.zeros_like(x), kl_coef=0.2)
+    want = wl.policy_loss(x.detach(), a, b, v, ref_logits=torch.zeros(40, 30, device=DEV), kl_coef=0.2)
+    (3 * loss).backward(retain_graph=True)
+    close(x.grad, 3 * want.grad, "policy", 1e-6)
+    (3 * loss).backward()
+    close(x.grad, 6 * want.grad, "policy twice", 2e-6)
+    x.grad = None
+    offsets = torch.tensor([0, 10, 20, 25, 40], device=DEV)
+    loss, *_ = wl.preference_objective(x, a, offsets, b, beta=0.4)
+    (2 * loss).backward()
+    close(x.grad, 2 * wl.preference_loss(x.detach(), a, offsets, b, beta=0.4).grad, "preference", 1e-6)
+
+
+@pytest.mark.parametrize("norm,gate_act", [("layer", "none"), ("rms", "sigmoid")])
+def test_residual_norm_module_against_float64(norm, gate_act):
+    """As the operator's own test: 2e-5 of the largest for float32."""
+    m = wl.ResidualNorm(72, norm=norm, gate_act=gate_act, scale=0.3, device=DEV)
+    g = torch.Generator(device=DEV).manual_seed(2)
+    with torch.no_grad():
+        for p in m.parameters():
+            p.add_(0.1 * torch.randn(p.shape, generator=g, device=DEV))
+    u, x, d1, d2 = (torch.randn(33, 72, generator=g, device=DEV) for _ in range(4))
+    u.requires_grad_(True)
+    x.requires_grad_(True)
+    torch.autograd.backward(m(u, x), [d1, d2])
+    v = {n: None if t is None else t.detach().cpu().double().requires_grad_(True) for n, t in (
+        ("block", u), ("stream", x), ("post_gain", m.post_gain), ("post_bias", m.post_bias), ("gate", m.gate),
+        ("pre_gain", m.pre_gain), ("pre_bias", m.pre_bias))}
+    torch.autograd.backward(R.residual_norm(**v, **m.kw), [d1.cpu().double(), d2.cpu().double()])
+    close(u.grad, v["block"].grad, "block", 2e-5)
+    close(x.grad, v["stream"].grad, "stream", 2e-5)
+    for n, p in m.named_parameters():
+        close(p.grad, v[n].grad, n, 2e-5 * 33 ** 0.5)
+
+
+def test_act_linear8_against_float64():
+    """Forward from the unrounded input; the gradients from what the 8 bits stand for. bf16 outputs: 2^-8 of the value
+    and of what is summed."""
+    g = torch.Generator(device=DEV).manual_seed(3)
+    z = torch.randn(130, 96, generator=g, device=DEV).bfloat16().requires_grad_(True)
+    w = (0.1 * torch.randn(96, 40, generator=g, device=DEV)).bfloat16().requires_grad_(True)
+    d = torch.randn(130, 40, generator=g, device=DEV).bfloat16()
+    y = wl.act_linear8(z, w, "gelu")
+    y.backward(d)
+    close(y.detach(), R.act(z.detach().cpu().double(), "gelu") @ w.detach().cpu().double(), "y", 2.0 ** -7)
+    kept = R.keep8(z.detach().cpu())[2].requires_grad_(True)
+    da = d.cpu().double() @ w.detach().cpu().double().t()
+    R.act(kept, "gelu").backward(da)
+    close(z.grad, kept.grad, "z", 2.0 ** -6)
+    close(w.grad, R.act(kept.detach(), "gelu").t() @ d.cpu().double(), "w", 2.0 ** -7)
+
+
+def test_the_training_example_learns_the_search_policy():
+    first, last, pref, pref_last = train_policy.train(trees=2, steps=40, width=128, blocks=2)
+    assert last < 0.5 * first
+    assert pref_last < 0.8 * pref

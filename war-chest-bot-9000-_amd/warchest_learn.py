@@ -447,3 +447,108 @@ def checkpoint8_weight_grad(ck, grad, *, act="none", bias=False, dtype=None):
         _WEIGHT.size, device.index, code, rows, width, out, a, wcode, *q, *e, *g, weight.data_ptr(), out,
         b.data_ptr() if bias else 0, work, need), device)
     return weight, b
+
+
+# ------------------------------------------------------- automatic differentiation
+
+def _upstream(g):
+    return g if g.dtype is torch.float32 else g.float()
+
+
+class _PolicyObjective(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, rows, kw):
+        r = policy_loss(logits, *rows, grad=False, **kw)
+        ctx.save_for_backward(logits)
+        ctx.call = rows, kw
+        ctx.mark_non_differentiable(r.logp, r.kl, r.entropy)
+        return r.loss, r.logp, r.kl, r.entropy
+
+    @staticmethod
+    def backward(ctx, d_loss, *_):
+        rows, kw = ctx.call
+        return policy_loss(ctx.saved_tensors[0], *rows, grad_out=_upstream(d_loss), **kw).grad, None, None
+
+
+def policy_objective(logits, actions, behaviour_logp, advantages, weights=None, **kw):
+    """policy_loss as a differentiable function of the logits: (loss, logp, kl, entropy). The backward pass reads the
+    logits again instead of keeping a gradient."""
+    return _PolicyObjective.apply(logits, (actions, behaviour_logp, advantages, weights), kw)
+
+
+class _PreferenceObjective(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, rows, kw):
+        r = preference_loss(logits, *rows, grad=False, **kw)
+        ctx.save_for_backward(logits)
+        ctx.call = rows, kw
+        ctx.mark_non_differentiable(r.margins, r.ratios)
+        return r.loss, r.margins, r.ratios
+
+    @staticmethod
+    def backward(ctx, d_loss, *_):
+        rows, kw = ctx.call
+        return preference_loss(ctx.saved_tensors[0], *rows, grad_out=_upstream(d_loss), **kw).grad, None, None
+
+
+def preference_objective(logits, tokens, offsets, ref_logp, weights=None, **kw):
+    """preference_loss as a differentiable function of the logits: (loss, margins, ratios)."""
+    return _PreferenceObjective.apply(logits, (tokens, offsets, ref_logp, weights), kw)
+
+
+class _ResidualNorm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, block, stream, post_gain, post_bias, gate, pre_gain, pre_bias, kw):
+        r = residual_norm(block, stream, post_gain, post_bias, gate, pre_gain, pre_bias, **kw)
+        ctx.save_for_backward(block, stream, r.stats, post_gain, post_bias, gate, pre_gain, pre_bias)
+        ctx.kw = kw
+        return r.stream, r.out
+
+    @staticmethod
+    def backward(ctx, d_stream, d_out):
+        saved = ctx.saved_tensors
+        g = residual_norm_backward(d_out.contiguous(), d_stream.contiguous(), *saved, **ctx.kw)
+        cast = [d if d is None else d.to(p.dtype) for d, p in zip(g[2:], saved[3:])]
+        return (g.block, g.stream, *cast, None)
+
+
+class ResidualNorm(torch.nn.Module):
+    """The residual update between two norms, with its parameters: (stream', out) of (block, stream)."""
+
+    def __init__(self, width, norm="layer", gate=True, gate_act="none", scale=1.0, eps=1e-5, device=None,
+                 dtype=torch.float32):
+        super().__init__()
+        make = lambda v: torch.nn.Parameter(torch.full((width,), v, device=device, dtype=dtype))  # noqa: E731
+        self.post_gain, self.pre_gain = make(1.0), make(1.0)
+        self.post_bias, self.pre_bias = (make(0.0), make(0.0)) if norm == "layer" else (None, None)
+        self.gate = make(1.0 if gate_act == "none" else 0.0) if gate else None
+        self.kw = {"norm": norm, "gate_act": gate_act, "scale": scale, "eps": eps}
+
+    def forward(self, block, stream, gate=None):
+        return _ResidualNorm.apply(block, stream, self.post_gain, self.post_bias, self.gate if gate is None else gate,
+                                   self.pre_gain, self.pre_bias, self.kw)
+
+
+class _ActLinear8(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, z, weight, act):
+        kept, a = checkpoint8_act(z, act)
+        ctx.save_for_backward(kept.q, kept.exps, weight)
+        ctx.act = act
+        return a @ weight
+
+    @staticmethod
+    def backward(ctx, d):
+        q, exps, weight = ctx.saved_tensors
+        kept, d = Checkpoint8(q, exps), d.contiguous()
+        d_z = checkpoint8_act_backward(kept, d @ weight.t(), ctx.act) if ctx.needs_input_grad[0] else None
+        d_w = None
+        if ctx.needs_input_grad[1]:
+            d_w = checkpoint8_weight_grad(kept, d, act=ctx.act, dtype=weight.dtype)[0]
+        return d_z, d_w, None
+
+
+def act_linear8(z, weight, act="gelu"):
+    """act(z) @ weight (z [rows, width], weight [width, out] of one type), keeping z for the backward pass in 8 bits and
+    act(z) not at all: its slope and the weight's gradient are taken from the 8-bit form."""
+    return _ActLinear8.apply(z, weight, act)
