@@ -89,20 +89,20 @@ struct RowSum {
     }
 };
 
-// act(g), and its slope in *d.
-__device__ __forceinline__ float gate_of(float g, int act, float* d) {
+// Eight gate values through their function, chosen once for all.
+__device__ __forceinline__ void gates(float (&w)[8], int act) {
     if (act == WC_GATE_SIGMOID) {
-        const float s = __builtin_amdgcn_rcpf(1.f + fast_exp(-g));
-        *d = s * (1.f - s);
-        return s;
+#pragma unroll
+        for (int i = 0; i < 8; i++) w[i] = __builtin_amdgcn_rcpf(1.f + fast_exp(-w[i]));
+    } else if (act == WC_GATE_TANH) {
+#pragma unroll
+        for (int i = 0; i < 8; i++) w[i] = tanhf(w[i]);
     }
-    if (act == WC_GATE_TANH) {
-        const float t = tanhf(g);
-        *d = 1.f - t * t;
-        return t;
-    }
-    *d = 1.f;
-    return g;
+}
+
+// The function's slope from its value.
+__device__ __forceinline__ float gate_slope(float w, int act) {
+    return act == WC_GATE_SIGMOID ? w * (1.f - w) : act == WC_GATE_TANH ? 1.f - w * w : 1.f;
 }
 
 // How a workgroup's threads hold rows: G lanes a row, or with G 0 all of them,
@@ -166,12 +166,11 @@ __device__ __forceinline__ void fold(const A& a, bool token, int col, int n, flo
     load_param<NARROW>(a.post_gain, a.param_dtype, col, n, 1.f, gain);
     load_param<NARROW>(a.post_bias, a.param_dtype, col, n, 0.f, bias);
     load_param<NARROW>(token ? nullptr : a.gate, a.param_dtype, col, n, 1.f, g);
+    if (a.gate && !token) gates(g, a.gate_act);
 #pragma unroll
     for (int i = 0; i < 8; i++) {
-        float slope;
-        const float f = a.scale * (a.gate && !token ? gate_of(g[i], a.gate_act, &slope) : 1.f);
-        gain[i] *= f;
-        bias[i] *= f;
+        gain[i] *= a.scale * g[i];
+        bias[i] *= a.scale * g[i];
     }
 }
 
@@ -216,12 +215,12 @@ __global__ __launch_bounds__(G ? 256 : 1024) void k_norm(wc_norm_args a) {
         const float2 s1 = row_stats<G, NV, LAYER>(u, at, width, a.eps, sum);
 #pragma unroll
         for (int k = 0; k < NV; k++) {
+            float w[8];
 #pragma unroll
-            for (int i = 0; i < 8; i++) {
-                float w = 1.f, slope;
-                if (TOKEN) w = gate_of((float)g[k][i], a.gate_act, &slope);
-                x[k][i] += w * ((u[k][i] - s1.x) * s1.y * g1[k][i] + b1[k][i]);
-            }
+            for (int i = 0; i < 8; i++) w[i] = TOKEN ? (float)g[TOKEN ? k : 0][i] : 1.f;
+            if (TOKEN) gates(w, a.gate_act);
+#pragma unroll
+            for (int i = 0; i < 8; i++) x[k][i] += w[i] * ((u[k][i] - s1.x) * s1.y * g1[k][i] + b1[k][i]);
             if (here && at.holds(k)) put8<T, NARROW>((T*)a.new_stream + r * a.new_stream_stride + at.col[k], at.n, x[k]);
         }
         const float2 s2 = row_stats<G, NV, LAYER>(x, at, width, a.eps, sum);
@@ -250,19 +249,35 @@ struct ColumnSums {
 // stays out of the sums: the gate vector's gradient is of the same two.
 // MOST: threads of the widest workgroup; 512 leave a thread the registers that it needs.
 template <class T, int G, int NV, bool LAYER, bool TOKEN, bool NARROW, int MOST>
-__global__ __launch_bounds__(G ? 256 : MOST) void k_norm_back(wc_norm_back_args a, ColumnSums sums, float* part) {
+__global__ __launch_bounds__(G ? 256 : MOST, MOST == 1024 ? 4 : TOKEN ? 2 : 3) void k_norm_back(wc_norm_back_args a, ColumnSums sums, float* part) {
     typedef typename Vec8<T>::type Raw;
     __shared__ float2 lds[2 * MOST_WAVES];
     __shared__ float cols[G ? G * NV * 8 : 1];
     const Layout<G, NV, NARROW> at((int)a.width);
     RowSum<G> sum{lds, (int)blockDim.x / 64};
     const float width = (float)(int)a.width;
+    // Workgroups of 1,024 have 128 registers a thread: there the parameters wait
+    // in LDS, each thread's own, and are read as a row needs them.
+    constexpr bool STAGED = MOST == 1024 && NV == 1;
+    __shared__ float4 stage[STAGED ? 6 * MOST : 1];
     float g1[NV][8], b1[NV][8], g2[NV][8], acc[4][NV][8] = {};
 #pragma unroll
     for (int k = 0; k < NV; k++) {
         fold<NARROW>(a, TOKEN, at.col[k], at.n, g1[k], b1[k]);
         load_param<NARROW>(a.pre_gain, a.param_dtype, at.col[k], at.n, 1.f, g2[k]);
     }
+    auto staged = [&](int q, float (&v)[8], bool put) {
+        float4* to = stage + 2 * q * MOST + threadIdx.x;
+        if (put) {
+            to[0] = make_float4(v[0], v[1], v[2], v[3]);
+            to[MOST] = make_float4(v[4], v[5], v[6], v[7]);
+        } else {
+            asm volatile("" ::: "memory");  // read here, not held from the row before
+            const float4 lo = to[0], hi = to[MOST];
+            v[0] = lo.x, v[1] = lo.y, v[2] = lo.z, v[3] = lo.w, v[4] = hi.x, v[5] = hi.y, v[6] = hi.z, v[7] = hi.w;
+        }
+    };
+    if constexpr (STAGED) staged(0, g1[0], true), staged(1, b1[0], true), staged(2, g2[0], true);
     const int64_t stride = int64_t(gridDim.x) * at.per;
     Raw ru[NV], rx[NV], rh[NV], rd[NV], rg[TOKEN ? NV : 1];
     float4 rs;
@@ -286,19 +301,20 @@ __global__ __launch_bounds__(G ? 256 : MOST) void k_norm_back(wc_norm_back_args 
         const bool here = r < a.rows;
         const float4 st = rs;
         // the block's norm, and the stream's after the update, as the forward computed them
-        float uh[NV][8], xh[NV][8], dx[NV][8];
-        Raw d[NV], g[TOKEN ? NV : 1];
+        float uh[NV][8], xh[NV][8], dx[NV][8], w[NV][8];
+        Raw d[NV];
         float s1 = 0.f, s2 = 0.f;
 #pragma unroll
         for (int k = 0; k < NV; k++) {
             d[k] = rd[k];
-            if (TOKEN) g[k] = rg[k];
+#pragma unroll
+            for (int i = 0; i < 8; i++) w[k][i] = TOKEN ? (float)rg[TOKEN ? k : 0][i] : 1.f;
+            if (TOKEN) gates(w[k], a.gate_act);
+            if constexpr (STAGED) staged(0, g1[k], false), staged(1, b1[k], false), staged(2, g2[k], false);
 #pragma unroll
             for (int i = 0; i < 8; i++) {
-                float w = 1.f, slope;
-                if (TOKEN) w = gate_of((float)g[k][i], a.gate_act, &slope);
                 uh[k][i] = ((float)ru[k][i] - st.x) * st.y;
-                const float x = (float)rx[k][i] + w * (uh[k][i] * g1[k][i] + b1[k][i]);
+                const float x = (float)rx[k][i] + w[k][i] * (uh[k][i] * g1[k][i] + b1[k][i]);
                 xh[k][i] = (x - st.z) * st.w;
                 const float dh = here ? (float)rh[k][i] : 0.f;
                 acc[2][k][i] += dh * xh[k][i];
@@ -316,17 +332,16 @@ __global__ __launch_bounds__(G ? 256 : MOST) void k_norm_back(wc_norm_back_args 
 #pragma unroll
         for (int k = 0; k < NV; k++) {
             float o[8], dg[8];
+            if constexpr (STAGED) {
+                staged(0, g1[k], false);
+                if (TOKEN) staged(1, b1[k], false);
+            }
 #pragma unroll
             for (int i = 0; i < 8; i++) {
                 const float v = st.w * (dx[k][i] - c1 - xh[k][i] * c2) + (float)d[k][i];
                 o[i] = v;
-                float wv = v;
-                if (TOKEN) {
-                    float slope;
-                    wv = gate_of((float)g[k][i], a.gate_act, &slope) * v;
-                    dg[i] = slope * v * (uh[k][i] * g1[k][i] + b1[k][i]);
-                }
-                if (!here) wv = 0.f;
+                const float wv = here ? w[k][i] * v : 0.f;
+                if (TOKEN) dg[i] = gate_slope(w[k][i], a.gate_act) * v * (uh[k][i] * g1[k][i] + b1[k][i]);
                 acc[0][k][i] += wv * uh[k][i];
                 acc[1][k][i] += wv;
                 dx[k][i] = wv * g1[k][i];
@@ -362,13 +377,13 @@ __global__ __launch_bounds__(G ? 256 : MOST) void k_norm_back(wc_norm_back_args 
                 load_param<NARROW>(a.post_gain, a.param_dtype, at.col[k], at.n, 1.f, gain);
                 load_param<NARROW>(a.post_bias, a.param_dtype, at.col[k], at.n, 0.f, bias);
                 load_param<NARROW>(TOKEN ? nullptr : a.gate, a.param_dtype, at.col[k], at.n, 1.f, gate);
+                if (!TOKEN && a.gate) gates(gate, a.gate_act);
             }
 #pragma unroll
             for (int i = 0; i < 8; i++) {
-                float w = 1.f, slope = 1.f;
-                if (q < 3 && !TOKEN && a.gate) w = gate_of(gate[i], a.gate_act, &slope);
-                if (q < 2) v[k][i] = a.scale * w * acc[q][k][i];
-                else if (q == 2) v[k][i] = a.scale * slope * (gain[i] * acc[0][k][i] + bias[i] * acc[1][k][i]);
+                if (q < 2) v[k][i] = a.scale * gate[i] * acc[q][k][i];
+                else if (q == 2)
+                    v[k][i] = a.scale * gate_slope(gate[i], a.gate_act) * (gain[i] * acc[0][k][i] + bias[i] * acc[1][k][i]);
                 else v[k][i] = acc[q - 1][k][i];
             }
         }
@@ -446,20 +461,21 @@ Threads threads_of(int64_t width) {
     return {0, 1024, 2};
 }
 
-// Workgroups: enough wavefronts to fill the device, and in the backward, whose
-// column sums are written and read again for each, no more than leave each
-// `turns` rows while every CU has one.
-int blocks_of(int64_t rows, const Threads& t, int64_t turns, int cus) {
+// Workgroups: as many as the device holds at once (its registers hold `waves`
+// wavefronts a CU), and in the backward, whose column sums are written and read
+// again for each, no more than leave each `turns` rows while every CU has one.
+int blocks_of(int64_t rows, const Threads& t, int waves, int64_t turns, int cus) {
     const int64_t per = t.g ? t.block / t.g : 1, want = (rows + per - 1) / per;
-    const int64_t full = int64_t(cus) * std::max(1, 16 * 64 / t.block);
+    const int64_t full = int64_t(cus) * std::max(1, waves * 64 / t.block);
     return (int)std::max<int64_t>(1, std::min({want, full, std::max<int64_t>(cus, want / turns)}));
 }
 
+constexpr int FORWARD_WAVES = 16, BACKWARD_WAVES = 12, BACKWARD_TOKEN_WAVES = 8;
 constexpr int64_t FORWARD_TURNS = 1, BACKWARD_TURNS = 8;
 
 template <class T, int G, int NV, bool NARROW = false>
 void norm_at(const wc_norm_args& a, const Threads& t, int cus, hipStream_t s) {
-    const dim3 grid(blocks_of(a.rows, t, FORWARD_TURNS, cus));
+    const dim3 grid(blocks_of(a.rows, t, FORWARD_WAVES, FORWARD_TURNS, cus));
     const bool layer = a.norm == WC_NORM_LAYER, token = a.gate && a.gate_stride;
     if (layer && token) k_norm<T, G, NV, true, true, NARROW><<<grid, t.block, 0, s>>>(a);
     else if (layer) k_norm<T, G, NV, true, false, NARROW><<<grid, t.block, 0, s>>>(a);
@@ -489,10 +505,15 @@ void back_at(const wc_norm_back_args& a, const Threads& t, int blocks, const Col
     else k_norm_back<T, G, NV, false, false, NARROW, MOST><<<dim3(blocks), t.block, 0, s>>>(a, c, w);
 }
 
+int back_blocks(const wc_norm_back_args& a, const Threads& t, int cus) {
+    const int waves = a.gate && a.gate_stride ? BACKWARD_TOKEN_WAVES : BACKWARD_WAVES;
+    return blocks_of(a.rows, t, waves, BACKWARD_TURNS, cus);
+}
+
 template <class T>
 void norm_back(const wc_norm_back_args& a, int cus, hipStream_t s) {
     const Threads t = threads_of(a.width);
-    const int blocks = blocks_of(a.rows, t, BACKWARD_TURNS, cus);
+    const int blocks = back_blocks(a, t, cus);
     ColumnSums c = {{a.d_post_gain, a.d_post_bias, a.gate && !a.gate_stride ? (float*)a.d_gate : nullptr, a.d_pre_gain,
                      a.d_pre_bias}, {}, 0};
     for (int q = 0; q < SUMS; q++) c.at[q] = c.out[q] ? c.wanted++ : -1;
@@ -514,7 +535,9 @@ void norm_back(const wc_norm_back_args& a, int cus, hipStream_t s) {
 }  // namespace
 
 size_t norm_back_scratch(const wc_norm_back_args& a, int cus) {
-    return pad256(size_t(blocks_of(a.rows, threads_of(a.width), BACKWARD_TURNS, cus)) * SUMS * size_t(a.width) * 4);
+    // with or without a gate of the rows' own: the binding asks by shape
+    const size_t blocks = blocks_of(a.rows, threads_of(a.width), BACKWARD_WAVES, BACKWARD_TURNS, cus);
+    return pad256(blocks * SUMS * size_t(a.width) * 4);
 }
 
 void launch_norm(const wc_norm_args& a, int cus, hipStream_t s) {
