@@ -645,3 +645,31 @@ def test_refusals_of_the_binding():
         with pytest.raises(ww.WaveError):
             call()
     torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("width", [24, 65, 513, 1025, 4097, 9001])
+def test_residual_norm_in_place(width):
+    """The new stream over the old one, and the stream's gradient over what arrived, through the C ABI: the same bits as
+    apart. At 513, 1025 and 4097 columns the last chunk's first columns are another wavefront's too."""
+    say(f"case norm in place: 2000 x {width}")
+    k, d = norm_inputs(2000, width, torch.bfloat16, width, "layer", "vector")
+    v = {n: to(t) for n, t in k.items()}
+    f = wl.residual_norm(**v)
+    b = wl.residual_norm_backward(to(d[0]), to(d[1]), v["block"], v["stream"], f.stats, *(
+        v[n] for n in ("post_gain", "post_bias", "gate", "pre_gain", "pre_bias")))
+    p = [v[n].data_ptr() for n in ("post_gain", "post_bias", "gate")]
+    q = [v[n].data_ptr() for n in ("pre_gain", "pre_bias")]
+    x, out = v["stream"].clone(), torch.empty_like(v["stream"])
+    wl._call("wc_residual_norm", wl._NORM.pack(
+        wl._NORM.size, 0, 2, 2, 0, 2000, width, v["block"].data_ptr(), width, x.data_ptr(), width, *p, 0, *q, 1.0, 1e-5, 1, 0,
+        x.data_ptr(), width, out.data_ptr(), width, 0), x.device)
+    assert torch.equal(x, f.stream) and torch.equal(out, f.out)
+    g, block = to(d[1]), torch.empty_like(x)
+    need = wl._norm_scratch(0, 2, 2000, width)
+    work = torch.empty(need, dtype=torch.uint8, device=DEV)
+    d_out = to(d[0])
+    wl._call("wc_residual_norm_backward", wl._NORM_BACK.pack(
+        wl._NORM_BACK.size, 0, 2, 2, 0, 2000, width, v["block"].data_ptr(), width, v["stream"].data_ptr(), width, *p, 0, q[0],
+        1.0, 1, 0, 0, f.stats.data_ptr(), d_out.data_ptr(), width, g.data_ptr(), width, block.data_ptr(), width,
+        g.data_ptr(), width, 0, 0, 0, 0, 0, 0, work.data_ptr(), need), x.device)
+    assert torch.equal(g, b.stream) and torch.equal(block, b.block)

@@ -60,6 +60,25 @@ __device__ __forceinline__ float power(float x) { return __builtin_amdgcn_exp2f(
 // less than a millionth.
 __device__ __forceinline__ float fast_exp(float x) { return power(x * 1.4426950408889634f); }
 
+// Waits for a load: its value is asked for here. Used before a barrier after
+// which another wavefront may write where it came from (outputs that may be
+// their inputs).
+__device__ __forceinline__ void settle(float& v) { asm volatile("" : "+v"(v)); }
+template <class V>
+__device__ __forceinline__ void settle(V& v) {
+    typedef uint32_t Words __attribute__((ext_vector_type(sizeof(V) / 4)));
+    Words w = __builtin_bit_cast(Words, v);
+    if constexpr (sizeof(V) == 32) {  // as two operands of four registers
+        typedef uint32_t Four __attribute__((ext_vector_type(4)));
+        Four lo = __builtin_shufflevector(w, w, 0, 1, 2, 3), hi = __builtin_shufflevector(w, w, 4, 5, 6, 7);
+        asm volatile("" : "+v"(lo), "+v"(hi));
+        w = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+    } else {
+        asm volatile("" : "+v"(w));
+    }
+    v = __builtin_bit_cast(V, w);
+}
+
 __device__ __forceinline__ int64_t index_at(const void* p, int bits, int64_t i) {
     return bits == 64 ? ((const int64_t*)p)[i] : (int64_t)((const int32_t*)p)[i];
 }

@@ -435,10 +435,12 @@ __global__ __launch_bounds__(group_block<G>(), (group_waves<NV * (FULL ? 2 : 1)>
         PolicyRow::Terms terms = {};
         if (head.read) {
             const uint8_t* legal = in.legal ? in.legal + r * in.legal_stride : nullptr;
-            x.load(in.x + r * in.x_stride, legal, n, lane);
-            if constexpr (FULL) y.load(in.y + r * in.y_stride, legal, n, lane);
             if constexpr (TOKEN) terms.xa = (float)in.x[r * in.x_stride + head.a];
             else terms = row.terms(in, r, head);
+            x.load(in.x + r * in.x_stride, legal, n, lane);
+            if constexpr (FULL) y.load(in.y + r * in.y_stride, legal, n, lane);
+            // every wavefront reads the action's logit, and one writes its gradient, perhaps there
+            if (G > 64) settle(terms.xa);
         } else {
             x.none();
             if constexpr (FULL) y.none();

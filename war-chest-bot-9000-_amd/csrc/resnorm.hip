@@ -206,6 +206,8 @@ __global__ __launch_bounds__(G ? 256 : 1024) void k_norm(wc_norm_args a) {
         Raw g[TOKEN ? NV : 1];
 #pragma unroll
         for (int k = 0; k < NV; k++) {
+            // a chunk moved back may be read here and written, as the next thread's, by another wavefront
+            if (G == 0) settle(rx[k]);
 #pragma unroll
             for (int i = 0; i < 8; i++) u[k][i] = (float)ru[k][i], x[k][i] = (float)rx[k][i];
             if (TOKEN) g[k] = rg[k];
@@ -307,6 +309,7 @@ __global__ __launch_bounds__(G ? 256 : MOST, MOST == 1024 ? 4 : TOKEN ? 2 : 3) v
 #pragma unroll
         for (int k = 0; k < NV; k++) {
             d[k] = rd[k];
+            if (G == 0) settle(d[k]);  // as in the forward
 #pragma unroll
             for (int i = 0; i < 8; i++) w[k][i] = TOKEN ? (float)rg[TOKEN ? k : 0][i] : 1.f;
             if (TOKEN) gates(w[k], a.gate_act);
