@@ -16,6 +16,16 @@ import warchest_learn as wl
 import warchest_wave as ww
 
 pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(autouse=True)
+def float32_by_default():
+    """Other test modules set torch's default type to float64 for the whole process."""
+    before = torch.get_default_dtype()
+    torch.set_default_dtype(torch.float32)
+    yield
+    torch.set_default_dtype(before)
+
 DEV = "cuda:0"
 TYPES = {"f32": torch.float32, "f16": torch.float16, "bf16": torch.bfloat16}
 ROUND = {torch.float32: 2.0 ** -23, torch.float16: 2.0 ** -11, torch.bfloat16: 2.0 ** -8}

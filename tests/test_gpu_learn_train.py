@@ -7,6 +7,16 @@ import train_policy
 import warchest_learn as wl
 
 pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(autouse=True)
+def float32_by_default():
+    """Other test modules set torch's default type to float64 for the whole process."""
+    before = torch.get_default_dtype()
+    torch.set_default_dtype(torch.float32)
+    yield
+    torch.set_default_dtype(before)
+
 DEV = "cuda:0"
 
 

@@ -13,6 +13,16 @@ import learn_ref as R
 import warchest_learn as wl
 import warchest_wave as ww
 
+
+@pytest.fixture(autouse=True)
+def float32_by_default():
+    """Other test modules set torch's default type to float64 for the whole process."""
+    before = torch.get_default_dtype()
+    torch.set_default_dtype(torch.float32)
+    yield
+    torch.set_default_dtype(before)
+
+
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 HEADER = os.path.join(ROOT, "include", "wc_learn.h")
 STRUCTS = {"wc_policy_args": wl._POLICY, "wc_preference_args": wl._PREFERENCE, "wc_norm_args": wl._NORM,

@@ -47,7 +47,7 @@ class PolicyNet(torch.nn.Module):
     def __init__(self, inputs, width, blocks, actions, device):
         super().__init__()
         def weight(i, o, gain=1.0):
-            return torch.nn.Parameter(torch.randn(i, o, device=device) * gain * i ** -0.5)
+            return torch.nn.Parameter(torch.randn(i, o, device=device, dtype=torch.float32) * gain * i ** -0.5)
 
         self.inp = weight(inputs, width)
         self.up = torch.nn.ParameterList(weight(width, 4 * width) for _ in range(blocks))
