@@ -534,7 +534,7 @@ def test_weight_gradient_long_sums_strides_and_the_same_bits(dtype):
     (16411, 2050, 4090, "relu", 2),
 ])
 def test_weight_gradient_of_large_products(rows, width, out, name, pad, dtype):
-    """Sizes that the large tiles are taken for, against a float64 product on the device."""
+    """Sizes of the large tiles, or near where they begin, against a float64 product on the device."""
     say(f"case weight: {rows} x {width} x {out} {dtype} {name}, {pad} between rows")
     t = TYPES[dtype]
     g = torch.Generator(device=DEV).manual_seed(rows + out)

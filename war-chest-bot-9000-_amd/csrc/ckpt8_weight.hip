@@ -10,6 +10,14 @@
 // tile's global loads in registers meanwhile. Where the tiles are too few for
 // the device the rows are cut into runs, whose partial products are added in
 // order.
+//
+// On one MI355X: 512 x 384 over 49,371 rows 39 us (k_weight, 492 workgroups of
+// which 41 share a tile) and 7 to add the runs; floor 17 us at the 1,142 TFLOP/s
+// of a large library product. A step of 64 rows takes 1.45 us with two workgroups
+// a CU, of which the matrix instructions are 0.42, arithmetic 0.4 and LDS 0.5 (a
+// third of the cycles wait on barriers and counters). 4,096 x 4,096 over 16,384
+// rows with GELU: 39 us to expand and 477 us (k_weight_big, 1.15 PFLOP/s); the
+// library's product of the same 16-bit operands takes 559.
 #include <algorithm>
 
 #include "ckpt8_dev.h"
@@ -370,7 +378,9 @@ __global__ __launch_bounds__(BLOCK, 2) void k_weight(Job job) {
 // (an activation recomputed for every column tile would cost more than the
 // products), the gradient as it is or copied. 256 x 256 tiles, four wavefronts
 // of 128 x 128; tiles go from memory to LDS without passing registers, four
-// buffers of 32 rows, three of them in flight.
+// buffers of 32 rows, three of them in flight. With a wait for all loads in each
+// step, and these in one block before the matrix instructions, it took 663 us
+// where it takes 477.
 constexpr int BIG = 256, BIG_DEPTH = 32, BIG_ROW = 2 * BIG, BIG_SIDE = BIG_DEPTH * BIG_ROW, BUFFERS = 4;
 
 static __device__ __align__(16) uint4 g_zeros;  // what rows past the end are read from
@@ -632,35 +642,45 @@ struct Plan {
     size_t x, g, part, bias, bytes;
 };
 
-// Microseconds that a product takes, from measured parts: a step of a
-// workgroup's, its start and end, a partial product written and read, and
-// what the large product's operands cost to lay out.
+// Microseconds that a product takes, from measured parts: a step of a round of
+// workgroups (alone on their CUs, or two to a CU), a round's start and end, the
+// runs' products written and read, and what the large product's operands cost
+// to lay out. Both kernels over 1 to 128 runs at fifteen shapes: the pick was
+// the best of all at thirteen, 7 and 15% above it at two. For instance 512 x 384 x
+// 49,371: small 45 us, large 61; with GELU 65 and 61; 4,096 x 4,096 x 16,384:
+// small 728, large 484; 1,024 x 1,024 x 8,192: 43 and 51; 300 x 200 x 1,000: 16
+// in eight runs, 24 in one.
 Plan plan_of(const wc_ckpt_weight_args& a, int cus) {
     Plan best = {};
     double least = -1;
     // (a lane's offset in two rows is held in 32 bits)
     const bool aligned = a.out % 8 == 0 && a.grad_stride % 8 == 0 && ((uintptr_t)a.grad & 15) == 0 &&
                          a.grad_stride < (1 << 29);
+    const bool value = a.act == WC_ACT_GELU || a.act == WC_ACT_SILU;
     for (int big = 0; big < 2; big++) {
         if (big && a.dtype == WC_DTYPE_F32) continue;
         const int tile = big ? BIG : Shape<2>::TILE, depth = big ? BIG_DEPTH : DEPTH;
         const int64_t ti = (a.width + tile - 1) / tile, tj = (a.out + tile - 1) / tile, tiles = ti * tj;
-        const int64_t steps = (a.rows + depth - 1) / depth, slots = big ? cus : 2 * cus;
-        const double value = a.act == WC_ACT_GELU || a.act == WC_ACT_SILU ? 1.3 : 0.0;
-        const double step = big ? 0.55 : 0.95 + value;
-        const double lay = big ? 3.0 + double(a.rows) * (a.width * 3 + (aligned ? 0 : a.out * 4)) / 4e6 : 0.0;
-        const int64_t most = std::max<int64_t>(1, std::min<int64_t>(steps / 8, 4 * slots / tiles));
-        for (int64_t runs = 1; runs <= most; runs++) {
-            const int64_t per = std::max<int64_t>(1, (steps + runs - 1) / runs);
-            const double t = lay + double((tiles * runs + slots - 1) / slots) * (per * step + 4.0) +
-                             (runs > 1 ? 3.0 + double(runs) * a.width * a.out * 8 / 4e6 : 0.0);
+        const int64_t steps = std::max<int64_t>(1, (a.rows + depth - 1) / depth), slots = big ? cus : 2 * cus;
+        const double one = big ? 0.8 : value ? 1.55 : 0.97, two = big ? 0.8 : value ? 2.6 : 1.58;
+        const double lay = big ? 4.0 + double(a.rows) * a.width * 3 / 5e6 +
+                                     (aligned ? 0.0 : 4.0 + double(a.rows) * a.out * 4 / 5e6)
+                               : 0.0;
+        // runs that fill one to eight times the device's CUs, a few, or as many as leave each a few steps
+        const int64_t most = std::max<int64_t>(1, std::min<int64_t>(steps / (big ? 4 : 2), 4 * slots / tiles));
+        for (int k = -3; k <= 8; k++) {
+            const int64_t runs = std::min(most, std::max<int64_t>(1, k == 0 ? most : k < 0 ? -k : k * cus / tiles));
+            const int64_t per = (steps + runs - 1) / runs, full = tiles * runs / slots, rest = tiles * runs % slots;
+            const double t = lay + double(full) * (double(per) * two + 4.0) +
+                             (rest ? double(per) * (rest <= cus ? one : two) + 4.0 : 0.0) +
+                             (runs > 1 ? 4.0 + double(runs) * a.width * a.out * 8 / 9e6 : 0.0);
             if (least >= 0 && t >= least) continue;
             least = t;
             best = {};
             best.big = big;
             best.tiles_i = (int)ti;
             best.tiles_j = (int)tj;
-            best.runs = (int)std::max<int64_t>(1, (steps + per - 1) / per);
+            best.runs = (int)((steps + per - 1) / per);
             best.run = per * depth;
             best.copy = big && !aligned;
         }

@@ -6,9 +6,19 @@
 // logit against some 20 operations. So a row is read once and held in
 // registers, as it came, from its load to its gradient's store (k_rows), by as
 // few threads as hold it: part of a wavefront for a few heads, one wavefront up
-// to 4 KB, a workgroup up to 256 KB. Longer rows are read twice (k_row_parts,
+// to 8 KB, a workgroup up to 256 KB. Longer rows are read twice (k_row_parts,
 // k_row_grads), and so are the preference loss's, whose gradient waits for
 // whole sequences.
+//
+// On one MI355X, where a large copy moves 5.09 TB/s (read and write):
+// - 4,096 x 65,536 bf16, a quarter of the rows left out: 203 us, 4.6 TB/s (two
+//   passes, 366 us; 512 threads a row with half the registers each, which
+//   spilled, 260);
+// - 49,371 x 567 float32 with a reference distribution and legal columns: 97 us,
+//   3.5 TB/s. A third of its wavefronts' cycles issue arithmetic, two thirds wait
+//   for memory at 3.2 wavefronts a SIMD; five wavefronts would spill (159 us),
+//   and workgroups that stay and take row after row were slower (114 us);
+// - 64 x 22: 4 us, one launch.
 #pragma once
 
 #include <algorithm>
@@ -576,7 +586,9 @@ __global__ __launch_bounds__(1024) void k_sum(LossSum l) { sum_losses<1024>(l); 
 
 // The gradient from the rows' coefficients, a second read of the logits. The
 // last rows go first: they are what the pass before left in the caches. The
-// last workgroup adds the losses beside the others.
+// last workgroup adds the losses beside the others. 4,608 x 65,536 bf16, 30% of
+// the rows left out: 151 us for 1.03 GB, 6.8 TB/s, more than memory gives; the
+// preference loss there 277 us in all, of which the first read takes 112.
 template <class T, bool FULL>
 __global__ __launch_bounds__(BLOCK) void k_row_grads(Rows<T> in, int64_t tiles, int splits, const RowGrad* grads,
                                                      const float* grad_out, T* out, int64_t out_stride,
@@ -659,7 +671,8 @@ int64_t rows_at(const Rows<T>& in, const PolicyRow& row, int64_t rows, RowGrad* 
 
 // The fewest threads that hold a row in at most eight loads each, and with the
 // least left empty: what a wavefront does once a row (the sums' butterflies,
-// the logarithms) it then does for several rows at once.
+// the logarithms) it then does for several rows at once. 567 float32 columns
+// with a reference: 110 us on 32 lanes of five loads, 147 on 64 lanes of three.
 template <class T, bool FULL, bool TOKEN>
 int64_t rows_held(const Rows<T>& in, const PolicyRow& row, int64_t rows, RowGrad* grads, const float* go, T* grad,
                   int64_t gs, hipStream_t s) {
@@ -681,7 +694,7 @@ int64_t rows_held(const Rows<T>& in, const PolicyRow& row, int64_t rows, RowGrad
     if (n <= 512) return rows_at<T, 64, 8, FULL, TOKEN>(in, row, rows, grads, go, grad, gs, s);
     if (n <= 1024) return rows_at<T, 256, 4, FULL, TOKEN>(in, row, rows, grads, go, grad, gs, s);
     if (n <= 2048) return rows_at<T, 256, 8, FULL, TOKEN>(in, row, rows, grads, go, grad, gs, s);
-    if constexpr (TOKEN) {  // no gradient to write: more threads, with less each, load faster
+    if constexpr (TOKEN) {  // no gradient to write: more threads, with less each, load faster (65,536 bf16: 112 us, 134)
         if (n <= 4096) return rows_at<T, 512, 8, FULL, TOKEN>(in, row, rows, grads, go, grad, gs, s);
         if (n <= 8192) return rows_at<T, 512, 16, FULL, TOKEN>(in, row, rows, grads, go, grad, gs, s);
         return rows_at<T, 512, 32, FULL, TOKEN>(in, row, rows, grads, go, grad, gs, s);
@@ -735,7 +748,7 @@ __device__ __forceinline__ int64_t clamp_row(int64_t x, int64_t rows) { return x
 
 // One pair per workgroup: both sequences' ratios in 64-bit sums (long sums of
 // differences that nearly cancel), the pair's loss, and the coefficient of
-// every row of both.
+// every row of both. 6 to 9 us of dependent loads; the pairs side by side.
 __global__ __launch_bounds__(BLOCK) void k_pairs(Pairs p, const float* logp, RowGrad* grads, double* losses,
                                                  float* margins, float* ratios) {
     __shared__ double lds[4][BLOCK / 64];
