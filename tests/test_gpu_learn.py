@@ -683,3 +683,42 @@ def test_residual_norm_in_place(width):
         1.0, 1, 0, 0, f.stats.data_ptr(), d_out.data_ptr(), width, g.data_ptr(), width, block.data_ptr(), width,
         g.data_ptr(), width, 0, 0, 0, 0, 0, 0, work.data_ptr(), need), x.device)
     assert torch.equal(g, b.stream) and torch.equal(block, b.block)
+
+
+def far_rows(x, stride):
+    """x's rows `stride` elements apart in memory that is otherwise left as it comes."""
+    buf = torch.empty((x.shape[0] - 1) * stride + x.shape[1], dtype=x.dtype, device=DEV)
+    v = buf.as_strided(x.shape, (stride, 1))
+    v.copy_(x)
+    return v
+
+
+def test_rows_past_32_bit_offsets():
+    """Rows a billion elements apart: the last one's offset passes what a signed 32-bit number holds in elements, and any
+    32-bit number in bytes. The same bits as from rows side by side."""
+    say("case far rows")
+    far = (1 << 30) + 8
+    k = {n: to(v) for n, v in policy_inputs(4, 900, torch.bfloat16, 3, False, "none").items()}
+    want = wl.policy_loss(**k, **COEFS)
+    g = far_rows(torch.zeros(4, 900, dtype=torch.bfloat16), far)
+    got = wl.policy_loss(**{**k, "logits": far_rows(k["logits"], far)}, **COEFS, grad=g)
+    assert torch.equal(got.loss, want.loss) and torch.equal(got.grad, want.grad)
+    del g, got
+    k, d = norm_inputs(4, 200, torch.bfloat16, 4, "layer", "none")
+    v = {n: to(t) for n, t in k.items()}
+    want = wl.residual_norm(**v)
+    got = wl.residual_norm(**{**v, "block": far_rows(v["block"], far)})
+    assert torch.equal(got.stream, want.stream) and torch.equal(got.out, want.out)
+    x = far_rows(v["block"], far)
+    ck, plain = wl.checkpoint8(x), wl.checkpoint8(v["block"])
+    assert torch.equal(ck.q, plain.q) and torch.equal(ck.exps, plain.exps)
+    del got, x
+    for out in (40, 41):
+        dy = torch.randn(4, out, generator=gen(out)).bfloat16().to(DEV)
+        want, _ = wl.checkpoint8_weight_grad(ck, dy)
+        got, _ = wl.checkpoint8_weight_grad(ck, far_rows(dy, far))
+        assert torch.equal(got, want)
+    q = far_rows(ck.q, 1 << 31)
+    got, _ = wl.checkpoint8_weight_grad(wl.Checkpoint8(q, ck.exps), dy)
+    assert torch.equal(got, want)
+    assert torch.equal(wl.checkpoint8_read(wl.Checkpoint8(q, ck.exps)), wl.checkpoint8_read(ck))
