@@ -459,7 +459,9 @@ __global__ __launch_bounds__(256) void k_norm_cols(const float* part, int blocks
 
 // Lanes per row (0: the workgroup) and threads of the workgroup: as many as the
 // row has chunks of eight, by powers of two inside a wavefront and by whole
-// wavefronts beyond; past 8,192 columns two chunks a thread.
+// wavefronts beyond; past 8,192 columns two chunks a thread. Forward over
+// 4,099 x 1,153 f16: 18 us with 192 threads, 21 with the next power of two,
+// 256; the backward takes 27 with either.
 struct Threads {
     int g, block, nv;
 };
