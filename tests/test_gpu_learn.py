@@ -722,3 +722,22 @@ def test_rows_past_32_bit_offsets():
     got, _ = wl.checkpoint8_weight_grad(wl.Checkpoint8(q, ck.exps), dy)
     assert torch.equal(got, want)
     assert torch.equal(wl.checkpoint8_read(wl.Checkpoint8(q, ck.exps)), wl.checkpoint8_read(ck))
+
+
+@pytest.mark.parametrize("rows,width", [(64, 9), (100, 15), (64, 17), (33, 31), (65, 33), (70, 100), (90, 257), (200, 321),
+                                        (300, 505), (64, 3), (64, 511)])
+def test_column_sums_of_odd_widths_count_every_row_once(rows, width):
+    """Rows of one wavefront, whose last chunk of columns lies over the one before: whole numbers, so that a column's sum
+    over the rows is exact and a row counted twice shows."""
+    say(f"case norm column sums: {rows} x {width}")
+    g = gen(rows + width)
+    d = torch.randint(-50, 51, (rows, width), generator=g).float()
+    u, x = torch.randn(rows, width, generator=g).to(DEV), torch.randn(rows, width, generator=g).to(DEV)
+    one, zero = torch.ones(width, device=DEV), torch.zeros(width, device=DEV)
+    for kind in ("layer", "rms"):
+        f = wl.residual_norm(u, x, one, zero, None, one, zero, norm=kind)
+        b = wl.residual_norm_backward(to(d), None, u, x, f.stats, one, zero, None, one, zero, norm=kind)
+        assert torch.equal(b.pre_bias.cpu(), d.sum(0))
+        # with no d_out the update's factor is 1: post_bias gets what arrives at the stream
+        b = wl.residual_norm_backward(None, to(d), u, x, f.stats, one, zero, None, one, zero, norm=kind)
+        assert torch.equal(b.post_bias.cpu(), d.sum(0)) and not b.pre_bias.any()

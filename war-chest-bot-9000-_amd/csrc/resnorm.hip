@@ -409,14 +409,10 @@ __global__ __launch_bounds__(G ? 256 : MOST, MOST == 1024 ? 4 : TOKEN ? 2 : 3) v
                 __syncthreads();
                 if (at.group == g) {
 #pragma unroll
-                    for (int k = 0; k < NV; k++) {
-                        if (!at.holds(k)) continue;
-                        float o[8];
+                    for (int k = 0; k < NV; k++)
 #pragma unroll
-                        for (int i = 0; i < 8; i++) o[i] = (g ? cols[at.col[k] + i] : 0.f) + v[k][i];
-#pragma unroll
-                        for (int i = 0; i < 8; i++) cols[at.col[k] + i] = o[i];
-                    }
+                        for (int i = 0; i < 8; i++)  // each column by one thread: the last chunk lies over the one before
+                            if (at.counts(k, i)) cols[at.col[k] + i] = (g ? cols[at.col[k] + i] : 0.f) + v[k][i];
                 }
             }
             __syncthreads();
