@@ -741,3 +741,27 @@ def test_column_sums_of_odd_widths_count_every_row_once(rows, width):
         # with no d_out the update's factor is 1: post_bias gets what arrives at the stream
         b = wl.residual_norm_backward(None, to(d), u, x, f.stats, one, zero, None, one, zero, norm=kind)
         assert torch.equal(b.post_bias.cpu(), d.sum(0)) and not b.pre_bias.any()
+
+
+def test_preference_more_pairs_than_a_launch_has_workgroups():
+    """Pairs whose threads, 256 each, pass 32 bits: the first, one in between and the last with rows, the others empty
+    (margin 0). Margins and ratios as of the three alone, and the loss log 2 but for three parts in 2^24."""
+    pairs = (1 << 24) + 3
+    say(f"case preference: {pairs} pairs")
+    k = preference_inputs([2, 1, 1, 2, 3, 1], 8, torch.float32, 12)
+    small = wl.preference_loss(**{n: to(v) for n, v in k.items()}, beta=0.3)
+    offsets = torch.zeros(2 * pairs + 1, dtype=torch.int32, device=DEV)
+    at = [0, 1 << 23, pairs - 1]
+    ends = k["offsets"].int().tolist()
+    for i, p in enumerate(at):  # sequences before a pair end where it starts
+        offsets[2 * p + 1:] = ends[2 * i + 1]
+        offsets[2 * p + 2:] = ends[2 * i + 2]
+    dev = {n: to(v) for n, v in k.items()} | {"offsets": offsets, "tokens": k["tokens"].int().to(DEV)}
+    got = wl.preference_loss(**dev, beta=0.3)
+    where = torch.tensor(at, device=DEV)
+    assert torch.equal(got.margins[where], small.margins)
+    assert torch.equal(got.ratios.view(-1, 2)[where], small.ratios.view(-1, 2))
+    assert int(got.margins.count_nonzero()) <= 3
+    assert abs(float(got.loss) - math.log(2)) < 2e-5
+    # every row's coefficient is 3 / pairs of what it is among three
+    near(got.grad * (pairs / 3), small.grad.cpu(), "grad")

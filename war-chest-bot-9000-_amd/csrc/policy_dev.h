@@ -749,61 +749,65 @@ __device__ __forceinline__ int64_t clamp_row(int64_t x, int64_t rows) { return x
 
 // One pair per workgroup: both sequences' ratios in 64-bit sums (long sums of
 // differences that nearly cancel), the pair's loss, and the coefficient of
-// every row of both. 6 to 9 us of dependent loads; the pairs side by side.
+// every row of both. 6 to 9 us of dependent loads; the pairs side by side, up
+// to what a launch's threads can be counted in 32 bits.
+constexpr int64_t MOST_PAIR_BLOCKS = 1 << 22;
 __global__ __launch_bounds__(BLOCK) void k_pairs(Pairs p, const float* logp, RowGrad* grads, double* losses,
                                                  float* margins, float* ratios) {
     __shared__ double lds[4][BLOCK / 64];
-    const int64_t i = blockIdx.x;
-    int64_t lo[2], hi[2];
-    double sum[4] = {};
-    for (int k = 0; k < 2; k++) {
-        lo[k] = clamp_row(index_at(p.offsets, p.bits, 2 * i + k), p.rows);
-        hi[k] = clamp_row(index_at(p.offsets, p.bits, 2 * i + k + 1), p.rows);
-        for (int64_t r = lo[k] + threadIdx.x; r < hi[k]; r += BLOCK) {
-            if (!grads[r].on) continue;
-            const float w = p.weights ? p.weights[r] : 1.f;
-            sum[2 * k] += (double)w * ((double)logp[r] - p.ref_logp[r]);
-            sum[2 * k + 1] += w;
+    for (int64_t i = blockIdx.x; i < p.pairs; i += gridDim.x) {
+        int64_t lo[2], hi[2];
+        double sum[4] = {};
+        for (int k = 0; k < 2; k++) {
+            lo[k] = clamp_row(index_at(p.offsets, p.bits, 2 * i + k), p.rows);
+            hi[k] = clamp_row(index_at(p.offsets, p.bits, 2 * i + k + 1), p.rows);
+            for (int64_t r = lo[k] + threadIdx.x; r < hi[k]; r += BLOCK) {
+                if (!grads[r].on) continue;
+                const float w = p.weights ? p.weights[r] : 1.f;
+                sum[2 * k] += (double)w * ((double)logp[r] - p.ref_logp[r]);
+                sum[2 * k + 1] += w;
+            }
         }
-    }
-    for (int q = 0; q < 4; q++) {
-        for (int mask = 32; mask; mask >>= 1) sum[q] += __shfl_xor(sum[q], mask);
-        if ((threadIdx.x & 63) == 0) lds[q][threadIdx.x >> 6] = sum[q];
-    }
-    __syncthreads();
-    for (int q = 0; q < 4; q++) sum[q] = (lds[q][0] + lds[q][1]) + (lds[q][2] + lds[q][3]);
-    double share[2], ratio[2];
-    for (int k = 0; k < 2; k++) {
-        share[k] = !p.average ? 1.0 : sum[2 * k + 1] != 0.0 ? 1.0 / sum[2 * k + 1] : 0.0;
-        ratio[k] = sum[2 * k] * share[k];
-    }
-    const double h = ratio[0] - ratio[1], z = p.beta * h;
-    double loss, d;
-    if (p.kind == WC_PREFERENCE_LOGISTIC) {
-        const double e = exp(-fabs(z)), tail = log1p(e);
-        loss = tail + (1.0 - p.smoothing) * fmax(-z, 0.0) + p.smoothing * fmax(z, 0.0);
-        d = p.beta * ((z >= 0 ? 1.0 / (1.0 + e) : e / (1.0 + e)) - (1.0 - p.smoothing));
-        if (z != z) loss = z;
-    } else if (p.kind == WC_PREFERENCE_SQUARED) {
-        const double t = h - 0.5 / p.beta;
-        loss = t * t;
-        d = 2.0 * t;
-    } else {
-        loss = z < 1.0 ? 1.0 - z : 0.0;
-        d = z < 1.0 ? -(double)p.beta : 0.0;
-        if (z != z) loss = d = z;
-    }
-    d /= (double)p.pairs;
-    for (int k = 0; k < 2; k++) {
-        const float c = (float)((k ? -d : d) * share[k]);
-        for (int64_t r = lo[k] + threadIdx.x; r < hi[k]; r += BLOCK)
-            if (grads[r].on) grads[r].coef = c * (p.weights ? p.weights[r] : 1.f);
-    }
-    if (threadIdx.x == 0) {
-        losses[i] = loss;
-        margins[i] = (float)z;
-        ratios[2 * i] = (float)ratio[0];
-        ratios[2 * i + 1] = (float)ratio[1];
+        for (int q = 0; q < 4; q++) {
+            for (int mask = 32; mask; mask >>= 1) sum[q] += __shfl_xor(sum[q], mask);
+            if ((threadIdx.x & 63) == 0) lds[q][threadIdx.x >> 6] = sum[q];
+        }
+        __syncthreads();
+        for (int q = 0; q < 4; q++) sum[q] = (lds[q][0] + lds[q][1]) + (lds[q][2] + lds[q][3]);
+        double share[2], ratio[2];
+        for (int k = 0; k < 2; k++) {
+            share[k] = !p.average ? 1.0 : sum[2 * k + 1] != 0.0 ? 1.0 / sum[2 * k + 1] : 0.0;
+            ratio[k] = sum[2 * k] * share[k];
+        }
+        const double h = ratio[0] - ratio[1], z = p.beta * h;
+        double loss, d;
+        if (p.kind == WC_PREFERENCE_LOGISTIC) {
+            const double e = exp(-fabs(z)), tail = log1p(e);
+            loss = tail + (1.0 - p.smoothing) * fmax(-z, 0.0) + p.smoothing * fmax(z, 0.0);
+            d = p.beta * ((z >= 0 ? 1.0 / (1.0 + e) : e / (1.0 + e)) - (1.0 - p.smoothing));
+            if (z != z) loss = z;
+        } else if (p.kind == WC_PREFERENCE_SQUARED) {
+            const double t = h - 0.5 / p.beta;
+            loss = t * t;
+            d = 2.0 * t;
+        } else {
+            loss = z < 1.0 ? 1.0 - z : 0.0;
+            d = z < 1.0 ? -(double)p.beta : 0.0;
+            if (z != z) loss = d = z;
+        }
+        d /= (double)p.pairs;
+        for (int k = 0; k < 2; k++) {
+            const float c = (float)((k ? -d : d) * share[k]);
+            for (int64_t r = lo[k] + threadIdx.x; r < hi[k]; r += BLOCK)
+                if (grads[r].on) grads[r].coef = c * (p.weights ? p.weights[r] : 1.f);
+        }
+        if (threadIdx.x == 0) {
+            losses[i] = loss;
+            margins[i] = (float)z;
+            ratios[2 * i] = (float)ratio[0];
+            ratios[2 * i + 1] = (float)ratio[1];
+        }
+        __syncthreads();  // the sums have been read
     }
 }
 
@@ -826,7 +830,9 @@ void preference(const wc_preference_args& a, hipStream_t s) {
     }
     const Pairs p = {a.offsets, a.ref_logp, a.weights, a.rows, a.pairs, a.beta, a.smoothing, a.kind, a.average,
                      a.index_bits};
-    if (a.pairs) k_pairs<<<dim3((uint32_t)a.pairs), BLOCK, 0, s>>>(p, a.logp, grads, losses, a.margins, a.ratios);
+    if (a.pairs)
+        k_pairs<<<dim3((uint32_t)std::min(a.pairs, MOST_PAIR_BLOCKS)), BLOCK, 0, s>>>(p, a.logp, grads, losses, a.margins,
+                                                                                      a.ratios);
     const LossSum sum = {losses, a.pairs, a.pairs ? 1.0 / (double)a.pairs : 0.0, a.loss};
     if (a.grad && a.rows)
         k_row_grads<T, false><<<tile_grid(tiles) + 1, BLOCK, 0, s>>>(in, tiles, splits, grads, a.grad_out, (T*)a.grad,
