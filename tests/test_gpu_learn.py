@@ -765,3 +765,39 @@ def test_preference_more_pairs_than_a_launch_has_workgroups():
     assert abs(float(got.loss) - math.log(2)) < 2e-5
     # every row's coefficient is 3 / pairs of what it is among three
     near(got.grad * (pairs / 3), small.grad.cpu(), "grad")
+
+
+@pytest.mark.parametrize("rows,vocab,dtype", [(3, 22, "f32"), (3, 567, "f32"), (3, 4099, "f16"), (2, 33001, "f32"),
+                                              (2, 70001, "bf16")])
+def test_policy_kl_does_not_depend_on_where_the_reference_lies(rows, vocab, dtype):
+    """Rows that registers hold, and rows in chunks (float32 beyond 32,768 columns, 16 bits beyond 65,536): a constant
+    added to the reference's logits, or to the policy's, changes nothing but their rounding, which the oracle shares; a
+    reference row at the type's lowest value is an even one; columns of the policy at its lowest value (whole chunks of
+    them among these) weigh nothing, whatever the reference holds there."""
+    say(f"case policy kl: {rows} x {vocab} {dtype}")
+    t = TYPES[dtype]
+    low = torch.finfo(t).min
+    k = policy_inputs(rows, vocab, t, vocab, False, "full")
+
+    def check(**edit):
+        e = {**k, **edit}
+        lp = torch.log_softmax(e["logits"].double() * COEFS["inv_temperature"], 1)[torch.arange(rows), e["actions"]]
+        e["behaviour_logp"] = lp.float() + 0.1  # ratios near 1: the loss is as well known as the log-probabilities
+        want = R.policy(**e, **COEFS)
+        got = wl.policy_loss(**{n: to(v) for n, v in e.items()}, **COEFS)
+        for n in ("logp", "kl", "entropy"):
+            near(getattr(got, n), want[n], n, scale=max(1.0, float(want[n].abs().max())))
+        near(got.loss, want["loss"], "loss", scale=1.0)
+        near(got.grad, want["grad"], "grad")
+
+    for far in (1e4, -3e4, 6e4):
+        check(ref_logits=(k["ref_logits"].float() + far).clamp(low, torch.finfo(t).max).to(t))
+    y = k["ref_logits"].clone()
+    y[0] = low
+    check(ref_logits=y)
+    x = k["logits"].clone()
+    x[:, vocab // 3:] = low
+    a = k["actions"] % (vocab // 3)
+    check(logits=x, actions=a)
+    check(logits=x.flip(1), actions=vocab - 1 - a)
+    check(logits=(x.float() + 5000).clamp(min=low).to(t), actions=a)

@@ -44,7 +44,9 @@ struct Rate {
 };
 
 // A softmax's statistics over part of a row: the maximum logit, the sums of
-// e = 2^z, of e z (for the entropy) and of e (x - y) (for the KL sum), and y's
+// e = 2^z, of e z (for the entropy) and of e ((x - m) - (y - my)) (for the KL
+// sum: each row's differences to its own maximum, so that a constant added to
+// either row, or a row at a mask's lowest value, changes nothing), and y's
 // maximum and sum.
 struct Part {
     float m, s, t, d, my, sy;
@@ -61,7 +63,10 @@ __device__ __forceinline__ Part join(const Part& a, const Part& b, float rate) {
     const float fa = power(da), fb = power(db);
     r.s = a.s * fa + b.s * fb;
     r.t = fa * (a.t + a.s * fmaxf(da, -300.f)) + fb * (b.t + b.s * fmaxf(db, -300.f));
-    r.d = a.d * fa + b.d * fb;
+    // the KL sums' differences are to other maxima now; a part that weighs nothing adds
+    // nothing, whatever the distance
+    r.d = (fa > 0.f && a.s > 0.f ? fa * (a.d + a.s * ((a.m - r.m) - (a.my - r.my))) : 0.f) +
+          (fb > 0.f && b.s > 0.f ? fb * (b.d + b.s * ((b.m - r.m) - (b.my - r.my))) : 0.f);
     r.sy = (a.my != -INFINITY ? a.sy * power((a.my - r.my) * rate) : a.sy) +
            (b.my != -INFINITY ? b.sy * power((b.my - r.my) * rate) : b.sy);
     return r;
@@ -219,8 +224,9 @@ __device__ __forceinline__ void count(Part& p, float x, float y, float m, float 
     p.s += e;
     p.t += e * fmaxf(z, -300.f);  // e is 0 there, and 0 * -infinity would be NaN
     if (FULL) {
-        p.d += e > 0.f ? e * (x - y) : 0.f;
-        p.sy += power((y - my) * rate);
+        const float v = y - my;
+        p.d += e > 0.f ? e * ((x - m) - v) : 0.f;
+        p.sy += power(v * rate);
     }
 }
 
@@ -393,7 +399,7 @@ struct PolicyRow {
         }
         if (full) {
             log2_sy = __log2f(p.sy);
-            kl = (p.d * over - (p.m - p.my)) * k.rate * LN2 - (log_s - logf(p.sy));
+            kl = p.d * over * k.rate * LN2 - (log_s - logf(p.sy));
         }
         *out = make_float3(lp, kl, h);
         *g = {p.m, log2_s, p.my, log2_sy, w * slope, w * entropy_coef, h, full ? w * kl_coef : 0.f, kl, 1};
