@@ -88,3 +88,44 @@ def test_the_training_example_learns_the_search_policy():
     first, last, pref, pref_last = train_policy.train(trees=2, steps=40, width=128, blocks=2)
     assert last < 0.5 * first
     assert pref_last < 0.8 * pref
+
+
+def objective_inputs(vocab=30):
+    g = torch.Generator(device=DEV).manual_seed(4)
+    rows = 12
+    draw = lambda *shape: torch.randn(*shape, generator=g, device=DEV)  # noqa: E731
+    k = {"actions": torch.randint(0, vocab, (rows,), generator=g, device=DEV), "behaviour_logp": draw(rows) - 3,
+         "advantages": draw(rows), "weights": torch.rand(rows, generator=g, device=DEV) + 0.1,
+         "legal": torch.ones(rows, vocab, dtype=torch.bool, device=DEV), "ref_logits": draw(rows, vocab)}
+    p = {"tokens": k["actions"].clone(), "offsets": torch.tensor([0, 3, 6, 8, 12], device=DEV), "ref_logp": draw(rows) - 3,
+         "weights": k["weights"].clone()}
+    return draw(rows, vocab).requires_grad_(True), k, p
+
+
+@pytest.mark.parametrize("which,name", [(0, n) for n in ("logits", "actions", "behaviour_logp", "advantages", "weights",
+                                                         "legal", "ref_logits", "ref_logp")] +
+                         [(1, n) for n in ("logits", "tokens", "offsets", "ref_logp", "weights")])
+def test_an_objective_whose_batch_was_written_since_refuses_its_backward_pass(which, name):
+    """What the backward pass would read again belongs to another batch then."""
+    x, k, p = objective_inputs()
+    if name == "ref_logp" and which == 0:
+        k["ref_logits"] = None
+        k["ref_logp"] = p["ref_logp"]
+    call, kw = ((wl.policy_objective, k), (wl.preference_objective, p))[which]
+    loss, *_ = call(x, **kw, **({"kl_coef": 0.1} if which == 0 else {}))
+    with torch.no_grad():
+        (x if name == "logits" else kw[name]).add_(0)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.backward()
+
+
+def test_objectives_of_a_batch_left_alone_after_other_calls():
+    """Two losses over one batch, backward in the other order: each its own gradient (the same float32 sums: 1e-6)."""
+    x, k, p = objective_inputs()
+    one, *_ = wl.policy_objective(x, **k, kl_coef=0.1, entropy_coef=0.01)
+    two, *_ = wl.preference_objective(x, **p, kind="squared")
+    two.backward()
+    close(x.grad, wl.preference_loss(x.detach(), **p, kind="squared").grad, "preference", 1e-6)
+    x.grad = None
+    one.backward()
+    close(x.grad, wl.policy_loss(x.detach(), **k, kl_coef=0.1, entropy_coef=0.01).grad, "policy", 1e-6)

@@ -456,44 +456,55 @@ def _upstream(g):
 
 
 class _PolicyObjective(torch.autograd.Function):
+    # The backward pass reads every tensor again: all of them are saved, so that torch refuses it if one was written since.
     @staticmethod
-    def forward(ctx, logits, rows, kw):
-        r = policy_loss(logits, *rows, grad=False, **kw)
-        ctx.save_for_backward(logits)
-        ctx.call = rows, kw
+    def forward(ctx, logits, kw, *rows):
+        r = _PolicyObjective.call(logits, kw, *rows, grad=False)
+        ctx.save_for_backward(logits, *rows)
+        ctx.kw = kw
         ctx.mark_non_differentiable(r.logp, r.kl, r.entropy)
         return r.loss, r.logp, r.kl, r.entropy
 
     @staticmethod
+    def call(logits, kw, actions, behaviour_logp, advantages, weights, legal, ref_logp, ref_logits, **more):
+        return policy_loss(logits, actions, behaviour_logp, advantages, weights, legal=legal, ref_logp=ref_logp,
+                           ref_logits=ref_logits, **kw, **more)
+
+    @staticmethod
     def backward(ctx, d_loss, *_):
-        rows, kw = ctx.call
-        return policy_loss(ctx.saved_tensors[0], *rows, grad_out=_upstream(d_loss), **kw).grad, None, None
+        logits, *rows = ctx.saved_tensors
+        grad = _PolicyObjective.call(logits, ctx.kw, *rows, grad_out=_upstream(d_loss)).grad
+        return grad, None, *(None for _ in rows)
 
 
-def policy_objective(logits, actions, behaviour_logp, advantages, weights=None, **kw):
-    """policy_loss as a differentiable function of the logits: (loss, logp, kl, entropy). The backward pass reads the
-    logits again instead of keeping a gradient."""
-    return _PolicyObjective.apply(logits, (actions, behaviour_logp, advantages, weights), kw)
+def policy_objective(logits, actions, behaviour_logp, advantages, weights=None, *, legal=None, ref_logp=None,
+                     ref_logits=None, **kw):
+    """policy_loss as a differentiable function of the logits, and of nothing else: (loss, logp, kl, entropy). The
+    backward pass reads the logits and the other tensors again instead of keeping a gradient; one that was written in
+    between makes it raise, as it does with torch's own operators."""
+    return _PolicyObjective.apply(logits, kw, actions, behaviour_logp, advantages, weights, legal, ref_logp, ref_logits)
 
 
 class _PreferenceObjective(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, logits, rows, kw):
+    def forward(ctx, logits, kw, *rows):
         r = preference_loss(logits, *rows, grad=False, **kw)
-        ctx.save_for_backward(logits)
-        ctx.call = rows, kw
+        ctx.save_for_backward(logits, *rows)
+        ctx.kw = kw
         ctx.mark_non_differentiable(r.margins, r.ratios)
         return r.loss, r.margins, r.ratios
 
     @staticmethod
     def backward(ctx, d_loss, *_):
-        rows, kw = ctx.call
-        return preference_loss(ctx.saved_tensors[0], *rows, grad_out=_upstream(d_loss), **kw).grad, None, None
+        logits, *rows = ctx.saved_tensors
+        grad = preference_loss(logits, *rows, grad_out=_upstream(d_loss), **ctx.kw).grad
+        return grad, None, *(None for _ in rows)
 
 
 def preference_objective(logits, tokens, offsets, ref_logp, weights=None, **kw):
-    """preference_loss as a differentiable function of the logits: (loss, margins, ratios)."""
-    return _PreferenceObjective.apply(logits, (tokens, offsets, ref_logp, weights), kw)
+    """preference_loss as a differentiable function of the logits, and of nothing else: (loss, margins, ratios). Its
+    backward pass reads every tensor again, as policy_objective's."""
+    return _PreferenceObjective.apply(logits, kw, tokens, offsets, ref_logp, weights)
 
 
 class _ResidualNorm(torch.autograd.Function):
