@@ -90,7 +90,7 @@ def test_the_training_example_learns_the_search_policy():
     assert pref_last < 0.8 * pref
 
 
-def objective_inputs(vocab=30):
+def objective_inputs(vocab=32):
     g = torch.Generator(device=DEV).manual_seed(4)
     rows = 12
     draw = lambda *shape: torch.randn(*shape, generator=g, device=DEV)  # noqa: E731
@@ -114,7 +114,8 @@ def test_an_objective_whose_batch_was_written_since_refuses_its_backward_pass(wh
     call, kw = ((wl.policy_objective, k), (wl.preference_objective, p))[which]
     loss, *_ = call(x, **kw, **({"kl_coef": 0.1} if which == 0 else {}))
     with torch.no_grad():
-        (x if name == "logits" else kw[name]).add_(0)
+        t = x if name == "logits" else kw[name]
+        t.copy_(t.clone())
     with pytest.raises(RuntimeError, match="modified by an inplace operation"):
         loss.backward()
 
