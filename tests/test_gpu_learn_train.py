@@ -5,6 +5,7 @@ import torch
 import learn_ref as R
 import train_policy
 import warchest_learn as wl
+import warchest_wave as ww
 
 pytestmark = pytest.mark.gpu
 
@@ -130,3 +131,24 @@ def test_objectives_of_a_batch_left_alone_after_other_calls():
     x.grad = None
     one.backward()
     close(x.grad, wl.policy_loss(x.detach(), **k, kl_coef=0.1, entropy_coef=0.01).grad, "policy", 1e-6)
+
+
+@pytest.mark.parametrize("which", ["policy", "preference", "norm", "act_linear8"])
+def test_second_derivatives_are_refused(which):
+    """The gradient itself is given with create_graph too; differentiating it again raises instead of giving 0."""
+    x, k, p = objective_inputs()
+    if which == "policy":
+        y = wl.policy_objective(x, **k, kl_coef=0.1)[0]
+    elif which == "preference":
+        y = wl.preference_objective(x, **p)[0]
+    elif which == "norm":
+        y = (wl.ResidualNorm(32, device=DEV)(x, torch.zeros_like(x))[1] * k["ref_logits"]).sum()
+    else:
+        y = (wl.act_linear8(x, torch.ones(32, 9, device=DEV), "relu") ** 2).sum()
+    [want] = torch.autograd.grad(y, x, retain_graph=True)
+    [got] = torch.autograd.grad(y, x, create_graph=True)
+    assert torch.equal(got.detach(), want) and want.any() and got.requires_grad
+    with pytest.raises(ww.WaveError, match="second derivative"):
+        torch.autograd.grad((got ** 2).sum(), x, retain_graph=True)
+    with pytest.raises(ww.WaveError, match="second derivative"):
+        (got ** 2).sum().backward()

@@ -451,6 +451,32 @@ def checkpoint8_weight_grad(ck, grad, *, act="none", bias=False, dtype=None):
 
 # ------------------------------------------------------- automatic differentiation
 
+class _First(torch.autograd.Function):
+    """A gradient as it is, whose own derivative raises."""
+
+    @staticmethod
+    def forward(ctx, grad, *sources):
+        return grad.view_as(grad)
+
+    @staticmethod
+    def backward(ctx, *_):
+        _fail("a second derivative: the backward passes are native calls without derivatives of their own")
+
+
+def _first_only(backward):
+    """With create_graph the gradients depend on what they were computed from, by a node that raises: torch's own
+    once_differentiable adds none where what arrives is a constant, and such a derivative would be 0."""
+    @functools.wraps(backward)
+    def first(ctx, *arrived):
+        with torch.no_grad():
+            grads = backward(ctx, *arrived)
+        if not torch.is_grad_enabled():
+            return grads
+        sources = [t for t in (*ctx.saved_tensors, *arrived) if t is not None and t.requires_grad]
+        return tuple(None if g is None else _First.apply(g, *sources) for g in grads)
+    return first
+
+
 def _upstream(g):
     return g if g.dtype is torch.float32 else g.float()
 
@@ -471,6 +497,7 @@ class _PolicyObjective(torch.autograd.Function):
                            ref_logits=ref_logits, **kw, **more)
 
     @staticmethod
+    @_first_only
     def backward(ctx, d_loss, *_):
         logits, *rows = ctx.saved_tensors
         grad = _PolicyObjective.call(logits, ctx.kw, *rows, grad_out=_upstream(d_loss)).grad
@@ -495,6 +522,7 @@ class _PreferenceObjective(torch.autograd.Function):
         return r.loss, r.margins, r.ratios
 
     @staticmethod
+    @_first_only
     def backward(ctx, d_loss, *_):
         logits, *rows = ctx.saved_tensors
         grad = preference_loss(logits, *rows, grad_out=_upstream(d_loss), **ctx.kw).grad
@@ -516,6 +544,7 @@ class _ResidualNorm(torch.autograd.Function):
         return r.stream, r.out
 
     @staticmethod
+    @_first_only
     def backward(ctx, d_stream, d_out):
         saved = ctx.saved_tensors
         g = residual_norm_backward(d_out.contiguous(), d_stream.contiguous(), *saved, **ctx.kw)
@@ -544,13 +573,15 @@ class _ActLinear8(torch.autograd.Function):
     @staticmethod
     def forward(ctx, z, weight, act):
         kept, a = checkpoint8_act(z, act)
-        ctx.save_for_backward(kept.q, kept.exps, weight)
+        link = z.new_empty(0)  # an output: leads from the backward pass to z, which is not kept
+        ctx.save_for_backward(kept.q, kept.exps, weight, link)
         ctx.act = act
-        return a @ weight
+        return a @ weight, link
 
     @staticmethod
-    def backward(ctx, d):
-        q, exps, weight = ctx.saved_tensors
+    @_first_only
+    def backward(ctx, d, _):
+        q, exps, weight, _ = ctx.saved_tensors
         kept, d = Checkpoint8(q, exps), d.contiguous()
         d_z = checkpoint8_act_backward(kept, d @ weight.t(), ctx.act) if ctx.needs_input_grad[0] else None
         d_w = None
@@ -562,4 +593,4 @@ class _ActLinear8(torch.autograd.Function):
 def act_linear8(z, weight, act="gelu"):
     """act(z) @ weight (z [rows, width], weight [width, out] of one type), keeping z for the backward pass in 8 bits and
     act(z) not at all: its slope and the weight's gradient are taken from the 8-bit form."""
-    return _ActLinear8.apply(z, weight, act)
+    return _ActLinear8.apply(z, weight, act)[0]
