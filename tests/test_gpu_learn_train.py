@@ -152,3 +152,32 @@ def test_second_derivatives_are_refused(which):
         torch.autograd.grad((got ** 2).sum(), x, retain_graph=True)
     with pytest.raises(ww.WaveError, match="second derivative"):
         (got ** 2).sum().backward()
+
+
+@pytest.mark.parametrize("act", ["none", "relu", "gelu", "silu"])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
+def test_act_linear8_of_every_type_and_activation(dtype, act):
+    """Outputs in the operands' type: half an ulp of the value, as much for each operand rounded on the way (the
+    activation, what arrives through the weight), and 2e-5 of the sums' magnitudes in float32."""
+    g = torch.Generator(device=DEV).manual_seed(5)
+    z = torch.randn(70, 64, generator=g, device=DEV).to(dtype).requires_grad_(True)
+    w = (0.2 * torch.randn(64, 24, generator=g, device=DEV)).to(dtype).requires_grad_(True)
+    d = torch.randn(70, 24, generator=g, device=DEV).to(dtype)
+    y = wl.act_linear8(z, w, act)
+    y.backward(d)
+    assert y.dtype is dtype and z.grad.dtype is dtype and w.grad.dtype is dtype
+    unit = {torch.float32: 0.0, torch.float16: 2.0 ** -11, torch.bfloat16: 2.0 ** -8}[dtype]
+    z64, w64, d64 = (t.detach().cpu().double() for t in (z, w, d))
+    kept = R.keep8(z.detach().cpu())[2].requires_grad_(True)
+    a = R.act(kept, act)
+    a.backward(d64 @ w64.t())
+
+    def held(got, want, size, what):
+        off = (got.detach().cpu().double() - want).abs()
+        assert not (off > 3 * unit * size + 2e-5 * size + 1e-6).any(), (what, float((off / size.clamp(min=1e-9)).max()))
+
+    forward = R.act(z64, act)
+    held(y, forward @ w64, forward.abs() @ w64.abs(), "y")
+    slope = torch.autograd.grad(R.act(kept, act).sum(), kept)[0]
+    held(z.grad, kept.grad, (d64.abs() @ w64.abs().t()) * slope.abs().clamp(min=0.1), "z")
+    held(w.grad, a.detach().t() @ d64, a.detach().abs().t() @ d64.abs(), "w")

@@ -586,11 +586,16 @@ class _ActLinear8(torch.autograd.Function):
         d_z = checkpoint8_act_backward(kept, d @ weight.t(), ctx.act) if ctx.needs_input_grad[0] else None
         d_w = None
         if ctx.needs_input_grad[1]:
-            d_w = checkpoint8_weight_grad(kept, d, act=ctx.act, dtype=weight.dtype)[0]
+            if d.dtype is torch.float32 and ctx.act in ("gelu", "silu"):
+                # not an 8-bit operand any more, and to be kept in 32 bits: a plain product, as the forward's
+                d_w = checkpoint8_read(kept, torch.float32, ctx.act).t() @ d
+            else:
+                d_w = checkpoint8_weight_grad(kept, d, act=ctx.act, dtype=weight.dtype)[0]
         return d_z, d_w, None
 
 
 def act_linear8(z, weight, act="gelu"):
     """act(z) @ weight (z [rows, width], weight [width, out] of one type), keeping z for the backward pass in 8 bits and
-    act(z) not at all: its slope and the weight's gradient are taken from the 8-bit form."""
+    act(z) not at all: its slope and the weight's gradient are taken from the 8-bit form. In float32 with gelu or silu the
+    backward pass makes act(kept) in float32 for the weight's gradient (rows x width x 4 bytes while it runs)."""
     return _ActLinear8.apply(z, weight, act)[0]
