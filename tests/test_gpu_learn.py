@@ -801,3 +801,35 @@ def test_policy_kl_does_not_depend_on_where_the_reference_lies(rows, vocab, dtyp
     check(logits=x, actions=a)
     check(logits=x.flip(1), actions=vocab - 1 - a)
     check(logits=(x.float() + 5000).clamp(min=low).to(t), actions=a)
+
+
+@pytest.mark.parametrize("rows", [2, 64, 200])
+def test_float32_weight_gradient_of_infinite_and_very_large_values(rows):
+    """Infinities, NaN and float32's largest values (past bf16's) in single rows: each product as in float32, the other
+    columns untouched. The one row that holds them has no kept value of 0."""
+    say(f"case weight: float32 ends, {rows} rows")
+    top = torch.finfo(torch.float32).max
+    row = torch.tensor([math.inf, -math.inf, math.nan, top, -3.4e38, 3.39e38, 1.5, -2.0 ** 100])
+    at = rows // 2
+    x = torch.zeros(rows, 40)
+    x[at] = torch.tensor([1.0, -0.5, 0.25, 127 / 256] * 10)
+    x[:at, ::2] = 1.0
+    d = torch.randint(-3, 4, (rows, 8), generator=gen(rows)).float()
+    d[at] = row
+    ck = wl.checkpoint8(x.to(DEV))
+    kept = wl.checkpoint8_read(ck, torch.float32).cpu()
+    assert kept[at].all() and torch.equal(kept[:at], x[:at])
+    small = d.clone()
+    small[at] = 0.0
+    # the sums of the other rows are small whole numbers: added to the row's exact products
+    want = (kept.double().t() @ small.double()) + kept[at].double()[:, None] * row.double()
+    weight, bias = wl.checkpoint8_weight_grad(ck, d.to(DEV), bias=True)
+    total = small.double().sum(0) + row.double()
+    for got, exact in ((weight, want), (bias, total)):
+        got, exact = got.cpu().double(), exact.clamp(-2.0 * top, 2.0 * top)
+        assert torch.equal(got.isnan(), exact.isnan())
+        ends = exact.abs() > top
+        assert torch.equal(got[ends].isinf(), torch.ones_like(got[ends], dtype=torch.bool))
+        assert torch.equal(got[ends] > 0, exact[ends] > 0)
+        fine = ~ends & ~exact.isnan()
+        assert ((got - exact)[fine].abs() <= 2e-6 * exact[fine].abs() + 1e-6).all()

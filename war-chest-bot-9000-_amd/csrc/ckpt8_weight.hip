@@ -72,6 +72,22 @@ struct Operand<float> {
     static constexpr int PARTS = 3;
 };
 
+// The first bf16 of a float32, its upper half: cut, not rounded, so that a value
+// past bf16's largest does not become infinite. A NaN stays one.
+__device__ __forceinline__ float cut(float v) {
+    return v == v ? __uint_as_float(__float_as_uint(v) & 0xFFFF0000u) : v;
+}
+
+// One of a float32's three parts. What an infinity leaves is 0, not infinity
+// less infinity: its products are infinite through the first part alone.
+__device__ __forceinline__ bf16 part_of(float v, int part) {
+    for (int i = 0; i < part; i++) {
+        const float rest = v - cut(v);
+        v = rest == rest ? rest : 0.f;
+    }
+    return (bf16)cut(v);
+}
+
 // One tile: 2 x 2 wavefronts of F x F fragments of 32 x 32.
 template <int F>
 struct Shape {
@@ -240,12 +256,7 @@ __device__ __forceinline__ void products(const wc_ckpt_weight_args& a, const Til
             o = l.g[k];
         } else {
 #pragma unroll
-            for (int i = 0; i < 8; i++) {
-                float v = l.g[k][i];
-                if (plane > 0) v -= (float)(E)v;
-                if (plane > 1) v -= (float)(E)v;
-                o[i] = (E)v;
-            }
+            for (int i = 0; i < 8; i++) o[i] = part_of(l.g[k][i], plane);
         }
         *(E8*)(to + SIDE + (br + k * BR) * PITCH + ((2 * bc) ^ ((br & 3) << 6))) = o;
     };
