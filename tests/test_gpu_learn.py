@@ -833,3 +833,32 @@ def test_float32_weight_gradient_of_infinite_and_very_large_values(rows):
         assert torch.equal(got[ends] > 0, exact[ends] > 0)
         fine = ~ends & ~exact.isnan()
         assert ((got - exact)[fine].abs() <= 2e-6 * exact[fine].abs() + 1e-6).all()
+
+
+@pytest.mark.parametrize("kind", ["logistic", "hinge"])
+def test_preference_at_infinite_margins(kind):
+    """A token of no probability: the margin is infinite. Without smoothing the loss is 0 where it is the rejected one's
+    and infinite where it is the chosen one's, and the slope finite either way."""
+    say(f"case preference: infinite margins, {kind}")
+    x = torch.randn(4, 6, generator=gen(2))
+    tokens, offsets = torch.tensor([0, 1, 2, 3], device=DEV), torch.tensor([0, 1, 2], device=DEV)
+    v = torch.full((4,), -1.5, device=DEV)
+    for lost, loss, slope in ((1, 0.0, 0.0), (0, math.inf, -0.3)):
+        y = x.clone()
+        y[lost, lost] = -math.inf
+        got = wl.preference_loss(y.to(DEV), tokens, offsets, v, beta=0.3, kind=kind)
+        assert float(got.loss) == loss and math.isinf(float(got.margins))
+        p = torch.softmax(y.double(), 1)
+        want = torch.zeros(4, 6, dtype=torch.float64)
+        for r, sign in ((0, 1.0), (1, -1.0)):
+            want[r] = -sign * slope * p[r]
+            want[r, r] += sign * slope
+        near(got.grad, want, "grad", scale=1.0)
+    for smoothing, lost in ((0.1, 0), (0.1, 1), (1.0, 1)):
+        y = x.clone()
+        y[lost, lost] = -math.inf
+        got = wl.preference_loss(y.to(DEV), tokens, offsets, v, beta=0.3, smoothing=smoothing)
+        assert float(got.loss) == math.inf and got.grad.isfinite().all()
+    y = x.clone()
+    y[0, 0] = -math.inf
+    assert float(wl.preference_loss(y.to(DEV), tokens, offsets, v, smoothing=1.0).loss) == 0.0

@@ -789,7 +789,9 @@ __global__ __launch_bounds__(BLOCK) void k_pairs(Pairs p, const float* logp, Row
         double loss, d;
         if (p.kind == WC_PREFERENCE_LOGISTIC) {
             const double e = exp(-fabs(z)), tail = log1p(e);
-            loss = tail + (1.0 - p.smoothing) * fmax(-z, 0.0) + p.smoothing * fmax(z, 0.0);
+            // an infinite margin, and a share of 0 of its infinite term
+            const double far = z > 0.0 ? p.smoothing : 1.0 - p.smoothing;
+            loss = tail + (far > 0.0 ? far * fabs(z) : 0.0);
             d = p.beta * ((z >= 0 ? 1.0 / (1.0 + e) : e / (1.0 + e)) - (1.0 - p.smoothing));
             if (z != z) loss = z;
         } else if (p.kind == WC_PREFERENCE_SQUARED) {
