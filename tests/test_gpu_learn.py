@@ -862,3 +862,37 @@ def test_preference_at_infinite_margins(kind):
     y = x.clone()
     y[0, 0] = -math.inf
     assert float(wl.preference_loss(y.to(DEV), tokens, offsets, v, smoothing=1.0).loss) == 0.0
+
+
+@pytest.mark.parametrize("rows,vocab,dtype", [(3, 50, "f32"), (3, 4099, "bf16"), (2, 33001, "f32"), (2, 70001, "f16")])
+def test_policy_an_infinite_kl_without_a_coefficient_has_no_effect(rows, vocab, dtype):
+    """A reference that gives a column no probability, a reference without any, and an action of no probability: the KL
+    is infinite (undefined without a reference's column), loss and gradient with a coefficient of 0 those without a
+    reference, and with one the loss infinite."""
+    say(f"case policy infinite kl: {rows} x {vocab} {dtype}")
+    coefs = {**COEFS, "kl_coef": 0.0}
+    k = policy_inputs(rows, vocab, TYPES[dtype], vocab, False, "full")
+    k["ref_logits"][0, vocab - 3] = -math.inf
+    dev = {n: to(v) for n, v in k.items()}
+    plain = wl.policy_loss(**{**dev, "ref_logits": None}, **coefs)
+
+    def as_plain(got, plain):
+        near(got.loss, plain.loss.cpu(), "loss", scale=1.0)
+        near(got.grad, plain.grad.cpu(), "grad")
+        near(got.entropy, plain.entropy.cpu(), "entropy")
+        assert got.loss.isfinite() and got.grad.isfinite().all() and got.entropy.isfinite().all()
+
+    got = wl.policy_loss(**dev, **coefs)
+    as_plain(got, plain)
+    assert float(got.kl[0]) == math.inf and got.kl[1:].isfinite().all()
+    assert float(wl.policy_loss(**dev, **COEFS).loss) == math.inf
+    dev["ref_logits"][0] = -math.inf
+    as_plain(wl.policy_loss(**dev, **coefs), plain)
+
+    token = policy_inputs(rows, vocab, TYPES[dtype], vocab, False, "token")
+    token["logits"][0, token["actions"][0]] = -math.inf
+    dev = {n: to(v) for n, v in token.items()}
+    plain = wl.policy_loss(**{**dev, "ref_logp": None}, **coefs)
+    got = wl.policy_loss(**dev, **coefs)
+    as_plain(got, plain)
+    assert float(got.kl[0]) == math.inf and float(wl.policy_loss(**dev, **COEFS).loss) == math.inf

@@ -162,6 +162,11 @@ struct Held {
             for (int i = 0; i < E; i++) v[k][i] = (T)-INFINITY;
         one = (T)-INFINITY;
     }
+    __device__ __forceinline__ void zero() {
+#pragma unroll
+        for (int k = 0; k < NV; k++) v[k] = Raw<T>{};
+        one = (T)0.f;
+    }
     // Takes away what the compiler knows of the logits, so that each pass over
     // them converts them anew: kept as floats from one pass to the next they
     // would not fit the registers.
@@ -394,8 +399,8 @@ struct PolicyRow {
         float slope = first ? -(float)open : 0.f, kl = 0.f, log2_sy = 0.f;
         if (ref_logp) {
             const float d = in.ref - lp, e = expm1f(d);
-            kl = e - d;
-            slope -= kl_coef * e;
+            kl = e == INFINITY ? e : e - d;  // an action of no probability: infinite
+            if (kl_coef != 0.f) slope -= kl_coef * e;
         }
         if (full) {
             log2_sy = __log2f(p.sy);
@@ -403,7 +408,9 @@ struct PolicyRow {
         }
         *out = make_float3(lp, kl, h);
         *g = {p.m, log2_s, p.my, log2_sy, w * slope, w * entropy_coef, h, full ? w * kl_coef : 0.f, kl, 1};
-        return w * ((double)kl_coef * kl - (first ? open : held) - (double)entropy_coef * h);
+        double more = (double)kl_coef * kl;
+        if (kl_coef == 0.f) more = g->my = g->log_sy = g->kl = 0.f;  // without it an infinite KL has no effect either
+        return w * (more - (first ? open : held) - (double)entropy_coef * h);
     }
 };
 
@@ -486,6 +493,7 @@ __global__ __launch_bounds__(group_block<G>(), (group_waves<NV * (FULL ? 2 : 1)>
             }
             if (!TOKEN && grad) {
                 T* to = grad + r * grad_stride;
+                if (FULL && row.kl_coef == 0.f) y.zero();  // no part of the gradient, -infinity among it
                 if (!g.any())
                     put_zero<T, G, NV>(to, n, lane);
                 else if (!FULL && g.ent == 0.f)
@@ -617,7 +625,10 @@ __global__ __launch_bounds__(BLOCK) void k_row_grads(Rows<T> in, int64_t tiles, 
         Held<T, BLOCK, FULL ? NV : 1> y;
         y.one = (T)0.f;
         x.load(in.x + r * in.x_stride + c0, legal, n, threadIdx.x);
-        if constexpr (FULL) y.load(in.y + r * in.y_stride + c0, legal, n, threadIdx.x);
+        if constexpr (FULL) {
+            if (g.klc != 0.f) y.load(in.y + r * in.y_stride + c0, legal, n, threadIdx.x);
+            else y.zero();  // as in k_rows
+        }
         const int at = a >= 0 && a < n ? (int)a : -1;
         if (!FULL && g.ent == 0.f)
             put_grad<T, BLOCK, NV, FULL, true>(to, n, threadIdx.x, x, y, Slope(g, go), in.rate.rate, at);
