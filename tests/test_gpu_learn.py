@@ -789,6 +789,7 @@ def test_policy_kl_does_not_depend_on_where_the_reference_lies(rows, vocab, dtyp
             near(getattr(got, n), want[n], n, scale=max(1.0, float(want[n].abs().max())))
         near(got.loss, want["loss"], "loss", scale=1.0)
         near(got.grad, want["grad"], "grad")
+        assert all(v.isfinite().all() for v in got)
 
     for far in (1e4, -3e4, 6e4):
         check(ref_logits=(k["ref_logits"].float() + far).clamp(low, torch.finfo(t).max).to(t))
