@@ -897,3 +897,16 @@ def test_policy_an_infinite_kl_without_a_coefficient_has_no_effect(rows, vocab, 
     got = wl.policy_loss(**dev, **coefs)
     as_plain(got, plain)
     assert float(got.kl[0]) == math.inf and float(wl.policy_loss(**dev, **COEFS).loss) == math.inf
+
+
+@pytest.mark.parametrize("stride", [8192, (1 << 29) - 8, 1 << 29, (1 << 29) + 8])
+def test_weight_gradient_scratch_of_rows_far_apart(stride):
+    """One row, which a view may give any stride: the scratch that the binding asks for is what the call takes. The same
+    bits as from a plain row."""
+    say(f"case weight: row stride {stride}")
+    g = gen(9)
+    ck = wl.checkpoint8(torch.randn(1, 8192, generator=g).to(DEV))
+    d = torch.randn(1, 8192, generator=g).bfloat16().to(DEV)
+    want, _ = wl.checkpoint8_weight_grad(ck, d, dtype=torch.bfloat16)
+    got, _ = wl.checkpoint8_weight_grad(ck, d.as_strided((1, 8192), (stride, 1)), dtype=torch.bfloat16)
+    assert torch.equal(got, want)

@@ -441,7 +441,9 @@ def checkpoint8_weight_grad(ck, grad, *, act="none", bias=False, dtype=None):
     wcode = _dtype(weight, "dtype")
     b = torch.empty(out, dtype=torch.float32, device=device) if bias else None
     a = _known(ACTS, act, "act")
-    need = _weight_scratch(device.index, code, rows, width, out, a, wcode, (g[0] | 2 * g[1] | 2 * out) % 16 == 0)
+    # (rows 2^29 elements apart count as unaligned: the library copies them)
+    aligned = (g[0] | 2 * g[1] | 2 * out) % 16 == 0 and g[1] < 1 << 29
+    need = _weight_scratch(device.index, code, rows, width, out, a, wcode, aligned)
     held, work = _scratch(need, device)
     _call("wc_ckpt_weight_grad", _WEIGHT.pack(
         _WEIGHT.size, device.index, code, rows, width, out, a, wcode, *q, *e, *g, weight.data_ptr(), out,
