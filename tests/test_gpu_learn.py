@@ -910,3 +910,135 @@ def test_weight_gradient_scratch_of_rows_far_apart(stride):
     want, _ = wl.checkpoint8_weight_grad(ck, d, dtype=torch.bfloat16)
     got, _ = wl.checkpoint8_weight_grad(ck, d.as_strided((1, 8192), (stride, 1)), dtype=torch.bfloat16)
     assert torch.equal(got, want)
+
+
+# ---------------------------------------------------------- rows in chunks
+
+def held_to(got, want, what, scale=None):
+    """near, and no NaN where the definition has none."""
+    assert torch.equal(got.isnan().cpu(), want.isnan()), what
+    near(got, want, what, scale)
+
+
+@pytest.mark.parametrize("ref", ["none", "token", "full"])
+@pytest.mark.parametrize("vocab,dtype", [(70001, "f32"), (140001, "f16"), (140001, "bf16")])
+def test_policy_rows_in_chunks(vocab, dtype, ref):
+    """Rows past what registers hold, read in chunks of 8,192 columns: legal columns with a whole chunk of them illegal
+    (NaN and infinities there), a row whose only legal columns are in the last chunk, rows left out of each kind, strided
+    rows with NaN between; without a gradient, and with the gradient over the logits."""
+    say(f"case policy in chunks: {vocab} {dtype} ref {ref}")
+    t = TYPES[dtype]
+    k = policy_inputs(9, vocab, t, vocab, True, ref)
+    row = torch.arange(9)
+    k["legal"][:, 16384:24576] = False
+    k["actions"] = torch.where(k["legal"][row, k["actions"]], k["actions"], k["legal"].int().argmax(1))
+    k["weights"][0], k["logits"][0] = 0.0, math.nan
+    k["actions"][1], k["actions"][2] = -3, vocab
+    k["legal"][3] = False
+    k["legal"][4, k["actions"][4]] = False
+    k["legal"][5, : vocab - 40] = False
+    k["legal"][5, vocab - 9] = True
+    k["actions"][5] = vocab - 9
+    k["logits"][6] = torch.where(k["legal"][6], k["logits"][6], torch.tensor(math.nan, dtype=t))
+    k["logits"][7] = torch.where(k["legal"][7], k["logits"][7], torch.tensor(math.inf, dtype=t))
+    k["logits"][8, :8192] = -math.inf
+    k["actions"][8] = 8192 + int(k["legal"][8, 8192:].int().argmax())
+    # (where a row has no legal column, or an action none, any number does)
+    lp = torch.log_softmax(k["logits"].double().masked_fill(~k["legal"], -math.inf) * COEFS["inv_temperature"], 1)
+    lp = lp[row, k["actions"].clamp(0, vocab - 1)].nan_to_num(neginf=0.0).float()
+    k["behaviour_logp"] = lp + 0.1
+    if ref == "token":
+        k["ref_logp"] = lp - 0.3
+    want = R.policy(**k, **COEFS)
+    dev = {n: to(v) for n, v in k.items()} | {"logits": strided(k["logits"], 3)}
+    got = wl.policy_loss(**dev, **COEFS)
+    for n in ("logp", "kl", "entropy"):
+        held_to(getattr(got, n), want[n], n, scale=max(1.0, float(want[n].abs().max())))
+    held_to(got.loss, want["loss"], "loss", scale=max(1.0, abs(float(want["loss"]))))
+    held_to(got.grad, want["grad"], "grad")
+    assert not got.grad[:5].any() and not got.logp[:5].any()
+    only = wl.policy_loss(**dev, **COEFS, grad=False)
+    assert only.grad is None
+    for a, b in zip(got[1:4], only[1:4]):
+        assert torch.equal(a, b)
+    held_to(only.loss, got.loss.cpu(), "loss without a gradient", scale=max(1.0, abs(float(want["loss"]))))
+    over = wl.policy_loss(**dev, **COEFS, grad=dev["logits"])
+    assert torch.equal(over.loss, got.loss) and torch.equal(dev["logits"], got.grad)
+
+
+@pytest.mark.parametrize("kind,average", [("logistic", True), ("squared", False), ("hinge", True)])
+@pytest.mark.parametrize("vocab,dtype", [(70001, "f32"), (140001, "f16"), (140001, "bf16")])
+def test_preference_rows_in_chunks(vocab, dtype, kind, average):
+    """Rows past what registers hold: ragged pairs, a row left out of each kind, a chunk at -infinity; without a gradient,
+    and with the gradient over the logits."""
+    say(f"case preference in chunks: {vocab} {dtype} {kind} average {average}")
+    k = preference_inputs([2, 3, 0, 4], vocab, TYPES[dtype], vocab, lead=1, tail=1)
+    k["weights"][:] = torch.linspace(0.5, 1.5, len(k["weights"]))
+    k["weights"][2], k["logits"][2] = 0.0, math.nan
+    k["tokens"][4] = vocab
+    k["logits"][5] = -math.inf
+    k["logits"][6, 8192:16384] = -math.inf
+    k["tokens"][6] = vocab - 1
+    k["ref_logp"][6] = -10.0
+    kw = dict(beta=0.3, smoothing=0.1, kind=kind, average=average, inv_temperature=0.8)
+    want = R.preference(**k, **kw)
+    dev = {n: to(v) for n, v in k.items()} | {"logits": strided(k["logits"], 5)}
+    got = wl.preference_loss(**dev, **kw)
+    for n in ("margins", "ratios", "logp"):
+        held_to(getattr(got, n), want[n], n, scale=max(1.0, float(want[n].abs().max())))
+    held_to(got.loss, want["loss"], "loss", scale=max(1.0, abs(float(want["loss"]))))
+    held_to(got.grad, want["grad"], "grad", scale=max(1e-3, float(want["grad"].abs().max())))
+    assert not got.grad[[0, 2, 4, 5, -1]].any()
+    only = wl.preference_loss(**dev, **kw, grad=False)
+    for a, b in zip(got[1:4], only[1:4]):
+        assert torch.equal(a, b)
+    held_to(only.loss, got.loss.cpu(), "loss without a gradient", scale=1.0)
+    over = wl.preference_loss(**dev, **kw, grad=dev["logits"])
+    assert torch.equal(over.loss, got.loss) and torch.equal(dev["logits"], got.grad)
+
+
+@pytest.mark.parametrize("step", [0.02, 0.05])
+def test_policy_gradient_against_differences_of_the_loss_per_row(step):
+    """Rows of weight 1. Differences of the float64 loss are off by 2.2e-6 at 0.02 and 1.3e-5 at 0.05 here; a float32 loss
+    of up to 4 adds 2^-22 twice over 2 steps, 1.2e-5 at 0.02, and its own terms' rounding as much: 1e-4."""
+    k = policy_inputs(3, 6, torch.float32, 11, True, "full")
+    k["weights"] = torch.ones(3)
+    dev = {n: to(v) for n, v in k.items()}
+    grad = wl.policy_loss(**dev, **COEFS).grad.cpu()
+    for i in range(18):
+        ends = []
+        for s in (step, -step):
+            x = k["logits"].clone()
+            x.view(-1)[i] += s
+            ends.append(float(wl.policy_loss(**{**dev, "logits": x.to(DEV)}, **COEFS, grad=False).loss))
+        assert abs((ends[0] - ends[1]) / (2 * step) - float(grad.view(-1)[i])) < 1e-4
+
+
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("rows,width", [(1, 1), (3, 8), (2, 31), (65, 100), (33, 513), (5, 1153), (9, 4099), (2, 9001)])
+def test_finite_inputs_give_finite_outputs(rows, width, dtype):
+    """A comparison with a bound lets a NaN pass: every output of every operator, over sizes of each kernel."""
+    say(f"case finite: {rows} x {width} {dtype}")
+    t = TYPES[dtype]
+    outs = []
+    for legal, ref in ((False, "none"), (True, "token"), (True, "full")):
+        k = policy_inputs(rows, width, t, rows + width, legal, ref)
+        outs += wl.policy_loss(**{n: to(v) for n, v in k.items()}, **COEFS)
+    k = preference_inputs([rows, rows // 2, 0, 1], width, t, rows)
+    for kind in ("logistic", "squared", "hinge"):
+        outs += wl.preference_loss(**{n: to(v) for n, v in k.items()}, kind=kind, average=True)
+    for kind, gate, act in (("rms", "none", "none"), ("layer", "vector", "tanh"), ("layer", "token", "sigmoid")):
+        k, d = norm_inputs(rows, width, t, rows + width, kind, gate)
+        v = {n: to(x) for n, x in k.items()}
+        f = wl.residual_norm(**v, norm=kind, gate_act=act)
+        b = wl.residual_norm_backward(to(d[0]), to(d[1]), v["block"], v["stream"], f.stats, *(
+            v[n] for n in ("post_gain", "post_bias", "gate", "pre_gain", "pre_bias")), norm=kind, gate_act=act)
+        outs += [x for x in (*f, *b) if x is not None]
+    x = to(norm_inputs(rows, width, t, 1, "rms", "none")[0]["block"])
+    for act in ("none", "relu", "gelu", "silu"):
+        ck, y = wl.checkpoint8_act(x, act)
+        outs += [y, wl.checkpoint8_read(ck, t, act), wl.checkpoint8_act_backward(ck, x, act)]
+        if dtype != "f32" or act in ("none", "relu"):
+            outs += wl.checkpoint8_weight_grad(ck, x[:, : (width + 1) // 2], act=act, bias=True)
+    for i, o in enumerate(outs):
+        assert o.isfinite().all(), i
