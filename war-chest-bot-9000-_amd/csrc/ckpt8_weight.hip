@@ -72,20 +72,30 @@ struct Operand<float> {
     static constexpr int PARTS = 3;
 };
 
-// The first bf16 of a float32, its upper half: cut, not rounded, so that a value
-// past bf16's largest does not become infinite. A NaN stays one.
-__device__ __forceinline__ float cut(float v) {
-    return v == v ? __uint_as_float(__float_as_uint(v) & 0xFFFF0000u) : v;
-}
+// The first of a float32's three parts is its upper half: cut, not rounded, so
+// that a value past bf16's largest does not become infinite. (The mark of a quiet
+// NaN, as arithmetic leaves it, is in that half too.)
+__device__ __forceinline__ float cut(float v) { return __uint_as_float(__float_as_uint(v) & 0xFFFF0000u); }
 
-// One of a float32's three parts. What an infinity leaves is 0, not infinity
-// less infinity: its products are infinite through the first part alone.
-__device__ __forceinline__ bf16 part_of(float v, int part) {
-    for (int i = 0; i < part; i++) {
-        const float rest = v - cut(v);
-        v = rest == rest ? rest : 0.f;
+// One of the three parts of eight values. What an infinity leaves is 0, not
+// infinity less infinity: its products are infinite through the first part alone.
+__device__ __forceinline__ bf16x8 part_of(const Vec8<float>::type& v, int part) {
+    typedef uint32_t Words __attribute__((ext_vector_type(4)));
+    uint32_t u[8];
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+        float x = v[i];
+        if (part > 0) {
+            x -= cut(x);
+            x = x == x ? x : 0.f;
+        }
+        if (part > 1) x -= cut(x);
+        u[i] = __float_as_uint(x);
     }
-    return (bf16)cut(v);
+    Words w;
+#pragma unroll
+    for (int i = 0; i < 4; i++) w[i] = __builtin_amdgcn_perm(u[2 * i + 1], u[2 * i], 0x07060302);  // both upper halves
+    return __builtin_bit_cast(bf16x8, w);
 }
 
 // One tile: 2 x 2 wavefronts of F x F fragments of 32 x 32.
@@ -255,8 +265,7 @@ __device__ __forceinline__ void products(const wc_ckpt_weight_args& a, const Til
         if constexpr (PARTS == 1) {
             o = l.g[k];
         } else {
-#pragma unroll
-            for (int i = 0; i < 8; i++) o[i] = part_of(l.g[k][i], plane);
+            o = part_of(l.g[k], plane);
         }
         *(E8*)(to + SIDE + (br + k * BR) * PITCH + ((2 * bc) ^ ((br & 3) << 6))) = o;
     };
