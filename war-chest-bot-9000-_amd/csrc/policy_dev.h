@@ -162,11 +162,6 @@ struct Held {
             for (int i = 0; i < E; i++) v[k][i] = (T)-INFINITY;
         one = (T)-INFINITY;
     }
-    __device__ __forceinline__ void zero() {
-#pragma unroll
-        for (int k = 0; k < NV; k++) v[k] = Raw<T>{};
-        one = (T)0.f;
-    }
     // Takes away what the compiler knows of the logits, so that each pass over
     // them converts them anew: kept as floats from one pass to the next they
     // would not fit the registers.
@@ -308,7 +303,8 @@ struct Slope {
     float m, log_s, my, log_sy, base, slope, toward, hit;
 
     __device__ __forceinline__ Slope(const RowGrad& g, float go)
-        : m(g.m), log_s(g.log_s), my(g.my), log_sy(g.log_sy), base(go * (g.ent * g.h - g.klc * g.kl - g.coef)),
+        : m(g.m), log_s(g.log_s), my(g.klc != 0.f ? g.my : 0.f), log_sy(g.klc != 0.f ? g.log_sy : 0.f),
+          base(go * (g.ent * g.h - (g.klc != 0.f ? g.klc * g.kl : 0.f) - g.coef)),
           slope(go * (g.ent + g.klc) * LN2), toward(go * g.klc * LN2), hit(go * g.coef) {}
 
     template <bool FULL, bool PLAIN>
@@ -316,7 +312,8 @@ struct Slope {
         const float lp = (x - m) * rate - log_s, p = power(lp);
         if (PLAIN) return p * base;
         float d = base + slope * lp;
-        if (FULL) d -= toward * ((y - my) * rate - log_sy);
+        // finite: a reference of no probability has no effect where the KL has no coefficient
+        if (FULL) d -= toward * fmaxf((y - my) * rate - log_sy, -3.4028234663852886e38f);
         return p == 0.f ? 0.f : p * d;
     }
 };
@@ -408,9 +405,9 @@ struct PolicyRow {
         }
         *out = make_float3(lp, kl, h);
         *g = {p.m, log2_s, p.my, log2_sy, w * slope, w * entropy_coef, h, full ? w * kl_coef : 0.f, kl, 1};
-        double more = (double)kl_coef * kl;
-        if (kl_coef == 0.f) more = g->my = g->log_sy = g->kl = 0.f;  // without it an infinite KL has no effect either
-        return w * (more - (first ? open : held) - (double)entropy_coef * h);
+        // an infinite KL has no effect where its coefficient is 0 (here and in Slope: a choice for each
+        // term; one that several terms hang on cost 10 registers, and 10% of 800,000 x 12 float32)
+        return w * ((double)kl_coef * (kl_coef != 0.f ? kl : 0.f) - (first ? open : held) - (double)entropy_coef * h);
     }
 };
 
@@ -493,7 +490,6 @@ __global__ __launch_bounds__(group_block<G>(), (group_waves<NV * (FULL ? 2 : 1)>
             }
             if (!TOKEN && grad) {
                 T* to = grad + r * grad_stride;
-                if (FULL && row.kl_coef == 0.f) y.zero();  // no part of the gradient, -infinity among it
                 if (!g.any())
                     put_zero<T, G, NV>(to, n, lane);
                 else if (!FULL && g.ent == 0.f)
@@ -625,10 +621,7 @@ __global__ __launch_bounds__(BLOCK) void k_row_grads(Rows<T> in, int64_t tiles, 
         Held<T, BLOCK, FULL ? NV : 1> y;
         y.one = (T)0.f;
         x.load(in.x + r * in.x_stride + c0, legal, n, threadIdx.x);
-        if constexpr (FULL) {
-            if (g.klc != 0.f) y.load(in.y + r * in.y_stride + c0, legal, n, threadIdx.x);
-            else y.zero();  // as in k_rows
-        }
+        if constexpr (FULL) y.load(in.y + r * in.y_stride + c0, legal, n, threadIdx.x);
         const int at = a >= 0 && a < n ? (int)a : -1;
         if (!FULL && g.ent == 0.f)
             put_grad<T, BLOCK, NV, FULL, true>(to, n, threadIdx.x, x, y, Slope(g, go), in.rate.rate, at);
@@ -766,67 +759,65 @@ __device__ __forceinline__ int64_t clamp_row(int64_t x, int64_t rows) { return x
 
 // One pair per workgroup: both sequences' ratios in 64-bit sums (long sums of
 // differences that nearly cancel), the pair's loss, and the coefficient of
-// every row of both. 6 to 9 us of dependent loads; the pairs side by side, up
-// to what a launch's threads can be counted in 32 bits.
+// every row of both. 6 to 9 us of dependent loads; the pairs side by side, in
+// launches whose threads 32 bits can count.
 constexpr int64_t MOST_PAIR_BLOCKS = 1 << 22;
-__global__ __launch_bounds__(BLOCK) void k_pairs(Pairs p, const float* logp, RowGrad* grads, double* losses,
-                                                 float* margins, float* ratios) {
+__global__ __launch_bounds__(BLOCK) void k_pairs(Pairs p, int64_t first, const float* logp, RowGrad* grads,
+                                                 double* losses, float* margins, float* ratios) {
     __shared__ double lds[4][BLOCK / 64];
-    for (int64_t i = blockIdx.x; i < p.pairs; i += gridDim.x) {
-        int64_t lo[2], hi[2];
-        double sum[4] = {};
-        for (int k = 0; k < 2; k++) {
-            lo[k] = clamp_row(index_at(p.offsets, p.bits, 2 * i + k), p.rows);
-            hi[k] = clamp_row(index_at(p.offsets, p.bits, 2 * i + k + 1), p.rows);
-            for (int64_t r = lo[k] + threadIdx.x; r < hi[k]; r += BLOCK) {
-                if (!grads[r].on) continue;
-                const float w = p.weights ? p.weights[r] : 1.f;
-                sum[2 * k] += (double)w * ((double)logp[r] - p.ref_logp[r]);
-                sum[2 * k + 1] += w;
-            }
+    const int64_t i = first + blockIdx.x;
+    int64_t lo[2], hi[2];
+    double sum[4] = {};
+    for (int k = 0; k < 2; k++) {
+        lo[k] = clamp_row(index_at(p.offsets, p.bits, 2 * i + k), p.rows);
+        hi[k] = clamp_row(index_at(p.offsets, p.bits, 2 * i + k + 1), p.rows);
+        for (int64_t r = lo[k] + threadIdx.x; r < hi[k]; r += BLOCK) {
+            if (!grads[r].on) continue;
+            const float w = p.weights ? p.weights[r] : 1.f;
+            sum[2 * k] += (double)w * ((double)logp[r] - p.ref_logp[r]);
+            sum[2 * k + 1] += w;
         }
-        for (int q = 0; q < 4; q++) {
-            for (int mask = 32; mask; mask >>= 1) sum[q] += __shfl_xor(sum[q], mask);
-            if ((threadIdx.x & 63) == 0) lds[q][threadIdx.x >> 6] = sum[q];
-        }
-        __syncthreads();
-        for (int q = 0; q < 4; q++) sum[q] = (lds[q][0] + lds[q][1]) + (lds[q][2] + lds[q][3]);
-        double share[2], ratio[2];
-        for (int k = 0; k < 2; k++) {
-            share[k] = !p.average ? 1.0 : sum[2 * k + 1] != 0.0 ? 1.0 / sum[2 * k + 1] : 0.0;
-            ratio[k] = sum[2 * k] * share[k];
-        }
-        const double h = ratio[0] - ratio[1], z = p.beta * h;
-        double loss, d;
-        if (p.kind == WC_PREFERENCE_LOGISTIC) {
-            const double e = exp(-fabs(z)), tail = log1p(e);
-            // an infinite margin, and a share of 0 of its infinite term
-            const double far = z > 0.0 ? p.smoothing : 1.0 - p.smoothing;
-            loss = tail + (far > 0.0 ? far * fabs(z) : 0.0);
-            d = p.beta * ((z >= 0 ? 1.0 / (1.0 + e) : e / (1.0 + e)) - (1.0 - p.smoothing));
-            if (z != z) loss = z;
-        } else if (p.kind == WC_PREFERENCE_SQUARED) {
-            const double t = h - 0.5 / p.beta;
-            loss = t * t;
-            d = 2.0 * t;
-        } else {
-            loss = z < 1.0 ? 1.0 - z : 0.0;
-            d = z < 1.0 ? -(double)p.beta : 0.0;
-            if (z != z) loss = d = z;
-        }
-        d /= (double)p.pairs;
-        for (int k = 0; k < 2; k++) {
-            const float c = (float)((k ? -d : d) * share[k]);
-            for (int64_t r = lo[k] + threadIdx.x; r < hi[k]; r += BLOCK)
-                if (grads[r].on) grads[r].coef = c * (p.weights ? p.weights[r] : 1.f);
-        }
-        if (threadIdx.x == 0) {
-            losses[i] = loss;
-            margins[i] = (float)z;
-            ratios[2 * i] = (float)ratio[0];
-            ratios[2 * i + 1] = (float)ratio[1];
-        }
-        __syncthreads();  // the sums have been read
+    }
+    for (int q = 0; q < 4; q++) {
+        for (int mask = 32; mask; mask >>= 1) sum[q] += __shfl_xor(sum[q], mask);
+        if ((threadIdx.x & 63) == 0) lds[q][threadIdx.x >> 6] = sum[q];
+    }
+    __syncthreads();
+    for (int q = 0; q < 4; q++) sum[q] = (lds[q][0] + lds[q][1]) + (lds[q][2] + lds[q][3]);
+    double share[2], ratio[2];
+    for (int k = 0; k < 2; k++) {
+        share[k] = !p.average ? 1.0 : sum[2 * k + 1] != 0.0 ? 1.0 / sum[2 * k + 1] : 0.0;
+        ratio[k] = sum[2 * k] * share[k];
+    }
+    const double h = ratio[0] - ratio[1], z = p.beta * h;
+    double loss, d;
+    if (p.kind == WC_PREFERENCE_LOGISTIC) {
+        const double e = exp(-fabs(z)), tail = log1p(e);
+        // an infinite margin, and a share of 0 of its infinite term
+        const double far = z > 0.0 ? p.smoothing : 1.0 - p.smoothing;
+        loss = tail + (far > 0.0 ? far * fabs(z) : 0.0);
+        d = p.beta * ((z >= 0 ? 1.0 / (1.0 + e) : e / (1.0 + e)) - (1.0 - p.smoothing));
+        if (z != z) loss = z;
+    } else if (p.kind == WC_PREFERENCE_SQUARED) {
+        const double t = h - 0.5 / p.beta;
+        loss = t * t;
+        d = 2.0 * t;
+    } else {
+        loss = z < 1.0 ? 1.0 - z : 0.0;
+        d = z < 1.0 ? -(double)p.beta : 0.0;
+        if (z != z) loss = d = z;
+    }
+    d /= (double)p.pairs;
+    for (int k = 0; k < 2; k++) {
+        const float c = (float)((k ? -d : d) * share[k]);
+        for (int64_t r = lo[k] + threadIdx.x; r < hi[k]; r += BLOCK)
+            if (grads[r].on) grads[r].coef = c * (p.weights ? p.weights[r] : 1.f);
+    }
+    if (threadIdx.x == 0) {
+        losses[i] = loss;
+        margins[i] = (float)z;
+        ratios[2 * i] = (float)ratio[0];
+        ratios[2 * i + 1] = (float)ratio[1];
     }
 }
 
@@ -849,9 +840,9 @@ void preference(const wc_preference_args& a, hipStream_t s) {
     }
     const Pairs p = {a.offsets, a.ref_logp, a.weights, a.rows, a.pairs, a.beta, a.smoothing, a.kind, a.average,
                      a.index_bits};
-    if (a.pairs)
-        k_pairs<<<dim3((uint32_t)std::min(a.pairs, MOST_PAIR_BLOCKS)), BLOCK, 0, s>>>(p, a.logp, grads, losses, a.margins,
-                                                                                      a.ratios);
+    for (int64_t i = 0; i < a.pairs; i += MOST_PAIR_BLOCKS)
+        k_pairs<<<dim3((uint32_t)std::min(a.pairs - i, MOST_PAIR_BLOCKS)), BLOCK, 0, s>>>(p, i, a.logp, grads, losses,
+                                                                                          a.margins, a.ratios);
     const LossSum sum = {losses, a.pairs, a.pairs ? 1.0 / (double)a.pairs : 0.0, a.loss};
     if (a.grad && a.rows)
         k_row_grads<T, false><<<tile_grid(tiles) + 1, BLOCK, 0, s>>>(in, tiles, splits, grads, a.grad_out, (T*)a.grad,
