@@ -43,7 +43,10 @@ extern "C" {
  *   loss = sum of weight * row loss
  * KL is expm1(d) - d with d = ref_logp - logp_a where ref_logp is given, or the
  * whole sum of p (logp - logq), q the softmax of inv_temperature * ref_logits
- * over the same legal columns, where ref_logits is given (not both), or 0.
+ * over the same legal columns, where ref_logits is given (not both), or 0. It is
+ * infinite where q leaves out a column that p does not, or the action has no
+ * probability, and so is the loss then; with a kl_coef of 0 it has no part in loss
+ * and gradient, whatever it is.
  *
  * A row is left out (its outputs and gradient are 0, its logits are not read
  * or have no effect) when its weight is 0, its action is outside [0, vocab) or
@@ -247,8 +250,10 @@ int wc_ckpt_act_backward(const wc_ckpt_args* a, void* stream);
  * bias[j] = sum over rows of grad[r][j]. Products on the matrix cores in grad's
  * 16-bit type with float32 sums: kept values are exact in bf16, and in f16
  * within f16's range (larger ones are taken as its largest, steps under 2^-24
- * are rounded); an activation recomputed from them is rounded to that type. float32 grad is taken with
- * WC_ACT_NONE and WC_ACT_RELU, as three bf16 parts whose products are exact. */
+ * are rounded); a GELU or SiLU recomputed from them is rounded to that type, for a
+ * float32 weight too: less than what the 8 bits left out. float32 grad is taken with
+ * WC_ACT_NONE and WC_ACT_RELU, as three bf16 parts whose products are exact (what of
+ * a part is under 2^-133 is lost: grad's last bits below 2^-110). */
 typedef struct wc_ckpt_weight_args {
     uint64_t bytes;
     int32_t device, dtype;      /* of grad */

@@ -342,7 +342,7 @@ def residual_norm_backward(d_out, d_stream, block, stream, stats, post_gain=None
 
     d_out arrives at out, d_stream at stream' (either may be None: 0). Returns ResidualNormGrads(block, stream,
     post_gain, post_bias, gate, pre_gain, pre_bias): matrices in the inputs' type, parameters in float32, None for a
-    parameter that was None."""
+    parameter that was None. The forward's keyword arguments fit: eps is in its stats already."""
     device, code, pcode, rows, width, b, s, pg, pb, g, ng, _ = _norm_inputs(block, stream, post_gain, post_bias, gate,
                                                                             pre_gain, pre_bias)
     dt, f32 = block.dtype, torch.float32
@@ -431,7 +431,8 @@ def checkpoint8_act_backward(ck, grad, act):
 
 def checkpoint8_weight_grad(ck, grad, *, act="none", bias=False, dtype=None):
     """(weight, bias): weight [width, out] = act(kept)^T grad, the gradient of x @ weight; bias [out] float32 = grad's
-    column sums (None unless asked for) (wc_ckpt_weight_grad). dtype: float32 (the default) or grad's."""
+    column sums (None unless asked for) (wc_ckpt_weight_grad). dtype: float32 (the default) or grad's. gelu and silu are
+    taken with a 16-bit grad, and rounded to its type; checkpoint8_read gives them in float32 for a plain product."""
     device, rows, width, q, e = _kept(ck)
     if _device(grad, "grad") != device or grad.dim() != 2:
         _fail(f"grad: shape {tuple(grad.shape)} on {grad.device}, expected rows x out on {device}")
