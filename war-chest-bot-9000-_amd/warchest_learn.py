@@ -471,10 +471,10 @@ def _first_only(backward):
     once_differentiable adds none where what arrives is a constant, and such a derivative would be 0."""
     @functools.wraps(backward)
     def first(ctx, *arrived):
+        if not torch.is_grad_enabled():
+            return backward(ctx, *arrived)
         with torch.no_grad():
             grads = backward(ctx, *arrived)
-        if not torch.is_grad_enabled():
-            return grads
         sources = [t for t in (*ctx.saved_tensors, *arrived) if t is not None and t.requires_grad]
         return tuple(None if g is None else _First.apply(g, *sources) for g in grads)
     return first
@@ -578,6 +578,7 @@ class _ActLinear8(torch.autograd.Function):
         kept, a = checkpoint8_act(z, act)
         link = z.new_empty(0)  # an output: leads from the backward pass to z, which is not kept
         ctx.save_for_backward(kept.q, kept.exps, weight, link)
+        ctx.set_materialize_grads(False)  # nothing arrives at link
         ctx.act = act
         return a @ weight, link
 
