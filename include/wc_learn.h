@@ -274,6 +274,155 @@ typedef struct wc_ckpt_weight_args {
 int wc_ckpt_weight_workspace(const wc_ckpt_weight_args* a, uint64_t* bytes);
 int wc_ckpt_weight_grad(const wc_ckpt_weight_args* a, void* stream);
 
+/* ------------------------------------------------------------- linear layer
+ * y = act(x W + bias) + residual, one product with its epilogue: sums, bias,
+ * activation and residual in float32, rounded once to y's type. W is width x
+ * out (WC_WEIGHT_IN_OUT) or out x width (WC_WEIGHT_OUT_IN, a row an output).
+ * pre, where given, gets x W + bias rounded to its type, for the backward pass.
+ * 16-bit matrices: products on the matrix cores with float32 sums. float32: as
+ * three bf16 parts an element and six products of parts (what is left out is
+ * below 2^-25 of a product); an infinite element's row or column of the result is not finite,
+ * and may be NaN where its product alone would be infinite.
+ * rows below 2^31, width and out at most 2^20. */
+#define WC_WEIGHT_IN_OUT 0
+#define WC_WEIGHT_OUT_IN 1
+typedef struct wc_linear_args {
+    uint64_t bytes;
+    int32_t device, dtype;      /* of every matrix */
+    int32_t bias_dtype, weight_layout; /* bias: float32 or the matrices' */
+    int64_t rows, width, out;
+    const void* x;              /* rows x width */
+    int64_t x_stride;
+    const void* weight;
+    int64_t weight_stride;
+    const void* bias;           /* out; NULL: 0 */
+    const void* residual;       /* rows x out; NULL: 0 */
+    int64_t residual_stride;
+    int32_t act, pad;           /* WC_ACT_* */
+    void* pre;                  /* rows x out; NULL: not kept */
+    int64_t pre_stride;
+    void* y;                    /* rows x out; may be residual itself */
+    int64_t y_stride;
+    void* workspace;
+    uint64_t workspace_bytes;
+} wc_linear_args;
+int wc_linear_workspace(const wc_linear_args* a, uint64_t* bytes);
+int wc_linear(const wc_linear_args* a, void* stream);
+
+/* Its gradients: d_pre = d_out act'(pre), d_x = d_pre W^T, d_weight = x^T d_pre
+ * in the weight's layout, d_bias = the column sums of d_pre, each NULL where not
+ * wanted (the residual's gradient is d_out). d_pre is rounded to the matrices'
+ * type for its products; d_bias is summed before that, in float32. */
+typedef struct wc_linear_back_args {
+    uint64_t bytes;
+    int32_t device, dtype;
+    int32_t weight_layout, act;
+    int32_t grad_dtype, pad;    /* of d_weight: float32 or the matrices' */
+    int64_t rows, width, out;
+    const void* d_out;          /* rows x out */
+    int64_t d_out_stride;
+    const void* pre;            /* rows x out; with WC_ACT_NONE not read */
+    int64_t pre_stride;
+    const void* x;              /* read for d_weight */
+    int64_t x_stride;
+    const void* weight;         /* read for d_x */
+    int64_t weight_stride;
+    void* d_x;                  /* rows x width */
+    int64_t d_x_stride;
+    void* d_weight;
+    int64_t d_weight_stride;
+    float* d_bias;              /* out */
+    void* workspace;
+    uint64_t workspace_bytes;
+} wc_linear_back_args;
+int wc_linear_backward_workspace(const wc_linear_back_args* a, uint64_t* bytes);
+int wc_linear_backward(const wc_linear_back_args* a, void* stream);
+
+/* ------------------------------------------------------------ orthogonalise
+ * A matrix's singular values brought towards 1 (a weight's update, before it is
+ * applied): X = update / (Frobenius norm + eps), then `steps` times
+ *   A = X X^T, X = a X + (b A + c A A) X
+ * (the transposed form where rows > width), and out = scale X. `batch` matrices
+ * of one shape. X is held in 22 bits an element, A and its polynomial too, but
+ * for a bf16 result of more than 128 rows and columns in 11 (off by about as much
+ * as that result's rounding); sums are float32, the norm's float64.
+ * Coefficients that let a singular value pass 60 overflow (infinities, NaN). */
+typedef struct wc_orthogonalise_args {
+    uint64_t bytes;
+    int32_t device, dtype;      /* of update */
+    int32_t out_dtype, steps;   /* steps: 1 .. 64 */
+    int64_t batch, rows, width; /* batch at most 65535, rows and width 2^20 */
+    const void* update;
+    int64_t update_stride, update_batch; /* elements from row to row, from matrix to matrix */
+    void* out;                  /* may be update itself */
+    int64_t out_stride, out_batch;
+    float a, b, c, eps, scale;
+    int32_t pad;
+    void* workspace;
+    uint64_t workspace_bytes;
+} wc_orthogonalise_args;
+int wc_orthogonalise_workspace(const wc_orthogonalise_args* a, uint64_t* bytes);
+int wc_orthogonalise(const wc_orthogonalise_args* a, void* stream);
+
+/* ------------------------------------------------- token log-probabilities
+ * Of rows of logits, over their legal columns:
+ *   z = inv_temperature * logits, logp = z - log sum exp z, p = exp logp
+ *   logp of the row's token, its rank (how many columns have a larger logit, or
+ *   an equal one and a lower index; 0: the likeliest), the entropy -sum p logp,
+ *   and the `top` likeliest columns in that order with their log-probabilities.
+ * A row is left out (logp and entropy 0, rank -1, its logits not read) when its
+ * token is outside [0, vocab) or no legal logit is above -infinity. A token that
+ * is not legal, or whose logit is -infinity, has logp -infinity. Alternatives
+ * are columns above -infinity: where there are fewer than `top`, and in a row
+ * that is left out, the others are column -1 with -infinity. Illegal columns may
+ * hold anything. A legal NaN or +infinity makes a row's values NaN (a NaN is no
+ * alternative). tokens NULL: every row counts; logp and rank are not written. */
+#define WC_TOP_MAX 64
+typedef struct wc_logp_args {
+    uint64_t bytes;
+    int32_t device, dtype;
+    int64_t rows, vocab;
+    const void* logits;
+    int64_t logits_stride;
+    const uint8_t* legal;       /* rows x vocab, nonzero = legal; NULL: all */
+    int64_t legal_stride;
+    const void* tokens;         /* rows, of index_bits; NULL: none */
+    float inv_temperature;
+    int32_t index_bits, top, pad; /* top: 0 .. WC_TOP_MAX */
+    float* logp;                /* rows each */
+    float* entropy;
+    int32_t* rank;
+    float* top_logp;            /* rows x top */
+    int32_t* top_index;
+    float* stats;               /* rows x 4, for the backward pass; NULL: not kept */
+    void* workspace;
+    uint64_t workspace_bytes;
+} wc_logp_args;
+int wc_token_logp_workspace(const wc_logp_args* a, uint64_t* bytes);
+int wc_token_logp(const wc_logp_args* a, void* stream);
+
+/* The gradient at the logits from what arrives at logp and at the entropy (each
+ * may be NULL: 0): inv_temperature (d_logp ([j = token] - p_j) - d_entropy p_j
+ * (logp_j + H)), 0 in illegal columns and in rows that were left out. */
+typedef struct wc_logp_back_args {
+    uint64_t bytes;
+    int32_t device, dtype;
+    int64_t rows, vocab;
+    const void* logits;
+    int64_t logits_stride;
+    const uint8_t* legal;
+    int64_t legal_stride;
+    const void* tokens;
+    float inv_temperature;
+    int32_t index_bits;
+    const float* stats;
+    const float* d_logp;        /* rows */
+    const float* d_entropy;     /* rows */
+    void* grad;                 /* rows x vocab; may be logits itself */
+    int64_t grad_stride;
+} wc_logp_back_args;
+int wc_token_logp_backward(const wc_logp_back_args* a, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

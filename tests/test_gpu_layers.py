@@ -1,0 +1,547 @@
+"""The layer, update and log-probability operators on the device (include/wc_learn.h), through the binding, against plain
+float64 code.
+
+Tolerances. A product's sum over K is made of matrix instructions of 16 terms, added one after the other, in up to 64 runs
+that are added at the end: (K / 16 + 80) additions of half a float32 ulp of the sum of magnitudes S = |x| |W|, and within an
+instruction and for the parts of float32 operands as much again: 2^-23 (K / 16 + 80) S. The activation's slope is at most
+1.2, its value off by 4e-6 of its argument. An output adds its type's rounding U of the value. The gradient at the
+pre-activations is rounded to U before its products: U (|d_pre| |W|). Singular values: see there. Log-probabilities: a row's
+log-sum is off by a few float32 ulps of the largest logit, 2e-5 as in the losses' tests. Indices and ranks are exact.
+"""
+import math
+
+import pytest
+import torch
+
+import layer_ref as R
+import warchest_learn as wl
+import warchest_wave as ww
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(autouse=True)
+def float32_by_default():
+    """Other test modules set torch's default type to float64 for the whole process."""
+    before = torch.get_default_dtype()
+    torch.set_default_dtype(torch.float32)
+    yield
+    torch.set_default_dtype(before)
+
+
+DEV = "cuda:0"
+TYPES = {"f32": torch.float32, "f16": torch.float16, "bf16": torch.bfloat16}
+
+
+def say(text):
+    print(text, flush=True)
+
+
+def gen(seed):
+    return torch.Generator().manual_seed(seed)
+
+
+def to(x):
+    return None if x is None else x.to(DEV)
+
+
+def within(got, want, bound, what):
+    got = got.detach().cpu().double()
+    assert got.shape == want.shape, (what, got.shape, want.shape)
+    off = (got - want).abs()
+    bad = ~(off <= bound)
+    assert not bad.any(), (what, int(bad.sum()), float(off.max()), float(torch.as_tensor(bound).max()))
+
+
+def strided(x, extra, fill=float("nan")):
+    """x on the device with `extra` columns more per row in memory (holding `fill`), at an offset of one element."""
+    rows, width = x.shape
+    buf = torch.full((rows * (width + extra) + 1,), fill, dtype=x.dtype, device=DEV)
+    v = buf[1:].view(rows, width + extra)[:, :width]
+    v.copy_(x)
+    return v
+
+
+# ------------------------------------------------------------------ layers
+
+def layer_inputs(rows, width, out, dtype, seed, bias=True, residual=True):
+    g = gen(seed)
+    k = {"x": torch.randn(rows, width, generator=g).to(dtype),
+         "weight": (torch.randn(width, out, generator=g) * width ** -0.5).to(dtype),
+         "bias": (0.3 * torch.randn(out, generator=g)).to(dtype) if bias else None,
+         "residual": torch.randn(rows, out, generator=g).to(dtype) if residual else None}
+    return k, torch.randn(rows, out, generator=g).to(dtype)
+
+
+def rounding(want, dtype):
+    return R.U[dtype] * want.abs() + R.LEAST[dtype]
+
+
+def sums(k):
+    return 2.0 ** -23 * (k / 16 + 80)
+
+
+def check_forward(got, k, act):
+    out, pre = R.linear(k["x"], k["weight"], k["bias"], act, k["residual"])
+    s = k["x"].double().abs() @ k["weight"].double().abs() + (0 if k["bias"] is None else k["bias"].double().abs())
+    off = sums(k["x"].shape[1]) * s
+    dt = k["x"].dtype
+    if got.pre is not None:
+        within(got.pre, pre, rounding(pre, dt) + off, "pre")
+    # a residual's own addition: a float32 rounding of either
+    more = 2.0 ** -22 * (out.abs() + pre.abs()) + 4e-6 * pre.abs()
+    within(got.out, out, rounding(out, dt) + 1.2 * off + more, "out")
+
+
+def check_backward(got, d, k, pre, act, dtype=None):
+    x, w, dt = k["x"], k["weight"], k["x"].dtype
+    dx, dw, db, dp = R.linear_backward(d, x, w, pre, act)
+    # d_pre: its slope off by 4e-6, and rounded to its type for the products
+    each = (4e-6 * d.double().abs() + rounding(dp, dt)) if act != "none" else torch.zeros_like(dp)
+    wa, xa, da = w.double().abs(), x.double().abs(), dp.abs() + each
+    if got.x is not None:
+        within(got.x, dx, rounding(dx, dt) + each @ wa.t() + sums(w.shape[1]) * (da @ wa.t()), "d_x")
+    if got.weight is not None:
+        within(got.weight, dw, rounding(dw, dtype or dt) + xa.t() @ each + sums(len(x)) * (xa.t() @ da), "d_weight")
+    if got.bias is not None:
+        within(got.bias, db, 2.0 ** -24 * 300 * da.sum(0) + 4e-6 * d.double().abs().sum(0), "d_bias")
+
+
+SIZES = [(1, 1, 1), (1, 8, 8), (3, 7, 5), (8, 16, 64), (5, 129, 128), (64, 64, 64), (65, 33, 67), (63, 72, 136), (2, 1000, 24),
+         (130, 256, 257), (257, 65, 31), (300, 128, 567), (33, 512, 1024), (700, 40, 264), (1, 2048, 333), (9, 300, 4000)]
+
+
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("rows,width,out", SIZES)
+def test_linear_over_sizes(rows, width, out, dtype):
+    for i, act in enumerate(("none", "relu", "gelu", "silu")):
+        for transposed in (False, True):
+            k, d = layer_inputs(rows, width, out, TYPES[dtype], rows + width + out + i, bias=i != 0, residual=i % 2 == 0)
+            say(f"case linear: {rows} x {width} x {out} {dtype} {act} transposed {transposed}")
+            v = {n: to(t) for n, t in k.items()}
+            if transposed:
+                v["weight"] = v["weight"].t().contiguous().t()
+            got = wl.linear(v["x"], v["weight"], v["bias"], act=act, residual=v["residual"], keep=i != 1)
+            assert (got.pre is None) == (act in ("none", "relu"))
+            check_forward(got, k, act)
+            if act == "relu":
+                got = got._replace(pre=wl.linear(v["x"], v["weight"], v["bias"]).out)
+            pre = None if got.pre is None else got.pre.cpu()
+            back = wl.linear_backward(to(d), v["x"], v["weight"], got.pre, act=act, bias=True)
+            assert back.weight.stride() == v["weight"].stride() or 1 in (width, out)
+            check_backward(back, d, k, pre, act)
+
+
+@pytest.mark.parametrize("rows,width,out,dtype", [(1030, 520, 776, "bf16"), (2500, 264, 520, "f16"), (600, 333, 401, "f32"),
+                                                  (20000, 96, 192, "bf16"), (20001, 97, 31, "f16"), (5000, 64, 128, "f32"),
+                                                  (16, 4096, 512, "bf16"), (1, 8192, 1024, "f32"), (31, 20000, 40, "f16")])
+def test_linear_with_larger_sizes(rows, width, out, dtype):
+    k, d = layer_inputs(rows, width, out, TYPES[dtype], 7)
+    say(f"case linear: {rows} x {width} x {out} {dtype}")
+    v = {n: to(t) for n, t in k.items()}
+    got = wl.linear(**{n: v[n] for n in ("x", "weight", "bias")}, residual=v["residual"], act="silu", keep=True)
+    check_forward(got, k, "silu")
+    back = wl.linear_backward(to(d), v["x"], v["weight"], got.pre, act="silu", bias=True)
+    check_backward(back, d, k, got.pre.cpu(), "silu")
+
+
+@pytest.mark.parametrize("dtype", list(TYPES))
+def test_linear_with_strides_and_what_lies_between_rows(dtype):
+    """Rows at any stride, at an offset of one element, with NaN between them; a broadcast row; a residual in a view."""
+    say(f"case linear: strides {dtype}")
+    for extra in (1, 7, 8):
+        k, d = layer_inputs(37, 83, 45, TYPES[dtype], extra)
+        v = {n: t if t is None or n == "bias" else strided(t, extra) for n, t in k.items()}
+        v["bias"] = to(k["bias"])
+        got = wl.linear(v["x"], v["weight"], v["bias"], act="gelu", residual=v["residual"], keep=True)
+        check_forward(got, k, "gelu")
+        back = wl.linear_backward(strided(d, extra), v["x"], v["weight"], strided(got.pre.cpu(), extra), act="gelu", bias=True)
+        check_backward(back, d, k, got.pre.cpu(), "gelu")
+    k, _ = layer_inputs(40, 64, 64, TYPES[dtype], 3)
+    for n in ("x", "residual"):
+        k[n] = k[n][:1].expand(40, -1)
+    got = wl.linear(to(k["x"][:1]).expand(40, -1), to(k["weight"]), to(k["bias"]), residual=to(k["residual"][:1]).expand(40, -1))
+    check_forward(got, k, "none")
+
+
+def test_linear_bias_and_weight_gradient_in_float32():
+    k, d = layer_inputs(200, 72, 88, torch.bfloat16, 5)
+    k["bias"] = k["bias"].float() + 1e-3
+    v = {n: to(t) for n, t in k.items()}
+    check_forward(wl.linear(v["x"], v["weight"], v["bias"], residual=v["residual"]), k, "none")
+    for transposed in (False, True):
+        w = v["weight"].t().contiguous().t() if transposed else v["weight"]
+        back = wl.linear_backward(to(d), v["x"], w, dtype=torch.float32, bias=True)
+        assert back.weight.dtype == torch.float32
+        check_backward(back, d, k, None, "none", torch.float32)
+        only = wl.linear_backward(to(d), v["x"], w, d_x=False, d_weight=False, bias=True)
+        assert only.x is None and only.weight is None
+        assert torch.equal(only.bias, back.bias)
+
+
+@pytest.mark.parametrize("dtype", list(TYPES))
+def test_linear_without_rows(dtype):
+    x, w = torch.empty(0, 24, dtype=TYPES[dtype], device=DEV), torch.ones(24, 40, dtype=TYPES[dtype], device=DEV)
+    assert wl.linear(x, w).out.shape == (0, 40)
+    b = wl.linear_backward(torch.empty(0, 40, dtype=TYPES[dtype], device=DEV), x, w, bias=True)
+    assert b.x.shape == (0, 24)
+    assert torch.equal(b.weight, torch.zeros_like(w)) and torch.equal(b.bias, torch.zeros(40, device=DEV))
+
+
+@pytest.mark.parametrize("dtype", list(TYPES))
+def test_linear_keeps_infinities_and_nan_in_their_rows(dtype):
+    """A row with an infinity or a NaN gives a row that is not finite, and no other; a float32 near the largest is exact."""
+    say(f"case linear: infinities {dtype}")
+    k, _ = layer_inputs(70, 96, 80, TYPES[dtype], 8, residual=False)
+    want = wl.linear(*(to(k[n]) for n in ("x", "weight", "bias"))).out
+    x = k["x"].clone()
+    x[3, 5], x[40, 95] = math.inf, math.nan
+    got = wl.linear(to(x), to(k["weight"]), to(k["bias"])).out
+    assert not got[[3, 40]].isfinite().any()
+    rest = [i for i in range(70) if i not in (3, 40)]
+    assert torch.equal(got[rest], want[rest])
+    top = torch.finfo(TYPES[dtype]).max
+    x = torch.zeros(2, 32, dtype=TYPES[dtype])
+    x[0, 0], x[1, 31] = top, -top
+    got = wl.linear(to(x), torch.eye(32, dtype=TYPES[dtype], device=DEV)).out.cpu()
+    assert torch.equal(got, x)
+
+
+def test_linear_is_the_same_from_run_to_run_and_in_a_graph():
+    """Split sums are added in a fixed order; a captured call replays on new inputs."""
+    k, d = layer_inputs(300, 1153, 72, torch.bfloat16, 9)
+    v = {n: to(t) for n, t in k.items()}
+    d = to(d)
+
+    def step():
+        f = wl.linear(v["x"], v["weight"], v["bias"], act="gelu", residual=v["residual"], keep=True)
+        return (*f, *wl.linear_backward(d, v["x"], v["weight"], f.pre, act="gelu", bias=True))
+
+    first = [t.clone() for t in step()]
+    for a, b in zip(first, step()):
+        assert torch.equal(a, b)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = step()
+    for i in range(3):
+        v["x"].copy_(to(layer_inputs(300, 1153, 72, torch.bfloat16, 20 + i)[0]["x"]))
+        graph.replay()
+        torch.cuda.synchronize()
+        for a, b in zip(held, step()):
+            assert torch.equal(a, b)
+
+
+def test_linear_refuses_what_does_not_fit():
+    x, w = torch.zeros(4, 16, device=DEV), torch.zeros(16, 8, device=DEV)
+    for bad, word in ((lambda: wl.linear(x[0], w), "rows x width"), (lambda: wl.linear(x, w[:15]), "weight"),
+                      (lambda: wl.linear(x, w.half()), "weight"), (lambda: wl.linear(x, w[:, ::2]), "weight"),
+                      (lambda: wl.linear(x, w, torch.zeros(7, device=DEV)), "bias"),
+                      (lambda: wl.linear(x, w, torch.zeros(8, device=DEV).half()), "bias"),
+                      (lambda: wl.linear(x, w, act="tanh"), "act"), (lambda: wl.linear(x, w, residual=x), "residual"),
+                      (lambda: wl.linear(x, w.cpu()), "weight"), (lambda: wl.linear(x.double(), w), "x:"),
+                      (lambda: wl.linear_backward(x, x, w), "d_out"),
+                      (lambda: wl.linear_backward(torch.zeros(4, 8, device=DEV), x, w, act="gelu"), "pre"),
+                      (lambda: wl.linear_backward(torch.zeros(4, 8, device=DEV), x, w, dtype=torch.float16), "dtype")):
+        with pytest.raises(ww.WaveError, match=word):
+            bad()
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_dense_under_automatic_differentiation(dtype):
+    """Gradients of all four inputs, the residual and the bias broadcast, against float64 and the calls themselves."""
+    k, d = layer_inputs(50, 40, 56, TYPES[dtype], 11)
+    v = {n: to(t).requires_grad_(True) for n, t in k.items()}
+    row = v["residual"].detach()[:1].clone().requires_grad_(True)
+    y = wl.dense(v["x"], v["weight"], v["bias"], act="silu", residual=row.expand(50, -1))
+    y.backward(to(d))
+    pre = wl.linear(*(v[n].detach() for n in ("x", "weight", "bias")), act="silu", keep=True).pre
+    got = wl.LinearGrads(v["x"].grad, v["weight"].grad, None)
+    check_backward(got, d, k, pre.cpu(), "silu")
+    assert v["bias"].grad.dtype == TYPES[dtype] and row.grad.shape == (1, 56)
+    within(row.grad, d.double().sum(0, keepdim=True), 60 * rounding(d.double().abs().sum(0, keepdim=True), TYPES[dtype]), "row")
+    x, w = (torch.randn(*s, device=DEV, requires_grad=True) for s in ((6, 5), (5, 4)))
+    g, = torch.autograd.grad(wl.dense(x, w).sum(), x, create_graph=True)
+    with pytest.raises(ww.WaveError, match="second"):
+        g.sum().backward()
+
+
+# ------------------------------------------------------------------ updates
+
+def check_ortho(got, u, dtype, **kw):
+    """Of a bf16 result beyond 128 rows and columns A (up to 1.5, which X' has times |b + 2 c A|, up to 4.8) and B (up to
+    2.8) are rounded to 11 bits, 2^-12 of them: up to 10 2^-12 of X's scale in each of five steps. An element is off by no
+    more than all of that, three times for one above the root mean square; as independent errors, sqrt(5) 10 2^-12 /
+    sqrt(3) = 3.2e-3 of the norm, and with the result's own 2^-8 / sqrt(6) less than 2^-8. With 22 bits, 15 products'
+    float32 sums over K: 15 2^-23 (K / 16 + 80) of the root mean square. And what rounds X (2^-23 of its largest element,
+    and as much in a product's sum) in a direction that has no singular value grows a-fold in each step: 3.4445^5 = 485,
+    times 2^-22 of the largest element of the normalised update."""
+    want = R.orthogonalise(u, **kw)
+    rms = want.square().mean((-2, -1), keepdim=True).sqrt()
+    k = max(u.shape[-2:])
+    one = dtype == torch.bfloat16 and min(u.shape[-2:]) > 128
+    x = u.double().abs()
+    grown = 485 * kw.get("scale", 1.0) * 2.0 ** -22 * (x.amax((-2, -1), keepdim=True) / x.square().sum((-2, -1), keepdim=True).sqrt())
+    off = rounding(want, dtype) + (150 * 2.0 ** -12 if one else 15 * sums(k)) * rms + grown
+    within(got, want, off, "orthogonalise")
+    if one:
+        assert float((got.cpu().double() - want).norm()) < 2.0 ** -8 * float(want.norm())
+
+
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("shape", [(1, 1), (1, 9), (17, 1), (3, 5), (8, 8), (64, 64), (63, 65), (40, 200), (200, 40), (96, 192),
+                                   (3, 96, 192), (5, 33, 17), (2, 130, 70), (256, 264), (300, 700), (1, 70, 70), (0, 4, 4)])
+def test_orthogonalise_over_sizes(shape, dtype):
+    say(f"case orthogonalise: {shape} {dtype}")
+    u = (0.01 * torch.randn(*shape, generator=gen(sum(shape)))).to(TYPES[dtype])
+    got = wl.orthogonalise(to(u))
+    assert got.shape == u.shape and got.dtype == u.dtype
+    check_ortho(got, u, u.dtype)
+
+
+@pytest.mark.parametrize("shape,dtype", [((1100, 530), "bf16"), ((520, 1400), "bf16"), ((600, 600), "f32"), ((4, 520, 260), "f16")])
+def test_orthogonalise_with_larger_sizes(shape, dtype):
+    say(f"case orthogonalise: {shape} {dtype}")
+    u = torch.randn(*shape, generator=gen(1)).to(TYPES[dtype])
+    check_ortho(wl.orthogonalise(to(u)), u, u.dtype)
+    # small directions beside three large ones
+    g = gen(2)
+    u = 1e-3 * torch.randn(*shape, generator=g)
+    for _ in range(3):
+        u += 0.02 * torch.randn(*shape[:-1], 1, generator=g) * torch.randn(*shape[:-2], 1, shape[-1], generator=g)
+    check_ortho(wl.orthogonalise(to(u), dtype=TYPES[dtype]), u, TYPES[dtype])
+
+
+def test_orthogonalise_types_strides_and_arguments():
+    say("case orthogonalise: strides")
+    u = torch.randn(3, 50, 90, generator=gen(2))
+    wide = torch.full((3, 55, 97), math.nan, device=DEV)
+    wide[:, :50, 3:93] = to(u)
+    view = wide[:, :50, 3:93]
+    for out in TYPES.values():
+        got = wl.orthogonalise(view, dtype=out, steps=3, coefficients=(2.0, -1.5, 0.5), scale=1.7)
+        assert got.dtype == out and got.is_contiguous()
+        check_ortho(got, u, out, steps=3, coefficients=(2.0, -1.5, 0.5), scale=1.7)
+    same = to(u[:1]).expand(4, -1, -1)
+    got = wl.orthogonalise(same)
+    assert torch.equal(got[0], got[3])
+    # a row, a rank of one, a norm beyond float32's squares, and nothing at all
+    for v in (torch.outer(torch.arange(1.0, 20), torch.arange(1.0, 33)), 1e30 * torch.randn(30, 20, generator=gen(3)),
+              1e-30 * torch.randn(20, 30, generator=gen(3)).bfloat16()):
+        eps = 0.0 if v.abs().max() < 1e-20 else 1e-7
+        check_ortho(wl.orthogonalise(to(v), eps=eps), v, v.dtype, eps=eps)
+    assert torch.equal(wl.orthogonalise(torch.zeros(9, 12, device=DEV)), torch.zeros(9, 12, device=DEV))
+
+
+def test_orthogonalise_keeps_matrices_apart():
+    """A NaN in one matrix of a batch makes that one NaN and leaves the others as they are alone."""
+    u = torch.randn(3, 24, 40, generator=gen(4))
+    u[1, 3, 3] = math.nan
+    got = wl.orthogonalise(to(u))
+    assert got[1].isnan().all()
+    for i in (0, 2):
+        check_ortho(got[i], u[i], torch.float32)
+    with pytest.raises(ww.WaveError, match="columns"):
+        wl.orthogonalise(torch.zeros(4, 6, device=DEV).t())
+    with pytest.raises(ww.WaveError, match="steps"):
+        wl.orthogonalise(torch.zeros(4, 6, device=DEV), steps=0)
+    with pytest.raises(ww.WaveError, match="update"):
+        wl.orthogonalise(torch.zeros(0, 6, device=DEV))
+
+
+# -------------------------------------------------------- log-probabilities
+
+def logp_inputs(rows, vocab, dtype, seed, legal):
+    g = gen(seed)
+    k = {"logits": (2 * torch.randn(rows, vocab, generator=g)).to(dtype),
+         "tokens": torch.randint(0, vocab, (rows,), generator=g), "legal": None}
+    if legal:
+        k["legal"] = torch.rand(rows, vocab, generator=g) < 0.5
+        k["legal"][torch.arange(rows), k["tokens"]] = True
+    return k, torch.randn(rows, generator=g), torch.randn(rows, generator=g)
+
+
+def check_values(got, want, what, scale=1.0):
+    """2e-5 of the larger of 1 and the value; infinities and NaN alike."""
+    got, want = got.detach().cpu().double(), want.double()
+    odd = ~want.isfinite()
+    assert torch.equal(torch.nan_to_num(got[odd], nan=7.0), torch.nan_to_num(want[odd], nan=7.0)), what
+    within(torch.where(odd, 0.0, got), torch.where(odd, 0.0, want), 2e-5 * want.abs().nan_to_num(0, 0, 0).clamp(min=scale), what)
+
+
+def check_logp(k, top, d1, d2, inv=0.7):
+    v = {n: to(t) for n, t in k.items()}
+    want = R.token_logp(**k, inv_temperature=inv, top=top, d_logp=d1, d_entropy=d2)
+    got = wl.token_logp(**v, inv_temperature=inv, top=top)
+    check_values(got.logp, want["logp"], "logp")
+    check_values(got.entropy, want["entropy"], "entropy")
+    assert torch.equal(got.rank.cpu(), want["rank"])
+    if top:
+        assert torch.equal(got.top_index.cpu(), want["top_index"])
+        check_values(got.top_logp, want["top_logp"], "top_logp")
+    grad = wl.token_logp_backward(to(d1), to(d2), v["logits"], v["tokens"], got.stats, legal=v["legal"], inv_temperature=inv)
+    w, dt = want["grad"], k["logits"].dtype
+    within(grad, w, rounding(w, dt) + 2e-5 * max(1e-3, float(w.abs().max())), "grad")
+    return got
+
+
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("rows,vocab", [(1, 1), (1, 8), (3, 22), (65, 7), (2, 64), (5, 63), (5, 65), (130, 97), (7, 511), (4, 513),
+                                        (7, 1000), (3, 2049), (4, 4099), (300, 567), (2, 9001), (1, 20011)])
+def test_token_logp_over_sizes(rows, vocab, dtype):
+    for legal, top in ((False, 0), (True, 5), (False, 20)):
+        say(f"case logp: {rows} x {vocab} {dtype} legal {legal} top {top}")
+        k, d1, d2 = logp_inputs(rows, vocab, TYPES[dtype], rows + vocab, legal)
+        if rows > 2:
+            k["tokens"][1], k["tokens"][2] = -1, vocab  # left out
+        check_logp(k, top, d1, d2)
+
+
+@pytest.mark.parametrize("rows,vocab,dtype,top", [(2, 131072, "bf16", 20), (300, 16500, "f16", 3), (520, 9000, "f32", 1),
+                                                  (1030, 8193, "f32", 2), (64, 40000, "bf16", 64)])
+def test_token_logp_with_a_large_vocabulary(rows, vocab, dtype, top):
+    """Against float64 torch over whole rows (the row-by-row code is for small ones)."""
+    say(f"case logp: {rows} x {vocab} {dtype} top {top}")
+    k, d1, d2 = logp_inputs(rows, vocab, TYPES[dtype], vocab, False)
+    v = {n: to(t) for n, t in k.items()}
+    x = k["logits"].double()
+    logp = torch.log_softmax(x, 1)
+    p = logp.exp()
+    h = -(p * logp).sum(1)
+    a = k["tokens"][:, None]
+    got = wl.token_logp(v["logits"], v["tokens"], top=top)
+    check_values(got.logp, logp.gather(1, a)[:, 0], "logp")
+    check_values(got.entropy, h, "entropy")
+    order = torch.sort(x, dim=1, descending=True, stable=True)
+    assert torch.equal(got.top_index.cpu().long(), order.indices[:, :top])
+    check_values(got.top_logp, logp.gather(1, order.indices[:, :top]), "top_logp")
+    assert torch.equal(got.rank.cpu().long(), (order.indices == a).int().argmax(1))
+    w = -p * (d1[:, None].double() + d2[:, None].double() * (logp + h[:, None]))
+    w.scatter_add_(1, a, d1[:, None].double())
+    grad = wl.token_logp_backward(to(d1), to(d2), v["logits"], v["tokens"], got.stats)
+    within(grad, w, rounding(w, TYPES[dtype]) + 2e-5 * w.abs().max(), "grad")
+
+
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("vocab", [40, 700, 5000, 30000])
+def test_token_logp_of_equal_and_ordered_logits(vocab, dtype):
+    """Ties go to the lowest index: rows of one value, of few values, ascending, descending, with zeros of both signs, and
+    with the largest side by side."""
+    say(f"case logp: ties {vocab} {dtype}")
+    n = torch.arange(vocab)
+    x = torch.stack([torch.zeros(vocab), (n % 3).float(), n / vocab, -n / vocab, torch.where(n % 2 == 0, 0.0, -0.0),
+                     torch.where((n >= vocab // 2) & (n < vocab // 2 + 30), 4.0, 0.0), torch.where(n % 256 == 7, 2.0, 1.0)])
+    k = {"logits": x.to(TYPES[dtype]), "tokens": torch.tensor([vocab - 1, 5, 0, 7, 9, vocab // 2 + 3, 8]), "legal": None}
+    check_logp(k, 20, torch.ones(7), torch.ones(7))
+
+
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("vocab", [30, 600, 20000])
+def test_token_logp_of_masks_infinities_and_nan(vocab, dtype):
+    say(f"case logp: masks {vocab} {dtype}")
+    dt = TYPES[dtype]
+    least = torch.finfo(dt).min
+    k, d1, d2 = logp_inputs(9, vocab, dt, 3, True)
+    x, on, a = k["logits"], k["legal"], k["tokens"]
+    a[:] = 4
+    on[:, 4] = True
+    on[0] = False                       # nothing legal: left out
+    on[1] = False
+    on[1, 4] = True                     # one alone
+    on[2, 4] = False                    # the token is not legal: -infinity
+    x[3, 4] = -math.inf                 # nor has this one a probability
+    x[4] = least                        # a mask's lowest value everywhere
+    x[5, 1:] = least                    # and everywhere but once
+    on[5, 0] = True
+    x[6] = -math.inf                    # legal, but nothing above -infinity
+    x[7][~on[7]] = math.nan             # what is illegal may be anything
+    x[8][~on[8]] = math.inf
+    got = check_logp(k, 6, d1, d2)
+    assert got.logp[2] == -math.inf and got.logp[3] == -math.inf and got.rank[0] == -1 and got.rank[6] == -1
+    # a legal NaN or +infinity: NaN, the other rows as they were
+    on[1, 5] = on[7, 5] = True
+    x[1, 5], x[7, 5] = math.nan, math.inf
+    again = wl.token_logp(to(x), to(a), legal=to(on), inv_temperature=0.7, top=6)
+    assert again.logp[[1, 7]].isnan().all() and again.entropy[[1, 7]].isnan().all()
+    rest = [0, 2, 3, 4, 5, 6, 8]
+    for one, two in zip(got, again):
+        assert torch.equal(one[rest], two[rest])
+
+
+@pytest.mark.parametrize("dtype", list(TYPES))
+def test_token_logp_with_strides_and_without_tokens(dtype):
+    say(f"case logp: strides {dtype}")
+    k, d1, d2 = logp_inputs(40, 301, TYPES[dtype], 6, True)
+    v = {"logits": strided(k["logits"], 3), "legal": strided(k["legal"], 5, True), "tokens": to(k["tokens"]).int()}
+    got = wl.token_logp(**v, top=4)
+    base = wl.token_logp(**{n: to(t) for n, t in k.items()}, top=4)
+    for one, two in zip(got, base):
+        assert torch.equal(one, two)
+    none = wl.token_logp(v["logits"], legal=v["legal"], top=4)
+    assert none.logp is None and none.rank is None
+    assert torch.equal(none.entropy, base.entropy) and torch.equal(none.top_index, base.top_index)
+    grad = strided(torch.zeros(40, 301, dtype=TYPES[dtype]), 3)
+    wl.token_logp_backward(to(d1), to(d2), v["logits"], v["tokens"], got.stats, legal=v["legal"], grad=grad)
+    want = wl.token_logp_backward(to(d1), to(d2), to(k["logits"]), to(k["tokens"]), base.stats, legal=to(k["legal"]))
+    assert torch.equal(grad, want)
+    # over the logits themselves, and one row for all
+    x = to(k["logits"]).clone()
+    wl.token_logp_backward(to(d1), to(d2), x, to(k["tokens"]), base.stats, legal=to(k["legal"]), grad=x)
+    assert torch.equal(x, want)
+    one = to(k["logits"][:1]).expand(40, -1)
+    many = wl.token_logp(one, v["tokens"], top=2)
+    assert torch.equal(many.entropy, many.entropy[:1].expand(40)) and (many.top_index == many.top_index[:1]).all()
+
+
+def test_token_logp_without_rows_and_refusals():
+    x = torch.zeros(0, 7, device=DEV)
+    got = wl.token_logp(x, torch.zeros(0, dtype=torch.int64, device=DEV), top=3)
+    assert got.logp.shape == (0,) and got.top_index.shape == (0, 3)
+    x, t = torch.zeros(4, 7, device=DEV), torch.zeros(4, dtype=torch.int64, device=DEV)
+    for bad, word in ((lambda: wl.token_logp(x, t[:3]), "tokens"), (lambda: wl.token_logp(x, t.float()), "tokens"),
+                      (lambda: wl.token_logp(x, t, top=65), "top"), (lambda: wl.token_logp(x, t, legal=x), "legal"),
+                      (lambda: wl.token_logp(x, t, inv_temperature=-1.0), "inv_temperature"),
+                      (lambda: wl.token_logp(x.t(), t[:1].expand(7)), "columns"),
+                      (lambda: wl.token_logp_backward(None, None, x, t, None), "stats"),
+                      (lambda: wl.token_logp_backward(x, None, x, t, torch.zeros(4, 4, device=DEV)), "d_logp")):
+        with pytest.raises(ww.WaveError, match=word):
+            bad()
+
+
+def test_token_logp_objective_and_its_graph():
+    """Gradients through logp and entropy; a captured forward and backward pass replays on new logits."""
+    k, d1, d2 = logp_inputs(64, 567, torch.float32, 12, True)
+    x = to(k["logits"]).requires_grad_(True)
+    logp, entropy, rank, top_logp, top_index = wl.token_logp_objective(x, to(k["tokens"]), legal=to(k["legal"]), top=2)
+    assert not top_logp.requires_grad and not rank.requires_grad
+    (logp * to(d1)).sum().backward(retain_graph=True)
+    want = R.token_logp(**k, d_logp=d1)["grad"]
+    within(x.grad, want, 2e-5 * want.abs().max(), "logp's")
+    x.grad = None
+    ((logp * to(d1)).sum() + (entropy * to(d2)).sum()).backward()
+    want = R.token_logp(**k, d_logp=d1, d_entropy=d2)["grad"]
+    within(x.grad, want, 2e-5 * want.abs().max(), "both's")
+    raw, t, on, d1, d2 = x.detach(), to(k["tokens"]), to(k["legal"]), to(d1), to(d2)
+
+    def step():
+        r = wl.token_logp(raw, t, legal=on, top=3)
+        return r.logp, r.top_index, wl.token_logp_backward(d1, d2, raw, t, r.stats, legal=on)
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = step()
+    for i in range(3):
+        raw.copy_(to(logp_inputs(64, 567, torch.float32, 30 + i, True)[0]["logits"]))
+        graph.replay()
+        torch.cuda.synchronize()
+        for a, b in zip(held, step()):
+            assert torch.equal(a, b)

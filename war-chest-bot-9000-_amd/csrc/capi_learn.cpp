@@ -228,6 +228,107 @@ void check(const wc_ckpt_weight_args& a, Check* c) {
     c->buffer(a.bias, 4, false, "bias");
 }
 
+// What both directions of a layer have.
+template <class A>
+bool check_layer(const A& a, Check* c) {
+    if (!c->is(known(a.dtype), "unknown dtype") || !shape(a.rows, a.width, c) || !shape(a.rows, a.out, c)) return false;
+    if (!c->is(a.rows < MOST_LANES, "rows beyond 2^31", WC_ERR_UNSUPPORTED) ||
+        !c->is(a.width <= (1 << 20) && a.out <= (1 << 20), "width or out beyond 2^20", WC_ERR_UNSUPPORTED))
+        return false;
+    c->is(a.weight_layout == WC_WEIGHT_IN_OUT || a.weight_layout == WC_WEIGHT_OUT_IN, "unknown weight_layout");
+    c->is(a.act >= WC_ACT_NONE && a.act <= WC_ACT_SILU, "unknown act");
+    return true;
+}
+
+template <class A>
+void check_weight(const A& a, const void* p, size_t n, int64_t stride, bool written, bool need, const char* name, Check* c) {
+    const bool io = a.weight_layout == WC_WEIGHT_IN_OUT;
+    c->matrix(p, n, stride, io ? a.out : a.width, io ? a.width : a.out, written, need, name);
+}
+
+void check(const wc_linear_args& a, Check* c) {
+    if (!check_layer(a, c)) return;
+    const size_t n = size_of(a.dtype);
+    const bool need = a.rows > 0;
+    c->is(a.bias_dtype == WC_DTYPE_F32 || a.bias_dtype == a.dtype, "bias_dtype is float32 or the matrices'");
+    c->matrix(a.x, n, a.x_stride, a.width, a.rows, false, need, "x");
+    check_weight(a, a.weight, n, a.weight_stride, false, need, "weight", c);
+    c->buffer(a.bias, known(a.bias_dtype) ? size_of(a.bias_dtype) : 4, false, "bias");
+    c->matrix(a.residual, n, a.residual_stride, a.out, a.rows, false, false, "residual");
+    c->matrix(a.pre, n, a.pre_stride, a.out, a.rows, true, false, "pre");
+    c->matrix(a.y, n, a.y_stride, a.out, a.rows, true, need, "y");
+}
+
+void check(const wc_linear_back_args& a, Check* c) {
+    if (!check_layer(a, c)) return;
+    const size_t n = size_of(a.dtype);
+    const bool need = a.rows > 0;
+    c->is(a.grad_dtype == WC_DTYPE_F32 || a.grad_dtype == a.dtype, "grad_dtype is float32 or the matrices'");
+    c->matrix(a.d_out, n, a.d_out_stride, a.out, a.rows, false, need, "d_out");
+    if (a.act != WC_ACT_NONE) c->matrix(a.pre, n, a.pre_stride, a.out, a.rows, false, need, "pre");
+    if (a.d_weight) {
+        c->matrix(a.x, n, a.x_stride, a.width, a.rows, false, need, "x");
+        check_weight(a, a.d_weight, known(a.grad_dtype) ? size_of(a.grad_dtype) : 4, a.d_weight_stride, true, true,
+                     "d_weight", c);
+    }
+    if (a.d_x) {
+        check_weight(a, a.weight, n, a.weight_stride, false, need, "weight", c);
+        c->matrix(a.d_x, n, a.d_x_stride, a.width, a.rows, true, need, "d_x");
+    }
+    c->buffer(a.d_bias, 4, false, "d_bias");
+}
+
+void check(const wc_orthogonalise_args& a, Check* c) {
+    if (!c->is(known(a.dtype) && known(a.out_dtype), "unknown dtype")) return;
+    c->is(a.batch >= 0 && a.batch <= 65535, "batch is 0 to 65535");
+    c->is(a.rows >= 1 && a.width >= 1, "rows and width are at least 1");
+    if (!c->is(a.rows <= (1 << 20) && a.width <= (1 << 20), "rows or width beyond 2^20", WC_ERR_UNSUPPORTED)) return;
+    c->is(a.steps >= 1 && a.steps <= 64, "steps is 1 to 64");
+    c->is(finite(a.a) && finite(a.b) && finite(a.c) && finite(a.scale), "coefficients and scale must be finite");
+    c->is(finite(a.eps) && a.eps >= 0.f, "eps must not be negative");
+    const size_t n = size_of(a.dtype), o = size_of(a.out_dtype);
+    c->matrix(a.update, n, a.update_stride, a.width, a.rows, false, a.batch > 0, "update");
+    c->matrix(a.out, o, a.out_stride, a.width, a.rows, true, a.batch > 0, "out");
+    // a matrix's own rows are apart already; matrices follow each other, or lie between each other's rows
+    const int64_t deep = (a.rows - 1) * a.out_stride + a.width;
+    c->is(a.batch <= 1 || (a.update_batch >= 0 && a.update_batch <= MOST), "update_batch out of range");
+    c->is(a.batch <= 1 || (a.out_batch >= deep && a.out_batch <= MOST), "out's matrices overlap");
+}
+
+template <class A>
+bool check_logits(const A& a, Check* c) {
+    if (!c->is(known(a.dtype), "unknown dtype") || !shape(a.rows, a.vocab, c)) return false;
+    if (!c->is(a.rows < MOST_LANES && a.rows * ((a.vocab + 1023) / 1024) < MOST_LANES, "more rows of this length than a launch holds",
+               WC_ERR_UNSUPPORTED))
+        return false;
+    c->is(a.index_bits == 32 || a.index_bits == 64, "index_bits is 32 or 64");
+    c->is(finite(a.inv_temperature) && a.inv_temperature > 0.f, "inv_temperature must be positive");
+    c->matrix(a.logits, size_of(a.dtype), a.logits_stride, a.vocab, a.rows, false, a.rows > 0, "logits");
+    c->matrix(a.legal, 1, a.legal_stride, a.vocab, a.rows, false, false, "legal");
+    c->buffer(a.tokens, a.index_bits == 32 ? 4 : 8, false, "tokens");
+    return true;
+}
+
+void check(const wc_logp_args& a, Check* c) {
+    if (!check_logits(a, c)) return;
+    const bool need = a.rows > 0;
+    c->is(a.top >= 0 && a.top <= WC_TOP_MAX, "top is 0 to 64");
+    c->buffer(a.logp, 4, need && a.tokens, "logp");
+    c->buffer(a.rank, 4, need && a.tokens, "rank");
+    c->buffer(a.entropy, 4, need, "entropy");
+    c->buffer(a.top_logp, 4, need && a.top, "top_logp");
+    c->buffer(a.top_index, 4, need && a.top, "top_index");
+    c->buffer(a.stats, 16, false, "stats");
+}
+
+void check(const wc_logp_back_args& a, Check* c) {
+    if (!check_logits(a, c)) return;
+    c->buffer(a.stats, 16, a.rows > 0, "stats");
+    c->buffer(a.d_logp, 4, false, "d_logp");
+    c->buffer(a.d_entropy, 4, false, "d_entropy");
+    c->matrix(a.grad, size_of(a.dtype), a.grad_stride, a.vocab, a.rows, true, a.rows > 0, "grad");
+}
+
 template <class A>
 void workspace(const A& a, size_t want, Check* c) {
     c->is(a.workspace_bytes >= want && (a.workspace || !want), "the workspace is too small");
@@ -323,6 +424,49 @@ int wc_ckpt_weight_workspace(const wc_ckpt_weight_args* a, uint64_t* bytes) {
 int wc_ckpt_weight_grad(const wc_ckpt_weight_args* a, void* stream) {
     return with_scratch("wc_ckpt_weight_grad", a, nullptr, learn::ckpt_weight_scratch, learn::launch_ckpt_weight,
                         stream);
+}
+
+int wc_linear_workspace(const wc_linear_args* a, uint64_t* bytes) {
+    if (!bytes) return fail(WC_ERR_INVALID, "wc_linear_workspace: null argument");
+    return with_scratch("wc_linear_workspace", a, bytes, learn::linear_scratch, learn::launch_linear, nullptr);
+}
+int wc_linear(const wc_linear_args* a, void* stream) {
+    return with_scratch("wc_linear", a, nullptr, learn::linear_scratch, learn::launch_linear, stream);
+}
+
+int wc_linear_backward_workspace(const wc_linear_back_args* a, uint64_t* bytes) {
+    if (!bytes) return fail(WC_ERR_INVALID, "wc_linear_backward_workspace: null argument");
+    return with_scratch("wc_linear_backward_workspace", a, bytes, learn::linear_back_scratch, learn::launch_linear_back, nullptr);
+}
+int wc_linear_backward(const wc_linear_back_args* a, void* stream) {
+    return with_scratch("wc_linear_backward", a, nullptr, learn::linear_back_scratch, learn::launch_linear_back, stream);
+}
+
+int wc_orthogonalise_workspace(const wc_orthogonalise_args* a, uint64_t* bytes) {
+    if (!bytes) return fail(WC_ERR_INVALID, "wc_orthogonalise_workspace: null argument");
+    return with_scratch("wc_orthogonalise_workspace", a, bytes, learn::orthogonalise_scratch, learn::launch_orthogonalise, nullptr);
+}
+int wc_orthogonalise(const wc_orthogonalise_args* a, void* stream) {
+    return with_scratch("wc_orthogonalise", a, nullptr, learn::orthogonalise_scratch, learn::launch_orthogonalise, stream);
+}
+
+int wc_token_logp_workspace(const wc_logp_args* a, uint64_t* bytes) {
+    if (!bytes) return fail(WC_ERR_INVALID, "wc_token_logp_workspace: null argument");
+    return with_scratch("wc_token_logp_workspace", a, bytes, learn::logp_scratch, learn::launch_logp, nullptr);
+}
+int wc_token_logp(const wc_logp_args* a, void* stream) {
+    return with_scratch("wc_token_logp", a, nullptr, learn::logp_scratch, learn::launch_logp, stream);
+}
+
+int wc_token_logp_backward(const wc_logp_back_args* a, void* stream) {
+    return shielded("wc_token_logp_backward", [&]() -> int {
+        Check c{"wc_token_logp_backward"};
+        if (whole(a, &c)) check(*a, &c);
+        const int cus = c.code == WC_OK ? cus_of(a->device, &c) : 0;
+        if (c.code != WC_OK) return fail(c.code, c.msg);
+        return on_device("wc_token_logp_backward", a->device,
+                         [&] { learn::launch_logp_back(*a, cus, (hipStream_t)stream); });
+    });
 }
 
 }  // extern "C"

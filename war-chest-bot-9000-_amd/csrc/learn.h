@@ -34,6 +34,40 @@ void preference_f32(const wc_preference_args& a, hipStream_t s);
 void preference_f16(const wc_preference_args& a, hipStream_t s);
 void preference_bf16(const wc_preference_args& a, hipStream_t s);
 
+size_t linear_scratch(const wc_linear_args& a, int cus);
+size_t linear_back_scratch(const wc_linear_back_args& a, int cus);
+size_t orthogonalise_scratch(const wc_orthogonalise_args& a, int cus);
+size_t logp_scratch(const wc_logp_args& a, int cus);
+
+void launch_linear(const wc_linear_args& a, int cus, hipStream_t s);
+void launch_linear_back(const wc_linear_back_args& a, int cus, hipStream_t s);
+void launch_orthogonalise(const wc_orthogonalise_args& a, int cus, hipStream_t s);
+void launch_logp(const wc_logp_args& a, int cus, hipStream_t s);
+void launch_logp_back(const wc_logp_back_args& a, int cus, hipStream_t s);
+
+// The layers and the log-probabilities by element type.
+size_t linear_scratch_f32(const wc_linear_args& a, int cus);
+size_t linear_back_scratch_f32(const wc_linear_back_args& a, int cus);
+void linear_f32(const wc_linear_args& a, int cus, hipStream_t s);
+void linear_back_f32(const wc_linear_back_args& a, int cus, hipStream_t s);
+size_t logp_scratch_f32(const wc_logp_args& a, int cus);
+void logp_f32(const wc_logp_args& a, int cus, hipStream_t s);
+void logp_back_f32(const wc_logp_back_args& a, hipStream_t s);
+size_t linear_scratch_f16(const wc_linear_args& a, int cus);
+size_t linear_back_scratch_f16(const wc_linear_back_args& a, int cus);
+void linear_f16(const wc_linear_args& a, int cus, hipStream_t s);
+void linear_back_f16(const wc_linear_back_args& a, int cus, hipStream_t s);
+size_t logp_scratch_f16(const wc_logp_args& a, int cus);
+void logp_f16(const wc_logp_args& a, int cus, hipStream_t s);
+void logp_back_f16(const wc_logp_back_args& a, hipStream_t s);
+size_t linear_scratch_bf16(const wc_linear_args& a, int cus);
+size_t linear_back_scratch_bf16(const wc_linear_back_args& a, int cus);
+void linear_bf16(const wc_linear_args& a, int cus, hipStream_t s);
+void linear_back_bf16(const wc_linear_back_args& a, int cus, hipStream_t s);
+size_t logp_scratch_bf16(const wc_logp_args& a, int cus);
+void logp_bf16(const wc_logp_args& a, int cus, hipStream_t s);
+void logp_back_bf16(const wc_logp_back_args& a, hipStream_t s);
+
 inline size_t pad256(size_t x) { return (x + 255) & ~size_t(255); }
 
 }  // namespace learn

@@ -1,0 +1,416 @@
+// A layer's product with bias, activation and residual in its epilogue, and its gradients (include/wc_learn.h), for one
+// element type: linear_f32.hip, linear_f16.hip and linear_bf16.hip build one each.
+//
+//   y = act(x W + b) + residual;  d_pre = d_y act'(pre);  d_x = d_pre W^T;  d_W = x^T d_pre;  d_b = column sums of d_pre
+//
+// The three products differ in which index of each operand is summed; one kernel takes all (product_dev.h). Sums, bias,
+// activation and residual are float32 and rounded once, to the output's type. d_pre is rounded to the 16-bit type for
+// its two products (as it would be between two operators): its own half ulp, 2^-9 of an element in bf16, against the
+// same for every element of the result. The kept pre-activations are rounded to the matrices' type.
+//
+// float32 operands are taken as three bf16 parts (8 + 8 + 8 bits), and of their nine products the six that matter:
+// the matrix cores' own float32 rate is a sixteenth of the 16-bit one.
+#pragma once
+
+#include "ckpt8_dev.h"
+#include "learn.h"
+#include "product_dev.h"
+
+#pragma clang fp contract(fast)
+
+namespace wc {
+namespace learn {
+namespace {
+
+// The 16-bit type that products are taken in, and the parts of an element.
+template <class T>
+struct Parts {
+    typedef T type;
+    static constexpr int COUNT = 1;
+};
+template <>
+struct Parts<float> {
+    typedef bf16 type;
+    static constexpr int COUNT = 3;
+};
+
+// Each part is what is left rounded to bf16; the third is exact, and the products that are left out are below 2^-25 of
+// the whole. A first part that would round past bf16's largest is cut. What an infinity leaves is 0.
+__device__ __forceinline__ void parts_of(float x, bf16 (&o)[3]) {
+    o[0] = (bf16)x;
+    if (fabsf((float)o[0]) == INFINITY) o[0] = __builtin_bit_cast(bf16, (uint16_t)(__float_as_uint(x) >> 16));
+    x -= (float)o[0];
+    x = x == x ? x : 0.f;
+    o[1] = (bf16)x;
+    o[2] = (bf16)(x - (float)o[1]);
+}
+
+// Eight values to a row of an operand's planes.
+template <class T>
+__device__ __forceinline__ void put_parts(char* to, int64_t plane, const float (&v)[8]) {
+    typedef typename Parts<T>::type E;
+    typedef E E8 __attribute__((ext_vector_type(8)));
+    if constexpr (Parts<T>::COUNT == 1) {
+        E8 o;
+#pragma unroll
+        for (int u = 0; u < 8; u++) o[u] = (E)v[u];
+        *(E8*)to = o;
+    } else {
+        E8 o[3];
+#pragma unroll
+        for (int u = 0; u < 8; u++) {
+            bf16 part[3];
+            parts_of(v[u], part);
+#pragma unroll
+            for (int k = 0; k < 3; k++) o[k][u] = part[k];
+        }
+#pragma unroll
+        for (int k = 0; k < 3; k++) *(E8*)(to + k * plane) = o[k];
+    }
+}
+
+// What a product reads of a matrix: the matrix itself, or a copy of it in the workspace, in parts, on 16-byte rows, with
+// zeros up to whole steps where there are several parts.
+struct Laid {
+    bool copy;
+    int64_t rows, cols, pitch, plane;  // of the copy: rows and columns with the zeros, bytes
+    size_t at;
+
+    size_t bytes(int parts) const { return copy ? size_t(plane) * parts : 0; }
+};
+
+template <class T>
+Laid laid(const void* p, int64_t stride, int64_t rows, int64_t cols) {
+    Laid l = {};
+    constexpr bool one = Parts<T>::COUNT == 1;
+    // (a lane's place in a tile is held in 32 bits)
+    const bool whole = cols % 8 == 0 && ((uintptr_t)p & 15) == 0 && (rows <= 1 || (stride % 8 == 0 && stride < (1 << 22)));
+    l.copy = !one || !whole;
+    if (!l.copy) {
+        l.rows = rows;
+        l.cols = cols;
+        l.pitch = rows <= 1 ? 2 * cols : 2 * stride;
+        return l;
+    }
+    l.rows = one ? rows : up(rows, STEP);
+    l.cols = up(cols, one ? 8 : STEP);
+    l.pitch = 2 * l.cols;
+    l.plane = l.pitch * l.rows;
+    return l;
+}
+
+struct Source {
+    const void* p;
+    int64_t stride, rows, cols;
+    char* to;
+    int64_t to_rows, to_cols, plane;
+};
+
+// Up to two matrices copied into planes, a chunk of eight a thread.
+template <class T>
+__global__ __launch_bounds__(256) void k_lay(Source one, Source two) {
+    const int64_t n1 = one.to_rows * (one.to_cols / 8), n2 = two.to_rows * (two.to_cols / 8);
+    for (int64_t at = int64_t(blockIdx.x) * 256 + threadIdx.x; at < n1 + n2; at += int64_t(gridDim.x) * 256) {
+        const Source& s = at < n1 ? one : two;
+        const int64_t chunk = at < n1 ? at : at - n1, per_row = s.to_cols / 8, r = chunk / per_row, c = 8 * (chunk - r * per_row);
+        float v[8] = {};
+        if (r < s.rows && c < s.cols) load_n((const T*)s.p + r * s.stride + c, (int)min<int64_t>(8, s.cols - c), 0.f, v);
+        put_parts<T>(s.to + 2 * (r * s.to_cols + c), s.plane, v);
+    }
+}
+
+// y = act(v + bias) + residual, and the kept v + bias.
+template <class T>
+struct LayerEpilogue {
+    static constexpr bool MIRROR = false;
+    const void* bias;
+    bool bias_f32;
+    const T* residual;
+    int64_t residual_stride;
+    T* pre;
+    int64_t pre_stride;
+    T* y;
+    int64_t y_stride;
+    int act;
+
+    __device__ __forceinline__ void operator()(int, int64_t i, int64_t j, int n, float (&v)[8]) const {
+        if (bias) {
+            float b[8];
+            if (bias_f32) load_n((const float*)bias + j, n, 0.f, b);
+            else load_n((const T*)bias + j, n, 0.f, b);
+#pragma unroll
+            for (int u = 0; u < 8; u++) v[u] += b[u];
+        }
+        if (pre) store_n(pre + i * pre_stride + j, n, v);
+        act_values(v, act);
+        if (residual) {
+            float r[8];
+            load_n(residual + i * residual_stride + j, n, 0.f, r);
+#pragma unroll
+            for (int u = 0; u < 8; u++) v[u] += r[u];
+        }
+        store_n(y + i * y_stride + j, n, v);
+    }
+};
+
+template <class T>
+Operand16 operand(const Laid& l, const void* p, char* workspace, int64_t outer) {
+    Operand16 o = {};
+    for (int k = 0; k < Parts<T>::COUNT; k++) o.plane[k] = l.copy ? workspace + l.at + k * l.plane : (const char*)p;
+    o.pitch = l.pitch;
+    o.outer = outer;
+    return o;
+}
+
+// a, b and k are set.
+template <class T, class Epilogue>
+void multiply(Product p, const Cut& cut, bool ai, bool bi, float* part, const Epilogue& e, hipStream_t s) {
+    typedef typename Parts<T>::type E;
+    if (Parts<T>::COUNT == 3) {
+        // the largest last: what is small is added to what is small
+        static constexpr uint8_t pa[] = {2, 1, 0, 1, 0, 0}, pb[] = {0, 1, 2, 0, 1, 0};
+        p.segments = 6;
+        for (int k = 0; k < 6; k++) p.pa[k] = pa[k], p.pb[k] = pb[k];
+    } else {
+        p.segments = 1;
+        p.pa[0] = p.pb[0] = 0;
+    }
+    p.batches = 1;
+    launch_product<E>(p, cut, ai, bi, part, e, s);
+}
+
+inline dim3 lay_grid(int64_t chunks, int cus) {
+    return dim3((uint32_t)std::max<int64_t>(1, std::min<int64_t>((chunks + 255) / 256, int64_t(cus) * 32)));
+}
+
+template <class T>
+void lay(const Laid& l1, const Source& s1, const Laid& l2, const Source& s2, char* workspace, int cus, hipStream_t s) {
+    auto full = [&](const Laid& l, Source src) {
+        if (!l.copy) return Source{};
+        src.to = workspace + l.at;
+        src.to_rows = l.rows;
+        src.to_cols = l.cols;
+        src.plane = l.plane;
+        return src;
+    };
+    const Source a = full(l1, s1), b = full(l2, s2);
+    const int64_t n = a.to_rows * (a.to_cols / 8) + b.to_rows * (b.to_cols / 8);
+    if (n) k_lay<T><<<lay_grid(n, cus), 256, 0, s>>>(a, b);
+}
+
+// ------------------------------------------------------------------ forward
+
+struct LinearPlan {
+    Laid x, w;
+    Cut cut;
+    int64_t k;
+    size_t part, bytes;
+};
+
+template <class T>
+LinearPlan linear_plan(const wc_linear_args& a, int cus) {
+    constexpr int parts = Parts<T>::COUNT;
+    LinearPlan p = {};
+    const bool io = a.weight_layout == WC_WEIGHT_IN_OUT;
+    p.x = laid<T>(a.x, a.x_stride, a.rows, a.width);
+    p.w = io ? laid<T>(a.weight, a.weight_stride, a.width, a.out) : laid<T>(a.weight, a.weight_stride, a.out, a.width);
+    p.k = parts > 1 ? up(a.width, STEP) : a.width;
+    p.cut = cut_of(a.rows, a.out, p.k, parts > 1 ? 6 : 1, cus);
+    size_t at = 0;
+    auto take = [&](size_t n) {
+        const size_t here = at;
+        at += pad256(n);
+        return here;
+    };
+    p.x.at = take(p.x.bytes(parts));
+    p.w.at = take(p.w.bytes(parts));
+    p.part = take(p.cut.bytes(a.rows * a.out));
+    p.bytes = at;
+    return p;
+}
+
+template <class T>
+void linear(const wc_linear_args& a, int cus, hipStream_t s) {
+    if (!a.rows) return;
+    const LinearPlan p = linear_plan<T>(a, cus);
+    char* w = (char*)a.workspace;
+    const bool io = a.weight_layout == WC_WEIGHT_IN_OUT;
+    lay<T>(p.x, {a.x, a.x_stride, a.rows, a.width}, p.w,
+           {a.weight, a.weight_stride, io ? a.width : a.out, io ? a.out : a.width}, w, cus, s);
+    Product m = {};
+    m.a = operand<T>(p.x, a.x, w, a.rows);
+    m.b = operand<T>(p.w, a.weight, w, a.out);
+    m.k = p.k;
+    const LayerEpilogue<T> e = {a.bias, a.bias_dtype == WC_DTYPE_F32, (const T*)a.residual, a.residual_stride,
+                                (T*)a.pre, a.pre_stride, (T*)a.y, a.y_stride, a.act};
+    multiply<T>(m, p.cut, true, !io, (float*)(w + p.part), e, s);
+}
+
+// ----------------------------------------------------------------- backward
+
+// d_pre = d_out act'(pre), in the parts that its products read (`to` may be null: not needed), and its column sums,
+// from the unrounded float32 values: 32 chunks of eight columns by eight rows a workgroup, over `per` rows.
+template <class T>
+__global__ __launch_bounds__(256) void k_slope(wc_linear_back_args a, Source d, int64_t per, float* sums) {
+    __shared__ float4 add[256][2];
+    const int64_t c = (int64_t(blockIdx.x) * 32 + threadIdx.x % 32) * 8, lo = int64_t(blockIdx.y) * per;
+    const int64_t rows = d.to ? d.to_rows : a.rows, hi = min(lo + per, rows);
+    const int lane = threadIdx.x / 32, have = (int)min<int64_t>(8, a.out - c);
+    float sum[8] = {};
+    for (int64_t r = lo + lane; r < hi; r += 8) {
+        float v[8] = {};
+        if (r < a.rows && have > 0) {
+            load_n((const T*)a.d_out + r * a.d_out_stride + c, have, 0.f, v);
+            if (a.act != WC_ACT_NONE) {
+                float z[8];
+                load_n((const T*)a.pre + r * a.pre_stride + c, have, 0.f, z);
+                act_slopes(z, a.act);
+#pragma unroll
+                for (int u = 0; u < 8; u++) v[u] = u < have ? v[u] * z[u] : 0.f;
+            }
+#pragma unroll
+            for (int u = 0; u < 8; u++) sum[u] += v[u];
+        }
+        if (d.to && c < d.to_cols) put_parts<T>(d.to + 2 * (r * d.to_cols + c), d.plane, v);
+    }
+    if (!sums) return;
+    add[threadIdx.x][0] = {sum[0], sum[1], sum[2], sum[3]};
+    add[threadIdx.x][1] = {sum[4], sum[5], sum[6], sum[7]};
+    __syncthreads();
+    // one column a thread
+    const int64_t j = int64_t(blockIdx.x) * 256 + threadIdx.x;
+    if (j >= a.out) return;
+    const float* one = (const float*)add + (threadIdx.x / 8) * 8 + threadIdx.x % 8;
+    float s = 0.f;
+#pragma unroll
+    for (int u = 0; u < 8; u++) s += one[u * 32 * 8];
+    sums[int64_t(blockIdx.y) * a.out + j] = s;
+}
+
+// The row blocks' column sums added in order.
+static __global__ __launch_bounds__(256) void k_slope_sum(const float* sums, int64_t out, int blocks, float* to) {
+    __shared__ float four[4][64];
+    const int64_t j = int64_t(blockIdx.x) * 64 + threadIdx.x % 64;
+    const int q = threadIdx.x / 64;
+    float s = 0.f;
+    if (j < out)
+        for (int k = q; k < blocks; k += 4) s += sums[k * out + j];
+    four[q][threadIdx.x % 64] = s;
+    __syncthreads();
+    if (!q && j < out) to[j] = (s + four[1][threadIdx.x]) + (four[2][threadIdx.x] + four[3][threadIdx.x]);
+}
+
+struct LinearBackPlan {
+    Laid d, x, w;
+    Cut cut_x, cut_w;
+    int64_t out_k, rows_k, per;
+    int blocks;
+    bool slope;
+    size_t sums, part, bytes;
+};
+
+template <class T>
+LinearBackPlan linear_back_plan(const wc_linear_back_args& a, int cus) {
+    constexpr int parts = Parts<T>::COUNT;
+    LinearBackPlan p = {};
+    const bool io = a.weight_layout == WC_WEIGHT_IN_OUT;
+    p.d = laid<T>(a.d_out, a.d_out_stride, a.rows, a.out);
+    if (a.act != WC_ACT_NONE && !p.d.copy) {
+        p.d.copy = true;
+        p.d.rows = a.rows;
+        p.d.cols = up(a.out, 8);
+        p.d.pitch = 2 * p.d.cols;
+        p.d.plane = p.d.pitch * p.d.rows;
+    }
+    const bool products = a.d_x || a.d_weight;
+    p.slope = (p.d.copy && products) || a.d_bias;
+    size_t at = 0;
+    auto take = [&](size_t n) {
+        const size_t here = at;
+        at += pad256(n);
+        return here;
+    };
+    if (products) p.d.at = take(p.d.bytes(parts));
+    size_t part = 0;
+    if (a.d_x) {
+        p.w = io ? laid<T>(a.weight, a.weight_stride, a.width, a.out) : laid<T>(a.weight, a.weight_stride, a.out, a.width);
+        p.w.at = take(p.w.bytes(parts));
+        p.out_k = parts > 1 ? up(a.out, STEP) : a.out;
+        p.cut_x = cut_of(a.rows, a.width, p.out_k, parts > 1 ? 6 : 1, cus);
+        part = std::max(part, p.cut_x.bytes(a.rows * a.width));
+    }
+    if (a.d_weight) {
+        p.x = laid<T>(a.x, a.x_stride, a.rows, a.width);
+        p.x.at = take(p.x.bytes(parts));
+        p.rows_k = parts > 1 ? up(a.rows, STEP) : a.rows;
+        p.cut_w = cut_of(io ? a.width : a.out, io ? a.out : a.width, p.rows_k, parts > 1 ? 6 : 1, cus);
+        part = std::max(part, p.cut_w.bytes(a.width * a.out));
+    }
+    p.part = take(part);  // one after the other in it
+    if (p.slope) {
+        const int64_t across = (a.out + 255) / 256;
+        const int64_t blocks = std::max<int64_t>(1, std::min<int64_t>((a.rows + 31) / 32, 8 * int64_t(cus) / across + 1));
+        p.per = up((std::max<int64_t>(p.d.copy ? p.d.rows : a.rows, 1) + blocks - 1) / blocks, 8);
+        p.blocks = (int)((std::max<int64_t>(p.d.copy ? p.d.rows : a.rows, 1) + p.per - 1) / p.per);
+        if (a.d_bias) p.sums = take(size_t(p.blocks) * a.out * 4);
+    }
+    p.bytes = at;
+    return p;
+}
+
+template <class T>
+LayerEpilogue<T> plain_to(void* y, int64_t stride) {
+    LayerEpilogue<T> e = {};
+    e.y = (T*)y;
+    e.y_stride = stride;
+    e.act = WC_ACT_NONE;
+    return e;
+}
+
+template <class T>
+void linear_back(const wc_linear_back_args& a, int cus, hipStream_t s) {
+    const LinearBackPlan p = linear_back_plan<T>(a, cus);
+    char* w = (char*)a.workspace;
+    const bool io = a.weight_layout == WC_WEIGHT_IN_OUT, products = a.d_x || a.d_weight;
+    if (p.slope) {
+        Source d = {};
+        if (products && p.d.copy) {
+            d.to = w + p.d.at;
+            d.to_rows = p.d.rows;
+            d.to_cols = p.d.cols;
+            d.plane = p.d.plane;
+        }
+        float* sums = a.d_bias ? (float*)(w + p.sums) : nullptr;
+        const int64_t across = ((d.to ? p.d.cols : a.out) + 255) / 256;
+        k_slope<T><<<dim3((uint32_t)across, (uint32_t)p.blocks), 256, 0, s>>>(a, d, p.per, sums);
+        if (sums) k_slope_sum<<<dim3((uint32_t)((a.out + 63) / 64)), 256, 0, s>>>(sums, a.out, p.blocks, a.d_bias);
+    }
+    if (!products) return;
+    // copies of x and the weight, in one launch
+    lay<T>(p.x, {a.x, a.x_stride, a.rows, a.width}, p.w,
+           {a.weight, a.weight_stride, io ? a.width : a.out, io ? a.out : a.width}, w, cus, s);
+    float* part = (float*)(w + p.part);
+    if (a.d_x && a.rows) {
+        Product m = {};
+        m.a = operand<T>(p.d, a.d_out, w, a.rows);
+        m.b = operand<T>(p.w, a.weight, w, a.width);
+        m.k = p.out_k;
+        multiply<T>(m, p.cut_x, true, io, part, plain_to<T>(a.d_x, a.d_x_stride), s);
+    }
+    if (a.d_weight) {
+        Product m = {};
+        const Operand16 x = operand<T>(p.x, a.x, w, a.width), d = operand<T>(p.d, a.d_out, w, a.out);
+        m.a = io ? x : d;
+        m.b = io ? d : x;
+        m.k = p.rows_k;
+        if (a.grad_dtype == a.dtype) {
+            multiply<T>(m, p.cut_w, false, false, part, plain_to<T>(a.d_weight, a.d_weight_stride), s);
+        } else if constexpr (Parts<T>::COUNT == 1) {
+            multiply<T>(m, p.cut_w, false, false, part, plain_to<float>(a.d_weight, a.d_weight_stride), s);
+        }
+    }
+}
+
+}  // namespace
+}  // namespace learn
+}  // namespace wc

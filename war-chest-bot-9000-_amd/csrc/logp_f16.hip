@@ -1,0 +1,12 @@
+// Token log-probabilities and their gradient over f16 logits.
+#include "logp_dev.h"
+
+namespace wc {
+namespace learn {
+
+size_t logp_scratch_f16(const wc_logp_args& a, int cus) { return logp_plan<f16>(a.rows, a.vocab, a.top, cus).bytes; }
+void logp_f16(const wc_logp_args& a, int cus, hipStream_t s) { logp<f16>(a, cus, s); }
+void logp_back_f16(const wc_logp_back_args& a, hipStream_t s) { logp_back<f16>(a, s); }
+
+}  // namespace learn
+}  // namespace wc

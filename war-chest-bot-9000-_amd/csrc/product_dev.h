@@ -1,0 +1,456 @@
+// Matrix products on the matrix cores, C[m x n] = sum over k of A[i][k] B[k][j], with an epilogue that the caller gives:
+// the layers' products (linear.hip) and the Newton-Schulz steps (newton.hip).
+//
+// An operand's index of summation is its contiguous one (INNER: A as rows of k, B as rows of k for each column) or its
+// outer one. Tiles go from memory to LDS without passing registers, four buffers of 32 values of k, three of them in
+// flight. INNER tiles come back as 16 bytes a lane, the others through the transposing LDS read. A workgroup of four
+// wavefronts owns a square tile of 64 F, each wavefront a quarter in F x F fragments of 32 x 32. Everything else goes
+// between the matrix instructions: F of them, then the loads and the reads of one part.
+//
+// An operand may have several planes that add up to it; the product is then a sum of segments, pairs of planes, one
+// after the other along k.
+#pragma once
+
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+#include <cstdint>
+
+#include "learn_dev.h"
+
+#pragma clang fp contract(fast)
+
+namespace wc {
+namespace learn {
+namespace {
+
+constexpr int PRODUCT_BLOCK = 256, STEP = 32, STEP_BUFFERS = 4;
+constexpr int MOST_SEGMENTS = 6, MOST_PLANES = 3;
+
+typedef f16 f16x8 __attribute__((ext_vector_type(8)));
+typedef bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) char* LdsAt;
+
+__device__ __forceinline__ f32x16 mfma(f16x8 a, f16x8 b, f32x16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
+}
+__device__ __forceinline__ f32x16 mfma(bf16x8 a, bf16x8 b, f32x16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+}
+
+// One operand: rows of `pitch` bytes on 16-byte bounds, the contiguous index in whole chunks of eight
+// (zeros past its end where it is k). `outer` rows of A or columns of B.
+struct Operand16 {
+    const char* plane[MOST_PLANES];
+    int64_t pitch, batch;  // bytes from row to row, from one matrix to the next
+    int64_t outer;
+};
+
+struct Product {
+    Operand16 a, b;
+    int64_t k;                 // of each segment
+    int32_t segments;
+    uint8_t pa[MOST_SEGMENTS], pb[MOST_SEGMENTS];  // a segment's planes
+    int32_t tiles_m, tiles_n, runs, batches;
+    int32_t triangle;          // the tiles' size where the result is symmetric and only those on and above the diagonal are made
+    int32_t steps, run_steps;  // steps of all segments together, and of one run
+    float* part;               // runs > 1: runs x batches x m x n partial products
+};
+
+static __device__ __align__(16) uint4 g_zeros;  // what lies past the end is read from here
+
+// Where a step's tiles are, the same for all lanes.
+struct Cursor {
+    const char *a, *b;
+    int segment, left;  // steps left in the segment
+};
+
+template <int F>
+struct TileShape {
+    static constexpr int TILE = 64 * F, SIDE = TILE * 2 * STEP, BUFFER = 2 * SIDE;
+    static constexpr int LDS = STEP_BUFFERS * BUFFER;
+    // where rows are on k: 64-byte units a row, exchanged so that the four rows of a transposing read lie in different
+    // banks. A pitch of 128 bytes puts rows 0 and 1 there by itself.
+    static __device__ __forceinline__ int turn(int row) { return F == 1 ? (row >> 1) & 1 : row & 3; }
+};
+
+// A wavefront's loads of one operand: F of 64 lanes x 16 bytes each, to places in LDS that follow each other.
+template <int F, bool INNER>
+struct Loads {
+    uint32_t at[F];  // the lane's place, from the tile's first row
+    int32_t k[F];    // the first of k that it brings
+
+    __device__ __forceinline__ void set(const Operand16& o, int64_t first, int wave, int lane) {
+        typedef TileShape<F> S;
+#pragma unroll
+        for (int q = 0; q < F; q++) {
+            const int g = (wave * F + q) * 64 + lane;
+            if (INNER) {
+                const int row = g / 4, chunk = (g % 4) ^ (row >> 1 & 3);
+                // past the last row any row will do: its products are not stored
+                const int64_t r = min(first + row, o.outer - 1) - first;
+                at[q] = (uint32_t)(r * o.pitch) + 16 * chunk;
+                k[q] = 8 * chunk;
+            } else {
+                const int row = g / (S::TILE / 8), chunk = (g % (S::TILE / 8)) ^ (S::turn(row) << 2);
+                at[q] = (uint32_t)(row * o.pitch) + (first + 8 * chunk < o.outer ? 16 * chunk : 0);
+                k[q] = row;
+            }
+        }
+    }
+    // ENDS: what lies at or past `left` of k is read from zeros.
+    template <bool ENDS>
+    __device__ __forceinline__ void load(const char* base, int q, int64_t left, LdsAt to) const {
+        const char* from = base + at[q];
+        if (ENDS && k[q] >= left) from = (const char*)&g_zeros;
+        __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)from,
+                                         (__attribute__((address_space(3))) void*)(to + 1024 * q), 16, 0, 0);
+    }
+};
+
+// A wavefront's reads of one operand's fragments: lane l has eight of k, from 8 (l / 32) on, of row or column l % 32.
+template <int F, bool INNER>
+struct Reads {
+    uint32_t at[INNER ? 2 : F];
+
+    __device__ __forceinline__ void set(int first, int lane) {
+        typedef TileShape<F> S;
+        if (INNER) {
+            const int row = first + (lane & 31);
+#pragma unroll
+            for (int h = 0; h < 2; h++) at[h] = row * 64 + 16 * ((2 * h + (lane >> 5)) ^ (row >> 1 & 3));
+        } else {
+            const int row = 8 * (lane >> 5) + ((lane & 15) >> 2);
+#pragma unroll
+            for (int m = 0; m < F; m++)
+                at[m] = row * 2 * S::TILE +
+                        ((2 * (first + 32 * m + (lane & 16) + 4 * (lane & 3))) ^ (S::turn(row) << 6));
+        }
+    }
+    template <class E8>
+    __device__ __forceinline__ E8 take(LdsAt from, int half, int m) const {
+        typedef TileShape<F> S;
+        if constexpr (INNER) {
+            typedef __attribute__((address_space(3))) E8* At;
+            return *(At)(from + at[half] + m * 32 * 64);
+        } else {
+            typedef __attribute__((address_space(3))) s16x4* At;
+            const LdsAt p = from + at[m] + half * 16 * 2 * S::TILE;
+            // four rows on, the exchange of units is the same
+            const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((At)p);
+            const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((At)(p + 4 * 2 * S::TILE));
+            return __builtin_bit_cast(E8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+        }
+    }
+};
+
+// Of the loads of three buffers the first third has arrived when the others are left.
+template <int LEFT>
+__device__ __forceinline__ void arrived() {
+    static_assert(LEFT == 4 || LEFT == 8 || LEFT == 16, "two steps' loads");
+    if constexpr (LEFT == 4) asm volatile("s_waitcnt vmcnt(4) lgkmcnt(0)" ::: "memory");
+    else if constexpr (LEFT == 8) asm volatile("s_waitcnt vmcnt(8) lgkmcnt(0)" ::: "memory");
+    else asm volatile("s_waitcnt vmcnt(16) lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+}
+
+template <class E, int F, bool AI, bool BI>
+struct Tiles {
+    typedef E E8 __attribute__((ext_vector_type(8)));
+    typedef TileShape<F> S;
+    const Product& p;
+    Loads<F, AI> la;
+    Loads<F, BI> lb;
+    Reads<F, AI> ra;
+    Reads<F, BI> rb;
+    Cursor c;
+    int64_t a0, b0;  // bytes from a plane's start to the tile's
+    int steps_in;    // of a segment
+
+    __device__ __forceinline__ Tiles(const Product& product, int batch, int64_t i0, int64_t j0, int wave, int lane)
+        : p(product) {
+        la.set(p.a, i0, wave, lane);
+        lb.set(p.b, j0, wave, lane);
+        ra.set((wave >> 1) * 32 * F, lane);
+        rb.set((wave & 1) * 32 * F, lane);
+        a0 = batch * p.a.batch + (AI ? i0 * p.a.pitch : 2 * i0);
+        b0 = batch * p.b.batch + (BI ? j0 * p.b.pitch : 2 * j0);
+        steps_in = (int)((p.k + STEP - 1) / STEP);
+    }
+    __device__ __forceinline__ int64_t a_step() const { return AI ? 2 * STEP : STEP * p.a.pitch; }
+    __device__ __forceinline__ int64_t b_step() const { return BI ? 2 * STEP : STEP * p.b.pitch; }
+    __device__ __forceinline__ void seek(int s) {
+        c.segment = p.segments > 1 ? s / steps_in : 0;
+        const int in = s - c.segment * steps_in;
+        c.left = steps_in - in;
+        c.a = p.a.plane[p.pa[c.segment]] + a0 + in * a_step();
+        c.b = p.b.plane[p.pb[c.segment]] + b0 + in * b_step();
+    }
+    __device__ __forceinline__ void next() {
+        c.a += a_step();
+        c.b += b_step();
+        if (--c.left == 0 && c.segment + 1 < p.segments) {
+            c.segment++;
+            c.left = steps_in;
+            c.a = p.a.plane[p.pa[c.segment]] + a0;
+            c.b = p.b.plane[p.pb[c.segment]] + b0;
+        }
+    }
+    // One part of a step's loads. left: what of k is there from the cursor on.
+    template <bool ENDS>
+    __device__ __forceinline__ void load(int q, int64_t left, LdsAt to) const {
+        la.template load<ENDS>(c.a, q, left, to);
+        lb.template load<ENDS>(c.b, q, left, to + S::SIDE);
+    }
+
+    // One step: the buffer `from`, whose first fragments are in fa and fb, and the first of `next`; the loads of three
+    // steps on go to `to`. The three are different buffers: told so, the compiler lets reads pass loads in flight.
+    template <bool ENDS>
+    __device__ __forceinline__ void step(LdsAt __restrict__ from, LdsAt __restrict__ following, LdsAt __restrict__ to,
+                                         int64_t left, E8 (&fa)[F], E8 (&fb)[F], f32x16 (&acc)[F][F]) {
+        E8 na[F], nb[F];
+#pragma unroll
+        for (int m = 0; m < F; m++) {
+            load<ENDS>(m, left, to);
+            na[m] = ra.template take<E8>(from, 1, m);
+            nb[m] = rb.template take<E8>(from + S::SIDE, 1, m);
+#pragma unroll
+            for (int n = 0; n < F; n++) acc[m][n] = mfma(fa[m], fb[n], acc[m][n]);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        next();
+        E8 oa[F], ob[F];
+#pragma unroll
+        for (int m = 0; m < F; m++) {
+#pragma unroll
+            for (int n = 0; n < F; n++) acc[m][n] = mfma(na[m], nb[n], acc[m][n]);
+            __builtin_amdgcn_sched_barrier(0);
+            if (m == 0) arrived<4 * F>();  // the next buffer's, and every wavefront has read this one's
+            oa[m] = ra.template take<E8>(following, 0, m);
+            ob[m] = rb.template take<E8>(following + S::SIDE, 0, m);
+        }
+#pragma unroll
+        for (int m = 0; m < F; m++) fa[m] = oa[m], fb[m] = ob[m];
+    }
+
+    // Steps lo .. hi of the product.
+    __device__ __forceinline__ void run(LdsAt base, int wave, int lo, int hi, f32x16 (&acc)[F][F]) {
+        const LdsAt mine = base + wave * F * 1024;
+        // steps whose loads are whole: the last of a segment may not be
+        const int whole = p.segments == 1 ? min(hi, (int)(p.k / STEP)) : p.k % STEP == 0 ? hi : 0;
+        auto left = [&](int s) -> int64_t { return s >= hi ? 0 : p.k - int64_t(steps_in - c.left) * STEP; };
+        auto buffer = [](LdsAt at, int s) { return at + (s & 3) * S::BUFFER; };
+        E8 fa[F], fb[F];
+        seek(lo);
+        for (int s = 0; s < 3; s++) {
+#pragma unroll
+            for (int q = 0; q < F; q++) load<true>(q, left(lo + s), buffer(mine, s));
+            next();
+        }
+        arrived<4 * F>();
+#pragma unroll
+        for (int m = 0; m < F; m++) {
+            fa[m] = ra.template take<E8>(base, 0, m);
+            fb[m] = rb.template take<E8>(base + S::SIDE, 0, m);
+        }
+        int s = 0;
+        for (; lo + s + 3 < whole; s++)
+            step<false>(buffer(base, s), buffer(base, s + 1), buffer(mine, s + 3), STEP, fa, fb, acc);
+        // the last steps load zeros past the end: the count of loads in flight stays the same
+        for (; lo + s < hi; s++)
+            step<true>(buffer(base, s), buffer(base, s + 1), buffer(mine, s + 3), left(lo + s + 3), fa, fb, acc);
+        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+        __builtin_amdgcn_s_barrier();
+    }
+};
+
+// What a product's epilogue sees: eight values of row i from column j, n of them in the matrix.
+//   struct Epilogue { __device__ void operator()(int batch, int64_t i, int64_t j, int n, float (&v)[8]) const; }
+// MIRROR: symmetric results; the epilogue also gets columns as rows.
+template <class E, int F, bool AI, bool BI, class Epilogue>
+__global__ __launch_bounds__(PRODUCT_BLOCK, F == 4 ? 1 : 2) void k_product(Product p, Epilogue epilogue) {
+    typedef TileShape<F> S;
+    __shared__ __align__(16) char lds[S::LDS];
+    const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
+    // Workgroups go round the eight XCDs; consecutive tiles, which share panels of both operands, go to one XCD's cache.
+    const unsigned total = gridDim.x, per = total / 8;
+    const int id = blockIdx.x < per * 8 ? (blockIdx.x % 8) * per + blockIdx.x / 8 : blockIdx.x;
+    const int tiles = p.triangle ? p.tiles_m * (p.tiles_m + 1) / 2 : p.tiles_m * p.tiles_n;
+    const int batch = id / (tiles * p.runs), run = id / tiles - batch * p.runs, tile = id % tiles;
+    int ti, tj;
+    if (p.triangle) {
+        // column tj has tiles 0 .. tj
+        tj = (int)((sqrtf(8.f * tile + 1.f) - 1.f) * 0.5f);
+        while (tj * (tj + 1) / 2 > tile) tj--;
+        while ((tj + 1) * (tj + 2) / 2 <= tile) tj++;
+        ti = tile - tj * (tj + 1) / 2;
+    } else {
+        // four rows of tiles at a time: 32 neighbouring workgroups share 4 + 8 panels
+        const int band = tile / (4 * p.tiles_n), high = min(4, p.tiles_m - 4 * band), in = tile - band * 4 * p.tiles_n;
+        ti = 4 * band + in % high, tj = in / high;
+    }
+    const int64_t i0 = int64_t(ti) * S::TILE, j0 = int64_t(tj) * S::TILE;
+    const int lo = run * p.run_steps, hi = min(lo + p.run_steps, p.steps);
+
+    f32x16 acc[F][F] = {};
+    if (lo < hi) {
+        Tiles<E, F, AI, BI> tiles_of(p, batch, i0, j0, wave, lane);
+        tiles_of.run((LdsAt)lds, wave, lo, hi, acc);
+    }
+
+    // Through LDS to whole rows: a lane has one column of sixteen rows, memory wants eight columns of one.
+    constexpr int WIDE = 32 * F, PITCH = WIDE + 4, CHUNKS = WIDE / 8, ROWS = 64 / CHUNKS;
+    static_assert(32 * PITCH * 4 <= S::LDS / 4, "a wavefront's fragments of 32 rows fit its part");
+    float* mine = (float*)(lds + wave * (S::LDS / 4));
+    const int64_t wi = i0 + (wave >> 1) * WIDE, wj = j0 + (wave & 1) * WIDE, m_all = p.a.outer, n_all = p.b.outer;
+    float* part = p.runs > 1 ? p.part + (int64_t(run) * p.batches + batch) * m_all * n_all : nullptr;
+#pragma unroll
+    for (int m = 0; m < F; m++) {
+#pragma unroll
+        for (int n = 0; n < F; n++)
+#pragma unroll
+            for (int k = 0; k < 16; k++)
+                mine[(8 * (k / 4) + 4 * (lane >> 5) + k % 4) * PITCH + 32 * n + (lane & 31)] = acc[m][n][k];
+        __builtin_amdgcn_wave_barrier();
+        for (int it = 0; it < 32 / ROWS; it++) {
+            const int r = it * ROWS + lane / CHUNKS, c = 8 * (lane % CHUNKS);
+            const int64_t i = wi + 32 * m + r, j = wj + c;
+            if (i >= m_all || j >= n_all) continue;
+            const float4 lo4 = *(const float4*)(mine + r * PITCH + c), hi4 = *(const float4*)(mine + r * PITCH + c + 4);
+            float v[8] = {lo4.x, lo4.y, lo4.z, lo4.w, hi4.x, hi4.y, hi4.z, hi4.w};
+            const int have = (int)min<int64_t>(8, n_all - j);
+            if (part) store_n(part + i * n_all + j, have, v);
+            else epilogue(batch, i, j, have, v);
+        }
+        if (Epilogue::MIRROR && p.triangle && ti != tj && !part) {
+            // a row of the other half: 32 of i, eight a lane
+            for (int it = 0; it < WIDE / 16; it++) {
+                const int c = it * 16 + lane / 4, r = 8 * (lane % 4);
+                const int64_t i = wj + c, j = wi + 32 * m + r;
+                if (i >= n_all || j >= m_all) continue;
+                float v[8];
+#pragma unroll
+                for (int u = 0; u < 8; u++) v[u] = mine[(r + u) * PITCH + c];
+                epilogue(batch, i, j, (int)min<int64_t>(8, m_all - j), v);
+            }
+        }
+        __builtin_amdgcn_wave_barrier();
+    }
+}
+
+// The runs' partial products added, in an order that does not change: eight elements of a row a thread, a quarter of
+// the runs each wavefront.
+template <class Epilogue>
+__global__ __launch_bounds__(PRODUCT_BLOCK) void k_product_sum(Product p, int64_t chunks, Epilogue epilogue) {
+    typedef float Eight __attribute__((ext_vector_type(8)));
+    __shared__ Eight quarters[3][64];
+    const int quarter = threadIdx.x >> 6, lane = threadIdx.x & 63;
+    const int64_t m = p.a.outer, n = p.b.outer, at = int64_t(blockIdx.x) * 64 + lane, per_row = (n + 7) / 8;
+    const bool there = at < chunks;
+    const int64_t row = at / per_row, j = (at - row * per_row) * 8;  // a row of all matrices
+    const int have = (int)min<int64_t>(8, n - j);
+    const int64_t i = row % m, batch = row / m;
+    // a symmetric result's lower tiles are read from their mirror images
+    const bool lower = p.triangle && i / p.triangle > j / p.triangle;
+    Eight s = {};
+    if (there) {
+        const float* from = p.part + batch * m * n;
+        const int64_t stride = int64_t(p.batches) * m * n;
+        for (int k = quarter; k < p.runs; k += 4) {
+            float v[8] = {};
+            if (!lower) {
+                load_n(from + k * stride + i * n + j, have, 0.f, v);
+            } else {
+                for (int u = 0; u < have; u++) v[u] = from[k * stride + (j + u) * n + i];
+            }
+#pragma unroll
+            for (int u = 0; u < 8; u++) s[u] += v[u];
+        }
+    }
+    if (quarter) quarters[quarter - 1][lane] = s;
+    __syncthreads();
+    if (quarter || !there) return;
+    s = (s + quarters[0][lane]) + (quarters[1][lane] + quarters[2][lane]);
+    float v[8];
+#pragma unroll
+    for (int u = 0; u < 8; u++) v[u] = s[u];
+    epilogue((int)batch, i, j, have, v);
+}
+
+// ---------------------------------------------------------------- the host's side
+
+inline int64_t up(int64_t n, int64_t to) { return (n + to - 1) / to * to; }
+
+// How a product is cut: tiles of 64 F, and runs along k.
+struct Cut {
+    int f, runs, run_steps, steps;
+    int64_t tiles_m, tiles_n;
+    bool triangle;
+
+    // of the runs' partial products; n all matrices' elements
+    size_t bytes(int64_t n) const { return runs > 1 ? size_t(runs) * n * 4 : 0; }
+};
+
+inline Cut cut_of(int64_t m, int64_t n, int64_t k, int segments, int cus, int64_t batches = 1, bool triangle = false) {
+    Cut best = {};
+    double least = -1;
+    const int64_t steps = (k + STEP - 1) / STEP * segments;
+    for (int f = 4; f >= 1; f /= 2) {
+        const int64_t tile = 64 * f, tm = (m + tile - 1) / tile, tn = (n + tile - 1) / tile, 
+                      tiles = std::max<int64_t>(1, batches * (triangle ? tm * (tm + 1) / 2 : tm * tn));
+        const int64_t slots = f == 4 ? cus : f == 2 ? 2 * cus : 4 * cus;
+        const double step = f == 4 ? 0.8 : f == 2 ? 0.5 : 0.4;
+        const int64_t most = std::max<int64_t>(1, std::min<int64_t>(steps / 4, 4 * slots / tiles));
+        for (int64_t r = 1; r <= 64; r = r < 8 ? r + 1 : r * 5 / 4) {
+            if (r > most) break;
+            const int64_t per = (steps + r - 1) / r, runs = per ? (steps + per - 1) / per : 1;
+            const int64_t rounds = (tiles * runs + slots - 1) / slots;
+            const double t = double(rounds) * (double(per) * step + 3.0) +
+                             (runs > 1 ? 4.0 + double(runs) * batches * m * n * 8 / 5e6 : 0.0);
+            if (least >= 0 && t >= least) continue;
+            least = t;
+            best.f = f;
+            best.runs = (int)std::max<int64_t>(1, runs);
+            best.run_steps = (int)per;
+            best.steps = (int)steps;
+            best.tiles_m = tm;
+            best.tiles_n = tn;
+            best.triangle = triangle;
+        }
+    }
+    return best;
+}
+
+template <class E, int F, class Epilogue>
+void product_of(const Product& p, bool ai, bool bi, const Epilogue& e, hipStream_t s) {
+    const int tiles = p.triangle ? p.tiles_m * (p.tiles_m + 1) / 2 : p.tiles_m * p.tiles_n;
+    const dim3 grid((uint32_t)(tiles * p.runs * p.batches));
+    if (ai && bi) k_product<E, F, true, true><<<grid, PRODUCT_BLOCK, 0, s>>>(p, e);
+    else if (ai) k_product<E, F, true, false><<<grid, PRODUCT_BLOCK, 0, s>>>(p, e);
+    else k_product<E, F, false, false><<<grid, PRODUCT_BLOCK, 0, s>>>(p, e);
+}
+
+// a, b, k, segments and batches are set.
+template <class E, class Epilogue>
+void launch_product(Product p, const Cut& cut, bool ai, bool bi, float* part, const Epilogue& e, hipStream_t s) {
+    p.tiles_m = (int)cut.tiles_m;
+    p.tiles_n = (int)cut.tiles_n;
+    p.runs = cut.runs;
+    p.run_steps = cut.run_steps;
+    p.steps = cut.steps;
+    p.triangle = cut.triangle ? 64 * cut.f : 0;
+    p.part = part;
+    if (cut.f == 4) product_of<E, 4>(p, ai, bi, e, s);
+    else if (cut.f == 2) product_of<E, 2>(p, ai, bi, e, s);
+    else product_of<E, 1>(p, ai, bi, e, s);
+    if (cut.runs > 1) {
+        const int64_t chunks = p.batches * p.a.outer * ((p.b.outer + 7) / 8);
+        k_product_sum<<<dim3((uint32_t)((chunks + 63) / 64)), PRODUCT_BLOCK, 0, s>>>(p, chunks, e);
+    }
+}
+
+}  // namespace
+}  // namespace learn
+}  // namespace wc

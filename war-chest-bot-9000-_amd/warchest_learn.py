@@ -7,13 +7,17 @@ What a trainer of the policy or value network runs on the solver's results, on t
 - `residual_norm`, `residual_norm_backward`: a block's output normed, gated, scaled and added to the residual stream, and
   the norm before the next block;
 - `checkpoint8`, `checkpoint8_act`, `checkpoint8_read`, `checkpoint8_act_backward`, `checkpoint8_weight_grad`:
-  activations kept in 8 bits for the backward pass, and what the backward pass does with them.
+  activations kept in 8 bits for the backward pass, and what the backward pass does with them;
+- `linear`, `linear_backward`: a layer's product with bias, activation and residual in its epilogue, and its gradients;
+- `orthogonalise`: a weight's update with its singular values brought towards 1 by Newton-Schulz products;
+- `token_logp`, `token_logp_backward`: log-probabilities of given tokens with their rank, the entropy and the top
+  alternatives of rows of logits, and the gradient.
 
 Every call is queued on the current stream of its tensors' device and returns at once. Outputs and scratch are allocated
 with torch on that stream; a tensor made on another stream must be ready there, and kept alive by its owner
 (`Tensor.record_stream`), as for torch's own operators. Matrices need unit column stride, rows may be at any stride.
-Arguments that do not fit raise `WaveError`, and then nothing was queued. The `*_objective` functions and `ResidualNorm`
-are the same calls with torch's automatic differentiation.
+Arguments that do not fit raise `WaveError`, and then nothing was queued. The `*_objective` functions, `ResidualNorm`,
+`dense` and `Dense` are the same calls with torch's automatic differentiation, `Muon` an optimiser on `orthogonalise`.
 
 Nothing here computes: every call goes through the native library.
 """
@@ -34,6 +38,9 @@ EXPORTS = [
     "wc_policy_workspace", "wc_policy_loss", "wc_preference_workspace", "wc_preference_loss",
     "wc_residual_norm", "wc_residual_norm_workspace", "wc_residual_norm_backward",
     "wc_ckpt_write", "wc_ckpt_read", "wc_ckpt_act_backward", "wc_ckpt_weight_workspace", "wc_ckpt_weight_grad",
+    "wc_linear_workspace", "wc_linear", "wc_linear_backward_workspace", "wc_linear_backward",
+    "wc_orthogonalise_workspace", "wc_orthogonalise",
+    "wc_token_logp_workspace", "wc_token_logp", "wc_token_logp_backward",
 ]
 
 DTYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
@@ -42,6 +49,7 @@ GATE_ACTS = {"none": 0, "sigmoid": 1, "tanh": 2}
 ACTS = {"none": 0, "relu": 1, "gelu": 2, "silu": 3}
 KINDS = {"logistic": 0, "squared": 1, "hinge": 2}
 GROUP = 32
+TOP_MAX = 64
 
 # The structures of the header, packed in C's own layout: a call fills one in one step.
 _POLICY = struct.Struct("@Qii qq PqPqPq PPPPPP fffffi PPPPPq PQ")
@@ -50,12 +58,20 @@ _NORM = struct.Struct("@Qiiii qq PqPq PPPqPP ffii PqPq P")
 _NORM_BACK = struct.Struct("@Qiiii qq PqPq PPPqP fiii PPqPq PqPq PPPPPq PQ")
 _CKPT = struct.Struct("@Qii qq ii PqPq PqPq")
 _WEIGHT = struct.Struct("@Qii qqq ii PqPqPqPq P PQ")
+_LINEAR = struct.Struct("@Qiiii qqq PqPq P Pq ii PqPq PQ")
+_LINEAR_BACK = struct.Struct("@Qiiiiii qqq PqPqPqPq PqPq P PQ")
+_ORTHO = struct.Struct("@Qiiii qqq Pqq Pqq fffffi PQ")
+_LOGP = struct.Struct("@Qii qq PqPq P fiii PPPPPP PQ")
+_LOGP_BACK = struct.Struct("@Qii qq PqPq P fi PPP Pq")
 
 PolicyLoss = namedtuple("PolicyLoss", "loss logp kl entropy grad")
 PreferenceLoss = namedtuple("PreferenceLoss", "loss margins ratios logp grad")
 ResidualNormOut = namedtuple("ResidualNormOut", "stream out stats")
 ResidualNormGrads = namedtuple("ResidualNormGrads", "block stream post_gain post_bias gate pre_gain pre_bias")
 Checkpoint8 = namedtuple("Checkpoint8", "q exps")
+Linear = namedtuple("Linear", "out pre")
+LinearGrads = namedtuple("LinearGrads", "x weight bias")
+TokenLogp = namedtuple("TokenLogp", "logp entropy rank top_logp top_index stats")
 
 _fn = {}
 
@@ -452,6 +468,221 @@ def checkpoint8_weight_grad(ck, grad, *, act="none", bias=False, dtype=None):
     return weight, b
 
 
+# ------------------------------------------------------------------ layers
+
+def _weight_of(t, name, device, dtype, width, out):
+    """(address, row stride, layout) of a weight [width, out] that is contiguous along either index."""
+    if not isinstance(t, torch.Tensor) or t.shape != (width, out):
+        _fail(f"{name}: shape {tuple(getattr(t, 'shape', ()))}, expected ({width}, {out})")
+    s = t.stride()
+    if s[1] == 1 or out == 1 or s[0] != 1:
+        return *_matrix(t, name, device, dtype, width, out), 0
+    if t.dtype is not dtype:
+        _fail(f"{name}: {t.dtype}, expected {dtype}")
+    if t.device != device:
+        _fail(f"{name} is on {t.device}, not on {device}")
+    return t.data_ptr(), s[1], 1
+
+
+# An address that passes for one, on 16 bytes or not: scratch depends on shapes and on where rows start, nothing is read.
+def _stand_in(aligned):
+    return 256 if aligned else 260
+
+
+@functools.lru_cache(maxsize=4096)
+def _linear_scratch(device, code, layout, rows, width, out, xs, ws, x_aligned, w_aligned):
+    p = 256
+    return _scratch_bytes("wc_linear_workspace", _LINEAR.pack(
+        _LINEAR.size, device, code, 0, layout, rows, width, out, _stand_in(x_aligned), xs, _stand_in(w_aligned), ws, 0, 0,
+        0, 0, 0, 0, 0, p, out, 0, 0))
+
+
+@functools.lru_cache(maxsize=4096)
+def _linear_back_scratch(device, code, layout, act, rows, width, out, ds, xs, ws, d_aligned, x_aligned, w_aligned, d_x,
+                         d_weight, d_bias):
+    p = 256
+    return _scratch_bytes("wc_linear_backward_workspace", _LINEAR_BACK.pack(
+        _LINEAR_BACK.size, device, code, layout, act, 0, 0, rows, width, out, _stand_in(d_aligned), ds, p, out,
+        _stand_in(x_aligned), xs, _stand_in(w_aligned), ws, p if d_x else 0, width, p if d_weight else 0,
+        width if layout else out, p if d_bias else 0, 0, 0))
+
+
+def linear(x, weight, bias=None, *, act="none", residual=None, keep=False):
+    """act(x @ weight + bias) + residual in one product (wc_linear).
+
+    x [rows, width], weight [width, out] (contiguous along either index: the transposed view of an [out, width] matrix
+    works as it is), bias [out] in their type or float32, residual [rows, out]. act: "none", "relu", "gelu" or "silu".
+    Returns Linear(out, pre): pre [rows, out], x @ weight + bias, is what linear_backward needs; None unless keep is
+    true and act is not "none"."""
+    device = _device(x, "x")
+    code, dt = _dtype(x, "x"), x.dtype
+    if x.dim() != 2:
+        _fail(f"x: shape {tuple(x.shape)}, expected rows x width")
+    if not isinstance(weight, torch.Tensor) or weight.dim() != 2:
+        _fail("weight: expected width x out")
+    rows, width = x.shape
+    out = weight.shape[1]
+    xp, xs = _matrix(x, "x", device, dt, rows, width)
+    wp, ws, layout = _weight_of(weight, "weight", device, dt, width, out)
+    bias_code = 0
+    if bias is not None:
+        if bias.dtype not in (dt, torch.float32):
+            _fail(f"bias: {bias.dtype}, expected {dt} or float32")
+        bias_code = DTYPES[bias.dtype]
+    b = _vector(bias, "bias", device, None if bias is None else bias.dtype, out)
+    r = (0, 0) if residual is None else _matrix(residual, "residual", device, dt, rows, out)
+    a = _known(ACTS, act, "act")
+    y = torch.empty((rows, out), dtype=dt, device=device)
+    pre = torch.empty((rows, out), dtype=dt, device=device) if keep and a else None
+    need = _linear_scratch(device.index, code, layout, rows, width, out, xs, ws, xp % 16 == 0, wp % 16 == 0)
+    held, work = _scratch(need, device)
+    _call("wc_linear", _LINEAR.pack(
+        _LINEAR.size, device.index, code, bias_code, layout, rows, width, out, xp, xs, wp, ws, b, *r, a, 0,
+        0 if pre is None else pre.data_ptr(), out, y.data_ptr(), out, work, need), device)
+    return Linear(y, pre)
+
+
+def linear_backward(d_out, x, weight, pre=None, *, act="none", bias=False, d_x=True, d_weight=True, dtype=None):
+    """The gradients of linear from its inputs and its pre (wc_linear_backward); the residual's is d_out itself.
+
+    d_out [rows, out]; pre may be None where act is "none". bias, d_x, d_weight: which are wanted. dtype: the weight's
+    gradient's type, x's (the default) or float32. Returns LinearGrads(x, weight, bias): weight contiguous along the
+    index that the weight is, bias in float32, None for what is not wanted."""
+    device = _device(x, "x")
+    code, dt = _dtype(x, "x"), x.dtype
+    if x.dim() != 2:
+        _fail(f"x: shape {tuple(x.shape)}, expected rows x width")
+    if not isinstance(weight, torch.Tensor) or weight.dim() != 2:
+        _fail("weight: expected width x out")
+    rows, width = x.shape
+    out = weight.shape[1]
+    a = _known(ACTS, act, "act")
+    if a and pre is None:
+        _fail("pre is missing")
+    xp, xs = _matrix(x, "x", device, dt, rows, width)
+    wp, ws, layout = _weight_of(weight, "weight", device, dt, width, out)
+    dp, ds = _matrix(d_out, "d_out", device, dt, rows, out)
+    z = _matrix(pre, "pre", device, dt, rows, out) if a else (0, 0)
+    gx = torch.empty((rows, width), dtype=dt, device=device) if d_x else None
+    gw = None
+    if d_weight:
+        gw = torch.empty((out, width) if layout else (width, out), dtype=dtype or dt, device=device)
+        if gw.dtype not in (dt, torch.float32):
+            _fail(f"dtype: {gw.dtype}, expected {dt} or float32")
+    gb = torch.empty(out, dtype=torch.float32, device=device) if bias else None
+    need = _linear_back_scratch(device.index, code, layout, a, rows, width, out, ds, xs, ws, dp % 16 == 0, xp % 16 == 0,
+                                wp % 16 == 0, bool(d_x), bool(d_weight), bool(bias))
+    held, work = _scratch(need, device)
+    at = lambda t: 0 if t is None else t.data_ptr()  # noqa: E731
+    _call("wc_linear_backward", _LINEAR_BACK.pack(
+        _LINEAR_BACK.size, device.index, code, layout, a, DTYPES[gw.dtype] if d_weight else 0, 0, rows, width, out, dp,
+        ds, *z, xp, xs, wp, ws, at(gx), width, at(gw), width if layout else out, at(gb), work, need), device)
+    return LinearGrads(gx, gw.t() if d_weight and layout else gw, gb)
+
+
+# ------------------------------------------------------------------ updates
+
+NEWTON_SCHULZ = (3.4445, -4.7750, 2.0315)
+
+
+@functools.lru_cache(maxsize=4096)
+def _ortho_scratch(device, code, out_code, batch, rows, width):
+    p = 256
+    return _scratch_bytes("wc_orthogonalise_workspace", _ORTHO.pack(
+        _ORTHO.size, device, code, out_code, 1, batch, rows, width, p, width, rows * width, p, width, rows * width, 1.0,
+        0.0, 0.0, 0.0, 1.0, 0, 0, 0))
+
+
+def orthogonalise(update, *, steps=5, coefficients=NEWTON_SCHULZ, eps=1e-7, scale=1.0, dtype=None):
+    """update [rows, width] or [batch, rows, width] with its singular values brought towards 1, times scale
+    (wc_orthogonalise): X = update / (its Frobenius norm + eps), then `steps` times X = a X + (b A + c A A) X with
+    A = X X^T (or the transposed form) and (a, b, c) = coefficients. dtype: the result's, float32, float16 or bfloat16
+    (the default is the update's); a bfloat16 result takes a third of the others' products. Returns a contiguous tensor."""
+    device = _device(update, "update")
+    code = _dtype(update, "update")
+    if update.dim() not in (2, 3) or 0 in update.shape[-2:]:
+        _fail(f"update: shape {tuple(update.shape)}, expected rows x width or batch x rows x width")
+    three = update if update.dim() == 3 else update[None]
+    batch, rows, width = three.shape
+    s = three.stride()
+    if s[2] != 1 and width > 1:
+        _fail("update: columns must be contiguous")
+    if len(coefficients) != 3:
+        _fail("coefficients: three are expected")
+    out = torch.empty(update.shape, dtype=dtype or update.dtype, device=device)
+    out_code = _dtype(out, "dtype")
+    need = _ortho_scratch(device.index, code, out_code, batch, rows, width)
+    held, work = _scratch(need, device)
+    _call("wc_orthogonalise", _ORTHO.pack(
+        _ORTHO.size, device.index, code, out_code, steps, batch, rows, width, three.data_ptr(), s[1], s[0],
+        out.data_ptr(), width, rows * width, *coefficients, eps, scale, 0, work, need), device)
+    return out
+
+
+# -------------------------------------------------------- log-probabilities
+
+@functools.lru_cache(maxsize=4096)
+def _logp_scratch(device, code, rows, vocab, top):
+    p = 256
+    return _scratch_bytes("wc_token_logp_workspace", _LOGP.pack(
+        _LOGP.size, device, code, rows, vocab, p, vocab, 0, 0, 0, 1.0, 64, top, 0, p, p, p, p, p, 0, 0, 0))
+
+
+def token_logp(logits, tokens=None, *, legal=None, inv_temperature=1.0, top=0, stats=True):
+    """Log-probabilities of the rows' tokens, their rank, the entropy and the `top` likeliest columns (wc_token_logp).
+
+    logits [rows, vocab]; tokens [rows] int64 or int32, or None; legal [rows, vocab] bool. A row whose token is out of
+    range, or without a legal logit above -infinity, is left out. Returns TokenLogp(logp, entropy, rank, top_logp,
+    top_index, stats): rank int32, how many columns come before the token (0: the likeliest, -1: left out); top_logp
+    and top_index [rows, top] (int32, -1 where there are no more), None for top=0; logp and rank None without tokens;
+    stats [rows, 4] is what token_logp_backward needs (stats=False: not kept)."""
+    device, code, rows, vocab, (x, xs) = _logits(logits)
+    f32, i32 = torch.float32, torch.int32
+    t, bits = (0, 64) if tokens is None else _indices(tokens, "tokens", device, rows)
+    lg, lgs = (0, 0) if legal is None else _matrix(legal, "legal", device, torch.bool, rows, vocab)
+    if not isinstance(top, int) or not 0 <= top <= TOP_MAX:
+        _fail(f"top: {top!r} is not 0 to {TOP_MAX}")
+    entropy = torch.empty(rows, dtype=f32, device=device)
+    logp = rank = top_logp = top_index = st = None
+    if tokens is not None:
+        logp = torch.empty(rows, dtype=f32, device=device)
+        rank = torch.empty(rows, dtype=i32, device=device)
+    if top:
+        top_logp = torch.empty((rows, top), dtype=f32, device=device)
+        top_index = torch.empty((rows, top), dtype=i32, device=device)
+    if stats:
+        st = torch.empty((rows, 4), dtype=f32, device=device)
+    need = _logp_scratch(device.index, code, rows, vocab, top)
+    held, work = _scratch(need, device)
+    at = lambda v: 0 if v is None else v.data_ptr()  # noqa: E731
+    _call("wc_token_logp", _LOGP.pack(
+        _LOGP.size, device.index, code, rows, vocab, x, xs, lg, lgs, t, inv_temperature, bits, top, 0, at(logp),
+        entropy.data_ptr(), at(rank), at(top_logp), at(top_index), at(st), work, need), device)
+    return TokenLogp(logp, entropy, rank, top_logp, top_index, st)
+
+
+def token_logp_backward(d_logp, d_entropy, logits, tokens, stats, *, legal=None, inv_temperature=1.0, grad=None):
+    """The gradient at the logits from what arrives at token_logp's logp and entropy ([rows] float32, either may be
+    None: 0), from the forward's inputs and its stats (wc_token_logp_backward). grad: a tensor like logits to write to
+    (logits itself works)."""
+    device, code, rows, vocab, (x, xs) = _logits(logits)
+    t, bits = (0, 64) if tokens is None else _indices(tokens, "tokens", device, rows)
+    lg, lgs = (0, 0) if legal is None else _matrix(legal, "legal", device, torch.bool, rows, vocab)
+    if stats is None:
+        _fail("stats is missing")
+    st, _ = _matrix(stats, "stats", device, torch.float32, rows, 4)
+    if rows > 1 and stats.stride(0) != 4:
+        _fail("stats must be contiguous")
+    if grad is None:
+        grad = _like(logits)
+    g, gs = _matrix(grad, "grad", device, logits.dtype, rows, vocab)
+    f32 = torch.float32
+    _call("wc_token_logp_backward", _LOGP_BACK.pack(
+        _LOGP_BACK.size, device.index, code, rows, vocab, x, xs, lg, lgs, t, inv_temperature, bits, st,
+        _vector(d_logp, "d_logp", device, f32, rows), _vector(d_entropy, "d_entropy", device, f32, rows), g, gs), device)
+    return grad
+
+
 # ------------------------------------------------------- automatic differentiation
 
 class _First(torch.autograd.Function):
@@ -603,3 +834,114 @@ def act_linear8(z, weight, act="gelu"):
     act(z) not at all: its slope and the weight's gradient are taken from the 8-bit form. In float32 with gelu or silu the
     backward pass makes act(kept) in float32 for the weight's gradient (rows x width x 4 bytes while it runs)."""
     return _ActLinear8.apply(z, weight, act)[0]
+
+
+class _Dense(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, residual, act):
+        r = linear(x, weight, bias, act=act, residual=residual, keep=any(ctx.needs_input_grad))
+        ctx.save_for_backward(x, weight, bias, r.pre)
+        ctx.act = act
+        return r.out
+
+    @staticmethod
+    @_first_only
+    def backward(ctx, d):
+        x, weight, bias, pre = ctx.saved_tensors
+        need = ctx.needs_input_grad
+        d_bias = None
+        g = LinearGrads(None, None, None)
+        if any(need[:3]):
+            g = linear_backward(d.contiguous(), x, weight, pre, act=ctx.act, bias=need[2], d_x=need[0], d_weight=need[1])
+            d_bias = g.bias.to(bias.dtype) if need[2] else None
+        return g.x, g.weight, d_bias, d if need[3] else None, None
+
+
+def dense(x, weight, bias=None, *, act="none", residual=None):
+    """linear as a differentiable function of x, the weight, the bias and the residual."""
+    return _Dense.apply(x, weight, bias, residual, act)
+
+
+class Dense(torch.nn.Module):
+    """A layer with its parameters: act(x @ weight + bias) + residual. The products are taken in x's type: parameters of
+    another are cast for them."""
+
+    def __init__(self, width, out, bias=True, act="none", gain=1.0, device=None, dtype=torch.float32):
+        super().__init__()
+        w = torch.randn(width, out, device=device, dtype=torch.float32) * gain * width ** -0.5
+        self.weight = torch.nn.Parameter(w.to(dtype))
+        self.bias = torch.nn.Parameter(torch.zeros(out, device=device, dtype=dtype)) if bias else None
+        self.act = act
+
+    def forward(self, x, residual=None):
+        b = self.bias
+        if b is not None and b.dtype is not torch.float32:
+            b = b.to(x.dtype)
+        return dense(x, self.weight.to(x.dtype), b, act=self.act, residual=residual)
+
+
+class _TokenLogp(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, tokens, legal, kw):
+        r = token_logp(logits, tokens, legal=legal, **kw)
+        ctx.save_for_backward(logits, tokens, legal, r.stats)
+        ctx.kw = kw
+        ctx.set_materialize_grads(False)
+        ctx.mark_non_differentiable(*(t for t in (r.rank, r.top_logp, r.top_index) if t is not None))
+        return r.logp, r.entropy, r.rank, r.top_logp, r.top_index
+
+    @staticmethod
+    @_first_only
+    def backward(ctx, d_logp, d_entropy, *_):
+        logits, tokens, legal, stats = ctx.saved_tensors
+        one = [None if d is None else _upstream(d).contiguous() for d in (d_logp, d_entropy)]
+        grad = token_logp_backward(*one, logits, tokens, stats, legal=legal, inv_temperature=ctx.kw["inv_temperature"])
+        return grad, None, None, None
+
+
+def token_logp_objective(logits, tokens, *, legal=None, inv_temperature=1.0, top=0):
+    """token_logp whose logp and entropy are differentiable functions of the logits: (logp, entropy, rank, top_logp,
+    top_index), the last three without gradients. The backward pass reads the logits again."""
+    return _TokenLogp.apply(logits, tokens, legal, {"inv_temperature": inv_temperature, "top": top})
+
+
+class Muon(torch.optim.Optimizer):
+    """Momentum whose update's singular values are brought towards 1 (orthogonalise), for weights of two dimensions, or
+    three (a stack of them). Weights of one shape and type are updated together. The step is lr max(1, out / in)^(1/2)
+    for a weight [in, out]; weight_decay is decoupled. dtype: the type that the update is computed to."""
+
+    def __init__(self, params, lr=0.02, momentum=0.95, nesterov=True, weight_decay=0.0, steps=5, dtype=torch.bfloat16):
+        super().__init__(params, {"lr": lr, "momentum": momentum, "nesterov": nesterov, "weight_decay": weight_decay,
+                                  "steps": steps, "dtype": dtype})
+        for group in self.param_groups:
+            for p in group["params"]:
+                if p.dim() not in (2, 3):
+                    _fail(f"a weight of shape {tuple(p.shape)}: two or three dimensions are expected")
+
+    @torch.no_grad()
+    def step(self, closure=None):
+        loss = None
+        if closure is not None:
+            with torch.enable_grad():
+                loss = closure()
+        for group in self.param_groups:
+            same = {}
+            for p in group["params"]:
+                if p.grad is None:
+                    continue
+                state = self.state[p]
+                if "momentum" not in state:
+                    state["momentum"] = torch.zeros_like(p)
+                held = state["momentum"]
+                held.mul_(group["momentum"]).add_(p.grad)
+                update = p.grad.add(held, alpha=group["momentum"]) if group["nesterov"] else held
+                same.setdefault((p.shape, p.dtype, p.device), []).append((p, update))
+            for (shape, _, _), pairs in same.items():
+                updates = torch.stack([u for _, u in pairs]) if len(pairs) > 1 else pairs[0][1].contiguous()
+                each = orthogonalise(updates.reshape(-1, *shape[-2:]), steps=group["steps"], dtype=group["dtype"],
+                                     scale=max(1.0, shape[-1] / shape[-2]) ** 0.5)
+                for (p, _), o in zip(pairs, each.reshape(len(pairs), *shape).unbind(0)):
+                    if group["weight_decay"]:
+                        p.mul_(1 - group["lr"] * group["weight_decay"])
+                    p.add_(o, alpha=-group["lr"])
+        return loss
