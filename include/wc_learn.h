@@ -278,7 +278,7 @@ int wc_ckpt_weight_grad(const wc_ckpt_weight_args* a, void* stream);
  * y = act(x W + bias) + residual, one product with its epilogue: sums, bias,
  * activation and residual in float32, rounded once to y's type. W is width x
  * out (WC_WEIGHT_IN_OUT) or out x width (WC_WEIGHT_OUT_IN, a row an output).
- * pre, where given, gets x W + bias rounded to its type, for the backward pass.
+ * pre, where given, gets x W + bias in float32, for the backward pass.
  * 16-bit matrices: products on the matrix cores with float32 sums. float32: as
  * three bf16 parts an element and six products of parts (what is left out is
  * below 2^-25 of a product); an infinite element's row or column of the result is not finite,
@@ -299,7 +299,7 @@ typedef struct wc_linear_args {
     const void* residual;       /* rows x out; NULL: 0 */
     int64_t residual_stride;
     int32_t act, pad;           /* WC_ACT_* */
-    void* pre;                  /* rows x out; NULL: not kept */
+    float* pre;                 /* rows x out; NULL: not kept */
     int64_t pre_stride;
     void* y;                    /* rows x out; may be residual itself */
     int64_t y_stride;
@@ -321,7 +321,7 @@ typedef struct wc_linear_back_args {
     int64_t rows, width, out;
     const void* d_out;          /* rows x out */
     int64_t d_out_stride;
-    const void* pre;            /* rows x out; with WC_ACT_NONE not read */
+    const float* pre;           /* rows x out; with WC_ACT_NONE not read */
     int64_t pre_stride;
     const void* x;              /* read for d_weight */
     int64_t x_stride;

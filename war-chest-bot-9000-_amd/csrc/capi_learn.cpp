@@ -255,7 +255,7 @@ void check(const wc_linear_args& a, Check* c) {
     check_weight(a, a.weight, n, a.weight_stride, false, need, "weight", c);
     c->buffer(a.bias, known(a.bias_dtype) ? size_of(a.bias_dtype) : 4, false, "bias");
     c->matrix(a.residual, n, a.residual_stride, a.out, a.rows, false, false, "residual");
-    c->matrix(a.pre, n, a.pre_stride, a.out, a.rows, true, false, "pre");
+    c->matrix(a.pre, 4, a.pre_stride, a.out, a.rows, true, false, "pre");
     c->matrix(a.y, n, a.y_stride, a.out, a.rows, true, need, "y");
 }
 
@@ -265,7 +265,7 @@ void check(const wc_linear_back_args& a, Check* c) {
     const bool need = a.rows > 0;
     c->is(a.grad_dtype == WC_DTYPE_F32 || a.grad_dtype == a.dtype, "grad_dtype is float32 or the matrices'");
     c->matrix(a.d_out, n, a.d_out_stride, a.out, a.rows, false, need, "d_out");
-    if (a.act != WC_ACT_NONE) c->matrix(a.pre, n, a.pre_stride, a.out, a.rows, false, need, "pre");
+    if (a.act != WC_ACT_NONE) c->matrix(a.pre, 4, a.pre_stride, a.out, a.rows, false, need, "pre");
     if (a.d_weight) {
         c->matrix(a.x, n, a.x_stride, a.width, a.rows, false, need, "x");
         check_weight(a, a.d_weight, known(a.grad_dtype) ? size_of(a.grad_dtype) : 4, a.d_weight_stride, true, true,

@@ -6,7 +6,8 @@
 // The three products differ in which index of each operand is summed; one kernel takes all (product_dev.h). Sums, bias,
 // activation and residual are float32 and rounded once, to the output's type. d_pre is rounded to the 16-bit type for
 // its two products (as it would be between two operators): its own half ulp, 2^-9 of an element in bf16, against the
-// same for every element of the result. The kept pre-activations are rounded to the matrices' type.
+// same for every element of the result. Pre-activations are kept in float32: in 16 bits their rounding would be 10^4 times
+// that of the float32 sums of d_b (1.3e-3 of its norm in bf16).
 //
 // float32 operands are taken as three bf16 parts (8 + 8 + 8 bits), and of their nine products the six that matter:
 // the matrix cores' own float32 rate is a sixteenth of the 16-bit one.
@@ -127,7 +128,7 @@ struct LayerEpilogue {
     bool bias_f32;
     const T* residual;
     int64_t residual_stride;
-    T* pre;
+    float* pre;
     int64_t pre_stride;
     T* y;
     int64_t y_stride;
@@ -242,7 +243,7 @@ void linear(const wc_linear_args& a, int cus, hipStream_t s) {
     m.b = operand<T>(p.w, a.weight, w, a.out);
     m.k = p.k;
     const LayerEpilogue<T> e = {a.bias, a.bias_dtype == WC_DTYPE_F32, (const T*)a.residual, a.residual_stride,
-                                (T*)a.pre, a.pre_stride, (T*)a.y, a.y_stride, a.act};
+                                (float*)a.pre, a.pre_stride, (T*)a.y, a.y_stride, a.act};
     multiply<T>(m, p.cut, true, !io, (float*)(w + p.part), e, s);
 }
 
@@ -263,7 +264,7 @@ __global__ __launch_bounds__(256) void k_slope(wc_linear_back_args a, Source d, 
             load_n((const T*)a.d_out + r * a.d_out_stride + c, have, 0.f, v);
             if (a.act != WC_ACT_NONE) {
                 float z[8];
-                load_n((const T*)a.pre + r * a.pre_stride + c, have, 0.f, z);
+                load_n((const float*)a.pre + r * a.pre_stride + c, have, 0.f, z);
                 act_slopes(z, a.act);
 #pragma unroll
                 for (int u = 0; u < 8; u++) v[u] = u < have ? v[u] * z[u] : 0.f;

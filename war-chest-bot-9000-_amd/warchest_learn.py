@@ -512,7 +512,7 @@ def linear(x, weight, bias=None, *, act="none", residual=None, keep=False):
 
     x [rows, width], weight [width, out] (contiguous along either index: the transposed view of an [out, width] matrix
     works as it is), bias [out] in their type or float32, residual [rows, out]. act: "none", "relu", "gelu" or "silu".
-    Returns Linear(out, pre): pre [rows, out], x @ weight + bias, is what linear_backward needs; None unless keep is
+    Returns Linear(out, pre): pre [rows, out] float32, x @ weight + bias, is what linear_backward needs; None unless keep is
     true and act is not "none"."""
     device = _device(x, "x")
     code, dt = _dtype(x, "x"), x.dtype
@@ -533,7 +533,7 @@ def linear(x, weight, bias=None, *, act="none", residual=None, keep=False):
     r = (0, 0) if residual is None else _matrix(residual, "residual", device, dt, rows, out)
     a = _known(ACTS, act, "act")
     y = torch.empty((rows, out), dtype=dt, device=device)
-    pre = torch.empty((rows, out), dtype=dt, device=device) if keep and a else None
+    pre = torch.empty((rows, out), dtype=torch.float32, device=device) if keep and a else None
     need = _linear_scratch(device.index, code, layout, rows, width, out, xs, ws, xp % 16 == 0, wp % 16 == 0)
     held, work = _scratch(need, device)
     _call("wc_linear", _LINEAR.pack(
@@ -562,7 +562,7 @@ def linear_backward(d_out, x, weight, pre=None, *, act="none", bias=False, d_x=T
     xp, xs = _matrix(x, "x", device, dt, rows, width)
     wp, ws, layout = _weight_of(weight, "weight", device, dt, width, out)
     dp, ds = _matrix(d_out, "d_out", device, dt, rows, out)
-    z = _matrix(pre, "pre", device, dt, rows, out) if a else (0, 0)
+    z = _matrix(pre, "pre", device, torch.float32, rows, out) if a else (0, 0)
     gx = torch.empty((rows, width), dtype=dt, device=device) if d_x else None
     gw = None
     if d_weight:
