@@ -288,17 +288,27 @@ __global__ __launch_bounds__(256) void k_slope(wc_linear_back_args a, Source d, 
     sums[int64_t(blockIdx.y) * a.out + j] = s;
 }
 
-// The row blocks' column sums added in order.
+// The row blocks' column sums added in order: a sixteenth of them each group of sixteen threads.
 static __global__ __launch_bounds__(256) void k_slope_sum(const float* sums, int64_t out, int blocks, float* to) {
-    __shared__ float four[4][64];
-    const int64_t j = int64_t(blockIdx.x) * 64 + threadIdx.x % 64;
-    const int q = threadIdx.x / 64;
+    __shared__ float some[16][17];
+    const int64_t j = int64_t(blockIdx.x) * 16 + threadIdx.x % 16;
+    const int q = threadIdx.x / 16;
     float s = 0.f;
-    if (j < out)
-        for (int k = q; k < blocks; k += 4) s += sums[k * out + j];
-    four[q][threadIdx.x % 64] = s;
+    if (j < out) {
+        int k = q;
+        for (; k + 48 < blocks; k += 64) {
+            float v[4];
+#pragma unroll
+            for (int u = 0; u < 4; u++) v[u] = sums[(k + 16 * u) * out + j];
+            s += (v[0] + v[1]) + (v[2] + v[3]);
+        }
+        for (; k < blocks; k += 16) s += sums[k * out + j];
+    }
+    some[q][threadIdx.x % 16] = s;
     __syncthreads();
-    if (!q && j < out) to[j] = (s + four[1][threadIdx.x]) + (four[2][threadIdx.x] + four[3][threadIdx.x]);
+    if (q || j >= out) return;
+    for (int u = 1; u < 16; u++) s += some[u][threadIdx.x];
+    to[j] = s;
 }
 
 struct LinearBackPlan {
@@ -384,7 +394,7 @@ void linear_back(const wc_linear_back_args& a, int cus, hipStream_t s) {
         float* sums = a.d_bias ? (float*)(w + p.sums) : nullptr;
         const int64_t across = ((d.to ? p.d.cols : a.out) + 255) / 256;
         k_slope<T><<<dim3((uint32_t)across, (uint32_t)p.blocks), 256, 0, s>>>(a, d, p.per, sums);
-        if (sums) k_slope_sum<<<dim3((uint32_t)((a.out + 63) / 64)), 256, 0, s>>>(sums, a.out, p.blocks, a.d_bias);
+        if (sums) k_slope_sum<<<dim3((uint32_t)((a.out + 15) / 16)), 256, 0, s>>>(sums, a.out, p.blocks, a.d_bias);
     }
     if (!products) return;
     // copies of x and the weight, in one launch

@@ -23,7 +23,7 @@ namespace learn {
 namespace {
 
 constexpr float HELD = 1024.f;
-constexpr int SUM_BLOCKS = 128;
+constexpr int SUM_BLOCKS = 1024;
 
 // Where X, A or B lies: planes of rows of whole chunks of eight, zeros behind a row's end.
 struct Held16 {

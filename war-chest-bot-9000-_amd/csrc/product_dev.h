@@ -1,11 +1,12 @@
 // Matrix products on the matrix cores, C[m x n] = sum over k of A[i][k] B[k][j], with an epilogue that the caller gives:
-// the layers' products (linear.hip) and the Newton-Schulz steps (newton.hip).
+// the layers' products (linear_dev.h) and the Newton-Schulz steps (newton.hip).
 //
 // An operand's index of summation is its contiguous one (INNER: A as rows of k, B as rows of k for each column) or its
-// outer one. Tiles go from memory to LDS without passing registers, four buffers of 32 values of k, three of them in
-// flight. INNER tiles come back as 16 bytes a lane, the others through the transposing LDS read. A workgroup of four
-// wavefronts owns a square tile of 64 F, each wavefront a quarter in F x F fragments of 32 x 32. Everything else goes
-// between the matrix instructions: F of them, then the loads and the reads of one part.
+// outer one. Tiles of 64 values of k go from memory to LDS without passing registers: A in three buffers and B in two,
+// so that a step's loads have at least a step to arrive and one barrier a step is enough; whole lines of 128 bytes of an
+// INNER operand. INNER tiles come back as 16 bytes a lane, the others through the transposing LDS read. A workgroup of
+// four wavefronts owns a square tile of 64 F, each wavefront a quarter in F x F fragments of 32 x 32. Everything else
+// goes between the matrix instructions: F of them, then the loads and the reads of one part.
 //
 // An operand may have several planes that add up to it; the product is then a sum of segments, pairs of planes, one
 // after the other along k.
@@ -24,7 +25,7 @@ namespace wc {
 namespace learn {
 namespace {
 
-constexpr int PRODUCT_BLOCK = 256, STEP = 32, STEP_BUFFERS = 4;
+constexpr int PRODUCT_BLOCK = 256, STEP = 64, A_BUFFERS = 3, B_BUFFERS = 2;
 constexpr int MOST_SEGMENTS = 6, MOST_PLANES = 3;
 
 typedef f16 f16x8 __attribute__((ext_vector_type(8)));
@@ -61,66 +62,83 @@ struct Product {
 
 static __device__ __align__(16) uint4 g_zeros;  // what lies past the end is read from here
 
-// Where a step's tiles are, the same for all lanes.
-struct Cursor {
-    const char *a, *b;
-    int segment, left;  // steps left in the segment
-};
-
 template <int F>
 struct TileShape {
-    static constexpr int TILE = 64 * F, SIDE = TILE * 2 * STEP, BUFFER = 2 * SIDE;
-    static constexpr int LDS = STEP_BUFFERS * BUFFER;
-    // where rows are on k: 64-byte units a row, exchanged so that the four rows of a transposing read lie in different
-    // banks. A pitch of 128 bytes puts rows 0 and 1 there by itself.
-    static __device__ __forceinline__ int turn(int row) { return F == 1 ? (row >> 1) & 1 : row & 3; }
+    static constexpr int TILE = 64 * F, SIDE = TILE * 2 * STEP;
+    static constexpr int LDS = (A_BUFFERS + B_BUFFERS) * SIDE;
+    static constexpr int PARTS = 2 * F;  // a wavefront's loads of one operand's tile
+    // Where rows are on k: 64-byte units a row, exchanged so that the four rows of a transposing read lie in different
+    // banks. A pitch of an odd number of 128 bytes puts rows 0 and 1 there by itself.
+    static __device__ __forceinline__ int turn(int row) { return F & 1 ? (row >> 1) & 1 : row & 3; }
 };
 
-// A wavefront's loads of one operand: F of 64 lanes x 16 bytes each, to places in LDS that follow each other.
+// One operand's way from memory to LDS, as one wavefront has it: PARTS loads a step of 64 lanes x 16 bytes each, to
+// places in LDS that follow each other.
 template <int F, bool INNER>
-struct Loads {
-    uint32_t at[F];  // the lane's place, from the tile's first row
-    int32_t k[F];    // the first of k that it brings
+struct Fetch {
+    typedef TileShape<F> S;
+    uint32_t at[S::PARTS];  // the lane's place, from the tile's first row
+    int first;              // the wavefront's first load and the lane, of the tile's 16-byte chunks
+    const char* p;          // the tile of the step to load, the same for all lanes
+    int64_t step, start;    // bytes from step to step, and from a plane's start to the tile's
+    int segment, left;      // of the segment: steps left
 
-    __device__ __forceinline__ void set(const Operand16& o, int64_t first, int wave, int lane) {
-        typedef TileShape<F> S;
+    __device__ __forceinline__ void set(const Product& q, const Operand16& o, const uint8_t* planes, int batch, int64_t at0,
+                                        int wave, int lane, int s, int steps_in) {
+        first = wave * S::PARTS * 64 + lane;
 #pragma unroll
-        for (int q = 0; q < F; q++) {
-            const int g = (wave * F + q) * 64 + lane;
+        for (int k = 0; k < S::PARTS; k++) {
+            const int g = first + 64 * k;
             if (INNER) {
-                const int row = g / 4, chunk = (g % 4) ^ (row >> 1 & 3);
+                const int row = g / 8, chunk = (g % 8) ^ (row & 7);
                 // past the last row any row will do: its products are not stored
-                const int64_t r = min(first + row, o.outer - 1) - first;
-                at[q] = (uint32_t)(r * o.pitch) + 16 * chunk;
-                k[q] = 8 * chunk;
+                const int64_t r = min(at0 + row, o.outer - 1) - at0;
+                at[k] = (uint32_t)(r * o.pitch) + 16 * chunk;
             } else {
-                const int row = g / (S::TILE / 8), chunk = (g % (S::TILE / 8)) ^ (S::turn(row) << 2);
-                at[q] = (uint32_t)(row * o.pitch) + (first + 8 * chunk < o.outer ? 16 * chunk : 0);
-                k[q] = row;
+                const int row = g / (8 * F), chunk = (g % (8 * F)) ^ (S::turn(row) << 2);
+                at[k] = (uint32_t)(row * o.pitch) + (at0 + 8 * chunk < o.outer ? 16 * chunk : 0);
             }
         }
+        step = INNER ? 2 * STEP : STEP * o.pitch;
+        start = batch * o.batch + (INNER ? at0 * o.pitch : 2 * at0);
+        segment = q.segments > 1 ? s / steps_in : 0;
+        const int in = s - segment * steps_in;
+        left = steps_in - in;
+        p = o.plane[planes[segment]] + start + in * step;
     }
-    // ENDS: what lies at or past `left` of k is read from zeros.
+    __device__ __forceinline__ void next(const Product& q, const Operand16& o, const uint8_t* planes, int steps_in) {
+        p += step;
+        if (--left == 0 && segment + 1 < q.segments) {
+            segment++;
+            left = steps_in;
+            p = o.plane[planes[segment]] + start;
+        }
+    }
+    // The first of k that load k brings.
+    __device__ __forceinline__ int k_of(int k) const {
+        const int g = first + 64 * k;
+        return INNER ? 8 * ((g % 8) ^ (g / 8 & 7)) : g / (8 * F);
+    }
+    // Load k of the step, to the wavefront's place. ENDS: what lies at or past `there` of the step's k is read from zeros.
     template <bool ENDS>
-    __device__ __forceinline__ void load(const char* base, int q, int64_t left, LdsAt to) const {
-        const char* from = base + at[q];
-        if (ENDS && k[q] >= left) from = (const char*)&g_zeros;
+    __device__ __forceinline__ void load(int k, int64_t there, LdsAt to) const {
+        const char* from = p + at[k];
+        if (ENDS && k_of(k) >= there) from = (const char*)&g_zeros;
         __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)from,
-                                         (__attribute__((address_space(3))) void*)(to + 1024 * q), 16, 0, 0);
+                                         (__attribute__((address_space(3))) void*)(to + 1024 * k), 16, 0, 0);
     }
 };
 
 // A wavefront's reads of one operand's fragments: lane l has eight of k, from 8 (l / 32) on, of row or column l % 32.
 template <int F, bool INNER>
 struct Reads {
-    uint32_t at[INNER ? 2 : F];
+    typedef TileShape<F> S;
+    uint32_t at[INNER ? 1 : F];
 
     __device__ __forceinline__ void set(int first, int lane) {
-        typedef TileShape<F> S;
         if (INNER) {
             const int row = first + (lane & 31);
-#pragma unroll
-            for (int h = 0; h < 2; h++) at[h] = row * 64 + 16 * ((2 * h + (lane >> 5)) ^ (row >> 1 & 3));
+            at[0] = row * 2 * STEP + 16 * ((lane >> 5) ^ (row & 7));
         } else {
             const int row = 8 * (lane >> 5) + ((lane & 15) >> 2);
 #pragma unroll
@@ -129,15 +147,15 @@ struct Reads {
                         ((2 * (first + 32 * m + (lane & 16) + 4 * (lane & 3))) ^ (S::turn(row) << 6));
         }
     }
+    // Fragment m of the sixteen of k from 16 part on.
     template <class E8>
-    __device__ __forceinline__ E8 take(LdsAt from, int half, int m) const {
-        typedef TileShape<F> S;
+    __device__ __forceinline__ E8 take(LdsAt from, int part, int m) const {
         if constexpr (INNER) {
             typedef __attribute__((address_space(3))) E8* At;
-            return *(At)(from + at[half] + m * 32 * 64);
+            return *(At)(from + (at[0] ^ (part << 5)) + m * 32 * 2 * STEP);
         } else {
             typedef __attribute__((address_space(3))) s16x4* At;
-            const LdsAt p = from + at[m] + half * 16 * 2 * S::TILE;
+            const LdsAt p = from + at[m] + part * 16 * 2 * S::TILE;
             // four rows on, the exchange of units is the same
             const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((At)p);
             const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((At)(p + 4 * 2 * S::TILE));
@@ -146,13 +164,14 @@ struct Reads {
     }
 };
 
-// Of the loads of three buffers the first third has arrived when the others are left.
+// All loads but the last LEFT have arrived, in every wavefront, and every wavefront's reads.
 template <int LEFT>
 __device__ __forceinline__ void arrived() {
-    static_assert(LEFT == 4 || LEFT == 8 || LEFT == 16, "two steps' loads");
-    if constexpr (LEFT == 4) asm volatile("s_waitcnt vmcnt(4) lgkmcnt(0)" ::: "memory");
-    else if constexpr (LEFT == 8) asm volatile("s_waitcnt vmcnt(8) lgkmcnt(0)" ::: "memory");
-    else asm volatile("s_waitcnt vmcnt(16) lgkmcnt(0)" ::: "memory");
+    static_assert(LEFT == 2 || LEFT == 4 || LEFT == 6 || LEFT == 8, "a step's loads of A");
+    if constexpr (LEFT == 2) asm volatile("s_waitcnt vmcnt(2) lgkmcnt(0)" ::: "memory");
+    else if constexpr (LEFT == 4) asm volatile("s_waitcnt vmcnt(4) lgkmcnt(0)" ::: "memory");
+    else if constexpr (LEFT == 6) asm volatile("s_waitcnt vmcnt(6) lgkmcnt(0)" ::: "memory");
+    else asm volatile("s_waitcnt vmcnt(8) lgkmcnt(0)" ::: "memory");
     __builtin_amdgcn_s_barrier();
 }
 
@@ -160,107 +179,108 @@ template <class E, int F, bool AI, bool BI>
 struct Tiles {
     typedef E E8 __attribute__((ext_vector_type(8)));
     typedef TileShape<F> S;
-    const Product& p;
-    Loads<F, AI> la;
-    Loads<F, BI> lb;
+    const Product& q;
+    Fetch<F, AI> fa;
+    Fetch<F, BI> fb;
     Reads<F, AI> ra;
     Reads<F, BI> rb;
-    Cursor c;
-    int64_t a0, b0;  // bytes from a plane's start to the tile's
-    int steps_in;    // of a segment
+    int steps_in;  // of a segment
 
-    __device__ __forceinline__ Tiles(const Product& product, int batch, int64_t i0, int64_t j0, int wave, int lane)
-        : p(product) {
-        la.set(p.a, i0, wave, lane);
-        lb.set(p.b, j0, wave, lane);
+    __device__ __forceinline__ Tiles(const Product& product, int batch, int64_t i0, int64_t j0, int wave, int lane, int s)
+        : q(product) {
+        steps_in = (int)((q.k + STEP - 1) / STEP);
+        fa.set(q, q.a, q.pa, batch, i0, wave, lane, s, steps_in);
+        fb.set(q, q.b, q.pb, batch, j0, wave, lane, s, steps_in);
         ra.set((wave >> 1) * 32 * F, lane);
         rb.set((wave & 1) * 32 * F, lane);
-        a0 = batch * p.a.batch + (AI ? i0 * p.a.pitch : 2 * i0);
-        b0 = batch * p.b.batch + (BI ? j0 * p.b.pitch : 2 * j0);
-        steps_in = (int)((p.k + STEP - 1) / STEP);
     }
-    __device__ __forceinline__ int64_t a_step() const { return AI ? 2 * STEP : STEP * p.a.pitch; }
-    __device__ __forceinline__ int64_t b_step() const { return BI ? 2 * STEP : STEP * p.b.pitch; }
-    __device__ __forceinline__ void seek(int s) {
-        c.segment = p.segments > 1 ? s / steps_in : 0;
-        const int in = s - c.segment * steps_in;
-        c.left = steps_in - in;
-        c.a = p.a.plane[p.pa[c.segment]] + a0 + in * a_step();
-        c.b = p.b.plane[p.pb[c.segment]] + b0 + in * b_step();
-    }
-    __device__ __forceinline__ void next() {
-        c.a += a_step();
-        c.b += b_step();
-        if (--c.left == 0 && c.segment + 1 < p.segments) {
-            c.segment++;
-            c.left = steps_in;
-            c.a = p.a.plane[p.pa[c.segment]] + a0;
-            c.b = p.b.plane[p.pb[c.segment]] + b0;
-        }
-    }
-    // One part of a step's loads. left: what of k is there from the cursor on.
-    template <bool ENDS>
-    __device__ __forceinline__ void load(int q, int64_t left, LdsAt to) const {
-        la.template load<ENDS>(c.a, q, left, to);
-        lb.template load<ENDS>(c.b, q, left, to + S::SIDE);
+    __device__ __forceinline__ void next_a() { fa.next(q, q.a, q.pa, steps_in); }
+    __device__ __forceinline__ void next_b() { fb.next(q, q.b, q.pb, steps_in); }
+    // What of k is there at an operand's step.
+    template <class Side>
+    __device__ __forceinline__ int64_t there(const Side& f, bool any) const {
+        return any ? q.k - int64_t(steps_in - f.left) * STEP : 0;
     }
 
-    // One step: the buffer `from`, whose first fragments are in fa and fb, and the first of `next`; the loads of three
-    // steps on go to `to`. The three are different buffers: told so, the compiler lets reads pass loads in flight.
+    // One step: the tiles a and b, whose first fragments are in xa and xb; B's next tile is loaded to to_b, A's after next
+    // to to_a, and the first fragments of the next step's tiles are read from na and nb once they have arrived. They are
+    // different buffers: told so, the compiler lets reads pass loads in flight.
     template <bool ENDS>
-    __device__ __forceinline__ void step(LdsAt __restrict__ from, LdsAt __restrict__ following, LdsAt __restrict__ to,
-                                         int64_t left, E8 (&fa)[F], E8 (&fb)[F], f32x16 (&acc)[F][F]) {
-        E8 na[F], nb[F];
+    __device__ __forceinline__ void step(LdsAt __restrict__ a, LdsAt __restrict__ b, LdsAt __restrict__ na,
+                                         LdsAt __restrict__ nb, LdsAt __restrict__ to_a, LdsAt __restrict__ to_b,
+                                         int64_t there_a, int64_t there_b, E8 (&xa)[F], E8 (&xb)[F], f32x16 (&acc)[F][F]) {
+        E8 ya[F], yb[F];
 #pragma unroll
-        for (int m = 0; m < F; m++) {
-            load<ENDS>(m, left, to);
-            na[m] = ra.template take<E8>(from, 1, m);
-            nb[m] = rb.template take<E8>(from + S::SIDE, 1, m);
+        for (int part = 0; part < 4; part++) {
+            E8(&ca)[F] = part & 1 ? ya : xa;
+            E8(&cb)[F] = part & 1 ? yb : xb;
+            E8(&da)[F] = part & 1 ? xa : ya;
+            E8(&db)[F] = part & 1 ? xb : yb;
 #pragma unroll
-            for (int n = 0; n < F; n++) acc[m][n] = mfma(fa[m], fb[n], acc[m][n]);
-            __builtin_amdgcn_sched_barrier(0);
+            for (int m = 0; m < F; m++) {
+                if (part == 0) {
+                    fb.template load<ENDS>(2 * m, there_b, to_b);
+                    fb.template load<ENDS>(2 * m + 1, there_b, to_b);
+                } else if (part < 3) {
+                    fa.template load<ENDS>((part - 1) * F + m, there_a, to_a);
+                }
+                if (part < 3) {
+                    da[m] = ra.template take<E8>(a, part + 1, m);
+                    db[m] = rb.template take<E8>(b, part + 1, m);
+                }
+#pragma unroll
+                for (int n = 0; n < F; n++) acc[m][n] = mfma(ca[m], cb[n], acc[m][n]);
+                __builtin_amdgcn_sched_barrier(0);
+                if (part == 3) {
+                    if (m == 0) arrived<S::PARTS>();
+                    da[m] = ra.template take<E8>(na, 0, m);
+                    db[m] = rb.template take<E8>(nb, 0, m);
+                }
+            }
         }
-        next();
-        E8 oa[F], ob[F];
-#pragma unroll
-        for (int m = 0; m < F; m++) {
-#pragma unroll
-            for (int n = 0; n < F; n++) acc[m][n] = mfma(na[m], nb[n], acc[m][n]);
-            __builtin_amdgcn_sched_barrier(0);
-            if (m == 0) arrived<4 * F>();  // the next buffer's, and every wavefront has read this one's
-            oa[m] = ra.template take<E8>(following, 0, m);
-            ob[m] = rb.template take<E8>(following + S::SIDE, 0, m);
-        }
-#pragma unroll
-        for (int m = 0; m < F; m++) fa[m] = oa[m], fb[m] = ob[m];
+        next_a();
+        next_b();
     }
 
     // Steps lo .. hi of the product.
     __device__ __forceinline__ void run(LdsAt base, int wave, int lo, int hi, f32x16 (&acc)[F][F]) {
-        const LdsAt mine = base + wave * F * 1024;
+        const LdsAt base_b = base + A_BUFFERS * S::SIDE;
+        const int mine = wave * S::PARTS * 1024;
         // steps whose loads are whole: the last of a segment may not be
-        const int whole = p.segments == 1 ? min(hi, (int)(p.k / STEP)) : p.k % STEP == 0 ? hi : 0;
-        auto left = [&](int s) -> int64_t { return s >= hi ? 0 : p.k - int64_t(steps_in - c.left) * STEP; };
-        auto buffer = [](LdsAt at, int s) { return at + (s & 3) * S::BUFFER; };
-        E8 fa[F], fb[F];
-        seek(lo);
-        for (int s = 0; s < 3; s++) {
+        const int whole = q.segments == 1 ? min(hi, (int)(q.k / STEP)) : q.k % STEP == 0 ? hi : 0;
+        auto load_a = [&](int s, LdsAt to) {
+            const int64_t n = there(fa, s < hi);
 #pragma unroll
-            for (int q = 0; q < F; q++) load<true>(q, left(lo + s), buffer(mine, s));
-            next();
+            for (int k = 0; k < S::PARTS; k++) fa.template load<true>(k, n, to + mine);
+            next_a();
+        };
+        load_a(lo, base);
+        {
+            const int64_t n = there(fb, true);
+#pragma unroll
+            for (int k = 0; k < S::PARTS; k++) fb.template load<true>(k, n, base_b + mine);
+            next_b();
         }
-        arrived<4 * F>();
+        load_a(lo + 1, base + S::SIDE);
+        arrived<S::PARTS>();
+        E8 xa[F], xb[F];
 #pragma unroll
         for (int m = 0; m < F; m++) {
-            fa[m] = ra.template take<E8>(base, 0, m);
-            fb[m] = rb.template take<E8>(base + S::SIDE, 0, m);
+            xa[m] = ra.template take<E8>(base, 0, m);
+            xb[m] = rb.template take<E8>(base_b, 0, m);
         }
-        int s = 0;
-        for (; lo + s + 3 < whole; s++)
-            step<false>(buffer(base, s), buffer(base, s + 1), buffer(mine, s + 3), STEP, fa, fb, acc);
+        LdsAt a = base, na = base + S::SIDE, to = base + 2 * S::SIDE, b = base_b, nb = base_b + S::SIDE;
+        auto turn = [&] {
+            const LdsAt was = a;
+            a = na, na = to, to = was;
+            const LdsAt old = b;
+            b = nb, nb = old;
+        };
+        int s = lo;
+        for (; s + 2 < whole; s++, turn()) step<false>(a, b, na, nb, to + mine, nb + mine, STEP, STEP, xa, xb, acc);
         // the last steps load zeros past the end: the count of loads in flight stays the same
-        for (; lo + s < hi; s++)
-            step<true>(buffer(base, s), buffer(base, s + 1), buffer(mine, s + 3), left(lo + s + 3), fa, fb, acc);
+        for (; s < hi; s++, turn())
+            step<true>(a, b, na, nb, to + mine, nb + mine, there(fa, s + 2 < hi), there(fb, s + 1 < hi), xa, xb, acc);
         asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
         __builtin_amdgcn_s_barrier();
     }
@@ -296,7 +316,7 @@ __global__ __launch_bounds__(PRODUCT_BLOCK, F == 4 ? 1 : 2) void k_product(Produ
 
     f32x16 acc[F][F] = {};
     if (lo < hi) {
-        Tiles<E, F, AI, BI> tiles_of(p, batch, i0, j0, wave, lane);
+        Tiles<E, F, AI, BI> tiles_of(p, batch, i0, j0, wave, lane, lo);
         tiles_of.run((LdsAt)lds, wave, lo, hi, acc);
     }
 
