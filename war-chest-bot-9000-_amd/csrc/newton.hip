@@ -139,6 +139,260 @@ __global__ __launch_bounds__(256) void k_start(Update<T> u, const double* sums, 
     }
 }
 
+// ------------------------------------------------------------ small matrices
+
+// A matrix whose X (in the form that is wide: small x large) and A fit in LDS, two parts each, in one launch: a workgroup
+// of eight wavefronts a matrix. Fragments of 32 x 32, of A those on and above the diagonal only. B takes A's place, and X'
+// X's, after a barrier. Vector arithmetic bounds it (splitting results into their parts, addresses): so the parts of eight
+// elements lie beside each other, 16 bytes and 16 bytes, and one address serves both.
+constexpr int SMALL_BLOCK = 512, SMALL_WAVES = SMALL_BLOCK / 64, SMALL_LDS = 160 * 1024, SMALL_TILES = 6;
+
+struct SmallShape {
+    int m, n, mp, np;  // small, large, and rounded up to whole fragments
+    int px, pa;        // bytes from row to row: 16 more than the row has, so that rows lie in different banks
+
+    __host__ __device__ SmallShape(int64_t small, int64_t large) {
+        m = (int)small, n = (int)large;
+        mp = (m + 31) / 32 * 32, np = (n + 31) / 32 * 32;
+        px = 4 * np + 16, pa = 4 * mp + 16;
+    }
+    bool fits() const {
+        return int64_t(mp) * (px + pa) <= SMALL_LDS && mp <= 128 &&
+               (mp / 32) * (np / 32) <= SMALL_WAVES * SMALL_TILES;
+    }
+};
+
+struct Pair16 {
+    f16x8 hi, lo;
+};
+
+// Where element c of a row is.
+__device__ __forceinline__ int place_of(int c) { return 4 * (c & ~7) + 2 * (c & 7); }
+
+// Fragments along k, 16 at a time. Lane l's eight of k, from 8 (l / 32) on, of row first + l % 32, where rows have k inside.
+struct ByRows {
+    const char* p;
+
+    __device__ __forceinline__ ByRows(const char* base, int pitch, int first, int lane)
+        : p(base + (first + (lane & 31)) * pitch + 32 * (lane >> 5)) {}
+    __device__ __forceinline__ Pair16 take(int part) const {
+        return {*(const f16x8*)(p + 64 * part), *(const f16x8*)(p + 64 * part + 16)};
+    }
+    __device__ __forceinline__ void next() { p += 128; }  // 32 of k
+};
+// The same of column first + l % 32, where rows are on k.
+struct ByColumns {
+    const char *p, *q;  // four rows apart
+    int pitch;
+
+    __device__ __forceinline__ ByColumns(const char* base, int row, int first, int lane)
+        : p(base + (8 * (lane >> 5) + ((lane & 15) >> 2)) * row + place_of(first + (lane & 16) + 4 * (lane & 3))),
+          q(p + 4 * row), pitch(row) {}
+    __device__ __forceinline__ Pair16 take(int part) const {
+        return {eight(p + part * 16 * pitch, q + part * 16 * pitch),
+                eight(p + part * 16 * pitch + 16, q + part * 16 * pitch + 16)};
+    }
+    __device__ __forceinline__ void next() { p += 32 * pitch, q += 32 * pitch; }
+    static __device__ __forceinline__ f16x8 eight(const char* p, const char* q) {
+        typedef __attribute__((address_space(3))) s16x4* At;
+        const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((At)p);
+        const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((At)q);
+        return __builtin_bit_cast(f16x8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+    }
+};
+
+// c and the sum over k, a multiple of 32, of p's rows by q's columns; the next fragments are loaded beside each product.
+template <class P, class Q>
+__device__ __forceinline__ f32x16 sum_of(int all, f32x16 c, P p, Q q) {
+    auto add = [&](const Pair16& a, const Pair16& b) {
+        c = mfma(a.lo, b.hi, c);  // small by large, large by small, large by large
+        c = mfma(a.hi, b.lo, c);
+        c = mfma(a.hi, b.hi, c);
+    };
+    Pair16 a = p.take(0), b = q.take(0);
+    for (int k = 32; k < all; k += 32) {
+        const Pair16 a1 = p.take(1), b1 = q.take(1);
+        p.next(), q.next();
+        add(a, b);
+        a = p.take(0), b = q.take(0);
+        add(a1, b1);
+    }
+    const Pair16 a1 = p.take(1), b1 = q.take(1);
+    add(a, b);
+    add(a1, b1);
+    return c;
+}
+
+typedef f16 f16x2 __attribute__((ext_vector_type(2)));
+typedef f16 f16x4 __attribute__((ext_vector_type(4)));
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+
+// The parts of two elements.
+__device__ __forceinline__ void split(float a, float b, f16x2& hi, f16x2& lo) {
+    hi = __builtin_convertvector(f32x2{a, b}, f16x2);
+    lo = __builtin_convertvector(f32x2{a - (float)hi[0], b - (float)hi[1]}, f16x2);
+}
+
+template <class T>
+__global__ __launch_bounds__(SMALL_BLOCK, 2) void k_newton_small(Update<T> u, wc_orthogonalise_args o) {
+    __shared__ __align__(16) char lds[SMALL_LDS];
+    const bool tall = u.rows > u.width;
+    const SmallShape s(tall ? u.width : u.rows, tall ? u.rows : u.width);
+    const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
+    char* const x = lds;
+    char* const a = lds + s.mp * s.px;
+    const int wide = s.mp / 32, deep = s.np / 32, tiles = wide * deep, halves = wide * (wide + 1) / 2;
+
+    // A wavefront's fragments of X stay in its registers in float32, and are what it adds to; LDS has what the products
+    // read. Lane l has of a fragment column l % 32 and rows 8 (k / 4) + 4 (l / 32) + k % 4.
+    f32x16 held[SMALL_TILES];
+    const int down = 4 * (lane >> 5), across = lane & 31;
+    auto each = [&](auto&& body) {
+#pragma unroll
+        for (int g = 0; g < SMALL_TILES; g++) {
+            const int tile = wave + g * SMALL_WAVES;
+            if (tile < tiles) body(held[g], 32 * (tile / deep), 32 * (tile % deep));
+        }
+    };
+    // A fragment's parts to rows i0 .. of `to`; as rows of its mirror image too.
+    auto put = [&](char* to, int pitch, const f32x16& c, int i0, int j0, bool mirror) {
+        char* p = to + (i0 + down) * pitch + place_of(j0 + across);
+        char* m = to + (j0 + across) * pitch + place_of(i0 + down);
+#pragma unroll
+        for (int q = 0; q < 4; q++) {
+            f16x2 hi[2], lo[2];
+#pragma unroll
+            for (int k = 0; k < 2; k++) split(c[4 * q + 2 * k], c[4 * q + 2 * k + 1], hi[k], lo[k]);
+#pragma unroll
+            for (int k = 0; k < 4; k++) {
+                *(f16*)(p + k * pitch) = hi[k / 2][k % 2];
+                *(f16*)(p + k * pitch + 16) = lo[k / 2][k % 2];
+            }
+            p += 8 * pitch;
+            if (mirror) {  // eight rows on are the next sixteen bytes and sixteen
+                *(f16x4*)(m + 32 * q) = __builtin_shufflevector(hi[0], hi[1], 0, 1, 2, 3);
+                *(f16x4*)(m + 32 * q + 16) = __builtin_shufflevector(lo[0], lo[1], 0, 1, 2, 3);
+            }
+        }
+    };
+
+    // The matrix in chunks of eight of a row, as float32 where X's parts will be, and its norm: squares summed in 64 bits,
+    // as in k_squares. Chunk c of a wide matrix is chunk c % per_row of a row, of a tall one a row's, rows first: then
+    // neighbours write beside each other either way.
+    const T* from = u.u + blockIdx.x * u.batch;
+    const uint32_t width = (uint32_t)u.width, rows = (uint32_t)u.rows, per_row = (width + 7) / 8, chunks = rows * per_row;
+    auto place = [&](uint32_t chunk, uint32_t& r, uint32_t& col) {
+        const uint32_t by = tall ? rows : per_row, q = chunk / by, rest = chunk - q * by;
+        r = tall ? rest : q, col = 8 * (tall ? q : rest);
+    };
+    for (int at = t * 16; at < s.mp * s.px; at += SMALL_BLOCK * 16) *(uint4*)(x + at) = uint4{};
+    __syncthreads();
+    double sum = 0;
+    for (uint32_t first = t; first < chunks; first += 4 * SMALL_BLOCK) {
+        float v[4][8] = {};
+        uint32_t r[4], col[4];
+#pragma unroll
+        for (int g = 0; g < 4; g++) {
+            const uint32_t chunk = first + g * SMALL_BLOCK;
+            place(chunk, r[g], col[g]);
+            if (chunk < chunks) load_n(from + r[g] * u.stride + col[g], (int)min(8u, width - col[g]), 0.f, v[g]);
+        }
+#pragma unroll
+        for (int g = 0; g < 4; g++) {
+            if (first + g * SMALL_BLOCK >= chunks) break;
+#pragma unroll
+            for (int k = 0; k < 8; k++) {
+                sum += (double)v[g][k] * (double)v[g][k];
+                if (col[g] + k < width) *(float*)(x + (tall ? (col[g] + k) * s.px + 4 * r[g] : r[g] * s.px + 4 * (col[g] + k))) = v[g][k];
+            }
+        }
+    }
+#pragma unroll
+    for (int mask = 32; mask; mask >>= 1) sum += __shfl_xor(sum, mask);
+    double* sums = (double*)a;
+    if (lane == 0) sums[wave] = sum;
+    __syncthreads();
+    sum = 0;
+    for (int w = 0; w < SMALL_WAVES; w++) sum += sums[w];
+    const double rate = HELD / (sqrt(sum) + (double)o.eps);
+    each([&](f32x16& c, int i0, int j0) {
+        const char* p = x + (i0 + down) * s.px + 4 * (j0 + across);
+#pragma unroll
+        for (int k = 0; k < 16; k++) c[k] = (float)((double)*(const float*)(p + (8 * (k / 4) + k % 4) * s.px) * rate);
+    });
+    __syncthreads();
+    each([&](f32x16& c, int i0, int j0) { put(x, s.px, c, i0, j0, false); });
+    __syncthreads();
+
+    // a wavefront's fragments of A and B, on or above the diagonal
+    constexpr int HALVES = (10 + SMALL_WAVES - 1) / SMALL_WAVES;
+    auto each_half = [&](f32x16(&c)[HALVES], auto&& body) {
+#pragma unroll
+        for (int g = 0; g < HALVES; g++) {
+            const int tile = wave + g * SMALL_WAVES;
+            if (tile >= halves) break;
+            int tj = 0;
+            while ((tj + 1) * (tj + 2) / 2 <= tile) tj++;
+            body(c[g], 32 * (tile - tj * (tj + 1) / 2), 32 * tj);
+        }
+    };
+    for (int step = 0; step < o.steps; step++) {
+        f32x16 c[HALVES];
+        // A = X X^T
+        each_half(c, [&](f32x16& d, int i0, int j0) {
+            d = sum_of(s.np, f32x16{}, ByRows(x, s.px, i0, lane), ByRows(x, s.px, j0, lane));
+#pragma unroll
+            for (int k = 0; k < 16; k++) d[k] *= 1.f / HELD;
+            put(a, s.pa, d, i0, j0, i0 != j0);
+        });
+        __syncthreads();
+        // B = b A + c A A
+        each_half(c, [&](f32x16& d, int i0, int j0) {
+            const f32x16 e = sum_of(s.mp, f32x16{}, ByRows(a, s.pa, i0, lane), ByRows(a, s.pa, j0, lane));
+#pragma unroll
+            for (int k = 0; k < 16; k++) d[k] = o.b * d[k] + o.c / HELD * e[k];
+        });
+        __syncthreads();
+        each_half(c, [&](f32x16& d, int i0, int j0) { put(a, s.pa, d, i0, j0, i0 != j0); });
+        __syncthreads();
+        // X' = a X + B X
+        each([&](f32x16& d, int i0, int j0) {
+#pragma unroll
+            for (int k = 0; k < 16; k++) d[k] *= HELD * o.a;
+            d = sum_of(s.mp, d, ByRows(a, s.pa, i0, lane), ByColumns(x, s.px, j0, lane));
+#pragma unroll
+            for (int k = 0; k < 16; k++) d[k] *= 1.f / HELD;
+        });
+        __syncthreads();
+        if (step + 1 == o.steps) break;
+        each([&](f32x16& d, int i0, int j0) { put(x, s.px, d, i0, j0, false); });
+        __syncthreads();
+    }
+    // and back the same way
+    const float scale = o.scale / HELD;
+    each([&](f32x16& c, int i0, int j0) {
+        char* p = x + (i0 + down) * s.px + 4 * (j0 + across);
+#pragma unroll
+        for (int k = 0; k < 16; k++) *(float*)(p + (8 * (k / 4) + k % 4) * s.px) = c[k] * scale;
+    });
+    __syncthreads();
+    for (uint32_t chunk = t; chunk < chunks; chunk += SMALL_BLOCK) {
+        uint32_t r, col;
+        place(chunk, r, col);
+        const int have = (int)min(8u, width - col);
+        float v[8];
+#pragma unroll
+        for (int k = 0; k < 8; k++) {
+            const uint32_t c = min(col + k, width - 1);
+            v[k] = *(const float*)(x + (tall ? c * s.px + 4 * r : r * s.px + 4 * c));
+        }
+        const int64_t to = blockIdx.x * o.out_batch + r * o.out_stride + col;
+        if (o.out_dtype == WC_DTYPE_F32) store_n((float*)o.out + to, have, v);
+        else if (o.out_dtype == WC_DTYPE_F16) store_n((f16*)o.out + to, have, v);
+        else store_n((bf16*)o.out + to, have, v);
+    }
+}
+
 struct Plan {
     int planes, segments, blocks;  // planes of A and B, and of X in products; X has two
     int64_t small, pitch, pitch_small, x_plane, a_plane;  // elements
@@ -189,9 +443,18 @@ Operand16 operand(const Held16& h, int planes, int64_t outer) {
     return o;
 }
 
+bool small_enough(const wc_orthogonalise_args& o) {
+    const int64_t small = std::min(o.rows, o.width), large = std::max(o.rows, o.width);
+    return small <= 128 && large <= 4096 && SmallShape(small, large).fits();
+}
+
 template <class T>
 void start(const wc_orthogonalise_args& o, const Plan& p, const Held16& x, hipStream_t s) {
     const Update<T> u = {(const T*)o.update, o.update_stride, o.update_batch, o.rows, o.width};
+    if (small_enough(o)) {
+        k_newton_small<T><<<dim3((uint32_t)o.batch), SMALL_BLOCK, 0, s>>>(u, o);
+        return;
+    }
     double* sums = (double*)((char*)o.workspace + p.sums);
     const dim3 grid((uint32_t)p.blocks, (uint32_t)o.batch);
     k_squares<T><<<grid, 256, 0, s>>>(u, sums);
@@ -202,7 +465,9 @@ void start(const wc_orthogonalise_args& o, const Plan& p, const Held16& x, hipSt
 
 }  // namespace
 
-size_t orthogonalise_scratch(const wc_orthogonalise_args& o, int cus) { return plan_of(o, cus).bytes; }
+size_t orthogonalise_scratch(const wc_orthogonalise_args& o, int cus) {
+    return small_enough(o) ? 0 : plan_of(o, cus).bytes;
+}
 
 void launch_orthogonalise(const wc_orthogonalise_args& o, int cus, hipStream_t s) {
     if (!o.batch) return;
@@ -214,6 +479,7 @@ void launch_orthogonalise(const wc_orthogonalise_args& o, int cus, hipStream_t s
     if (o.dtype == WC_DTYPE_F32) start<float>(o, p, x[0], s);
     else if (o.dtype == WC_DTYPE_F16) start<f16>(o, p, x[0], s);
     else start<bf16>(o, p, x[0], s);
+    if (small_enough(o)) return;
 
     const bool tall = o.rows > o.width;
     float* part = (float*)(w + p.part);
