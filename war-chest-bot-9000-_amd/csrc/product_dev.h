@@ -86,17 +86,17 @@ struct Fetch {
     __device__ __forceinline__ void set(const Product& q, const Operand16& o, const uint8_t* planes, int batch, int64_t at0,
                                         int wave, int lane, int s, int steps_in) {
         first = wave * S::PARTS * 64 + lane;
+        const uint32_t pitch = (uint32_t)o.pitch;
+        const int beyond = (int)min<int64_t>(o.outer - at0, S::TILE);  // rows or columns of the tile that are there
 #pragma unroll
         for (int k = 0; k < S::PARTS; k++) {
             const int g = first + 64 * k;
             if (INNER) {
-                const int row = g / 8, chunk = (g % 8) ^ (row & 7);
                 // past the last row any row will do: its products are not stored
-                const int64_t r = min(at0 + row, o.outer - 1) - at0;
-                at[k] = (uint32_t)(r * o.pitch) + 16 * chunk;
+                at[k] = (uint32_t)min(g / 8, beyond - 1) * pitch + 16 * ((g % 8) ^ (g / 8 & 7));
             } else {
                 const int row = g / (8 * F), chunk = (g % (8 * F)) ^ (S::turn(row) << 2);
-                at[k] = (uint32_t)(row * o.pitch) + (at0 + 8 * chunk < o.outer ? 16 * chunk : 0);
+                at[k] = (uint32_t)row * pitch + (8 * chunk < beyond ? 16 * chunk : 0);
             }
         }
         step = INNER ? 2 * STEP : STEP * o.pitch;
@@ -290,7 +290,7 @@ struct Tiles {
 //   struct Epilogue { __device__ void operator()(int batch, int64_t i, int64_t j, int n, float (&v)[8]) const; }
 // MIRROR: symmetric results; the epilogue also gets columns as rows.
 template <class E, int F, bool AI, bool BI, class Epilogue>
-__global__ __launch_bounds__(PRODUCT_BLOCK, F == 4 ? 1 : 2) void k_product(Product p, Epilogue epilogue) {
+__global__ __launch_bounds__(PRODUCT_BLOCK, F > 2 ? 1 : 2) void k_product(Product p, Epilogue epilogue) {
     typedef TileShape<F> S;
     __shared__ __align__(16) char lds[S::LDS];
     const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
@@ -334,10 +334,10 @@ __global__ __launch_bounds__(PRODUCT_BLOCK, F == 4 ? 1 : 2) void k_product(Produ
             for (int k = 0; k < 16; k++)
                 mine[(8 * (k / 4) + 4 * (lane >> 5) + k % 4) * PITCH + 32 * n + (lane & 31)] = acc[m][n][k];
         __builtin_amdgcn_wave_barrier();
-        for (int it = 0; it < 32 / ROWS; it++) {
+        for (int it = 0; it < (32 + ROWS - 1) / ROWS; it++) {
             const int r = it * ROWS + lane / CHUNKS, c = 8 * (lane % CHUNKS);
             const int64_t i = wi + 32 * m + r, j = wj + c;
-            if (i >= m_all || j >= n_all) continue;
+            if (i >= m_all || j >= n_all || (64 % CHUNKS && (lane >= ROWS * CHUNKS || r >= 32))) continue;
             const float4 lo4 = *(const float4*)(mine + r * PITCH + c), hi4 = *(const float4*)(mine + r * PITCH + c + 4);
             float v[8] = {lo4.x, lo4.y, lo4.z, lo4.w, hi4.x, hi4.y, hi4.z, hi4.w};
             const int have = (int)min<int64_t>(8, n_all - j);
@@ -413,22 +413,39 @@ struct Cut {
     size_t bytes(int64_t n) const { return runs > 1 ? size_t(runs) * n * 4 : 0; }
 };
 
+// What a round of workgroups costs, in microseconds: a step with so many workgroups a CU, and all else (the start, the
+// first loads, the epilogue, the end). Measured on products of 1 to 2,048 tiles and 1 to 64 steps; a tile of 256 reaches
+// 1.41 PFLOP/s in its steps on all CUs, one of 192 1.3, of 128 1.12, of 64 0.59, but costs 15 us beside them, 11, 7 and 4.
+struct RoundCost {
+    int most;            // workgroups a CU
+    double step[4], fixed[4];
+};
+inline const RoundCost& round_cost(int f) {
+    static const RoundCost cost[4] = {{4, {0.33, 0.51, 0.72, 0.91}, {4.0, 4.6, 5.3, 6.0}},
+                                      {2, {0.57, 1.0}, {6.8, 8.5}},
+                                      {1, {0.95}, {11.5}},
+                                      {1, {1.52}, {15.5}}};
+    return cost[f - 1];
+}
+
 inline Cut cut_of(int64_t m, int64_t n, int64_t k, int segments, int cus, int64_t batches = 1, bool triangle = false) {
     Cut best = {};
     double least = -1;
     const int64_t steps = (k + STEP - 1) / STEP * segments;
-    for (int f = 4; f >= 1; f /= 2) {
-        const int64_t tile = 64 * f, tm = (m + tile - 1) / tile, tn = (n + tile - 1) / tile, 
+    for (int f = 4; f >= 1; f--) {
+        const RoundCost& cost = round_cost(f);
+        const int64_t tile = 64 * f, tm = (m + tile - 1) / tile, tn = (n + tile - 1) / tile,
                       tiles = std::max<int64_t>(1, batches * (triangle ? tm * (tm + 1) / 2 : tm * tn));
-        const int64_t slots = f == 4 ? cus : f == 2 ? 2 * cus : 4 * cus;
-        const double step = f == 4 ? 0.8 : f == 2 ? 0.5 : 0.4;
-        const int64_t most = std::max<int64_t>(1, std::min<int64_t>(steps / 4, 4 * slots / tiles));
-        for (int64_t r = 1; r <= 64; r = r < 8 ? r + 1 : r * 5 / 4) {
+        const int64_t slots = int64_t(cost.most) * cus;
+        const int64_t most = std::max<int64_t>(1, std::min<int64_t>(steps / 2, 4 * slots / tiles));
+        for (int64_t r = 1; r <= 128; r = r < 8 ? r + 1 : r * 5 / 4) {
             if (r > most) break;
             const int64_t per = (steps + r - 1) / r, runs = per ? (steps + per - 1) / per : 1;
-            const int64_t rounds = (tiles * runs + slots - 1) / slots;
-            const double t = double(rounds) * (double(per) * step + 3.0) +
-                             (runs > 1 ? 4.0 + double(runs) * batches * m * n * 8 / 5e6 : 0.0);
+            const int64_t full = tiles * runs / slots, rest = tiles * runs % slots, beside = (rest + cus - 1) / cus;
+            double t = double(full) * (double(per) * cost.step[cost.most - 1] + cost.fixed[cost.most - 1]);
+            if (rest) t += double(per) * cost.step[beside - 1] + cost.fixed[beside - 1];
+            // the runs' products written, read and added by a launch of its own
+            if (runs > 1) t += 4.0 + double(runs) * batches * m * n * 8 / 4.5e6;
             if (least >= 0 && t >= least) continue;
             least = t;
             best.f = f;
@@ -463,6 +480,7 @@ void launch_product(Product p, const Cut& cut, bool ai, bool bi, float* part, co
     p.triangle = cut.triangle ? 64 * cut.f : 0;
     p.part = part;
     if (cut.f == 4) product_of<E, 4>(p, ai, bi, e, s);
+    else if (cut.f == 3) product_of<E, 3>(p, ai, bi, e, s);
     else if (cut.f == 2) product_of<E, 2>(p, ai, bi, e, s);
     else product_of<E, 1>(p, ai, bi, e, s);
     if (cut.runs > 1) {
