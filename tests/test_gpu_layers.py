@@ -135,11 +135,15 @@ def test_linear_over_sizes(rows, width, out, dtype):
 
 @pytest.mark.parametrize("rows,width,out,dtype", [(1030, 520, 776, "bf16"), (2500, 264, 520, "f16"), (600, 333, 401, "f32"),
                                                   (20000, 96, 192, "bf16"), (20001, 97, 31, "f16"), (5000, 64, 128, "f32"),
-                                                  (16, 4096, 512, "bf16"), (1, 8192, 1024, "f32"), (31, 20000, 40, "f16")])
+                                                  (16, 4096, 512, "bf16"), (1, 8192, 1024, "f32"), (31, 20000, 40, "f16"),
+                                                  (1, 4099, 16391, "bf16"), (7, 3001, 2057, "f16"), (13, 2500, 1029, "f32"),
+                                                  (3, 70000, 65, "bf16"), (4, 512, 13000, "f32")])
 def test_linear_with_larger_sizes(rows, width, out, dtype):
     k, d = layer_inputs(rows, width, out, TYPES[dtype], 7)
     say(f"case linear: {rows} x {width} x {out} {dtype}")
     v = {n: to(t) for n, t in k.items()}
+    other = wl.linear(v["x"], v["weight"].t().contiguous().t(), v["bias"], residual=v["residual"], act="silu", keep=True)
+    check_forward(other, k, "silu")
     got = wl.linear(**{n: v[n] for n in ("x", "weight", "bias")}, residual=v["residual"], act="silu", keep=True)
     check_forward(got, k, "silu")
     back = wl.linear_backward(to(d), v["x"], v["weight"], got.pre, act="silu", bias=True)

@@ -53,6 +53,17 @@ __device__ __forceinline__ void store_n(T* __restrict__ p, int n, const float (&
         if (i < n) p[i] = (T)v[i];
 }
 
+// The first n (0 .. N) of N elements, zeros in the place of the others.
+template <int N, class T>
+__device__ __forceinline__ typename VecN<T, N>::type load_some(const T* p, int n) {
+    if (n >= N) return *(const typename VecN<T, N>::type*)p;
+    typename VecN<T, N>::type v = {};
+#pragma unroll
+    for (int i = 0; i < N - 1; i++)
+        if (i < n) v[i] = p[i];
+    return v;
+}
+
 // 2^x by the hardware (1 ulp; a result under 2^-126 is 0).
 __device__ __forceinline__ float power(float x) { return __builtin_amdgcn_exp2f(x); }
 

@@ -199,9 +199,195 @@ void lay(const Laid& l1, const Source& s1, const Laid& l2, const Source& s2, cha
     if (n) k_lay<T><<<lay_grid(n, cus), 256, 0, s>>>(a, b);
 }
 
+// ------------------------------------------------------------------ few rows
+
+// A few rows against a weight: the weight is read once, and nothing else matters. No matrix instruction, no copy: a lane
+// has 16 bytes of a weight's row at a time, eight rows of it, times eight of k of every row of x. A wavefront's loads are
+// whole lines of 128 bytes, eight of them in flight while the last eight are multiplied. 4,096 x 16,384 bf16, one row: 28
+// us, 4.8 TB/s (a large copy moves 5.16; the tiles of 64, with split sums, take 33).
+//
+// Where rows of the weight are on k (IN_OUT) a wavefront has eight lanes across, 128 bytes of columns, and 64 of k, the
+// workgroup's wavefronts follow each other along k and add up at the end. Where they are outputs (OUT_IN) a wavefront has
+// eight outputs and all lanes along k.
+constexpr int FEW_BLOCK = 512, FEW_WAVES = FEW_BLOCK / 64;
+
+struct FewJob {
+    int64_t rows, width, out, x_stride, w_stride, run;  // run: of k, a multiple of 512
+    int runs;
+    float* part;
+};
+
+template <class T, int R, bool IO, class Epilogue>
+__global__ __launch_bounds__(FEW_BLOCK) void k_few(const T* x, const T* w, FewJob job, Epilogue epilogue) {
+    constexpr int E = 16 / sizeof(T);
+    typedef typename VecN<T, E>::type Chunk;
+    __shared__ float lds[IO ? FEW_WAVES : 1][R][8 * E];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int groups = gridDim.x / job.runs, run = blockIdx.x / groups, group = blockIdx.x - run * groups;
+    const int64_t lo = run * job.run, hi = min(lo + job.run, job.width);
+    const T* rows[R];
+#pragma unroll
+    for (int r = 0; r < R; r++) rows[r] = x + min<int64_t>(r, job.rows - 1) * job.x_stride;  // what is not there is not stored
+    auto to = [&](int64_t r, int64_t j, int n, float (&v)[8]) {
+        if (job.runs > 1) store_n(job.part + (run * job.rows + r) * job.out + j, n, v);
+        else epilogue(0, r, j, n, v);
+    };
+
+    if constexpr (IO) {
+        const int64_t j = int64_t(group) * 8 * E + (lane & 7) * E;
+        const int have = (int)max<int64_t>(0, min<int64_t>(E, job.out - j));
+        float acc[R][E] = {};
+        const T* at = w + (lo + wave * 64 + (lane >> 3) * 8) * job.w_stride + (have == E ? j : 0);
+        auto add = [&](int64_t k, const Chunk (&c)[8], int there) {
+            float v[R][8];
+#pragma unroll
+            for (int r = 0; r < R; r++) load_n(rows[r] + k, there, 0.f, v[r]);
+#pragma unroll
+            for (int i = 0; i < 8; i++)
+#pragma unroll
+                for (int e = 0; e < E; e++) {
+                    const float f = (float)c[i][e];
+#pragma unroll
+                    for (int r = 0; r < R; r++) acc[r][e] += v[r][i] * f;
+                }
+        };
+        int64_t k = lo + wave * 64 + (lane >> 3) * 8;
+        if (have == E) {
+            Chunk c[8];
+            auto load = [&](const T* p, Chunk (&d)[8]) {
+#pragma unroll
+                for (int i = 0; i < 8; i++) d[i] = *(const Chunk*)(p + i * job.w_stride);
+            };
+            bool whole = k + 8 <= hi;
+            if (whole) load(at, c);
+            while (whole) {
+                const int64_t next = k + 64 * FEW_WAVES;
+                at += 64 * FEW_WAVES * job.w_stride;
+                whole = next + 8 <= hi;
+                Chunk d[8];
+                if (whole) load(at, d);
+                add(k, c, 8);
+#pragma unroll
+                for (int i = 0; i < 8; i++) c[i] = d[i];
+                k = next;
+            }
+        }
+        // the last of k, and the last columns
+        for (; k < hi && have; k += 64 * FEW_WAVES) {
+            const int there = (int)min<int64_t>(8, hi - k);
+            Chunk c[8] = {};
+#pragma unroll
+            for (int i = 0; i < 8; i++)
+                if (i < there) c[i] = load_some<E>(w + (k + i) * job.w_stride + j, have);
+            add(k, c, there);
+        }
+#pragma unroll
+        for (int r = 0; r < R; r++)
+#pragma unroll
+            for (int e = 0; e < E; e++) {
+                float s = acc[r][e];
+#pragma unroll
+                for (int mask = 8; mask < 64; mask <<= 1) s += __shfl_xor(s, mask);
+                if (lane < 8) lds[wave][r][lane * E + e] = s;
+            }
+        __syncthreads();
+        if (threadIdx.x >= 8 * R) return;
+        const int r = threadIdx.x / 8, at_e = threadIdx.x % 8 * E;
+        if (r >= job.rows || j >= job.out) return;
+        float v[8] = {};
+#pragma unroll
+        for (int e = 0; e < E; e++)
+            for (int u = 0; u < FEW_WAVES; u++) v[e] += lds[u][r][at_e + e];
+        to(r, j, have, v);
+    } else {
+        const int64_t j = (int64_t(group) * FEW_WAVES + wave) * 8;  // eight outputs
+        const int have = (int)max<int64_t>(0, min<int64_t>(8, job.out - j));
+        float acc[R][8] = {};
+        auto add = [&](int64_t k, const Chunk (&c)[8], int there) {
+            float v[R][E];
+#pragma unroll
+            for (int r = 0; r < R; r++) {
+                const Chunk d = load_some<E>(rows[r] + k, there);
+#pragma unroll
+                for (int e = 0; e < E; e++) v[r][e] = (float)d[e];
+            }
+#pragma unroll
+            for (int i = 0; i < 8; i++)
+#pragma unroll
+                for (int e = 0; e < E; e++) {
+                    const float f = (float)c[i][e];
+#pragma unroll
+                    for (int r = 0; r < R; r++) acc[r][i] += v[r][e] * f;
+                }
+        };
+        auto load = [&](int64_t k, int there, Chunk (&d)[8]) {
+#pragma unroll
+            for (int i = 0; i < 8; i++)  // past the last output the last again
+                d[i] = load_some<E>(w + min<int64_t>(j + i, job.out - 1) * job.w_stride + k, there);
+        };
+        Chunk c[8];
+        int64_t k = lo + lane * E;
+        auto there = [&](int64_t at) { return (int)max<int64_t>(0, min<int64_t>(E, hi - at)); };
+        if (have) {
+            load(k, there(k), c);
+            while (k < hi) {
+                const int64_t next = k + 64 * E;
+                Chunk d[8] = {};
+                if (next < hi) load(next, there(next), d);
+                add(k, c, there(k));
+#pragma unroll
+                for (int i = 0; i < 8; i++) c[i] = d[i];
+                k = next;
+            }
+        }
+#pragma unroll
+        for (int r = 0; r < R; r++) {
+            float v[8];
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                v[i] = acc[r][i];
+#pragma unroll
+                for (int mask = 1; mask < 64; mask <<= 1) v[i] += __shfl_xor(v[i], mask);
+            }
+            if (lane == r && r < job.rows && have) to(r, j, have, v);
+        }
+    }
+}
+
+// Whether a product is of few rows. Microseconds of k_few and of the tiles, IN_OUT: bf16 4,096 x 16,384 28 and 46 (1 row),
+// 40 and 46 (8); 4,096 x 4,096 12.6 and 12.6 (2), 15.1 and 12.6 (4); 1,024 x 1,024 5.9 and 7.1 (2), 8.3 and 7.1 (4).
+// float32, whose tiles read three parts of six products: 4,096 x 4,096 16.6 and 66 (1), 36.6 and 66 (16); OUT_IN 24 and 65
+// (8), 54 and 65 (16), but 1,024 x 1,024 16.4 and 19.2 (8), 39 and 19.2 (16).
+// Its runs: two workgroups a CU, or one where the columns give that many already and the second launch that adds the runs
+// is not needed.
+struct Few {
+    bool is;
+    int lanes_rows, runs;  // rows a lane has
+    int64_t groups, run;
+};
+
+template <class T>
+Few few_of(const wc_linear_args& a, int cus) {
+    constexpr int64_t E = 16 / sizeof(T);
+    const bool io = a.weight_layout == WC_WEIGHT_IN_OUT;
+    Few f = {};
+    f.is = sizeof(T) == 4 ? a.rows <= (io ? 16 : 8) : a.rows <= (a.width * a.out >= 1 << 25 ? 8 : 2);
+    if (!f.is) return f;
+    f.lanes_rows = a.rows <= 1 ? 1 : a.rows <= 2 ? 2 : a.rows <= 4 ? 4 : a.rows <= 8 ? 8 : 16;
+    const int64_t each = io ? 8 * E : 8 * FEW_WAVES;
+    f.groups = (a.out + each - 1) / each;
+    const int64_t most = std::max<int64_t>(1, a.width / 1024);
+    const int64_t want = f.groups * 4 >= int64_t(cus) * 3 ? 1 : (2 * int64_t(cus) + f.groups - 1) / f.groups;
+    const int64_t runs = std::min(most, want);
+    f.run = up((a.width + runs - 1) / runs, 512);
+    f.runs = (int)((a.width + f.run - 1) / f.run);
+    return f;
+}
+
 // ------------------------------------------------------------------ forward
 
 struct LinearPlan {
+    Few few;
     Laid x, w;
     Cut cut;
     int64_t k;
@@ -213,6 +399,11 @@ LinearPlan linear_plan(const wc_linear_args& a, int cus) {
     constexpr int parts = Parts<T>::COUNT;
     LinearPlan p = {};
     const bool io = a.weight_layout == WC_WEIGHT_IN_OUT;
+    p.few = few_of<T>(a, cus);
+    if (p.few.is) {
+        p.bytes = p.few.runs > 1 ? pad256(size_t(p.few.runs) * a.rows * a.out * 4) : 0;
+        return p;
+    }
     p.x = laid<T>(a.x, a.x_stride, a.rows, a.width);
     p.w = io ? laid<T>(a.weight, a.weight_stride, a.width, a.out) : laid<T>(a.weight, a.weight_stride, a.out, a.width);
     p.k = parts > 1 ? up(a.width, STEP) : a.width;
@@ -236,14 +427,39 @@ void linear(const wc_linear_args& a, int cus, hipStream_t s) {
     const LinearPlan p = linear_plan<T>(a, cus);
     char* w = (char*)a.workspace;
     const bool io = a.weight_layout == WC_WEIGHT_IN_OUT;
+    const LayerEpilogue<T> e = {a.bias, a.bias_dtype == WC_DTYPE_F32, (const T*)a.residual, a.residual_stride,
+                                a.pre, a.pre_stride, (T*)a.y, a.y_stride, a.act};
+    if (p.few.is) {
+        const FewJob job = {a.rows, a.width, a.out, a.x_stride, a.weight_stride, p.few.run, p.few.runs, (float*)w};
+        const dim3 grid((uint32_t)(p.few.groups * p.few.runs));
+        auto run = [&](auto rows) {
+            if (io) k_few<T, rows(), true><<<grid, FEW_BLOCK, 0, s>>>((const T*)a.x, (const T*)a.weight, job, e);
+            else if constexpr (rows() <= 8)
+                k_few<T, rows(), false><<<grid, FEW_BLOCK, 0, s>>>((const T*)a.x, (const T*)a.weight, job, e);
+        };
+        if (p.few.lanes_rows == 1) run(std::integral_constant<int, 1>());
+        else if (p.few.lanes_rows == 2) run(std::integral_constant<int, 2>());
+        else if (p.few.lanes_rows == 4) run(std::integral_constant<int, 4>());
+        else if (p.few.lanes_rows == 8) run(std::integral_constant<int, 8>());
+        else if constexpr (sizeof(T) == 4) run(std::integral_constant<int, 16>());
+        if (p.few.runs > 1) {
+            Product m = {};
+            m.a.outer = a.rows;
+            m.b.outer = a.out;
+            m.runs = p.few.runs;
+            m.batches = 1;
+            m.part = (float*)w;
+            const int64_t chunks = a.rows * ((a.out + 7) / 8);
+            k_product_sum<<<dim3((uint32_t)((chunks + 63) / 64)), PRODUCT_BLOCK, 0, s>>>(m, chunks, e);
+        }
+        return;
+    }
     lay<T>(p.x, {a.x, a.x_stride, a.rows, a.width}, p.w,
            {a.weight, a.weight_stride, io ? a.width : a.out, io ? a.out : a.width}, w, cus, s);
     Product m = {};
     m.a = operand<T>(p.x, a.x, w, a.rows);
     m.b = operand<T>(p.w, a.weight, w, a.out);
     m.k = p.k;
-    const LayerEpilogue<T> e = {a.bias, a.bias_dtype == WC_DTYPE_F32, (const T*)a.residual, a.residual_stride,
-                                (float*)a.pre, a.pre_stride, (T*)a.y, a.y_stride, a.act};
     multiply<T>(m, p.cut, true, !io, (float*)(w + p.part), e, s);
 }
 
