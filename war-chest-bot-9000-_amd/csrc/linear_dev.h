@@ -134,7 +134,12 @@ struct LayerEpilogue {
     int64_t y_stride;
     int act;
 
-    __device__ __forceinline__ void operator()(int, int64_t i, int64_t j, int n, float (&v)[8]) const {
+    __device__ __forceinline__ bool reads() const { return residual != nullptr; }
+    typedef typename Vec8<T>::type Raw;
+    __device__ __forceinline__ Raw raw(int, int64_t i, int64_t j, int n) const {
+        return residual ? load_some<8>(residual + i * residual_stride + j, n) : Raw{};
+    }
+    __device__ __forceinline__ void operator()(const Raw& r, int, int64_t i, int64_t j, int n, float (&v)[8]) const {
         if (bias) {
             float b[8];
             if (bias_f32) load_n((const float*)bias + j, n, 0.f, b);
@@ -145,10 +150,8 @@ struct LayerEpilogue {
         if (pre) store_n(pre + i * pre_stride + j, n, v);
         act_values(v, act);
         if (residual) {
-            float r[8];
-            load_n(residual + i * residual_stride + j, n, 0.f, r);
 #pragma unroll
-            for (int u = 0; u < 8; u++) v[u] += r[u];
+            for (int u = 0; u < 8; u++) v[u] += (float)r[u];
         }
         store_n(y + i * y_stride + j, n, v);
     }
@@ -163,10 +166,9 @@ Operand16 operand(const Laid& l, const void* p, char* workspace, int64_t outer) 
     return o;
 }
 
-// a, b and k are set.
-template <class T, class Epilogue>
-void multiply(Product p, const Cut& cut, bool ai, bool bi, float* part, const Epilogue& e, hipStream_t s) {
-    typedef typename Parts<T>::type E;
+// The segments of a product whose a, b and k are set.
+template <class T>
+Product segments_of(Product p) {
     if (Parts<T>::COUNT == 3) {
         // the largest last: what is small is added to what is small
         static constexpr uint8_t pa[] = {2, 1, 0, 1, 0, 0}, pb[] = {0, 1, 2, 0, 1, 0};
@@ -174,10 +176,14 @@ void multiply(Product p, const Cut& cut, bool ai, bool bi, float* part, const Ep
         for (int k = 0; k < 6; k++) p.pa[k] = pa[k], p.pb[k] = pb[k];
     } else {
         p.segments = 1;
-        p.pa[0] = p.pb[0] = 0;
     }
     p.batches = 1;
-    launch_product<E>(p, cut, ai, bi, part, e, s);
+    return p;
+}
+
+template <class T, class Epilogue>
+void multiply(const Product& p, const Cut& cut, bool ai, bool bi, float* part, const Epilogue& e, hipStream_t s) {
+    launch_product<typename Parts<T>::type>(segments_of<T>(p), cut, ai, bi, part, e, s);
 }
 
 inline dim3 lay_grid(int64_t chunks, int cus) {
@@ -230,7 +236,7 @@ __global__ __launch_bounds__(FEW_BLOCK) void k_few(const T* x, const T* w, FewJo
     for (int r = 0; r < R; r++) rows[r] = x + min<int64_t>(r, job.rows - 1) * job.x_stride;  // what is not there is not stored
     auto to = [&](int64_t r, int64_t j, int n, float (&v)[8]) {
         if (job.runs > 1) store_n(job.part + (run * job.rows + r) * job.out + j, n, v);
-        else epilogue(0, r, j, n, v);
+        else epilogue(epilogue.raw(0, r, j, n), 0, r, j, n, v);
     };
 
     if constexpr (IO) {
@@ -505,9 +511,18 @@ __global__ __launch_bounds__(256) void k_slope(wc_linear_back_args a, Source d, 
 }
 
 // The row blocks' column sums added in order: a sixteenth of them each group of sixteen threads.
-static __global__ __launch_bounds__(256) void k_slope_sum(const float* sums, int64_t out, int blocks, float* to) {
+struct ColumnSums {
+    const float* sums;
+    int64_t out;
+    int blocks;
+    float* to;
+};
+__device__ __forceinline__ void column_sums(const ColumnSums& c, int64_t block) {
+    const float* sums = c.sums;
+    const int64_t out = c.out;
+    const int blocks = c.blocks;
     __shared__ float some[16][17];
-    const int64_t j = int64_t(blockIdx.x) * 16 + threadIdx.x % 16;
+    const int64_t j = block * 16 + threadIdx.x % 16;
     const int q = threadIdx.x / 16;
     float s = 0.f;
     if (j < out) {
@@ -524,7 +539,16 @@ static __global__ __launch_bounds__(256) void k_slope_sum(const float* sums, int
     __syncthreads();
     if (q || j >= out) return;
     for (int u = 1; u < 16; u++) s += some[u][threadIdx.x];
-    to[j] = s;
+    c.to[j] = s;
+}
+static __global__ __launch_bounds__(256) void k_slope_sum(ColumnSums c) { column_sums(c, blockIdx.x); }
+
+// The weight gradient's runs and the bias's blocks, in one launch.
+template <class Epilogue>
+__global__ __launch_bounds__(PRODUCT_BLOCK) void k_back_sum(Product p, int64_t chunks, Epilogue epilogue, unsigned blocks,
+                                                            ColumnSums c) {
+    if (blockIdx.x < blocks) product_sum(p, chunks, epilogue, blockIdx.x);
+    else column_sums(c, blockIdx.x - blocks);
 }
 
 struct LinearBackPlan {
@@ -533,7 +557,8 @@ struct LinearBackPlan {
     int64_t out_k, rows_k, per;
     int blocks;
     bool slope;
-    size_t sums, part, bytes;
+    size_t sums, part_x, part, bytes;
+    bool together;
 };
 
 template <class T>
@@ -558,22 +583,27 @@ LinearBackPlan linear_back_plan(const wc_linear_back_args& a, int cus) {
         return here;
     };
     if (products) p.d.at = take(p.d.bytes(parts));
-    size_t part = 0;
     if (a.d_x) {
         p.w = io ? laid<T>(a.weight, a.weight_stride, a.width, a.out) : laid<T>(a.weight, a.weight_stride, a.out, a.width);
         p.w.at = take(p.w.bytes(parts));
         p.out_k = parts > 1 ? up(a.out, STEP) : a.out;
         p.cut_x = cut_of(a.rows, a.width, p.out_k, parts > 1 ? 6 : 1, cus);
-        part = std::max(part, p.cut_x.bytes(a.rows * a.width));
     }
     if (a.d_weight) {
         p.x = laid<T>(a.x, a.x_stride, a.rows, a.width);
         p.x.at = take(p.x.bytes(parts));
         p.rows_k = parts > 1 ? up(a.rows, STEP) : a.rows;
         p.cut_w = cut_of(io ? a.width : a.out, io ? a.out : a.width, p.rows_k, parts > 1 ? 6 : 1, cus);
-        part = std::max(part, p.cut_w.bytes(a.width * a.out));
     }
-    p.part = take(part);  // one after the other in it
+    // Small tiles of both: one launch, whose second product starts where the first leaves CUs free.
+    p.together = a.d_x && a.d_weight && a.rows && p.cut_x.f == p.cut_w.f && p.cut_x.f <= 2;
+    const size_t px = a.d_x ? p.cut_x.bytes(a.rows * a.width) : 0, pw = a.d_weight ? p.cut_w.bytes(a.width * a.out) : 0;
+    if (p.together) {
+        p.part_x = take(px);
+        p.part = take(pw);
+    } else {
+        p.part_x = p.part = take(std::max(px, pw));  // one after the other in it
+    }
     if (p.slope) {
         const int64_t across = (a.out + 255) / 256;
         const int64_t blocks = std::max<int64_t>(1, std::min<int64_t>((a.rows + 31) / 32, 8 * int64_t(cus) / across + 1));
@@ -610,31 +640,64 @@ void linear_back(const wc_linear_back_args& a, int cus, hipStream_t s) {
         float* sums = a.d_bias ? (float*)(w + p.sums) : nullptr;
         const int64_t across = ((d.to ? p.d.cols : a.out) + 255) / 256;
         k_slope<T><<<dim3((uint32_t)across, (uint32_t)p.blocks), 256, 0, s>>>(a, d, p.per, sums);
-        if (sums) k_slope_sum<<<dim3((uint32_t)((a.out + 15) / 16)), 256, 0, s>>>(sums, a.out, p.blocks, a.d_bias);
+    }
+    const ColumnSums bias = {(const float*)(w + p.sums), a.out, p.blocks, a.d_bias};
+    const uint32_t bias_blocks = a.d_bias ? (uint32_t)((a.out + 15) / 16) : 0;
+    if (!a.d_weight || p.cut_w.runs == 1) {
+        if (bias_blocks) k_slope_sum<<<dim3(bias_blocks), 256, 0, s>>>(bias);
     }
     if (!products) return;
     // copies of x and the weight, in one launch
     lay<T>(p.x, {a.x, a.x_stride, a.rows, a.width}, p.w,
            {a.weight, a.weight_stride, io ? a.width : a.out, io ? a.out : a.width}, w, cus, s);
-    float* part = (float*)(w + p.part);
-    if (a.d_x && a.rows) {
-        Product m = {};
-        m.a = operand<T>(p.d, a.d_out, w, a.rows);
-        m.b = operand<T>(p.w, a.weight, w, a.width);
-        m.k = p.out_k;
-        multiply<T>(m, p.cut_x, true, io, part, plain_to<T>(a.d_x, a.d_x_stride), s);
+    const bool with_x = a.d_x && a.rows;
+    Product mx = {}, mw = {};
+    if (with_x) {
+        mx.a = operand<T>(p.d, a.d_out, w, a.rows);
+        mx.b = operand<T>(p.w, a.weight, w, a.width);
+        mx.k = p.out_k;
+        mx = cut_product(segments_of<T>(mx), p.cut_x, (float*)(w + p.part_x));
     }
-    if (a.d_weight) {
-        Product m = {};
-        const Operand16 x = operand<T>(p.x, a.x, w, a.width), d = operand<T>(p.d, a.d_out, w, a.out);
-        m.a = io ? x : d;
-        m.b = io ? d : x;
-        m.k = p.rows_k;
-        if (a.grad_dtype == a.dtype) {
-            multiply<T>(m, p.cut_w, false, false, part, plain_to<T>(a.d_weight, a.d_weight_stride), s);
-        } else if constexpr (Parts<T>::COUNT == 1) {
-            multiply<T>(m, p.cut_w, false, false, part, plain_to<float>(a.d_weight, a.d_weight_stride), s);
+    const auto ex = plain_to<T>(a.d_x, a.d_x_stride);
+    if (!a.d_weight) {
+        if (with_x) multiply<T>(mx, p.cut_x, true, io, mx.part, ex, s);
+        return;
+    }
+    const Operand16 x = operand<T>(p.x, a.x, w, a.width), d = operand<T>(p.d, a.d_out, w, a.out);
+    mw.a = io ? x : d;
+    mw.b = io ? d : x;
+    mw.k = p.rows_k;
+    mw = cut_product(segments_of<T>(mw), p.cut_w, (float*)(w + p.part));
+    auto both = [&](const auto& ew) {
+        typedef typename Parts<T>::type E;
+        auto sums = [&] {
+            const int64_t chunks = sum_chunks(mw);
+            const uint32_t blocks = (uint32_t)((chunks + 63) / 64);
+            if (p.cut_w.runs > 1) k_back_sum<<<dim3(blocks + bias_blocks), PRODUCT_BLOCK, 0, s>>>(mw, chunks, ew, blocks, bias);
+        };
+        const uint32_t nx = (uint32_t)(mx.tiles_m * mx.tiles_n * mx.runs), nw = (uint32_t)(mw.tiles_m * mw.tiles_n * mw.runs);
+        auto together = [&](auto f) {
+            if (io) k_products<E, f(), true><<<dim3(nx + nw), PRODUCT_BLOCK, 0, s>>>(mx, ex, nx, mw, ew);
+            else k_products<E, f(), false><<<dim3(nx + nw), PRODUCT_BLOCK, 0, s>>>(mx, ex, nx, mw, ew);
+        };
+        if (with_x && p.together) {
+            if (p.cut_x.f == 2) together(std::integral_constant<int, 2>());
+            else together(std::integral_constant<int, 1>());
+            if (p.cut_x.runs > 1)
+                k_product_sum<<<dim3((uint32_t)((sum_chunks(mx) + 63) / 64)), PRODUCT_BLOCK, 0, s>>>(mx, sum_chunks(mx), ex);
+        } else {
+            if (with_x) multiply<T>(mx, p.cut_x, true, io, mx.part, ex, s);
+            if (p.cut_w.f == 4) product_of<E, 4>(mw, false, false, ew, s);
+            else if (p.cut_w.f == 3) product_of<E, 3>(mw, false, false, ew, s);
+            else if (p.cut_w.f == 2) product_of<E, 2>(mw, false, false, ew, s);
+            else product_of<E, 1>(mw, false, false, ew, s);
         }
+        sums();
+    };
+    if (a.grad_dtype == a.dtype) {
+        both(plain_to<T>(a.d_weight, a.d_weight_stride));
+    } else if constexpr (Parts<T>::COUNT == 1) {
+        both(plain_to<float>(a.d_weight, a.d_weight_stride));
     }
 }
 

@@ -42,16 +42,14 @@ struct Held16 {
         *(f16x8*)to = hi;
         if (planes > 1) *(f16x8*)(to + plane) = lo;
     }
-    __device__ __forceinline__ void get(int planes, int batch_of, int64_t i, int64_t j, float (&v)[8]) const {
+    struct Eight {
+        f16x8 hi, lo;
+    };
+    __device__ __forceinline__ Eight get(int planes, int batch_of, int64_t i, int64_t j) const {
         const f16* from = p + batch_of * batch + i * pitch + j;
-        const f16x8 hi = *(const f16x8*)from;
-#pragma unroll
-        for (int u = 0; u < 8; u++) v[u] = (float)hi[u];
-        if (planes > 1) {
-            const f16x8 lo = *(const f16x8*)(from + plane);
-#pragma unroll
-            for (int u = 0; u < 8; u++) v[u] += (float)lo[u];
-        }
+        Eight e = {*(const f16x8*)from, f16x8{}};
+        if (planes > 1) e.lo = *(const f16x8*)(from + plane);
+        return e;
     }
 };
 
@@ -68,14 +66,16 @@ struct StepEpilogue {
     __device__ __forceinline__ void result(int batch, int64_t i, int64_t j, int n, const float (&v)[8]) const {
         store_n((T*)out + batch * out_batch + i * out_stride + j, n, v);
     }
-    __device__ __forceinline__ void operator()(int batch, int64_t i, int64_t j, int n, float (&v)[8]) const {
+    __device__ __forceinline__ bool reads() const { return from.p != nullptr; }
+    typedef Held16::Eight Raw;
+    __device__ __forceinline__ Raw raw(int batch, int64_t i, int64_t j, int) const {
+        return from.p ? from.get(from_planes, batch, i, j) : Raw{};
+    }
+    __device__ __forceinline__ void operator()(const Raw& r, int batch, int64_t i, int64_t j, int n, float (&v)[8]) const {
 #pragma unroll
-        for (int u = 0; u < 8; u++) v[u] *= alpha;
-        if (from.p) {
-            float x[8];
-            from.get(from_planes, batch, i, j, x);
-#pragma unroll
-            for (int u = 0; u < 8; u++) v[u] += beta * x[u];
+        for (int u = 0; u < 8; u++) {
+            v[u] *= alpha;
+            if (from.p) v[u] += beta * ((float)r.hi[u] + (float)r.lo[u]);
         }
         if (!out) to.put(to_planes, batch, i, j, n, v);
         else if (out_dtype == WC_DTYPE_F32) result<float>(batch, i, j, n, v);

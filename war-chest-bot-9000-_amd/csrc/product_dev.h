@@ -287,16 +287,22 @@ struct Tiles {
 };
 
 // What a product's epilogue sees: eight values of row i from column j, n of them in the matrix.
-//   struct Epilogue { __device__ void operator()(int batch, int64_t i, int64_t j, int n, float (&v)[8]) const; }
+// Raw is what it reads for them, before, if reads().
+//   struct Epilogue {
+//       bool reads() const;
+//       Raw raw(int batch, int64_t i, int64_t j, int n) const;
+//       void operator()(const Raw&, int batch, int64_t i, int64_t j, int n, float (&v)[8]) const;
+//   };
 // MIRROR: symmetric results; the epilogue also gets columns as rows.
+// Workgroup `block` of `total` of a product.
 template <class E, int F, bool AI, bool BI, class Epilogue>
-__global__ __launch_bounds__(PRODUCT_BLOCK, F > 2 ? 1 : 2) void k_product(Product p, Epilogue epilogue) {
+__device__ __forceinline__ void product(const Product& p, const Epilogue& epilogue, char* lds, unsigned block,
+                                        unsigned total) {
     typedef TileShape<F> S;
-    __shared__ __align__(16) char lds[S::LDS];
     const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
     // Workgroups go round the eight XCDs; consecutive tiles, which share panels of both operands, go to one XCD's cache.
-    const unsigned total = gridDim.x, per = total / 8;
-    const int id = blockIdx.x < per * 8 ? (blockIdx.x % 8) * per + blockIdx.x / 8 : blockIdx.x;
+    const unsigned per = total / 8;
+    const int id = block < per * 8 ? (block % 8) * per + block / 8 : block;
     const int tiles = p.triangle ? p.tiles_m * (p.tiles_m + 1) / 2 : p.tiles_m * p.tiles_n;
     const int batch = id / (tiles * p.runs), run = id / tiles - batch * p.runs, tile = id % tiles;
     int ti, tj;
@@ -334,15 +340,44 @@ __global__ __launch_bounds__(PRODUCT_BLOCK, F > 2 ? 1 : 2) void k_product(Produc
             for (int k = 0; k < 16; k++)
                 mine[(8 * (k / 4) + 4 * (lane >> 5) + k % 4) * PITCH + 32 * n + (lane & 31)] = acc[m][n][k];
         __builtin_amdgcn_wave_barrier();
-        for (int it = 0; it < (32 + ROWS - 1) / ROWS; it++) {
-            const int r = it * ROWS + lane / CHUNKS, c = 8 * (lane % CHUNKS);
-            const int64_t i = wi + 32 * m + r, j = wj + c;
-            if (i >= m_all || j >= n_all || (64 % CHUNKS && (lane >= ROWS * CHUNKS || r >= 32))) continue;
+        // What the epilogue reads for a few rows goes before the first of them is written; where it reads nothing, a row
+        // at a time is faster (16,384 x 4,096 x 4,096: 464 and 497 us; with a residual 625 and 587).
+        constexpr int TURNS = (32 + ROWS - 1) / ROWS, SOME = sizeof(typename Epilogue::Raw) > 16 && F > 2 ? 2 : 4,
+                      AT_ONCE = TURNS < SOME ? TURNS : SOME;
+        const int c = 8 * (lane % CHUNKS);
+        const int64_t j = wj + c;
+        const int have = (int)max<int64_t>(0, min<int64_t>(8, n_all - j));
+        auto there = [&](int r) {
+            return have > 0 && wi + 32 * m + r < m_all && !(64 % CHUNKS && (lane >= ROWS * CHUNKS || r >= 32));
+        };
+        auto values = [&](int r, float(&v)[8]) {
             const float4 lo4 = *(const float4*)(mine + r * PITCH + c), hi4 = *(const float4*)(mine + r * PITCH + c + 4);
-            float v[8] = {lo4.x, lo4.y, lo4.z, lo4.w, hi4.x, hi4.y, hi4.z, hi4.w};
-            const int have = (int)min<int64_t>(8, n_all - j);
-            if (part) store_n(part + i * n_all + j, have, v);
-            else epilogue(batch, i, j, have, v);
+            v[0] = lo4.x, v[1] = lo4.y, v[2] = lo4.z, v[3] = lo4.w, v[4] = hi4.x, v[5] = hi4.y, v[6] = hi4.z, v[7] = hi4.w;
+        };
+        if (!part && epilogue.reads()) {
+            for (int it = 0; it < TURNS; it += AT_ONCE) {
+                typename Epilogue::Raw raw[AT_ONCE] = {};
+                const int r = it * ROWS + lane / CHUNKS;
+#pragma unroll
+                for (int u = 0; u < AT_ONCE; u++)
+                    if (there(r + u * ROWS)) raw[u] = epilogue.raw(batch, wi + 32 * m + r + u * ROWS, j, have);
+#pragma unroll
+                for (int u = 0; u < AT_ONCE; u++) {
+                    if (!there(r + u * ROWS)) continue;
+                    float v[8];
+                    values(r + u * ROWS, v);
+                    epilogue(raw[u], batch, wi + 32 * m + r + u * ROWS, j, have, v);
+                }
+            }
+        } else {
+            for (int it = 0; it < TURNS; it++) {
+                const int r = it * ROWS + lane / CHUNKS;
+                if (!there(r)) continue;
+                float v[8];
+                values(r, v);
+                if (part) store_n(part + (wi + 32 * m + r) * n_all + j, have, v);
+                else epilogue({}, batch, wi + 32 * m + r, j, have, v);
+            }
         }
         if (Epilogue::MIRROR && p.triangle && ti != tj && !part) {
             // a row of the other half: 32 of i, eight a lane
@@ -353,21 +388,38 @@ __global__ __launch_bounds__(PRODUCT_BLOCK, F > 2 ? 1 : 2) void k_product(Produc
                 float v[8];
 #pragma unroll
                 for (int u = 0; u < 8; u++) v[u] = mine[(r + u) * PITCH + c];
-                epilogue(batch, i, j, (int)min<int64_t>(8, m_all - j), v);
+                const int n = (int)min<int64_t>(8, m_all - j);
+                epilogue(epilogue.raw(batch, i, j, n), batch, i, j, n, v);
             }
         }
         __builtin_amdgcn_wave_barrier();
     }
 }
 
+template <class E, int F, bool AI, bool BI, class Epilogue>
+__global__ __launch_bounds__(PRODUCT_BLOCK, F > 2 ? 1 : 2) void k_product(Product p, Epilogue epilogue) {
+    __shared__ __align__(16) char lds[TileShape<F>::LDS];
+    product<E, F, AI, BI>(p, epilogue, lds, blockIdx.x, gridDim.x);
+}
+
+// Two products that do not wait for each other in one launch: the first's workgroups, and the second's, whose operands both
+// have rows on k.
+template <class E, int F, bool BI, class Epilogue, class Second>
+__global__ __launch_bounds__(PRODUCT_BLOCK, 2) void k_products(Product p, Epilogue epilogue, unsigned blocks, Product q,
+                                                               Second second) {
+    __shared__ __align__(16) char lds[TileShape<F>::LDS];
+    if (blockIdx.x < blocks) product<E, F, true, BI>(p, epilogue, lds, blockIdx.x, blocks);
+    else product<E, F, false, false>(q, second, lds, blockIdx.x - blocks, gridDim.x - blocks);
+}
+
 // The runs' partial products added, in an order that does not change: eight elements of a row a thread, a quarter of
 // the runs each wavefront.
 template <class Epilogue>
-__global__ __launch_bounds__(PRODUCT_BLOCK) void k_product_sum(Product p, int64_t chunks, Epilogue epilogue) {
+__device__ __forceinline__ void product_sum(const Product& p, int64_t chunks, const Epilogue& epilogue, int64_t block) {
     typedef float Eight __attribute__((ext_vector_type(8)));
     __shared__ Eight quarters[3][64];
     const int quarter = threadIdx.x >> 6, lane = threadIdx.x & 63;
-    const int64_t m = p.a.outer, n = p.b.outer, at = int64_t(blockIdx.x) * 64 + lane, per_row = (n + 7) / 8;
+    const int64_t m = p.a.outer, n = p.b.outer, at = block * 64 + lane, per_row = (n + 7) / 8;
     const bool there = at < chunks;
     const int64_t row = at / per_row, j = (at - row * per_row) * 8;  // a row of all matrices
     const int have = (int)min<int64_t>(8, n - j);
@@ -396,7 +448,12 @@ __global__ __launch_bounds__(PRODUCT_BLOCK) void k_product_sum(Product p, int64_
     float v[8];
 #pragma unroll
     for (int u = 0; u < 8; u++) v[u] = s[u];
-    epilogue((int)batch, i, j, have, v);
+    epilogue(epilogue.raw((int)batch, i, j, have), (int)batch, i, j, have, v);
+}
+
+template <class Epilogue>
+__global__ __launch_bounds__(PRODUCT_BLOCK) void k_product_sum(Product p, int64_t chunks, Epilogue epilogue) {
+    product_sum(p, chunks, epilogue, blockIdx.x);
 }
 
 // ---------------------------------------------------------------- the host's side
@@ -470,8 +527,7 @@ void product_of(const Product& p, bool ai, bool bi, const Epilogue& e, hipStream
 }
 
 // a, b, k, segments and batches are set.
-template <class E, class Epilogue>
-void launch_product(Product p, const Cut& cut, bool ai, bool bi, float* part, const Epilogue& e, hipStream_t s) {
+inline Product cut_product(Product p, const Cut& cut, float* part) {
     p.tiles_m = (int)cut.tiles_m;
     p.tiles_n = (int)cut.tiles_n;
     p.runs = cut.runs;
@@ -479,14 +535,19 @@ void launch_product(Product p, const Cut& cut, bool ai, bool bi, float* part, co
     p.steps = cut.steps;
     p.triangle = cut.triangle ? 64 * cut.f : 0;
     p.part = part;
+    return p;
+}
+inline int64_t sum_chunks(const Product& p) { return p.batches * p.a.outer * ((p.b.outer + 7) / 8); }
+
+template <class E, class Epilogue>
+void launch_product(Product p, const Cut& cut, bool ai, bool bi, float* part, const Epilogue& e, hipStream_t s) {
+    p = cut_product(p, cut, part);
     if (cut.f == 4) product_of<E, 4>(p, ai, bi, e, s);
     else if (cut.f == 3) product_of<E, 3>(p, ai, bi, e, s);
     else if (cut.f == 2) product_of<E, 2>(p, ai, bi, e, s);
     else product_of<E, 1>(p, ai, bi, e, s);
-    if (cut.runs > 1) {
-        const int64_t chunks = p.batches * p.a.outer * ((p.b.outer + 7) / 8);
-        k_product_sum<<<dim3((uint32_t)((chunks + 63) / 64)), PRODUCT_BLOCK, 0, s>>>(p, chunks, e);
-    }
+    if (cut.runs > 1)
+        k_product_sum<<<dim3((uint32_t)((sum_chunks(p) + 63) / 64)), PRODUCT_BLOCK, 0, s>>>(p, sum_chunks(p), e);
 }
 
 }  // namespace
