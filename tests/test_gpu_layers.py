@@ -300,7 +300,8 @@ def check_ortho(got, u, dtype, **kw):
 @pytest.mark.parametrize("dtype", list(TYPES))
 @pytest.mark.parametrize("shape", [(1, 1), (1, 9), (17, 1), (3, 5), (8, 8), (64, 64), (63, 65), (40, 200), (200, 40), (96, 192),
                                    (3, 96, 192), (5, 33, 17), (2, 130, 70), (256, 264), (300, 700), (1, 70, 70), (0, 4, 4), (128, 128), (130, 128), (97, 161), (128, 160),
-                                   (32, 1200), (1000, 30), (64, 570)])
+                                   (32, 1200), (1000, 30), (64, 570), (1030, 257), (131, 2000), (6, 140, 333), (500, 512),
+                                   (513, 700)])
 def test_orthogonalise_over_sizes(shape, dtype):
     say(f"case orthogonalise: {shape} {dtype}")
     u = (0.01 * torch.randn(*shape, generator=gen(sum(shape)))).to(TYPES[dtype])

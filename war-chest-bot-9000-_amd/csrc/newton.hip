@@ -393,9 +393,126 @@ __global__ __launch_bounds__(SMALL_BLOCK, 2) void k_newton_small(Update<T> u, wc
     }
 }
 
+// ----------------------------------------------------------- narrow matrices
+
+// A = X X^T and B = b A + c A A where tiles of 64 would be few: a workgroup of eight wavefronts a fragment of 32 x 32 on
+// or above the diagonal, each an eighth of k, straight from memory (rows have k inside: 16 bytes a lane), added in LDS.
+// 256 x 1,024, one part: 7.8 us and 3.6, on tiles of 64 12 and 6. A call with 512 rows, and with 520 on tiles: 2,048
+// columns 133 us and 187, 4,096 182 and 222, 8,192 280 and 284; in two parts 220 and 304, 315 and 378, 491 and 466.
+constexpr int NARROW_BLOCK = 512, NARROW_WAVES = NARROW_BLOCK / 64;
+
+struct NarrowJob {
+    Held16 x;       // rows of k
+    int64_t m, k;
+    Held16 from, to;
+    float alpha, beta;
+};
+
+template <int PARTS>
+__global__ __launch_bounds__(NARROW_BLOCK) void k_narrow(NarrowJob o) {
+    __shared__ float sums[NARROW_WAVES][32][33];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, batch = blockIdx.y;
+    int tj = (int)((sqrtf(8.f * blockIdx.x + 1.f) - 1.f) * 0.5f);
+    while (tj * (tj + 1) / 2 > (int)blockIdx.x) tj--;
+    while ((tj + 1) * (tj + 2) / 2 <= (int)blockIdx.x) tj++;
+    const int64_t i0 = 32 * (blockIdx.x - tj * (tj + 1) / 2), j0 = 32 * tj;
+    // past the last row any row will do: its products are not stored
+    const f16* base = o.x.p + batch * o.x.batch + 8 * (lane >> 5);
+    const f16* pa = base + min(i0 + (lane & 31), o.m - 1) * o.x.pitch;
+    const f16* pb = base + min(j0 + (lane & 31), o.m - 1) * o.x.pitch;
+    const int steps = (int)((o.k + 15) / 16), each = (steps + NARROW_WAVES - 1) / NARROW_WAVES;
+    const int lo = wave * each, hi = min(lo + each, steps);
+    f32x16 c = {};
+#pragma unroll 8
+    for (int s = lo; s < hi; s++) {
+        f16x8 a[PARTS], b[PARTS];
+        const bool there = 16 * s + 8 * (lane >> 5) < o.k;  // whole eights, zeros in the last
+#pragma unroll
+        for (int u = 0; u < PARTS; u++) {
+            a[u] = there ? *(const f16x8*)(pa + 16 * s + u * o.x.plane) : f16x8{};
+            b[u] = there ? *(const f16x8*)(pb + 16 * s + u * o.x.plane) : f16x8{};
+        }
+        if constexpr (PARTS > 1) {
+            c = mfma(a[1], b[0], c);
+            c = mfma(a[0], b[1], c);
+        }
+        c = mfma(a[0], b[0], c);
+    }
+#pragma unroll
+    for (int k = 0; k < 16; k++) sums[wave][8 * (k / 4) + 4 * (lane >> 5) + k % 4][lane & 31] = c[k];
+    __syncthreads();
+    const int r = threadIdx.x / 16, col = threadIdx.x % 16 * 2;
+    const int64_t padded = (o.m + 7) & ~int64_t(7);
+#pragma unroll
+    for (int u = 0; u < 2; u++) {
+        const int64_t i = i0 + r, j = j0 + col + u;
+        float v = 0.f;
+        if (i < o.m && j < o.m) {
+            for (int w = 0; w < NARROW_WAVES; w++) v += sums[w][r][col + u];
+            v *= o.alpha;
+            if (o.from.p) {
+                const f16* from = o.from.p + batch * o.from.batch + i * o.from.pitch + j;
+                v += o.beta * ((float)from[0] + (PARTS > 1 ? (float)from[o.from.plane] : 0.f));
+            }
+        }
+        const f16 hi = (f16)v, low = (f16)(v - (float)hi);
+        f16* to = o.to.p + batch * o.to.batch;
+        if (i < o.m && j < padded) {
+            to[i * o.to.pitch + j] = hi;
+            if (PARTS > 1) to[i * o.to.pitch + j + o.to.plane] = low;
+        }
+        if (i0 != j0 && j < o.m && i < padded) {
+            to[j * o.to.pitch + i] = hi;
+            if (PARTS > 1) to[j * o.to.pitch + i + o.to.plane] = low;
+        }
+    }
+}
+
+// A tall matrix turned, as X's parts, and back as the result: eight of a row a thread, rows first.
+template <class T>
+__global__ __launch_bounds__(256) void k_start_turned(Update<T> u, const double* sums, int blocks, float eps, Held16 to) {
+    __shared__ double lds[4];
+    double s = 0;
+    for (int k = threadIdx.x; k < blocks; k += 256) s += sums[int64_t(blockIdx.y) * blocks + k];
+    s = all_of(s, lds);
+    const double rate = HELD / (sqrt(s) + (double)eps);
+    const int64_t rows = to.pitch, chunks = rows * ((u.width + 7) / 8);  // with zeros to the end of to's rows
+    for (int64_t at = int64_t(blockIdx.x) * 256 + threadIdx.x; at < chunks; at += int64_t(gridDim.x) * 256) {
+        const int64_t c = at / rows * 8, r = at % rows;
+        float v[8] = {};
+        if (r < u.rows) load_n(u.u + blockIdx.y * u.batch + r * u.stride + c, (int)min<int64_t>(8, u.width - c), 0.f, v);
+        f16* p = to.p + blockIdx.y * to.batch + c * to.pitch + r;
+#pragma unroll
+        for (int k = 0; k < 8; k++) {
+            if (c + k >= u.width) break;
+            const float x = (float)((double)v[k] * rate);
+            const f16 hi = (f16)x;
+            p[k * to.pitch] = hi;
+            p[k * to.pitch + to.plane] = (f16)(x - (float)hi);
+        }
+    }
+}
+
+template <class T>
+__global__ __launch_bounds__(256) void k_finish_turned(Held16 x, int64_t rows, int64_t width, float scale, T* out,
+                                                       int64_t stride, int64_t batch) {
+    const int64_t chunks = rows * ((width + 7) / 8);
+    for (int64_t at = int64_t(blockIdx.x) * 256 + threadIdx.x; at < chunks; at += int64_t(gridDim.x) * 256) {
+        const int64_t c = at / rows * 8, r = at % rows;
+        const f16* p = x.p + blockIdx.y * x.batch + c * x.pitch + r;
+        float v[8] = {};
+#pragma unroll
+        for (int k = 0; k < 8; k++)
+            if (c + k < width) v[k] = scale * ((float)p[k * x.pitch] + (float)p[k * x.pitch + x.plane]);
+        store_n(out + blockIdx.y * batch + r * stride + c, (int)min<int64_t>(8, width - c), v);
+    }
+}
+
 struct Plan {
     int planes, segments, blocks;  // planes of A and B, and of X in products; X has two
     int64_t small, pitch, pitch_small, x_plane, a_plane;  // elements
+    bool narrow, turned;  // narrow: k_narrow, for which a tall matrix is turned
+    int64_t x_rows, x_cols;
     Cut gram, square, step;
     size_t x[2], a, b, sums, part, bytes;
 };
@@ -407,14 +524,19 @@ Plan plan_of(const wc_orthogonalise_args& o, int cus) {
     p.planes = o.out_dtype == WC_DTYPE_BF16 && p.small > 128 ? 1 : 2;
     p.segments = p.planes == 1 ? 1 : 3;
     const int64_t large = tall ? o.rows : o.width;
-    p.pitch = up(o.width, 8);
+    const int64_t fragments = (p.small + 31) / 32;
+    p.narrow = p.small <= 512 && large <= 4096 && fragments * (fragments + 1) / 2 * o.batch <= 2 * int64_t(cus);
+    p.turned = p.narrow && tall;
+    p.x_rows = p.turned ? o.width : o.rows;
+    p.x_cols = p.turned ? o.rows : o.width;
+    p.pitch = up(p.x_cols, 8);
     p.pitch_small = up(p.small, 8);
-    p.x_plane = o.rows * p.pitch;
+    p.x_plane = p.x_rows * p.pitch;
     p.a_plane = p.small * p.pitch_small;
     p.gram = cut_of(p.small, p.small, large, p.segments, cus, o.batch, true);
     p.square = cut_of(p.small, p.small, p.small, p.segments, cus, o.batch, true);
-    p.step = cut_of(o.rows, o.width, p.small, p.segments, cus, o.batch);
-    const int64_t chunks = o.rows * (p.pitch / 8);
+    p.step = cut_of(p.x_rows, p.x_cols, p.small, p.segments, cus, o.batch);
+    const int64_t chunks = o.rows * ((o.width + 7) / 8);
     p.blocks = (int)std::max<int64_t>(1, std::min<int64_t>((chunks + 1023) / 1024, SUM_BLOCKS));
     size_t at = 0;
     auto take = [&](size_t n) {
@@ -428,8 +550,8 @@ Plan plan_of(const wc_orthogonalise_args& o, int cus) {
     p.a = take(each * p.a_plane);
     p.b = take(each * p.a_plane);
     p.sums = take(size_t(o.batch) * p.blocks * 8);
-    p.part = take(std::max({p.gram.bytes(o.batch * p.small * p.small), p.square.bytes(o.batch * p.small * p.small),
-                            p.step.bytes(o.batch * o.rows * o.width)}));
+    const int64_t small = p.narrow ? 0 : o.batch * p.small * p.small;
+    p.part = take(std::max({p.gram.bytes(small), p.square.bytes(small), p.step.bytes(o.batch * o.rows * o.width)}));
     p.bytes = at;
     return p;
 }
@@ -458,9 +580,10 @@ void start(const wc_orthogonalise_args& o, const Plan& p, const Held16& x, hipSt
     double* sums = (double*)((char*)o.workspace + p.sums);
     const dim3 grid((uint32_t)p.blocks, (uint32_t)o.batch);
     k_squares<T><<<grid, 256, 0, s>>>(u, sums);
-    const int64_t chunks = o.rows * (p.pitch / 8);
+    const int64_t chunks = p.x_rows * (p.pitch / 8);
     const dim3 wide((uint32_t)std::min<int64_t>((chunks + 255) / 256, 4096), (uint32_t)o.batch);
-    k_start<T><<<wide, 256, 0, s>>>(u, sums, p.blocks, o.eps, x, 2);
+    if (p.turned) k_start_turned<T><<<wide, 256, 0, s>>>(u, sums, p.blocks, o.eps, x);
+    else k_start<T><<<wide, 256, 0, s>>>(u, sums, p.blocks, o.eps, x, 2);
 }
 
 }  // namespace
@@ -481,7 +604,7 @@ void launch_orthogonalise(const wc_orthogonalise_args& o, int cus, hipStream_t s
     else start<bf16>(o, p, x[0], s);
     if (small_enough(o)) return;
 
-    const bool tall = o.rows > o.width;
+    const bool tall = o.rows > o.width && !p.turned;
     float* part = (float*)(w + p.part);
     for (int k = 0; k < o.steps; k++) {
         const Held16 &from = x[k & 1], &to = x[k + 1 & 1];
@@ -493,22 +616,34 @@ void launch_orthogonalise(const wc_orthogonalise_args& o, int cus, hipStream_t s
         }
         StepEpilogue e = {};
         e.from_planes = e.to_planes = p.planes;
-        // A
-        m.a = m.b = operand(from, p.planes, p.small);
-        m.k = tall ? o.rows : o.width;
-        e.to = a;
-        e.alpha = 1.f / HELD;
-        launch_product<f16>(m, p.gram, !tall, !tall, part, e, s);
-        // b A + c A A
-        m.a = m.b = operand(a, p.planes, p.small);
+        if (p.narrow) {
+            const int64_t fragments = (p.small + 31) / 32;
+            const dim3 grid((uint32_t)(fragments * (fragments + 1) / 2), (uint32_t)o.batch);
+            auto narrow = [&](const NarrowJob& job) {
+                if (p.planes == 1) k_narrow<1><<<grid, NARROW_BLOCK, 0, s>>>(job);
+                else k_narrow<2><<<grid, NARROW_BLOCK, 0, s>>>(job);
+            };
+            narrow({from, p.small, p.x_cols, {}, a, 1.f / HELD, 0.f});
+            narrow({a, p.small, p.small, a, b, o.c / HELD, o.b});
+        } else {
+            // A
+            m.a = m.b = operand(from, p.planes, p.small);
+            m.k = tall ? o.rows : o.width;
+            e.to = a;
+            e.alpha = 1.f / HELD;
+            launch_product<f16>(m, p.gram, !tall, !tall, part, e, s);
+            // b A + c A A
+            m.a = m.b = operand(a, p.planes, p.small);
+            m.k = p.small;
+            e.from = a;
+            e.to = b;
+            e.alpha = o.c / HELD;
+            e.beta = o.b;
+            launch_product<f16>(m, p.square, true, true, part, e, s);
+        }
         m.k = p.small;
-        e.from = a;
-        e.to = b;
-        e.alpha = o.c / HELD;
-        e.beta = o.b;
-        launch_product<f16>(m, p.square, true, true, part, e, s);
         // a X + B X, or X B
-        const Operand16 ob = operand(b, p.planes, p.small), ox = operand(from, p.planes, tall ? o.rows : o.width);
+        const Operand16 ob = operand(b, p.planes, p.small), ox = operand(from, p.planes, tall ? o.rows : p.x_cols);
         m.a = tall ? ox : ob;
         m.b = tall ? ob : ox;
         e.from = from;
@@ -516,7 +651,7 @@ void launch_orthogonalise(const wc_orthogonalise_args& o, int cus, hipStream_t s
         e.from_planes = e.to_planes = 2;
         e.alpha = 1.f / HELD;
         e.beta = o.a;
-        if (k + 1 == o.steps) {
+        if (k + 1 == o.steps && !p.turned) {
             e.alpha *= o.scale / HELD;
             e.beta *= o.scale / HELD;
             e.out = o.out;
@@ -525,6 +660,16 @@ void launch_orthogonalise(const wc_orthogonalise_args& o, int cus, hipStream_t s
             e.out_batch = o.out_batch;
         }
         launch_product<f16>(m, p.step, true, tall, part, e, s);
+    }
+    if (p.turned) {
+        const int64_t chunks = o.rows * ((o.width + 7) / 8);
+        const dim3 grid((uint32_t)std::min<int64_t>((chunks + 255) / 256, 4096), (uint32_t)o.batch);
+        auto finish = [&](auto* out) {
+            k_finish_turned<<<grid, 256, 0, s>>>(x[o.steps & 1], o.rows, o.width, o.scale / HELD, out, o.out_stride, o.out_batch);
+        };
+        if (o.out_dtype == WC_DTYPE_F32) finish((float*)o.out);
+        else if (o.out_dtype == WC_DTYPE_F16) finish((f16*)o.out);
+        else finish((bf16*)o.out);
     }
 }
 
