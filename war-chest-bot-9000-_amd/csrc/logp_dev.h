@@ -253,8 +253,7 @@ struct LogpRows {
 // A chunk's share, for the rows that have several.
 struct ChunkPart {
     Part p;
-    float before;
-    float pad;
+    int32_t before, pad;
 };
 
 // A row's outputs from its statistics: what the alternatives need in every thread, and written by one.
@@ -378,7 +377,7 @@ __global__ __launch_bounds__(G > 64 ? G : LOGP_BLOCK, G > 256 ? 4 : 1) void k_lo
     }
     float fix = 0.f, log_s = 0.f;
     if constexpr (CHUNKS) {
-        if (lane == 0) parts[unit] = {p, sums[2], 0.f};
+        if (lane == 0) parts[unit] = {p, (int32_t)sums[2], 0};
     } else if (there) {
         row_out(o, in.rate, r, p, mine, (int)sums[2], on, lane == 0, &fix, &log_s);
     }
@@ -428,7 +427,7 @@ __global__ __launch_bounds__(LOGP_BLOCK) void k_logp_join(Rows<T> in, LogpRows o
     if (read && o.tokens && (!in.legal || in.legal[r * in.legal_stride + a])) v = (float)in.x[r * in.x_stride + a];
     // a chunk's list is in order: its head is its largest
     const Pick* lists = picks + r * o.splits * o.top;
-    ChunkPart mine = {{-INFINITY, 0.f, 0.f, 0.f, -INFINITY, 0.f}, 0.f, 0.f};
+    ChunkPart mine = {{-INFINITY, 0.f, 0.f, 0.f, -INFINITY, 0.f}, 0, 0};
     float own = -INFINITY;
     if (read)
         for (int k = t; k < o.splits; k += LOGP_BLOCK) {
@@ -454,7 +453,7 @@ __global__ __launch_bounds__(LOGP_BLOCK) void k_logp_join(Rows<T> in, LogpRows o
     }
     const bool on = read && counts(mine.p);
     float fix = 0.f, log_s = 0.f;
-    row_out(o, in.rate, r, mine.p, v, (int)mine.before, on, t == 0, &fix, &log_s);
+    row_out(o, in.rate, r, mine.p, v, mine.before, on, t == 0, &fix, &log_s);
     if (!o.top) return;
     top_of<LOGP_BLOCK>(
         on ? own : -INFINITY, on ? mine.p.m : -INFINITY, o.top, t, team, candidates,

@@ -357,11 +357,9 @@ __global__ __launch_bounds__(SMALL_BLOCK, 2) void k_newton_small(Update<T> u, wc
         __syncthreads();
         // X' = a X + B X
         each([&](f32x16& d, int i0, int j0) {
+            const f32x16 e = sum_of(s.mp, f32x16{}, ByRows(a, s.pa, i0, lane), ByColumns(x, s.px, j0, lane));
 #pragma unroll
-            for (int k = 0; k < 16; k++) d[k] *= HELD * o.a;
-            d = sum_of(s.mp, d, ByRows(a, s.pa, i0, lane), ByColumns(x, s.px, j0, lane));
-#pragma unroll
-            for (int k = 0; k < 16; k++) d[k] *= 1.f / HELD;
+            for (int k = 0; k < 16; k++) d[k] = o.a * d[k] + e[k] * (1.f / HELD);
         });
         __syncthreads();
         if (step + 1 == o.steps) break;

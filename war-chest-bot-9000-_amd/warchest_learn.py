@@ -907,7 +907,7 @@ def token_logp_objective(logits, tokens, *, legal=None, inv_temperature=1.0, top
 
 class Muon(torch.optim.Optimizer):
     """Momentum whose update's singular values are brought towards 1 (orthogonalise), for weights of two dimensions, or
-    three (a stack of them). Weights of one shape and type are updated together. The step is lr max(1, out / in)^(1/2)
+    three (a stack of them). Weights of one shape and type are updated together; momentum is kept in float32. The step is lr max(1, out / in)^(1/2)
     for a weight [in, out]; weight_decay is decoupled. dtype: the type that the update is computed to."""
 
     def __init__(self, params, lr=0.02, momentum=0.95, nesterov=True, weight_decay=0.0, steps=5, dtype=torch.bfloat16):
@@ -931,10 +931,10 @@ class Muon(torch.optim.Optimizer):
                     continue
                 state = self.state[p]
                 if "momentum" not in state:
-                    state["momentum"] = torch.zeros_like(p)
-                held = state["momentum"]
-                held.mul_(group["momentum"]).add_(p.grad)
-                update = p.grad.add(held, alpha=group["momentum"]) if group["nesterov"] else held
+                    state["momentum"] = torch.zeros_like(p, dtype=torch.float32, memory_format=torch.contiguous_format)
+                held, g = state["momentum"], p.grad.float()
+                held.mul_(group["momentum"]).add_(g)
+                update = g.add(held, alpha=group["momentum"]) if group["nesterov"] else held
                 same.setdefault((p.shape, p.dtype, p.device), []).append((p, update))
             for (shape, _, _), pairs in same.items():
                 updates = torch.stack([u for _, u in pairs]) if len(pairs) > 1 else pairs[0][1].contiguous()
