@@ -67,7 +67,8 @@ struct TileShape {
     static constexpr int TILE = 64 * F, SIDE = TILE * 2 * STEP;
     static constexpr int LDS = (A_BUFFERS + B_BUFFERS) * SIDE;
     static constexpr int PARTS = 2 * F;  // a wavefront's loads of one operand's tile
-    // Where rows are on k: 64-byte units a row, exchanged so that the four rows of a transposing read lie in different
+    // Sixteen lanes' reads of 16 bytes are taken together, 256 bytes: an INNER row's 16-byte units are exchanged by its pair
+    // of rows modulo 8. Where rows are on k: 64-byte units a row, exchanged so that the four rows of a transposing read lie in different
     // banks. A pitch of an odd number of 128 bytes puts rows 0 and 1 there by itself.
     static __device__ __forceinline__ int turn(int row) { return F & 1 ? (row >> 1) & 1 : row & 3; }
 };
@@ -93,7 +94,7 @@ struct Fetch {
             const int g = first + 64 * k;
             if (INNER) {
                 // past the last row any row will do: its products are not stored
-                at[k] = (uint32_t)min(g / 8, beyond - 1) * pitch + 16 * ((g % 8) ^ (g / 8 & 7));
+                at[k] = (uint32_t)min(g / 8, beyond - 1) * pitch + 16 * ((g % 8) ^ (g / 16 & 7));
             } else {
                 const int row = g / (8 * F), chunk = (g % (8 * F)) ^ (S::turn(row) << 2);
                 at[k] = (uint32_t)row * pitch + (8 * chunk < beyond ? 16 * chunk : 0);
@@ -117,7 +118,7 @@ struct Fetch {
     // The first of k that load k brings.
     __device__ __forceinline__ int k_of(int k) const {
         const int g = first + 64 * k;
-        return INNER ? 8 * ((g % 8) ^ (g / 8 & 7)) : g / (8 * F);
+        return INNER ? 8 * ((g % 8) ^ (g / 16 & 7)) : g / (8 * F);
     }
     // Load k of the step, to the wavefront's place. ENDS: what lies at or past `there` of the step's k is read from zeros.
     template <bool ENDS>
@@ -138,7 +139,7 @@ struct Reads {
     __device__ __forceinline__ void set(int first, int lane) {
         if (INNER) {
             const int row = first + (lane & 31);
-            at[0] = row * 2 * STEP + 16 * ((lane >> 5) ^ (row & 7));
+            at[0] = row * 2 * STEP + 16 * ((lane >> 5) ^ (row >> 1 & 7));
         } else {
             const int row = 8 * (lane >> 5) + ((lane & 15) >> 2);
 #pragma unroll
