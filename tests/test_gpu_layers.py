@@ -552,3 +552,68 @@ def test_token_logp_objective_and_its_graph():
         torch.cuda.synchronize()
         for a, b in zip(held, step()):
             assert torch.equal(a, b)
+
+
+# ------------------------------------------------------------------ far places
+
+def far(x, stride):
+    """x on the device with rows `stride` elements apart; what lies between is not written."""
+    buf = torch.empty(len(x) * stride, dtype=x.dtype, device=DEV)
+    v = buf.view(len(x), stride)[:, : x.shape[1]]
+    v.copy_(x)
+    return v
+
+
+@pytest.mark.parametrize("stride", [4_000_000, 4_000_004])
+def test_linear_with_rows_whose_offsets_pass_32_bits(stride):
+    """2.4e9 elements from the first row to the last: read where they lie (whole 16 bytes), and copied."""
+    say(f"case linear: row stride {stride}")
+    k, d = layer_inputs(600, 72, 40, torch.bfloat16, 41)
+    v = {n: to(t) for n, t in k.items()}
+    x = far(k["x"], stride)
+    got = wl.linear(x, v["weight"], v["bias"], act="gelu", residual=v["residual"], keep=True)
+    check_forward(got, k, "gelu")
+    check_backward(wl.linear_backward(to(d), x, v["weight"], got.pre, act="gelu", bias=True), d, k, got.pre.cpu(), "gelu")
+    few = far(k["x"][:2], 2_200_000_000)
+    check_forward(wl.linear(few, v["weight"], v["bias"]), {n: t[:2] if n in ("x",) else t if n != "residual" else None
+                                                           for n, t in k.items()}, "none")
+
+
+def test_linear_whose_result_passes_32_bits():
+    """1,100,000 x 2,048: the last rows, and the gradients' against the first thousand rows alone."""
+    say("case linear: 1,100,000 x 16 x 2,048")
+    k, _ = layer_inputs(300, 16, 2048, torch.bfloat16, 42, residual=False)
+    x = to(k["x"]).repeat(1_100_000 // 300 + 1, 1)[:1_100_000]
+    w, b = to(k["weight"]), to(k["bias"])
+    got = wl.linear(x, w, b, act="silu", keep=True)
+    at = torch.tensor([0, 299, 1_048_576, 1_099_999])
+    part = {"x": x[at.to(DEV)].cpu(), "weight": k["weight"], "bias": k["bias"], "residual": None}
+    check_forward(wl.Linear(got.out[at.to(DEV)], got.pre[at.to(DEV)]), part, "silu")
+    back = wl.linear_backward(got.out, x, w, got.pre, act="silu", d_weight=False)
+    check_backward(wl.LinearGrads(back.x[at.to(DEV)], None, None), got.out[at.to(DEV)].cpu(), part, got.pre[at.to(DEV)].cpu(), "silu")
+
+
+def test_token_logp_with_rows_whose_offsets_pass_32_bits():
+    say("case logp: far rows")
+    for vocab in (300, 30000):
+        k, d1, d2 = logp_inputs(40, vocab, torch.float16, vocab, True)
+        v = {n: to(t) for n, t in k.items()}
+        base = wl.token_logp(**v, top=4)
+        x, on = far(k["logits"], 60_000_000), far(k["legal"], 60_000_000)
+        got = wl.token_logp(x, v["tokens"], legal=on, top=4)
+        for one, two in zip(got, base):
+            assert torch.equal(one, two)
+        want = wl.token_logp_backward(to(d1), to(d2), v["logits"], v["tokens"], base.stats, legal=v["legal"])
+        wl.token_logp_backward(to(d1), to(d2), x, v["tokens"], got.stats, legal=on, grad=x)
+        assert torch.equal(x, want)
+
+
+def test_orthogonalise_with_matrices_whose_offsets_pass_32_bits():
+    say("case orthogonalise: far matrices")
+    for shape in ((3, 40, 60), (3, 140, 200), (2, 600, 700)):
+        u = torch.randn(*shape, generator=gen(7))
+        buf = torch.empty(shape[0] * 1_200_000_000, dtype=torch.float32, device=DEV)
+        v = torch.as_strided(buf, shape, (1_200_000_000, 1_000_001, 1))
+        v.copy_(u)
+        assert torch.equal(wl.orthogonalise(v), wl.orthogonalise(to(u)))
+        del buf, v
