@@ -171,3 +171,19 @@ def test_the_reference_orthogonalise_acts_on_singular_values():
         for _ in range(5):
             t = 3.4445 * t - 4.7750 * t ** 3 + 2.0315 * t ** 5
         torch.testing.assert_close(R.orthogonalise(x), (u * t) @ v, rtol=0, atol=1e-5)  # float32 coefficients: 1e-7 each
+
+
+def test_muon_keeps_its_momentum_in_float32_over_a_checkpoint():
+    """torch casts what it loads to the parameter's type: of a bf16 weight's momentum 16 bits would be lost."""
+    def optimiser():
+        w = [torch.nn.Parameter(torch.zeros(3, 4, dtype=torch.bfloat16)), torch.nn.Parameter(torch.zeros(5, 4))]
+        return w, wl.Muon(w)
+
+    (a, b), one = optimiser()
+    one.state[a]["momentum"] = torch.randn(3, 4, dtype=torch.float32)
+    held = one.state_dict()
+    (c, d), two = optimiser()
+    two.load_state_dict(held)
+    got = two.state[c]["momentum"]
+    assert got.dtype is torch.float32 and torch.equal(got, one.state[a]["momentum"])
+    assert got.data_ptr() != one.state[a]["momentum"].data_ptr() and not two.state[d]

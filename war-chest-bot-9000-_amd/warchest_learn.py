@@ -918,6 +918,15 @@ class Muon(torch.optim.Optimizer):
                 if p.dim() not in (2, 3):
                     _fail(f"a weight of shape {tuple(p.shape)}: two or three dimensions are expected")
 
+    def load_state_dict(self, state_dict):
+        super().load_state_dict(state_dict)
+        # which casts what it loads to the weight's type
+        order = [i for group in state_dict["param_groups"] for i in group["params"]]
+        for i, p in zip(order, (p for group in self.param_groups for p in group["params"])):
+            if "momentum" in self.state.get(p, ()):
+                held = state_dict["state"][i]["momentum"]
+                self.state[p]["momentum"] = held.to(device=p.device, dtype=torch.float32, copy=True)
+
     @torch.no_grad()
     def step(self, closure=None):
         loss = None
