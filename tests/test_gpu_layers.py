@@ -617,3 +617,56 @@ def test_orthogonalise_with_matrices_whose_offsets_pass_32_bits():
         v.copy_(u)
         assert torch.equal(wl.orthogonalise(v), wl.orthogonalise(to(u)))
         del buf, v
+
+
+# ---------------------------------------------- more than one launch's threads
+
+def test_linear_of_more_rows_than_a_launch_has_threads_for_in_small_tiles():
+    """2^30 rows in tiles of 64 would be 2^32 threads. One row again and again: every result is the first's."""
+    say("case linear: 1,073,741,894 x 8 x 1")
+    rows = 2 ** 30 + 70
+    k, d = layer_inputs(1, 8, 1, torch.bfloat16, 43, residual=False)
+    v = {n: to(t) for n, t in k.items()}
+    got = wl.linear(v["x"].expand(rows, -1), v["weight"], v["bias"], act="silu").out
+    check_forward(wl.Linear(got[-1:], None), k, "silu")
+    assert got.min() == got.max() == got[0, 0]
+    del got
+    grad = wl.linear_backward(to(d).expand(rows, -1), v["x"].expand(rows, -1), v["weight"], d_weight=False).x
+    within(grad[-1:], d.double() @ k["weight"].double().t(), 2.0 ** -7 * (d.double() @ k["weight"].double().t()).abs(), "d_x")
+    for part in grad.split(2 ** 27):
+        assert torch.equal(part[:1], part[-1:]) and bool((part.amin(0) == part.amax(0)).all())
+
+
+@pytest.mark.parametrize("rows,vocab", [(2 ** 22 + 3, 12), (2 ** 22 // 5 + 3, 70000)])
+def test_token_logp_of_more_rows_than_one_launch_takes(rows, vocab):
+    """The rows behind the first launch's have their own tokens, masks and gradients."""
+    say(f"case logp: {rows} x {vocab}")
+    k, d1, d2 = logp_inputs(6, vocab, torch.bfloat16, vocab, False)
+    on = torch.rand(6, vocab, generator=gen(1)) < 0.5
+    on[torch.arange(6), k["tokens"]] = True
+    x, a, legal = to(k["logits"]), to(k["tokens"]), to(on)
+    want = wl.token_logp(x[:1].expand(6, -1), a, legal=legal[:1].expand(6, -1), top=3)
+    last = torch.arange(rows, device=DEV) % 6
+    got = wl.token_logp(x[:1].expand(rows, -1), a[last], legal=legal[:1].expand(rows, -1), top=3)
+    for n in ("logp", "rank", "top_index", "entropy", "top_logp"):
+        one, two = getattr(got, n), getattr(want, n)[last]
+        if n in ("rank", "top_index"):
+            assert torch.equal(one, two), n
+        else:  # another cut of the row: the sums' own tolerance
+            assert bool(((one - two).abs().nan_to_num(0.0) <= 4e-5 * two.abs().clamp(min=1)).all()), n
+            assert torch.equal(one.isinf(), two.isinf())
+    if vocab < 100:
+        grad = wl.token_logp_backward(to(d1)[last], to(d2)[last], x[:1].expand(rows, -1), a[last], got.stats,
+                                      legal=legal[:1].expand(rows, -1))
+        few = wl.token_logp_backward(to(d1), to(d2), x[:1].expand(6, -1), a, want.stats, legal=legal[:1].expand(6, -1))
+        assert torch.equal(grad, few[last])
+
+
+@pytest.mark.parametrize("shape", [(2050, 1, 4104), (2050, 130, 132)])
+def test_orthogonalise_of_more_matrices_than_one_launch_takes(shape):
+    say(f"case orthogonalise: {shape}")
+    at = [0, 1, 2046, 2047, 2048, 2049]
+    u = torch.randn(*shape, generator=gen(44))
+    check_ortho(wl.orthogonalise(to(u))[at], u[at], u.dtype)
+    v = to(u)[:, :, : shape[2] - 1]
+    check_ortho(wl.orthogonalise(v, dtype=torch.bfloat16)[at], u[at][:, :, : shape[2] - 1], torch.bfloat16)

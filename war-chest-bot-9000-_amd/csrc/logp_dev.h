@@ -571,10 +571,11 @@ Rows<T> logp_rows(const void* logits, int64_t stride, const uint8_t* legal, int6
             bits, 1.f};
 }
 
+// Rows of a launch, which holds fewer than 2^32 threads: at most 512 a row or chunk.
+inline int64_t rows_at_once(int64_t splits) { return std::max<int64_t>(1, (int64_t(1) << 22) / splits); }
+
 template <class T>
-void logp(const wc_logp_args& a, int cus, hipStream_t s) {
-    if (!a.rows) return;
-    const LogpPlan p = logp_plan<T>(a.rows, a.vocab, a.top, cus);
+void logp_of(const wc_logp_args& a, const LogpPlan& p, hipStream_t s) {
     const Rows<T> in = logp_rows<T>(a.logits, a.logits_stride, a.legal, a.legal_stride, a.vocab, a.inv_temperature,
                                     a.index_bits);
     LogpRows o = {a.rows, a.tokens, a.top, p.splits, 0, a.logp, a.entropy, a.rank, a.top_logp, a.top_index,
@@ -607,8 +608,25 @@ void logp(const wc_logp_args& a, int cus, hipStream_t s) {
 }
 
 template <class T>
-void logp_back(const wc_logp_back_args& a, hipStream_t s) {
-    if (!a.rows) return;
+void logp(const wc_logp_args& a, int cus, hipStream_t s) {
+    const LogpPlan p = logp_plan<T>(a.rows, a.vocab, a.top, cus);
+    wc_logp_args o = a;
+    for (int64_t lo = 0; lo < a.rows; lo += o.rows) {
+        o.rows = std::min(a.rows - lo, rows_at_once(p.splits));
+        o.logits = (const T*)a.logits + lo * a.logits_stride;
+        if (a.legal) o.legal = a.legal + lo * a.legal_stride;
+        if (a.tokens) o.tokens = (const char*)a.tokens + lo * (a.index_bits / 8);
+        if (a.logp) o.logp = a.logp + lo;
+        if (a.rank) o.rank = a.rank + lo;
+        o.entropy = a.entropy + lo;
+        if (a.top) o.top_logp = a.top_logp + lo * a.top, o.top_index = a.top_index + lo * a.top;
+        if (a.stats) o.stats = a.stats + 4 * lo;
+        logp_of<T>(o, p, s);
+    }
+}
+
+template <class T>
+void logp_back_of(const wc_logp_back_args& a, hipStream_t s) {
     const Rows<T> in = logp_rows<T>(a.logits, a.logits_stride, a.legal, a.legal_stride, a.vocab, a.inv_temperature,
                                     a.index_bits);
     constexpr int64_t E = EACH<T>, CHUNK_COLUMNS = LOGP_BLOCK * E * 8;
@@ -625,6 +643,23 @@ void logp_back(const wc_logp_back_args& a, hipStream_t s) {
         k_logp_back<T, g(), nv()><<<dim3((uint32_t)((a.rows * splits + per - 1) / per)), LOGP_BLOCK, 0, s>>>(
             in, o, a.d_logp, a.d_entropy, (T*)a.grad, a.grad_stride);
     });
+}
+
+template <class T>
+void logp_back(const wc_logp_back_args& a, hipStream_t s) {
+    const int64_t most = rows_at_once((a.vocab + LOGP_BLOCK * EACH<T> * 8 - 1) / (LOGP_BLOCK * EACH<T> * 8));
+    wc_logp_back_args o = a;
+    for (int64_t lo = 0; lo < a.rows; lo += o.rows) {
+        o.rows = std::min(a.rows - lo, most);
+        o.logits = (const T*)a.logits + lo * a.logits_stride;
+        if (a.legal) o.legal = a.legal + lo * a.legal_stride;
+        if (a.tokens) o.tokens = (const char*)a.tokens + lo * (a.index_bits / 8);
+        o.stats = a.stats + 4 * lo;
+        if (a.d_logp) o.d_logp = a.d_logp + lo;
+        if (a.d_entropy) o.d_entropy = a.d_entropy + lo;
+        o.grad = (T*)a.grad + lo * a.grad_stride;
+        logp_back_of<T>(o, s);
+    }
 }
 
 }  // namespace

@@ -563,6 +563,10 @@ Operand16 operand(const Held16& h, int planes, int64_t outer) {
     return o;
 }
 
+// Matrices of a launch, unless each is a workgroup's: 2^20 elements in a row are 2^12 tiles of 256, and a launch holds
+// fewer than 2^24 workgroups of 256.
+constexpr int64_t MOST_MATRICES = 2048;
+
 bool small_enough(const wc_orthogonalise_args& o) {
     const int64_t small = std::min(o.rows, o.width), large = std::max(o.rows, o.width);
     return small <= 128 && large <= 4096 && SmallShape(small, large).fits();
@@ -586,13 +590,18 @@ void start(const wc_orthogonalise_args& o, const Plan& p, const Held16& x, hipSt
 
 }  // namespace
 
-size_t orthogonalise_scratch(const wc_orthogonalise_args& o, int cus) {
-    return small_enough(o) ? 0 : plan_of(o, cus).bytes;
+// The plan of a launch's matrices; the last launch may have fewer.
+static Plan launch_plan(const wc_orthogonalise_args& o, int cus) {
+    wc_orthogonalise_args some = o;
+    some.batch = std::min(o.batch, MOST_MATRICES);
+    return plan_of(some, cus);
 }
 
-void launch_orthogonalise(const wc_orthogonalise_args& o, int cus, hipStream_t s) {
-    if (!o.batch) return;
-    const Plan p = plan_of(o, cus);
+size_t orthogonalise_scratch(const wc_orthogonalise_args& o, int cus) {
+    return small_enough(o) ? 0 : launch_plan(o, cus).bytes;
+}
+
+static void orthogonalise(const wc_orthogonalise_args& o, const Plan& p, hipStream_t s) {
     char* w = (char*)o.workspace;
     Held16 x[2], a = {(f16*)(w + p.a), p.pitch_small, p.a_plane, p.a_plane * p.planes}, b = a;
     b.p = (f16*)(w + p.b);
@@ -668,6 +677,19 @@ void launch_orthogonalise(const wc_orthogonalise_args& o, int cus, hipStream_t s
         if (o.out_dtype == WC_DTYPE_F32) finish((float*)o.out);
         else if (o.out_dtype == WC_DTYPE_F16) finish((f16*)o.out);
         else finish((bf16*)o.out);
+    }
+}
+
+void launch_orthogonalise(const wc_orthogonalise_args& o, int cus, hipStream_t s) {
+    if (!o.batch) return;
+    const Plan p = launch_plan(o, cus);
+    if (small_enough(o)) return orthogonalise(o, p, s);
+    for (int64_t lo = 0; lo < o.batch; lo += MOST_MATRICES) {
+        wc_orthogonalise_args some = o;
+        some.batch = std::min(o.batch - lo, MOST_MATRICES);
+        some.update = (const char*)o.update + lo * o.update_batch * (o.dtype == WC_DTYPE_F32 ? 4 : 2);
+        some.out = (char*)o.out + lo * o.out_batch * (o.out_dtype == WC_DTYPE_F32 ? 4 : 2);
+        orthogonalise(some, p, s);
     }
 }
 

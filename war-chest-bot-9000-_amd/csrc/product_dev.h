@@ -333,6 +333,10 @@ __device__ __forceinline__ void product(const Product& p, const Epilogue& epilog
     float* mine = (float*)(lds + wave * (S::LDS / 4));
     const int64_t wi = i0 + (wave >> 1) * WIDE, wj = j0 + (wave & 1) * WIDE, m_all = p.a.outer, n_all = p.b.outer;
     float* part = p.runs > 1 ? p.part + (int64_t(run) * p.batches + batch) * m_all * n_all : nullptr;
+    auto sync = [] {  // a wavefront's own: its LDS accesses stay in order, and the compiler keeps them so
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+    };
 #pragma unroll
     for (int m = 0; m < F; m++) {
 #pragma unroll
@@ -340,7 +344,7 @@ __device__ __forceinline__ void product(const Product& p, const Epilogue& epilog
 #pragma unroll
             for (int k = 0; k < 16; k++)
                 mine[(8 * (k / 4) + 4 * (lane >> 5) + k % 4) * PITCH + 32 * n + (lane & 31)] = acc[m][n][k];
-        __builtin_amdgcn_wave_barrier();
+        sync();
         // What the epilogue reads for a few rows goes before the first of them is written; where it reads nothing, a row
         // at a time is faster (16,384 x 4,096 x 4,096: 464 and 497 us; with a residual 625 and 587).
         constexpr int TURNS = (32 + ROWS - 1) / ROWS, SOME = sizeof(typename Epilogue::Raw) > 16 && F > 2 ? 2 : 4,
@@ -393,7 +397,7 @@ __device__ __forceinline__ void product(const Product& p, const Epilogue& epilog
                 epilogue(epilogue.raw(batch, i, j, n), batch, i, j, n, v);
             }
         }
-        __builtin_amdgcn_wave_barrier();
+        sync();
     }
 }
 
@@ -461,6 +465,10 @@ __global__ __launch_bounds__(PRODUCT_BLOCK) void k_product_sum(Product p, int64_
 
 inline int64_t up(int64_t n, int64_t to) { return (n + to - 1) / to * to; }
 
+// A launch holds fewer than 2^32 threads: 2^24 workgroups, and two products may share it. Tiles of 256 stay below
+// this for any result that fits the memory.
+constexpr int64_t MOST_TILES = int64_t(1) << 23;
+
 // How a product is cut: tiles of 64 F, and runs along k.
 struct Cut {
     int f, runs, run_steps, steps;
@@ -494,6 +502,7 @@ inline Cut cut_of(int64_t m, int64_t n, int64_t k, int segments, int cus, int64_
         const RoundCost& cost = round_cost(f);
         const int64_t tile = 64 * f, tm = (m + tile - 1) / tile, tn = (n + tile - 1) / tile,
                       tiles = std::max<int64_t>(1, batches * (triangle ? tm * (tm + 1) / 2 : tm * tn));
+        if (f < 4 && tiles > MOST_TILES) break;
         const int64_t slots = int64_t(cost.most) * cus;
         const int64_t most = std::max<int64_t>(1, std::min<int64_t>(steps / 2, 4 * slots / tiles));
         for (int64_t r = 1; r <= 128; r = r < 8 ? r + 1 : r * 5 / 4) {
