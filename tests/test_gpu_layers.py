@@ -670,3 +670,24 @@ def test_orthogonalise_of_more_matrices_than_one_launch_takes(shape):
     check_ortho(wl.orthogonalise(to(u))[at], u[at], u.dtype)
     v = to(u)[:, :, : shape[2] - 1]
     check_ortho(wl.orthogonalise(v, dtype=torch.bfloat16)[at], u[at][:, :, : shape[2] - 1], torch.bfloat16)
+
+
+@pytest.mark.parametrize("act", ["none", "gelu"])
+@pytest.mark.parametrize("rows,width,out", [(64, 2600, 70), (5000, 40, 64), (1024, 512, 512), (1024, 1024, 1024), (70, 4096, 2048),
+                                            (300, 300, 4100), (2500, 1, 1), (40, 9, 6000)])
+def test_linear_in_float32_with_each_gradient_alone(rows, width, out, act):
+    """Straight from memory or in parts, summed in one run or several, by sizes and by what is wanted."""
+    say(f"case linear: {rows} x {width} x {out} f32 {act}, gradients one at a time")
+    k, d = layer_inputs(rows, width, out, torch.float32, rows + width)
+    v = {n: to(t) for n, t in k.items()}
+    for transposed in (False, True):
+        w = v["weight"].t().contiguous().t() if transposed else v["weight"]
+        got = wl.linear(v["x"], w, v["bias"], residual=v["residual"], act=act, keep=True)
+        check_forward(got, k, act)
+        pre = None if got.pre is None else got.pre.cpu()
+        for kw in ({"d_weight": False}, {"d_x": False}, {"d_x": False, "bias": True}, {"d_weight": False, "bias": True},
+                   {"bias": True}, {"d_x": False, "d_weight": False, "bias": True}):
+            back = wl.linear_backward(to(d), v["x"], w, got.pre, act=act, **kw)
+            for value, name in ((back.x, "d_x"), (back.weight, "d_weight")):
+                assert (value is not None) == kw.get(name, True)
+            check_backward(back, d, k, pre, act)

@@ -14,6 +14,7 @@
 #pragma once
 
 #include "ckpt8_dev.h"
+#include "direct_dev.h"
 #include "learn.h"
 #include "product_dev.h"
 
@@ -390,10 +391,70 @@ Few few_of(const wc_linear_args& a, int cus) {
     return f;
 }
 
+// ------------------------------------------------------------------ direct
+
+// A float32 product made straight from memory, in how many runs along k, and the microseconds that it takes (within 20%
+// from 64 x 64 x 64 to 1,024 x 1,024 x 1,024).
+//
+// Microseconds of it and of the tiles of parts: forward 567 x 129 x 128 4.3 and 12.1, 512 x 512 x 512 8.1 and 19, 64 x 4,096 x
+// 4,096 40 and 65, 1,024 x 1,024 x 1,024 37 and 35, 8,192 x 64 x 8,192 265 and 135. Both gradients through a GELU, with
+// the bias's: 8.3 and 23.4, 16.7 and 34.8, 161 and 104, 105 and 61; 4,096 x 128 x 128 18 and 32, 1,024 x 512 x 512 43 and 40.
+// The slopes are computed again in each tile: 1.45 times the products' time.
+struct DirectCut {
+    int runs;
+    int64_t run;
+    double us;
+
+    size_t bytes(int64_t n) const { return runs > 1 ? pad256(size_t(runs) * n * 4) : 0; }
+};
+
+inline DirectCut direct_cut(int64_t m, int64_t n, int64_t k, bool slopes, int cus) {
+    const int64_t tiles = ((m + 31) / 32) * ((n + 31) / 32);
+    DirectCut best = {1, k, -1};
+    for (int64_t r = 1; r <= 64; r = r < 4 ? r + 1 : r * 3 / 2) {
+        const int64_t run = std::max<int64_t>(8 * DIRECT_WAVES, up((k + r - 1) / r, 8 * DIRECT_WAVES)),
+                      runs = std::max<int64_t>(1, (k + run - 1) / run);
+        if (r > 1 && (run < 128 || tiles * runs > 2 * cus)) break;
+        const double rounds = double(tiles * runs) / cus, each = 0.0035 + 0.006 * std::max(1.0, rounds),
+                     us = 3.5 + 0.75 * std::max(0.0, rounds - 2.0) + double(std::min(run, k)) * each * (slopes ? 1.45 : 1.0) + (runs > 1 ? 4.5 : 0.0);
+        if (best.us < 0 || us < best.us) best = {(int)runs, run, us};
+    }
+    return best;
+}
+
+inline Direct direct_of(const DirectSide& a, const DirectSide& b, int64_t k, int act, const DirectCut& cut, float* part, float* sums) {
+    const int64_t tiles_n = (b.outer + 31) / 32;
+    return {a, b, k, cut.run, tiles_n, act, cut.runs, (unsigned)(((a.outer + 31) / 32) * tiles_n * cut.runs), part, sums};
+}
+
+// What adds the runs' products.
+inline Product direct_parts(const Direct& d) {
+    Product m = {};
+    m.a.outer = d.a.outer;
+    m.b.outer = d.b.outer;
+    m.runs = d.runs;
+    m.batches = 1;
+    m.part = d.part;
+    return m;
+}
+template <class Epilogue>
+void direct_sum(const Direct& d, const Epilogue& e, hipStream_t s) {
+    if (d.runs <= 1) return;
+    const Product m = direct_parts(d);
+    k_product_sum<<<dim3((uint32_t)((sum_chunks(m) + 63) / 64)), PRODUCT_BLOCK, 0, s>>>(m, sum_chunks(m), e);
+}
+
+// What the other way costs: its launches and steps at the sizes in question, and the copies in parts of so many elements.
+inline bool direct_pays(double us, int products, double copied) {
+    return us < (products > 1 ? 30.0 : 25.0) + copied * 10 / 4.5e6;
+}
+
 // ------------------------------------------------------------------ forward
 
 struct LinearPlan {
     Few few;
+    bool direct;
+    DirectCut one;
     Laid x, w;
     Cut cut;
     int64_t k;
@@ -408,6 +469,12 @@ LinearPlan linear_plan(const wc_linear_args& a, int cus) {
     p.few = few_of<T>(a, cus);
     if (p.few.is) {
         p.bytes = p.few.runs > 1 ? pad256(size_t(p.few.runs) * a.rows * a.out * 4) : 0;
+        return p;
+    }
+    if (parts > 1) p.one = direct_cut(a.rows, a.out, a.width, false, cus);
+    p.direct = parts > 1 && direct_pays(p.one.us, 1, double(a.rows + a.out) * a.width);
+    if (p.direct) {
+        p.bytes = p.one.bytes(a.rows * a.out);
         return p;
     }
     p.x = laid<T>(a.x, a.x_stride, a.rows, a.width);
@@ -459,6 +526,16 @@ void linear(const wc_linear_args& a, int cus, hipStream_t s) {
             k_product_sum<<<dim3((uint32_t)((chunks + 63) / 64)), PRODUCT_BLOCK, 0, s>>>(m, chunks, e);
         }
         return;
+    }
+    if constexpr (sizeof(T) == 4) {
+        if (p.direct) {
+            const Direct d = direct_of({(const float*)a.x, a.x_stride, a.rows}, {(const float*)a.weight, a.weight_stride, a.out}, a.width, 0,
+                                       p.one, (float*)w, nullptr);
+            if (io) k_direct<false><<<dim3(d.blocks), DIRECT_BLOCK, 0, s>>>(d, e);
+            else k_direct<true><<<dim3(d.blocks), DIRECT_BLOCK, 0, s>>>(d, e);
+            direct_sum(d, e, s);
+            return;
+        }
     }
     lay<T>(p.x, {a.x, a.x_stride, a.rows, a.width}, p.w,
            {a.weight, a.weight_stride, io ? a.width : a.out, io ? a.out : a.width}, w, cus, s);
@@ -556,7 +633,8 @@ struct LinearBackPlan {
     Cut cut_x, cut_w;
     int64_t out_k, rows_k, per;
     int blocks;
-    bool slope;
+    bool slope, direct;
+    DirectCut one_x, one_w;
     size_t sums, part_x, part, bytes;
     bool together;
 };
@@ -566,6 +644,20 @@ LinearBackPlan linear_back_plan(const wc_linear_back_args& a, int cus) {
     constexpr int parts = Parts<T>::COUNT;
     LinearBackPlan p = {};
     const bool io = a.weight_layout == WC_WEIGHT_IN_OUT;
+    if (parts > 1 && (a.d_weight || (a.d_x && !a.d_bias))) {  // (the bias's alone is column sums, and nothing to multiply)
+        const bool slopes = a.act != WC_ACT_NONE;
+        if (a.d_x) p.one_x = direct_cut(a.rows, a.width, a.out, slopes, cus);
+        if (a.d_weight) p.one_w = direct_cut(a.width, a.out, a.rows, slopes, cus);
+        const double copied = double(a.rows) * a.out + (a.d_x ? double(a.width) * a.out : 0.0) + (a.d_weight ? double(a.rows) * a.width : 0.0);
+        p.direct = direct_pays(p.one_x.us + p.one_w.us, (a.d_x != nullptr) + (a.d_weight != nullptr), copied);
+        if (p.direct) {
+            p.part_x = 0;
+            p.part = p.part_x + p.one_x.bytes(a.rows * a.width);
+            p.sums = p.part + p.one_w.bytes(a.width * a.out);
+            p.bytes = p.sums + p.one_w.bytes(a.out);
+            return p;
+        }
+    }
     p.d = laid<T>(a.d_out, a.d_out_stride, a.rows, a.out);
     if (a.act != WC_ACT_NONE && !p.d.copy) {
         p.d.copy = true;
@@ -629,6 +721,35 @@ void linear_back(const wc_linear_back_args& a, int cus, hipStream_t s) {
     const LinearBackPlan p = linear_back_plan<T>(a, cus);
     char* w = (char*)a.workspace;
     const bool io = a.weight_layout == WC_WEIGHT_IN_OUT, products = a.d_x || a.d_weight;
+    if constexpr (sizeof(T) == 4) {
+        if (p.direct) {
+            const float* z = a.act == WC_ACT_NONE ? nullptr : a.pre;
+            const float* d = (const float*)a.d_out;
+            Direct dx = {}, dw = {};
+            if (a.d_x && a.rows)
+                dx = direct_of({d, a.d_out_stride, a.rows, z, a.pre_stride}, {(const float*)a.weight, a.weight_stride, a.width},
+                               a.out, a.act, p.one_x, (float*)(w + p.part_x), nullptr);
+            if (a.d_weight) {
+                const DirectSide side = {d, a.d_out_stride, a.out, z, a.pre_stride}, x = {(const float*)a.x, a.x_stride, a.width};
+                float* sums = !a.d_bias || p.one_w.runs == 1 ? a.d_bias : (float*)(w + p.sums);
+                dw = direct_of(io ? x : side, io ? side : x, a.rows, a.act, p.one_w, (float*)(w + p.part), sums);
+            }
+            const dim3 grid(dx.blocks + dw.blocks);
+            const auto ex = plain_to<float>(a.d_x, a.d_x_stride), ew = plain_to<float>(a.d_weight, a.d_weight_stride);
+            if (!grid.x) return;
+            if (io) k_direct_back<true><<<grid, DIRECT_BLOCK, 0, s>>>(dx, ex, dw, ew);
+            else k_direct_back<false><<<grid, DIRECT_BLOCK, 0, s>>>(dx, ex, dw, ew);
+            direct_sum(dx, ex, s);
+            if (dw.runs > 1) {
+                const Product m = direct_parts(dw);
+                const uint32_t blocks = (uint32_t)((sum_chunks(m) + 63) / 64);
+                const ColumnSums bias = {dw.sums, a.out, dw.runs, a.d_bias};
+                k_back_sum<<<dim3(blocks + (a.d_bias ? (uint32_t)((a.out + 15) / 16) : 0)), PRODUCT_BLOCK, 0, s>>>(
+                    m, sum_chunks(m), ew, blocks, bias);
+            }
+            return;
+        }
+    }
     if (p.slope) {
         Source d = {};
         if (products && p.d.copy) {
