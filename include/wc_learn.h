@@ -279,10 +279,11 @@ int wc_ckpt_weight_grad(const wc_ckpt_weight_args* a, void* stream);
  * activation and residual in float32, rounded once to y's type. W is width x
  * out (WC_WEIGHT_IN_OUT) or out x width (WC_WEIGHT_OUT_IN, a row an output).
  * pre, where given, gets x W + bias in float32, for the backward pass.
- * 16-bit matrices: products on the matrix cores with float32 sums. float32: as
- * three bf16 parts an element and six products of parts (what is left out is
- * below 2^-25 of a product); an infinite element's row or column of the result is not finite,
- * and may be NaN where its product alone would be infinite.
+ * 16-bit matrices: products on the matrix cores with float32 sums. float32:
+ * small ones as they are, larger ones as three bf16 parts an element and six
+ * products of parts (what is left out is below 2^-25 of a product); there an
+ * infinite element's row or column of the result is not finite, and may be NaN
+ * where its product alone would be infinite.
  * rows below 2^31, width and out at most 2^20. */
 #define WC_WEIGHT_IN_OUT 0
 #define WC_WEIGHT_OUT_IN 1

@@ -691,3 +691,23 @@ def test_linear_in_float32_with_each_gradient_alone(rows, width, out, act):
             for value, name in ((back.x, "d_x"), (back.weight, "d_weight")):
                 assert (value is not None) == kw.get(name, True)
             check_backward(back, d, k, pre, act)
+
+
+def test_linear_in_float32_parts_of_infinities_and_of_the_largest():
+    """Sizes that are taken in parts: as the small ones."""
+    say("case linear: infinities f32, 1,200 x 1,024 x 1,100")
+    k, _ = layer_inputs(1200, 1024, 1100, torch.float32, 8, residual=False)
+    want = wl.linear(*(to(k[n]) for n in ("x", "weight", "bias"))).out
+    x = k["x"].clone()
+    x[3, 5], x[40, 1000] = math.inf, math.nan
+    got = wl.linear(to(x), to(k["weight"]), to(k["bias"])).out
+    assert not got[[3, 40]].isfinite().any()
+    rest = [i for i in range(1200) if i not in (3, 40)]
+    assert torch.equal(got[rest], want[rest])
+    top = torch.finfo(torch.float32).max
+    x = torch.zeros(1200, 1024)
+    x[0, 0], x[1199, 1023] = top, -top
+    w = torch.zeros(1024, 1100)
+    w[0, 7] = w[1023, 1099] = 1.0
+    got = wl.linear(to(x), to(w)).out.cpu()
+    assert got[0, 7] == top and got[1199, 1099] == -top and int((got != 0).sum()) == 2

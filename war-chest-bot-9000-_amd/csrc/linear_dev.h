@@ -10,7 +10,8 @@
 // that of the float32 sums of d_b (1.3e-3 of its norm in bf16).
 //
 // float32 operands are taken as three bf16 parts (8 + 8 + 8 bits), and of their nine products the six that matter:
-// the matrix cores' own float32 rate is a sixteenth of the 16-bit one.
+// the matrix cores' own float32 rate is a sixteenth of the 16-bit one. Small ones, whose launches cost more than their
+// products, are left as they are (direct_dev.h).
 #pragma once
 
 #include "ckpt8_dev.h"
@@ -37,13 +38,16 @@ struct Parts<float> {
 };
 
 // Each part is what is left rounded to bf16; the third is exact, and the products that are left out are below 2^-25 of
-// the whole. A first part that would round past bf16's largest is cut. What an infinity leaves is 0.
+// the whole. A first part that would round past bf16's largest is cut, and the second too: together they are no
+// larger than x, in whatever order they are added. What an infinity leaves is 0.
+__device__ __forceinline__ bf16 cut_bf16(float x) { return __builtin_bit_cast(bf16, (uint16_t)(__float_as_uint(x) >> 16)); }
 __device__ __forceinline__ void parts_of(float x, bf16 (&o)[3]) {
     o[0] = (bf16)x;
-    if (fabsf((float)o[0]) == INFINITY) o[0] = __builtin_bit_cast(bf16, (uint16_t)(__float_as_uint(x) >> 16));
+    const bool past = fabsf((float)o[0]) == INFINITY;
+    if (past) o[0] = cut_bf16(x);
     x -= (float)o[0];
     x = x == x ? x : 0.f;
-    o[1] = (bf16)x;
+    o[1] = past ? cut_bf16(x) : (bf16)x;
     o[2] = (bf16)(x - (float)o[1]);
 }
 
