@@ -13,6 +13,8 @@
 // what is large already. A gradient with three large directions and 256 x 1,024 with 11-bit X comes out 8e-3 off (of its
 // norm; all of it in bf16, 7e-2), with 22-bit X 9e-5; a random matrix 1.7e-3, as much as the result's own rounding.
 // Up to 128 rows or columns (2.7e-3 at 40 x 200) the three products cost next to nothing, and are taken.
+//
+// 4,096 x 4,096 bf16, five steps: 1.57 ms, 867 TFLOP/s of the operations that symmetry leaves, 74% of a large product's rate.
 #include "learn.h"
 #include "product_dev.h"
 
@@ -144,7 +146,8 @@ __global__ __launch_bounds__(256) void k_start(Update<T> u, const double* sums, 
 // A matrix whose X (in the form that is wide: small x large) and A fit in LDS, two parts each, in one launch: a workgroup
 // of eight wavefronts a matrix. Fragments of 32 x 32, of A those on and above the diagonal only. B takes A's place, and X'
 // X's, after a barrier. Vector arithmetic bounds it (splitting results into their parts, addresses): so the parts of eight
-// elements lie beside each other, 16 bytes and 16 bytes, and one address serves both.
+// elements lie beside each other, 16 bytes and 16 bytes, and one address serves both. 8 of 192 x 96, five steps: 45 us,
+// 6.2 a step and 13 to load, norm and store; through memory, 17 launches, 123.
 constexpr int SMALL_BLOCK = 512, SMALL_WAVES = SMALL_BLOCK / 64, SMALL_LDS = 160 * 1024, SMALL_TILES = 6;
 
 struct SmallShape {

