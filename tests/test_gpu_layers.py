@@ -637,6 +637,33 @@ def test_linear_of_more_rows_than_a_launch_has_threads_for_in_small_tiles():
         assert torch.equal(part[:1], part[-1:]) and bool((part.amin(0) == part.amax(0)).all())
 
 
+def test_linear_in_float32_of_more_rows_than_a_launch_has_threads_for():
+    """2^28 rows straight from memory are 2^23 fragments of 512 threads, 2^32. One row again and again, with a residual of
+    its own each; x's gradient alone, and beside the weight's."""
+    say("case linear: 268,435,526 x 64 x 1 f32")
+    rows = 2 ** 28 + 70
+    k, _ = layer_inputs(1, 64, 1, torch.float32, 45, residual=False)
+    v = {n: to(t) for n, t in k.items()}
+    residual = (torch.arange(rows, device=DEV, dtype=torch.int32) % 1024).float()[:, None]
+    got = wl.linear(v["x"].expand(rows, -1), v["weight"], v["bias"], act="silu", residual=residual, keep=True)
+    check_forward(wl.Linear(got.out[:1], got.pre[:1]), k, "silu")
+    assert got.pre.min() == got.pre.max()
+    assert float((got.out - residual - got.out[0]).abs().max()) <= 2.0 ** -13  # half an ulp of 1,025, and of the difference
+    del got, residual
+    say("case linear: 268,435,526 x 1 x 100 f32, x's gradient")
+    k, d = layer_inputs(1, 1, 100, torch.float32, 46)
+    grad = wl.linear_backward(to(d).expand(rows, -1), to(k["x"]).expand(rows, -1), to(k["weight"]), d_weight=False).x
+    check_backward(wl.LinearGrads(grad[-1:], None, None), d, k, None, "none")
+    assert grad.min() == grad.max()
+    del grad
+    say("case linear: 268,435,526 x 32 x 200 f32, both gradients")
+    k, d = layer_inputs(1, 32, 200, torch.float32, 47)
+    back = wl.linear_backward(to(d).expand(rows, -1), to(k["x"]).expand(rows, -1), to(k["weight"]))
+    check_backward(wl.LinearGrads(back.x[-1:], None, None), d, k, None, "none")
+    for part in back.x.split(2 ** 26):
+        assert torch.equal(part[:1], part[-1:]) and bool((part.amin(0) == part.amax(0)).all())
+
+
 @pytest.mark.parametrize("rows,vocab", [(2 ** 22 + 3, 12), (2 ** 22 // 5 + 3, 70000)])
 def test_token_logp_of_more_rows_than_one_launch_takes(rows, vocab):
     """The rows behind the first launch's have their own tokens, masks and gradients."""

@@ -139,6 +139,14 @@ struct LayerEpilogue {
     int64_t y_stride;
     int act;
 
+    // The same from row lo on.
+    LayerEpilogue from(int64_t lo) const {
+        LayerEpilogue e = *this;
+        if (residual) e.residual += lo * residual_stride;
+        if (pre) e.pre += lo * pre_stride;
+        e.y += lo * y_stride;
+        return e;
+    }
     __device__ __forceinline__ bool reads() const { return residual != nullptr; }
     typedef typename Vec8<T>::type Raw;
     __device__ __forceinline__ Raw raw(int, int64_t i, int64_t j, int n) const {
@@ -426,6 +434,11 @@ inline DirectCut direct_cut(int64_t m, int64_t n, int64_t k, bool slopes, int cu
     return best;
 }
 
+// Fragments of a launch, and the rows of a product that they are (width or out is at most 2^20): 2^22 workgroups are 2^31
+// threads, and a launch, which two products may share, holds fewer than 2^32.
+constexpr int64_t MOST_DIRECT = int64_t(1) << 22;
+inline int64_t direct_rows(int64_t n) { return 32 * (MOST_DIRECT / ((n + 31) / 32)); }
+
 inline Direct direct_of(const DirectSide& a, const DirectSide& b, int64_t k, int act, const DirectCut& cut, float* part, float* sums) {
     const int64_t tiles_n = (b.outer + 31) / 32;
     return {a, b, k, cut.run, tiles_n, act, cut.runs, (unsigned)(((a.outer + 31) / 32) * tiles_n * cut.runs), part, sums};
@@ -533,11 +546,16 @@ void linear(const wc_linear_args& a, int cus, hipStream_t s) {
     }
     if constexpr (sizeof(T) == 4) {
         if (p.direct) {
-            const Direct d = direct_of({(const float*)a.x, a.x_stride, a.rows}, {(const float*)a.weight, a.weight_stride, a.out}, a.width, 0,
-                                       p.one, (float*)w, nullptr);
-            if (io) k_direct<false><<<dim3(d.blocks), DIRECT_BLOCK, 0, s>>>(d, e);
-            else k_direct<true><<<dim3(d.blocks), DIRECT_BLOCK, 0, s>>>(d, e);
-            direct_sum(d, e, s);
+            // (runs are of few fragments: all in one launch)
+            const int64_t most = direct_rows(a.out);
+            for (int64_t lo = 0; lo < a.rows; lo += most) {
+                const Direct d = direct_of({(const float*)a.x + lo * a.x_stride, a.x_stride, std::min(most, a.rows - lo)},
+                                           {(const float*)a.weight, a.weight_stride, a.out}, a.width, 0, p.one, (float*)w, nullptr);
+                const auto el = e.from(lo);
+                if (io) k_direct<false><<<dim3(d.blocks), DIRECT_BLOCK, 0, s>>>(d, el);
+                else k_direct<true><<<dim3(d.blocks), DIRECT_BLOCK, 0, s>>>(d, el);
+                direct_sum(d, el, s);
+            }
             return;
         }
     }
@@ -654,7 +672,8 @@ LinearBackPlan linear_back_plan(const wc_linear_back_args& a, int cus) {
         if (a.d_x) p.one_x = direct_cut(a.rows, a.width, a.out, slopes, cus);
         if (a.d_weight) p.one_w = direct_cut(a.width, a.out, a.rows, slopes, cus);
         const double copied = double(a.rows) * a.out + (a.d_x ? double(a.width) * a.out : 0.0) + (a.d_weight ? double(a.rows) * a.width : 0.0);
-        p.direct = direct_pays(p.one_x.us + p.one_w.us, (a.d_x != nullptr) + (a.d_weight != nullptr), copied);
+        p.direct = direct_pays(p.one_x.us + p.one_w.us, (a.d_x != nullptr) + (a.d_weight != nullptr), copied) &&
+                   (!a.d_weight || ((a.width + 31) / 32) * ((a.out + 31) / 32) * p.one_w.runs <= MOST_DIRECT);
         if (p.direct) {
             p.part_x = 0;
             p.part = p.part_x + p.one_x.bytes(a.rows * a.width);
@@ -730,21 +749,30 @@ void linear_back(const wc_linear_back_args& a, int cus, hipStream_t s) {
         if (p.direct) {
             const float* z = a.act == WC_ACT_NONE ? nullptr : a.pre;
             const float* d = (const float*)a.d_out;
-            Direct dx = {}, dw = {};
-            if (a.d_x && a.rows)
-                dx = direct_of({d, a.d_out_stride, a.rows, z, a.pre_stride}, {(const float*)a.weight, a.weight_stride, a.width},
-                               a.out, a.act, p.one_x, (float*)(w + p.part_x), nullptr);
+            Direct dw = {};
             if (a.d_weight) {
                 const DirectSide side = {d, a.d_out_stride, a.out, z, a.pre_stride}, x = {(const float*)a.x, a.x_stride, a.width};
                 float* sums = !a.d_bias || p.one_w.runs == 1 ? a.d_bias : (float*)(w + p.sums);
                 dw = direct_of(io ? x : side, io ? side : x, a.rows, a.act, p.one_w, (float*)(w + p.part), sums);
             }
-            const dim3 grid(dx.blocks + dw.blocks);
-            const auto ex = plain_to<float>(a.d_x, a.d_x_stride), ew = plain_to<float>(a.d_weight, a.d_weight_stride);
-            if (!grid.x) return;
-            if (io) k_direct_back<true><<<grid, DIRECT_BLOCK, 0, s>>>(dx, ex, dw, ew);
-            else k_direct_back<false><<<grid, DIRECT_BLOCK, 0, s>>>(dx, ex, dw, ew);
-            direct_sum(dx, ex, s);
+            const auto ew = plain_to<float>(a.d_weight, a.d_weight_stride);
+            // x's gradient in parts that a launch holds, the weight's beside the first
+            const int64_t rows_x = a.d_x ? a.rows : 0, most = direct_rows(a.width);
+            for (int64_t lo = 0; lo == 0 || lo < rows_x; lo += most) {
+                Direct dx = {};
+                if (rows_x)
+                    dx = direct_of({d + lo * a.d_out_stride, a.d_out_stride, std::min(most, rows_x - lo), z ? z + lo * a.pre_stride : nullptr,
+                                    a.pre_stride},
+                                   {(const float*)a.weight, a.weight_stride, a.width}, a.out, a.act, p.one_x, (float*)(w + p.part_x),
+                                   nullptr);
+                const Direct beside = lo ? Direct{} : dw;
+                const auto ex = plain_to<float>(rows_x ? (float*)a.d_x + lo * a.d_x_stride : nullptr, a.d_x_stride);
+                const dim3 grid(dx.blocks + beside.blocks);
+                if (!grid.x) return;
+                if (io) k_direct_back<true><<<grid, DIRECT_BLOCK, 0, s>>>(dx, ex, beside, ew);
+                else k_direct_back<false><<<grid, DIRECT_BLOCK, 0, s>>>(dx, ex, beside, ew);
+                direct_sum(dx, ex, s);
+            }
             if (dw.runs > 1) {
                 const Product m = direct_parts(dw);
                 const uint32_t blocks = (uint32_t)((sum_chunks(m) + 63) / 64);
