@@ -344,6 +344,28 @@ def test_orthogonalise_types_strides_and_arguments():
     assert torch.equal(wl.orthogonalise(torch.zeros(9, 12, device=DEV)), torch.zeros(9, 12, device=DEV))
 
 
+@pytest.mark.parametrize("shape", [(40, 60), (60, 40), (300, 700), (700, 300), (600, 700), (700, 600), (3, 20, 30)])
+def test_orthogonalise_close_to_what_its_parts_hold(shape):
+    """One element, and so a singular value that is an element of X, A and B: A at 62.41 and the result there, B at -62.
+    X, A and B are held to 2^-22, a product leaves out as much: 62 (3 roundings + X's two + 3 of float32) 2^-22 at most. A
+    bf16 result of more than 128 rows and columns has A, B and X's large part to 2^-11 each."""
+    say(f"case orthogonalise: {shape} near the largest that is held")
+    u = torch.zeros(shape)
+    at = (*(n // 2 for n in shape),) if len(shape) == 2 else (1, 7, 29)
+    u[at] = 3.0
+    for out in (torch.float32, torch.bfloat16):
+        one = out == torch.bfloat16 and min(shape[-2:]) > 128
+        for coefficients, steps, want in (((7.9, 0.0, 0.0), 2, 62.41), ((63.0, -62.0, 0.0), 1, 1.0)):
+            got = wl.orthogonalise(to(u), coefficients=coefficients, steps=steps, eps=0.0, dtype=out).cpu().double()
+            off = 62 * (3 * 2.0 ** -11 if one and steps == 1 else 12 * 2.0 ** -22) + R.U[out] * want
+            assert abs(float(got[at]) - want) <= off, (coefficients, out, float(got[at]))
+            got[at] = 0
+            if len(shape) == 2:
+                assert not got.any()
+            else:
+                assert got[[0, 2]].isnan().all() and not got[1].any()  # 0 / 0, eps being 0
+
+
 def test_orthogonalise_keeps_matrices_apart():
     """A NaN in one matrix of a batch makes that one NaN and leaves the others as they are alone."""
     u = torch.randn(3, 24, 40, generator=gen(4))

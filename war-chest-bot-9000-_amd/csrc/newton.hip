@@ -4,9 +4,10 @@
 //
 // A and A A are symmetric: only tiles on and above the diagonal are computed, and written twice.
 //
-// X, A and B are held as sums of two f16 (22 bits), times 2^10: no element of X or A is larger than the largest singular
-// value and its square, so that nothing overflows below 60, and an element of 2^-13 still has all its bits. A product is
-// then three matrix products: the one of the two small parts is left out.
+// X, A and B are held as sums of two f16 (22 bits), times 2^10, so that an element of 2^-13 still has all its bits. No
+// element of X, A or B is larger than its largest singular value, s, s^2 and |b s^2 + c s^4|: below 63 each fits (f16 ends
+// at 65504). A is what passes it first, at s = 7.9, or B, where the coefficients are large. A product is then three matrix
+// products: the one of the two small parts is left out.
 //
 // For a bf16 result one product of the large parts is enough, with A and B in one f16 (11 bits), but X stays in 22: its
 // rounding would fall on every direction, on small singular values that grow 500-fold too, where A's and B's fall on

@@ -597,7 +597,9 @@ def orthogonalise(update, *, steps=5, coefficients=NEWTON_SCHULZ, eps=1e-7, scal
     """update [rows, width] or [batch, rows, width] with its singular values brought towards 1, times scale
     (wc_orthogonalise): X = update / (its Frobenius norm + eps), then `steps` times X = a X + (b A + c A A) X with
     A = X X^T (or the transposed form) and (a, b, c) = coefficients. dtype: the result's, float32, float16 or bfloat16
-    (the default is the update's); a bfloat16 result takes a third of the others' products. Returns a contiguous tensor."""
+    (the default is the update's); a bfloat16 result takes a third of the others' products, in 11 bits where they have 22
+    (float32 and a cast keep these). Coefficients under which a singular value s of any step has s^2 or |b s^2 + c s^4| past
+    63, or the result one past 63 before scale, give infinities or NaN. Returns a contiguous tensor."""
     device = _device(update, "update")
     code = _dtype(update, "update")
     if update.dim() not in (2, 3) or 0 in update.shape[-2:]:
