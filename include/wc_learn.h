@@ -15,6 +15,8 @@
  *
  * Matrices are row-major with unit column stride; row strides are in elements,
  * may be 0 (one row broadcast) for inputs and at least the width for outputs.
+ * An output that may be one of the inputs itself starts where that starts and has
+ * its row stride; no other output may overlap an input.
  * No alignment beyond the element's own is needed. `bytes` is the size of the
  * structure as the caller compiled it; another size is refused.
  */
@@ -359,7 +361,7 @@ typedef struct wc_orthogonalise_args {
     int64_t batch, rows, width; /* batch at most 65535, rows and width 2^20 */
     const void* update;
     int64_t update_stride, update_batch; /* elements from row to row, from matrix to matrix */
-    void* out;                  /* may be update itself */
+    void* out;                  /* may be update itself: one matrix, or of its type and strides */
     int64_t out_stride, out_batch;
     float a, b, c, eps, scale;
     int32_t pad;

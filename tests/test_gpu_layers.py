@@ -241,6 +241,27 @@ def test_linear_is_the_same_from_run_to_run_and_in_a_graph():
             assert torch.equal(a, b)
 
 
+@pytest.mark.parametrize("rows,width,out,dtype", [(1, 96, 200, "bf16"), (2, 4096, 40, "f16"), (300, 128, 264, "bf16"),
+                                                  (1030, 520, 776, "f16"), (64, 9000, 72, "bf16"), (70, 50, 90, "f32"),
+                                                  (40, 4096, 40, "f32"), (1201, 1027, 1103, "f32")])
+def test_linear_over_its_residual(rows, width, out, dtype):
+    """y may be the residual itself: one row, split sums, tiles, straight from memory and in parts, as into another matrix."""
+    say(f"case linear: {rows} x {width} x {out} {dtype} over its residual")
+    k, _ = layer_inputs(rows, width, out, TYPES[dtype], 12)
+    for extra in (0, 3):
+        x, w, b = to(k["x"]), to(k["weight"]), to(k["bias"])
+        r = strided(k["residual"], extra)
+        want = wl.linear(x, w, b, act="gelu", residual=r).out
+        need = wl._linear_scratch(0, wl.DTYPES[x.dtype], 0, rows, width, out, width, out, x.data_ptr() % 16 == 0,
+                                  w.data_ptr() % 16 == 0)
+        work = torch.empty(need + 1, dtype=torch.uint8, device=DEV)
+        s = r.stride(0) if rows > 1 else out
+        wl._call("wc_linear", wl._LINEAR.pack(
+            wl._LINEAR.size, 0, wl.DTYPES[x.dtype], wl.DTYPES[x.dtype], 0, rows, width, out, x.data_ptr(), width, w.data_ptr(),
+            out, b.data_ptr(), r.data_ptr(), s, wl.ACTS["gelu"], 0, 0, out, r.data_ptr(), s, work.data_ptr(), need), x.device)
+        assert torch.equal(r, want)
+
+
 def test_linear_refuses_what_does_not_fit():
     x, w = torch.zeros(4, 16, device=DEV), torch.zeros(16, 8, device=DEV)
     for bad, word in ((lambda: wl.linear(x[0], w), "rows x width"), (lambda: wl.linear(x, w[:15]), "weight"),
@@ -364,6 +385,25 @@ def test_orthogonalise_close_to_what_its_parts_hold(shape):
                 assert not got.any()
             else:
                 assert got[[0, 2]].isnan().all() and not got[1].any()  # 0 / 0, eps being 0
+
+
+@pytest.mark.parametrize("shape,out", [((5, 33, 70), "f32"), ((70, 33), "bf16"), ((3, 140, 333), "f32"), ((3, 333, 140), "f32"),
+                                       ((2, 520, 600), "bf16"), ((600, 700), "f32"), ((2050, 1, 4104), "f32")])
+def test_orthogonalise_over_its_update(shape, out):
+    """out may be update itself: of one type and strides, or a single matrix, as into another tensor."""
+    say(f"case orthogonalise: {shape} {out} over its update")
+    batch, rows, width = shape if len(shape) == 3 else (1, *shape)
+    same = TYPES[out] if batch > 1 else torch.float32
+    u = torch.randn(batch, rows, width, generator=gen(13)).to(same).to(DEV)
+    want = wl.orthogonalise(u, dtype=TYPES[out])
+    code, to_code = wl.DTYPES[same], wl.DTYPES[TYPES[out]]
+    need = wl._ortho_scratch(0, code, to_code, batch, rows, width)
+    work = torch.empty(need + 1, dtype=torch.uint8, device=DEV)
+    wl._call("wc_orthogonalise", wl._ORTHO.pack(
+        wl._ORTHO.size, 0, code, to_code, 5, batch, rows, width, u.data_ptr(), width, rows * width, u.data_ptr(), width,
+        rows * width, *wl.NEWTON_SCHULZ, 1e-7, 1.0, 0, work.data_ptr(), need), u.device)
+    got = u if same == TYPES[out] else u.view(-1).view(TYPES[out])[: rows * width].view(1, rows, width)
+    assert torch.equal(got, want)
 
 
 def test_orthogonalise_keeps_matrices_apart():

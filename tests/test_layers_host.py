@@ -111,6 +111,24 @@ def test_refusals_name_their_reason(entry, name, packed, base, edit, word):
     assert word in ww.lib().wc_last_error().decode(), ww.lib().wc_last_error()
 
 
+OVER = 1 << 16  # another address: what is written over itself
+
+
+@pytest.mark.parametrize("entry,packed,fields,edit,allowed", [
+    ("wc_linear", wl._LINEAR, LINEAR, dict(residual=OVER, y=OVER, residual_stride=8, y_stride=9), dict(y_stride=8)),
+    ("wc_linear", wl._LINEAR, LINEAR, dict(residual=OVER, y=OVER, residual_stride=0), dict(rows=1)),
+    ("wc_orthogonalise", wl._ORTHO, ORTHO, dict(update=OVER, out=OVER), dict(out_dtype=0)),
+    ("wc_orthogonalise", wl._ORTHO, ORTHO, dict(update=OVER, out=OVER, out_dtype=0, out_stride=17, out_batch=68), dict(batch=1)),
+    ("wc_orthogonalise", wl._ORTHO, ORTHO, dict(update=OVER, out=OVER, out_dtype=0, out_batch=65), dict(batch=1)),
+    ("wc_token_logp_backward", wl._LOGP_BACK, LOGP_BACK, dict(logits=OVER, grad=OVER, grad_stride=11), dict(grad_stride=10))])
+def test_an_output_over_an_input_has_its_layout(entry, packed, fields, edit, allowed):
+    """Other strides or another type would be written where rows are still to be read: refused. What is allowed passes these
+    checks, and is stopped by the one of the device."""
+    for more, word in ((edit, "itself needs"), ({**edit, **allowed, "device": -1}, "device")):
+        assert wl._entry(entry)(packed.pack(*{**fields, **more}.values()), None) == -1
+        assert word in ww.lib().wc_last_error().decode(), ww.lib().wc_last_error()
+
+
 def test_the_binding_refuses_tensors_that_are_not_on_a_gpu():
     x = torch.zeros(2, 3)
     for call in (lambda: wl.linear(x, x.t()), lambda: wl.linear_backward(x, x, x.t()), lambda: wl.orthogonalise(x),

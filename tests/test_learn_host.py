@@ -82,6 +82,25 @@ WEIGHT = dict(bytes=136, device=0, dtype=1, rows=4, width=40, out=8, act=0, wdty
               exps_stride=2, grad=P, grad_stride=8, weight=P, weight_stride=8, bias=P, work=P, work_bytes=1 << 30)
 
 
+OVER = 1 << 16  # another address: what is written over itself
+
+
+@pytest.mark.parametrize("entry,packed,base,edit,allowed", [
+    ("wc_policy_loss", wl._POLICY, POLICY, dict(logits=OVER, grad=OVER, grad_stride=11), dict(logits_stride=11)),
+    ("wc_policy_loss", wl._POLICY, POLICY, dict(logits=OVER, grad=OVER, logits_stride=0), dict(rows=1)),
+    ("wc_preference_loss", wl._PREFERENCE, PREFERENCE, dict(logits=OVER, grad=OVER, grad_stride=11), dict(logits_stride=11)),
+    ("wc_residual_norm", wl._NORM, NORM, dict(stream=OVER, new=OVER, new_stride=17), dict(stream_stride=17)),
+    ("wc_residual_norm_backward", wl._NORM_BACK, NORM_BACK, dict(d_new=OVER, d_stream=OVER, d_new_stride=17),
+     dict(d_stream_stride=17)),
+    ("wc_ckpt_act_backward", wl._CKPT, CKPT, dict(x=OVER, y=OVER, y_stride=41), dict(x_stride=41))])
+def test_an_output_over_an_input_has_its_row_stride(entry, packed, base, edit, allowed):
+    """At another stride it would be written where rows are still to be read: refused. What is allowed passes these checks,
+    and is stopped by the one of the device."""
+    for more, word in ((edit, "itself needs"), ({**edit, **allowed, "device": -1}, "device")):
+        assert wl._entry(entry)(packed.pack(*{**base, **more}.values()), None) == -1
+        assert word in ww.lib().wc_last_error().decode(), ww.lib().wc_last_error()
+
+
 @pytest.mark.parametrize("entry,packed,base,edit,word", [
     ("wc_policy_loss", wl._POLICY, POLICY, dict(bytes=208), "size"),
     ("wc_policy_loss", wl._POLICY, POLICY, dict(dtype=3), "dtype"),

@@ -41,6 +41,11 @@ struct Check {
         if (stride < 0 || stride > MOST || (written && rows > 1 && stride < width) || (stride && rows > 1 && stride < width))
             is(false, (std::string(name) + ": rows overlap or the stride is out of range").c_str());
     }
+    // An output that may be an input itself lies as that does: its rows are read where they are written, and by no one else.
+    void over(const void* out, int64_t out_stride, const void* in, int64_t in_stride, int64_t rows, const char* names) {
+        if (out && out == in && rows > 1 && out_stride != in_stride)
+            is(false, (std::string(names) + " itself needs its row stride").c_str());
+    }
 };
 
 size_t size_of(int dtype) { return dtype == WC_DTYPE_F32 ? 4 : 2; }
@@ -127,6 +132,7 @@ void check(const wc_policy_args& a, Check* c) {
     c->buffer(a.kl, 4, need, "kl");
     c->buffer(a.entropy, 4, need, "entropy");
     c->matrix(a.grad, n, a.grad_stride, a.vocab, a.rows, true, false, "grad");
+    c->over(a.grad, a.grad_stride, a.logits, a.logits_stride, a.rows, "grad over logits");
 }
 
 void check(const wc_preference_args& a, Check* c) {
@@ -150,6 +156,7 @@ void check(const wc_preference_args& a, Check* c) {
     c->buffer(a.ratios, 4, a.pairs > 0, "ratios");
     c->buffer(a.logp, 4, need, "logp");
     c->matrix(a.grad, n, a.grad_stride, a.vocab, a.rows, true, false, "grad");
+    c->over(a.grad, a.grad_stride, a.logits, a.logits_stride, a.rows, "grad over logits");
 }
 
 template <class A>
@@ -175,6 +182,7 @@ void check(const wc_norm_args& a, Check* c) {
     c->is(a.eps >= 0.f, "eps must not be negative");
     c->buffer(a.pre_bias, size_of(a.param_dtype), false, "pre_bias");
     c->matrix(a.new_stream, n, a.new_stream_stride, a.width, a.rows, true, a.rows > 0, "new_stream");
+    c->over(a.new_stream, a.new_stream_stride, a.stream, a.stream_stride, a.rows, "new_stream over stream");
     c->matrix(a.out, n, a.out_stride, a.width, a.rows, true, a.rows > 0, "out");
     c->buffer(a.stats, 16, false, "stats");
 }
@@ -188,6 +196,7 @@ void check(const wc_norm_back_args& a, Check* c) {
     c->matrix(a.d_new_stream, n, a.d_new_stream_stride, a.width, a.rows, false, false, "d_new_stream");
     c->matrix(a.d_block, n, a.d_block_stride, a.width, a.rows, true, need, "d_block");
     c->matrix(a.d_stream, n, a.d_stream_stride, a.width, a.rows, true, need, "d_stream");
+    c->over(a.d_stream, a.d_stream_stride, a.d_new_stream, a.d_new_stream_stride, a.rows, "d_stream over d_new_stream");
     c->buffer(a.d_post_gain, 4, false, "d_post_gain");
     c->buffer(a.d_post_bias, 4, false, "d_post_bias");
     c->buffer(a.d_pre_gain, 4, false, "d_pre_gain");
@@ -211,6 +220,7 @@ void check(const wc_ckpt_args& a, Ckpt use, Check* c) {
     c->matrix(a.exps, 1, a.exps_stride, (a.width + WC_CKPT_GROUP - 1) / WC_CKPT_GROUP, a.rows, write, need, "exps");
     if (use != Ckpt::read) c->matrix(a.x, n, a.x_stride, a.width, a.rows, false, need, "x");
     c->matrix(a.y, n, a.y_stride, a.width, a.rows, true, need && !write, "y");
+    if (use == Ckpt::back) c->over(a.y, a.y_stride, a.x, a.x_stride, a.rows, "y over x");
 }
 
 void check(const wc_ckpt_weight_args& a, Check* c) {
@@ -257,6 +267,7 @@ void check(const wc_linear_args& a, Check* c) {
     c->matrix(a.residual, n, a.residual_stride, a.out, a.rows, false, false, "residual");
     c->matrix(a.pre, 4, a.pre_stride, a.out, a.rows, true, false, "pre");
     c->matrix(a.y, n, a.y_stride, a.out, a.rows, true, need, "y");
+    c->over(a.y, a.y_stride, a.residual, a.residual_stride, a.rows, "y over residual");
 }
 
 void check(const wc_linear_back_args& a, Check* c) {
@@ -293,6 +304,10 @@ void check(const wc_orthogonalise_args& a, Check* c) {
     const int64_t deep = (a.rows - 1) * a.out_stride + a.width;
     c->is(a.batch <= 1 || (a.update_batch >= 0 && a.update_batch <= MOST), "update_batch out of range");
     c->is(a.batch <= 1 || (a.out_batch >= deep && a.out_batch <= MOST), "out's matrices overlap");
+    // one matrix is read whole before its result is written; of several, each only before its own
+    if (a.out && a.out == a.update && a.batch > 1)
+        c->is(a.out_dtype == a.dtype && a.out_batch == a.update_batch && (a.rows <= 1 || a.out_stride == a.update_stride),
+              "out over update itself needs its type and its strides");
 }
 
 template <class A>
@@ -327,6 +342,7 @@ void check(const wc_logp_back_args& a, Check* c) {
     c->buffer(a.d_logp, 4, false, "d_logp");
     c->buffer(a.d_entropy, 4, false, "d_entropy");
     c->matrix(a.grad, size_of(a.dtype), a.grad_stride, a.vocab, a.rows, true, a.rows > 0, "grad");
+    c->over(a.grad, a.grad_stride, a.logits, a.logits_stride, a.rows, "grad over logits");
 }
 
 template <class A>

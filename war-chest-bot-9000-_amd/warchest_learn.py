@@ -587,9 +587,9 @@ NEWTON_SCHULZ = (3.4445, -4.7750, 2.0315)
 
 @functools.lru_cache(maxsize=4096)
 def _ortho_scratch(device, code, out_code, batch, rows, width):
-    p = 256
+    p, q = 256, 512
     return _scratch_bytes("wc_orthogonalise_workspace", _ORTHO.pack(
-        _ORTHO.size, device, code, out_code, 1, batch, rows, width, p, width, rows * width, p, width, rows * width, 1.0,
+        _ORTHO.size, device, code, out_code, 1, batch, rows, width, p, width, rows * width, q, width, rows * width, 1.0,
         0.0, 0.0, 0.0, 1.0, 0, 0, 0))
 
 
