@@ -315,7 +315,9 @@ int wc_linear(const wc_linear_args* a, void* stream);
 /* Its gradients: d_pre = d_out act'(pre), d_x = d_pre W^T, d_weight = x^T d_pre
  * in the weight's layout, d_bias = the column sums of d_pre, each NULL where not
  * wanted (the residual's gradient is d_out). d_pre is rounded to the matrices'
- * type for its products; d_bias is summed before that, in float32. */
+ * type for its products, as it would be between two operators; d_bias is summed
+ * before that, in float32. A d_pre that float32 holds is no reason for an
+ * infinity, where it passes f16's largest (a slope is up to 1.13) either. */
 typedef struct wc_linear_back_args {
     uint64_t bytes;
     int32_t device, dtype;

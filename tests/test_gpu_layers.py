@@ -241,6 +241,82 @@ def test_linear_is_the_same_from_run_to_run_and_in_a_graph():
             assert torch.equal(a, b)
 
 
+@pytest.mark.parametrize("act", ["gelu", "silu"])
+@pytest.mark.parametrize("rows,width,out", [(1, 40, 24), (70, 96, 80), (257, 333, 72), (1030, 520, 776), (70, 6000, 61)])
+def test_linear_gradients_of_float16_past_its_largest(rows, width, out, act):
+    """Of |d_out| up to 65,504 by a slope of 1.1: d_pre leaves f16's range, its products do not. Halved and doubled it is off
+    by half a step of 2^-23 where it is small, 2^-24, which the bound has."""
+    say(f"case linear: {rows} x {width} x {out} f16 {act}, gradients past 65,504")
+    k, d = layer_inputs(rows, width, out, torch.float16, 14, residual=False)
+    k["x"], k["weight"] = (1e-3 * k["x"].float()).half(), (1e-2 * k["weight"].float()).half()
+    pre = torch.randn(rows, out, generator=gen(15))
+    for r, j, v in ((0, 0, 65504.0), (rows // 2, out - 1, -65504.0), (rows - 1, out // 2, 61000.0)):
+        d[r, j], pre[r, j] = v, {"gelu": 1.4, "silu": 2.4}[act]
+    assert float((d.double() * R.slope(pre, act)).abs().max()) > 70000
+    for transposed in (False, True):
+        w = to(k["weight"].t().contiguous()).t() if transposed else to(k["weight"])
+        for kw in ({"bias": True}, {"d_x": False}, {"d_weight": False}, {"dtype": torch.float32}):
+            back = wl.linear_backward(to(d), to(k["x"]), w, to(pre), act=act, **kw)
+            check_backward(back, d, k, pre, act, kw.get("dtype"))
+    # what is infinite already stays so, in its own row and column
+    d[rows - 1, out // 2] = math.inf
+    back = wl.linear_backward(to(d), to(k["x"]), to(k["weight"]), to(pre), act=act)
+    rest, columns = [i for i in range(rows - 1)], [j for j in range(out) if j != out // 2]
+    assert not back.x[rows - 1].isfinite().any() and not back.weight[:, out // 2].isfinite().any()
+    assert back.x[rest].isfinite().all() and back.weight[:, columns].isfinite().all()
+
+
+def test_linear_gradients_of_float16_past_its_largest_in_a_graph():
+    """Whether any is past is found anew in every replay."""
+    k, d = layer_inputs(300, 72, 264, torch.float16, 16, residual=False)
+    x, w, pre = to((1e-3 * k["x"].float()).half()), to(k["weight"]), torch.full((300, 264), 1.4, device=DEV)
+    small, large = to(d), to(d)
+    large = large.clone()
+    large[7, 9] = 65504.0
+    held_d = small.clone()
+
+    def step():
+        return wl.linear_backward(held_d, x, w, pre, act="gelu")
+
+    want = []
+    for v in (small, large):
+        held_d.copy_(v)
+        want.append([t.clone() for t in step()[:2]])
+    assert want[1][0].isfinite().all() and want[1][1].isfinite().all()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step()
+    for i in (1, 0, 0, 1, 0):
+        held_d.copy_((small, large)[i])
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(got.x, want[i][0]) and torch.equal(got.weight, want[i][1])
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+def test_linear_gradients_next_to_the_largest(dtype):
+    """3.4e38, which float32 holds and bf16 rounds to infinity: cut, less than a step of 2^-8 of it."""
+    k, d = layer_inputs(70, 96, 80, TYPES[dtype], 17, residual=False)
+    k["x"], k["weight"] = 1e-10 * k["x"], 1e-10 * k["weight"]
+    pre = torch.randn(70, 80, generator=gen(18))
+    # the place on the way up to the slope's maximum where it makes 3.4e38 of bf16's largest
+    d[3, 5] = 3.3895313892515355e38
+    lo, hi = 0.0, 1.4
+    for _ in range(60):
+        mid = (lo + hi) / 2
+        lo, hi = (mid, hi) if float(R.slope(torch.tensor(mid), "gelu")) * float(d[3, 5]) < 3.4e38 else (lo, mid)
+    pre[3, 5] = lo
+    assert 3.3962e38 < float(d[3, 5]) * float(R.slope(pre[3, 5], "gelu")) < 3.4028e38
+    back = wl.linear_backward(to(d), to(k["x"]), to(k["weight"]), to(pre), act="gelu", bias=True)
+    assert back.x.isfinite().all() and back.weight.isfinite().all()
+    check_backward(back, d, k, pre, "gelu")
+
+
 @pytest.mark.parametrize("rows,width,out,dtype", [(1, 96, 200, "bf16"), (2, 4096, 40, "f16"), (300, 128, 264, "bf16"),
                                                   (1030, 520, 776, "f16"), (64, 9000, 72, "bf16"), (70, 50, 90, "f32"),
                                                   (40, 4096, 40, "f32"), (1201, 1027, 1103, "f32")])

@@ -59,7 +59,12 @@ __device__ __forceinline__ void put_parts(char* to, int64_t plane, const float (
     if constexpr (Parts<T>::COUNT == 1) {
         E8 o;
 #pragma unroll
-        for (int u = 0; u < 8; u++) o[u] = (E)v[u];
+        for (int u = 0; u < 8; u++) {
+            o[u] = (E)v[u];
+            // what float32 holds and would round past bf16's largest
+            if constexpr (__is_same(E, bf16))
+                if (fabsf((float)o[u]) == INFINITY && fabsf(v[u]) != INFINITY) o[u] = cut_bf16(v[u]);
+        }
         *(E8*)to = o;
     } else {
         E8 o[3];
@@ -112,17 +117,21 @@ struct Source {
     int64_t to_rows, to_cols, plane;
 };
 
-// Up to two matrices copied into planes, a chunk of eight a thread.
+// Up to two matrices copied into planes, a chunk of eight a thread, by workgroup `block` of `blocks`.
 template <class T>
-__global__ __launch_bounds__(256) void k_lay(Source one, Source two) {
+__device__ __forceinline__ void lay_chunks(const Source& one, const Source& two, int64_t block, int64_t blocks) {
     const int64_t n1 = one.to_rows * (one.to_cols / 8), n2 = two.to_rows * (two.to_cols / 8);
-    for (int64_t at = int64_t(blockIdx.x) * 256 + threadIdx.x; at < n1 + n2; at += int64_t(gridDim.x) * 256) {
+    for (int64_t at = block * 256 + threadIdx.x; at < n1 + n2; at += blocks * 256) {
         const Source& s = at < n1 ? one : two;
         const int64_t chunk = at < n1 ? at : at - n1, per_row = s.to_cols / 8, r = chunk / per_row, c = 8 * (chunk - r * per_row);
         float v[8] = {};
         if (r < s.rows && c < s.cols) load_n((const T*)s.p + r * s.stride + c, (int)min<int64_t>(8, s.cols - c), 0.f, v);
         put_parts<T>(s.to + 2 * (r * s.to_cols + c), s.plane, v);
     }
+}
+template <class T>
+__global__ __launch_bounds__(256) void k_lay(Source one, Source two) {
+    lay_chunks<T>(one, two, blockIdx.x, gridDim.x);
 }
 
 // y = act(v + bias) + residual, and the kept v + bias.
@@ -138,6 +147,7 @@ struct LayerEpilogue {
     T* y;
     int64_t y_stride;
     int act;
+    const float* rate;  // what the product is times first; null: 1
 
     // The same from row lo on.
     LayerEpilogue from(int64_t lo) const {
@@ -153,6 +163,11 @@ struct LayerEpilogue {
         return residual ? load_some<8>(residual + i * residual_stride + j, n) : Raw{};
     }
     __device__ __forceinline__ void operator()(const Raw& r, int, int64_t i, int64_t j, int n, float (&v)[8]) const {
+        if (rate) {
+            const float by = *rate;
+#pragma unroll
+            for (int u = 0; u < 8; u++) v[u] *= by;
+        }
         if (bias) {
             float b[8];
             if (bias_f32) load_n((const float*)bias + j, n, 0.f, b);
@@ -203,19 +218,20 @@ inline dim3 lay_grid(int64_t chunks, int cus) {
     return dim3((uint32_t)std::max<int64_t>(1, std::min<int64_t>((chunks + 255) / 256, int64_t(cus) * 32)));
 }
 
+// Where a matrix is copied to; nothing where it is read as it lies.
+inline Source copy_of(const Laid& l, Source s, char* workspace) {
+    if (!l.copy) return {};
+    s.to = workspace + l.at;
+    s.to_rows = l.rows;
+    s.to_cols = l.cols;
+    s.plane = l.plane;
+    return s;
+}
+inline int64_t chunks_of(const Source& a, const Source& b) { return a.to_rows * (a.to_cols / 8) + b.to_rows * (b.to_cols / 8); }
+
 template <class T>
-void lay(const Laid& l1, const Source& s1, const Laid& l2, const Source& s2, char* workspace, int cus, hipStream_t s) {
-    auto full = [&](const Laid& l, Source src) {
-        if (!l.copy) return Source{};
-        src.to = workspace + l.at;
-        src.to_rows = l.rows;
-        src.to_cols = l.cols;
-        src.plane = l.plane;
-        return src;
-    };
-    const Source a = full(l1, s1), b = full(l2, s2);
-    const int64_t n = a.to_rows * (a.to_cols / 8) + b.to_rows * (b.to_cols / 8);
-    if (n) k_lay<T><<<lay_grid(n, cus), 256, 0, s>>>(a, b);
+void lay(const Source& a, const Source& b, int cus, hipStream_t s) {
+    if (const int64_t n = chunks_of(a, b)) k_lay<T><<<lay_grid(n, cus), 256, 0, s>>>(a, b);
 }
 
 // ------------------------------------------------------------------ few rows
@@ -559,8 +575,8 @@ void linear(const wc_linear_args& a, int cus, hipStream_t s) {
             return;
         }
     }
-    lay<T>(p.x, {a.x, a.x_stride, a.rows, a.width}, p.w,
-           {a.weight, a.weight_stride, io ? a.width : a.out, io ? a.out : a.width}, w, cus, s);
+    lay<T>(copy_of(p.x, {a.x, a.x_stride, a.rows, a.width}, w),
+           copy_of(p.w, {a.weight, a.weight_stride, io ? a.width : a.out, io ? a.out : a.width}, w), cus, s);
     Product m = {};
     m.a = operand<T>(p.x, a.x, w, a.rows);
     m.b = operand<T>(p.w, a.weight, w, a.out);
@@ -570,32 +586,46 @@ void linear(const wc_linear_args& a, int cus, hipStream_t s) {
 
 // ----------------------------------------------------------------- backward
 
-// d_pre = d_out act'(pre), in the parts that its products read (`to` may be null: not needed), and its column sums,
-// from the unrounded float32 values: 32 chunks of eight columns by eight rows a workgroup, over `per` rows. Memory bounds
-// it: 16,384 x 4,096 bf16 through a GELU 110 us for 537 MB, 4.9 TB/s.
+// d_pre = d_out act'(pre), eight columns of a row.
 template <class T>
-__global__ __launch_bounds__(256) void k_slope(wc_linear_back_args a, Source d, int64_t per, float* sums) {
+__device__ __forceinline__ void slope_values(const wc_linear_back_args& a, int64_t r, int64_t c, int have, float (&v)[8]) {
+    load_n((const T*)a.d_out + r * a.d_out_stride + c, have, 0.f, v);
+    if (a.act == WC_ACT_NONE) return;
+    float z[8];
+    load_n((const float*)a.pre + r * a.pre_stride + c, have, 0.f, z);
+    act_slopes(z, a.act);
+#pragma unroll
+    for (int u = 0; u < 8; u++) v[u] = u < have ? v[u] * z[u] : 0.f;
+}
+
+// d_pre in the parts that its products read (`to` may be null: not needed), and its column sums, from the unrounded
+// float32 values: 32 chunks of eight columns by eight rows a workgroup, over `per` rows. Memory bounds it: 16,384 x 4,096
+// bf16 through a GELU 110 us for 537 MB, 4.9 TB/s. past (f16): marks the workgroups that found what f16 does not hold.
+template <class T>
+__global__ __launch_bounds__(256) void k_slope(wc_linear_back_args a, Source d, int64_t per, float* sums, uint32_t* past) {
     __shared__ float4 add[256][2];
     const int64_t c = (int64_t(blockIdx.x) * 32 + threadIdx.x % 32) * 8, lo = int64_t(blockIdx.y) * per;
     const int64_t rows = d.to ? d.to_rows : a.rows, hi = min(lo + per, rows);
     const int lane = threadIdx.x / 32, have = (int)min<int64_t>(8, a.out - c);
     float sum[8] = {};
+    bool found = false;
     for (int64_t r = lo + lane; r < hi; r += 8) {
         float v[8] = {};
         if (r < a.rows && have > 0) {
-            load_n((const T*)a.d_out + r * a.d_out_stride + c, have, 0.f, v);
-            if (a.act != WC_ACT_NONE) {
-                float z[8];
-                load_n((const float*)a.pre + r * a.pre_stride + c, have, 0.f, z);
-                act_slopes(z, a.act);
-#pragma unroll
-                for (int u = 0; u < 8; u++) v[u] = u < have ? v[u] * z[u] : 0.f;
-            }
+            slope_values<T>(a, r, c, have, v);
 #pragma unroll
             for (int u = 0; u < 8; u++) sum[u] += v[u];
+            if constexpr (__is_same(T, f16))
+#pragma unroll
+                for (int u = 0; u < 8; u++) found |= fabsf(v[u]) > 65504.f && fabsf(v[u]) != INFINITY;
         }
         if (d.to && c < d.to_cols) put_parts<T>(d.to + 2 * (r * d.to_cols + c), d.plane, v);
     }
+    if constexpr (__is_same(T, f16))
+        if (past) {
+            const int any = __syncthreads_or(found);
+            if (threadIdx.x == 0) past[blockIdx.y * gridDim.x + blockIdx.x] = any;
+        }
     if (!sums) return;
     add[threadIdx.x][0] = {sum[0], sum[1], sum[2], sum[3]};
     add[threadIdx.x][1] = {sum[4], sum[5], sum[6], sum[7]};
@@ -608,6 +638,37 @@ __global__ __launch_bounds__(256) void k_slope(wc_linear_back_args a, Source d, 
 #pragma unroll
     for (int u = 0; u < 8; u++) s += one[u * 32 * 8];
     sums[int64_t(blockIdx.y) * a.out + j] = s;
+}
+
+// A GELU's slope is up to 1.13, a SiLU's 1.10: of an f16 d_out from 58,000 on d_pre may pass f16's largest. Where the first
+// pass marked any, all of it is written again by halves, and the products' results are doubled (rate); the halves of less
+// than 2^-13 lose a bit, which is why it is done for these only. In the launch that copies x and the weight, whose `first`
+// workgroups those are (4,099 x 1,153 x 567: 87.3 us for the call, 86.5 without); with nothing to copy and no mark it takes 4.4 us.
+struct Half {
+    Source d;
+    int64_t per;
+    const uint32_t* past;
+    int marks, across;
+    float* rate;
+};
+static __global__ __launch_bounds__(256) void k_lay_half(Source one, Source two, unsigned first, wc_linear_back_args a, Half h) {
+    if (blockIdx.x < first) return lay_chunks<f16>(one, two, blockIdx.x, first);
+    const unsigned block = blockIdx.x - first;
+    bool found = false;
+    for (int k = threadIdx.x; k < h.marks; k += 256) found |= h.past[k] != 0;
+    const int any = __syncthreads_or(found);
+    if (block == 0 && threadIdx.x == 0) *h.rate = any ? 2.f : 1.f;
+    if (!any) return;
+    const int64_t c = (int64_t(block % h.across) * 32 + threadIdx.x % 32) * 8, lo = block / h.across * h.per, hi = min(lo + h.per, a.rows);
+    const int have = (int)min<int64_t>(8, a.out - c);
+    if (have <= 0) return;
+    for (int64_t r = lo + threadIdx.x / 32; r < hi; r += 8) {
+        float v[8];
+        slope_values<f16>(a, r, c, have, v);
+#pragma unroll
+        for (int u = 0; u < 8; u++) v[u] *= 0.5f;
+        put_parts<f16>(h.d.to + 2 * (r * h.d.to_cols + c), h.d.plane, v);
+    }
 }
 
 // The row blocks' column sums added in order: a sixteenth of them each group of sixteen threads.
@@ -658,7 +719,8 @@ struct LinearBackPlan {
     int blocks;
     bool slope, direct;
     DirectCut one_x, one_w;
-    size_t sums, part_x, part, bytes;
+    size_t sums, past, part_x, part, bytes;
+    int marks;  // of what f16 does not hold, a workgroup of k_slope each; 0: d_pre is no larger than d_out
     bool together;
 };
 
@@ -726,14 +788,19 @@ LinearBackPlan linear_back_plan(const wc_linear_back_args& a, int cus) {
         p.per = up((std::max<int64_t>(p.d.copy ? p.d.rows : a.rows, 1) + blocks - 1) / blocks, 8);
         p.blocks = (int)((std::max<int64_t>(p.d.copy ? p.d.rows : a.rows, 1) + p.per - 1) / p.per);
         if (a.d_bias) p.sums = take(size_t(p.blocks) * a.out * 4);
+        if (__is_same(T, f16) && products && a.rows && (a.act == WC_ACT_GELU || a.act == WC_ACT_SILU)) {
+            p.marks = (int)((p.d.cols + 255) / 256) * p.blocks;
+            p.past = take(4 * (size_t(p.marks) + 1));  // and the rate behind them
+        }
     }
     p.bytes = at;
     return p;
 }
 
 template <class T>
-LayerEpilogue<T> plain_to(void* y, int64_t stride) {
+LayerEpilogue<T> plain_to(void* y, int64_t stride, const float* rate = nullptr) {
     LayerEpilogue<T> e = {};
+    e.rate = rate;
     e.y = (T*)y;
     e.y_stride = stride;
     e.act = WC_ACT_NONE;
@@ -783,18 +850,14 @@ void linear_back(const wc_linear_back_args& a, int cus, hipStream_t s) {
             return;
         }
     }
+    uint32_t* const past = p.marks ? (uint32_t*)(w + p.past) : nullptr;
+    const Source d_pre = products ? copy_of(p.d, {}, w) : Source{};
     if (p.slope) {
-        Source d = {};
-        if (products && p.d.copy) {
-            d.to = w + p.d.at;
-            d.to_rows = p.d.rows;
-            d.to_cols = p.d.cols;
-            d.plane = p.d.plane;
-        }
         float* sums = a.d_bias ? (float*)(w + p.sums) : nullptr;
-        const int64_t across = ((d.to ? p.d.cols : a.out) + 255) / 256;
-        k_slope<T><<<dim3((uint32_t)across, (uint32_t)p.blocks), 256, 0, s>>>(a, d, p.per, sums);
+        const int64_t across = ((d_pre.to ? p.d.cols : a.out) + 255) / 256;
+        k_slope<T><<<dim3((uint32_t)across, (uint32_t)p.blocks), 256, 0, s>>>(a, d_pre, p.per, sums, past);
     }
+    const float* rate = past ? (const float*)(past + p.marks) : nullptr;
     const ColumnSums bias = {(const float*)(w + p.sums), a.out, p.blocks, a.d_bias};
     const uint32_t bias_blocks = a.d_bias ? (uint32_t)((a.out + 15) / 16) : 0;
     if (!a.d_weight || p.cut_w.runs == 1) {
@@ -802,8 +865,16 @@ void linear_back(const wc_linear_back_args& a, int cus, hipStream_t s) {
     }
     if (!products) return;
     // copies of x and the weight, in one launch
-    lay<T>(p.x, {a.x, a.x_stride, a.rows, a.width}, p.w,
-           {a.weight, a.weight_stride, io ? a.width : a.out, io ? a.out : a.width}, w, cus, s);
+    const Source to_x = copy_of(p.x, {a.x, a.x_stride, a.rows, a.width}, w),
+                 to_w = copy_of(p.w, {a.weight, a.weight_stride, io ? a.width : a.out, io ? a.out : a.width}, w);
+    if (!p.marks) {
+        lay<T>(to_x, to_w, cus, s);
+    } else if constexpr (__is_same(T, f16)) {
+        const int64_t n = chunks_of(to_x, to_w);
+        const unsigned first = n ? lay_grid(n, cus).x : 0;
+        const Half h = {d_pre, p.per, past, p.marks, p.marks / p.blocks, (float*)(past + p.marks)};
+        k_lay_half<<<dim3(first + (unsigned)p.marks), 256, 0, s>>>(to_x, to_w, first, a, h);
+    }
     const bool with_x = a.d_x && a.rows;
     Product mx = {}, mw = {};
     if (with_x) {
@@ -812,7 +883,7 @@ void linear_back(const wc_linear_back_args& a, int cus, hipStream_t s) {
         mx.k = p.out_k;
         mx = cut_product(segments_of<T>(mx), p.cut_x, (float*)(w + p.part_x));
     }
-    const auto ex = plain_to<T>(a.d_x, a.d_x_stride);
+    const auto ex = plain_to<T>(a.d_x, a.d_x_stride, rate);
     if (!a.d_weight) {
         if (with_x) multiply<T>(mx, p.cut_x, true, io, mx.part, ex, s);
         return;
@@ -849,9 +920,9 @@ void linear_back(const wc_linear_back_args& a, int cus, hipStream_t s) {
         sums();
     };
     if (a.grad_dtype == a.dtype) {
-        both(plain_to<T>(a.d_weight, a.d_weight_stride));
+        both(plain_to<T>(a.d_weight, a.d_weight_stride, rate));
     } else if constexpr (Parts<T>::COUNT == 1) {
-        both(plain_to<float>(a.d_weight, a.d_weight_stride));
+        both(plain_to<float>(a.d_weight, a.d_weight_stride, rate));
     }
 }
 
