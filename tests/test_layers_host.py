@@ -137,6 +137,29 @@ def test_the_binding_refuses_tensors_that_are_not_on_a_gpu():
             call()
 
 
+def test_dense_keeps_pre_activations_only_for_gradients_that_read_them(monkeypatch):
+    """Not under no_grad or inference_mode, whatever requires a gradient, nor for the residual's, which does not read them."""
+    kept = []
+
+    def linear(x, weight, bias=None, *, act="none", residual=None, keep=False):
+        kept.append(keep)
+        out = x @ weight
+        return wl.Linear(out if residual is None else out + residual, out.clone() if keep else None)
+    monkeypatch.setattr(wl, "linear", linear)
+    x, w, b, r = torch.randn(3, 4), torch.randn(4, 5), torch.randn(5), torch.randn(3, 5)
+    parameters = [torch.nn.Parameter(t.clone()) for t in (w, b)]
+    with torch.no_grad():
+        wl.dense(x, *parameters, act="gelu")
+    with torch.inference_mode():
+        wl.dense(x, *parameters, act="gelu")
+    wl.dense(x, w, b, act="gelu")
+    wl.dense(x, w, b, act="gelu", residual=r.clone().requires_grad_(True)).sum().backward()
+    assert kept == [False] * 4
+    for one in range(3):
+        wl.dense(*(t.clone().requires_grad_(i == one) for i, t in enumerate((x, w, b))), act="gelu")
+    assert kept[4:] == [True] * 3
+
+
 def test_muon_refuses_vectors():
     with pytest.raises(ww.WaveError, match="dimensions"):
         wl.Muon([torch.nn.Parameter(torch.zeros(3))])

@@ -840,8 +840,8 @@ def act_linear8(z, weight, act="gelu"):
 
 class _Dense(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, weight, bias, residual, act):
-        r = linear(x, weight, bias, act=act, residual=residual, keep=any(ctx.needs_input_grad))
+    def forward(ctx, x, weight, bias, residual, act, keep):
+        r = linear(x, weight, bias, act=act, residual=residual, keep=keep)
         ctx.save_for_backward(x, weight, bias, r.pre)
         ctx.act = act
         return r.out
@@ -856,12 +856,14 @@ class _Dense(torch.autograd.Function):
         if any(need[:3]):
             g = linear_backward(d.contiguous(), x, weight, pre, act=ctx.act, bias=need[2], d_x=need[0], d_weight=need[1])
             d_bias = g.bias.to(bias.dtype) if need[2] else None
-        return g.x, g.weight, d_bias, d if need[3] else None, None
+        return g.x, g.weight, d_bias, d if need[3] else None, None, None
 
 
 def dense(x, weight, bias=None, *, act="none", residual=None):
-    """linear as a differentiable function of x, the weight, the bias and the residual."""
-    return _Dense.apply(x, weight, bias, residual, act)
+    """linear as a differentiable function of x, the weight, the bias and the residual. Pre-activations are kept where a
+    gradient of the first three may be asked for: not under no_grad, nor for the residual alone."""
+    keep = torch.is_grad_enabled() and any(isinstance(t, torch.Tensor) and t.requires_grad for t in (x, weight, bias))
+    return _Dense.apply(x, weight, bias, residual, act, keep)
 
 
 class Dense(torch.nn.Module):
