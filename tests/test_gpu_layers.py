@@ -372,6 +372,59 @@ def test_dense_under_automatic_differentiation(dtype):
         g.sum().backward()
 
 
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("held", ["f32", "bf16"])
+@pytest.mark.parametrize("bias,residual,act", [(True, False, "gelu"), (False, True, "none"), (True, True, "silu")])
+def test_dense_module_of_parameters_in_their_own_type(dtype, held, bias, residual, act):
+    """Dense takes its products in x's type; the parameters' gradients come in the parameters', a float32 weight's to
+    float32's own rounding."""
+    dt, own = TYPES[dtype], TYPES[held]
+    layer = wl.Dense(72, 88, bias=bias, act=act, gain=1.5, device=DEV, dtype=own)
+    assert layer.weight.dtype == own and (layer.bias is None) == (not bias)
+    assert abs(float(layer.weight.detach().float().std()) / (1.5 * 72 ** -0.5) - 1) < 0.06  # 6,336 normal values: 0.9% each
+    k, d = layer_inputs(60, 72, 88, dt, 19)
+    with torch.no_grad():
+        k["weight"] = layer.weight.detach().cpu().to(dt)
+        if bias:
+            layer.bias.copy_(k["bias"])
+            k["bias"] = layer.bias.detach().cpu()
+            if own != torch.float32:
+                k["bias"] = k["bias"].to(dt)
+        else:
+            k["bias"] = None
+        if not residual:
+            k["residual"] = None
+    x = to(k["x"]).requires_grad_(True)
+    r = to(k["residual"]).requires_grad_(True) if residual else None
+    y = layer(x, r)
+    check_forward(wl.Linear(y, None), k, act)
+    y.backward(to(d))
+    pre = None if act == "none" else wl.linear(to(k["x"]), to(k["weight"]), to(k["bias"]), act=act, keep=True).pre.cpu()
+    assert x.grad.dtype == dt and layer.weight.grad.dtype == own
+    check_backward(wl.LinearGrads(x.grad, None, None), d, k, pre, act)
+    check_backward(wl.LinearGrads(None, layer.weight.grad, None), d, k, pre, act, own)
+    if bias:
+        assert layer.bias.grad.dtype == own
+        # its sums' bound (which call makes them decides their order), and the roundings to x's type and to its own
+        db = R.linear_backward(d, k["x"], k["weight"], pre, act)[2]
+        size = d.double().abs().sum(0)
+        off = (2.0 ** -24 * 300 * 1.2 + 4e-6) * size + (R.U[own] + (R.U[dt] if own != torch.float32 else 0.0)) * 1.01 * db.abs()
+        within(layer.bias.grad, db, off, "d_bias")
+    if residual:
+        assert torch.equal(r.grad, to(d))
+
+
+def test_dense_of_a_cast_weight_has_no_second_derivative():
+    x, w = torch.randn(6, 5, device=DEV).bfloat16(), torch.randn(5, 4, device=DEV, requires_grad=True)
+    g, = torch.autograd.grad(wl.dense(x, w, act="gelu").sum(), w, create_graph=True)
+    assert g.dtype == torch.float32
+    with pytest.raises(ww.WaveError, match="second"):
+        g.sum().backward()
+    for bad in (w.double(), w.detach().int()):
+        with pytest.raises(ww.WaveError, match="weight"):
+            wl.dense(x, bad)
+
+
 # ------------------------------------------------------------------ updates
 
 def check_ortho(got, u, dtype, **kw):

@@ -75,12 +75,12 @@ class PolicyNet(torch.nn.Module):
         return (out @ self.head.bfloat16()).float()
 
     def forward_fused(self, x):
-        stream = wl.dense(x, self.inp.bfloat16())
+        stream = wl.dense(x, self.inp)
         out = stream
         for up, ub, down, db, norm in zip(self.up, self.up_bias, self.down, self.down_bias, self.norms):
-            hidden = wl.dense(out, up.bfloat16(), ub, act="gelu")
-            stream, out = norm(wl.dense(hidden, down.bfloat16(), db), stream)
-        return wl.dense(out, self.head.bfloat16()).float()
+            hidden = wl.dense(out, up, ub, act="gelu")
+            stream, out = norm(wl.dense(hidden, down, db), stream)
+        return wl.dense(out, self.head).float()
 
 
 class Both:

@@ -841,34 +841,42 @@ def act_linear8(z, weight, act="gelu"):
 class _Dense(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, residual, act, keep):
-        r = linear(x, weight, bias, act=act, residual=residual, keep=keep)
-        ctx.save_for_backward(x, weight, bias, r.pre)
+        cast = None
+        if all(isinstance(t, torch.Tensor) and t.dtype in DTYPES for t in (x, weight)) and weight.dtype is not x.dtype:
+            cast = weight.to(x.dtype)
+        r = linear(x, weight if cast is None else cast, bias, act=act, residual=residual, keep=keep)
+        ctx.save_for_backward(x, weight, bias, r.pre, cast)
         ctx.act = act
         return r.out
 
     @staticmethod
     @_first_only
     def backward(ctx, d):
-        x, weight, bias, pre = ctx.saved_tensors
+        x, weight, bias, pre, cast = ctx.saved_tensors
         need = ctx.needs_input_grad
-        d_bias = None
+        d_weight = d_bias = None
         g = LinearGrads(None, None, None)
         if any(need[:3]):
-            g = linear_backward(d.contiguous(), x, weight, pre, act=ctx.act, bias=need[2], d_x=need[0], d_weight=need[1])
+            # of a weight that was cast the gradient is not rounded to the products' type
+            g = linear_backward(d.contiguous(), x, weight if cast is None else cast, pre, act=ctx.act, bias=need[2],
+                                d_x=need[0], d_weight=need[1], dtype=None if cast is None else torch.float32)
+            d_weight = g.weight.to(weight.dtype) if need[1] else None
             d_bias = g.bias.to(bias.dtype) if need[2] else None
-        return g.x, g.weight, d_bias, d if need[3] else None, None, None
+        return g.x, d_weight, d_bias, d if need[3] else None, None, None
 
 
 def dense(x, weight, bias=None, *, act="none", residual=None):
-    """linear as a differentiable function of x, the weight, the bias and the residual. Pre-activations are kept where a
-    gradient of the first three may be asked for: not under no_grad, nor for the residual alone."""
+    """linear as a differentiable function of x, the weight, the bias and the residual. The products are taken in x's type:
+    a weight of another type is cast for them, and its gradient is summed and returned in its own (float32 for a float32
+    weight, whatever x is). Pre-activations are kept where a gradient of the first three may be asked for: not under
+    no_grad, nor for the residual alone."""
     keep = torch.is_grad_enabled() and any(isinstance(t, torch.Tensor) and t.requires_grad for t in (x, weight, bias))
     return _Dense.apply(x, weight, bias, residual, act, keep)
 
 
 class Dense(torch.nn.Module):
-    """A layer with its parameters: act(x @ weight + bias) + residual. The products are taken in x's type: parameters of
-    another are cast for them."""
+    """A layer with its parameters: act(x @ weight + bias) + residual. The products are taken in x's type, for which
+    parameters of another are cast; their gradients come in their own (dense)."""
 
     def __init__(self, width, out, bias=True, act="none", gain=1.0, device=None, dtype=torch.float32):
         super().__init__()
@@ -881,7 +889,7 @@ class Dense(torch.nn.Module):
         b = self.bias
         if b is not None and b.dtype is not torch.float32:
             b = b.to(x.dtype)
-        return dense(x, self.weight.to(x.dtype), b, act=self.act, residual=residual)
+        return dense(x, self.weight, b, act=self.act, residual=residual)
 
 
 class _TokenLogp(torch.autograd.Function):
