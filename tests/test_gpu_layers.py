@@ -911,6 +911,38 @@ def test_linear_in_float32_with_each_gradient_alone(rows, width, out, act):
             check_backward(back, d, k, pre, act)
 
 
+@pytest.mark.parametrize("rows,width,out", [(1201, 1027, 1103), (701, 2053, 1301)])
+@pytest.mark.parametrize("layout", ["as they come", "strided", "transposed", "transposed and strided", "broadcast"])
+def test_linear_in_float32_parts_of_odd_sizes_strides_and_layouts(rows, width, out, layout):
+    """Sizes that are taken in parts whatever is wanted, with a remainder of k in each product: zeros are laid behind it. The
+    scratch tells the way: the copies in parts are six bytes an element."""
+    say(f"case linear: {rows} x {width} x {out} f32 in parts, {layout}")
+    k, d = layer_inputs(rows, width, out, torch.float32, 21)
+    if layout == "broadcast":
+        k["x"] = k["x"][:1].expand(rows, -1)
+    v = {n: to(t) for n, t in k.items()}
+    d_out = to(d)
+    if "strided" in layout:
+        v["x"], v["residual"], d_out = strided(k["x"], 7), strided(k["residual"], 3), strided(d, 1)
+        v["weight"] = strided(k["weight"].t(), 5).t() if "transposed" in layout else strided(k["weight"], 5)
+    elif layout == "transposed":
+        v["weight"] = v["weight"].t().contiguous().t()
+    elif layout == "broadcast":
+        v["x"], d_out = v["x"][:1].expand(rows, -1), d_out[:1].expand(rows, -1)
+        d = d[:1].expand(rows, -1)
+    got = wl.linear(v["x"], v["weight"], v["bias"], act="gelu", residual=v["residual"], keep=True)
+    check_forward(got, k, "gelu")
+    pre = strided(got.pre.cpu(), 2) if "strided" in layout else got.pre
+    for kw in ({"bias": True}, {"d_weight": False}, {"d_x": False}):
+        check_backward(wl.linear_backward(d_out, v["x"], v["weight"], pre, act="gelu", **kw), d, k, got.pre.cpu(), "gelu")
+    transposed = int("transposed" in layout)
+    ws = v["weight"].stride(1 if transposed else 0)
+    assert wl._linear_scratch(0, 0, transposed, rows, width, out, v["x"].stride(0), ws, False, False) >= 6 * (rows + out) * width
+    for dx, dw in ((True, True), (True, False), (False, True)):
+        assert wl._linear_back_scratch(0, 0, transposed, wl.ACTS["gelu"], rows, width, out, d_out.stride(0), v["x"].stride(0), ws, False,
+                                       False, False, dx, dw, dx and dw) >= 6 * rows * out
+
+
 def test_linear_in_float32_parts_of_infinities_and_of_the_largest():
     """Sizes that are taken in parts: as the small ones."""
     say("case linear: infinities f32, 1,200 x 1,024 x 1,100")
