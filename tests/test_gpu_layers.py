@@ -671,6 +671,27 @@ def test_token_logp_of_masks_infinities_and_nan(vocab, dtype):
 
 
 @pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("rows,loads,threads", [(300, 4, 256), (300, 8, 256), (300, 8, 512), (3, 1, 256), (3, 2, 256)])
+def test_token_logp_alternatives_where_all_that_a_thread_holds_is_nan(rows, loads, threads, dtype):
+    """A NaN is no alternative, and does not stand in the way of the others: here all of one thread's columns, the single one
+    behind the last whole load among them."""
+    each = 16 // TYPES[dtype].itemsize
+    vocab = loads * threads * each + 1
+    say(f"case logp: {rows} x {vocab} {dtype}, a thread's columns NaN")
+    for top in (1, 2, 20):
+        k, _, _ = logp_inputs(3, vocab, TYPES[dtype], vocab, False)
+        for c in range(loads):
+            k["logits"][1, c * threads * each: c * threads * each + each] = math.nan
+        k["logits"][1, vocab - 1] = math.nan
+        x = k["logits"].double().nan_to_num(nan=-math.inf)
+        want = torch.sort(x, dim=1, descending=True, stable=True).indices[:, :top]
+        at = torch.arange(rows) % 3
+        got = wl.token_logp(to(k["logits"][at]), to(k["tokens"][at]), top=top)
+        assert torch.equal(got.top_index.cpu().long(), want[at])
+        assert got.logp[1].isnan() and got.logp[0].isfinite()
+
+
+@pytest.mark.parametrize("dtype", list(TYPES))
 def test_token_logp_with_strides_and_without_tokens(dtype):
     say(f"case logp: strides {dtype}")
     k, d1, d2 = logp_inputs(40, 301, TYPES[dtype], 6, True)

@@ -321,7 +321,7 @@ __global__ __launch_bounds__(G > 64 ? G : LOGP_BLOCK, G > 256 ? 4 : 1) void k_lo
         x.none();
     }
 
-    float own = (float)x.one;
+    float own = fmaxf((float)x.one, -INFINITY);  // of nothing but NaN: -infinity, which no bound counts
 #pragma unroll
     for (int k = 0; k < NV; k++) {
 #pragma unroll
