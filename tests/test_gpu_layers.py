@@ -671,6 +671,31 @@ def test_token_logp_of_masks_infinities_and_nan(vocab, dtype):
 
 
 @pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("vocab", [13, 60, 600, 5003, 20001])
+def test_token_logp_gradient_of_illegal_columns_is_zero_whatever_the_row(vocab, dtype):
+    """A legal NaN or infinity makes the row's legal columns NaN, those at -infinity aside, which have none anyway; what
+    arrives infinite or as NaN has no effect on illegal columns either. The other rows are as without these."""
+    say(f"case logp: gradients of spoiled rows {vocab} {dtype}")
+    k, d1, d2 = logp_inputs(7, vocab, TYPES[dtype], vocab, True)
+    x, on, a = k["logits"], k["legal"], k["tokens"]
+    on[:, :4] = torch.tensor([False, True, True, True])
+    a[:] = 2
+    calm = {n: to(t.clone()) for n, t in k.items()}
+    x[1, 1], x[2, 1], x[2, 0], x[5, 1], x[5, 2] = math.nan, math.inf, math.nan, math.nan, -math.inf
+    for d_entropy in (None, d2):
+        e1, e2 = d1.clone(), None if d_entropy is None else d_entropy.clone()
+        e1[3], e1[4] = math.nan, math.inf
+        got = wl.token_logp(to(x), to(a), legal=to(on))
+        g = wl.token_logp_backward(to(e1), to(e2), to(x), to(a), got.stats, legal=to(on)).cpu()
+        assert not g[~on].any(), g[~on].isnan().sum()
+        for r in (1, 2, 5):
+            assert g[r][on[r] & (x[r] != -math.inf)].isnan().all(), r
+        before = wl.token_logp_backward(to(d1), to(d2) if d_entropy is not None else None, calm["logits"], calm["tokens"],
+                                        wl.token_logp(**calm).stats, legal=calm["legal"]).cpu()
+        assert torch.equal(g[[0, 6]], before[[0, 6]])
+
+
+@pytest.mark.parametrize("dtype", list(TYPES))
 @pytest.mark.parametrize("rows,loads,threads", [(300, 4, 256), (300, 8, 256), (300, 8, 512), (3, 1, 256), (3, 2, 256)])
 def test_token_logp_alternatives_where_all_that_a_thread_holds_is_nan(rows, loads, threads, dtype):
     """A NaN is no alternative, and does not stand in the way of the others: here all of one thread's columns, the single one

@@ -167,6 +167,28 @@ def test_policy_nan_in_a_counted_row_shows():
     assert got.grad[[0, 1, 3]].isfinite().all()
 
 
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("ref", ["none", "full"])
+@pytest.mark.parametrize("vocab", [13, 60, 600, 5003, 20001, 90001])
+def test_policy_gradient_of_illegal_columns_is_zero_whatever_the_row(vocab, ref, dtype):
+    """A legal NaN or infinity, and an advantage that is NaN or infinite, show in the row's legal columns only."""
+    for entropy_coef in (0.0, 0.02):
+        k = policy_inputs(6, vocab, TYPES[dtype], vocab, True, ref)
+        k["legal"][:, :4] = torch.tensor([False, True, True, True])
+        k["actions"][:] = 2
+        k["logits"][:, 2] = 1.0
+        coefs = {**COEFS, "entropy_coef": entropy_coef}
+        before = wl.policy_loss(**{n: to(v) for n, v in k.items()}, **coefs).grad
+        k["logits"][1, 1], k["logits"][2, 1], k["logits"][2, 0] = math.nan, math.inf, math.nan
+        k["advantages"][3], k["advantages"][4] = math.nan, math.inf
+        got = wl.policy_loss(**{n: to(v) for n, v in k.items()}, **coefs).grad
+        on, x = to(k["legal"]), to(k["logits"])
+        assert not got[~on].any()
+        for r in (1, 2):
+            assert got[r][on[r] & (x[r] != -math.inf)].isnan().all(), r
+        assert torch.equal(got[[0, 5]], before[[0, 5]])
+
+
 @pytest.mark.parametrize("rows,vocab,dtype", [(5, 22, "f32"), (6, 3001, "bf16"), (2, 40000, "f16")])
 def test_policy_in_place_without_gradient_scaled_and_again(rows, vocab, dtype):
     """grad written over the logits, not at all, or scaled by what arrives; the same bits every time."""

@@ -515,8 +515,9 @@ __global__ __launch_bounds__(LOGP_BLOCK) void k_logp_back(Rows<T> in, LogpRows o
     x.load(in.x + r * in.x_stride + c0, legal, n, lane);
     int at = a >= c0 && a < c0 + n ? (int)(a - c0) : -1;
     if (at >= 0 && legal && !legal[at]) at = -1;
-    if (g.ent == 0.f) put_grad<T, G, NV, false, true>(to, n, lane, x, none, Slope(g, in.rate.inv_temp), in.rate.rate, at);
-    else put_grad<T, G, NV, false, false>(to, n, lane, x, none, Slope(g, in.rate.inv_temp), in.rate.rate, at);
+    const Slope slope(g, in.rate.inv_temp);
+    if (g.ent == 0.f && slope.finite()) put_grad<T, G, NV, false, true>(to, n, lane, x, none, slope, in.rate.rate, at);
+    else put_grad<T, G, NV, false, false>(to, n, lane, x, none, slope, in.rate.rate, at);
 }
 
 // ------------------------------------------------------------------ launches

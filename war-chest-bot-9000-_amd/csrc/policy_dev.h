@@ -159,12 +159,13 @@ __global__ __launch_bounds__(group_block<G>(), (group_waves<NV * (FULL ? 2 : 1)>
             }
             if (!TOKEN && grad) {
                 T* to = grad + r * grad_stride;
+                const Slope slope(g, go);
                 if (!g.any())
                     put_zero<T, G, NV>(to, n, lane);
-                else if (!FULL && g.ent == 0.f)
-                    put_grad<T, G, NV, FULL, true>(to, n, lane, x, y, Slope(g, go), in.rate.rate, (int)head.a);
+                else if (!FULL && g.ent == 0.f && slope.finite())
+                    put_grad<T, G, NV, FULL, true>(to, n, lane, x, y, slope, in.rate.rate, (int)head.a);
                 else
-                    put_grad<T, G, NV, FULL, false>(to, n, lane, x, y, Slope(g, go), in.rate.rate, (int)head.a);
+                    put_grad<T, G, NV, FULL, false>(to, n, lane, x, y, slope, in.rate.rate, (int)head.a);
             }
         }
     }
@@ -296,10 +297,11 @@ __global__ __launch_bounds__(BLOCK) void k_row_grads(Rows<T> in, int64_t tiles, 
         x.load(in.x + r * in.x_stride + c0, legal, n, threadIdx.x);
         if constexpr (FULL) y.load(in.y + r * in.y_stride + c0, legal, n, threadIdx.x);
         const int at = a >= 0 && a < n ? (int)a : -1;
-        if (!FULL && g.ent == 0.f)
-            put_grad<T, BLOCK, NV, FULL, true>(to, n, threadIdx.x, x, y, Slope(g, go), in.rate.rate, at);
+        const Slope slope(g, go);
+        if (!FULL && g.ent == 0.f && slope.finite())
+            put_grad<T, BLOCK, NV, FULL, true>(to, n, threadIdx.x, x, y, slope, in.rate.rate, at);
         else
-            put_grad<T, BLOCK, NV, FULL, false>(to, n, threadIdx.x, x, y, Slope(g, go), in.rate.rate, at);
+            put_grad<T, BLOCK, NV, FULL, false>(to, n, threadIdx.x, x, y, slope, in.rate.rate, at);
     }
 }
 

@@ -277,14 +277,23 @@ constexpr float LN2 = 0.6931471805599453f;
 
 // A row's gradient as a function of a logit: p (base + slope logp - toward logq),
 // logarithms to base 2; PLAIN without the two. Where p is 0 the gradient is (0
-// times infinity would be NaN).
+// times infinity would be NaN). A row whose sum is NaN (a NaN or +infinity among
+// its logits) is NaN, but 0 where its logits' own powers are, as in illegal
+// columns, which are -infinity here.
 struct Slope {
     float m, log_s, my, log_sy, base, slope, toward, hit;
 
     __device__ __forceinline__ Slope(const RowGrad& g, float go)
         : m(g.m), log_s(g.log_s), my(g.klc != 0.f ? g.my : 0.f), log_sy(g.klc != 0.f ? g.log_sy : 0.f),
           base(go * (g.ent * g.h - (g.klc != 0.f ? g.klc * g.kl : 0.f) - g.coef)),
-          slope(go * (g.ent + g.klc) * LN2), toward(go * g.klc * LN2), hit(go * g.coef) {}
+          slope(go * (g.ent + g.klc) * LN2), toward(go * g.klc * LN2), hit(go * g.coef) {
+        const bool spoiled = log_s != log_s;
+        base = spoiled ? log_s : base;
+        m = spoiled ? 0.f : m;
+        log_s = spoiled ? 0.f : log_s;
+    }
+    // Whether PLAIN is right where p is 0, too.
+    __device__ __forceinline__ bool finite() const { return base - base == 0.f; }
 
     template <bool FULL, bool PLAIN>
     __device__ __forceinline__ float at(float x, float y, float rate) const {
