@@ -6,7 +6,7 @@
 // The three products differ in which index of each operand is summed; one kernel takes all (product_dev.h). Sums, bias,
 // activation and residual are float32 and rounded once, to the output's type. d_pre is rounded to the 16-bit type for
 // its two products (as it would be between two operators): its own half ulp, 2^-9 of an element in bf16, against the
-// same for every element of the result. Pre-activations are kept in float32: in 16 bits their rounding would be 10^4 times
+// same for every element of the result, which is then 2.3e-3 of its norm off in place of 1.7e-3. Pre-activations are kept in float32: in 16 bits their rounding would be 10^4 times
 // that of the float32 sums of d_b (1.3e-3 of its norm in bf16).
 //
 // float32 operands are taken as three bf16 parts (8 + 8 + 8 bits), and of their nine products the six that matter:
@@ -147,7 +147,6 @@ struct LayerEpilogue {
     T* y;
     int64_t y_stride;
     int act;
-    const float* rate;  // what the product is times first; null: 1
 
     // The same from row lo on.
     LayerEpilogue from(int64_t lo) const {
@@ -163,11 +162,6 @@ struct LayerEpilogue {
         return residual ? load_some<8>(residual + i * residual_stride + j, n) : Raw{};
     }
     __device__ __forceinline__ void operator()(const Raw& r, int, int64_t i, int64_t j, int n, float (&v)[8]) const {
-        if (rate) {
-            const float by = *rate;
-#pragma unroll
-            for (int u = 0; u < 8; u++) v[u] *= by;
-        }
         if (bias) {
             float b[8];
             if (bias_f32) load_n((const float*)bias + j, n, 0.f, b);
@@ -180,6 +174,27 @@ struct LayerEpilogue {
         if (residual) {
 #pragma unroll
             for (int u = 0; u < 8; u++) v[u] += (float)r[u];
+        }
+        store_n(y + i * y_stride + j, n, v);
+    }
+};
+
+// A gradient, as the product is or times a number in memory.
+template <class T>
+struct GradEpilogue {
+    static constexpr bool MIRROR = false;
+    T* y;
+    int64_t y_stride;
+    const float* rate;  // null: 1
+
+    struct Raw {};
+    __device__ __forceinline__ bool reads() const { return false; }
+    __device__ __forceinline__ Raw raw(int, int64_t, int64_t, int) const { return {}; }
+    __device__ __forceinline__ void operator()(const Raw&, int, int64_t i, int64_t j, int n, float (&v)[8]) const {
+        if (rate) {
+            const float by = *rate;
+#pragma unroll
+            for (int u = 0; u < 8; u++) v[u] *= by;
         }
         store_n(y + i * y_stride + j, n, v);
     }
@@ -643,7 +658,8 @@ __global__ __launch_bounds__(256) void k_slope(wc_linear_back_args a, Source d, 
 // A GELU's slope is up to 1.13, a SiLU's 1.10: of an f16 d_out from 58,000 on d_pre may pass f16's largest. Where the first
 // pass marked any, all of it is written again by halves, and the products' results are doubled (rate); the halves of less
 // than 2^-13 lose a bit, which is why it is done for these only. In the launch that copies x and the weight, whose `first`
-// workgroups those are (4,099 x 1,153 x 567: 87.3 us for the call, 86.5 without); with nothing to copy and no mark it takes 4.4 us.
+// workgroups those are (both gradients of 4,099 x 1,153 x 567 57.4 us, 58.1 without it and with the forward pass's epilogue);
+// with nothing to copy it is a launch more (4,096 x 256 x 1,024: 29.6 and 26.7).
 struct Half {
     Source d;
     int64_t per;
@@ -798,16 +814,6 @@ LinearBackPlan linear_back_plan(const wc_linear_back_args& a, int cus) {
 }
 
 template <class T>
-LayerEpilogue<T> plain_to(void* y, int64_t stride, const float* rate = nullptr) {
-    LayerEpilogue<T> e = {};
-    e.rate = rate;
-    e.y = (T*)y;
-    e.y_stride = stride;
-    e.act = WC_ACT_NONE;
-    return e;
-}
-
-template <class T>
 void linear_back(const wc_linear_back_args& a, int cus, hipStream_t s) {
     const LinearBackPlan p = linear_back_plan<T>(a, cus);
     char* w = (char*)a.workspace;
@@ -822,7 +828,7 @@ void linear_back(const wc_linear_back_args& a, int cus, hipStream_t s) {
                 float* sums = !a.d_bias || p.one_w.runs == 1 ? a.d_bias : (float*)(w + p.sums);
                 dw = direct_of(io ? x : side, io ? side : x, a.rows, a.act, p.one_w, (float*)(w + p.part), sums);
             }
-            const auto ew = plain_to<float>(a.d_weight, a.d_weight_stride);
+            const GradEpilogue<float> ew = {(float*)a.d_weight, a.d_weight_stride, nullptr};
             // x's gradient in parts that a launch holds, the weight's beside the first
             const int64_t rows_x = a.d_x ? a.rows : 0, most = direct_rows(a.width);
             for (int64_t lo = 0; lo == 0 || lo < rows_x; lo += most) {
@@ -833,7 +839,7 @@ void linear_back(const wc_linear_back_args& a, int cus, hipStream_t s) {
                                    {(const float*)a.weight, a.weight_stride, a.width}, a.out, a.act, p.one_x, (float*)(w + p.part_x),
                                    nullptr);
                 const Direct beside = lo ? Direct{} : dw;
-                const auto ex = plain_to<float>(rows_x ? (float*)a.d_x + lo * a.d_x_stride : nullptr, a.d_x_stride);
+                const GradEpilogue<float> ex = {rows_x ? (float*)a.d_x + lo * a.d_x_stride : nullptr, a.d_x_stride, nullptr};
                 const dim3 grid(dx.blocks + beside.blocks);
                 if (!grid.x) return;
                 if (io) k_direct_back<true><<<grid, DIRECT_BLOCK, 0, s>>>(dx, ex, beside, ew);
@@ -883,7 +889,7 @@ void linear_back(const wc_linear_back_args& a, int cus, hipStream_t s) {
         mx.k = p.out_k;
         mx = cut_product(segments_of<T>(mx), p.cut_x, (float*)(w + p.part_x));
     }
-    const auto ex = plain_to<T>(a.d_x, a.d_x_stride, rate);
+    const GradEpilogue<T> ex = {(T*)a.d_x, a.d_x_stride, rate};
     if (!a.d_weight) {
         if (with_x) multiply<T>(mx, p.cut_x, true, io, mx.part, ex, s);
         return;
@@ -920,9 +926,9 @@ void linear_back(const wc_linear_back_args& a, int cus, hipStream_t s) {
         sums();
     };
     if (a.grad_dtype == a.dtype) {
-        both(plain_to<T>(a.d_weight, a.d_weight_stride, rate));
+        both(GradEpilogue<T>{(T*)a.d_weight, a.d_weight_stride, rate});
     } else if constexpr (Parts<T>::COUNT == 1) {
-        both(plain_to<float>(a.d_weight, a.d_weight_stride, rate));
+        both(GradEpilogue<float>{(float*)a.d_weight, a.d_weight_stride, rate});
     }
 }
 
