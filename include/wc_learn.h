@@ -283,7 +283,8 @@ int wc_ckpt_weight_grad(const wc_ckpt_weight_args* a, void* stream);
  * pre, where given, gets x W + bias in float32, for the backward pass.
  * 16-bit matrices: products on the matrix cores with float32 sums. float32:
  * small ones as they are, larger ones as three bf16 parts an element and six
- * products of parts (what is left out is below 2^-25 of a product); there an
+ * products of parts (what is left out is below 2^-25 of a product, and of a part
+ * what is under 2^-133: an element's last bits below 2^-110); there an
  * infinite element's row or column of the result is not finite, and may be NaN
  * where its product alone would be infinite.
  * rows below 2^31, width and out at most 2^20. */
@@ -315,8 +316,10 @@ int wc_linear(const wc_linear_args* a, void* stream);
 /* Its gradients: d_pre = d_out act'(pre), d_x = d_pre W^T, d_weight = x^T d_pre
  * in the weight's layout, d_bias = the column sums of d_pre, each NULL where not
  * wanted (the residual's gradient is d_out). d_pre is rounded to the matrices'
- * type for its products, as it would be between two operators; d_bias is summed
- * before that, in float32. A d_pre that float32 holds is no reason for an
+ * type for its products, as it would be between two operators, which is as much
+ * again as d_x and d_weight's own rounding (in bf16 2.3e-3 of their norm in all,
+ * 1.7e-3 without; float32 matrices have none); d_bias is summed before that, in
+ * float32. A d_pre that float32 holds is no reason for an
  * infinity, where it passes f16's largest (a slope is up to 1.13) either. */
 typedef struct wc_linear_back_args {
     uint64_t bytes;
@@ -348,9 +351,10 @@ int wc_linear_backward(const wc_linear_back_args* a, void* stream);
  * applied): X = update / (Frobenius norm + eps), then `steps` times
  *   A = X X^T, X = a X + (b A + c A A) X
  * (the transposed form where rows > width), and out = scale X. `batch` matrices
- * of one shape. X is held in 22 bits an element, A and its polynomial too, but
- * for a bf16 result of more than 128 rows and columns in 11 (off by about as much
- * as that result's rounding); sums are float32, the norm's float64.
+ * of one shape. X is held in 22 bits an element (in steps of 2^-34, so that one
+ * below 2^-13 has fewer), A and its polynomial too, but for a bf16 result of more
+ * than 128 rows and columns in 11 (off by about as much as that result's
+ * rounding); sums are float32, the norm's float64.
  * X, A and B = b A + c A A are held times 2^10 in f16: an element of any of them
  * that passes 63 may make the result infinite or NaN. None does while every
  * singular value s of the matrix that a step starts from has s^2 and |b s^2 + c s^4|
@@ -381,7 +385,8 @@ int wc_orthogonalise(const wc_orthogonalise_args* a, void* stream);
  *   and the `top` likeliest columns in that order with their log-probabilities.
  * A row is left out (logp and entropy 0, rank -1, its logits not read) when its
  * token is outside [0, vocab) or no legal logit is above -infinity. A token that
- * is not legal, or whose logit is -infinity, has logp -infinity. Alternatives
+ * is not legal, or whose logit is -infinity, has logp -infinity, and its rank
+ * counts all columns of a lower index beside those above -infinity. Alternatives
  * are columns above -infinity: where there are fewer than `top`, and in a row
  * that is left out, the others are column -1 with -infinity. Illegal columns may
  * hold anything. A legal NaN or +infinity makes a row's values NaN (a NaN is no

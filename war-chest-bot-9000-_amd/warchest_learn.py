@@ -19,7 +19,8 @@ with torch on that stream; a tensor made on another stream must be ready there, 
 Arguments that do not fit raise `WaveError`, and then nothing was queued. The `*_objective` functions, `ResidualNorm`,
 `dense` and `Dense` are the same calls with torch's automatic differentiation, `Muon` an optimiser on `orthogonalise`.
 
-Nothing here computes: every call goes through the native library.
+Every operator goes through the native library; what `Muon` does around its update (momentum, decay, the step) and the
+casts of `dense` are torch's.
 """
 from __future__ import annotations
 
@@ -546,7 +547,8 @@ def linear_backward(d_out, x, weight, pre=None, *, act="none", bias=False, d_x=T
     """The gradients of linear from its inputs and its pre (wc_linear_backward); the residual's is d_out itself.
 
     d_out [rows, out]; pre may be None where act is "none". bias, d_x, d_weight: which are wanted. dtype: the weight's
-    gradient's type, x's (the default) or float32. Returns LinearGrads(x, weight, bias): weight contiguous along the
+    gradient's type, x's (the default) or float32. The gradient at the pre-activations is rounded to x's type for its
+    products, as between two operators; float32 matrices keep it. Returns LinearGrads(x, weight, bias): weight contiguous along the
     index that the weight is, bias in float32, None for what is not wanted."""
     device = _device(x, "x")
     code, dt = _dtype(x, "x"), x.dtype
@@ -635,7 +637,8 @@ def token_logp(logits, tokens=None, *, legal=None, inv_temperature=1.0, top=0, s
 
     logits [rows, vocab]; tokens [rows] int64 or int32, or None; legal [rows, vocab] bool. A row whose token is out of
     range, or without a legal logit above -infinity, is left out. Returns TokenLogp(logp, entropy, rank, top_logp,
-    top_index, stats): rank int32, how many columns come before the token (0: the likeliest, -1: left out); top_logp
+    top_index, stats): rank int32, how many columns come before the token (0: the likeliest, -1: left out; of a token
+    without a probability all of a lower index do); top_logp
     and top_index [rows, top] (int32, -1 where there are no more), None for top=0; logp and rank None without tokens;
     stats [rows, 4] is what token_logp_backward needs (stats=False: not kept)."""
     device, code, rows, vocab, (x, xs) = _logits(logits)
