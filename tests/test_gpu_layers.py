@@ -671,6 +671,26 @@ def test_token_logp_of_masks_infinities_and_nan(vocab, dtype):
 
 
 @pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("vocab", [2, 7, 15, 19, 30, 135, 603, 5003, 20007])
+def test_token_logp_rank_of_a_token_without_a_probability(vocab, dtype):
+    """At -infinity or not legal, in every place of the last columns, which a whole load does not reach, and before them:
+    each column above -infinity comes before it once, and each other of a lower index."""
+    say(f"case logp: ranks of tokens at -infinity {vocab} {dtype}")
+    at = [c for c in (0, 1, vocab // 2, *range(vocab - 9, vocab)) if 0 <= c < vocab]
+    for legal in (False, True):
+        k, d1, d2 = logp_inputs(len(at), vocab, TYPES[dtype], vocab, legal)
+        k["tokens"] = torch.tensor(at)
+        x = k["logits"]
+        x[torch.rand(x.shape, generator=gen(22)) < 0.3] = -math.inf
+        for r, a in enumerate(at):
+            if legal and r % 2:
+                k["legal"][r, a] = False
+            else:
+                x[r, a] = -math.inf
+        check_logp(k, 3, d1, d2)
+
+
+@pytest.mark.parametrize("dtype", list(TYPES))
 @pytest.mark.parametrize("vocab", [13, 60, 600, 5003, 20001])
 def test_token_logp_gradient_of_illegal_columns_is_zero_whatever_the_row(vocab, dtype):
     """A legal NaN or infinity makes the row's legal columns NaN, those at -infinity aside, which have none anyway; what

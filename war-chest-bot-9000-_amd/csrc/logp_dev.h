@@ -367,9 +367,10 @@ __global__ __launch_bounds__(G > 64 ? G : LOGP_BLOCK, G > 256 ? 4 : 1) void k_lo
         auto late = [&](float v, int i) { more[0] += v > -INFINITY || i < at; };
 #pragma unroll
         for (int k = 0; k < NV; k++) {
+            // past the last whole load the columns are loads of one
 #pragma unroll
             for (int i = 0; i < E; i++)
-                if ((lane + k * G) * E + i < n) late((float)x.v[k][i], (lane + k * G) * E + i);
+                if (lane + k * G < whole) late((float)x.v[k][i], (lane + k * G) * E + i);
             __builtin_amdgcn_sched_barrier(0);
         }
         x.forget();
