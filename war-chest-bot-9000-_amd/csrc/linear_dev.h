@@ -6,8 +6,8 @@
 // The three products differ in which index of each operand is summed; one kernel takes all (product_dev.h). Sums, bias,
 // activation and residual are float32 and rounded once, to the output's type. d_pre is rounded to the 16-bit type for
 // its two products (as it would be between two operators): its own half ulp, 2^-9 of an element in bf16, against the
-// same for every element of the result, which is then 2.3e-3 of its norm off in place of 1.7e-3. Pre-activations are kept in float32: in 16 bits their rounding would be 10^4 times
-// that of the float32 sums of d_b (1.3e-3 of its norm in bf16).
+// same for every element of the result, which is then 2.3e-3 of its norm off in place of 1.7e-3. Pre-activations are kept
+// in float32: in 16 bits their rounding would be 10^4 times that of the float32 sums of d_b (1.3e-3 of its norm in bf16).
 //
 // float32 operands are taken as three bf16 parts (8 + 8 + 8 bits), and of their nine products the six that matter:
 // the matrix cores' own float32 rate is a sixteenth of the 16-bit one. Small ones, whose launches cost more than their
